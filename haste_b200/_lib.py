@@ -62,6 +62,9 @@ SIGNATURES = {
     "haste_ffi_topk_fused_scratch": [I64, I64, I64, I64, I64, I32],
     "haste_ffi_topk_fused": [P, P, P, P, P, I64, I64, I64, I64, I64, I64, I32, I64, P, P, P],
     "haste_ffi_check_locations": [P, I64, I64, P],
+    "haste_layer_norm_forward": [P, P, P, P, P, P, I64, I64, I64, F32, I32, I32, P],
+    "haste_layer_norm_backward_scratch": [I64, I64],
+    "haste_layer_norm_backward": [P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I32, I32, I32, P],
     "haste_ffi_set_max_ctas": [I32],
     "haste_poll_status": [],
     "haste_debug_set_wait_limit": [c_longlong],
@@ -80,11 +83,13 @@ lib.haste_last_error_string.restype = c_char_p
 lib.haste_last_error_string.argtypes = []
 lib.haste_version.restype = c_int
 lib.haste_ffi_topk_fused_scratch.restype = I64          # bytes, not a status
+lib.haste_layer_norm_backward_scratch.restype = I64
 lib.haste_version.argtypes = []
 
 # status codes and flags (include/haste_ffi.h)
 OK, ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_INDEX_RANGE, ERR_LAUNCH, ERR_TIMEOUT, ERR_TOO_LARGE = range(7)
 LOSS_BCE, LOSS_SQHINGE = 0, 1
+BF16, FP32 = 0, 1
 F_SR, F_CONTRACT, F_RNG_PACKED, F_ZERO_DXT, F_LOSS = 1, 2, 4, 8, 16
 
 

@@ -482,4 +482,51 @@ int haste_ffi_check_locations(const int32_t* loc, int64_t n, int64_t D, haste_st
   return launch_check_loc(loc, n, D, static_cast<cudaStream_t>(stream));
 }
 
+// ---------------------------------------------------------------- layer norm
+static int check_type(const char* who, const char* what, int32_t type) {
+  if (type != HASTE_BF16 && type != HASTE_F32) return fail(HASTE_ERR_UNSUPPORTED, "%s: unknown %s type %d", who, what, type);
+  return HASTE_OK;
+}
+static int check_layer_norm(const char* who, int64_t rows, int64_t D, int64_t ldx) {
+  if (rows < 0 || D < 1) return fail(HASTE_ERR_BAD_ARG, "%s: rows=%lld must not be negative, D=%lld must be positive", who, (long long)rows, (long long)D);
+  if (D >= (1ll << 31)) return fail(HASTE_ERR_UNSUPPORTED, "%s: D=%lld exceeds int32", who, (long long)D);
+  if (ldx < 0) return fail(HASTE_ERR_BAD_ARG, "%s: row strides must not be negative", who);
+  return HASTE_OK;
+}
+
+int haste_layer_norm_forward(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows, int64_t D, int64_t ldx,
+                             float eps, int32_t x_type, int32_t w_type, haste_stream_t stream) {
+  const char* who = "haste_layer_norm_forward";
+  if (int rc = check_layer_norm(who, rows, D, ldx)) return rc;
+  if (int rc = check_type(who, "x", x_type)) return rc;
+  if (int rc = check_type(who, "weight", w_type)) return rc;
+  if (!(eps >= 0.f)) return fail(HASTE_ERR_BAD_ARG, "%s: eps must not be negative", who);
+  if ((mean == nullptr) != (rstd == nullptr)) return fail(HASTE_ERR_BAD_ARG, "%s: mean and rstd go together", who);
+  if (rows > 0) { REQUIRE_PTR(x, who); REQUIRE_PTR(y, who); }
+  return launch_layer_norm_forward(x, w, b, y, mean, rstd, rows, D, ldx, eps, x_type, w_type, static_cast<cudaStream_t>(stream));
+}
+
+int64_t haste_layer_norm_backward_scratch(int64_t rows, int64_t D) {
+  if (rows < 0 || D < 1) return 0;
+  return 4 * layer_norm_backward_scratch(rows, D);
+}
+
+int haste_layer_norm_backward(const void* dy, const void* x, const void* w, const float* mean, const float* rstd, void* dx, void* dw, void* db,
+                              void* scratch, int64_t scratch_bytes, int64_t rows, int64_t D, int64_t lddy, int64_t ldx, int32_t x_type, int32_t dy_type,
+                              int32_t w_type, haste_stream_t stream) {
+  const char* who = "haste_layer_norm_backward";
+  if (int rc = check_layer_norm(who, rows, D, ldx < lddy ? ldx : lddy)) return rc;
+  if (int rc = check_type(who, "x", x_type)) return rc;
+  if (int rc = check_type(who, "dy", dy_type)) return rc;
+  if (int rc = check_type(who, "weight", w_type)) return rc;
+  if (rows > 0) { REQUIRE_PTR(dy, who); REQUIRE_PTR(x, who); REQUIRE_PTR(mean, who); REQUIRE_PTR(rstd, who); REQUIRE_PTR(dx, who); }
+  const int64_t need = 4 * layer_norm_backward_scratch(rows, D);
+  if ((dw || db) && need > 0) {
+    REQUIRE_PTR(scratch, who); REQUIRE_ALIGNED(scratch, who);
+    if (scratch_bytes < need) return fail(HASTE_ERR_BAD_ARG, "%s: %lld bytes of scratch, %lld needed", who, (long long)scratch_bytes, (long long)need);
+  }
+  return launch_layer_norm_backward(dy, x, w, mean, rstd, dx, dw, db, static_cast<float*>(scratch), rows, D, lddy, ldx, x_type, dy_type, w_type,
+                                    static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

@@ -144,4 +144,11 @@ int launch_rewire_select_begin(const void* w, int64_t F, int64_t L, int64_t G, i
 int launch_rewire_select_refine(int64_t F, int64_t L, int64_t G, int64_t k, void* scratch, cudaStream_t st);
 int launch_rewire_select_finish(int64_t F, int64_t L, int64_t G, void* scratch, cudaStream_t st);
 
+// Layer norm (layernorm.cu); *_type: HASTE_BF16 / HASTE_F32
+int launch_layer_norm_forward(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows, int64_t D, int64_t ldx,
+                              float eps, int x_type, int w_type, cudaStream_t st);
+int64_t layer_norm_backward_scratch(int64_t rows, int64_t D);      // floats
+int launch_layer_norm_backward(const void* dy, const void* x, const void* w, const float* mean, const float* rstd, void* dx, void* dw, void* db,
+                               float* scratch, int64_t rows, int64_t D, int64_t lddy, int64_t ldx, int x_type, int dy_type, int w_type, cudaStream_t st);
+
 }  // namespace haste

@@ -388,6 +388,99 @@ def topk_update(z, C, col0, vals, idx):
         check(lib.haste_topk_update(_ptr(z), z.stride(0), B, C, col0, k, _ptr(vals), _ptr(idx), _stream(z)), "topk_update")
 
 
+# ---------------------------------------------------------------- layer norm
+_TYPES = {torch.bfloat16: _lib.BF16, torch.float32: _lib.FP32}
+
+
+def _type_of(t, name):
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        raise RuntimeError(f"{name} must be torch.bfloat16 or torch.float32, got {t.dtype}")
+    return code
+
+
+def _rows_of(t, D):
+    """``t`` [..., D] as rows of unit column stride, and their stride; copied only where no such view exists."""
+    if t.is_contiguous():
+        return t, D
+    t = t.reshape(-1, D)
+    if D > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else D)
+
+
+def _norm_parameters(x, weight, bias):
+    """(D, rows, element type of weight and bias) after the checks that both directions share."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise RuntimeError("x must be a CUDA tensor (this library has no CPU path)")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError(f"x must be [..., D] with D >= 1, got {tuple(x.shape)}")
+    D = x.shape[-1]
+    w_type = _lib.FP32
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        _req(t, name)
+        if t.device != x.device:
+            raise RuntimeError(f"{name} must be on {x.device}, as x is, got {t.device}")
+        if t.dim() != 1 or t.shape[0] != D:
+            raise RuntimeError(f"{name} must be [{D}], got {tuple(t.shape)}")
+        w_type = _type_of(t, name)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise RuntimeError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
+    return D, x.numel() // D, w_type
+
+
+def layer_norm_forward(x, weight, bias, eps=1e-5, stats=True):
+    """Layer norm over the last dimension of ``x`` [..., D] (bf16 or fp32; any strides, copied if its rows are not of unit
+    stride): ``(y, mean, rstd)``, y of x's type, the statistics fp32 [...]; y alone with ``stats=False`` (inference).
+    ``weight`` and ``bias``: [D], bf16 or fp32 whatever x is, or None."""
+    D, rows, w_type = _norm_parameters(x, weight, bias)
+    x_type = _type_of(x, "x")
+    src, ldx = _rows_of(x, D)
+    with _on(x.device):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        mean = rstd = None
+        if stats:
+            mean, rstd = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device)
+        check(lib.haste_layer_norm_forward(_ptr(src), _ptr(weight), _ptr(bias), _ptr(y), _ptr(mean), _ptr(rstd), rows, D, ldx, eps, x_type,
+                                           w_type, _stream(x)), "layer_norm_forward")
+    return (y, mean, rstd) if stats else y
+
+
+def layer_norm_backward(dy, x, weight, mean, rstd, want_weight=True, want_bias=True, param_dtype=None):
+    """``(dx, dweight, dbias)`` of ``layer_norm_forward``: dx of x's type, the other two of ``param_dtype`` (default: the weight's type,
+    x's without a weight), None where not wanted.  ``dy`` [..., D] is bf16 or fp32, whatever x is; a broadcast gradient (row stride 0) is
+    read in place.  The sums over rows are fp32 and give the same bits on every call."""
+    D, rows, w_type = _norm_parameters(x, weight, None)
+    if not isinstance(dy, torch.Tensor) or dy.device != x.device or dy.shape != x.shape:
+        raise RuntimeError(f"dy must be a tensor of x's shape {tuple(x.shape)} on {x.device}")
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        _req(t, name, torch.float32)
+        if t.numel() != rows or t.device != x.device:
+            raise RuntimeError(f"{name} must hold {rows} values on {x.device}")
+    if param_dtype is None:
+        param_dtype = x.dtype if weight is None else weight.dtype
+    if weight is None:
+        w_type = _TYPES.get(param_dtype)
+    if param_dtype not in _TYPES or (weight is not None and weight.dtype != param_dtype):
+        raise RuntimeError(f"param_dtype must be the weight's type, torch.bfloat16 or torch.float32, got {param_dtype}")
+    x_type, dy_type = _type_of(x, "x"), _type_of(dy, "dy")
+    src, ldx = _rows_of(x, D)
+    grad, lddy = _rows_of(dy, D)
+    with _on(x.device):
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dw = torch.empty(D, dtype=param_dtype, device=x.device) if want_weight else None
+        db = torch.empty(D, dtype=param_dtype, device=x.device) if want_bias else None
+        scratch, n = None, 0
+        if want_weight or want_bias:
+            n = lib.haste_layer_norm_backward_scratch(rows, D)
+            scratch = torch.empty(n, dtype=torch.uint8, device=x.device)
+        check(lib.haste_layer_norm_backward(_ptr(grad), _ptr(src), _ptr(weight), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dw), _ptr(db), _ptr(scratch), n,
+                                            rows, D, lddy, ldx, x_type, dy_type, w_type, _stream(x)), "layer_norm_backward")
+    return dx, dw, db
+
+
 def check_locations(loc, D):
     _req(loc, "group_locations", torch.int32)
     with _on(loc.device):

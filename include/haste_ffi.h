@@ -43,6 +43,9 @@ enum {
 /* loss_kind */
 enum { HASTE_LOSS_BCE = 0, HASTE_LOSS_SQHINGE = 1 };
 
+/* element types of the dense operators */
+enum { HASTE_BF16 = 0, HASTE_F32 = 1 };
+
 /* flags for the update / train-step entry points */
 enum {
   HASTE_F_SR = 1u << 0,          /* stochastic rounding to bf16 (else round-to-nearest-even) */
@@ -355,6 +358,21 @@ int haste_ffi_step_ldx(const void* x, const int32_t* coo, int64_t nnz, const int
 int haste_ffi_topk_ldx(const int32_t* loc, const void* xt, const void* w, const void* bias, void* zbuf, int64_t ldz, int64_t B,
                        int64_t D, int64_t F, int64_t L, int64_t G, int64_t groups_per_chunk, int32_t k, int64_t label0,
                        float* vals, int32_t* idx, int64_t ldxt, haste_stream_t stream);
+
+/* Layer norm over the last dimension of x [rows, D] (row stride ldx elements), for the features ahead of this layer:
+ *   y[r,j] = (x[r,j] - mean_r) * rstd_r * w[j] + b[j],   rstd_r = 1 / sqrt(var_r + eps),   var_r = sum_j (x[r,j] - mean_r)^2 / D
+ * y is contiguous, of x's type; w and b (either may be NULL: ones, zeros) share w_type.  mean and rstd (fp32 [rows], both or
+ * neither) are kept for the backward pass.  fp32 sums; nothing needs alignment beyond that of its type.  rows may be 0. */
+int haste_layer_norm_forward(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows, int64_t D, int64_t ldx,
+                             float eps, int32_t x_type, int32_t w_type, haste_stream_t stream);
+
+/* Its backward: dx (contiguous, x's type), and dw, db (w_type; either may be NULL) summed over the rows in fp32, in an order that
+ * depends on the sizes alone.  dy [rows, D] has row stride lddy (0 = one row for all).  With rows = 0 dw and db are zeros.
+ * scratch: 16-byte aligned, haste_layer_norm_backward_scratch(rows, D) bytes, not needed without dw and db. */
+int64_t haste_layer_norm_backward_scratch(int64_t rows, int64_t D);
+int haste_layer_norm_backward(const void* dy, const void* x, const void* w, const float* mean, const float* rstd, void* dx, void* dw, void* db,
+                              void* scratch, int64_t scratch_bytes, int64_t rows, int64_t D, int64_t lddy, int64_t ldx, int32_t x_type, int32_t dy_type,
+                              int32_t w_type, haste_stream_t stream);
 
 /* Rate probes (measurement only; timed by the benchmark's auxiliary mode; no counterpart in the reference).  Each
  * isolates one access pattern of the fused train step at the step's own sizes:
