@@ -5,7 +5,7 @@ CPU or PyTorch fallback.  Build it with ``python -m haste_b200.build``.
 """
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_longlong, c_uint32, c_uint64, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_longlong, c_uint32, c_uint64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libhaste_ffi.so")
@@ -17,7 +17,7 @@ if not os.path.exists(LIB_PATH):
 
 lib = ctypes.CDLL(LIB_PATH)
 
-P, I64, F32, U64, U32, I32 = c_void_p, c_int64, c_float, c_uint64, c_uint32, c_int32
+P, I64, F32, F64, U64, U32, I32 = c_void_p, c_int64, c_float, c_double, c_uint64, c_uint32, c_int32
 
 # name -> argtypes, in the order of include/haste_ffi.h
 SIGNATURES = {
@@ -65,6 +65,10 @@ SIGNATURES = {
     "haste_layer_norm_forward": [P, P, P, P, P, P, I64, I64, I64, F32, I32, I32, P],
     "haste_layer_norm_backward_scratch": [I64, I64],
     "haste_layer_norm_backward": [P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I32, I32, I32, P],
+    "haste_adamw_step": [P, P, P, I64, P, P, P, P, I64, I32, I32, I32, F64, F64, F64, F64, F64, I64, F32, F32, P, U64, U32, U32, P],
+    "haste_grad_norm": [P, P, P, I64, F32, P, P, P],
+    "haste_quantize_moment": [P, P, P, I64, I32, P],
+    "haste_dequantize_moment": [P, P, P, I64, I32, I32, P],
     "haste_ffi_set_max_ctas": [I32],
     "haste_poll_status": [],
     "haste_debug_set_wait_limit": [c_longlong],
@@ -90,6 +94,7 @@ lib.haste_version.argtypes = []
 OK, ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_INDEX_RANGE, ERR_LAUNCH, ERR_TIMEOUT, ERR_TOO_LARGE = range(7)
 LOSS_BCE, LOSS_SQHINGE = 0, 1
 BF16, FP32 = 0, 1
+GRAD_NORM_PARTIALS = 4096
 F_SR, F_CONTRACT, F_RNG_PACKED, F_ZERO_DXT, F_LOSS = 1, 2, 4, 8, 16
 
 

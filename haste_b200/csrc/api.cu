@@ -529,4 +529,79 @@ int haste_layer_norm_backward(const void* dy, const void* x, const void* w, cons
                                     static_cast<cudaStream_t>(stream));
 }
 
+// ---------------------------------------------------------------- AdamW over many tensors
+static int check_tensors(const char* who, const void* const* grads, const int64_t* sizes, int64_t count, int64_t* moments) {
+  if (count < 0) return fail(HASTE_ERR_BAD_ARG, "%s: count=%lld < 0", who, (long long)count);
+  if (count > 0) { REQUIRE_PTR(grads, who); REQUIRE_PTR(sizes, who); }
+  *moments = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (sizes[i] < 0) return fail(HASTE_ERR_BAD_ARG, "%s: size %lld of tensor %lld is negative", who, (long long)sizes[i], (long long)i);
+    if (sizes[i] >= (1ll << 38)) return fail(HASTE_ERR_TOO_LARGE, "%s: tensor %lld has %lld elements (fewer than 2^38 are supported)", who, (long long)i, (long long)sizes[i]);
+    *moments += (sizes[i] + 255) / 256 * 256;
+  }
+  return HASTE_OK;
+}
+static bool is_finite(double v) { return v - v == 0.0; }
+
+int haste_adamw_step(void* const* params, const void* const* grads, const int64_t* sizes, int64_t count, void* exp_avg, float* exp_avg_scale,
+                     void* exp_avg_sq, float* exp_avg_sq_scale, int64_t moments, int32_t bits, int32_t p_type, int32_t g_type, double lr, double beta1,
+                     double beta2, double eps, double weight_decay, int64_t step, float grad_scale, float max_norm, const float* norm, uint64_t seed,
+                     uint32_t stream_index, uint32_t flags, haste_stream_t stream) {
+  const char* who = "haste_adamw_step";
+  int64_t need = 0;
+  if (int rc = check_tensors(who, grads, sizes, count, &need)) return rc;
+  if (int rc = check_type(who, "parameter", p_type)) return rc;
+  if (int rc = check_type(who, "gradient", g_type)) return rc;
+  if (bits != 8 && bits != 32) return fail(HASTE_ERR_UNSUPPORTED, "%s: moments of %d bits (8 or 32 are supported)", who, bits);
+  if (!(lr >= 0.0 && is_finite(lr) && weight_decay >= 0.0 && is_finite(weight_decay))) return fail(HASTE_ERR_BAD_ARG, "%s: lr and weight_decay must not be negative", who);
+  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) return fail(HASTE_ERR_BAD_ARG, "%s: betas must be in [0, 1)", who);
+  if (!(eps > 0.0 && is_finite(eps))) return fail(HASTE_ERR_BAD_ARG, "%s: eps must be positive", who);
+  if (step < 1) return fail(HASTE_ERR_BAD_ARG, "%s: step=%lld (the first step is 1)", who, (long long)step);
+  if (!is_finite(grad_scale)) return fail(HASTE_ERR_BAD_ARG, "%s: grad_scale must be finite", who);
+  if (norm != nullptr && !(max_norm > 0.f)) return fail(HASTE_ERR_BAD_ARG, "%s: max_norm must be positive", who);
+  if (moments < need) return fail(HASTE_ERR_BAD_ARG, "%s: moments of %lld elements, %lld needed", who, (long long)moments, (long long)need);
+  if (need == 0) return HASTE_OK;
+  REQUIRE_PTR(params, who); REQUIRE_PTR(exp_avg, who); REQUIRE_PTR(exp_avg_sq, who); REQUIRE_ALIGNED(exp_avg, who); REQUIRE_ALIGNED(exp_avg_sq, who);
+  if (bits == 8) { REQUIRE_PTR(exp_avg_scale, who); REQUIRE_PTR(exp_avg_sq_scale, who); }
+  for (int64_t i = 0; i < count; ++i)
+    if (grads[i] != nullptr && sizes[i] > 0 && params[i] == nullptr) return fail(HASTE_ERR_BAD_ARG, "%s: parameter %lld is NULL", who, (long long)i);
+  AdamWCall c;
+  c.params = params; c.grads = grads; c.sizes = sizes; c.count = count;
+  c.exp_avg = exp_avg; c.exp_avg_sq = exp_avg_sq; c.avg_scale = exp_avg_scale; c.sq_scale = exp_avg_sq_scale;
+  c.bits = bits; c.p_type = p_type; c.g_type = g_type;
+  c.lr = lr; c.beta1 = beta1; c.beta2 = beta2; c.eps = eps; c.weight_decay = weight_decay; c.step = step;
+  c.grad_scale = grad_scale; c.max_norm = max_norm; c.norm = norm; c.seed = seed; c.stream = stream_index; c.flags = flags;
+  return launch_adamw(c, static_cast<cudaStream_t>(stream));
+}
+
+int haste_grad_norm(const void* const* grads, const int32_t* types, const int64_t* sizes, int64_t count, float grad_scale, float* scratch, float* norm,
+                    haste_stream_t stream) {
+  const char* who = "haste_grad_norm";
+  int64_t need = 0;
+  if (int rc = check_tensors(who, grads, sizes, count, &need)) return rc;
+  REQUIRE_PTR(norm, who); REQUIRE_PTR(scratch, who);
+  if (count > 0) REQUIRE_PTR(types, who);
+  if (!is_finite(grad_scale)) return fail(HASTE_ERR_BAD_ARG, "%s: grad_scale must be finite", who);
+  for (int64_t i = 0; i < count; ++i) {
+    if (int rc = check_type(who, "gradient", types[i])) return rc;
+    if (sizes[i] > 0 && grads[i] == nullptr) return fail(HASTE_ERR_BAD_ARG, "%s: gradient %lld is NULL", who, (long long)i);
+  }
+  return launch_grad_norm(grads, types, sizes, count, grad_scale, scratch, norm, static_cast<cudaStream_t>(stream));
+}
+
+int haste_quantize_moment(const float* x, uint8_t* codes, float* scales, int64_t n, int32_t is_signed, haste_stream_t stream) {
+  const char* who = "haste_quantize_moment";
+  if (n < 0 || n % 256 != 0) return fail(HASTE_ERR_BAD_ARG, "%s: n=%lld must be a multiple of 256", who, (long long)n);
+  if (n > 0) { REQUIRE_PTR(x, who); REQUIRE_PTR(codes, who); REQUIRE_PTR(scales, who); REQUIRE_ALIGNED(x, who); REQUIRE_ALIGNED(codes, who); }
+  return launch_quantize(x, codes, scales, n, is_signed, static_cast<cudaStream_t>(stream));
+}
+
+int haste_dequantize_moment(const uint8_t* codes, const float* scales, void* out, int64_t n, int32_t is_signed, int32_t out_type, haste_stream_t stream) {
+  const char* who = "haste_dequantize_moment";
+  if (n < 0 || n % 256 != 0) return fail(HASTE_ERR_BAD_ARG, "%s: n=%lld must be a multiple of 256", who, (long long)n);
+  if (int rc = check_type(who, "output", out_type)) return rc;
+  if (n > 0) { REQUIRE_PTR(codes, who); REQUIRE_PTR(scales, who); REQUIRE_PTR(out, who); REQUIRE_ALIGNED(codes, who); REQUIRE_ALIGNED(out, who); }
+  return launch_dequantize(codes, scales, out, n, is_signed, out_type, static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

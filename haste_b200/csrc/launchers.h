@@ -151,4 +151,26 @@ int64_t layer_norm_backward_scratch(int64_t rows, int64_t D);      // floats
 int launch_layer_norm_backward(const void* dy, const void* x, const void* w, const float* mean, const float* rstd, void* dx, void* dw, void* db,
                                float* scratch, int64_t rows, int64_t D, int64_t lddy, int64_t ldx, int x_type, int dy_type, int w_type, cudaStream_t st);
 
+// AdamW and gradient norm (adamw.cu)
+struct AdamWCall {
+  void* const* params;               // host arrays of `count` device pointers and sizes; a NULL gradient: the tensor is left alone
+  const void* const* grads;
+  const int64_t* sizes;
+  int64_t count;
+  void *exp_avg, *exp_avg_sq;        // of all tensors, each at a multiple of 256 elements: fp32, or codes with their scales
+  float *avg_scale, *sq_scale;
+  int bits, p_type, g_type;
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;
+  float grad_scale, max_norm;
+  const float* norm;                 // device; NULL: not clipped
+  uint64_t seed;
+  uint32_t stream, flags;
+};
+int launch_adamw(const AdamWCall& c, cudaStream_t st);
+int launch_grad_norm(const void* const* grads, const int32_t* types, const int64_t* sizes, int64_t count, float grad_scale, float* partial, float* norm,
+                     cudaStream_t st);
+int launch_quantize(const float* x, uint8_t* codes, float* scales, int64_t n, int is_signed, cudaStream_t st);
+int launch_dequantize(const uint8_t* codes, const float* scales, void* out, int64_t n, int is_signed, int type, cudaStream_t st);
+
 }  // namespace haste

@@ -3,6 +3,7 @@
 PyTorch is used for device memory and streams only.  Every function validates what the C side cannot
 see (device, dtype, contiguity) and raises RuntimeError otherwise.
 """
+import array
 import contextlib
 
 import torch
@@ -479,6 +480,117 @@ def layer_norm_backward(dy, x, weight, mean, rstd, want_weight=True, want_bias=T
         check(lib.haste_layer_norm_backward(_ptr(grad), _ptr(src), _ptr(weight), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dw), _ptr(db), _ptr(scratch), n,
                                             rows, D, lddy, ldx, x_type, dy_type, w_type, _stream(x)), "layer_norm_backward")
     return dx, dw, db
+
+
+# ---------------------------------------------------------------- AdamW and gradient norm over many tensors
+MOMENT_BLOCK = 256           # elements of a moment that share a scale; every tensor's moments start at a multiple of it
+
+
+def _tensor_list(tensors, what):
+    """(device index, [device pointers], array of sizes) of a list of contiguous CUDA tensors; None has pointer and size 0."""
+    dev, ptrs, sizes = None, [], array.array("q")
+    for t in tensors:
+        if t is None:
+            ptrs.append(0)
+            sizes.append(0)
+            continue
+        d = t.get_device()
+        if d != dev:
+            if d < 0 or dev is not None:
+                raise RuntimeError(f"{what} must be CUDA tensors on one device (this library has no CPU path)")
+            dev = d
+        if not t.is_contiguous():
+            raise RuntimeError(f"{what} must be contiguous")
+        ptrs.append(t.data_ptr())
+        sizes.append(t.numel())
+    return dev, ptrs, sizes
+
+
+def _addresses(ptrs):
+    """Host array of pointers: keep the result until the call has returned."""
+    return array.array("Q", ptrs)
+
+
+def grad_norm(grads, grad_scale=1.0):
+    """2-norm of all tensors of ``grads`` (bf16 or fp32, mixed or not) together, times |grad_scale|: fp32 scalar on the device, the same bits
+    on every call."""
+    grads = [g for g in grads if g is not None]
+    if not grads:
+        raise RuntimeError("grad_norm needs at least one tensor")
+    dev, ptrs, sizes = _tensor_list(grads, "gradients")
+    try:
+        types = array.array("i", [_TYPES[g.dtype] for g in grads])
+    except KeyError as e:
+        raise RuntimeError(f"gradients must be torch.bfloat16 or torch.float32, got {e}") from None
+    device = grads[0].device
+    with _on(device):
+        buf = torch.empty(1 + _lib.GRAD_NORM_PARTIALS, dtype=torch.float32, device=device)
+        norm = buf[0]
+        ptrs = _addresses(ptrs)
+        check(lib.haste_grad_norm(ptrs.buffer_info()[0], types.buffer_info()[0], sizes.buffer_info()[0], len(types), grad_scale, _ptr(buf) + 4, _ptr(norm),
+                                  _raw_stream(dev)), "grad_norm")
+    return norm
+
+
+def adamw_step(params, grads, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, bits, *, step, lr, betas, eps, weight_decay, grad_scale=1.0, norm=None,
+               max_norm=0.0, seed=123, stream_index=0, flags=0):
+    """One launch of the AdamW kernel (haste_adamw_step).  ``grads`` may hold None: that tensor is left alone."""
+    if len(params) != len(grads):
+        raise RuntimeError(f"{len(params)} parameters and {len(grads)} gradients")
+    dev, ptrs, sizes = _tensor_list(params, "parameters")
+    gdev, gptrs, _ = _tensor_list(grads, "gradients")
+    if gdev is None:
+        return                                           # nothing to do
+    if dev != gdev:
+        raise RuntimeError("parameters and gradients must be on one device")
+    p_dtype, g_dtype = params[0].dtype, next(g.dtype for g in grads if g is not None)
+    for p, g in zip(params, grads):
+        if p.dtype != p_dtype or (g is not None and (g.dtype != g_dtype or g.shape != p.shape)):
+            raise RuntimeError("all parameters must have one type, all gradients one type, and every gradient its parameter's shape")
+    p_type, g_type = _type_of(params[0], "parameters"), _TYPES.get(g_dtype)
+    if g_type is None:
+        raise RuntimeError(f"gradients must be torch.bfloat16 or torch.float32, got {g_dtype}")
+    device = params[0].device
+    for t in (exp_avg, exp_avg_sq):
+        _req(t, "moments", torch.float32 if bits == 32 else torch.uint8)
+    if bits == 8:
+        for t in (exp_avg_scale, exp_avg_sq_scale):
+            _req(t, "scales", torch.float32)
+            if t.numel() * MOMENT_BLOCK < exp_avg.numel():
+                raise RuntimeError(f"scales must hold one value per {MOMENT_BLOCK} elements of the moments")
+    if exp_avg.numel() != exp_avg_sq.numel() or any(t is not None and t.device != device for t in (exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale)):
+        raise RuntimeError("both moments must be of one size, on the parameters' device")
+    if norm is not None:
+        _req(norm, "norm", torch.float32)
+        if norm.numel() != 1 or norm.device != device:
+            raise RuntimeError("norm must be one fp32 value on the parameters' device")
+    ptrs, gptrs = _addresses(ptrs), _addresses(gptrs)
+    with _on(device):
+        check(lib.haste_adamw_step(ptrs.buffer_info()[0], gptrs.buffer_info()[0], sizes.buffer_info()[0], len(ptrs), _ptr(exp_avg), _ptr(exp_avg_scale),
+                                   _ptr(exp_avg_sq), _ptr(exp_avg_sq_scale), exp_avg.numel(), bits, p_type, g_type, lr, betas[0], betas[1], eps, weight_decay,
+                                   step, grad_scale, max_norm, _ptr(norm), seed & 0xFFFFFFFFFFFFFFFF, stream_index, flags, _raw_stream(dev)), "adamw_step")
+
+
+def quantize_moment(x, signed):
+    """(codes uint8, scales fp32) of fp32 values, a multiple of 256 of them, rounded to the nearest code."""
+    _req(x, "x", torch.float32)
+    codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(x.numel() // MOMENT_BLOCK, dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        check(lib.haste_quantize_moment(_ptr(x), _ptr(codes), _ptr(scales), x.numel(), int(signed), _stream(x)), "quantize_moment")
+    return codes, scales
+
+
+def dequantize_moment(codes, scales, signed, dtype=torch.float32):
+    _req(codes, "codes", torch.uint8); _req(scales, "scales", torch.float32)
+    if scales.numel() * MOMENT_BLOCK != codes.numel() or scales.device != codes.device:
+        raise RuntimeError(f"scales must hold one value per {MOMENT_BLOCK} codes, on their device")
+    if dtype not in _TYPES:
+        raise RuntimeError(f"dtype must be torch.bfloat16 or torch.float32, got {dtype}")
+    out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    with _on(codes.device):
+        check(lib.haste_dequantize_moment(_ptr(codes), _ptr(scales), _ptr(out), codes.numel(), int(signed), _TYPES[dtype], _stream(codes)), "dequantize_moment")
+    return out
 
 
 def check_locations(loc, D):

@@ -374,6 +374,40 @@ int haste_layer_norm_backward(const void* dy, const void* x, const void* w, cons
                               void* scratch, int64_t scratch_bytes, int64_t rows, int64_t D, int64_t lddy, int64_t ldx, int32_t x_type, int32_t dy_type,
                               int32_t w_type, haste_stream_t stream);
 
+/* One AdamW step over `count` tensors in one launch (per 1024 tensors), for the dense parameters next to this layer:
+ *   g = grad * grad_scale * min(1, max_norm / (*norm + 1e-6))         (without the last factor when norm is NULL)
+ *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2
+ *   w = w (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * in fp32.  params, grads, sizes: host arrays of `count` device pointers and element counts, read before the call returns; the
+ * parameters all of p_type, the gradients of g_type, both contiguous, aligned as their type.  A tensor whose gradient is NULL is left
+ * alone.  bf16 parameters are rounded stochastically with HASTE_F_SR, else to nearest.
+ * The moments of all tensors lie in one buffer each (16-byte aligned, `moments` elements of room), tensor after tensor, every one at a
+ * multiple of 256 elements: fp32 (bits = 32, no scales), or codes of 8 bits (bits = 8) and one fp32 scale per 256 elements.  Zeros before the
+ * first step.  A code c stands for scale times
+ *   first moment    0 for c % 128 = 0, else +-(1 + (c % 8) / 8) 2^((c % 128) / 8 - 15), negative for c > 127
+ *   second moment   0 for c = 0, else (1 + (c % 8) / 8) 2^(c / 8 - 31)                        (divisions of integers)
+ * and is rounded stochastically.  A block with a value that is inf or NaN has scale NaN.
+ * Random bits: Philox4x32 with 7 rounds, key (lower half of seed, step), counter (i, i >> 32, stream_index, 1) for elements 4i .. 4i+3 of the
+ * buffers, one word each: bits 0-15 for the parameter, 16-23 for the first, 24-31 for the second moment.  Calls that update other tensors in
+ * the same step need another stream_index.
+ * norm (device, fp32; from haste_grad_norm with the same grad_scale): where it is inf or NaN, nothing is changed.
+ * (The reference's training loop takes AdamW from packages that are not part of it: src/runner.py:8-10, 22.) */
+int haste_adamw_step(void* const* params, const void* const* grads, const int64_t* sizes, int64_t count, void* exp_avg, float* exp_avg_scale,
+                     void* exp_avg_sq, float* exp_avg_sq_scale, int64_t moments, int32_t bits, int32_t p_type, int32_t g_type, double lr, double beta1,
+                     double beta2, double eps, double weight_decay, int64_t step, float grad_scale, float max_norm, const float* norm, uint64_t seed,
+                     uint32_t stream_index, uint32_t flags, haste_stream_t stream);
+
+/* 2-norm of all gradients together, times |grad_scale|, into *norm (device): sums of squares in fp32, joined in 64 bits in an order
+ * that depends on the sizes alone.  types: one of HASTE_BF16 / HASTE_F32 per tensor.  scratch: HASTE_GRAD_NORM_PARTIALS floats of device memory.  No tensors: 0. */
+#define HASTE_GRAD_NORM_PARTIALS 4096
+int haste_grad_norm(const void* const* grads, const int32_t* types, const int64_t* sizes, int64_t count, float grad_scale, float* scratch, float* norm,
+                    haste_stream_t stream);
+
+/* The 8-bit form of moments on its own, for checkpoints: n (a multiple of 256) fp32 values to codes (nearest) and scales, and back to
+ * bf16 or fp32.  is_signed: as the first moment, else as the second (no negative values).  x, codes and out 16-byte aligned. */
+int haste_quantize_moment(const float* x, uint8_t* codes, float* scales, int64_t n, int32_t is_signed, haste_stream_t stream);
+int haste_dequantize_moment(const uint8_t* codes, const float* scales, void* out, int64_t n, int32_t is_signed, int32_t out_type, haste_stream_t stream);
+
 /* Rate probes (measurement only; timed by the benchmark's auxiliary mode; no counterpart in the reference).  Each
  * isolates one access pattern of the fused train step at the step's own sizes:
  *   haste_probe_red_rate     fp32 reduce-add of `tiles_per_cta` tiles of 64 rows x 128 floats per SM into dxt [D,B]
