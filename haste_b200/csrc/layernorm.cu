@@ -7,10 +7,11 @@
 // All sums are fp32; the variance is taken around the mean, not from the sum of squares, which cancels for rows whose mean is large
 // against their spread.  Inputs and outputs are bf16 or fp32, rounded once (nearest even) when stored.
 //
-// Memory bounds all of it: x in and y out, or dy and x in and dx out.  A row is read once and stays in registers: a group of 1 to 32
-// lanes of a warp has it, or a thread block where it is wider, each thread up to 4 vectors of 16 bytes (16 single elements where rows
-// do not start on 16 bytes).  Groups walk over the rows with the next row's loads in flight, so that in the backward pass a thread owns
-// its columns for good and sums dw and db in registers; the blocks' sums go to memory and are added in a second, small launch.
+// Memory bounds all of it: x in and y out, or dy and x in and dx out.  A row is read once and stays on the chip: 1 to 32 lanes of a
+// warp have it, or a thread block where it is wider, each thread up to 4 vectors of 16 bytes.  These groups walk over the rows with the
+// next rows on their way, so that in the backward pass a thread owns its columns for good and sums dw and db in registers; the blocks'
+// sums go to memory and are added in a second, small launch.  Rows of more than 8192 elements (16384 bf16 in the forward pass) are
+// read again for each pass.
 #include "common.cuh"
 
 #include <atomic>
@@ -139,53 +140,72 @@ __global__ void __launch_bounds__(LN_FINISH_THREADS) ln_bwd_finish_kernel(const 
   }
 }
 
-// ---------------------------------------------------------------- rows that stay in registers
-// VEC elements of type T as they lie in memory (a single element: as fp32).
-template <class T, int VEC> struct Raw;
-template <> struct Raw<__nv_bfloat16, 8> {
-  uint4 v;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldcs(reinterpret_cast<const uint4*>(p)); }
-  __device__ __forceinline__ void clear() { v = make_uint4(0u, 0u, 0u, 0u); }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// ---------------------------------------------------------------- rows that stay on the chip
+// A row is cut at the 16-byte boundaries of the (contiguous, aligned) output, so that vector q of a row holds its columns
+// q VEC - s .. q VEC - s + VEC - 1, s being the row's distance from the boundary before it; of the first and the last vector a part may
+// belong to the neighbouring rows.  Groups of threads take rows at distances that are multiples of VEC: s stays the same, and a thread
+// its columns.  An input whose rows have the same s (contiguous ones do) is copied in vectors as well, any other element by element.
+//
+// Each thread copies its own vectors of the row after next into its own slots of shared memory (cp.async: no registers, no barrier) while
+// it works on the row that has arrived.  What lies outside the row or the rows reads as zero, so that most sums need no masks: the copies
+// fill up with zeros, and of a row's first vector the part before the row is dropped when it is read.
+__device__ __forceinline__ uint32_t smem_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+// 16 bytes (8, 4), of which `bytes` are read and the rest become zeros
+__device__ __forceinline__ void copy_async16(void* dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_address(dst)), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_async8(void* dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_address(dst)), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+constexpr int LN_STAGES = 3;              // rows on their way or at work, per group
+constexpr int LN_WARP_THREADS = 128;      // block of the variant whose groups are within a warp
+
+// VEC elements of type T in a slot: WORDS accesses of 16 bytes (one of 8 for 4 bf16), `step` bytes apart, so that the lanes of a
+// warp touch consecutive 16 bytes each time.
+template <class T, int VEC> struct Slot {
+  static constexpr int BYTES = VEC * static_cast<int>(sizeof(T)), WORDS = (BYTES + 15) / 16, UNIT = BYTES < 16 ? BYTES : 16, PER = UNIT / static_cast<int>(sizeof(T));
+  // n: how many of the elements exist (from the first on)
+  static __device__ __forceinline__ void copy(char* dst, int step, const T* src, int n) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+    for (int k = 0; k < WORDS; ++k) {
+      const int left = (n - k * PER) * static_cast<int>(sizeof(T)), bytes = left < 0 ? 0 : left < UNIT ? left : UNIT;
+      const T* from = bytes > 0 ? src + k * PER : src;
+      if (UNIT == 16) copy_async16(dst + k * step, from, bytes); else copy_async8(dst + k * step, from, bytes);
+    }
   }
-};
-template <> struct Raw<__nv_bfloat16, 4> {
-  uint2 v;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldcs(reinterpret_cast<const uint2*>(p)); }
-  __device__ __forceinline__ void clear() { v = make_uint2(0u, 0u); }
-  __device__ __forceinline__ void get(float (&f)[4]) const {
-    f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xFFFF0000u); f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xFFFF0000u);
-  }
-};
-template <int VEC> struct Raw<float, VEC> {
-  float4 v[VEC / 4];
-  __device__ __forceinline__ void load(const float* p) {
+  static __device__ void copy_single(char* dst, int step, const T* src, int first, int n) {      // elements first .. n-1, zeros elsewhere
 #pragma unroll
-    for (int i = 0; i < VEC / 4; ++i) v[i] = __ldcs(reinterpret_cast<const float4*>(p) + i);
+    for (int e = 0; e < VEC; ++e) {
+      T v;
+      st_f(&v, 0.f);
+      if (e >= first && e < n) v = src[e];
+      reinterpret_cast<T*>(dst + e / PER * step)[e % PER] = v;
+    }
   }
-  __device__ __forceinline__ void clear() {
+  // MASK: the elements before `first` belong to another row and read as 0
+  template <bool MASK>
+  static __device__ __forceinline__ void get(const char* src, int step, float (&f)[VEC], int first) {
 #pragma unroll
-    for (int i = 0; i < VEC / 4; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-  __device__ __forceinline__ void get(float (&f)[VEC]) const {
+    for (int k = 0; k < WORDS; ++k) {
+      if constexpr (sizeof(T) == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src + k * step);
+        f[4 * k] = v.x; f[4 * k + 1] = v.y; f[4 * k + 2] = v.z; f[4 * k + 3] = v.w;
+      } else {
+        uint32_t u[PER / 2];
+        if constexpr (UNIT == 16) { const uint4 v = *reinterpret_cast<const uint4*>(src + k * step); u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w; }
+        else { const uint2 v = *reinterpret_cast<const uint2*>(src + k * step); u[0] = v.x; u[1] = v.y; }
 #pragma unroll
-    for (int i = 0; i < VEC / 4; ++i) { f[4 * i] = v[i].x; f[4 * i + 1] = v[i].y; f[4 * i + 2] = v[i].z; f[4 * i + 3] = v[i].w; }
+        for (int e = 0; e < PER / 2; ++e) { f[2 * e] = __uint_as_float(u[e] << 16); f[2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u); }
+      }
+    }
+    if (MASK) {
+#pragma unroll
+      for (int e = 0; e < VEC - 1; ++e) f[e] = e < first ? 0.f : f[e];
+    }
   }
-};
-template <> struct Raw<float, 1> {
-  float v;
-  __device__ __forceinline__ void load(const float* p) { v = __ldcs(p); }
-  __device__ __forceinline__ void clear() { v = 0.f; }
-  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = v; }
-};
-template <> struct Raw<__nv_bfloat16, 1> {
-  float v;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __bfloat162float(__ldcs(p)); }
-  __device__ __forceinline__ void clear() { v = 0.f; }
-  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = v; }
 };
 
 __device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&f)[8]) {
@@ -198,38 +218,51 @@ __device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&f)[8])
   __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
 }
 __device__ __forceinline__ void store_vec(float* p, const float (&f)[4]) { __stcs(reinterpret_cast<float4*>(p), make_float4(f[0], f[1], f[2], f[3])); }
-template <class T>
-__device__ __forceinline__ void store_vec(T* p, const float (&f)[1]) { st_f(p, f[0]); }
+// Columns j0 .. of a row: the whole vector, or those of its elements that belong to the row.
+template <class T, int VEC>
+__device__ __forceinline__ void store_row(T* row, int j0, int D, const float (&f)[VEC]) {
+  if (j0 >= 0 && j0 + VEC <= D) store_vec(row + j0, f);
+  else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) if (j0 + k >= 0 && j0 + k < D) st_f(row + j0 + k, f[k]);
+  }
+}
 
-// Weights j .. j+VEC-1: hot in L1 (x and dy go past it), so they are read for every row rather than held in registers.
+// Weights of a thread's columns, once per kernel; 0 outside the row.  vec: whole vectors only, on 16 bytes.
 template <int VEC>
-__device__ __forceinline__ void load_weights(const void* w, int w_type, int64_t j, float fill, float (&f)[VEC]) {
+__device__ __forceinline__ void load_weights(const void* w, int w_type, bool vec, int j0, int D, float fill, float (&f)[VEC]) {
   if (w == nullptr) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = fill;
+    for (int k = 0; k < VEC; ++k) f[k] = static_cast<unsigned>(j0 + k) < static_cast<unsigned>(D) ? fill : 0.f;
   } else if (w_type == HASTE_BF16) {
-    const uint16_t* p = static_cast<const uint16_t*>(w) + j;
-    if constexpr (VEC == 8) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(u[i] << 16); f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u); }
-    } else if constexpr (VEC == 4) {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-      f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xFFFF0000u); f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xFFFF0000u);
-    } else {
-      f[0] = bf16_bits_to_float(__ldg(p));
-    }
-  } else {
-    const float* p = static_cast<const float*>(w) + j;
-    if constexpr (VEC >= 4) {
-#pragma unroll
-      for (int i = 0; i < VEC / 4; ++i) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(p) + i);
-        f[4 * i] = v.x; f[4 * i + 1] = v.y; f[4 * i + 2] = v.z; f[4 * i + 3] = v.w;
+    const uint16_t* p = static_cast<const uint16_t*>(w) + j0;
+    uint32_t u[VEC];
+    if (vec) {
+      if constexpr (VEC == 8) {
+        const uint4 v = j0 < D ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0u, 0u, 0u, 0u);
+        u[0] = v.x << 16; u[1] = v.x & 0xFFFF0000u; u[2] = v.y << 16; u[3] = v.y & 0xFFFF0000u;
+        u[4] = v.z << 16; u[5] = v.z & 0xFFFF0000u; u[6] = v.w << 16; u[7] = v.w & 0xFFFF0000u;
+      } else {
+        const uint2 v = j0 < D ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0u, 0u);
+        u[0] = v.x << 16; u[1] = v.x & 0xFFFF0000u; u[2] = v.y << 16; u[3] = v.y & 0xFFFF0000u;
       }
     } else {
-      f[0] = __ldg(p);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) u[k] = static_cast<unsigned>(j0 + k) < static_cast<unsigned>(D) ? static_cast<uint32_t>(__ldg(p + k)) << 16 : 0u;
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) f[k] = __uint_as_float(u[k]);
+  } else {
+    const float* p = static_cast<const float*>(w) + j0;
+    if (vec) {
+#pragma unroll
+      for (int k = 0; k < VEC; k += 4) {
+        const float4 v = j0 < D ? __ldg(reinterpret_cast<const float4*>(p + k)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        f[k] = v.x; f[k + 1] = v.y; f[k + 2] = v.z; f[k + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) f[k] = static_cast<unsigned>(j0 + k) < static_cast<unsigned>(D) ? __ldg(p + k) : 0.f;
     }
   }
 }
@@ -270,176 +303,224 @@ struct RowGroup {
   }
 };
 
-constexpr int LN_WARP_THREADS = 128;      // block of the variant whose groups are within a warp
+struct Sums {            // partial sums that do not wait for one another
+  float v[4];
+  __device__ __forceinline__ Sums() : v{0.f, 0.f, 0.f, 0.f} {}
+  __device__ __forceinline__ float total() const { return (v[0] + v[1]) + (v[2] + v[3]); }
+};
 
-template <class X, int VEC, int NV, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 512 : LN_WARP_THREADS) ln_fwd_kernel(const X* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b,
-                                                                              int w_type, X* __restrict__ y, float* __restrict__ mean_out,
-                                                                              float* __restrict__ rstd_out, int64_t rows, int D, int64_t ldx, float eps, int t) {
+// EDGE: D is no multiple of VEC, rows have first and last vectors that are theirs in part.
+template <class X, int VEC, int NV, bool BLOCK, bool EDGE>
+__global__ void __launch_bounds__(BLOCK ? 512 : LN_WARP_THREADS, BLOCK ? 1 : 4)
+    ln_fwd_kernel(const X* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b, int w_type, X* __restrict__ y, float* __restrict__ mean_out,
+                  float* __restrict__ rstd_out, int64_t rows, int D, int64_t ldx, float eps, int t, bool x_vec, bool w_vec) {
+  using SX = Slot<X, VEC>;
   __shared__ float buf[2][1][16];
+  extern __shared__ __align__(16) char slots[];
   RowGroup<BLOCK> grp(t);
+  const int step = blockDim.x * SX::UNIT, row_bytes = NV * SX::WORDS * step;
+  char* const mine = slots + threadIdx.x * SX::UNIT;
   const float inv_d = 1.f / static_cast<float>(D);
-  Raw<X, VEC> cur[NV], nxt[NV];
-  auto fetch = [&](int64_t r, Raw<X, VEC> (&v)[NV]) {
-    const X* xr = x + r * ldx;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j = (grp.c + i * grp.T) * VEC;
-      if (r < rows && j < D) v[i].load(xr + j); else v[i].clear();
-    }
-  };
+  const int64_t stride = grp.stride();
   int64_t r0 = grp.first_row();
-  fetch(r0 + grp.own(), cur);
-  for (; r0 < rows; r0 += grp.stride()) {
+  const int s = EDGE ? static_cast<int>((r0 + grp.own()) * D % VEC) : 0, first = grp.c == 0 ? s : 0;
+  auto fetch = [&](int64_t from_row, int stage) {
+    const int64_t r = from_row + grp.own();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j0 = (grp.c + i * grp.T) * VEC - s, n = r < rows ? D - j0 : 0;
+      char* to = mine + stage * row_bytes + i * SX::WORDS * step;
+      const X* from = n > 0 ? x + r * ldx + j0 : x;
+      if (x_vec) SX::copy(to, step, from, n); else SX::copy_single(to, step, from, -j0, n);
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int k = 0; k < LN_STAGES - 1; ++k) fetch(r0 + k * stride, k);
+  float wf[NV][VEC], bf[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j0 = (grp.c + i * grp.T) * VEC - s;
+    load_weights<VEC>(w, w_type, !EDGE && w_vec, j0, D, 1.f, wf[i]);
+    load_weights<VEC>(b, w_type, !EDGE && w_vec, j0, D, 0.f, bf[i]);
+  }
+  for (int stage = 0; r0 < rows; r0 += stride, stage = stage + 1 < LN_STAGES ? stage + 1 : 0) {
     const int64_t r = r0 + grp.own();
-    fetch(r + grp.stride(), nxt);
-    float s[1] = {0.f};
+    copies_wait<LN_STAGES - 2>();
+    fetch(r0 + (LN_STAGES - 1) * stride, stage == 0 ? LN_STAGES - 1 : stage - 1);      // where the last row was
+    float f[NV][VEC];
+    Sums s1, s2;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float f[VEC];
-      cur[i].get(f);
+      if (i == 0) SX::template get<EDGE>(mine + stage * row_bytes, step, f[0], first);
+      else SX::template get<false>(mine + stage * row_bytes + i * SX::WORDS * step, step, f[i], 0);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) s[0] += f[k];
+      for (int k = 0; k < VEC; ++k) s1.v[k & 3] += f[i][k];
     }
-    grp.sum(s, buf);
-    const float mean = s[0] * inv_d;
-    s[0] = 0.f;
+    float sum[1] = {s1.total()};
+    grp.sum(sum, buf);
+    const float mean = sum[0] * inv_d;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float f[VEC];
-      cur[i].get(f);
-      const bool in = (grp.c + i * grp.T) * VEC < D;
+      const int j0 = (grp.c + i * grp.T) * VEC - s;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) { const float d = f[k] - mean; if (in) s[0] = fmaf(d, d, s[0]); }
+      for (int k = 0; k < VEC; ++k) {
+        const bool in = EDGE ? static_cast<unsigned>(j0 + k) < static_cast<unsigned>(D) : j0 < D;
+        f[i][k] -= mean;
+        if (in) s2.v[k & 3] = fmaf(f[i][k], f[i][k], s2.v[k & 3]);
+      }
     }
-    grp.sum(s, buf);
-    const float rstd = 1.f / sqrtf(fmaf(s[0], inv_d, eps));
+    sum[0] = s2.total();
+    grp.sum(sum, buf);
+    const float rstd = 1.f / sqrtf(fmaf(sum[0], inv_d, eps));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = (grp.c + i * grp.T) * VEC;
-      if (r < rows && j < D) {
-        float f[VEC], wf[VEC], bf[VEC];
-        cur[i].get(f);
-        load_weights<VEC>(w, w_type, j, 1.f, wf);
-        load_weights<VEC>(b, w_type, j, 0.f, bf);
+      const int j0 = (grp.c + i * grp.T) * VEC - s;
+      if (r < rows && j0 < D) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) f[k] = fmaf((f[k] - mean) * rstd, wf[k], bf[k]);
-        store_vec(y + r * D + j, f);
+        for (int k = 0; k < VEC; ++k) f[i][k] = fmaf(f[i][k] * rstd, wf[i][k], bf[i][k]);
+        if (EDGE) store_row<X, VEC>(y + r * D, j0, D, f[i]); else store_vec(y + r * D + j0, f[i]);
       }
     }
     if (grp.c == 0 && r < rows && mean_out != nullptr) { mean_out[r] = mean; rstd_out[r] = rstd; }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) cur[i] = nxt[i];
   }
+  copies_wait<0>();
 }
 
 // dx, and the block's part of dw and db: partial[block][0][.] and [1][.] (NULL: only dx is wanted).
-template <class X, class G, int VEC, int NV, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? (VEC * NV > 16 ? 256 : 512) : LN_WARP_THREADS)
+template <class X, class G, int VEC, int NV, bool BLOCK, bool EDGE>
+__global__ void __launch_bounds__(BLOCK ? (VEC * NV > 16 ? 256 : 512) : LN_WARP_THREADS) __maxnreg__(VEC * NV > 16 ? 168 : 128)
     ln_bwd_kernel(const G* __restrict__ dy, const X* __restrict__ x, const void* __restrict__ w, int w_type, const float* __restrict__ mean_in,
-                  const float* __restrict__ rstd_in, X* __restrict__ dx, float* __restrict__ partial, int64_t rows, int D, int64_t lddy, int64_t ldx, int t) {
+                  const float* __restrict__ rstd_in, X* __restrict__ dx, float* __restrict__ partial, int64_t rows, int D, int64_t lddy, int64_t ldx, int t,
+                  bool x_vec, bool dy_vec, bool w_vec) {
+  using SX = Slot<X, VEC>;
+  using SG = Slot<G, VEC>;
   __shared__ float buf[2][2][16];
+  extern __shared__ __align__(16) char slots[];
   RowGroup<BLOCK> grp(t);
+  const int xstep = blockDim.x * SX::UNIT, gstep = blockDim.x * SG::UNIT, x_bytes = NV * SX::WORDS * xstep, row_bytes = x_bytes + NV * SG::WORDS * gstep;
+  char* const my_x = slots + threadIdx.x * SX::UNIT;
+  char* const my_g = slots + x_bytes + threadIdx.x * SG::UNIT;
   const float inv_d = 1.f / static_cast<float>(D);
-  float aw[NV][VEC], ab[NV][VEC];
+  const int64_t stride = grp.stride();
+  int64_t r0 = grp.first_row();
+  const int s = EDGE ? static_cast<int>((r0 + grp.own()) * D % VEC) : 0, first = grp.c == 0 ? s : 0;
+  auto fetch = [&](int64_t from_row, int stage) {
+    const int64_t r = from_row + grp.own();
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      const int j0 = (grp.c + i * grp.T) * VEC - s, n = r < rows ? D - j0 : 0;
+      char* xto = my_x + stage * row_bytes + i * SX::WORDS * xstep;
+      char* gto = my_g + stage * row_bytes + i * SG::WORDS * gstep;
+      const X* xfrom = n > 0 ? x + r * ldx + j0 : x;
+      const G* gfrom = n > 0 ? dy + r * lddy + j0 : dy;
+      if (x_vec) SX::copy(xto, xstep, xfrom, n); else SX::copy_single(xto, xstep, xfrom, -j0, n);
+      if (dy_vec) SG::copy(gto, gstep, gfrom, n); else SG::copy_single(gto, gstep, gfrom, -j0, n);
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int k = 0; k < LN_STAGES - 1; ++k) fetch(r0 + k * stride, k);
+  float wf[NV][VEC], aw[NV][VEC], ab[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    load_weights<VEC>(w, w_type, !EDGE && w_vec, (grp.c + i * grp.T) * VEC - s, D, 1.f, wf[i]);
 #pragma unroll
     for (int k = 0; k < VEC; ++k) aw[i][k] = ab[i][k] = 0.f;
-  Raw<X, VEC> cx[NV], nx[NV];
-  Raw<G, VEC> cg[NV], ng[NV];
-  float cmean, crstd, nmean, nrstd;
-  auto fetch = [&](int64_t r, Raw<X, VEC> (&xv)[NV], Raw<G, VEC> (&gv)[NV], float& mean, float& rstd) {
-    const X* xr = x + r * ldx;
-    const G* gr = dy + r * lddy;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j = (grp.c + i * grp.T) * VEC;
-      if (r < rows && j < D) { xv[i].load(xr + j); gv[i].load(gr + j); } else { xv[i].clear(); gv[i].clear(); }
-    }
-    mean = r < rows ? __ldg(mean_in + r) : 0.f;
-    rstd = r < rows ? __ldg(rstd_in + r) : 0.f;
-  };
-  int64_t r0 = grp.first_row();
-  fetch(r0 + grp.own(), cx, cg, cmean, crstd);
-  for (; r0 < rows; r0 += grp.stride()) {
-    const int64_t r = r0 + grp.own();
-    fetch(r + grp.stride(), nx, ng, nmean, nrstd);
-    float s[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j = (grp.c + i * grp.T) * VEC;
-      if (j < D) {
-        float f[VEC], g[VEC], wf[VEC];
-        cx[i].get(f);
-        cg[i].get(g);
-        load_weights<VEC>(w, w_type, j, 1.f, wf);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          const float z = (f[k] - cmean) * crstd, h = g[k] * wf[k];
-          aw[i][k] = fmaf(g[k], z, aw[i][k]);
-          ab[i][k] += g[k];
-          s[0] += h;
-          s[1] = fmaf(h, z, s[1]);
-        }
-      }
-    }
-    grp.sum(s, buf);
-    const float mh = s[0] * inv_d, mhz = s[1] * inv_d;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j = (grp.c + i * grp.T) * VEC;
-      if (r < rows && j < D) {
-        float f[VEC], g[VEC], wf[VEC];
-        cx[i].get(f);
-        cg[i].get(g);
-        load_weights<VEC>(w, w_type, j, 1.f, wf);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          const float z = (f[k] - cmean) * crstd;
-          f[k] = crstd * (fmaf(g[k], wf[k], -mh) - z * mhz);
-        }
-        store_vec(dx + r * D + j, f);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) { cx[i] = nx[i]; cg[i] = ng[i]; }
-    cmean = nmean; crstd = nrstd;
   }
+  float next_mean = 0.f, next_rstd = 0.f;
+  if (r0 + grp.own() < rows) { next_mean = __ldg(mean_in + r0 + grp.own()); next_rstd = __ldg(rstd_in + r0 + grp.own()); }
+  for (int stage = 0; r0 < rows; r0 += stride, stage = stage + 1 < LN_STAGES ? stage + 1 : 0) {
+    const int64_t r = r0 + grp.own();
+    const float mean = next_mean, rstd = next_rstd;
+    if (r + stride < rows) { next_mean = __ldg(mean_in + r + stride); next_rstd = __ldg(rstd_in + r + stride); }
+    copies_wait<LN_STAGES - 2>();
+    fetch(r0 + (LN_STAGES - 1) * stride, stage == 0 ? LN_STAGES - 1 : stage - 1);      // where the last row was
+    const char* const xs = my_x + stage * row_bytes;
+    const char* const gs = my_g + stage * row_bytes;
+    auto values = [&](int i, float (&f)[VEC], float (&g)[VEC]) {
+      if (i == 0) { SX::template get<EDGE>(xs, xstep, f, first); SG::template get<EDGE>(gs, gstep, g, first); }
+      else { SX::template get<false>(xs + i * SX::WORDS * xstep, xstep, f, 0); SG::template get<false>(gs + i * SG::WORDS * gstep, gstep, g, 0); }
+    };
+    Sums sh, shz;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float f[VEC], g[VEC];
+      values(i, f, g);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {           // outside the row g is 0
+        const float z = (f[k] - mean) * rstd, h = g[k] * wf[i][k];
+        aw[i][k] = fmaf(g[k], z, aw[i][k]);
+        ab[i][k] += g[k];
+        sh.v[k & 3] += h;
+        shz.v[k & 3] = fmaf(h, z, shz.v[k & 3]);
+      }
+    }
+    float sum[2] = {sh.total(), shz.total()};
+    grp.sum(sum, buf);
+    // dx = r (h - mean(h) - z mean(h z)) = r h + ((x - mean) A + B)
+    const float A = -rstd * rstd * (sum[1] * inv_d), B = -rstd * (sum[0] * inv_d);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j0 = (grp.c + i * grp.T) * VEC - s;
+      float f[VEC], g[VEC];
+      values(i, f, g);
+      if (r < rows && j0 < D) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) f[k] = fmaf(g[k] * wf[i][k], rstd, fmaf(f[k] - mean, A, B));
+        if (EDGE) store_row<X, VEC>(dx + r * D, j0, D, f); else store_vec(dx + r * D + j0, f);
+      }
+    }
+  }
+  copies_wait<0>();
   if (partial == nullptr) return;
   float* out = partial + static_cast<int64_t>(blockIdx.x) * 2 * D;
   if (BLOCK) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j = (grp.c + i * grp.T) * VEC;
-      if (j < D)
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) { out[j + k] = aw[i][k]; out[D + j + k] = ab[i][k]; }
-    }
-    return;
-  }
-  // the groups of a warp by shuffles, its four warps through shared memory
-  constexpr int WARPS = LN_WARP_THREADS / 32;
-  __shared__ float cols[WARPS][32 * NV * VEC];
-#pragma unroll
-  for (int which = 0; which < 2; ++which) {
-#pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
-        float a = which ? ab[i][k] : aw[i][k];
-        for (int o = 16; o >= grp.T; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-        const int j = (grp.c + i * grp.T) * VEC + k;
-        if ((threadIdx.x & 31) < grp.T && j < D) cols[threadIdx.x >> 5][j] = a;
+        const int j = (grp.c + i * grp.T) * VEC - s + k;
+        if (j >= 0 && j < D) { out[j] = aw[i][k]; out[D + j] = ab[i][k]; }
       }
-    __syncthreads();
-    for (int j = threadIdx.x; j < D; j += LN_WARP_THREADS) {
-      float a = cols[0][j];
+    return;
+  }
+  // The groups of a block have rows of different s where D is no multiple of VEC, so their sums meet by column: the groups of a warp one
+  // after the other in shared memory (by shuffles where s is the same for all), the four warps in the end.
+  constexpr int WARPS = LN_WARP_THREADS / 32;
+  float* const cols = reinterpret_cast<float*>(slots);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr bool same = !EDGE;
 #pragma unroll
-      for (int k = 1; k < WARPS; ++k) a += cols[k][j];
-      out[which * D + j] = a;
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();
+    if (!same) {
+      for (int j = lane; j < D; j += 32) cols[warp * D + j] = 0.f;
+      __syncwarp();
+    }
+    for (int g = 0; g < (same ? 1 : 32 / grp.T); ++g) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          float a = which ? ab[i][k] : aw[i][k];
+          const int j = (grp.c + i * grp.T) * VEC - s + k;
+          if (same) {
+            for (int o = 16; o >= grp.T; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+            if (lane < grp.T && j < D) cols[warp * D + j] = a;
+          } else if (lane / grp.T == g && j >= 0 && j < D) {
+            cols[warp * D + j] += a;
+          }
+        }
+      __syncwarp();
     }
     __syncthreads();
+    for (int j = threadIdx.x; j < D; j += LN_WARP_THREADS) {
+      float a = cols[j];
+#pragma unroll
+      for (int k = 1; k < WARPS; ++k) a += cols[k * D + j];
+      out[which * D + j] = a;
+    }
   }
 }
 
@@ -458,40 +539,55 @@ static int sm_count() {
 }
 static unsigned capped(int64_t want, int64_t cap) { return static_cast<unsigned>(want < cap ? want : cap); }
 
-// How a row of D elements is held: vec elements a vector, nv vectors a thread, T threads (within a warp, or a block), or `wide`.
+// How a row of D elements is held: nv vectors of `vec` elements a thread, T threads (lanes of a warp, or a block), or `wide`.
 struct RowPlan {
   bool wide = false, block = false;
-  int vec = 1, nv = 1, T = 32;
+  int nv = 1, T = 32;
 };
 // most: threads of a block that a row may take
-static RowPlan plan_rows(int64_t D, int vec, bool aligned, int most_vec, int most_single) {
+static RowPlan plan_rows(int64_t D, int vec, int most) {
   RowPlan p;
-  p.vec = aligned ? vec : 1;
-  const int64_t units = (D + p.vec - 1) / p.vec;      // vectors of a row
-  const int per_thread = aligned ? 4 : 16;
-  if (units <= 32 * per_thread) {
-    // the fewest threads: a group of few lanes leaves the others to more rows
+  const int64_t units = D % vec == 0 ? D / vec : (D + 2 * vec - 2) / vec;      // vectors that a row may touch
+  if (units <= 32 * 4) {
+    // the fewest threads with at most 2 vectors each: a group of few lanes leaves the others to more rows
     p.T = 1;
-    while (p.T < 32 && p.T * (aligned ? 2 : 4) < units) p.T *= 2;
-    const int64_t need = (units + p.T - 1) / p.T;
-    p.nv = aligned ? static_cast<int>(need) : need <= 1 ? 1 : need <= 4 ? 4 : 16;
+    while (p.T < 32 && p.T * 2 < units) p.T *= 2;
+    p.nv = static_cast<int>((units + p.T - 1) / p.T);
     return p;
   }
   p.block = true;
-  p.nv = per_thread;
-  const int64_t T = (units + 32 * per_thread - 1) / (32 * per_thread) * 32;
-  if (T > (aligned ? most_vec : most_single)) p.wide = true;
+  p.nv = 4;
+  const int64_t T = (units + 127) / 128 * 32;
+  p.wide = T > most;
   p.T = static_cast<int>(T);
   return p;
 }
-static bool on(const void* p, int64_t ld_bytes, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld_bytes % bytes == 0; }
 
-// Blocks of the row kernels: as many as stay resident (registers allow about 3 to 4 blocks of 128 threads with 24 to 32 elements a
-// thread and twice that with fewer), since each of them leaves a part of dw and db.
-static unsigned row_blocks(const RowPlan& p, int64_t rows, int resident_threads) {
+// Blocks of the row kernels: as many as stay resident, since each of them leaves a part of dw and db.  Where rows do not all start on a
+// 16-byte boundary, a group's rows have to be a multiple of 8 apart.
+static unsigned row_blocks(const RowPlan& p, int64_t rows, int64_t D, int vec, int resident_threads) {
   const int64_t groups = p.block ? 1 : LN_WARP_THREADS / p.T, threads = p.block ? p.T : LN_WARP_THREADS;
-  const int64_t want = (rows + groups - 1) / groups, per_sm = resident_threads / threads < 1 ? 1 : resident_threads / threads;
-  return capped(want < 1 ? 1 : want, per_sm * sm_count());
+  const int64_t want = (rows + groups - 1) / groups, per_sm = resident_threads / threads < 1 ? 1 : resident_threads / threads, most = per_sm * sm_count();
+  if (want <= most) return static_cast<unsigned>(want);
+  return static_cast<unsigned>(D % vec == 0 ? most : most < 8 ? 8 : most / 8 * 8);
+}
+// Whether the rows of an input can be copied in vectors: the same distances from a boundary as the output's.
+static bool in_vectors(const void* p, int64_t ld, int64_t D, int vec, int64_t bytes) {
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && (ld - D) % vec == 0;
+}
+
+// Dynamic shared memory of a kernel, allowed once per device.
+template <class K>
+static int allow_slots(K kernel, std::atomic<uint64_t>& allowed) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (dev < 64 && (allowed.load(std::memory_order_acquire) & bit)) return HASTE_OK;
+  if (int rc = allow_dynamic_smem(kernel)) return rc;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaFuncSetAttribute(carveout): %s", cudaGetErrorString(e));
+  if (dev < 64) allowed.fetch_or(bit, std::memory_order_release);
+  return HASTE_OK;
 }
 
 template <class X, class W>
@@ -500,42 +596,54 @@ static int ln_fwd_wide(const X* x, const W* w, const W* b, X* y, float* mean, fl
   return check_launch("layer_norm_forward");
 }
 
-template <class X>
-static int ln_fwd(const X* x, const void* w, const void* b, X* y, float* mean, float* rstd, int64_t rows, int64_t D, int64_t ldx, float eps, int w_type,
-                  cudaStream_t st) {
-  if (rows == 0) return HASTE_OK;
-  constexpr int VEC = 16 / sizeof(X);
-  const int64_t w_bytes = w_type == HASTE_BF16 && VEC == 4 ? 8 : 16;
-  const bool aligned = D % VEC == 0 && on(x, ldx * sizeof(X), 16) && on(y, 0, 16) && on(w, 0, w_bytes) && on(b, 0, w_bytes);
-  const RowPlan p = plan_rows(D, VEC, aligned, 512, 512);
-  if (p.wide) {
-    if (w_type == HASTE_BF16) return ln_fwd_wide(x, (const __nv_bfloat16*)w, (const __nv_bfloat16*)b, y, mean, rstd, rows, D, ldx, eps, st);
-    return ln_fwd_wide(x, (const float*)w, (const float*)b, y, mean, rstd, rows, D, ldx, eps, st);
-  }
-  const unsigned blocks = row_blocks(p, rows, 1024), threads = p.block ? p.T : LN_WARP_THREADS;
-#define HASTE_LN_FWD(V, NV, BLOCK) \
-  ln_fwd_kernel<X, V, NV, BLOCK><<<blocks, threads, 0, st>>>(x, w, b, w_type, y, mean, rstd, rows, static_cast<int>(D), ldx, eps, p.T)
-  if (aligned) {
-    if (p.block) HASTE_LN_FWD(VEC, 4, true);
-    else if (p.nv == 1) HASTE_LN_FWD(VEC, 1, false);
-    else if (p.nv == 2) HASTE_LN_FWD(VEC, 2, false);
-    else if (p.nv == 3) HASTE_LN_FWD(VEC, 3, false);
-    else HASTE_LN_FWD(VEC, 4, false);
-  } else {
-    if (p.block) HASTE_LN_FWD(1, 16, true);
-    else if (p.nv == 1) HASTE_LN_FWD(1, 1, false);
-    else if (p.nv == 4) HASTE_LN_FWD(1, 4, false);
-    else HASTE_LN_FWD(1, 16, false);
-  }
-#undef HASTE_LN_FWD
+struct FwdCall {
+  const void *x, *w, *b;
+  void* y;
+  float *mean, *rstd;
+  int64_t rows, D, ldx;
+  float eps;
+  int w_type;
+  cudaStream_t st;
+};
+
+template <class X, int VEC, int NV, bool BLOCK, bool EDGE>
+static int ln_fwd_rows(const FwdCall& c, const RowPlan& p) {
+  static std::atomic<uint64_t> allowed{0};
+  const int threads = BLOCK ? p.T : LN_WARP_THREADS, smem = LN_STAGES * NV * threads * VEC * static_cast<int>(sizeof(X));
+  if (int rc = allow_slots(ln_fwd_kernel<X, VEC, NV, BLOCK, EDGE>, allowed)) return rc;
+  const unsigned blocks = row_blocks(p, c.rows, c.D, VEC, VEC * NV > 16 ? 512 : VEC * NV > 8 ? 768 : 1024);
+  ln_fwd_kernel<X, VEC, NV, BLOCK, EDGE><<<blocks, threads, smem, c.st>>>((const X*)c.x, c.w, c.b, c.w_type, (X*)c.y, c.mean, c.rstd, c.rows, static_cast<int>(c.D), c.ldx,
+                                                                    c.eps, p.T, in_vectors(c.x, c.ldx, c.D, VEC, 16), aligned16(c.w) && aligned16(c.b));
   return check_launch("layer_norm_forward");
+}
+
+template <class X, int VEC, bool EDGE>
+static int ln_fwd_plan(const FwdCall& c, const RowPlan& p) {
+  if (p.block) return ln_fwd_rows<X, VEC, 4, true, EDGE>(c, p);
+  if (p.nv == 1) return ln_fwd_rows<X, VEC, 1, false, EDGE>(c, p);
+  if (p.nv == 2) return ln_fwd_rows<X, VEC, 2, false, EDGE>(c, p);
+  if (p.nv == 3) return ln_fwd_rows<X, VEC, 3, false, EDGE>(c, p);
+  return ln_fwd_rows<X, VEC, 4, false, EDGE>(c, p);
+}
+
+template <class X>
+static int ln_fwd(const FwdCall& c) {
+  if (c.rows == 0) return HASTE_OK;
+  constexpr int VEC = 16 / sizeof(X);
+  RowPlan p = plan_rows(c.D, VEC, 512);
+  if (!aligned16(c.y)) p.wide = true;
+  if (p.wide) {
+    using B = __nv_bfloat16;
+    if (c.w_type == HASTE_BF16) return ln_fwd_wide((const X*)c.x, (const B*)c.w, (const B*)c.b, (X*)c.y, c.mean, c.rstd, c.rows, c.D, c.ldx, c.eps, c.st);
+    return ln_fwd_wide((const X*)c.x, (const float*)c.w, (const float*)c.b, (X*)c.y, c.mean, c.rstd, c.rows, c.D, c.ldx, c.eps, c.st);
+  }
+  return c.D % VEC ? ln_fwd_plan<X, VEC, true>(c, p) : ln_fwd_plan<X, VEC, false>(c, p);
 }
 
 int launch_layer_norm_forward(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows, int64_t D, int64_t ldx,
                               float eps, int x_type, int w_type, cudaStream_t st) {
-  using B = __nv_bfloat16;
-  if (x_type == HASTE_BF16) return ln_fwd((const B*)x, w, b, (B*)y, mean, rstd, rows, D, ldx, eps, w_type, st);
-  return ln_fwd((const float*)x, w, b, (float*)y, mean, rstd, rows, D, ldx, eps, w_type, st);
+  const FwdCall c{x, w, b, y, mean, rstd, rows, D, ldx, eps, w_type, st};
+  return x_type == HASTE_BF16 ? ln_fwd<__nv_bfloat16>(c) : ln_fwd<float>(c);
 }
 
 // Parts of dw and db that the wide rows' kernel makes; the others make at most MAX_PARTS (one per block).
@@ -558,46 +666,63 @@ static int ln_bwd_wide(const G* dy, const X* x, const W* w, const float* mean, c
   return check_launch("layer_norm_backward");
 }
 
+struct BwdCall {
+  const void *dy, *x, *w;
+  const float *mean, *rstd;
+  void *dx, *dw, *db;
+  float* scratch;
+  int64_t rows, D, lddy, ldx;
+  int w_type;
+  cudaStream_t st;
+};
+
+template <class X, class G, int VEC, int NV, bool BLOCK, bool EDGE>
+static int ln_bwd_rows(const BwdCall& c, const RowPlan& p, float* partial, unsigned& parts) {
+  static std::atomic<uint64_t> allowed{0};
+  const int threads = BLOCK ? p.T : LN_WARP_THREADS, slots = LN_STAGES * NV * threads * VEC * static_cast<int>(sizeof(X) + sizeof(G));
+  const int cols = BLOCK ? 0 : LN_WARP_THREADS / 32 * static_cast<int>(c.D) * 4, smem = slots > cols ? slots : cols;
+  if (int rc = allow_slots(ln_bwd_kernel<X, G, VEC, NV, BLOCK, EDGE>, allowed)) return rc;
+  parts = row_blocks(p, c.rows, c.D, VEC, VEC * NV > 16 ? 384 : VEC * NV > 8 ? 512 : 1024);
+  const int64_t g_bytes = VEC * sizeof(G) < 16 ? 8 : 16;
+  ln_bwd_kernel<X, G, VEC, NV, BLOCK, EDGE><<<parts, threads, smem, c.st>>>((const G*)c.dy, (const X*)c.x, c.w, c.w_type, c.mean, c.rstd, (X*)c.dx, partial, c.rows,
+                                                                      static_cast<int>(c.D), c.lddy, c.ldx, p.T, in_vectors(c.x, c.ldx, c.D, VEC, 16),
+                                                                      in_vectors(c.dy, c.lddy, c.D, VEC, g_bytes), aligned16(c.w));
+  return check_launch("layer_norm_backward");
+}
+
+template <class X, class G, int VEC, bool EDGE>
+static int ln_bwd_plan(const BwdCall& c, const RowPlan& p, float* partial, unsigned& parts) {
+  if (p.block) return ln_bwd_rows<X, G, VEC, 4, true, EDGE>(c, p, partial, parts);
+  if (p.nv == 1) return ln_bwd_rows<X, G, VEC, 1, false, EDGE>(c, p, partial, parts);
+  if (p.nv == 2) return ln_bwd_rows<X, G, VEC, 2, false, EDGE>(c, p, partial, parts);
+  if (p.nv == 3) return ln_bwd_rows<X, G, VEC, 3, false, EDGE>(c, p, partial, parts);
+  return ln_bwd_rows<X, G, VEC, 4, false, EDGE>(c, p, partial, parts);
+}
+
 template <class X, class G>
-static int ln_bwd(const G* dy, const X* x, const void* w, const float* mean, const float* rstd, X* dx, void* dw, void* db, float* scratch, int64_t rows,
-                  int64_t D, int64_t lddy, int64_t ldx, int w_type, cudaStream_t st) {
+static int ln_bwd(const BwdCall& c) {
   constexpr int VEC = 16 / sizeof(X);
-  const bool want = dw != nullptr || db != nullptr;
-  float* partial = want ? scratch : nullptr;
+  using B = __nv_bfloat16;
+  const bool want = c.dw != nullptr || c.db != nullptr;
+  float* partial = want ? c.scratch : nullptr;
   unsigned parts = 0;
-  if (rows > 0) {
-    const int64_t w_bytes = w_type == HASTE_BF16 && VEC == 4 ? 8 : 16, g_bytes = VEC * sizeof(G) < 16 ? 8 : 16;
-    const bool aligned = D % VEC == 0 && on(x, ldx * sizeof(X), 16) && on(dx, 0, 16) && on(dy, lddy * sizeof(G), g_bytes) && on(w, 0, w_bytes);
-    const RowPlan p = plan_rows(D, VEC, aligned, VEC == 8 ? 256 : 512, 512);
+  if (c.rows > 0) {
+    RowPlan p = plan_rows(c.D, VEC, VEC == 8 ? 256 : 512);
+    if (!aligned16(c.dx)) p.wide = true;
+    int rc = HASTE_OK;
     if (p.wide) {
-      parts = static_cast<unsigned>(wide_parts(rows));
-      const int rc = w_type == HASTE_BF16 ? ln_bwd_wide(dy, x, (const __nv_bfloat16*)w, mean, rstd, dx, partial, rows, D, lddy, ldx, st)
-                                          : ln_bwd_wide(dy, x, (const float*)w, mean, rstd, dx, partial, rows, D, lddy, ldx, st);
-      if (rc != HASTE_OK) return rc;
+      parts = static_cast<unsigned>(wide_parts(c.rows));
+      rc = c.w_type == HASTE_BF16 ? ln_bwd_wide((const G*)c.dy, (const X*)c.x, (const B*)c.w, c.mean, c.rstd, (X*)c.dx, partial, c.rows, c.D, c.lddy, c.ldx, c.st)
+                                  : ln_bwd_wide((const G*)c.dy, (const X*)c.x, (const float*)c.w, c.mean, c.rstd, (X*)c.dx, partial, c.rows, c.D, c.lddy, c.ldx, c.st);
     } else {
-      parts = row_blocks(p, rows, p.vec * p.nv > 16 ? 384 : p.vec * p.nv > 8 ? 512 : 1024);
-      const unsigned threads = p.block ? p.T : LN_WARP_THREADS;
-#define HASTE_LN_BWD(V, NV, BLOCK) \
-  ln_bwd_kernel<X, G, V, NV, BLOCK><<<parts, threads, 0, st>>>(dy, x, w, w_type, mean, rstd, dx, partial, rows, static_cast<int>(D), lddy, ldx, p.T)
-      if (aligned) {
-        if (p.block) HASTE_LN_BWD(VEC, 4, true);
-        else if (p.nv == 1) HASTE_LN_BWD(VEC, 1, false);
-        else if (p.nv == 2) HASTE_LN_BWD(VEC, 2, false);
-        else if (p.nv == 3) HASTE_LN_BWD(VEC, 3, false);
-        else HASTE_LN_BWD(VEC, 4, false);
-      } else {
-        if (p.block) HASTE_LN_BWD(1, 16, true);
-        else if (p.nv == 1) HASTE_LN_BWD(1, 1, false);
-        else if (p.nv == 4) HASTE_LN_BWD(1, 4, false);
-        else HASTE_LN_BWD(1, 16, false);
-      }
-#undef HASTE_LN_BWD
+      rc = c.D % VEC ? ln_bwd_plan<X, G, VEC, true>(c, p, partial, parts) : ln_bwd_plan<X, G, VEC, false>(c, p, partial, parts);
     }
+    if (rc != HASTE_OK) return rc;
   }
   if (want) {
-    const unsigned grid = static_cast<unsigned>((2 * D + 31) / 32);
-    if (w_type == HASTE_BF16) ln_bwd_finish_kernel<<<grid, LN_FINISH_THREADS, 0, st>>>(scratch, static_cast<int>(parts), D, (__nv_bfloat16*)dw, (__nv_bfloat16*)db);
-    else ln_bwd_finish_kernel<<<grid, LN_FINISH_THREADS, 0, st>>>(scratch, static_cast<int>(parts), D, (float*)dw, (float*)db);
+    const unsigned grid = static_cast<unsigned>((2 * c.D + 31) / 32);
+    if (c.w_type == HASTE_BF16) ln_bwd_finish_kernel<<<grid, LN_FINISH_THREADS, 0, c.st>>>(c.scratch, static_cast<int>(parts), c.D, (B*)c.dw, (B*)c.db);
+    else ln_bwd_finish_kernel<<<grid, LN_FINISH_THREADS, 0, c.st>>>(c.scratch, static_cast<int>(parts), c.D, (float*)c.dw, (float*)c.db);
   }
   return check_launch("layer_norm_backward");
 }
@@ -605,13 +730,9 @@ static int ln_bwd(const G* dy, const X* x, const void* w, const float* mean, con
 int launch_layer_norm_backward(const void* dy, const void* x, const void* w, const float* mean, const float* rstd, void* dx, void* dw, void* db,
                                float* scratch, int64_t rows, int64_t D, int64_t lddy, int64_t ldx, int x_type, int dy_type, int w_type, cudaStream_t st) {
   using B = __nv_bfloat16;
-  using F = float;
-  if (x_type == HASTE_BF16) {
-    if (dy_type == HASTE_BF16) return ln_bwd((const B*)dy, (const B*)x, w, mean, rstd, (B*)dx, dw, db, scratch, rows, D, lddy, ldx, w_type, st);
-    return ln_bwd((const F*)dy, (const B*)x, w, mean, rstd, (B*)dx, dw, db, scratch, rows, D, lddy, ldx, w_type, st);
-  }
-  if (dy_type == HASTE_BF16) return ln_bwd((const B*)dy, (const F*)x, w, mean, rstd, (F*)dx, dw, db, scratch, rows, D, lddy, ldx, w_type, st);
-  return ln_bwd((const F*)dy, (const F*)x, w, mean, rstd, (F*)dx, dw, db, scratch, rows, D, lddy, ldx, w_type, st);
+  const BwdCall c{dy, x, w, mean, rstd, dx, dw, db, scratch, rows, D, lddy, ldx, w_type, st};
+  if (x_type == HASTE_BF16) return dy_type == HASTE_BF16 ? ln_bwd<B, B>(c) : ln_bwd<B, float>(c);
+  return dy_type == HASTE_BF16 ? ln_bwd<float, B>(c) : ln_bwd<float, float>(c);
 }
 
 }  // namespace haste
