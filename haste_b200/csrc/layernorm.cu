@@ -150,33 +150,54 @@ __global__ void __launch_bounds__(LN_FINISH_THREADS) ln_bwd_finish_kernel(const 
 // it works on the row that has arrived.  What lies outside the row or the rows reads as zero, so that most sums need no masks: the copies
 // fill up with zeros, and of a row's first vector the part before the row is dropped when it is read.
 __device__ __forceinline__ uint32_t smem_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-// 16 bytes (8, 4), of which `bytes` are read and the rest become zeros
-__device__ __forceinline__ void copy_async16(void* dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_address(dst)), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copy_async8(void* dst, const void* src, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_address(dst)), "l"(src), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 constexpr int LN_STAGES = 3;              // rows on their way or at work, per group
 constexpr int LN_WARP_THREADS = 128;      // block of the variant whose groups are within a warp
 
+// Two fp32 numbers as one operand: one instruction for both.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
+      "l"(reinterpret_cast<const uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 // VEC elements of type T in a slot: WORDS accesses of 16 bytes (one of 8 for 4 bf16), `step` bytes apart, so that the lanes of a
-// warp touch consecutive 16 bytes each time.
+// warp touch consecutive 16 bytes each time.  Addresses `dst` are shared memory's.
 template <class T, int VEC> struct Slot {
   static constexpr int BYTES = VEC * static_cast<int>(sizeof(T)), WORDS = (BYTES + 15) / 16, UNIT = BYTES < 16 ? BYTES : 16, PER = UNIT / static_cast<int>(sizeof(T));
-  // n: how many of the elements exist (from the first on)
-  static __device__ __forceinline__ void copy(char* dst, int step, const T* src, int n) {
+  static __device__ __forceinline__ void copy_unit(uint32_t dst, const void* src, int bytes) {       // of which `bytes` are read, the rest becomes zeros
+    if (UNIT == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+  }
+  static __device__ __forceinline__ void copy(uint32_t dst, int step, const T* src) {
 #pragma unroll
     for (int k = 0; k < WORDS; ++k) {
-      const int left = (n - k * PER) * static_cast<int>(sizeof(T)), bytes = left < 0 ? 0 : left < UNIT ? left : UNIT;
-      const T* from = bytes > 0 ? src + k * PER : src;
-      if (UNIT == 16) copy_async16(dst + k * step, from, bytes); else copy_async8(dst + k * step, from, bytes);
+      if (UNIT == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + k * step), "l"(src + k * PER) : "memory");
+      else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst + k * step), "l"(src + k * PER) : "memory");
     }
   }
-  static __device__ void copy_single(char* dst, int step, const T* src, int first, int n) {      // elements first .. n-1, zeros elsewhere
+  static __device__ __forceinline__ void copy_part(uint32_t dst, int step, const T* src, int n) {    // the first n > 0 elements, then zeros
+#pragma unroll
+    for (int k = 0; k < WORDS; ++k) {
+      const int bytes = min(max((n - k * PER) * static_cast<int>(sizeof(T)), 0), UNIT);
+      copy_unit(dst + k * step, bytes > 0 ? src + k * PER : src, bytes);
+    }
+  }
+  static __device__ void copy_single(char* dst, int step, const T* src, int first, int n) {          // elements first .. n-1, zeros elsewhere
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       T v;
@@ -185,52 +206,60 @@ template <class T, int VEC> struct Slot {
       reinterpret_cast<T*>(dst + e / PER * step)[e % PER] = v;
     }
   }
+  static __device__ __forceinline__ void clear(char* dst, int step) {
+#pragma unroll
+    for (int k = 0; k < WORDS; ++k) {
+      if (UNIT == 16) *reinterpret_cast<uint4*>(dst + k * step) = make_uint4(0u, 0u, 0u, 0u);
+      else *reinterpret_cast<uint2*>(dst + k * step) = make_uint2(0u, 0u);
+    }
+  }
   // MASK: the elements before `first` belong to another row and read as 0
   template <bool MASK>
-  static __device__ __forceinline__ void get(const char* src, int step, float (&f)[VEC], int first) {
+  static __device__ __forceinline__ void get(const char* src, int step, float2 (&f)[VEC / 2], int first) {
 #pragma unroll
     for (int k = 0; k < WORDS; ++k) {
       if constexpr (sizeof(T) == 4) {
         const float4 v = *reinterpret_cast<const float4*>(src + k * step);
-        f[4 * k] = v.x; f[4 * k + 1] = v.y; f[4 * k + 2] = v.z; f[4 * k + 3] = v.w;
+        f[2 * k] = make_float2(v.x, v.y); f[2 * k + 1] = make_float2(v.z, v.w);
       } else {
         uint32_t u[PER / 2];
         if constexpr (UNIT == 16) { const uint4 v = *reinterpret_cast<const uint4*>(src + k * step); u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w; }
         else { const uint2 v = *reinterpret_cast<const uint2*>(src + k * step); u[0] = v.x; u[1] = v.y; }
 #pragma unroll
-        for (int e = 0; e < PER / 2; ++e) { f[2 * e] = __uint_as_float(u[e] << 16); f[2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u); }
+        for (int e = 0; e < PER / 2; ++e) f[e] = make_float2(__uint_as_float(u[e] << 16), __uint_as_float(u[e] & 0xFFFF0000u));
       }
     }
     if (MASK) {
 #pragma unroll
-      for (int e = 0; e < VEC - 1; ++e) f[e] = e < first ? 0.f : f[e];
+      for (int e = 0; e < VEC / 2; ++e) { f[e].x = 2 * e < first ? 0.f : f[e].x; f[e].y = 2 * e + 1 < first ? 0.f : f[e].y; }
     }
   }
 };
 
-__device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&f)[8]) {
+__device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float2 (&f)[4]) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f[i].x, f[i].y);
     w[i] = *reinterpret_cast<const uint32_t*>(&h);
   }
   __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
 }
-__device__ __forceinline__ void store_vec(float* p, const float (&f)[4]) { __stcs(reinterpret_cast<float4*>(p), make_float4(f[0], f[1], f[2], f[3])); }
-// Columns j0 .. of a row: the whole vector, or those of its elements that belong to the row.
-template <class T, int VEC>
-__device__ __forceinline__ void store_row(T* row, int j0, int D, const float (&f)[VEC]) {
-  if (j0 >= 0 && j0 + VEC <= D) store_vec(row + j0, f);
+__device__ __forceinline__ void store_vec(float* p, const float2 (&f)[2]) { __stcs(reinterpret_cast<float4*>(p), make_float4(f[0].x, f[0].y, f[1].x, f[1].y)); }
+// Columns j0 .. of a row, p the first one's place: the whole vector, or those of its elements that belong to the row.
+template <int VEC, class T>
+__device__ __forceinline__ void store_part(T* p, int j0, int D, const float2 (&f)[VEC / 2]) {
+  if (j0 >= 0 && j0 + VEC <= D) store_vec(p, f);
   else {
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) if (j0 + k >= 0 && j0 + k < D) st_f(row + j0 + k, f[k]);
+    for (int k = 0; k < VEC; ++k) if (static_cast<unsigned>(j0 + k) < static_cast<unsigned>(D)) st_f(p + k, k & 1 ? f[k / 2].y : f[k / 2].x);
   }
 }
 
 // Weights of a thread's columns, once per kernel; 0 outside the row.  vec: whole vectors only, on 16 bytes.
 template <int VEC>
-__device__ __forceinline__ void load_weights(const void* w, int w_type, bool vec, int j0, int D, float fill, float (&f)[VEC]) {
+__device__ __forceinline__ void load_weights(const void* w, int w_type, bool vec, int j0, int D, float fill, float2 (&out)[VEC / 2]) {
+  float f[VEC];
   if (w == nullptr) {
 #pragma unroll
     for (int k = 0; k < VEC; ++k) f[k] = static_cast<unsigned>(j0 + k) < static_cast<unsigned>(D) ? fill : 0.f;
@@ -265,6 +294,8 @@ __device__ __forceinline__ void load_weights(const void* w, int w_type, bool vec
       for (int k = 0; k < VEC; ++k) f[k] = static_cast<unsigned>(j0 + k) < static_cast<unsigned>(D) ? __ldg(p + k) : 0.f;
     }
   }
+#pragma unroll
+  for (int k = 0; k < VEC / 2; ++k) out[k] = make_float2(f[2 * k], f[2 * k + 1]);
 }
 
 // The threads that share a row: T lanes of a warp (a power of two), or the block.
@@ -303,10 +334,53 @@ struct RowGroup {
   }
 };
 
-struct Sums {            // partial sums that do not wait for one another
-  float v[4];
-  __device__ __forceinline__ Sums() : v{0.f, 0.f, 0.f, 0.f} {}
-  __device__ __forceinline__ float total() const { return (v[0] + v[1]) + (v[2] + v[3]); }
+// A row group's walk over an input: the copies of its next row.
+template <class T, int VEC, int NV, bool EDGE>
+struct Feed {
+  using S = Slot<T, VEC>;
+  const T* next;           // column j0 of the row to be copied next
+  int64_t row_step;        // elements from a row of the group to its next one
+  int vec_step, step;      // elements from a vector of the thread to its next one; bytes between the words of a slot
+  int j0, D;
+  bool vec;
+  char* slots;             // the thread's own, of the first stage
+  uint32_t to;
+  __device__ __forceinline__ Feed(const T* p, int64_t ld, int64_t row, int64_t stride, int j0_, int D_, int T_, bool vec_, char* area)
+      : next(p + row * ld + j0_), row_step(stride * ld), vec_step(T_ * VEC), step(static_cast<int>(blockDim.x) * S::UNIT), j0(j0_), D(D_), vec(vec_),
+        slots(area + threadIdx.x * S::UNIT), to(smem_address(slots)) {}
+  static __device__ __forceinline__ int bytes() { return NV * S::WORDS * S::UNIT * static_cast<int>(blockDim.x); }
+  // Slots that no copy reaches (vectors right of the row) hold zeros for good.
+  __device__ __forceinline__ void clear(int stage_bytes) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (j0 + i * vec_step >= D)
+        for (int k = 0; k < LN_STAGES; ++k) S::clear(slots + k * stage_bytes + i * S::WORDS * step, step);
+  }
+  __device__ __forceinline__ void fetch(int at, bool there) {
+    if (there) {
+      if (vec) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int j = j0 + i * vec_step;
+          if (j < D) {
+            if (!EDGE) S::copy(to + at + i * S::WORDS * step, step, next + i * vec_step);
+            else S::copy_part(to + at + i * S::WORDS * step, step, next + i * vec_step, min(D - j, VEC));
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < NV; ++i) {
+          const int j = j0 + i * vec_step;
+          if (j < D) S::copy_single(slots + at + i * S::WORDS * step, step, next + i * vec_step, -j, D - j);
+        }
+      }
+    }
+    next += row_step;
+  }
+  __device__ __forceinline__ void get(int at, int i, int first, float2 (&f)[VEC / 2]) const {
+    if (i == 0) S::template get<EDGE>(slots + at, step, f, first);
+    else S::template get<false>(slots + at + i * S::WORDS * step, step, f, 0);
+  }
 };
 
 // EDGE: D is no multiple of VEC, rows have first and last vectors that are theirs in part.
@@ -314,75 +388,74 @@ template <class X, int VEC, int NV, bool BLOCK, bool EDGE>
 __global__ void __launch_bounds__(BLOCK ? 512 : LN_WARP_THREADS, BLOCK ? 1 : 4)
     ln_fwd_kernel(const X* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b, int w_type, X* __restrict__ y, float* __restrict__ mean_out,
                   float* __restrict__ rstd_out, int64_t rows, int D, int64_t ldx, float eps, int t, bool x_vec, bool w_vec) {
-  using SX = Slot<X, VEC>;
   __shared__ float buf[2][1][16];
   extern __shared__ __align__(16) char slots[];
   RowGroup<BLOCK> grp(t);
-  const int step = blockDim.x * SX::UNIT, row_bytes = NV * SX::WORDS * step;
-  char* const mine = slots + threadIdx.x * SX::UNIT;
   const float inv_d = 1.f / static_cast<float>(D);
   const int64_t stride = grp.stride();
-  int64_t r0 = grp.first_row();
-  const int s = EDGE ? static_cast<int>((r0 + grp.own()) * D % VEC) : 0, first = grp.c == 0 ? s : 0;
-  auto fetch = [&](int64_t from_row, int stage) {
-    const int64_t r = from_row + grp.own();
+  int64_t r = grp.first_row() + grp.own(), left = rows - grp.first_row();       // left: rows from the warp's (block's) first one on
+  const int s = EDGE ? static_cast<int>(r * D % VEC) : 0, first = grp.c == 0 ? s : 0, j0 = grp.c * VEC - s, vec_step = grp.T * VEC;
+  Feed<X, VEC, NV, EDGE> in(x, ldx, r, stride, j0, D, grp.T, x_vec, slots);
+  const int stage_bytes = in.bytes(), all = LN_STAGES * stage_bytes;
+  in.clear(stage_bytes);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j0 = (grp.c + i * grp.T) * VEC - s, n = r < rows ? D - j0 : 0;
-      char* to = mine + stage * row_bytes + i * SX::WORDS * step;
-      const X* from = n > 0 ? x + r * ldx + j0 : x;
-      if (x_vec) SX::copy(to, step, from, n); else SX::copy_single(to, step, from, -j0, n);
-    }
-    copies_commit();
-  };
-#pragma unroll
-  for (int k = 0; k < LN_STAGES - 1; ++k) fetch(r0 + k * stride, k);
-  float wf[NV][VEC], bf[NV][VEC];
+  for (int k = 0; k < LN_STAGES - 1; ++k) { in.fetch(k * stage_bytes, r + k * stride < rows); copies_commit(); }
+  float2 wf[NV][VEC / 2], bf[NV][VEC / 2];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int j0 = (grp.c + i * grp.T) * VEC - s;
-    load_weights<VEC>(w, w_type, !EDGE && w_vec, j0, D, 1.f, wf[i]);
-    load_weights<VEC>(b, w_type, !EDGE && w_vec, j0, D, 0.f, bf[i]);
+    load_weights<VEC>(w, w_type, !EDGE && w_vec, j0 + i * vec_step, D, 1.f, wf[i]);
+    load_weights<VEC>(b, w_type, !EDGE && w_vec, j0 + i * vec_step, D, 0.f, bf[i]);
   }
-  for (int stage = 0; r0 < rows; r0 += stride, stage = stage + 1 < LN_STAGES ? stage + 1 : 0) {
-    const int64_t r = r0 + grp.own();
+  X* out = y + r * D + j0;
+  for (int at = 0, next_at = all - stage_bytes; left > 0; left -= stride, r += stride, out += stride * D) {
     copies_wait<LN_STAGES - 2>();
-    fetch(r0 + (LN_STAGES - 1) * stride, stage == 0 ? LN_STAGES - 1 : stage - 1);      // where the last row was
-    float f[NV][VEC];
-    Sums s1, s2;
+    in.fetch(next_at, r + (LN_STAGES - 1) * stride < rows);          // to where the last row was
+    copies_commit();
+    float2 f[NV][VEC / 2], s1 = both(0.f), s2 = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (i == 0) SX::template get<EDGE>(mine + stage * row_bytes, step, f[0], first);
-      else SX::template get<false>(mine + stage * row_bytes + i * SX::WORDS * step, step, f[i], 0);
+      in.get(at, i, first, f[i]);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) s1.v[k & 3] += f[i][k];
+      for (int k = 0; k < VEC / 2; ++k) { if (k & 1) s2 = add2(s2, f[i][k]); else s1 = add2(s1, f[i][k]); }
     }
-    float sum[1] = {s1.total()};
+    s1 = add2(s1, s2);
+    float sum[1] = {s1.x + s1.y};
     grp.sum(sum, buf);
     const float mean = sum[0] * inv_d;
+    s1 = s2 = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j0 = (grp.c + i * grp.T) * VEC - s;
+      const int j = j0 + i * vec_step;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const bool in = EDGE ? static_cast<unsigned>(j0 + k) < static_cast<unsigned>(D) : j0 < D;
-        f[i][k] -= mean;
-        if (in) s2.v[k & 3] = fmaf(f[i][k], f[i][k], s2.v[k & 3]);
+      for (int k = 0; k < VEC / 2; ++k) {
+        f[i][k] = add2(f[i][k], both(-mean));
+        if (EDGE) {
+          const float2 d = make_float2(static_cast<unsigned>(j + 2 * k) < static_cast<unsigned>(D) ? f[i][k].x : 0.f,
+                                       static_cast<unsigned>(j + 2 * k + 1) < static_cast<unsigned>(D) ? f[i][k].y : 0.f);
+          if (k & 1) s2 = fma2(d, d, s2); else s1 = fma2(d, d, s1);
+        } else if (i < NV - 1 || j < D) {                            // (the host gives a thread no more vectors than a row has)
+          if (k & 1) s2 = fma2(f[i][k], f[i][k], s2); else s1 = fma2(f[i][k], f[i][k], s1);
+        }
       }
     }
-    sum[0] = s2.total();
+    s1 = add2(s1, s2);
+    sum[0] = s1.x + s1.y;
     grp.sum(sum, buf);
     const float rstd = 1.f / sqrtf(fmaf(sum[0], inv_d, eps));
+    if (r < rows) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j0 = (grp.c + i * grp.T) * VEC - s;
-      if (r < rows && j0 < D) {
+      for (int i = 0; i < NV; ++i) {
+        const int j = j0 + i * vec_step;
+        if (j < D) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) f[i][k] = fmaf(f[i][k] * rstd, wf[i][k], bf[i][k]);
-        if (EDGE) store_row<X, VEC>(y + r * D, j0, D, f[i]); else store_vec(y + r * D + j0, f[i]);
+          for (int k = 0; k < VEC / 2; ++k) f[i][k] = fma2(mul2(f[i][k], both(rstd)), wf[i][k], bf[i][k]);
+          if (EDGE) store_part<VEC>(out + i * vec_step, j, D, f[i]); else store_vec(out + i * vec_step, f[i]);
+        }
       }
+      if (grp.c == 0 && mean_out != nullptr) { mean_out[r] = mean; rstd_out[r] = rstd; }
     }
-    if (grp.c == 0 && r < rows && mean_out != nullptr) { mean_out[r] = mean; rstd_out[r] = rstd; }
+    next_at = at;
+    at = at + stage_bytes < all ? at + stage_bytes : 0;
   }
   copies_wait<0>();
 }
@@ -393,95 +466,89 @@ __global__ void __launch_bounds__(BLOCK ? (VEC * NV > 16 ? 256 : 512) : LN_WARP_
     ln_bwd_kernel(const G* __restrict__ dy, const X* __restrict__ x, const void* __restrict__ w, int w_type, const float* __restrict__ mean_in,
                   const float* __restrict__ rstd_in, X* __restrict__ dx, float* __restrict__ partial, int64_t rows, int D, int64_t lddy, int64_t ldx, int t,
                   bool x_vec, bool dy_vec, bool w_vec) {
-  using SX = Slot<X, VEC>;
-  using SG = Slot<G, VEC>;
   __shared__ float buf[2][2][16];
   extern __shared__ __align__(16) char slots[];
   RowGroup<BLOCK> grp(t);
-  const int xstep = blockDim.x * SX::UNIT, gstep = blockDim.x * SG::UNIT, x_bytes = NV * SX::WORDS * xstep, row_bytes = x_bytes + NV * SG::WORDS * gstep;
-  char* const my_x = slots + threadIdx.x * SX::UNIT;
-  char* const my_g = slots + x_bytes + threadIdx.x * SG::UNIT;
   const float inv_d = 1.f / static_cast<float>(D);
   const int64_t stride = grp.stride();
-  int64_t r0 = grp.first_row();
-  const int s = EDGE ? static_cast<int>((r0 + grp.own()) * D % VEC) : 0, first = grp.c == 0 ? s : 0;
-  auto fetch = [&](int64_t from_row, int stage) {
-    const int64_t r = from_row + grp.own();
+  int64_t r = grp.first_row() + grp.own(), left = rows - grp.first_row();
+  const int s = EDGE ? static_cast<int>(r * D % VEC) : 0, first = grp.c == 0 ? s : 0, j0 = grp.c * VEC - s, vec_step = grp.T * VEC;
+  Feed<X, VEC, NV, EDGE> xin(x, ldx, r, stride, j0, D, grp.T, x_vec, slots);
+  Feed<G, VEC, NV, EDGE> gin(dy, lddy, r, stride, j0, D, grp.T, dy_vec, slots + xin.bytes());
+  const int stage_bytes = xin.bytes() + gin.bytes(), all = LN_STAGES * stage_bytes;
+  xin.clear(stage_bytes);
+  gin.clear(stage_bytes);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j0 = (grp.c + i * grp.T) * VEC - s, n = r < rows ? D - j0 : 0;
-      char* xto = my_x + stage * row_bytes + i * SX::WORDS * xstep;
-      char* gto = my_g + stage * row_bytes + i * SG::WORDS * gstep;
-      const X* xfrom = n > 0 ? x + r * ldx + j0 : x;
-      const G* gfrom = n > 0 ? dy + r * lddy + j0 : dy;
-      if (x_vec) SX::copy(xto, xstep, xfrom, n); else SX::copy_single(xto, xstep, xfrom, -j0, n);
-      if (dy_vec) SG::copy(gto, gstep, gfrom, n); else SG::copy_single(gto, gstep, gfrom, -j0, n);
-    }
+  for (int k = 0; k < LN_STAGES - 1; ++k) {
+    xin.fetch(k * stage_bytes, r + k * stride < rows);
+    gin.fetch(k * stage_bytes, r + k * stride < rows);
     copies_commit();
-  };
-#pragma unroll
-  for (int k = 0; k < LN_STAGES - 1; ++k) fetch(r0 + k * stride, k);
-  float wf[NV][VEC], aw[NV][VEC], ab[NV][VEC];
+  }
+  float2 wf[NV][VEC / 2], aw[NV][VEC / 2], ab[NV][VEC / 2];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    load_weights<VEC>(w, w_type, !EDGE && w_vec, (grp.c + i * grp.T) * VEC - s, D, 1.f, wf[i]);
+    load_weights<VEC>(w, w_type, !EDGE && w_vec, j0 + i * vec_step, D, 1.f, wf[i]);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) aw[i][k] = ab[i][k] = 0.f;
+    for (int k = 0; k < VEC / 2; ++k) aw[i][k] = ab[i][k] = both(0.f);
   }
   float next_mean = 0.f, next_rstd = 0.f;
-  if (r0 + grp.own() < rows) { next_mean = __ldg(mean_in + r0 + grp.own()); next_rstd = __ldg(rstd_in + r0 + grp.own()); }
-  for (int stage = 0; r0 < rows; r0 += stride, stage = stage + 1 < LN_STAGES ? stage + 1 : 0) {
-    const int64_t r = r0 + grp.own();
+  if (r < rows) { next_mean = __ldg(mean_in + r); next_rstd = __ldg(rstd_in + r); }
+  X* out = dx + r * D + j0;
+  for (int at = 0, next_at = all - stage_bytes; left > 0; left -= stride, r += stride, out += stride * D) {
     const float mean = next_mean, rstd = next_rstd;
     if (r + stride < rows) { next_mean = __ldg(mean_in + r + stride); next_rstd = __ldg(rstd_in + r + stride); }
     copies_wait<LN_STAGES - 2>();
-    fetch(r0 + (LN_STAGES - 1) * stride, stage == 0 ? LN_STAGES - 1 : stage - 1);      // where the last row was
-    const char* const xs = my_x + stage * row_bytes;
-    const char* const gs = my_g + stage * row_bytes;
-    auto values = [&](int i, float (&f)[VEC], float (&g)[VEC]) {
-      if (i == 0) { SX::template get<EDGE>(xs, xstep, f, first); SG::template get<EDGE>(gs, gstep, g, first); }
-      else { SX::template get<false>(xs + i * SX::WORDS * xstep, xstep, f, 0); SG::template get<false>(gs + i * SG::WORDS * gstep, gstep, g, 0); }
-    };
-    Sums sh, shz;
+    xin.fetch(next_at, r + (LN_STAGES - 1) * stride < rows);         // to where the last row was
+    gin.fetch(next_at, r + (LN_STAGES - 1) * stride < rows);
+    copies_commit();
+    float2 sh = both(0.f), shz = both(0.f);
+    if (r < rows) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      float f[VEC], g[VEC];
-      values(i, f, g);
+      for (int i = 0; i < NV; ++i) {
+        float2 f[VEC / 2], g[VEC / 2];
+        xin.get(at, i, first, f);
+        gin.get(at, i, first, g);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {           // outside the row g is 0
-        const float z = (f[k] - mean) * rstd, h = g[k] * wf[i][k];
-        aw[i][k] = fmaf(g[k], z, aw[i][k]);
-        ab[i][k] += g[k];
-        sh.v[k & 3] += h;
-        shz.v[k & 3] = fmaf(h, z, shz.v[k & 3]);
+        for (int k = 0; k < VEC / 2; ++k) {       // outside the row g is 0
+          const float2 z = mul2(add2(f[k], both(-mean)), both(rstd)), h = mul2(g[k], wf[i][k]);
+          aw[i][k] = fma2(g[k], z, aw[i][k]);
+          ab[i][k] = add2(ab[i][k], g[k]);
+          sh = add2(sh, h);
+          shz = fma2(h, z, shz);
+        }
       }
     }
-    float sum[2] = {sh.total(), shz.total()};
+    float sum[2] = {sh.x + sh.y, shz.x + shz.y};
     grp.sum(sum, buf);
-    // dx = r (h - mean(h) - z mean(h z)) = r h + ((x - mean) A + B)
-    const float A = -rstd * rstd * (sum[1] * inv_d), B = -rstd * (sum[0] * inv_d);
+    if (r < rows) {
+      // dx = r (h - mean(h) - z mean(h z)) = r h + ((x - mean) A + B)
+      const float A = -rstd * rstd * (sum[1] * inv_d), B = -rstd * (sum[0] * inv_d);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j0 = (grp.c + i * grp.T) * VEC - s;
-      float f[VEC], g[VEC];
-      values(i, f, g);
-      if (r < rows && j0 < D) {
+      for (int i = 0; i < NV; ++i) {
+        const int j = j0 + i * vec_step;
+        if (j < D) {
+          float2 f[VEC / 2], g[VEC / 2];
+          xin.get(at, i, first, f);
+          gin.get(at, i, first, g);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) f[k] = fmaf(g[k] * wf[i][k], rstd, fmaf(f[k] - mean, A, B));
-        if (EDGE) store_row<X, VEC>(dx + r * D, j0, D, f); else store_vec(dx + r * D + j0, f);
+          for (int k = 0; k < VEC / 2; ++k) f[k] = fma2(mul2(g[k], wf[i][k]), both(rstd), fma2(add2(f[k], both(-mean)), both(A), both(B)));
+          if (EDGE) store_part<VEC>(out + i * vec_step, j, D, f); else store_vec(out + i * vec_step, f);
+        }
       }
     }
+    next_at = at;
+    at = at + stage_bytes < all ? at + stage_bytes : 0;
   }
   copies_wait<0>();
   if (partial == nullptr) return;
-  float* out = partial + static_cast<int64_t>(blockIdx.x) * 2 * D;
+  float* const part = partial + static_cast<int64_t>(blockIdx.x) * 2 * D;
   if (BLOCK) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
-        const int j = (grp.c + i * grp.T) * VEC - s + k;
-        if (j >= 0 && j < D) { out[j] = aw[i][k]; out[D + j] = ab[i][k]; }
+        const int j = j0 + i * vec_step + k;
+        if (j >= 0 && j < D) { part[j] = k & 1 ? aw[i][k / 2].y : aw[i][k / 2].x; part[D + j] = k & 1 ? ab[i][k / 2].y : ab[i][k / 2].x; }
       }
     return;
   }
@@ -503,8 +570,9 @@ __global__ void __launch_bounds__(BLOCK ? (VEC * NV > 16 ? 256 : 512) : LN_WARP_
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
-          float a = which ? ab[i][k] : aw[i][k];
-          const int j = (grp.c + i * grp.T) * VEC - s + k;
+          const float2 pair = which ? ab[i][k / 2] : aw[i][k / 2];
+          float a = k & 1 ? pair.y : pair.x;
+          const int j = j0 + i * vec_step + k;
           if (same) {
             for (int o = 16; o >= grp.T; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
             if (lane < grp.T && j < D) cols[warp * D + j] = a;
@@ -519,7 +587,7 @@ __global__ void __launch_bounds__(BLOCK ? (VEC * NV > 16 ? 256 : 512) : LN_WARP_
       float a = cols[j];
 #pragma unroll
       for (int k = 1; k < WARPS; ++k) a += cols[k * D + j];
-      out[which * D + j] = a;
+      part[which * D + j] = a;
     }
   }
 }
@@ -556,8 +624,9 @@ static RowPlan plan_rows(int64_t D, int vec, int most) {
     return p;
   }
   p.block = true;
-  p.nv = 4;
-  const int64_t T = (units + 127) / 128 * 32;
+  const int64_t by3 = (units + 95) / 96 * 32, by4 = (units + 127) / 128 * 32;
+  p.nv = by3 * 3 <= by4 * 4 && by3 <= most ? 3 : 4;                              // what leaves fewer of the threads without work
+  const int64_t T = p.nv == 3 ? by3 : by4;
   p.wide = T > most;
   p.T = static_cast<int>(T);
   return p;
@@ -619,7 +688,7 @@ static int ln_fwd_rows(const FwdCall& c, const RowPlan& p) {
 
 template <class X, int VEC, bool EDGE>
 static int ln_fwd_plan(const FwdCall& c, const RowPlan& p) {
-  if (p.block) return ln_fwd_rows<X, VEC, 4, true, EDGE>(c, p);
+  if (p.block) return p.nv == 3 ? ln_fwd_rows<X, VEC, 3, true, EDGE>(c, p) : ln_fwd_rows<X, VEC, 4, true, EDGE>(c, p);
   if (p.nv == 1) return ln_fwd_rows<X, VEC, 1, false, EDGE>(c, p);
   if (p.nv == 2) return ln_fwd_rows<X, VEC, 2, false, EDGE>(c, p);
   if (p.nv == 3) return ln_fwd_rows<X, VEC, 3, false, EDGE>(c, p);
@@ -692,7 +761,7 @@ static int ln_bwd_rows(const BwdCall& c, const RowPlan& p, float* partial, unsig
 
 template <class X, class G, int VEC, bool EDGE>
 static int ln_bwd_plan(const BwdCall& c, const RowPlan& p, float* partial, unsigned& parts) {
-  if (p.block) return ln_bwd_rows<X, G, VEC, 4, true, EDGE>(c, p, partial, parts);
+  if (p.block) return p.nv == 3 ? ln_bwd_rows<X, G, VEC, 3, true, EDGE>(c, p, partial, parts) : ln_bwd_rows<X, G, VEC, 4, true, EDGE>(c, p, partial, parts);
   if (p.nv == 1) return ln_bwd_rows<X, G, VEC, 1, false, EDGE>(c, p, partial, parts);
   if (p.nv == 2) return ln_bwd_rows<X, G, VEC, 2, false, EDGE>(c, p, partial, parts);
   if (p.nv == 3) return ln_bwd_rows<X, G, VEC, 3, false, EDGE>(c, p, partial, parts);
