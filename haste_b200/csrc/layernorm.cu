@@ -298,113 +298,146 @@ __device__ __forceinline__ void load_weights(const void* w, int w_type, bool vec
   for (int k = 0; k < VEC / 2; ++k) out[k] = make_float2(f[2 * k], f[2 * k + 1]);
 }
 
-// The threads that share a row: T lanes of a warp (a power of two), or the block.
-template <bool BLOCK>
+// The threads that share a row: T lanes of a warp (a power of two), or the block.  Thread c of a warp's group has vectors c, c + T, c + 2 T ..
+// of the row; warp v of a block has its vectors 32 NV v and following in the same way, so that from one vector of a thread to its next it
+// is 32 vectors, a constant, wherever T >= 32 (FULL).
+enum RowMode { SUB, FULL, BLOCK };       // groups of up to 32 lanes, of 32, blocks
+template <int MODE, int NV>
 struct RowGroup {
-  int T, c;              // threads of the group, this thread's place among them
+  int T, c;              // threads of a warp's group; first vector of this thread
   int slot = 0;          // buffer of the next sum over a block: a buffer is written again two sums (two barriers) later
-  __device__ explicit RowGroup(int t) : T(BLOCK ? static_cast<int>(blockDim.x) : t), c(static_cast<int>(threadIdx.x) & (BLOCK ? 0x7FFFFFFF : t - 1)) {}
+  __device__ explicit RowGroup(int t) : T(MODE == SUB ? t : 32), c(MODE == SUB ? static_cast<int>(threadIdx.x) & (t - 1) : MODE == FULL ? static_cast<int>(threadIdx.x & 31) : static_cast<int>((threadIdx.x >> 5) * 32 * NV + (threadIdx.x & 31))) {}
   // rows of a warp (of a block) are neighbours; first: that of its first group
-  __device__ int64_t first_row() const { return BLOCK ? blockIdx.x : (static_cast<int64_t>(blockIdx.x) * blockDim.x + (threadIdx.x & ~31u)) / T; }
-  __device__ int64_t stride() const { return BLOCK ? gridDim.x : static_cast<int64_t>(gridDim.x) * blockDim.x / T; }
-  __device__ int64_t own() const { return BLOCK ? 0 : static_cast<int64_t>((threadIdx.x & 31u) / T); }
-  template <int N>
-  __device__ __forceinline__ void sum(float (&v)[N], float (*buf)[N][16]) {
-    if (BLOCK) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-      if ((threadIdx.x & 31) == 0)
-#pragma unroll
-        for (int k = 0; k < N; ++k) buf[slot][k][threadIdx.x >> 5] = v[k];
-      __syncthreads();
-      const int warps = blockDim.x >> 5;
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        v[k] = buf[slot][k][0];
-        for (int i = 1; i < warps; ++i) v[k] += buf[slot][k][i];
-      }
-      slot ^= 1;
-    } else {
-      for (int o = T >> 1; o > 0; o >>= 1)
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  __device__ int64_t first_row() const { return MODE == BLOCK ? blockIdx.x : (static_cast<int64_t>(blockIdx.x) * blockDim.x + (threadIdx.x & ~31u)) / T; }
+  __device__ int64_t stride() const { return MODE == BLOCK ? gridDim.x : static_cast<int64_t>(gridDim.x) * blockDim.x / T; }
+  __device__ int64_t own() const { return MODE == SUB ? static_cast<int64_t>((threadIdx.x & 31u) / T) : 0; }
+  __device__ __forceinline__ void sum_warps(float& v, float* buf) {        // buf: of the slot
+    if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.f;
+    for (int i = 0; i < (static_cast<int>(blockDim.x) + 127) >> 7; ++i) {  // slots of warps that the block has not got hold zeros
+      const float4 q = reinterpret_cast<const float4*>(buf)[i];
+      v += (q.x + q.y) + (q.z + q.w);
     }
+  }
+  __device__ __forceinline__ float sum(float v, float (*buf)[2][16]) {
+    if (MODE == SUB) {
+      for (int o = T >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      return v;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (MODE == BLOCK) { sum_warps(v, buf[slot][0]); slot ^= 1; }
+    return v;
+  }
+  // Two sums for little more than one: after the first exchange the lower half of a warp adds up a, the upper half b.
+  __device__ __forceinline__ void sum2_lanes(float& a, float& b) {
+    if (MODE == SUB) {
+      for (int o = T >> 1; o > 0; o >>= 1) { a += __shfl_xor_sync(0xffffffffu, a, o); b += __shfl_xor_sync(0xffffffffu, b, o); }
+      return;
+    }
+    const bool upper = threadIdx.x & 16;
+    const float other = __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
+    float v = (upper ? b : a) + other;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (MODE == BLOCK) { a = v; return; }                                  // sum2_warps takes it from lanes 0 and 16
+    a = __shfl_sync(0xffffffffu, v, 0);
+    b = __shfl_sync(0xffffffffu, v, 16);
+  }
+  __device__ __forceinline__ void sum2_warps(float& a, float& b, float (*buf)[2][16]) {
+    if (MODE != BLOCK) return;
+    if ((threadIdx.x & 15) == 0) buf[slot][(threadIdx.x >> 4) & 1][threadIdx.x >> 5] = a;
+    __syncthreads();
+    a = b = 0.f;
+    for (int i = 0; i < (static_cast<int>(blockDim.x) + 127) >> 7; ++i) {
+      const float4 q = reinterpret_cast<const float4*>(buf[slot][0])[i], p = reinterpret_cast<const float4*>(buf[slot][1])[i];
+      a += (q.x + q.y) + (q.z + q.w);
+      b += (p.x + p.y) + (p.z + p.w);
+    }
+    slot ^= 1;
+  }
+  // Zeros for the warps that the block has not got; a barrier follows before the first sum is read.
+  __device__ __forceinline__ void clear(float (*buf)[2][16]) {
+    if (MODE == BLOCK && threadIdx.x < 64) (&buf[0][0][0])[threadIdx.x] = 0.f;
+    if (MODE == BLOCK) __syncthreads();
   }
 };
 
-// A row group's walk over an input: the copies of its next row.
-template <class T, int VEC, int NV, bool EDGE>
+// A row group's walk over an input: the copies of its next row.  A warp's slots lie together, 32 units for each word of a vector.
+template <class T, int VEC, int NV, int MODE, bool EDGE>
 struct Feed {
   using S = Slot<T, VEC>;
+  static constexpr int STEP = 32 * S::UNIT, WARP_BYTES = NV * S::WORDS * STEP;      // between the words of a slot; of a warp and stage
   const T* next;           // column j0 of the row to be copied next
   int64_t row_step;        // elements from a row of the group to its next one
-  int vec_step, step;      // elements from a vector of the thread to its next one; bytes between the words of a slot
+  int t_step;              // elements from a vector of the thread to its next one (SUB)
   int j0, D;
   bool vec;
   char* slots;             // the thread's own, of the first stage
   uint32_t to;
   __device__ __forceinline__ Feed(const T* p, int64_t ld, int64_t row, int64_t stride, int j0_, int D_, int T_, bool vec_, char* area)
-      : next(p + row * ld + j0_), row_step(stride * ld), vec_step(T_ * VEC), step(static_cast<int>(blockDim.x) * S::UNIT), j0(j0_), D(D_), vec(vec_),
-        slots(area + threadIdx.x * S::UNIT), to(smem_address(slots)) {}
-  static __device__ __forceinline__ int bytes() { return NV * S::WORDS * S::UNIT * static_cast<int>(blockDim.x); }
+      : next(p + row * ld + j0_), row_step(stride * ld), t_step(T_ * VEC), j0(j0_), D(D_), vec(vec_),
+        slots(area + (threadIdx.x >> 5) * WARP_BYTES + (threadIdx.x & 31) * S::UNIT), to(smem_address(slots)) {}
+  __device__ __forceinline__ int vec_step() const { return MODE == SUB ? t_step : 32 * VEC; }
+  static __device__ __forceinline__ int bytes() { return WARP_BYTES * static_cast<int>(blockDim.x >> 5); }
   // Slots that no copy reaches (vectors right of the row) hold zeros for good.
-  __device__ __forceinline__ void clear(int stage_bytes) const {
+  __device__ __forceinline__ void clear(int stages, int stage_bytes) const {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (j0 + i * vec_step >= D)
-        for (int k = 0; k < LN_STAGES; ++k) S::clear(slots + k * stage_bytes + i * S::WORDS * step, step);
+      if (j0 + i * vec_step() >= D)
+        for (int k = 0; k < stages; ++k) S::clear(slots + k * stage_bytes + i * S::WORDS * STEP, STEP);
   }
   __device__ __forceinline__ void fetch(int at, bool there) {
     if (there) {
       if (vec) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          const int j = j0 + i * vec_step;
+          const int j = j0 + i * vec_step();
           if (j < D) {
-            if (!EDGE) S::copy(to + at + i * S::WORDS * step, step, next + i * vec_step);
-            else S::copy_part(to + at + i * S::WORDS * step, step, next + i * vec_step, min(D - j, VEC));
+            if (!EDGE) S::copy(to + at + i * S::WORDS * STEP, STEP, next + i * vec_step());
+            else S::copy_part(to + at + i * S::WORDS * STEP, STEP, next + i * vec_step(), min(D - j, VEC));
           }
         }
       } else {
 #pragma unroll 1
         for (int i = 0; i < NV; ++i) {
-          const int j = j0 + i * vec_step;
-          if (j < D) S::copy_single(slots + at + i * S::WORDS * step, step, next + i * vec_step, -j, D - j);
+          const int j = j0 + i * vec_step();
+          if (j < D) S::copy_single(slots + at + i * S::WORDS * STEP, STEP, next + i * vec_step(), -j, D - j);
         }
       }
     }
     next += row_step;
   }
   __device__ __forceinline__ void get(int at, int i, int first, float2 (&f)[VEC / 2]) const {
-    if (i == 0) S::template get<EDGE>(slots + at, step, f, first);
-    else S::template get<false>(slots + at + i * S::WORDS * step, step, f, 0);
+    if (i == 0) S::template get<EDGE>(slots + at, STEP, f, first);
+    else S::template get<false>(slots + at + i * S::WORDS * STEP, STEP, f, 0);
   }
 };
 
 // EDGE: D is no multiple of VEC, rows have first and last vectors that are theirs in part.
-template <class X, int VEC, int NV, bool BLOCK, bool EDGE>
-__global__ void __launch_bounds__(BLOCK ? 512 : LN_WARP_THREADS, BLOCK ? 1 : 4)
+template <class X, int VEC, int NV, int MODE, bool EDGE>
+__global__ void __launch_bounds__(MODE == BLOCK ? 512 : LN_WARP_THREADS, MODE == BLOCK ? 1 : 4)
     ln_fwd_kernel(const X* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b, int w_type, X* __restrict__ y, float* __restrict__ mean_out,
                   float* __restrict__ rstd_out, int64_t rows, int D, int64_t ldx, float eps, int t, bool x_vec, bool w_vec) {
-  __shared__ float buf[2][1][16];
+  __shared__ __align__(16) float buf[2][2][16];
   extern __shared__ __align__(16) char slots[];
-  RowGroup<BLOCK> grp(t);
+  RowGroup<MODE, NV> grp(t);
+  grp.clear(buf);
   const float inv_d = 1.f / static_cast<float>(D);
   const int64_t stride = grp.stride();
   int64_t r = grp.first_row() + grp.own(), left = rows - grp.first_row();       // left: rows from the warp's (block's) first one on
-  const int s = EDGE ? static_cast<int>(r * D % VEC) : 0, first = grp.c == 0 ? s : 0, j0 = grp.c * VEC - s, vec_step = grp.T * VEC;
-  Feed<X, VEC, NV, EDGE> in(x, ldx, r, stride, j0, D, grp.T, x_vec, slots);
+  const int s = EDGE ? static_cast<int>(r * D % VEC) : 0, first = grp.c == 0 ? s : 0, j0 = grp.c * VEC - s;
+  Feed<X, VEC, NV, MODE, EDGE> in(x, ldx, r, stride, j0, D, grp.T, x_vec, slots);
   const int stage_bytes = in.bytes(), all = LN_STAGES * stage_bytes;
-  in.clear(stage_bytes);
+  in.clear(LN_STAGES, stage_bytes);
 #pragma unroll
   for (int k = 0; k < LN_STAGES - 1; ++k) { in.fetch(k * stage_bytes, r + k * stride < rows); copies_commit(); }
   float2 wf[NV][VEC / 2], bf[NV][VEC / 2];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    load_weights<VEC>(w, w_type, !EDGE && w_vec, j0 + i * vec_step, D, 1.f, wf[i]);
-    load_weights<VEC>(b, w_type, !EDGE && w_vec, j0 + i * vec_step, D, 0.f, bf[i]);
+    load_weights<VEC>(w, w_type, !EDGE && w_vec, j0 + i * in.vec_step(), D, 1.f, wf[i]);
+    load_weights<VEC>(b, w_type, !EDGE && w_vec, j0 + i * in.vec_step(), D, 0.f, bf[i]);
   }
   X* out = y + r * D + j0;
   for (int at = 0, next_at = all - stage_bytes; left > 0; left -= stride, r += stride, out += stride * D) {
@@ -419,37 +452,38 @@ __global__ void __launch_bounds__(BLOCK ? 512 : LN_WARP_THREADS, BLOCK ? 1 : 4)
       for (int k = 0; k < VEC / 2; ++k) { if (k & 1) s2 = add2(s2, f[i][k]); else s1 = add2(s1, f[i][k]); }
     }
     s1 = add2(s1, s2);
-    float sum[1] = {s1.x + s1.y};
-    grp.sum(sum, buf);
-    const float mean = sum[0] * inv_d;
+    const float mean = grp.sum(s1.x + s1.y, buf) * inv_d;
     s1 = s2 = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = j0 + i * vec_step;
+      const int j = j0 + i * in.vec_step();
+      float2 d[VEC / 2];
 #pragma unroll
-      for (int k = 0; k < VEC / 2; ++k) {
-        f[i][k] = add2(f[i][k], both(-mean));
-        if (EDGE) {
-          const float2 d = make_float2(static_cast<unsigned>(j + 2 * k) < static_cast<unsigned>(D) ? f[i][k].x : 0.f,
-                                       static_cast<unsigned>(j + 2 * k + 1) < static_cast<unsigned>(D) ? f[i][k].y : 0.f);
-          if (k & 1) s2 = fma2(d, d, s2); else s1 = fma2(d, d, s1);
-        } else if (i < NV - 1 || j < D) {                            // (the host gives a thread no more vectors than a row has)
-          if (k & 1) s2 = fma2(f[i][k], f[i][k], s2); else s1 = fma2(f[i][k], f[i][k], s1);
-        }
+      for (int k = 0; k < VEC / 2; ++k) d[k] = f[i][k] = add2(f[i][k], both(-mean));
+      // what is not the row's counts for nothing (a row ends in one of a thread's last two vectors; a block may have whole warps beyond it)
+      if (EDGE && i == 0) {
+#pragma unroll
+        for (int k = 0; k < VEC / 2; ++k) { d[k].x = 2 * k < first ? 0.f : d[k].x; d[k].y = 2 * k + 1 < first ? 0.f : d[k].y; }
+      }
+      if (EDGE && (MODE == BLOCK || i >= NV - 2)) {
+#pragma unroll
+        for (int k = 0; k < VEC / 2; ++k) { d[k].x = j + 2 * k < D ? d[k].x : 0.f; d[k].y = j + 2 * k + 1 < D ? d[k].y : 0.f; }
+      }
+      if (EDGE || j < D) {
+#pragma unroll
+        for (int k = 0; k < VEC / 2; ++k) { if (k & 1) s2 = fma2(d[k], d[k], s2); else s1 = fma2(d[k], d[k], s1); }
       }
     }
     s1 = add2(s1, s2);
-    sum[0] = s1.x + s1.y;
-    grp.sum(sum, buf);
-    const float rstd = 1.f / sqrtf(fmaf(sum[0], inv_d, eps));
+    const float rstd = 1.f / sqrtf(fmaf(grp.sum(s1.x + s1.y, buf), inv_d, eps));
     if (r < rows) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int j = j0 + i * vec_step;
+        const int j = j0 + i * in.vec_step();
         if (j < D) {
 #pragma unroll
           for (int k = 0; k < VEC / 2; ++k) f[i][k] = fma2(mul2(f[i][k], both(rstd)), wf[i][k], bf[i][k]);
-          if (EDGE) store_part<VEC>(out + i * vec_step, j, D, f[i]); else store_vec(out + i * vec_step, f[i]);
+          if (EDGE) store_part<VEC>(out + i * in.vec_step(), j, D, f[i]); else store_vec(out + i * in.vec_step(), f[i]);
         }
       }
       if (grp.c == 0 && mean_out != nullptr) { mean_out[r] = mean; rstd_out[r] = rstd; }
@@ -461,25 +495,28 @@ __global__ void __launch_bounds__(BLOCK ? 512 : LN_WARP_THREADS, BLOCK ? 1 : 4)
 }
 
 // dx, and the block's part of dw and db: partial[block][0][.] and [1][.] (NULL: only dx is wanted).
-template <class X, class G, int VEC, int NV, bool BLOCK, bool EDGE>
-__global__ void __launch_bounds__(BLOCK ? (VEC * NV > 16 ? 256 : 512) : LN_WARP_THREADS) __maxnreg__(VEC * NV > 16 ? 168 : 128)
+// A row's sums are on their way through the warps while the next row's are taken, so two rows have arrived and the others (two of STAGES = 4,
+// one of 3) are being copied.
+template <class X, class G, int VEC, int NV, int MODE, bool EDGE, int STAGES>
+__global__ void __launch_bounds__(MODE == BLOCK ? (VEC * NV > 16 ? 256 : 512) : LN_WARP_THREADS) __maxnreg__(VEC * NV > 16 ? 168 : 128)
     ln_bwd_kernel(const G* __restrict__ dy, const X* __restrict__ x, const void* __restrict__ w, int w_type, const float* __restrict__ mean_in,
                   const float* __restrict__ rstd_in, X* __restrict__ dx, float* __restrict__ partial, int64_t rows, int D, int64_t lddy, int64_t ldx, int t,
                   bool x_vec, bool dy_vec, bool w_vec) {
-  __shared__ float buf[2][2][16];
+  __shared__ __align__(16) float buf[2][2][16];
   extern __shared__ __align__(16) char slots[];
-  RowGroup<BLOCK> grp(t);
+  RowGroup<MODE, NV> grp(t);
+  grp.clear(buf);
   const float inv_d = 1.f / static_cast<float>(D);
   const int64_t stride = grp.stride();
   int64_t r = grp.first_row() + grp.own(), left = rows - grp.first_row();
-  const int s = EDGE ? static_cast<int>(r * D % VEC) : 0, first = grp.c == 0 ? s : 0, j0 = grp.c * VEC - s, vec_step = grp.T * VEC;
-  Feed<X, VEC, NV, EDGE> xin(x, ldx, r, stride, j0, D, grp.T, x_vec, slots);
-  Feed<G, VEC, NV, EDGE> gin(dy, lddy, r, stride, j0, D, grp.T, dy_vec, slots + xin.bytes());
-  const int stage_bytes = xin.bytes() + gin.bytes(), all = LN_STAGES * stage_bytes;
-  xin.clear(stage_bytes);
-  gin.clear(stage_bytes);
+  const int s = EDGE ? static_cast<int>(r * D % VEC) : 0, first = grp.c == 0 ? s : 0, j0 = grp.c * VEC - s;
+  Feed<X, VEC, NV, MODE, EDGE> xin(x, ldx, r, stride, j0, D, grp.T, x_vec, slots);
+  Feed<G, VEC, NV, MODE, EDGE> gin(dy, lddy, r, stride, j0, D, grp.T, dy_vec, slots + xin.bytes());
+  const int stage_bytes = xin.bytes() + gin.bytes(), all = STAGES * stage_bytes;
+  xin.clear(STAGES, stage_bytes);
+  gin.clear(STAGES, stage_bytes);
 #pragma unroll
-  for (int k = 0; k < LN_STAGES - 1; ++k) {
+  for (int k = 0; k < STAGES - 1; ++k) {
     xin.fetch(k * stage_bytes, r + k * stride < rows);
     gin.fetch(k * stage_bytes, r + k * stride < rows);
     copies_commit();
@@ -487,62 +524,75 @@ __global__ void __launch_bounds__(BLOCK ? (VEC * NV > 16 ? 256 : 512) : LN_WARP_
   float2 wf[NV][VEC / 2], aw[NV][VEC / 2], ab[NV][VEC / 2];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    load_weights<VEC>(w, w_type, !EDGE && w_vec, j0 + i * vec_step, D, 1.f, wf[i]);
+    load_weights<VEC>(w, w_type, !EDGE && w_vec, j0 + i * xin.vec_step(), D, 1.f, wf[i]);
 #pragma unroll
     for (int k = 0; k < VEC / 2; ++k) aw[i][k] = ab[i][k] = both(0.f);
   }
-  float next_mean = 0.f, next_rstd = 0.f;
-  if (r < rows) { next_mean = __ldg(mean_in + r); next_rstd = __ldg(rstd_in + r); }
-  X* out = dx + r * D + j0;
-  for (int at = 0, next_at = all - stage_bytes; left > 0; left -= stride, r += stride, out += stride * D) {
-    const float mean = next_mean, rstd = next_rstd;
-    if (r + stride < rows) { next_mean = __ldg(mean_in + r + stride); next_rstd = __ldg(rstd_in + r + stride); }
-    copies_wait<LN_STAGES - 2>();
-    xin.fetch(next_at, r + (LN_STAGES - 1) * stride < rows);         // to where the last row was
-    gin.fetch(next_at, r + (LN_STAGES - 1) * stride < rows);
-    copies_commit();
+  // sums of h and h z over a thread's columns of the row at `at`
+  auto row_sums = [&](int at, float mean, float rstd, float& a, float& b) {
     float2 sh = both(0.f), shz = both(0.f);
-    if (r < rows) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        float2 f[VEC / 2], g[VEC / 2];
-        xin.get(at, i, first, f);
-        gin.get(at, i, first, g);
+    for (int i = 0; i < NV; ++i) {
+      float2 f[VEC / 2], g[VEC / 2];
+      xin.get(at, i, first, f);
+      gin.get(at, i, first, g);
 #pragma unroll
-        for (int k = 0; k < VEC / 2; ++k) {       // outside the row g is 0
-          const float2 z = mul2(add2(f[k], both(-mean)), both(rstd)), h = mul2(g[k], wf[i][k]);
-          aw[i][k] = fma2(g[k], z, aw[i][k]);
-          ab[i][k] = add2(ab[i][k], g[k]);
-          sh = add2(sh, h);
-          shz = fma2(h, z, shz);
-        }
+      for (int k = 0; k < VEC / 2; ++k) {       // outside the row g is 0
+        const float2 z = mul2(add2(f[k], both(-mean)), both(rstd)), h = mul2(g[k], wf[i][k]);
+        aw[i][k] = fma2(g[k], z, aw[i][k]);
+        ab[i][k] = add2(ab[i][k], g[k]);
+        sh = add2(sh, h);
+        shz = fma2(h, z, shz);
       }
     }
-    float sum[2] = {sh.x + sh.y, shz.x + shz.y};
-    grp.sum(sum, buf);
+    a = sh.x + sh.y;
+    b = shz.x + shz.y;
+  };
+  const float *mean_at = mean_in + r, *rstd_at = rstd_in + r;
+  float mean = 0.f, rstd = 0.f, next_mean = 0.f, next_rstd = 0.f, a = 0.f, b = 0.f;
+  if (r < rows) { mean = __ldg(mean_at); rstd = __ldg(rstd_at); }
+  if (r + stride < rows) { next_mean = __ldg(mean_at + stride); next_rstd = __ldg(rstd_at + stride); }
+  copies_wait<STAGES - 2>();
+  if (r < rows) row_sums(0, mean, rstd, a, b);
+  X* out = dx + r * D + j0;
+  for (int at = 0, free_at = all - stage_bytes; left > 0; left -= stride, r += stride, out += stride * D) {
+    const int next_at = at + stage_bytes < all ? at + stage_bytes : 0;
+    copies_wait<STAGES - 3>();
+    xin.fetch(free_at, r + (STAGES - 1) * stride < rows);     // to where the last row was
+    gin.fetch(free_at, r + (STAGES - 1) * stride < rows);
+    copies_commit();
+    mean_at += stride;
+    rstd_at += stride;
+    float after_mean = 0.f, after_rstd = 0.f, next_a = 0.f, next_b = 0.f;
+    if (r + 2 * stride < rows) { after_mean = __ldg(mean_at + stride); after_rstd = __ldg(rstd_at + stride); }
+    grp.sum2_lanes(a, b);
+    if (r + stride < rows) row_sums(next_at, next_mean, next_rstd, next_a, next_b);
+    grp.sum2_warps(a, b, buf);
     if (r < rows) {
       // dx = r (h - mean(h) - z mean(h z)) = r h + ((x - mean) A + B)
-      const float A = -rstd * rstd * (sum[1] * inv_d), B = -rstd * (sum[0] * inv_d);
+      const float A = -rstd * rstd * (b * inv_d), B = -rstd * (a * inv_d);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int j = j0 + i * vec_step;
+        const int j = j0 + i * xin.vec_step();
         if (j < D) {
           float2 f[VEC / 2], g[VEC / 2];
           xin.get(at, i, first, f);
           gin.get(at, i, first, g);
 #pragma unroll
           for (int k = 0; k < VEC / 2; ++k) f[k] = fma2(mul2(g[k], wf[i][k]), both(rstd), fma2(add2(f[k], both(-mean)), both(A), both(B)));
-          if (EDGE) store_part<VEC>(out + i * vec_step, j, D, f); else store_vec(out + i * vec_step, f);
+          if (EDGE) store_part<VEC>(out + i * xin.vec_step(), j, D, f); else store_vec(out + i * xin.vec_step(), f);
         }
       }
     }
-    next_at = at;
-    at = at + stage_bytes < all ? at + stage_bytes : 0;
+    mean = next_mean; rstd = next_rstd; next_mean = after_mean; next_rstd = after_rstd; a = next_a; b = next_b;
+    free_at = at;
+    at = next_at;
   }
   copies_wait<0>();
   if (partial == nullptr) return;
   float* const part = partial + static_cast<int64_t>(blockIdx.x) * 2 * D;
-  if (BLOCK) {
+  const int vec_step = xin.vec_step();
+  if (MODE == BLOCK) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -675,24 +725,24 @@ struct FwdCall {
   cudaStream_t st;
 };
 
-template <class X, int VEC, int NV, bool BLOCK, bool EDGE>
+template <class X, int VEC, int NV, int MODE, bool EDGE>
 static int ln_fwd_rows(const FwdCall& c, const RowPlan& p) {
   static std::atomic<uint64_t> allowed{0};
-  const int threads = BLOCK ? p.T : LN_WARP_THREADS, smem = LN_STAGES * NV * threads * VEC * static_cast<int>(sizeof(X));
-  if (int rc = allow_slots(ln_fwd_kernel<X, VEC, NV, BLOCK, EDGE>, allowed)) return rc;
+  const int threads = MODE == BLOCK ? p.T : LN_WARP_THREADS, smem = LN_STAGES * NV * threads * VEC * static_cast<int>(sizeof(X));
+  if (int rc = allow_slots(ln_fwd_kernel<X, VEC, NV, MODE, EDGE>, allowed)) return rc;
   const unsigned blocks = row_blocks(p, c.rows, c.D, VEC, VEC * NV > 16 ? 512 : VEC * NV > 8 ? 768 : 1024);
-  ln_fwd_kernel<X, VEC, NV, BLOCK, EDGE><<<blocks, threads, smem, c.st>>>((const X*)c.x, c.w, c.b, c.w_type, (X*)c.y, c.mean, c.rstd, c.rows, static_cast<int>(c.D), c.ldx,
+  ln_fwd_kernel<X, VEC, NV, MODE, EDGE><<<blocks, threads, smem, c.st>>>((const X*)c.x, c.w, c.b, c.w_type, (X*)c.y, c.mean, c.rstd, c.rows, static_cast<int>(c.D), c.ldx,
                                                                     c.eps, p.T, in_vectors(c.x, c.ldx, c.D, VEC, 16), aligned16(c.w) && aligned16(c.b));
   return check_launch("layer_norm_forward");
 }
 
 template <class X, int VEC, bool EDGE>
 static int ln_fwd_plan(const FwdCall& c, const RowPlan& p) {
-  if (p.block) return p.nv == 3 ? ln_fwd_rows<X, VEC, 3, true, EDGE>(c, p) : ln_fwd_rows<X, VEC, 4, true, EDGE>(c, p);
-  if (p.nv == 1) return ln_fwd_rows<X, VEC, 1, false, EDGE>(c, p);
-  if (p.nv == 2) return ln_fwd_rows<X, VEC, 2, false, EDGE>(c, p);
-  if (p.nv == 3) return ln_fwd_rows<X, VEC, 3, false, EDGE>(c, p);
-  return ln_fwd_rows<X, VEC, 4, false, EDGE>(c, p);
+  if (p.block) return p.nv == 3 ? ln_fwd_rows<X, VEC, 3, BLOCK, EDGE>(c, p) : ln_fwd_rows<X, VEC, 4, BLOCK, EDGE>(c, p);
+  if (p.nv == 1) return ln_fwd_rows<X, VEC, 1, SUB, EDGE>(c, p);
+  if (p.nv == 2) return ln_fwd_rows<X, VEC, 2, SUB, EDGE>(c, p);
+  if (p.nv == 3) return ln_fwd_rows<X, VEC, 3, FULL, EDGE>(c, p);
+  return ln_fwd_rows<X, VEC, 4, FULL, EDGE>(c, p);
 }
 
 template <class X>
@@ -745,15 +795,18 @@ struct BwdCall {
   cudaStream_t st;
 };
 
-template <class X, class G, int VEC, int NV, bool BLOCK, bool EDGE>
+template <class X, class G, int VEC, int NV, int MODE, bool EDGE, int STAGES = 4>
 static int ln_bwd_rows(const BwdCall& c, const RowPlan& p, float* partial, unsigned& parts) {
   static std::atomic<uint64_t> allowed{0};
-  const int threads = BLOCK ? p.T : LN_WARP_THREADS, slots = LN_STAGES * NV * threads * VEC * static_cast<int>(sizeof(X) + sizeof(G));
-  const int cols = BLOCK ? 0 : LN_WARP_THREADS / 32 * static_cast<int>(c.D) * 4, smem = slots > cols ? slots : cols;
-  if (int rc = allow_slots(ln_bwd_kernel<X, G, VEC, NV, BLOCK, EDGE>, allowed)) return rc;
+  const int threads = MODE == BLOCK ? p.T : LN_WARP_THREADS;
+  if constexpr (MODE == BLOCK && STAGES == 4 && VEC * sizeof(G) == 16)          // fp32 rows of more than 6144 elements: 4 stages do not fit
+    if (STAGES * NV * threads * VEC * static_cast<int>(sizeof(X) + sizeof(G)) > DYN_SMEM_MAX) return ln_bwd_rows<X, G, VEC, NV, MODE, EDGE, 3>(c, p, partial, parts);
+  const int slots = STAGES * NV * threads * VEC * static_cast<int>(sizeof(X) + sizeof(G));
+  const int cols = MODE == BLOCK ? 0 : LN_WARP_THREADS / 32 * static_cast<int>(c.D) * 4, smem = slots > cols ? slots : cols;
+  if (int rc = allow_slots(ln_bwd_kernel<X, G, VEC, NV, MODE, EDGE, STAGES>, allowed)) return rc;
   parts = row_blocks(p, c.rows, c.D, VEC, VEC * NV > 16 ? 384 : VEC * NV > 8 ? 512 : 1024);
   const int64_t g_bytes = VEC * sizeof(G) < 16 ? 8 : 16;
-  ln_bwd_kernel<X, G, VEC, NV, BLOCK, EDGE><<<parts, threads, smem, c.st>>>((const G*)c.dy, (const X*)c.x, c.w, c.w_type, c.mean, c.rstd, (X*)c.dx, partial, c.rows,
+  ln_bwd_kernel<X, G, VEC, NV, MODE, EDGE, STAGES><<<parts, threads, smem, c.st>>>((const G*)c.dy, (const X*)c.x, c.w, c.w_type, c.mean, c.rstd, (X*)c.dx, partial, c.rows,
                                                                       static_cast<int>(c.D), c.lddy, c.ldx, p.T, in_vectors(c.x, c.ldx, c.D, VEC, 16),
                                                                       in_vectors(c.dy, c.lddy, c.D, VEC, g_bytes), aligned16(c.w));
   return check_launch("layer_norm_backward");
@@ -761,11 +814,11 @@ static int ln_bwd_rows(const BwdCall& c, const RowPlan& p, float* partial, unsig
 
 template <class X, class G, int VEC, bool EDGE>
 static int ln_bwd_plan(const BwdCall& c, const RowPlan& p, float* partial, unsigned& parts) {
-  if (p.block) return p.nv == 3 ? ln_bwd_rows<X, G, VEC, 3, true, EDGE>(c, p, partial, parts) : ln_bwd_rows<X, G, VEC, 4, true, EDGE>(c, p, partial, parts);
-  if (p.nv == 1) return ln_bwd_rows<X, G, VEC, 1, false, EDGE>(c, p, partial, parts);
-  if (p.nv == 2) return ln_bwd_rows<X, G, VEC, 2, false, EDGE>(c, p, partial, parts);
-  if (p.nv == 3) return ln_bwd_rows<X, G, VEC, 3, false, EDGE>(c, p, partial, parts);
-  return ln_bwd_rows<X, G, VEC, 4, false, EDGE>(c, p, partial, parts);
+  if (p.block) return p.nv == 3 ? ln_bwd_rows<X, G, VEC, 3, BLOCK, EDGE>(c, p, partial, parts) : ln_bwd_rows<X, G, VEC, 4, BLOCK, EDGE>(c, p, partial, parts);
+  if (p.nv == 1) return ln_bwd_rows<X, G, VEC, 1, SUB, EDGE>(c, p, partial, parts);
+  if (p.nv == 2) return ln_bwd_rows<X, G, VEC, 2, SUB, EDGE>(c, p, partial, parts);
+  if (p.nv == 3) return ln_bwd_rows<X, G, VEC, 3, FULL, EDGE>(c, p, partial, parts);
+  return ln_bwd_rows<X, G, VEC, 4, FULL, EDGE>(c, p, partial, parts);
 }
 
 template <class X, class G>
