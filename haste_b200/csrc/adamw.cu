@@ -100,6 +100,15 @@ __device__ __forceinline__ uint4 philox4x32_7(uint32_t c0, uint32_t c1, uint32_t
   return make_uint4(c0, c1, c2, c3);
 }
 
+// Root and quotient of the update to a few units in the last place: the update is a small part of the weight, whose own rounding hides
+// them, and neither enters the moments.  (133 M bf16 weights with 32-bit moments: 663 us with correctly rounded ones, 460 so; 56 M with
+// 8-bit moments 386 and 244.)
+__device__ __forceinline__ float root_of(float v) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 // ---------------------------------------------------------------- 8-bit codes
 // Code c of a value y in (0, 1.875]: the upper 12 bits of its fp32 pattern less BASE.
 constexpr uint32_t M_BASE = 0x380u, V_BASE = 0x300u;      // pattern of 1.875 is 0x3FF.....: 0x3FF - 127 and 0x3FF - 255
@@ -200,7 +209,7 @@ __global__ void __launch_bounds__(ADAM_THREADS) adamw_kernel(const __grid_consta
       const float gi = g[i] * scale;
       m[i] = fmaf(a.b1, m[i], a.c1 * gi);
       v[i] = fmaf(a.b2, v[i], a.c2 * gi * gi);
-      const float wn = fmaf(-a.rate, m[i] / fmaf(sqrtf(v[i]), a.root, a.eps), w[i] * a.decay);
+      const float wn = fmaf(-a.rate, __fdividef(m[i], fmaf(root_of(v[i]), a.root, a.eps)), w[i] * a.decay);
       if (sizeof(P) == 4) out[i] = __float_as_uint(wn);
       // (a NaN's pattern is 0x7FFFFFFF: with bits added it would read as -0)
       else out[i] = sr ? __float_as_uint(wn) + (wn == wn ? rnd[i] & 0xFFFFu : 0u) : static_cast<uint32_t>(rn_bf16_bits(wn)) << 16;
