@@ -30,7 +30,8 @@
 namespace haste {
 
 constexpr int ADAM_BLOCK = 256;        // elements that share a scale; the place of a tensor in the moments is a multiple of it
-constexpr int ADAM_THREADS = 256;
+constexpr int ADAM_THREADS = 256, ADAM_WARPS = ADAM_THREADS / 32;
+constexpr int AHEAD = 4;               // blocks of gradients that a warp of the norm has on their way, and the most of a turn
 constexpr float CODE_TOP = 1.875f;
 constexpr float CODE_TINY = 0x1p-120f; // a block whose largest value is below holds zeros (1.875 / it is finite)
 
@@ -44,26 +45,57 @@ struct TensorTable {
   int32_t count;
 };
 
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+// The tensor that block b of the launch belongs to.
+template <int N>
+__device__ __forceinline__ int tensor_of(const TensorTable<N>& tab, int b) {
+  int lo = 0, hi = tab.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (tab.first[mid + 1] <= b) lo = mid + 1; else hi = mid;
+  }
+  return lo;
 }
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
-}
-__device__ __forceinline__ float load1(const float* p) { return *p; }
-__device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
-// 8 elements of a lane; left: how many exist (the others read as 0).  vec: all 8 are there and the address is on 16 bytes.
+// 8 elements of a lane as they lie in memory.  Loading does not look at them: a load that is unpacked in its own branch is waited for
+// there, before the next one starts (56 M gradients: norm 35 us so unpacked).
 template <class T>
-__device__ __forceinline__ void load_lane(const T* p, bool vec, int64_t left, float (&v)[8]) {
-  if (vec) { load8(p, v); return; }
+struct Lane8 {
+  static constexpr int WORDS = static_cast<int>(sizeof(T)) / 2;       // of 16 bytes
+  uint4 q[WORDS];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = i < left ? load1(p + i) : 0.f;
-}
+    for (int i = 0; i < WORDS; ++i) q[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  // the first `left` elements one by one, then zeros
+  __device__ __forceinline__ void load_part(const T* p, int64_t left) {
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (sizeof(T) == 4) u[i] = i < left ? __float_as_uint(p[i]) : 0u;
+      else u[i] = i < left ? reinterpret_cast<const uint16_t*>(p)[i] : 0u;
+    }
+    if constexpr (sizeof(T) == 4) { q[0] = make_uint4(u[0], u[1], u[2], u[3]); q[1] = make_uint4(u[4], u[5], u[6], u[7]); }
+    else q[0] = make_uint4(u[0] | (u[1] << 16), u[2] | (u[3] << 16), u[4] | (u[5] << 16), u[6] | (u[7] << 16));
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) q[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ void get(float2 (&v)[4]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        v[2 * i] = make_float2(__uint_as_float(q[i].x), __uint_as_float(q[i].y));
+        v[2 * i + 1] = make_float2(__uint_as_float(q[i].z), __uint_as_float(q[i].w));
+      }
+    } else {
+      const uint32_t u[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xFFFF0000u));
+    }
+  }
+};
+__device__ __forceinline__ bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // The fp32 patterns in u become weights: stored as they are, or their upper halves.
 __device__ __forceinline__ void store_lane(float* p, bool vec, int64_t left, const uint32_t (&u)[8]) {
@@ -100,50 +132,114 @@ __device__ __forceinline__ uint4 philox4x32_7(uint32_t c0, uint32_t c1, uint32_t
   return make_uint4(c0, c1, c2, c3);
 }
 
+// Two fp32 numbers as one operand: one instruction for both.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
+      "l"(reinterpret_cast<const uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 // Root and quotient of the update to a few units in the last place: the update is a small part of the weight, whose own rounding hides
 // them, and neither enters the moments.  (133 M bf16 weights with 32-bit moments: 663 us with correctly rounded ones, 460 so; 56 M with
-// 8-bit moments 386 and 244.)
+// 8-bit moments 386 and 244.)  A second moment below 2^-126 counts as 0 here.
 __device__ __forceinline__ float root_of(float v) {
   float r;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float inverse_of(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
 
 // ---------------------------------------------------------------- 8-bit codes
-// Code c of a value y in (0, 1.875]: the upper 12 bits of its fp32 pattern less BASE.
-constexpr uint32_t M_BASE = 0x380u, V_BASE = 0x300u;      // pattern of 1.875 is 0x3FF.....: 0x3FF - 127 and 0x3FF - 255
+// The code of a value y in (0, 1.875] is the upper 12 bits of its fp32 pattern less a base: 0x300 for the second moment (0x3FF, the pattern
+// of 1.875, becomes 255), 0x380 for the first one's magnitude (0x3FF becomes 127).  Integer instructions that are not products have half the
+// rate of the others and were what bounded the 8-bit step, so codes are taken apart two at a time, as bf16 (whose pattern is the upper
+// half of fp32's), and put together by byte selection: 56 M bf16 weights 244 us one at a time, 154 so (148 with what came after).
+// Copying the next block ahead of time, which takes 15 registers, changed nothing (151 to 155 us).
+constexpr uint32_t M_LEAST = 0x38000000u, V_LEAST = 0x30100000u;      // patterns of the first moment's (unused) code 0 and the second's code 1
 
-__device__ __forceinline__ float decode_m(uint32_t c) {
-  const uint32_t mag = c & 0x7Fu;
-  const float y = mag ? __uint_as_float((mag + M_BASE) << 20) : 0.f;
-  return c & 0x80u ? -y : y;
+__device__ __forceinline__ float2 halves(uint32_t u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u)); }
+// u holds two bf16; those not above `least` become 0
+__device__ __forceinline__ uint32_t drop_least(uint32_t u, uint32_t least) {
+  const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&u), l = *reinterpret_cast<const __nv_bfloat162*>(&least);
+  const __nv_bfloat162 r = __hmul2(v, __hgt2(v, l));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ float decode_v(uint32_t c) { return c ? __uint_as_float((c + V_BASE) << 20) : 0.f; }
+// Codes 0, 1 (PAIR 0) or 2, 3 (PAIR 1) of a word
+template <int PAIR>
+__device__ __forceinline__ float2 decode_m(uint32_t codes) {
+  const uint32_t c = __byte_perm(codes, 0u, PAIR ? 0x4342 : 0x4140);                  // one code in each half
+  const uint32_t mag = drop_least((c & 0x007F007Fu) * 16u + 0x38003800u, 0x38003800u);
+  return halves(mag | ((c * 256u) & 0x80008000u));
+}
+template <int PAIR>
+__device__ __forceinline__ float2 decode_v(uint32_t codes) {
+  return halves(drop_least(__byte_perm(codes, 0u, PAIR ? 0x4342 : 0x4140) * 16u + 0x30003000u, 0x30003000u));
+}
+template <bool SIGNED>
+__device__ __forceinline__ void decode8(uint2 codes, float scale, float2 (&x)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t c = i < 2 ? codes.x : codes.y;
+    if (SIGNED) x[i] = i & 1 ? decode_m<1>(c) : decode_m<0>(c); else x[i] = i & 1 ? decode_v<1>(c) : decode_v<0>(c);
+    x[i] = mul2(x[i], both(scale));
+  }
+}
 
-// r8: 8 random bits.  Half of the last random place is added, so that the sum's truncation is right on average.
-__device__ __forceinline__ uint32_t encode_m(float y, uint32_t r8) {
-  const uint32_t bits = __float_as_uint(y), u = (bits & 0x7FFFFFFFu) + (r8 << 12) + 0x800u;
-  const int c = min(max(static_cast<int>(u >> 20) - static_cast<int>(M_BASE), 0), 127);
-  return c ? (static_cast<uint32_t>(c) | ((bits >> 24) & 0x80u)) : 0u;
+// The highest bytes of four words
+__device__ __forceinline__ uint32_t high_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
 }
-__device__ __forceinline__ uint32_t encode_v(float y, uint32_t r8) {
-  const uint32_t u = __float_as_uint(y) + (r8 << 12) + 0x800u;
-  const int c = min(max(static_cast<int>(u >> 20) - static_cast<int>(V_BASE), 1), 255);
-  return y > 0.f ? static_cast<uint32_t>(c) : 0u;
+// With 8 random bits r, code = floor((pattern + r 2^12 + 2^11) / 2^20) - base: half of the last random place is added, so that cutting is right
+// on average.  All of it is taken times 16, which puts the code into the highest byte; nothing rounds up beyond the highest code, the
+// pattern of which is 0xFF7FF short of the next one's.  rnd: bits 16-23 for the first, 24-31 for the second moment.
+__device__ __forceinline__ uint32_t encode4_m(const float (&x)[4], float inv, const uint32_t (&rnd)[4]) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u[i] = max(__float_as_uint(fabsf(x[i]) * inv), M_LEAST) * 16u + __byte_perm(rnd[i], 0x00008000u, 0x6254);
+  const uint32_t mag = high_bytes(u[0], u[1], u[2], u[3]) & 0x7F7F7F7Fu;              // (the base leaves 0x80 in each)
+  const uint32_t sign = high_bytes(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  return mag | ((mag + 0x7F7F7F7Fu) & sign & 0x80808080u);                            // no sign for code 0
+}
+__device__ __forceinline__ uint32_t encode4_v(const float (&x)[4], float inv, const uint32_t (&rnd)[4]) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)      // less 1, which makes 0 the largest number: it stays 0 where the other small ones become code 1
+    u[i] = __viaddmax_u32(__float_as_uint(x[i] * inv), 0xFFFFFFFFu, V_LEAST - 1u) * 16u + __byte_perm(rnd[i], 0x00008010u, 0x6354);
+  return high_bytes(u[0], u[1], u[2], u[3]);
+}
+template <bool SIGNED>
+__device__ __forceinline__ uint2 encode8(const float (&x)[8], float inv, const uint32_t (&rnd)[8]) {
+  const float a[4] = {x[0], x[1], x[2], x[3]}, b[4] = {x[4], x[5], x[6], x[7]};
+  const uint32_t r[4] = {rnd[0], rnd[1], rnd[2], rnd[3]}, q[4] = {rnd[4], rnd[5], rnd[6], rnd[7]};
+  return SIGNED ? make_uint2(encode4_m(a, inv, r), encode4_m(b, inv, q)) : make_uint2(encode4_v(a, inv, r), encode4_v(b, inv, q));
 }
 // Scale of a block and what its values are multiplied with.  Where a value is inf or NaN the scale is NaN, and the block reads as NaN.
 __device__ __forceinline__ float block_scale(float top, float& inv) {
   if (!(top < __uint_as_float(0x7F800000u))) { inv = 0.f; return __uint_as_float(0x7FC00000u); }
   const bool fine = top >= CODE_TINY;
-  inv = fine ? CODE_TOP / top : 0.f;
+  inv = fine ? inverse_of(top * 0.0625f) * (CODE_TOP * 0.0625f) : 0.f;      // (2^-4: the inverse of the largest numbers would be subnormal)
   return fine ? top * (1.0f / CODE_TOP) : 0.f;
 }
-// Largest pattern over a warp; patterns of non-negative floats compare as the floats do, inf and NaN above all.
+// Largest magnitude over a warp; patterns of non-negative floats compare as the floats do, inf and NaN above all.
+template <bool SIGNED>
 __device__ __forceinline__ float warp_top(const float (&x)[8]) {
-  uint32_t top = 0u;
+  uint32_t u[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-  return __uint_as_float(__reduce_max_sync(0xffffffffu, top));
+  for (int i = 0; i < 8; ++i) u[i] = SIGNED ? __float_as_uint(x[i]) * 2u : __float_as_uint(x[i]);
+  const uint32_t top = max(__vimax3_u32(u[0], u[1], u[2]), max(__vimax3_u32(u[3], u[4], u[5]), max(u[6], u[7])));
+  const uint32_t t = __reduce_max_sync(0xffffffffu, top);
+  return __uint_as_float(SIGNED ? t >> 1 : t);
 }
 
 struct AdamArgs {
@@ -166,55 +262,79 @@ __global__ void __launch_bounds__(ADAM_THREADS) adamw_kernel(const __grid_consta
     if (!(norm < __uint_as_float(0x7F800000u))) return;       // a gradient is not finite: nothing is changed
     scale *= fminf(1.f, a.max_norm / (norm + 1e-6f));
   }
-  const int lane = threadIdx.x & 31, blocks = tab.first[tab.count];
-  const int warps = gridDim.x * (ADAM_THREADS / 32);
-  int t = 0;
-  for (int b = blockIdx.x * (ADAM_THREADS / 32) + (threadIdx.x >> 5); b < blocks; b += warps) {
+  const int lane = threadIdx.x & 31;
+  const int blocks = tab.first[tab.count], step = gridDim.x * ADAM_WARPS;
+  int b = blockIdx.x * ADAM_WARPS + (threadIdx.x >> 5), t = tensor_of(tab, b);
+  for (; b < blocks; b += step) {
     while (tab.first[t + 1] <= b) ++t;
     if (tab.g[t] == nullptr) continue;
-    const int64_t at = static_cast<int64_t>(b - tab.first[t]) * ADAM_BLOCK + lane * 8, left = tab.n[t] - at;
-    P* p = static_cast<P*>(tab.p[t]) + at;
-    const G* gp = static_cast<const G*>(tab.g[t]) + at;
-    const bool vec_p = left >= 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0, vec_g = left >= 8 && (reinterpret_cast<uintptr_t>(gp) & 15) == 0;
+    const int64_t at = static_cast<int64_t>(b - tab.first[t]) * ADAM_BLOCK, size = tab.n[t], left = size - at - lane * 8;
+    P* p = static_cast<P*>(tab.p[t]) + at + lane * 8;
+    const G* gp = static_cast<const G*>(tab.g[t]) + at + lane * 8;
+    const bool whole = size - at >= ADAM_BLOCK && on16(tab.p[t]) && on16(tab.g[t]);        // for the warp: 16 bytes at a time
     const int64_t e = static_cast<int64_t>(b) * ADAM_BLOCK + lane * 8;
-    float w[8], g[8], m[8], v[8];
-    load_lane(p, vec_p, left, w);
-    load_lane(gp, vec_g, left, g);
+    Lane8<P> wl;
+    Lane8<G> gl;
+    Lane8<float> ml, vl;
+    uint2 mc, vc;
+    float sm, sv;
     if (BITS == 32) {
-      load8(static_cast<const float*>(m_all) + e, m);
-      load8(static_cast<const float*>(v_all) + e, v);
+      ml.load(static_cast<const float*>(m_all) + e);
+      vl.load(static_cast<const float*>(v_all) + e);
     } else {
-      const uint2 mc = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(m_all) + e), vc = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(v_all) + e);
-      const float sm = ms[b], sv = vs[b];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        m[i] = decode_m(((i < 4 ? mc.x : mc.y) >> (8 * (i & 3))) & 0xFFu) * sm;
-        v[i] = decode_v(((i < 4 ? vc.x : vc.y) >> (8 * (i & 3))) & 0xFFu) * sv;
-      }
+      mc = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(m_all) + e);
+      vc = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(v_all) + e);
+      sm = ms[b];
+      sv = vs[b];
     }
-    if (left < 8) {                       // what pads a tensor's last block counts for nothing, whatever the buffer held
-#pragma unroll
-      for (int i = 0; i < 8; ++i) if (i >= left) m[i] = v[i] = 0.f;
-    }
+    if (whole) { wl.load(p); gl.load(gp); } else { wl.load_part(p, left); gl.load_part(gp, left); }
     uint32_t rnd[8], out[8];
     const bool sr = sizeof(P) == 2 && a.sr;
-    if (BITS == 8 || sr) {
+    if (BITS == 8 || sr) {                // while the loads are on their way
       const uint64_t i = (static_cast<uint64_t>(block0 + b) * ADAM_BLOCK + lane * 8) / 4;      // even
       const uint4 r0 = philox4x32_7(static_cast<uint32_t>(i), static_cast<uint32_t>(i >> 32), a.stream, 1u, a.seed, a.step);
       const uint4 r1 = philox4x32_7(static_cast<uint32_t>(i) + 1u, static_cast<uint32_t>(i >> 32), a.stream, 1u, a.seed, a.step);
       rnd[0] = r0.x; rnd[1] = r0.y; rnd[2] = r0.z; rnd[3] = r0.w; rnd[4] = r1.x; rnd[5] = r1.y; rnd[6] = r1.z; rnd[7] = r1.w;
     }
+    float2 w[4], g[4], m2[4], v2[4];
+    if (BITS == 32) { ml.get(m2); vl.get(v2); } else { decode8<true>(mc, sm, m2); decode8<false>(vc, sv, v2); }
+    if (left < 8) {                       // what pads a tensor's last block counts for nothing, whatever the buffer held
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float gi = g[i] * scale;
-      m[i] = fmaf(a.b1, m[i], a.c1 * gi);
-      v[i] = fmaf(a.b2, v[i], a.c2 * gi * gi);
-      const float wn = fmaf(-a.rate, __fdividef(m[i], fmaf(root_of(v[i]), a.root, a.eps)), w[i] * a.decay);
-      if (sizeof(P) == 4) out[i] = __float_as_uint(wn);
-      // (a NaN's pattern is 0x7FFFFFFF: with bits added it would read as -0)
-      else out[i] = sr ? __float_as_uint(wn) + (wn == wn ? rnd[i] & 0xFFFFu : 0u) : static_cast<uint32_t>(rn_bf16_bits(wn)) << 16;
+      for (int i = 0; i < 4; ++i) {
+        if (2 * i >= left) m2[i].x = v2[i].x = 0.f;
+        if (2 * i + 1 >= left) m2[i].y = v2[i].y = 0.f;
+      }
     }
-    store_lane(p, vec_p, left, out);
+    wl.get(w);
+    gl.get(g);
+    float m[8], v[8];
+    float2 bad = both(0.f);               // becomes NaN with any weight that is inf or NaN
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 gi = mul2(g[i], both(scale));
+      const float2 mi = fma2(both(a.b1), m2[i], mul2(both(a.c1), gi)), vi = fma2(both(a.b2), v2[i], mul2(mul2(both(a.c2), gi), gi));
+      const float2 den = fma2(make_float2(root_of(vi.x), root_of(vi.y)), both(a.root), both(a.eps));
+      const float2 q = mul2(mi, make_float2(inverse_of(den.x), inverse_of(den.y)));
+      const float2 wn = fma2(both(-a.rate), q, mul2(w[i], both(a.decay)));
+      m[2 * i] = mi.x; m[2 * i + 1] = mi.y; v[2 * i] = vi.x; v[2 * i + 1] = vi.y;
+      out[2 * i] = __float_as_uint(wn.x); out[2 * i + 1] = __float_as_uint(wn.y);
+      if (sizeof(P) == 2) bad = fma2(wn, both(0.f), bad);
+    }
+    if (sizeof(P) == 2) {
+      if (sr) {
+        // a NaN is 0x7FFFFFFF here: it must not run over into the sign
+        if (bad.x + bad.y != 0.f) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) rnd[i] = (out[i] & 0x7FFFFFFFu) > 0x7F800000u ? rnd[i] & 0xFFFF0000u : rnd[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) out[i] += rnd[i] & 0xFFFFu;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) out[i] = static_cast<uint32_t>(rn_bf16_bits(__uint_as_float(out[i]))) << 16;
+      }
+    }
+    store_lane(p, whole, left, out);
     if (BITS == 32) {
       float* mp = static_cast<float*>(m_all) + e;
       float* vp = static_cast<float*>(v_all) + e;
@@ -224,44 +344,68 @@ __global__ void __launch_bounds__(ADAM_THREADS) adamw_kernel(const __grid_consta
       *reinterpret_cast<float4*>(vp + 4) = make_float4(v[4], v[5], v[6], v[7]);
     } else {
       float im, iv;
-      const float sm = block_scale(warp_top(m), im), sv = block_scale(warp_top(v), iv);
-      uint32_t mc[2] = {0u, 0u}, vc[2] = {0u, 0u};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        mc[i >> 2] |= encode_m(m[i] * im, (rnd[i] >> 16) & 0xFFu) << (8 * (i & 3));
-        vc[i >> 2] |= encode_v(v[i] * iv, rnd[i] >> 24) << (8 * (i & 3));
-      }
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(m_all) + e) = make_uint2(mc[0], mc[1]);
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(v_all) + e) = make_uint2(vc[0], vc[1]);
+      const float sm = block_scale(warp_top<true>(m), im), sv = block_scale(warp_top<false>(v), iv);
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(m_all) + e) = encode8<true>(m, im, rnd);
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(v_all) + e) = encode8<false>(v, iv, rnd);
       if (lane == 0) { ms[b] = sm; vs[b] = sv; }
     }
   }
 }
 
 // ---------------------------------------------------------------- 2-norm of the gradients
-// Sums of squares of the launch's blocks, one per thread block, into partial[part0 + blockIdx.x].
+// Sums of squares of the launch's blocks, one per thread block, into partial[part0 + blockIdx.x].  A warp has the loads of 4 blocks on their
+// way at once: 56 M bf16 gradients 35 us with one, 27 with 4.
 template <int N>
 __global__ void __launch_bounds__(ADAM_THREADS) grad_squares_kernel(const __grid_constant__ TensorTable<N> tab, float* __restrict__ partial, int part0) {
   __shared__ float sums[ADAM_THREADS / 32];
-  const int lane = threadIdx.x & 31, blocks = tab.first[tab.count];
-  const int warps = gridDim.x * (ADAM_THREADS / 32);
-  float s = 0.f;
-  int t = 0;
-  for (int b = blockIdx.x * (ADAM_THREADS / 32) + (threadIdx.x >> 5); b < blocks; b += warps) {
-    while (tab.first[t + 1] <= b) ++t;
-    const int64_t at = static_cast<int64_t>(b - tab.first[t]) * ADAM_BLOCK + lane * 8, left = tab.n[t] - at;
-    float g[8];
-    const char* gp = static_cast<const char*>(tab.g[t]);
-    if (reinterpret_cast<uintptr_t>(tab.p[t]) == HASTE_BF16) {
-      gp += 2 * at;
-      load_lane(reinterpret_cast<const __nv_bfloat16*>(gp), left >= 8 && (reinterpret_cast<uintptr_t>(gp) & 15) == 0, left, g);
-    } else {
-      gp += 4 * at;
-      load_lane(reinterpret_cast<const float*>(gp), left >= 8 && (reinterpret_cast<uintptr_t>(gp) & 15) == 0, left, g);
+  const int lane = threadIdx.x & 31;
+  float2 acc[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) acc[k] = both(0.f);
+  // a share of the blocks of its own for each thread block: a warp stays with a tensor, which it looks up once
+  const int64_t blocks = tab.first[tab.count];
+  const int lo = static_cast<int>(blocks * blockIdx.x / gridDim.x), hi = static_cast<int>(blocks * (blockIdx.x + 1) / gridDim.x);
+  int t = tensor_of(tab, lo) - 1, next = 0, first = 0, type = HASTE_BF16;
+  int64_t size = 0;
+  const char* from = nullptr;
+  for (int b0 = lo + (threadIdx.x >> 5); b0 < hi; b0 += ADAM_WARPS * AHEAD) {
+    Lane8<float> g[AHEAD];            // fp32, or in the first word bf16
+    bool half[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int b = b0 + k * ADAM_WARPS;
+      g[k].clear();
+      half[k] = false;
+      if (b >= hi) continue;
+      if (b >= next) {
+        do ++t; while (tab.first[t + 1] <= b);
+        first = tab.first[t]; next = tab.first[t + 1]; size = tab.n[t]; from = static_cast<const char*>(tab.g[t]);
+        type = static_cast<int>(reinterpret_cast<uintptr_t>(tab.p[t]));
+      }
+      const int64_t at = static_cast<int64_t>(b - first) * ADAM_BLOCK;
+      const bool whole = size - at >= ADAM_BLOCK && on16(from);
+      half[k] = type == HASTE_BF16;
+      if (half[k]) {
+        const __nv_bfloat16* gp = reinterpret_cast<const __nv_bfloat16*>(from) + at + lane * 8;
+        Lane8<__nv_bfloat16> h;
+        if (whole) h.load(gp); else h.load_part(gp, size - at - lane * 8);
+        g[k].q[0] = h.q[0];
+      } else {
+        const float* gp = reinterpret_cast<const float*>(from) + at + lane * 8;
+        if (whole) g[k].load(gp); else g[k].load_part(gp, size - at - lane * 8);
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s = fmaf(g[i], g[i], s);
+    for (int k = 0; k < AHEAD; ++k) {
+      float2 f[4];
+      if (half[k]) { Lane8<__nv_bfloat16> h; h.q[0] = g[k].q[0]; h.get(f); } else g[k].get(f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[k] = fma2(f[i], f[i], acc[k]);
+    }
   }
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) s += acc[k].x + acc[k].y;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane == 0) sums[threadIdx.x >> 5] = s;
@@ -295,41 +439,63 @@ __global__ void __launch_bounds__(ADAM_THREADS) quantize_kernel(const float* __r
   for (int64_t b = static_cast<int64_t>(blockIdx.x) * (ADAM_THREADS / 32) + (threadIdx.x >> 5); b < blocks; b += warps) {
     const int64_t e = b * ADAM_BLOCK + lane * 8;
     float v[8], inv;
-    load8(x + e, v);
-    const float s = block_scale(warp_top(v), inv);
-    uint32_t c[2] = {0u, 0u};
+    Lane8<float> l;
+    float2 f[4];
+    l.load(x + e);
+    l.get(f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i >> 2] |= (SIGNED ? encode_m(v[i] * inv, 127u) : encode_v(v[i] * inv, 127u)) << (8 * (i & 3));
-    *reinterpret_cast<uint2*>(codes + e) = make_uint2(c[0], c[1]);
+    for (int i = 0; i < 4; ++i) { v[2 * i] = f[i].x; v[2 * i + 1] = f[i].y; }
+    const float s = block_scale(warp_top<SIGNED>(v), inv);
+    constexpr uint32_t half = 0x7F7F0000u;
+    const uint32_t rnd[8] = {half, half, half, half, half, half, half, half};
+    *reinterpret_cast<uint2*>(codes + e) = encode8<SIGNED>(v, inv, rnd);
     if (lane == 0) scales[b] = s;
   }
 }
 
+// A lane takes 8 codes at a time, so that a warp stores whole lines, and 4 such pieces of them at once.
 template <class O, bool SIGNED>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales, O* __restrict__ out, int64_t n8) {
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n8; i += stride) {
-    const uint2 c = *reinterpret_cast<const uint2*>(codes + i * 8);
-    const float s = scales[i / (ADAM_BLOCK / 8)];
-    uint32_t u[8];
+  constexpr int PIECES = 4;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * 256 * PIECES + threadIdx.x; base < n8; base += static_cast<int64_t>(gridDim.x) * 256 * PIECES) {
+    uint2 c[PIECES];
+    float s[PIECES];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint32_t code = ((k < 4 ? c.x : c.y) >> (8 * (k & 3))) & 0xFFu;
-      const float x = (SIGNED ? decode_m(code) : decode_v(code)) * s;
-      u[k] = sizeof(O) == 4 ? __float_as_uint(x) : static_cast<uint32_t>(rn_bf16_bits(x)) << 16;
+    for (int k = 0; k < PIECES; ++k) {
+      const int64_t i = base + k * 256;
+      c[k] = i < n8 ? __ldcs(reinterpret_cast<const uint2*>(codes + i * 8)) : make_uint2(0u, 0u);
+      s[k] = i < n8 ? __ldg(scales + i / (ADAM_BLOCK / 8)) : 0.f;
     }
-    store_lane(out + i * 8, true, 8, u);
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+      const int64_t i = base + k * 256;
+      float2 x[4];
+      decode8<SIGNED>(c[k], s[k], x);
+      uint32_t u[8];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        u[2 * q] = sizeof(O) == 4 ? __float_as_uint(x[q].x) : static_cast<uint32_t>(rn_bf16_bits(x[q].x)) << 16;
+        u[2 * q + 1] = sizeof(O) == 4 ? __float_as_uint(x[q].y) : static_cast<uint32_t>(rn_bf16_bits(x[q].y)) << 16;
+      }
+      if (i < n8) store_lane(out + i * 8, true, 8, u);
+    }
   }
 }
 
 // ================================================================ launchers
-static int adam_grid(int64_t blocks) {
+// Thread blocks for a number of blocks of elements: one for 8 of them, at most `per_sm` times the SMs.
+static int adam_grid(int64_t blocks, int per_sm) {
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int64_t want = (blocks + ADAM_THREADS / 32 - 1) / (ADAM_THREADS / 32);
-  return static_cast<int>(want < sms * 4 ? want : sms * 4);
+  const int64_t want = (blocks + ADAM_WARPS - 1) / ADAM_WARPS, most = static_cast<int64_t>(sms) * per_sm;
+  return static_cast<int>(want < most ? want : most);
 }
+
+// The 32-bit step is bound by memory, which is fastest when all of the GPU works on one short stretch of the buffers at a time: many
+// thread blocks that take a few blocks of elements each and are started in order (56 M weights, fp32: 272 us with 4 a SM, 228 with 64;
+// bf16: 214 and 180).  The 8-bit step is bound by its instructions and pays for starting up: 151 us with 4, 191 with 64.
+constexpr int ADAM_PER_SM_32 = 64, ADAM_PER_SM_8 = 4;
 
 constexpr int TABLE_SMALL = 112, TABLE_LARGE = 1024;      // 3.2 KB and 28.7 KB of kernel parameters (32,764 bytes at most)
 constexpr int64_t MAX_BLOCKS = (int64_t(1) << 31) - 1 - 65536;
@@ -375,7 +541,7 @@ static int adamw_typed(const AdamWCall& c, const AdamArgs& a, cudaStream_t st) {
     char* v = static_cast<char*>(c.exp_avg_sq) + block0 * ADAM_BLOCK * (BITS / 8);
     float* ms = BITS == 8 ? c.avg_scale + block0 : nullptr;
     float* vs = BITS == 8 ? c.sq_scale + block0 : nullptr;
-    const int grid = adam_grid(blocks);
+    const int grid = adam_grid(blocks, BITS == 32 ? ADAM_PER_SM_32 : ADAM_PER_SM_8);
     if (tab.count <= TABLE_SMALL) adamw_kernel<P, G, BITS, TABLE_SMALL><<<grid, ADAM_THREADS, 0, st>>>(small_table(tab), m, ms, v, vs, block0, a);
     else adamw_kernel<P, G, BITS, TABLE_LARGE><<<grid, ADAM_THREADS, 0, st>>>(tab, m, ms, v, vs, block0, a);
     return check_launch("adamw_kernel");
@@ -410,7 +576,7 @@ int launch_grad_norm(const void* const* grads, const int32_t* types, const int64
   const int64_t cap = HASTE_GRAD_NORM_PARTIALS / 2 / tables;
   int parts = 0;
   const int rc = for_each_table(nullptr, types, grads, sizes, count, [&](const TensorTable<TABLE_LARGE>& tab, int64_t, int64_t blocks) {
-    const int grid = static_cast<int>(imin64(adam_grid(blocks), cap));
+    const int grid = static_cast<int>(imin64(adam_grid(blocks, 4), cap));
     if (grid < 1 || parts + grid > HASTE_GRAD_NORM_PARTIALS) return fail(HASTE_ERR_TOO_LARGE, "haste_grad_norm: too many tensors for one call");
     if (tab.count <= TABLE_SMALL) grad_squares_kernel<TABLE_SMALL><<<grid, ADAM_THREADS, 0, st>>>(small_table(tab), partial, parts);
     else grad_squares_kernel<TABLE_LARGE><<<grid, ADAM_THREADS, 0, st>>>(tab, partial, parts);
@@ -424,7 +590,7 @@ int launch_grad_norm(const void* const* grads, const int32_t* types, const int64
 
 int launch_quantize(const float* x, uint8_t* codes, float* scales, int64_t n, int is_signed, cudaStream_t st) {
   if (n == 0) return HASTE_OK;
-  const int grid = adam_grid(n / ADAM_BLOCK);
+  const int grid = adam_grid(n / ADAM_BLOCK, 4);
   if (is_signed) quantize_kernel<true><<<grid, ADAM_THREADS, 0, st>>>(x, codes, scales, n / ADAM_BLOCK);
   else quantize_kernel<false><<<grid, ADAM_THREADS, 0, st>>>(x, codes, scales, n / ADAM_BLOCK);
   return check_launch("quantize_kernel");
@@ -432,7 +598,7 @@ int launch_quantize(const float* x, uint8_t* codes, float* scales, int64_t n, in
 
 int launch_dequantize(const uint8_t* codes, const float* scales, void* out, int64_t n, int is_signed, int type, cudaStream_t st) {
   if (n == 0) return HASTE_OK;
-  const int64_t n8 = n / 8, want = (n8 + 255) / 256;
+  const int64_t n8 = n / 8, want = (n8 + 1023) / 1024;
   const unsigned grid = static_cast<unsigned>(want < 148 * 16 ? want : 148 * 16);
   if (type == HASTE_BF16) {
     if (is_signed) dequantize_kernel<__nv_bfloat16, true><<<grid, 256, 0, st>>>(codes, scales, (__nv_bfloat16*)out, n8);

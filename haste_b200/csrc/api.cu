@@ -555,7 +555,7 @@ int haste_adamw_step(void* const* params, const void* const* grads, const int64_
   if (bits != 8 && bits != 32) return fail(HASTE_ERR_UNSUPPORTED, "%s: moments of %d bits (8 or 32 are supported)", who, bits);
   if (!(lr >= 0.0 && is_finite(lr) && weight_decay >= 0.0 && is_finite(weight_decay))) return fail(HASTE_ERR_BAD_ARG, "%s: lr and weight_decay must not be negative", who);
   if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) return fail(HASTE_ERR_BAD_ARG, "%s: betas must be in [0, 1)", who);
-  if (!(eps > 0.0 && is_finite(eps))) return fail(HASTE_ERR_BAD_ARG, "%s: eps must be positive", who);
+  if (!(eps >= 0x1p-126 && is_finite(eps))) return fail(HASTE_ERR_BAD_ARG, "%s: eps must be positive (and at least 2^-126)", who);
   if (step < 1) return fail(HASTE_ERR_BAD_ARG, "%s: step=%lld (the first step is 1)", who, (long long)step);
   if (!is_finite(grad_scale)) return fail(HASTE_ERR_BAD_ARG, "%s: grad_scale must be finite", who);
   if (norm != nullptr && !(max_norm > 0.f)) return fail(HASTE_ERR_BAD_ARG, "%s: max_norm must be positive", who);
