@@ -24,6 +24,7 @@
 // 24-31 the second.
 #include "common.cuh"
 
+#include <cooperative_groups.h>
 #include <math.h>
 #include "launchers.h"
 
@@ -34,6 +35,8 @@ constexpr int ADAM_THREADS = 256, ADAM_WARPS = ADAM_THREADS / 32;
 constexpr int AHEAD = 4;               // blocks of gradients that a warp of the norm has on their way, and the most of a turn
 constexpr float CODE_TOP = 1.875f;
 constexpr float CODE_TINY = 0x1p-120f; // a block whose largest value is below holds zeros (1.875 / it is finite)
+
+constexpr int TABLE_SMALL = 112, TABLE_LARGE = 1024;      // 3.2 KB and 28.7 KB of kernel parameters (32,764 bytes at most)
 
 // The tensors of one launch, as a kernel parameter.  first[i]: first block of tensor i among the launch's blocks.
 template <int N>
@@ -353,27 +356,25 @@ __global__ void __launch_bounds__(ADAM_THREADS) adamw_kernel(const __grid_consta
 }
 
 // ---------------------------------------------------------------- 2-norm of the gradients
-// Sums of squares of the launch's blocks, one per thread block, into partial[part0 + blockIdx.x].  A warp has the loads of 4 blocks on their
-// way at once: 56 M bf16 gradients 35 us with one, 27 with 4.
-template <int N>
-__global__ void __launch_bounds__(ADAM_THREADS) grad_squares_kernel(const __grid_constant__ TensorTable<N> tab, float* __restrict__ partial, int part0) {
-  __shared__ float sums[ADAM_THREADS / 32];
+// Sum of squares of blocks lo .. hi - 1 of the launch over THREADS threads, in thread 0.  A warp has the loads of 4 blocks on their way at
+// once (56 M bf16 gradients 35 us with one, 27 with 4), and stays with a tensor, which it looks up once (30 us where each block was looked up).
+template <int THREADS, int N>
+__device__ __forceinline__ float sum_of_squares(const TensorTable<N>& tab, int lo, int hi) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ float sums[WARPS];
   const int lane = threadIdx.x & 31;
   float2 acc[AHEAD];
 #pragma unroll
   for (int k = 0; k < AHEAD; ++k) acc[k] = both(0.f);
-  // a share of the blocks of its own for each thread block: a warp stays with a tensor, which it looks up once
-  const int64_t blocks = tab.first[tab.count];
-  const int lo = static_cast<int>(blocks * blockIdx.x / gridDim.x), hi = static_cast<int>(blocks * (blockIdx.x + 1) / gridDim.x);
   int t = tensor_of(tab, lo) - 1, next = 0, first = 0, type = HASTE_BF16;
   int64_t size = 0;
   const char* from = nullptr;
-  for (int b0 = lo + (threadIdx.x >> 5); b0 < hi; b0 += ADAM_WARPS * AHEAD) {
+  for (int b0 = lo + (threadIdx.x >> 5); b0 < hi; b0 += WARPS * AHEAD) {
     Lane8<float> g[AHEAD];            // fp32, or in the first word bf16
     bool half[AHEAD];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
-      const int b = b0 + k * ADAM_WARPS;
+      const int b = b0 + k * WARPS;
       g[k].clear();
       half[k] = false;
       if (b >= hi) continue;
@@ -410,9 +411,35 @@ __global__ void __launch_bounds__(ADAM_THREADS) grad_squares_kernel(const __grid
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane == 0) sums[threadIdx.x >> 5] = s;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < ADAM_THREADS / 32; ++i) s += sums[i];
-    partial[part0 + blockIdx.x] = s;
+  if (threadIdx.x == 0)
+    for (int i = 1; i < WARPS; ++i) s += sums[i];
+  return s;
+}
+
+// One sum per thread block, each of which has a share of the blocks of its own, into partial[part0 + blockIdx.x].
+template <int N>
+__global__ void __launch_bounds__(ADAM_THREADS) grad_squares_kernel(const __grid_constant__ TensorTable<N> tab, float* __restrict__ partial, int part0) {
+  const int64_t blocks = tab.first[tab.count];
+  const float s = sum_of_squares<ADAM_THREADS>(tab, static_cast<int>(blocks * blockIdx.x / gridDim.x), static_cast<int>(blocks * (blockIdx.x + 1) / gridDim.x));
+  if (threadIdx.x == 0) partial[part0 + blockIdx.x] = s;
+}
+
+// Up to 2^20 elements: one cluster, whose blocks hand their sums to the first one, and no second launch (0.4 M elements, calls back to back:
+// 12.0 us instead of 14.2; the launch costs more than the other SMs would bring).
+constexpr int NORM_CLUSTER = 8, NORM_THREADS = 1024;
+constexpr int64_t NORM_SMALL_BLOCKS = 4096;
+__global__ void __cluster_dims__(NORM_CLUSTER, 1, 1) __launch_bounds__(NORM_THREADS) grad_norm_small_kernel(const __grid_constant__ TensorTable<TABLE_SMALL> tab,
+                                                                                                           float grad_scale, float* __restrict__ norm) {
+  __shared__ float sums[NORM_CLUSTER];
+  auto cluster = cooperative_groups::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank()), blocks = tab.first[tab.count];
+  const float s = sum_of_squares<NORM_THREADS>(tab, blocks * rank / NORM_CLUSTER, blocks * (rank + 1) / NORM_CLUSTER);
+  if (threadIdx.x == 0) *cluster.map_shared_rank(&sums[rank], 0) = s;
+  cluster.sync();
+  if (rank == 0 && threadIdx.x == 0) {
+    double total = 0.0;
+    for (int i = 0; i < NORM_CLUSTER; ++i) total += sums[i];
+    *norm = static_cast<float>(sqrt(total) * fabsf(grad_scale));
   }
 }
 
@@ -485,10 +512,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
 // ================================================================ launchers
 // Thread blocks for a number of blocks of elements: one for 8 of them, at most `per_sm` times the SMs.
 static int adam_grid(int64_t blocks, int per_sm) {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int64_t want = (blocks + ADAM_WARPS - 1) / ADAM_WARPS, most = static_cast<int64_t>(sms) * per_sm;
+  const int64_t want = (blocks + ADAM_WARPS - 1) / ADAM_WARPS, most = static_cast<int64_t>(sm_count()) * per_sm;
   return static_cast<int>(want < most ? want : most);
 }
 
@@ -497,7 +521,6 @@ static int adam_grid(int64_t blocks, int per_sm) {
 // bf16: 214 and 180).  The 8-bit step is bound by its instructions and pays for starting up: 151 us with 4, 191 with 64.
 constexpr int ADAM_PER_SM_32 = 64, ADAM_PER_SM_8 = 4;
 
-constexpr int TABLE_SMALL = 112, TABLE_LARGE = 1024;      // 3.2 KB and 28.7 KB of kernel parameters (32,764 bytes at most)
 constexpr int64_t MAX_BLOCKS = (int64_t(1) << 31) - 1 - 65536;
 
 // Calls f(table, first block of the part) for consecutive parts of the tensors; a tensor with more than 2^31 blocks is refused before.
@@ -575,7 +598,13 @@ int launch_grad_norm(const void* const* grads, const int32_t* types, const int64
   const int64_t tables = count / TABLE_LARGE + 1;           // or one more for every 2^31 blocks, whose grids are as large as they get
   const int64_t cap = HASTE_GRAD_NORM_PARTIALS / 2 / tables;
   int parts = 0;
+  bool done = false;
   const int rc = for_each_table(nullptr, types, grads, sizes, count, [&](const TensorTable<TABLE_LARGE>& tab, int64_t, int64_t blocks) {
+    if (count <= TABLE_SMALL && blocks <= NORM_SMALL_BLOCKS) {            // (all of them: one table)
+      grad_norm_small_kernel<<<NORM_CLUSTER, NORM_THREADS, 0, st>>>(small_table(tab), grad_scale, norm);
+      done = true;
+      return check_launch("grad_norm_small_kernel");
+    }
     const int grid = static_cast<int>(imin64(adam_grid(blocks, 4), cap));
     if (grid < 1 || parts + grid > HASTE_GRAD_NORM_PARTIALS) return fail(HASTE_ERR_TOO_LARGE, "haste_grad_norm: too many tensors for one call");
     if (tab.count <= TABLE_SMALL) grad_squares_kernel<TABLE_SMALL><<<grid, ADAM_THREADS, 0, st>>>(small_table(tab), partial, parts);
@@ -583,7 +612,7 @@ int launch_grad_norm(const void* const* grads, const int32_t* types, const int64
     parts += grid;
     return check_launch("grad_squares_kernel");
   });
-  if (rc != HASTE_OK) return rc;
+  if (rc != HASTE_OK || done) return rc;
   grad_norm_finish_kernel<<<1, ADAM_THREADS, 0, st>>>(partial, parts, grad_scale, norm);
   return check_launch("grad_norm_finish_kernel");
 }
@@ -599,7 +628,7 @@ int launch_quantize(const float* x, uint8_t* codes, float* scales, int64_t n, in
 int launch_dequantize(const uint8_t* codes, const float* scales, void* out, int64_t n, int is_signed, int type, cudaStream_t st) {
   if (n == 0) return HASTE_OK;
   const int64_t n8 = n / 8, want = (n8 + 1023) / 1024;
-  const unsigned grid = static_cast<unsigned>(want < 148 * 16 ? want : 148 * 16);
+  const unsigned grid = static_cast<unsigned>(imin64(want, static_cast<int64_t>(sm_count()) * 16));
   if (type == HASTE_BF16) {
     if (is_signed) dequantize_kernel<__nv_bfloat16, true><<<grid, 256, 0, st>>>(codes, scales, (__nv_bfloat16*)out, n8);
     else dequantize_kernel<__nv_bfloat16, false><<<grid, 256, 0, st>>>(codes, scales, (__nv_bfloat16*)out, n8);

@@ -5,6 +5,8 @@
 #include "launchers.h"
 #include "runtime.h"
 
+#include <atomic>
+
 namespace haste {
 
 static thread_local char g_err[512] = "no error";
@@ -20,6 +22,18 @@ int check_launch(const char* what) {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
   return HASTE_OK;
+}
+int sm_count() {
+  static std::atomic<int> cached[64];              // of each device, 0 = not asked yet
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  int sms = cached[dev].load(std::memory_order_relaxed);
+  if (sms == 0) {
+    sms = 148;
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    cached[dev].store(sms, std::memory_order_relaxed);
+  }
+  return sms;
 }
 int validate_shape(const char* who, int64_t B, int64_t D, int64_t F, int64_t L, int64_t G) {
   if (B < 1 || D < 1 || L < 1) return fail(HASTE_ERR_BAD_ARG, "%s: B=%lld D=%lld L=%lld must be positive", who, (long long)B, (long long)D, (long long)L);

@@ -14,6 +14,7 @@ namespace haste {
 // ---------------------------------------------------------------- host error plumbing
 int fail(int code, const char* fmt, ...);
 int check_launch(const char* what);
+int sm_count();                  // of the current device; asked for once per device
 int validate_shape(const char* who, int64_t B, int64_t D, int64_t F, int64_t L, int64_t G);
 
 __host__ __device__ __forceinline__ int64_t imin64(int64_t a, int64_t b) { return a < b ? a : b; }

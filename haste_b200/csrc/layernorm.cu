@@ -643,18 +643,6 @@ __global__ void __launch_bounds__(MODE == BLOCK ? (VEC * NV > 16 ? 256 : 512) : 
 }
 
 // ================================================================ launchers
-static int sm_count() {
-  static std::atomic<int> cached[64];              // of each device, 0 = not asked yet
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  int sms = cached[dev].load(std::memory_order_relaxed);
-  if (sms == 0) {
-    sms = 148;
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    cached[dev].store(sms, std::memory_order_relaxed);
-  }
-  return sms;
-}
 static unsigned capped(int64_t want, int64_t cap) { return static_cast<unsigned>(want < cap ? want : cap); }
 
 // How a row of D elements is held: nv vectors of `vec` elements a thread, T threads (lanes of a warp, or a block), or `wide`.

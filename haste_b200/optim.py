@@ -56,13 +56,10 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step, lr=1e-3, betas=(0.9,
     quantized = isinstance(exp_avg, Quantized)
     if quantized != isinstance(exp_avg_sq, Quantized) or (quantized and not (exp_avg.signed and not exp_avg_sq.signed)):
         raise RuntimeError("both moments in 32 bits, or a signed and an unsigned Quantized")
-    if max_norm is not None and norm is None:
-        norm = grad_norm(grads, grad_scale)
     m, ms, v, vs = (*exp_avg[:2], *exp_avg_sq[:2]) if quantized else (exp_avg, None, exp_avg_sq, None)
-    _ffi.adamw_step(params, grads, m, ms, v, vs, 8 if quantized else 32, step=step, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, grad_scale=grad_scale,
-                    norm=norm if max_norm is not None else None, max_norm=max_norm or 0.0, seed=seed, stream_index=stream_index,
-                    flags=_lib.F_SR if stochastic_rounding else 0)
-    return norm
+    return _ffi.adamw_step(params, grads, m, ms, v, vs, 8 if quantized else 32, step=step, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                           grad_scale=grad_scale, norm=norm, max_norm=max_norm, seed=seed, stream_index=stream_index,
+                           flags=_lib.F_SR if stochastic_rounding else 0)
 
 
 class _Moments:
