@@ -521,9 +521,9 @@ static int adam_grid(int64_t blocks, int per_sm) {
 // bf16: 214 and 180).  The 8-bit step is bound by its instructions and pays for starting up: 151 us with 4, 191 with 64.
 constexpr int ADAM_PER_SM_32 = 64, ADAM_PER_SM_8 = 4;
 
-constexpr int64_t MAX_BLOCKS = (int64_t(1) << 31) - 1 - 65536;
+constexpr int64_t MAX_BLOCKS = int64_t(1) << 30;          // of a launch: a block's number and one more round of all warps fit 32 bits
 
-// Calls f(table, first block of the part) for consecutive parts of the tensors; a tensor with more than 2^31 blocks is refused before.
+// Calls f(table, first block of the part, its blocks) for consecutive parts of the tensors; a tensor of more than 2^30 blocks is refused before.
 template <class F>
 static int for_each_table(void* const* params, const int32_t* types, const void* const* grads, const int64_t* sizes, int64_t count, F&& f) {
   int64_t i = 0, block0 = 0;

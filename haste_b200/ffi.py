@@ -532,12 +532,16 @@ def _tensor_list(tensors, what):
         raise RuntimeError(f"{what} must be CUDA tensors on one device (this library has no CPU path)")
     if not all(map(_is_contiguous, tensors)):
         raise RuntimeError(f"{what} must be contiguous")
-    return devs.pop(), array.array("Q", map(_data_ptr, tensors))
+    return devs.pop(), array.array("Q", list(map(_data_ptr, tensors)))
+
+
+def _sizes(tensors):
+    return array.array("q", list(map(_numel, tensors)))
 
 
 def _present(tensors):
     """The list, without its None if it has any."""
-    return [t for t in tensors if t is not None] if any(t is None for t in tensors) else tensors
+    return [t for t in tensors if t is not None] if type(None) in set(map(type, tensors)) else tensors
 
 
 def _address(a):
@@ -563,7 +567,7 @@ def grad_norm(grads, grad_scale=1.0):
     if not types[1] <= _TYPES.keys():
         raise RuntimeError(f"gradients must be torch.bfloat16 or torch.float32, got {types[1]}")
     types = array.array("i", [types[0]]) * len(grads) if len(types[1]) == 1 else array.array("i", map(_TYPES.__getitem__, map(_dtype, grads)))
-    return _norm_of(dev, ptrs, types, array.array("q", map(_numel, grads)), grad_scale)
+    return _norm_of(dev, ptrs, types, _sizes(grads), grad_scale)
 
 
 def adamw_step(params, grads, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, bits, *, step, lr, betas, eps, weight_decay, grad_scale=1.0, norm=None,
@@ -579,16 +583,16 @@ def adamw_step(params, grads, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_sca
     gdev, gptrs = _tensor_list(there, "gradients")
     if dev != gdev:
         raise RuntimeError("parameters and gradients must be on one device")
-    sizes = array.array("q", map(_numel, params))
+    sizes = _sizes(params)
     all_gptrs, paired, paired_sizes = gptrs, params, sizes
     if there is not grads:
         paired = [p for p, g in zip(params, grads) if g is not None]
-        paired_sizes = array.array("q", map(_numel, paired))
+        paired_sizes = _sizes(paired)
         rest = iter(gptrs)
         all_gptrs = array.array("Q", [0 if g is None else next(rest) for g in grads])
     p_dtype, g_dtype = set(map(_dtype, params)), set(map(_dtype, there))
     dims = list(map(_dim, paired))
-    if (len(p_dtype) != 1 or len(g_dtype) != 1 or dims != list(map(_dim, there)) or paired_sizes != array.array("q", map(_numel, there))
+    if (len(p_dtype) != 1 or len(g_dtype) != 1 or dims != list(map(_dim, there)) or paired_sizes != _sizes(there)
             or (max(dims) > 1 and any(d > 1 and p.shape != g.shape for d, p, g in zip(dims, paired, there)))):
         raise RuntimeError("all parameters must have one type, all gradients one type, and every gradient its parameter's shape")
     p_type, g_type = _type_of(params[0], "parameters"), _type_of(there[0], "gradients")
@@ -610,7 +614,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_sca
     elif norm.get_device() != dev or norm.dtype != torch.float32 or norm.numel() != 1:
         raise RuntimeError("norm must be one fp32 value on the parameters' device")
     _call(dev, "adamw_step", lib.haste_adamw_step, _address(ptrs), _address(all_gptrs), _address(sizes), len(ptrs), exp_avg.data_ptr(), ms, exp_avg_sq.data_ptr(), vs,
-          moments, bits, p_type, g_type, lr, betas[0], betas[1], eps, weight_decay, step, grad_scale, max_norm or 0.0, _ptr(norm), seed & 0xFFFFFFFFFFFFFFFF,
+          moments, bits, p_type, g_type, float(lr), betas[0], betas[1], eps, weight_decay, step, grad_scale, max_norm or 0.0, _ptr(norm), seed & 0xFFFFFFFFFFFFFFFF,
           stream_index, flags)
     return norm
 

@@ -149,6 +149,8 @@ class AdamW(Optimizer):
     def load_state_dict(self, state_dict):
         """As ``Optimizer.load_state_dict``, but the moments keep their types (that one casts them to the parameters'), and a state dict of
         ``torch.optim.AdamW`` brings its step count along."""
+        if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
+            raise RuntimeError("state dicts with amsgrad or maximize are not supported")
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         for saved, group in zip(state_dict["param_groups"], self.param_groups):
             for key, p in zip(saved["params"], group["params"]):

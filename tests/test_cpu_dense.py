@@ -151,3 +151,19 @@ def test_adamw_bounds_see_mistakes():
     assert do.check_bf16(right, w1, tw, words & 0xFFFF) is None
     for wrong in (w1.bfloat16(), do.stochastic_bf16(w1, words >> 16).bfloat16()):
         assert do.check_bf16(wrong, w1, tw, words & 0xFFFF) is not None
+
+
+def test_optimizer_refuses_what_it_does_not_do():
+    from haste_b200.optim import AdamW
+    p = torch.nn.Parameter(torch.zeros(4))
+    for kw in (dict(amsgrad=True), dict(maximize=True)):
+        with pytest.raises(RuntimeError, match="amsgrad or maximize"):
+            AdamW([p]).load_state_dict(torch.optim.AdamW([p], **kw).state_dict())
+    opt = AdamW([p], lr=0.5)
+    opt.load_state_dict(torch.optim.AdamW([p], lr=0.25, weight_decay=0.125).state_dict())
+    assert opt.param_groups[0]["lr"] == 0.25 and opt.param_groups[0]["state_bits"] == 32 and opt.param_groups[0]["step_count"] == 0
+    opt.step()                                             # no gradients: nothing to do
+    assert opt.param_groups[0]["step_count"] == 1
+    for kw in (dict(lr=-1.0), dict(weight_decay=-1.0), dict(betas=(0.9, 1.0)), dict(eps=0.0), dict(state_bits=4), dict(max_grad_norm=-1.0)):
+        with pytest.raises(ValueError):
+            AdamW([p], **kw)
