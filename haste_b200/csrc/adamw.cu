@@ -36,7 +36,9 @@ constexpr int AHEAD = 4;               // blocks of gradients that a warp of the
 constexpr float CODE_TOP = 1.875f;
 constexpr float CODE_TINY = 0x1p-120f; // a block whose largest value is below holds zeros (1.875 / it is finite)
 
-constexpr int TABLE_SMALL = 112, TABLE_LARGE = 1024;      // 3.2 KB and 28.7 KB of kernel parameters (32,764 bytes at most)
+// 0.7, 7 and 28.7 KB of kernel parameters (32,764 bytes at most); the larger ones cost the host more (launching a step
+// over 150 tensors 9.6 us with the largest, 7.5 with the middle one).
+constexpr int TABLE_SMALL = 24, TABLE_MIDDLE = 256, TABLE_LARGE = 1024;
 
 // The tensors of one launch, as a kernel parameter.  first[i]: first block of tensor i among the launch's blocks.
 template <int N>
@@ -428,7 +430,8 @@ __global__ void __launch_bounds__(ADAM_THREADS) grad_squares_kernel(const __grid
 // 12.0 us instead of 14.2; the launch costs more than the other SMs would bring).
 constexpr int NORM_CLUSTER = 8, NORM_THREADS = 1024;
 constexpr int64_t NORM_SMALL_BLOCKS = 4096;
-__global__ void __cluster_dims__(NORM_CLUSTER, 1, 1) __launch_bounds__(NORM_THREADS) grad_norm_small_kernel(const __grid_constant__ TensorTable<TABLE_SMALL> tab,
+template <int N>
+__global__ void __cluster_dims__(NORM_CLUSTER, 1, 1) __launch_bounds__(NORM_THREADS) grad_norm_small_kernel(const __grid_constant__ TensorTable<N> tab,
                                                                                                            float grad_scale, float* __restrict__ norm) {
   __shared__ float sums[NORM_CLUSTER];
   auto cluster = cooperative_groups::this_cluster();
@@ -549,8 +552,9 @@ static int for_each_table(void* const* params, const int32_t* types, const void*
   return HASTE_OK;
 }
 
-static TensorTable<TABLE_SMALL> small_table(const TensorTable<TABLE_LARGE>& tab) {
-  TensorTable<TABLE_SMALL> s;
+template <int N>
+static TensorTable<N> cut_table(const TensorTable<TABLE_LARGE>& tab) {
+  TensorTable<N> s;
   s.count = tab.count;
   s.first[0] = 0;
   for (int i = 0; i < tab.count; ++i) { s.p[i] = tab.p[i]; s.g[i] = tab.g[i]; s.n[i] = tab.n[i]; s.first[i + 1] = tab.first[i + 1]; }
@@ -565,7 +569,8 @@ static int adamw_typed(const AdamWCall& c, const AdamArgs& a, cudaStream_t st) {
     float* ms = BITS == 8 ? c.avg_scale + block0 : nullptr;
     float* vs = BITS == 8 ? c.sq_scale + block0 : nullptr;
     const int grid = adam_grid(blocks, BITS == 32 ? ADAM_PER_SM_32 : ADAM_PER_SM_8);
-    if (tab.count <= TABLE_SMALL) adamw_kernel<P, G, BITS, TABLE_SMALL><<<grid, ADAM_THREADS, 0, st>>>(small_table(tab), m, ms, v, vs, block0, a);
+    if (tab.count <= TABLE_SMALL) adamw_kernel<P, G, BITS, TABLE_SMALL><<<grid, ADAM_THREADS, 0, st>>>(cut_table<TABLE_SMALL>(tab), m, ms, v, vs, block0, a);
+    else if (tab.count <= TABLE_MIDDLE) adamw_kernel<P, G, BITS, TABLE_MIDDLE><<<grid, ADAM_THREADS, 0, st>>>(cut_table<TABLE_MIDDLE>(tab), m, ms, v, vs, block0, a);
     else adamw_kernel<P, G, BITS, TABLE_LARGE><<<grid, ADAM_THREADS, 0, st>>>(tab, m, ms, v, vs, block0, a);
     return check_launch("adamw_kernel");
   });
@@ -600,14 +605,15 @@ int launch_grad_norm(const void* const* grads, const int32_t* types, const int64
   int parts = 0;
   bool done = false;
   const int rc = for_each_table(nullptr, types, grads, sizes, count, [&](const TensorTable<TABLE_LARGE>& tab, int64_t, int64_t blocks) {
-    if (count <= TABLE_SMALL && blocks <= NORM_SMALL_BLOCKS) {            // (all of them: one table)
-      grad_norm_small_kernel<<<NORM_CLUSTER, NORM_THREADS, 0, st>>>(small_table(tab), grad_scale, norm);
+    if (count <= TABLE_MIDDLE && blocks <= NORM_SMALL_BLOCKS) {           // (all of them: one table)
+      if (count <= TABLE_SMALL) grad_norm_small_kernel<<<NORM_CLUSTER, NORM_THREADS, 0, st>>>(cut_table<TABLE_SMALL>(tab), grad_scale, norm);
+      else grad_norm_small_kernel<<<NORM_CLUSTER, NORM_THREADS, 0, st>>>(cut_table<TABLE_MIDDLE>(tab), grad_scale, norm);
       done = true;
       return check_launch("grad_norm_small_kernel");
     }
     const int grid = static_cast<int>(imin64(adam_grid(blocks, 4), cap));
     if (grid < 1 || parts + grid > HASTE_GRAD_NORM_PARTIALS) return fail(HASTE_ERR_TOO_LARGE, "haste_grad_norm: too many tensors for one call");
-    if (tab.count <= TABLE_SMALL) grad_squares_kernel<TABLE_SMALL><<<grid, ADAM_THREADS, 0, st>>>(small_table(tab), partial, parts);
+    if (tab.count <= TABLE_MIDDLE) grad_squares_kernel<TABLE_MIDDLE><<<grid, ADAM_THREADS, 0, st>>>(cut_table<TABLE_MIDDLE>(tab), partial, parts);
     else grad_squares_kernel<TABLE_LARGE><<<grid, ADAM_THREADS, 0, st>>>(tab, partial, parts);
     parts += grid;
     return check_launch("grad_squares_kernel");

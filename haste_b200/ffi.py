@@ -464,7 +464,7 @@ def layer_norm_forward(x, weight, bias, eps=1e-5, stats=True):
         return y
     rows = x.numel() // D
     mean = torch.empty(rows, dtype=torch.float32, device=dev)
-    rstd = torch.empty(rows, dtype=torch.float32, device=dev)
+    rstd = torch.empty_like(mean)
     _call(dev, "layer_norm_forward", lib.haste_layer_norm_forward, src.data_ptr(), w, b, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), rows, D, ldx, eps, x_type,
           w_type or 0)
     if x.dim() != 2:
@@ -579,8 +579,17 @@ def adamw_step(params, grads, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_sca
     there = _present(grads)
     if not there:
         return None                                      # nothing to do
-    dev, ptrs = _tensor_list(params, "parameters")
     gdev, gptrs = _tensor_list(there, "gradients")
+    g_sizes, g_dtype = _sizes(there), set(map(_dtype, there))
+    g_type = _type_of(there[0], "gradients")
+    if max_norm is None:
+        norm = None
+    elif norm is None:
+        if len(g_dtype) == 1:                            # (else refused below) the norm is on its way while the parameters are looked at
+            norm = _norm_of(gdev, gptrs, array.array("i", [g_type]) * len(gptrs), g_sizes, grad_scale)
+    elif norm.get_device() != gdev or norm.dtype != torch.float32 or norm.numel() != 1:
+        raise RuntimeError("norm must be one fp32 value on the parameters' device")
+    dev, ptrs = _tensor_list(params, "parameters")
     if dev != gdev:
         raise RuntimeError("parameters and gradients must be on one device")
     sizes = _sizes(params)
@@ -590,12 +599,11 @@ def adamw_step(params, grads, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_sca
         paired_sizes = _sizes(paired)
         rest = iter(gptrs)
         all_gptrs = array.array("Q", [0 if g is None else next(rest) for g in grads])
-    p_dtype, g_dtype = set(map(_dtype, params)), set(map(_dtype, there))
     dims = list(map(_dim, paired))
-    if (len(p_dtype) != 1 or len(g_dtype) != 1 or dims != list(map(_dim, there)) or paired_sizes != _sizes(there)
+    if (len(set(map(_dtype, params))) != 1 or len(g_dtype) != 1 or dims != list(map(_dim, there)) or paired_sizes != g_sizes
             or (max(dims) > 1 and any(d > 1 and p.shape != g.shape for d, p, g in zip(dims, paired, there)))):
         raise RuntimeError("all parameters must have one type, all gradients one type, and every gradient its parameter's shape")
-    p_type, g_type = _type_of(params[0], "parameters"), _type_of(there[0], "gradients")
+    p_type = _type_of(params[0], "parameters")
     moments = exp_avg.numel()
     dtype = torch.float32 if bits == 32 else torch.uint8
     for t in (exp_avg, exp_avg_sq):
@@ -607,12 +615,6 @@ def adamw_step(params, grads, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_sca
             if t.get_device() != dev or t.dtype != torch.float32 or t.numel() * MOMENT_BLOCK < moments or not t.is_contiguous():
                 raise RuntimeError(f"scales must be contiguous, fp32, one value per {MOMENT_BLOCK} elements of the moments, on the parameters' device")
         ms, vs = exp_avg_scale.data_ptr(), exp_avg_sq_scale.data_ptr()
-    if max_norm is None:
-        norm = None
-    elif norm is None:
-        norm = _norm_of(dev, gptrs, array.array("i", [g_type]) * len(gptrs), paired_sizes, grad_scale)
-    elif norm.get_device() != dev or norm.dtype != torch.float32 or norm.numel() != 1:
-        raise RuntimeError("norm must be one fp32 value on the parameters' device")
     _call(dev, "adamw_step", lib.haste_adamw_step, _address(ptrs), _address(all_gptrs), _address(sizes), len(ptrs), exp_avg.data_ptr(), ms, exp_avg_sq.data_ptr(), vs,
           moments, bits, p_type, g_type, float(lr), betas[0], betas[1], eps, weight_decay, step, grad_scale, max_norm or 0.0, _ptr(norm), seed & 0xFFFFFFFFFFFFFFFF,
           stream_index, flags)
