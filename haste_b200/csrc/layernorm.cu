@@ -667,7 +667,9 @@ __global__ void __launch_bounds__(MODE == BLOCK ? (VEC * NV > 16 ? 256 : 512) : 
 // ================================================================ launchers
 static unsigned capped(int64_t want, int64_t cap) { return static_cast<unsigned>(want < cap ? want : cap); }
 
-// How a row of D elements is held: nv vectors of `vec` elements a thread, T threads (lanes of a warp, or a block), or `wide`.
+// How a row of D elements is held: nv vectors of `vec` elements a thread, T threads (lanes of a warp, or a block), or `wide`.  Few threads with
+// many vectors: sums over threads and barriers cost more than warps that wait (32768 x 4096 bf16 backward 175 us with 4 vectors a thread, 214 with
+// 3, 211 with 2, before the last changes); a fifth vector does not fit the registers (65536 x 1280 backward 152 us instead of 116).
 struct RowPlan {
   bool wide = false, block = false;
   int nv = 1, T = 32;
@@ -692,11 +694,17 @@ static RowPlan plan_rows(int64_t D, int vec, int most) {
   return p;
 }
 
-// Blocks of the row kernels: as many as stay resident, since each of them leaves a part of dw and db.  Where rows do not all start on a
+// Blocks a SM of the backward pass, each of which leaves a part of dw and db in the scratch: at most this many.
+constexpr int LN_MOST_PER_SM = 8;
+
+// Blocks of the row kernels: as many as stay resident (in the backward pass more are slower: 65536 x 1024 bf16 72 us with these, 80 with
+// twice and 90 with four times as many).  Where rows do not all start on a
 // 16-byte boundary, a group's rows have to be a multiple of 8 apart.
-static unsigned row_blocks(const RowPlan& p, int64_t rows, int64_t D, int vec, int resident_threads) {
+static unsigned row_blocks(const RowPlan& p, int64_t rows, int64_t D, int vec, int resident_threads, int most_per_sm, int turns) {
   const int64_t groups = p.block ? 1 : LN_WARP_THREADS / p.T, threads = p.block ? p.T : LN_WARP_THREADS;
-  const int64_t want = (rows + groups - 1) / groups, per_sm = resident_threads / threads < 1 ? 1 : resident_threads / threads, most = per_sm * sm_count();
+  const int64_t want = (rows + groups - 1) / groups, per_sm = imin64(resident_threads / threads < 1 ? 1 : resident_threads / threads, most_per_sm);
+  int64_t most = per_sm * sm_count();
+  if (turns > 1) most *= want / (4 * most) < 1 ? 1 : imin64(want / (4 * most), turns);
   if (want <= most) return static_cast<unsigned>(want);
   return static_cast<unsigned>(D % vec == 0 ? most : most < 8 ? 8 : most / 8 * 8);
 }
@@ -740,7 +748,11 @@ static int ln_fwd_rows(const FwdCall& c, const RowPlan& p) {
   static std::atomic<uint64_t> allowed{0};
   const int threads = MODE == BLOCK ? p.T : LN_WARP_THREADS, smem = LN_STAGES * NV * threads * VEC * static_cast<int>(sizeof(X));
   if (int rc = allow_slots(ln_fwd_kernel<X, VEC, NV, MODE, EDGE>, allowed)) return rc;
-  const unsigned blocks = row_blocks(p, c.rows, c.D, VEC, VEC * NV > 16 ? 512 : VEC * NV > 8 ? 768 : 1024);
+  // Where D is a multiple of VEC and a thread has 3 vectors or more, up to 4 times (fp32: 8 times) as many blocks as stay resident, each with
+  // at least 4 rows to a group: started in order they stay closer together in memory than blocks that walk over all of it (65536 x 1024
+  // bf16 51 -> 47 us, fp32 99 -> 81).  With fewer vectors, or weights to be loaded one by one, starting up costs more than that.
+  const int turns = !EDGE && NV >= 3 ? (sizeof(X) == 2 ? 4 : 8) : 1;
+  const unsigned blocks = row_blocks(p, c.rows, c.D, VEC, VEC * NV > 16 ? 512 : VEC * NV > 8 ? 768 : 1024, 32, turns);
   ln_fwd_kernel<X, VEC, NV, MODE, EDGE><<<blocks, threads, smem, c.st>>>((const X*)c.x, c.w, c.b, c.w_type, (X*)c.y, c.mean, c.rstd, c.rows, static_cast<int>(c.D), c.ldx,
                                                                     c.eps, p.T, in_vectors(c.x, c.ldx, c.D, VEC, 16), aligned16(c.w) && aligned16(c.b));
   return check_launch("layer_norm_forward");
@@ -777,7 +789,7 @@ int launch_layer_norm_forward(const void* x, const void* w, const void* b, void*
 
 // Parts of dw and db that the wide rows' kernel makes; the others make at most MAX_PARTS (one per block).
 static int64_t wide_parts(int64_t rows) { return rows < 16 * 64 ? (rows + 63) / 64 : 16; }
-static int64_t max_parts() { return static_cast<int64_t>(sm_count()) * 8; }
+static int64_t max_parts() { return static_cast<int64_t>(sm_count()) * LN_MOST_PER_SM; }
 
 int64_t layer_norm_backward_scratch(int64_t rows, int64_t D) {
   const int64_t parts = rows < max_parts() ? rows : max_parts();
@@ -814,7 +826,7 @@ static int ln_bwd_rows(const BwdCall& c, const RowPlan& p, float* partial, unsig
   const int slots = STAGES * NV * threads * VEC * static_cast<int>(sizeof(X) + sizeof(G));
   const int cols = MODE == BLOCK ? 0 : LN_WARP_THREADS / 32 * static_cast<int>(c.D) * 4, smem = slots > cols ? slots : cols;
   if (int rc = allow_slots(ln_bwd_kernel<X, G, VEC, NV, MODE, EDGE, STAGES>, allowed)) return rc;
-  parts = row_blocks(p, c.rows, c.D, VEC, VEC * NV > 16 ? 384 : VEC * NV > 8 ? 512 : 1024);
+  parts = row_blocks(p, c.rows, c.D, VEC, VEC * NV > 16 ? 384 : VEC * NV > 8 ? 512 : 1024, LN_MOST_PER_SM, 1);
   const int64_t g_bytes = VEC * sizeof(G) < 16 ? 8 : 16;
   ln_bwd_kernel<X, G, VEC, NV, MODE, EDGE, STAGES><<<parts, threads, smem, c.st>>>((const G*)c.dy, (const X*)c.x, c.w, c.w_type, c.mean, c.rstd, (X*)c.dx, partial, c.rows,
                                                                       static_cast<int>(c.D), c.lddy, c.ldx, p.T, in_vectors(c.x, c.ldx, c.D, VEC, 16),
