@@ -32,7 +32,7 @@ namespace haste {
 
 constexpr int ADAM_BLOCK = 256;        // elements that share a scale; the place of a tensor in the moments is a multiple of it
 constexpr int ADAM_THREADS = 256, ADAM_WARPS = ADAM_THREADS / 32;
-constexpr int AHEAD = 4;               // blocks of gradients that a warp of the norm has on their way, and the most of a turn
+constexpr int AHEAD = 4;               // blocks of gradients that a warp of the norm has on their way
 constexpr float CODE_TOP = 1.875f;
 constexpr float CODE_TINY = 0x1p-120f; // a block whose largest value is below holds zeros (1.875 / it is finite)
 

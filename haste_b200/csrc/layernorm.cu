@@ -698,8 +698,7 @@ static RowPlan plan_rows(int64_t D, int vec, int most) {
 constexpr int LN_MOST_PER_SM = 8;
 
 // Blocks of the row kernels: as many as stay resident (in the backward pass more are slower: 65536 x 1024 bf16 72 us with these, 80 with
-// twice and 90 with four times as many).  Where rows do not all start on a
-// 16-byte boundary, a group's rows have to be a multiple of 8 apart.
+// twice and 90 with four times as many).  Where rows do not all start on a 16-byte boundary, a group's rows have to be a multiple of 8 apart.
 static unsigned row_blocks(const RowPlan& p, int64_t rows, int64_t D, int vec, int resident_threads, int most_per_sm, int turns) {
   const int64_t groups = p.block ? 1 : LN_WARP_THREADS / p.T, threads = p.block ? p.T : LN_WARP_THREADS;
   const int64_t want = (rows + groups - 1) / groups, per_sm = imin64(resident_threads / threads < 1 ? 1 : resident_threads / threads, most_per_sm);
@@ -787,13 +786,24 @@ int launch_layer_norm_forward(const void* x, const void* w, const void* b, void*
   return x_type == HASTE_BF16 ? ln_fwd<__nv_bfloat16>(c) : ln_fwd<float>(c);
 }
 
-// Parts of dw and db that the wide rows' kernel makes; the others make at most MAX_PARTS (one per block).
+// Threads that stay resident on a SM with `per_thread` elements each, in the backward pass.
+constexpr int bwd_resident(int per_thread) { return per_thread > 16 ? 384 : per_thread > 8 ? 512 : 1024; }
+// Threads of a block that a row may take there: with 8 elements a vector, more would leave too few registers.
+constexpr int bwd_most(int vec) { return vec == 8 ? 256 : 512; }
+
+// Parts of dw and db: as many as blocks; of the wide rows' kernel, as many as it makes ranges of rows.
 static int64_t wide_parts(int64_t rows) { return rows < 16 * 64 ? (rows + 63) / 64 : 16; }
-static int64_t max_parts() { return static_cast<int64_t>(sm_count()) * LN_MOST_PER_SM; }
 
 int64_t layer_norm_backward_scratch(int64_t rows, int64_t D) {
-  const int64_t parts = rows < max_parts() ? rows : max_parts();
-  return (D > 8192 ? wide_parts(rows) : parts) * 2 * D;
+  int64_t parts = wide_parts(rows);
+  for (int vec = 4; vec <= 8; vec += 4) {              // fp32 and bf16 rows
+    const RowPlan p = plan_rows(D, vec, bwd_most(vec));
+    if (!p.wide && rows > 0) {
+      const int64_t n = row_blocks(p, rows, D, vec, bwd_resident(vec * p.nv), LN_MOST_PER_SM, 1);
+      if (n > parts) parts = n;
+    }
+  }
+  return parts * 2 * D;
 }
 
 template <class X, class G, class W>
@@ -826,7 +836,7 @@ static int ln_bwd_rows(const BwdCall& c, const RowPlan& p, float* partial, unsig
   const int slots = STAGES * NV * threads * VEC * static_cast<int>(sizeof(X) + sizeof(G));
   const int cols = MODE == BLOCK ? 0 : LN_WARP_THREADS / 32 * static_cast<int>(c.D) * 4, smem = slots > cols ? slots : cols;
   if (int rc = allow_slots(ln_bwd_kernel<X, G, VEC, NV, MODE, EDGE, STAGES>, allowed)) return rc;
-  parts = row_blocks(p, c.rows, c.D, VEC, VEC * NV > 16 ? 384 : VEC * NV > 8 ? 512 : 1024, LN_MOST_PER_SM, 1);
+  parts = row_blocks(p, c.rows, c.D, VEC, bwd_resident(VEC * NV), LN_MOST_PER_SM, 1);
   const int64_t g_bytes = VEC * sizeof(G) < 16 ? 8 : 16;
   ln_bwd_kernel<X, G, VEC, NV, MODE, EDGE, STAGES><<<parts, threads, smem, c.st>>>((const G*)c.dy, (const X*)c.x, c.w, c.w_type, c.mean, c.rstd, (X*)c.dx, partial, c.rows,
                                                                       static_cast<int>(c.D), c.lddy, c.ldx, p.T, in_vectors(c.x, c.ldx, c.D, VEC, 16),
@@ -860,7 +870,7 @@ static int ln_bwd(const BwdCall& c) {
   float* partial = want ? c.scratch : nullptr;
   unsigned parts = 0;
   if (c.rows > 0) {
-    RowPlan p = plan_rows(c.D, VEC, VEC == 8 ? 256 : 512);
+    RowPlan p = plan_rows(c.D, VEC, bwd_most(VEC));
     if (!aligned16(c.dx)) p.wide = true;
     int rc = HASTE_OK;
     if (p.wide) {
