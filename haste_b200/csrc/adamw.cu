@@ -431,6 +431,7 @@ __device__ __forceinline__ float sum_of_squares(const TensorTable<N>& tab, int l
 // One sum per thread block, each of which has a share of the blocks of its own, into partial[part0 + blockIdx.x].
 template <int N>
 __global__ void __launch_bounds__(ADAM_THREADS) grad_squares_kernel(const __grid_constant__ TensorTable<N> tab, float* __restrict__ partial, int part0) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t blocks = tab.first[tab.count];
   const float s = sum_of_squares<ADAM_THREADS>(tab, static_cast<int>(blocks * blockIdx.x / gridDim.x), static_cast<int>(blocks * (blockIdx.x + 1) / gridDim.x));
   if (threadIdx.x == 0) partial[part0 + blockIdx.x] = s;
@@ -459,6 +460,7 @@ __global__ void __cluster_dims__(NORM_CLUSTER, 1, 1) __launch_bounds__(NORM_THRE
 // sqrt of the sum of the partial sums (in 64 bits: one block adds a few hundred), in an order that depends on their number alone.
 __global__ void __launch_bounds__(ADAM_THREADS) grad_norm_finish_kernel(const float* __restrict__ partial, int parts, float grad_scale, float* __restrict__ norm) {
   __shared__ double sums[ADAM_THREADS / 32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   double s = 0.0;
   for (int i = threadIdx.x; i < parts; i += ADAM_THREADS) s += partial[i];
 #pragma unroll
@@ -629,7 +631,8 @@ int launch_grad_norm(const void* const* grads, const int32_t* types, const int64
     return check_launch("grad_squares_kernel");
   });
   if (rc != HASTE_OK || done) return rc;
-  grad_norm_finish_kernel<<<1, ADAM_THREADS, 0, st>>>(partial, parts, grad_scale, norm);
+  if (parts > 0) return launch_behind(grad_norm_finish_kernel, 1, ADAM_THREADS, st, static_cast<const float*>(partial), parts, grad_scale, norm);
+  grad_norm_finish_kernel<<<1, ADAM_THREADS, 0, st>>>(partial, parts, grad_scale, norm);           // no elements: no kernel of this call comes before
   return check_launch("grad_norm_finish_kernel");
 }
 

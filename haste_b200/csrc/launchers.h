@@ -18,6 +18,23 @@ int allow_dynamic_smem(K kernel) {
   return HASTE_OK;
 }
 
+// Launches a kernel whose blocks may be placed while the kernel before it in the stream, one of the same call, is still at work; it waits for that one's
+// end itself (griddepcontrol.wait) before it reads anything.  (Layer norm backward of 4099 x 1021: 24.6 us a call without, 23.2 so.)
+template <class K, class... A>
+int launch_behind(K kernel, unsigned grid, unsigned threads, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaLaunchKernelEx: %s", cudaGetErrorString(e));
+  return HASTE_OK;
+}
 
 // Everything the fused weight/bias update needs.  mom_* are NULL when momentum is off.
 struct UpdateArgs {

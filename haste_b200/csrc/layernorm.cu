@@ -127,6 +127,7 @@ __device__ __forceinline__ void finish_columns(const float* __restrict__ partial
   __shared__ float shares[CLUSTER][32];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, rank = blockIdx.x % CLUSTER;
   const int64_t c = static_cast<int64_t>(blockIdx.x / CLUSTER) * 32 + tx;      // column of the [2 D] row of one part
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   float s = 0.f;
   if (c < 2 * D) {
 #pragma unroll 8
@@ -611,6 +612,7 @@ __global__ void __launch_bounds__(MODE == BLOCK ? (VEC * NV > 16 ? 256 : 512) : 
     at = next_at;
   }
   copies_wait<0>();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (partial == nullptr) return;
   float* const part = partial + static_cast<int64_t>(blockIdx.x) * 2 * D;
   const int vec_step = xin.vec_step();
@@ -856,10 +858,15 @@ static int ln_bwd_plan(const BwdCall& c, const RowPlan& p, float* partial, unsig
 // Four blocks to 32 columns where there are many parts and few columns: 888 parts of 1021 columns 6.3 us by one, 4.7 by four; 444 of 4096
 // 5.3 and 9.0.
 template <class W>
-static void ln_finish(const BwdCall& c, int parts, W* dw, W* db) {
+static int ln_finish(const BwdCall& c, int parts, W* dw, W* db) {
   const unsigned grid = static_cast<unsigned>((2 * c.D + 31) / 32);
-  if (parts >= 256 && grid <= 128) ln_bwd_finish_many_kernel<W><<<grid * LN_FINISH_CLUSTER, LN_FINISH_THREADS, 0, c.st>>>(c.scratch, parts, c.D, dw, db);
-  else ln_bwd_finish_kernel<W><<<grid, LN_FINISH_THREADS, 0, c.st>>>(c.scratch, parts, c.D, dw, db);
+  if (parts >= 256 && grid <= 128)
+    return launch_behind(ln_bwd_finish_many_kernel<W>, grid * LN_FINISH_CLUSTER, LN_FINISH_THREADS, c.st, static_cast<const float*>(c.scratch), parts, c.D, dw, db);
+  if (c.rows == 0) {                    // no kernel of this call comes before
+    ln_bwd_finish_kernel<W><<<grid, LN_FINISH_THREADS, 0, c.st>>>(c.scratch, parts, c.D, dw, db);
+    return check_launch("layer_norm_backward");
+  }
+  return launch_behind(ln_bwd_finish_kernel<W>, grid, LN_FINISH_THREADS, c.st, static_cast<const float*>(c.scratch), parts, c.D, dw, db);
 }
 
 template <class X, class G>
@@ -883,8 +890,7 @@ static int ln_bwd(const BwdCall& c) {
     if (rc != HASTE_OK) return rc;
   }
   if (want) {
-    if (c.w_type == HASTE_BF16) ln_finish(c, static_cast<int>(parts), (B*)c.dw, (B*)c.db);
-    else ln_finish(c, static_cast<int>(parts), (float*)c.dw, (float*)c.db);
+    return c.w_type == HASTE_BF16 ? ln_finish(c, static_cast<int>(parts), (B*)c.dw, (B*)c.db) : ln_finish(c, static_cast<int>(parts), (float*)c.dw, (float*)c.db);
   }
   return check_launch("layer_norm_backward");
 }
