@@ -5,7 +5,8 @@
 //   h  = dy w             dx = r (h - mean(h) - z mean(h z))     dw = sum_rows dy z     db = sum_rows dy
 //
 // All sums are fp32; the variance is taken around the mean, not from the sum of squares, which cancels for rows whose mean is large
-// against their spread.  Inputs and outputs are bf16 or fp32, rounded once (nearest even) when stored.
+// against their spread.  x is added up times a power of two, 1 / D or the next below, so that a row of the largest numbers has a mean.
+// Inputs and outputs are bf16 or fp32, rounded once (nearest even) when stored.
 //
 // Memory bounds all of it: x in and y out, or dy and x in and dx out.  A row is read once and stays on the chip: 1 to 32 lanes of a
 // warp have it, or a thread block where it is wider, each thread up to 4 vectors of 16 bytes.  These groups walk over the rows with the
@@ -41,6 +42,9 @@ __device__ __forceinline__ float block_sum(float v, float* buf) {
   return s;
 }
 
+// The largest power of two that is not above 1 / D.
+__device__ __forceinline__ float power_below(int64_t D) { return __int_as_float((127 - (64 - __clzll(D - 1))) << 23); }
+
 constexpr int LN_THREADS = 256;
 
 // ---------------------------------------------------------------- rows of any width: one block a row, the row read again for each pass
@@ -49,11 +53,12 @@ __global__ void __launch_bounds__(LN_THREADS) ln_fwd_wide_kernel(const X* __rest
                                                                  float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows, int64_t D,
                                                                  int64_t ldx, float eps) {
   __shared__ float buf[LN_THREADS / 32];
+  const float part = power_below(D);
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const X* xr = x + r * ldx;
     float s = 0.f;
-    for (int64_t j = threadIdx.x; j < D; j += LN_THREADS) s += ld_f(xr + j);
-    const float mean = block_sum(s, buf) / static_cast<float>(D);
+    for (int64_t j = threadIdx.x; j < D; j += LN_THREADS) s = fmaf(ld_f(xr + j), part, s);
+    const float mean = block_sum(s, buf) / (static_cast<float>(D) * part);
     s = 0.f;
     for (int64_t j = threadIdx.x; j < D; j += LN_THREADS) { const float d = ld_f(xr + j) - mean; s += d * d; }
     const float rstd = 1.f / sqrtf(block_sum(s, buf) / static_cast<float>(D) + eps);
@@ -447,7 +452,7 @@ __global__ void __launch_bounds__(MODE == BLOCK ? 512 : LN_WARP_THREADS, MODE ==
   extern __shared__ __align__(16) char slots[];
   RowGroup<MODE, NV> grp(t);
   grp.clear(buf);
-  const float inv_d = 1.f / static_cast<float>(D);
+  const float inv_d = 1.f / static_cast<float>(D), part = power_below(D), inv_dp = 1.f / (static_cast<float>(D) * part);
   const int64_t stride = grp.stride();
   int64_t r = grp.first_row() + grp.own(), left = rows - grp.first_row();       // left: rows from the warp's (block's) first one on
   const int s = EDGE ? static_cast<int>(r * D % VEC) : 0, first = grp.c == 0 ? s : 0, j0 = grp.c * VEC - s;
@@ -472,10 +477,10 @@ __global__ void __launch_bounds__(MODE == BLOCK ? 512 : LN_WARP_THREADS, MODE ==
     for (int i = 0; i < NV; ++i) {
       in.get(at, i, first, f[i]);
 #pragma unroll
-      for (int k = 0; k < VEC / 2; ++k) { if (k & 1) s2 = add2(s2, f[i][k]); else s1 = add2(s1, f[i][k]); }
+      for (int k = 0; k < VEC / 2; ++k) { if (k & 1) s2 = fma2(f[i][k], both(part), s2); else s1 = fma2(f[i][k], both(part), s1); }
     }
     s1 = add2(s1, s2);
-    const float mean = grp.sum(s1.x + s1.y, buf) * inv_d;
+    const float mean = grp.sum(s1.x + s1.y, buf) * inv_dp;
     s1 = s2 = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -551,7 +556,8 @@ __global__ void __launch_bounds__(MODE == BLOCK ? (VEC * NV > 16 ? 256 : 512) : 
 #pragma unroll
     for (int k = 0; k < VEC / 2; ++k) aw[i][k] = ab[i][k] = both(0.f);
   }
-  // sums of h and h z over a thread's columns of the row at `at`
+  // Sums of h and h z over a thread's columns of the row at `at`.  Outside the row g and x are 0, and x - mean is finite where z might not be
+  // (a row of the largest numbers): z is not formed, its factor r goes to dy and to the sum.
   auto row_sums = [&](int at, float mean, float rstd, float& a, float& b) {
     float2 sh = both(0.f), shz = both(0.f);
 #pragma unroll
@@ -560,16 +566,16 @@ __global__ void __launch_bounds__(MODE == BLOCK ? (VEC * NV > 16 ? 256 : 512) : 
       xin.get(at, i, first, f);
       gin.get(at, i, first, g);
 #pragma unroll
-      for (int k = 0; k < VEC / 2; ++k) {       // outside the row g is 0
-        const float2 z = mul2(add2(f[k], both(-mean)), both(rstd)), h = mul2(g[k], wf[i][k]);
-        aw[i][k] = fma2(g[k], z, aw[i][k]);
+      for (int k = 0; k < VEC / 2; ++k) {
+        const float2 c = add2(f[k], both(-mean)), h = mul2(g[k], wf[i][k]);
+        aw[i][k] = fma2(mul2(g[k], both(rstd)), c, aw[i][k]);
         ab[i][k] = add2(ab[i][k], g[k]);
         sh = add2(sh, h);
-        shz = fma2(h, z, shz);
+        shz = fma2(h, c, shz);
       }
     }
     a = sh.x + sh.y;
-    b = shz.x + shz.y;
+    b = (shz.x + shz.y) * rstd;
   };
   const float *mean_at = mean_in + r, *rstd_at = rstd_in + r;
   float mean = 0.f, rstd = 0.f, next_mean = 0.f, next_rstd = 0.f, a = 0.f, b = 0.f;

@@ -148,6 +148,34 @@ def test_rows_of_unusual_values(D):
     assert torch.equal(dx[keep], grads[0][keep]) and bool(dx[~keep].isnan().any(1).all()) and torch.equal(db, grads[2])
 
 
+@pytest.mark.parametrize("xt", [BF, F32])
+@pytest.mark.parametrize("value", [torch.finfo(BF).min, torch.finfo(BF).max])
+@pytest.mark.parametrize("D", [1, 2, 4, 16, 64, 1024, 2048, 16384])
+def test_rows_of_the_largest_numbers(D, value, xt):
+    """A constant row has itself as mean, variance 0, z = 0: y = b and dx = r (h - mean(h)), however large the constant is.  Where D is a power of two
+    and the constant has 8 significant bits, every partial sum is exact."""
+    from haste_b200.norm import layer_norm_backward, layer_norm_forward
+    x, w, b, dy = _inputs(9, D, xt, F32)
+    x[1::2] = value
+    dy = dy.to(F32)
+    y, mean, rstd = layer_norm_forward(x, w, b, 1e-5)
+    big = slice(1, None, 2)
+    assert torch.equal(y[big], b.to(xt).expand_as(y[big])) and bool((mean[big] == value).all())
+    assert bool(((rstd[big].double() - 1e-5 ** -0.5).abs() <= 6 * do.U * 1e-5 ** -0.5).all())      # eps, its root and the quotient rounded
+    dx, dw, db = layer_norm_backward(dy, x, w, mean, rstd)
+    h, r = dy[big].double() * w.double(), rstd[big].double()[:, None]
+    mh = h.mean(-1, keepdim=True)
+    tol = r * (4 * do.U * (h.abs() + mh.abs()) + do.chain(D) * h.abs().mean(-1, keepdim=True))
+    bad = do.outside(dx[big], r * (h - mh), tol, "dx")
+    assert bad is None, bad
+    # the other rows have what they would have alone, and the large ones add nothing to dw
+    alone = layer_norm_backward(dy[::2].contiguous(), x[::2].contiguous(), w, mean[::2].contiguous(), rstd[::2].contiguous())
+    assert torch.equal(dx[::2], alone[0]) and bool(torch.isfinite(dw).all())
+    want, tol = do.layer_norm_grad(dy[::2], x[::2], w, mean[::2], rstd[::2])
+    bad = do.outside(dw, want[1], tol[1], "dw") or do.outside(db, dy.double().sum(0), 73 * do.U * dy.double().abs().sum(0), "db")
+    assert bad is None, bad
+
+
 @pytest.mark.parametrize("D", [40, 768, 1021])
 def test_gradients_against_differences(D):
     """Directional derivatives of sum(y * dy) by central differences of the forward kernel.  With steps of 2^-7 in directions of unit size
