@@ -254,44 +254,78 @@ template <class T, int VEC> struct Slot {
       else *reinterpret_cast<uint2*>(dst + k * step) = make_uint2(0u, 0u);
     }
   }
-  // MASK: the elements before `first` belong to another row and read as 0
+  // Masks of the words that hold elements `first` and following: what lies before belongs to another row and reads as 0.
+  static constexpr int REGS = BYTES / 4;
+  static __device__ __forceinline__ void head_masks(int first, uint32_t (&m)[REGS]) {
+#pragma unroll
+    for (int e = 0; e < REGS; ++e) {
+      if constexpr (sizeof(T) == 4) m[e] = e < first ? 0u : 0xFFFFFFFFu;
+      else m[e] = (2 * e < first ? 0u : 0x0000FFFFu) | (2 * e + 1 < first ? 0u : 0xFFFF0000u);
+    }
+  }
   template <bool MASK>
-  static __device__ __forceinline__ void get(const char* src, int step, float2 (&f)[VEC / 2], int first) {
+  static __device__ __forceinline__ void get(const char* src, int step, float2 (&f)[VEC / 2], const uint32_t (&m)[REGS]) {
+    uint32_t u[REGS];
 #pragma unroll
     for (int k = 0; k < WORDS; ++k) {
-      if constexpr (sizeof(T) == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(src + k * step);
-        f[2 * k] = make_float2(v.x, v.y); f[2 * k + 1] = make_float2(v.z, v.w);
-      } else {
-        uint32_t u[PER / 2];
-        if constexpr (UNIT == 16) { const uint4 v = *reinterpret_cast<const uint4*>(src + k * step); u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w; }
-        else { const uint2 v = *reinterpret_cast<const uint2*>(src + k * step); u[0] = v.x; u[1] = v.y; }
-#pragma unroll
-        for (int e = 0; e < PER / 2; ++e) f[e] = make_float2(__uint_as_float(u[e] << 16), __uint_as_float(u[e] & 0xFFFF0000u));
-      }
+      if constexpr (UNIT == 16) { const uint4 v = *reinterpret_cast<const uint4*>(src + k * step); u[4 * k] = v.x; u[4 * k + 1] = v.y; u[4 * k + 2] = v.z; u[4 * k + 3] = v.w; }
+      else { const uint2 v = *reinterpret_cast<const uint2*>(src + k * step); u[0] = v.x; u[1] = v.y; }
     }
-    if (MASK) {
 #pragma unroll
-      for (int e = 0; e < VEC / 2; ++e) { f[e].x = 2 * e < first ? 0.f : f[e].x; f[e].y = 2 * e + 1 < first ? 0.f : f[e].y; }
+    for (int e = 0; e < REGS; ++e) if (MASK) u[e] &= m[e];
+#pragma unroll
+    for (int e = 0; e < VEC / 2; ++e) {
+      if constexpr (sizeof(T) == 4) f[e] = make_float2(__uint_as_float(u[2 * e]), __uint_as_float(u[2 * e + 1]));
+      else f[e] = make_float2(__uint_as_float(u[e] << 16), __uint_as_float(u[e] & 0xFFFF0000u));
     }
   }
 };
 
-__device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float2 (&f)[4]) {
-  uint32_t w[4];
+__device__ __forceinline__ void pack(const float2 (&f)[4], uint32_t (&w)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(f[i].x, f[i].y);
     w[i] = *reinterpret_cast<const uint32_t*>(&h);
   }
+}
+__device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float2 (&f)[4]) {
+  uint32_t w[4];
+  pack(f, w);
   __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
 }
 __device__ __forceinline__ void store_vec(float* p, const float2 (&f)[2]) { __stcs(reinterpret_cast<float4*>(p), make_float4(f[0].x, f[0].y, f[1].x, f[1].y)); }
-// Columns j0 .. of a row, p the first one's place: the whole vector, or those of its elements that belong to the row.
-template <int VEC, class T>
+// A row's end of one of its vectors, elements first .. VEC - 1 or 0 .. n - 1, in powers of two: three stores instead of up to seven (the
+// warp waits for the lane that has them).
+__device__ __forceinline__ void store_head(__nv_bfloat16* p, int first, const float2 (&f)[4]) {
+  uint32_t w[4];
+  pack(f, w);
+  if (first <= 4) *reinterpret_cast<uint2*>(p + 4) = make_uint2(w[2], w[3]);
+  if ((first + 1) & 2) *reinterpret_cast<uint32_t*>(p + (first <= 2 ? 2 : 6)) = first <= 2 ? w[1] : w[3];
+  if (first & 1) *reinterpret_cast<uint16_t*>(p + first) = static_cast<uint16_t>((first < 4 ? (first < 2 ? w[0] : w[1]) : (first < 6 ? w[2] : w[3])) >> 16);
+}
+__device__ __forceinline__ void store_tail(__nv_bfloat16* p, int n, const float2 (&f)[4]) {
+  uint32_t w[4];
+  pack(f, w);
+  if (n & 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  if (n & 2) *reinterpret_cast<uint32_t*>(p + (n & 4)) = n & 4 ? w[2] : w[0];
+  if (n & 1) *reinterpret_cast<uint16_t*>(p + n - 1) = static_cast<uint16_t>(n & 4 ? (n & 2 ? w[3] : w[2]) : (n & 2 ? w[1] : w[0]));
+}
+__device__ __forceinline__ void store_head(float* p, int first, const float2 (&f)[2]) {
+  if (first <= 2) *reinterpret_cast<float2*>(p + 2) = f[1];
+  if (first & 1) p[first] = first < 2 ? f[0].y : f[1].y;
+}
+__device__ __forceinline__ void store_tail(float* p, int n, const float2 (&f)[2]) {
+  if (n & 2) *reinterpret_cast<float2*>(p) = f[0];
+  if (n & 1) p[n - 1] = n & 2 ? f[1].x : f[0].x;
+}
+// Columns j0 .. of a row, p the first one's place: the whole vector, or those of its elements that belong to the row.  HEAD, TAIL: whether
+// the row may begin, end in it.
+template <int VEC, bool HEAD, bool TAIL, class T>
 __device__ __forceinline__ void store_part(T* p, int j0, int D, const float2 (&f)[VEC / 2]) {
-  if (j0 >= 0 && j0 + VEC <= D) store_vec(p, f);
-  else {
+  if ((!HEAD || j0 >= 0) && (!TAIL || j0 + VEC <= D)) store_vec(p, f);
+  else if (HEAD && j0 < 0 && j0 + VEC <= D) store_head(p, -j0, f);
+  else if (TAIL && j0 >= 0) store_tail(p, D - j0, f);
+  else if (HEAD && TAIL) {                                             // both: D < VEC
 #pragma unroll
     for (int k = 0; k < VEC; ++k) if (static_cast<unsigned>(j0 + k) < static_cast<unsigned>(D)) st_f(p + k, k & 1 ? f[k / 2].y : f[k / 2].x);
   }
@@ -417,9 +451,10 @@ struct Feed {
   bool vec;
   char* slots;             // the thread's own, of the first stage
   uint32_t to;
+  uint32_t masks[S::REGS]; // of the thread's first vector
   __device__ __forceinline__ Feed(const T* p, int64_t ld, int64_t row, int64_t stride, int j0_, int D_, int T_, bool vec_, char* area)
       : next(p + row * ld + j0_), row_step(stride * ld), t_step(T_ * VEC), j0(j0_), D(D_), vec(vec_),
-        slots(area + (threadIdx.x >> 5) * WARP_BYTES + (threadIdx.x & 31) * S::UNIT), to(smem_address(slots)) {}
+        slots(area + (threadIdx.x >> 5) * WARP_BYTES + (threadIdx.x & 31) * S::UNIT), to(smem_address(slots)) { S::head_masks(-j0_, masks); }
   __device__ __forceinline__ int vec_step() const { return MODE == SUB ? t_step : 32 * VEC; }
   static __device__ __forceinline__ int bytes() { return WARP_BYTES * static_cast<int>(blockDim.x >> 5); }
   // Slots that no copy reaches (vectors right of the row) hold zeros for good.
@@ -436,7 +471,7 @@ struct Feed {
         for (int i = 0; i < NV; ++i) {
           const int j = j0 + i * vec_step();
           if (j < D) {
-            if (!EDGE) S::copy(to + at + i * S::WORDS * STEP, STEP, next + i * vec_step());
+            if (!EDGE || !may_end(i)) S::copy(to + at + i * S::WORDS * STEP, STEP, next + i * vec_step());
             else S::copy_part(to + at + i * S::WORDS * STEP, STEP, next + i * vec_step(), min(D - j, VEC));
           }
         }
@@ -450,11 +485,19 @@ struct Feed {
     }
     next += row_step;
   }
-  __device__ __forceinline__ void get(int at, int i, int first, float2 (&f)[VEC / 2]) const {
-    if (i == 0) S::template get<EDGE>(slots + at, STEP, f, first);
-    else S::template get<false>(slots + at + i * S::WORDS * STEP, STEP, f, 0);
+  // Whether the row may end in a thread's vector i: one of the last two, or any (a block may have whole warps beyond the row).
+  static __device__ __forceinline__ constexpr bool may_end(int i) { return MODE == BLOCK || i >= NV - 2; }
+  __device__ __forceinline__ void get(int at, int i, float2 (&f)[VEC / 2]) const {
+    if (i == 0) S::template get<EDGE>(slots + at, STEP, f, masks);
+    else S::template get<false>(slots + at + i * S::WORDS * STEP, STEP, f, masks);
   }
 };
+
+template <int VEC, class FEED, class T>
+__device__ __forceinline__ void store_at(T* p, int i, int j, int D, const float2 (&f)[VEC / 2]) {
+  if (i == 0) { if (FEED::may_end(0)) store_part<VEC, true, true>(p, j, D, f); else store_part<VEC, true, false>(p, j, D, f); }
+  else { if (FEED::may_end(i)) store_part<VEC, false, true>(p, j, D, f); else store_vec(p, f); }
+}
 
 // EDGE: D is no multiple of VEC, rows have first and last vectors that are theirs in part.
 template <class X, int VEC, int NV, int MODE, bool EDGE>
@@ -488,7 +531,7 @@ __global__ void __launch_bounds__(MODE == BLOCK ? 512 : LN_WARP_THREADS, MODE ==
     float2 f[NV][VEC / 2], s1 = both(0.f), s2 = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      in.get(at, i, first, f[i]);
+      in.get(at, i, f[i]);
 #pragma unroll
       for (int k = 0; k < VEC / 2; ++k) { if (k & 1) s2 = fma2(f[i][k], both(part), s2); else s1 = fma2(f[i][k], both(part), s1); }
     }
@@ -501,12 +544,12 @@ __global__ void __launch_bounds__(MODE == BLOCK ? 512 : LN_WARP_THREADS, MODE ==
       float2 d[VEC / 2];
 #pragma unroll
       for (int k = 0; k < VEC / 2; ++k) d[k] = f[i][k] = add2(f[i][k], both(-mean));
-      // what is not the row's counts for nothing (a row ends in one of a thread's last two vectors; a block may have whole warps beyond it)
+      // what is not the row's counts for nothing
       if (EDGE && i == 0) {
 #pragma unroll
         for (int k = 0; k < VEC / 2; ++k) { d[k].x = 2 * k < first ? 0.f : d[k].x; d[k].y = 2 * k + 1 < first ? 0.f : d[k].y; }
       }
-      if (EDGE && (MODE == BLOCK || i >= NV - 2)) {
+      if (EDGE && in.may_end(i)) {
 #pragma unroll
         for (int k = 0; k < VEC / 2; ++k) { d[k].x = j + 2 * k < D ? d[k].x : 0.f; d[k].y = j + 2 * k + 1 < D ? d[k].y : 0.f; }
       }
@@ -524,7 +567,7 @@ __global__ void __launch_bounds__(MODE == BLOCK ? 512 : LN_WARP_THREADS, MODE ==
         if (j < D) {
 #pragma unroll
           for (int k = 0; k < VEC / 2; ++k) f[i][k] = fma2(mul2(f[i][k], both(rstd)), wf[i][k], bf[i][k]);
-          if (EDGE) store_part<VEC>(out + i * in.vec_step(), j, D, f[i]); else store_vec(out + i * in.vec_step(), f[i]);
+          if (EDGE) store_at<VEC, decltype(in)>(out + i * in.vec_step(), i, j, D, f[i]); else store_vec(out + i * in.vec_step(), f[i]);
         }
       }
       if (grp.c == 0 && mean_out != nullptr) { mean_out[r] = mean; rstd_out[r] = rstd; }
@@ -550,7 +593,7 @@ __global__ void __launch_bounds__(MODE == BLOCK ? (VEC * NV > 16 ? 256 : 512) : 
   const float inv_d = 1.f / static_cast<float>(D);
   const int64_t stride = grp.stride();
   int64_t r = grp.first_row() + grp.own(), left = rows - grp.first_row();
-  const int s = EDGE ? static_cast<int>(r * D % VEC) : 0, first = grp.c == 0 ? s : 0, j0 = grp.c * VEC - s;
+  const int s = EDGE ? static_cast<int>(r * D % VEC) : 0, j0 = grp.c * VEC - s;
   Feed<X, VEC, NV, MODE, EDGE> xin(x, ldx, r, stride, j0, D, grp.T, x_vec, slots);
   Feed<G, VEC, NV, MODE, EDGE> gin(dy, lddy, r, stride, j0, D, grp.T, dy_vec, slots + xin.bytes());
   const int stage_bytes = xin.bytes() + gin.bytes(), all = STAGES * stage_bytes;
@@ -576,8 +619,8 @@ __global__ void __launch_bounds__(MODE == BLOCK ? (VEC * NV > 16 ? 256 : 512) : 
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float2 f[VEC / 2], g[VEC / 2];
-      xin.get(at, i, first, f);
-      gin.get(at, i, first, g);
+      xin.get(at, i, f);
+      gin.get(at, i, g);
 #pragma unroll
       for (int k = 0; k < VEC / 2; ++k) {
         const float2 c = add2(f[k], both(-mean)), h = mul2(g[k], wf[i][k]);
@@ -618,11 +661,11 @@ __global__ void __launch_bounds__(MODE == BLOCK ? (VEC * NV > 16 ? 256 : 512) : 
         const int j = j0 + i * xin.vec_step();
         if (j < D) {
           float2 f[VEC / 2], g[VEC / 2];
-          xin.get(at, i, first, f);
-          gin.get(at, i, first, g);
+          xin.get(at, i, f);
+          gin.get(at, i, g);
 #pragma unroll
           for (int k = 0; k < VEC / 2; ++k) f[k] = fma2(mul2(g[k], wf[i][k]), both(rstd), fma2(add2(f[k], both(-mean)), both(A), both(B)));
-          if (EDGE) store_part<VEC>(out + i * xin.vec_step(), j, D, f); else store_vec(out + i * xin.vec_step(), f);
+          if (EDGE) store_at<VEC, decltype(xin)>(out + i * xin.vec_step(), i, j, D, f); else store_vec(out + i * xin.vec_step(), f);
         }
       }
     }
@@ -718,15 +761,11 @@ static RowPlan plan_rows(int64_t D, int vec, int most) {
   return p;
 }
 
-// Blocks a SM of the backward pass, each of which leaves a part of dw and db in the scratch: at most this many.
-constexpr int LN_MOST_PER_SM = 8;
-
 // Blocks of the row kernels: as many as stay resident (in the backward pass more are slower: 65536 x 1024 bf16 72 us with these, 80 with
 // twice and 90 with four times as many).  Where rows do not all start on a 16-byte boundary, a group's rows have to be a multiple of 8 apart.
-static unsigned row_blocks(const RowPlan& p, int64_t rows, int64_t D, int vec, int resident_threads, int most_per_sm, int turns) {
-  const int64_t groups = p.block ? 1 : LN_WARP_THREADS / p.T, threads = p.block ? p.T : LN_WARP_THREADS;
-  const int64_t want = (rows + groups - 1) / groups, per_sm = imin64(resident_threads / threads < 1 ? 1 : resident_threads / threads, most_per_sm);
-  int64_t most = per_sm * sm_count();
+static unsigned row_blocks(const RowPlan& p, int64_t rows, int64_t D, int vec, int per_sm, int turns) {
+  const int64_t groups = p.block ? 1 : LN_WARP_THREADS / p.T, want = (rows + groups - 1) / groups;
+  int64_t most = static_cast<int64_t>(per_sm) * sm_count();
   if (turns > 1) most *= want / (4 * most) < 1 ? 1 : imin64(want / (4 * most), turns);
   if (want <= most) return static_cast<unsigned>(want);
   return static_cast<unsigned>(D % vec == 0 ? most : most < 8 ? 8 : most / 8 * 8);
@@ -736,18 +775,33 @@ static bool in_vectors(const void* p, int64_t ld, int64_t D, int vec, int64_t by
   return reinterpret_cast<uintptr_t>(p) % bytes == 0 && (ld - D) % vec == 0;
 }
 
-// Dynamic shared memory of a kernel, allowed once per device.
+// A kernel on the devices it was used on: its dynamic shared memory is allowed once on each.
+struct KernelState {
+  std::atomic<uint64_t> allowed{0};
+  std::atomic<int> regs{0};
+};
 template <class K>
-static int allow_slots(K kernel, std::atomic<uint64_t>& allowed) {
+static int allow_slots(K kernel, KernelState& state) {
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t bit = uint64_t(1) << (dev & 63);
-  if (dev < 64 && (allowed.load(std::memory_order_acquire) & bit)) return HASTE_OK;
+  if (dev < 64 && (state.allowed.load(std::memory_order_acquire) & bit)) return HASTE_OK;
   if (int rc = allow_dynamic_smem(kernel)) return rc;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-  if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaFuncSetAttribute(carveout): %s", cudaGetErrorString(e));
-  if (dev < 64) allowed.fetch_or(bit, std::memory_order_release);
+  cudaFuncAttributes attr;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, kernel);
+  if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "layer norm: attributes of a kernel: %s", cudaGetErrorString(e));
+  state.regs.store(attr.numRegs, std::memory_order_relaxed);
+  if (dev < 64) state.allowed.fetch_or(bit, std::memory_order_release);
   return HASTE_OK;
+}
+// Blocks that stay resident on a SM: a quarter of its 64 K registers to each scheduler, in units of 8 a thread; 228 KB of shared memory, of
+// which a block takes 1 KB more than its own.  One block more has a turn to itself: 131072 x 512 bf16 forward 48 us with the 5 that fit, 65
+// with 6; 32768 x 1024 fp32 backward 62 and 74.
+static int resident_blocks(const KernelState& state, int threads, int smem) {
+  const int regs = (state.regs.load(std::memory_order_relaxed) + 7) / 8 * 8, warps = 16384 / (32 * (regs > 0 ? regs : 8)) * 4;
+  const int by_regs = (warps < 64 ? warps : 64) / (threads / 32), by_smem = 228 * 1024 / (smem + 1024 + 256);
+  return by_regs < 1 ? 1 : by_regs < by_smem ? by_regs : by_smem < 1 ? 1 : by_smem;
 }
 
 template <class X, class W>
@@ -768,14 +822,14 @@ struct FwdCall {
 
 template <class X, int VEC, int NV, int MODE, bool EDGE>
 static int ln_fwd_rows(const FwdCall& c, const RowPlan& p) {
-  static std::atomic<uint64_t> allowed{0};
+  static KernelState state;
   const int threads = MODE == BLOCK ? p.T : LN_WARP_THREADS, smem = LN_STAGES * NV * threads * VEC * static_cast<int>(sizeof(X));
-  if (int rc = allow_slots(ln_fwd_kernel<X, VEC, NV, MODE, EDGE>, allowed)) return rc;
+  if (int rc = allow_slots(ln_fwd_kernel<X, VEC, NV, MODE, EDGE>, state)) return rc;
   // Where D is a multiple of VEC and a thread has 3 vectors or more, up to 4 times (fp32: 8 times) as many blocks as stay resident, each with
   // at least 4 rows to a group: started in order they stay closer together in memory than blocks that walk over all of it (65536 x 1024
   // bf16 51 -> 47 us, fp32 99 -> 81).  With fewer vectors, or weights to be loaded one by one, starting up costs more than that.
   const int turns = !EDGE && NV >= 3 ? (sizeof(X) == 2 ? 4 : 8) : 1;
-  const unsigned blocks = row_blocks(p, c.rows, c.D, VEC, VEC * NV > 16 ? 512 : VEC * NV > 8 ? 768 : 1024, 32, turns);
+  const unsigned blocks = row_blocks(p, c.rows, c.D, VEC, resident_blocks(state, threads, smem), turns);
   ln_fwd_kernel<X, VEC, NV, MODE, EDGE><<<blocks, threads, smem, c.st>>>((const X*)c.x, c.w, c.b, c.w_type, (X*)c.y, c.mean, c.rstd, c.rows, static_cast<int>(c.D), c.ldx,
                                                                     c.eps, p.T, in_vectors(c.x, c.ldx, c.D, VEC, 16), aligned16(c.w) && aligned16(c.b));
   return check_launch("layer_norm_forward");
@@ -810,8 +864,12 @@ int launch_layer_norm_forward(const void* x, const void* w, const void* b, void*
   return x_type == HASTE_BF16 ? ln_fwd<__nv_bfloat16>(c) : ln_fwd<float>(c);
 }
 
-// Threads that stay resident on a SM with `per_thread` elements each, in the backward pass.
-constexpr int bwd_resident(int per_thread) { return per_thread > 16 ? 384 : per_thread > 8 ? 512 : 1024; }
+// Blocks a SM of the backward pass, each of which leaves a part of dw and db in the scratch, with `per_thread` elements to a thread: at most
+// this many, whatever registers and shared memory would allow.
+static int bwd_most_blocks(const RowPlan& p, int per_thread) {
+  const int threads = p.block ? p.T : LN_WARP_THREADS, most = (per_thread > 16 ? 384 : per_thread > 8 ? 512 : 1024) / threads;
+  return most < 1 ? 1 : most < 8 ? most : 8;
+}
 // Threads of a block that a row may take there: with 8 elements a vector, more would leave too few registers.
 constexpr int bwd_most(int vec) { return vec == 8 ? 256 : 512; }
 
@@ -823,7 +881,7 @@ int64_t layer_norm_backward_scratch(int64_t rows, int64_t D) {
   for (int vec = 4; vec <= 8; vec += 4) {              // fp32 and bf16 rows
     const RowPlan p = plan_rows(D, vec, bwd_most(vec));
     if (!p.wide && rows > 0) {
-      const int64_t n = row_blocks(p, rows, D, vec, bwd_resident(vec * p.nv), LN_MOST_PER_SM, 1);
+      const int64_t n = row_blocks(p, rows, D, vec, bwd_most_blocks(p, vec * p.nv), 1);
       const int64_t elements = n * row_units(D, vec) * vec;
       if (elements > most) most = elements;
     }
@@ -854,14 +912,15 @@ struct BwdCall {
 
 template <class X, class G, int VEC, int NV, int MODE, bool EDGE, int STAGES = 4>
 static int ln_bwd_rows(const BwdCall& c, const RowPlan& p, float* partial, Parts& parts) {
-  static std::atomic<uint64_t> allowed{0};
+  static KernelState state;
   const int threads = MODE == BLOCK ? p.T : LN_WARP_THREADS;
   if constexpr (MODE == BLOCK && STAGES == 4 && VEC * sizeof(G) == 16)          // fp32 rows of more than 6144 elements: 4 stages do not fit
     if (STAGES * NV * threads * VEC * static_cast<int>(sizeof(X) + sizeof(G)) > DYN_SMEM_MAX) return ln_bwd_rows<X, G, VEC, NV, MODE, EDGE, 3>(c, p, partial, parts);
   const int slots = STAGES * NV * threads * VEC * static_cast<int>(sizeof(X) + sizeof(G));
   const int cols = MODE == BLOCK ? 0 : LN_WARP_THREADS / 32 * static_cast<int>(c.D) * 4, smem = slots > cols ? slots : cols;
-  if (int rc = allow_slots(ln_bwd_kernel<X, G, VEC, NV, MODE, EDGE, STAGES>, allowed)) return rc;
-  const unsigned blocks = row_blocks(p, c.rows, c.D, VEC, bwd_resident(VEC * NV), LN_MOST_PER_SM, 1);
+  if (int rc = allow_slots(ln_bwd_kernel<X, G, VEC, NV, MODE, EDGE, STAGES>, state)) return rc;
+  const int per_sm = resident_blocks(state, threads, smem), most = bwd_most_blocks(p, VEC * NV);
+  const unsigned blocks = row_blocks(p, c.rows, c.D, VEC, per_sm < most ? per_sm : most, 1);
   parts = Parts{static_cast<int>(blocks), row_units(c.D, VEC) * VEC, static_cast<unsigned>(c.D), MODE == BLOCK && EDGE ? VEC - 1 : 0u};
   const int64_t g_bytes = VEC * sizeof(G) < 16 ? 8 : 16;
   ln_bwd_kernel<X, G, VEC, NV, MODE, EDGE, STAGES><<<blocks, threads, smem, c.st>>>((const G*)c.dy, (const X*)c.x, c.w, c.w_type, c.mean, c.rstd, (X*)c.dx, partial, c.rows,
