@@ -742,14 +742,14 @@ struct RowPlan {
   int nv = 1, T = 32;
 };
 // most: threads of a block that a row may take
-static RowPlan plan_rows(int64_t D, int vec, int most) {
+static RowPlan plan_rows(int64_t D, int vec, int most, bool few) {
   RowPlan p;
   const int64_t units = row_units(D, vec);
   if (units <= 32 * 4) {
-    // the fewest threads with at most 2 vectors each: a group of few lanes leaves the others to more rows
     p.T = 1;
-    while (p.T < 32 && p.T * 2 < units) p.T *= 2;
+    while (p.T < 32 && p.T * 4 < units) p.T *= 2;
     p.nv = static_cast<int>((units + p.T - 1) / p.T);
+    if (p.T < 32 && (p.nv == 3 ? few : p.nv > 1 && D % vec == 0)) { p.T *= 2; p.nv = p.nv / 2 + (p.nv & 1); }
     return p;
   }
   p.block = true;
@@ -840,6 +840,7 @@ static int ln_fwd_plan(const FwdCall& c, const RowPlan& p) {
   if (p.block) return p.nv == 3 ? ln_fwd_rows<X, VEC, 3, BLOCK, EDGE>(c, p) : ln_fwd_rows<X, VEC, 4, BLOCK, EDGE>(c, p);
   if (p.nv == 1) return ln_fwd_rows<X, VEC, 1, SUB, EDGE>(c, p);
   if (p.nv == 2) return ln_fwd_rows<X, VEC, 2, SUB, EDGE>(c, p);
+  if (p.T < 32) return p.nv == 3 ? ln_fwd_rows<X, VEC, 3, SUB, EDGE>(c, p) : ln_fwd_rows<X, VEC, 4, SUB, EDGE>(c, p);
   if (p.nv == 3) return ln_fwd_rows<X, VEC, 3, FULL, EDGE>(c, p);
   return ln_fwd_rows<X, VEC, 4, FULL, EDGE>(c, p);
 }
@@ -848,7 +849,7 @@ template <class X>
 static int ln_fwd(const FwdCall& c) {
   if (c.rows == 0) return HASTE_OK;
   constexpr int VEC = 16 / sizeof(X);
-  RowPlan p = plan_rows(c.D, VEC, 512);
+  RowPlan p = plan_rows(c.D, VEC, 512, VEC == 4 && c.D % VEC == 0);
   if (!aligned16(c.y)) p.wide = true;
   if (p.wide) {
     using B = __nv_bfloat16;
@@ -879,7 +880,7 @@ static int64_t wide_parts(int64_t rows) { return rows < 16 * 64 ? (rows + 63) / 
 int64_t layer_norm_backward_scratch(int64_t rows, int64_t D) {
   int64_t most = wide_parts(rows) * D;
   for (int vec = 4; vec <= 8; vec += 4) {              // fp32 and bf16 rows
-    const RowPlan p = plan_rows(D, vec, bwd_most(vec));
+    const RowPlan p = plan_rows(D, vec, bwd_most(vec), false);
     if (!p.wide && rows > 0) {
       const int64_t n = row_blocks(p, rows, D, vec, bwd_most_blocks(p, vec * p.nv), 1);
       const int64_t elements = n * row_units(D, vec) * vec;
@@ -934,6 +935,7 @@ static int ln_bwd_plan(const BwdCall& c, const RowPlan& p, float* partial, Parts
   if (p.block) return p.nv == 3 ? ln_bwd_rows<X, G, VEC, 3, BLOCK, EDGE>(c, p, partial, parts) : ln_bwd_rows<X, G, VEC, 4, BLOCK, EDGE>(c, p, partial, parts);
   if (p.nv == 1) return ln_bwd_rows<X, G, VEC, 1, SUB, EDGE>(c, p, partial, parts);
   if (p.nv == 2) return ln_bwd_rows<X, G, VEC, 2, SUB, EDGE>(c, p, partial, parts);
+  if (p.T < 32) return p.nv == 3 ? ln_bwd_rows<X, G, VEC, 3, SUB, EDGE>(c, p, partial, parts) : ln_bwd_rows<X, G, VEC, 4, SUB, EDGE>(c, p, partial, parts);
   if (p.nv == 3) return ln_bwd_rows<X, G, VEC, 3, FULL, EDGE>(c, p, partial, parts);
   return ln_bwd_rows<X, G, VEC, 4, FULL, EDGE>(c, p, partial, parts);
 }
@@ -960,7 +962,7 @@ static int ln_bwd(const BwdCall& c) {
   float* partial = want ? c.scratch : nullptr;
   Parts parts{0, c.D, 0u, 0u};
   if (c.rows > 0) {
-    RowPlan p = plan_rows(c.D, VEC, bwd_most(VEC));
+    RowPlan p = plan_rows(c.D, VEC, bwd_most(VEC), false);
     if (!aligned16(c.dx)) p.wide = true;
     int rc = HASTE_OK;
     if (p.wide) {
