@@ -741,7 +741,11 @@ struct RowPlan {
   bool wide = false, block = false;
   int nv = 1, T = 32;
 };
-// most: threads of a block that a row may take
+// most: threads of a block that a row may take; few: no 3 vectors in part of a warp.
+// Within a warp: as few lanes as 4 vectors each allow, which leaves the others to more rows.  Whole vectors want twice the lanes with
+// half of them each (bf16 rows of 64 elements, 134 MB: forward 45 us and 60, backward 79 and 95; 256 elements 46 and 48, the same), rows that are
+// cut do not (101 elements fp32: 63 us and 49, 89 and 78).  3 vectors stay 3 (384 elements bf16: 49 us in 16 lanes, 62 with 2 vectors in 32; backward
+// 75 and 100), but in the forward pass over whole vectors of fp32 (96 elements: 51 us, 47 with 2).
 static RowPlan plan_rows(int64_t D, int vec, int most, bool few) {
   RowPlan p;
   const int64_t units = row_units(D, vec);
