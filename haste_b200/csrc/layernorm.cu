@@ -325,9 +325,11 @@ __device__ __forceinline__ void store_part(T* p, int j0, int D, const float2 (&f
   if ((!HEAD || j0 >= 0) && (!TAIL || j0 + VEC <= D)) store_vec(p, f);
   else if (HEAD && j0 < 0 && j0 + VEC <= D) store_head(p, -j0, f);
   else if (TAIL && j0 >= 0) store_tail(p, D - j0, f);
-  else if (HEAD && TAIL) {                                             // both: D < VEC
+  else {
+    if constexpr (HEAD && TAIL) {                                      // both: D < VEC
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) if (static_cast<unsigned>(j0 + k) < static_cast<unsigned>(D)) st_f(p + k, k & 1 ? f[k / 2].y : f[k / 2].x);
+      for (int k = 0; k < VEC; ++k) if (static_cast<unsigned>(j0 + k) < static_cast<unsigned>(D)) st_f(p + k, k & 1 ? f[k / 2].y : f[k / 2].x);
+    }
   }
 }
 
@@ -493,19 +495,45 @@ struct Feed {
   }
 };
 
+// Factors 1 and 0 of a vector's elements that belong to the row and that do not, in shared memory: entry n <= VEC has the first n,
+// entry VEC + s the elements s and following, entry 2 VEC + s elements s .. s + D - 1 (a row within a vector).
+template <int VEC>
+struct EdgeTable {
+  static constexpr int ENTRIES = 3 * VEC;
+  float4 q[ENTRIES][VEC / 4];
+  __device__ __forceinline__ void fill(int D) {
+    for (int i = threadIdx.x; i < ENTRIES * VEC; i += blockDim.x) {
+      const int e = i / VEC, k = i % VEC, s = e % VEC;
+      reinterpret_cast<float*>(q)[i] = (e <= VEC ? k < e : e < 2 * VEC ? k >= s : k >= s && k < s + D) ? 1.f : 0.f;
+    }
+  }
+  static __device__ __forceinline__ int entry(int j, int D) {             // of the vector that begins at column j, in bytes
+    const int n = min(max(D - j, 0), VEC);
+    return (j >= 0 ? n : D - j >= VEC ? VEC - j : 2 * VEC - j) * VEC * 4;
+  }
+  __device__ __forceinline__ const float4& get(int at, int k) const { return *reinterpret_cast<const float4*>(reinterpret_cast<const char*>(q) + at + 16 * k); }
+};
+
 template <int VEC, class FEED, class T>
 __device__ __forceinline__ void store_at(T* p, int i, int j, int D, const float2 (&f)[VEC / 2]) {
   if (i == 0) { if (FEED::may_end(0)) store_part<VEC, true, true>(p, j, D, f); else store_part<VEC, true, false>(p, j, D, f); }
   else { if (FEED::may_end(i)) store_part<VEC, false, true>(p, j, D, f); else store_vec(p, f); }
 }
 
+// Blocks of at most LN_WARP_THREADS: 4 on a SM, but 3 with 4 vectors of 8 elements where rows are cut (67041 x 1001 68 us with 4, for which the registers
+// do not suffice, 49 with 3; with 3 vectors a thread 68 and 74).
+// The factors of cut rows (EdgeTable) are read where a vector has 8 elements: 130816 x 513 bf16 68 us, 94 with comparisons; with 4 elements these cost
+// less (332222 x 101 fp32 51 and 49).
 // EDGE: D is no multiple of VEC, rows have first and last vectors that are theirs in part.
 template <class X, int VEC, int NV, int MODE, bool EDGE>
-__global__ void __launch_bounds__(MODE == BLOCK ? 512 : LN_WARP_THREADS, MODE == BLOCK ? 1 : 4)
+__global__ void __launch_bounds__(MODE == BLOCK ? 512 : LN_WARP_THREADS, MODE == BLOCK ? 1 : EDGE && VEC * NV > 24 ? 3 : 4)
     ln_fwd_kernel(const X* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b, int w_type, X* __restrict__ y, float* __restrict__ mean_out,
                   float* __restrict__ rstd_out, int64_t rows, int D, int64_t ldx, float eps, int t, bool x_vec, bool w_vec) {
   __shared__ __align__(16) float buf[2][2][16];
   extern __shared__ __align__(16) char slots[];
+  constexpr bool TABLE = EDGE && VEC == 8;
+  __shared__ EdgeTable<VEC> edges;
+  if (TABLE) { edges.fill(D); __syncthreads(); }
   RowGroup<MODE, NV> grp(t);
   grp.clear(buf);
   const float inv_d = 1.f / static_cast<float>(D), part = power_below(D), inv_dp = 1.f / (static_cast<float>(D) * part);
@@ -523,6 +551,9 @@ __global__ void __launch_bounds__(MODE == BLOCK ? 512 : LN_WARP_THREADS, MODE ==
     load_weights<VEC>(w, w_type, !EDGE && w_vec, j0 + i * in.vec_step(), D, 1.f, wf[i]);
     load_weights<VEC>(b, w_type, !EDGE && w_vec, j0 + i * in.vec_step(), D, 0.f, bf[i]);
   }
+  int edge_at[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) edge_at[i] = TABLE ? EdgeTable<VEC>::entry(j0 + i * in.vec_step(), D) : 0;
   X* out = y + r * D + j0;
   for (int at = 0, next_at = all - stage_bytes; left > 0; left -= stride, r += stride, out += stride * D) {
     copies_wait<LN_STAGES - 2>();
@@ -541,21 +572,29 @@ __global__ void __launch_bounds__(MODE == BLOCK ? 512 : LN_WARP_THREADS, MODE ==
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = j0 + i * in.vec_step();
-      float2 d[VEC / 2];
-#pragma unroll
-      for (int k = 0; k < VEC / 2; ++k) d[k] = f[i][k] = add2(f[i][k], both(-mean));
       // what is not the row's counts for nothing
-      if (EDGE && i == 0) {
+      if (TABLE && (i == 0 || in.may_end(i))) {
 #pragma unroll
-        for (int k = 0; k < VEC / 2; ++k) { d[k].x = 2 * k < first ? 0.f : d[k].x; d[k].y = 2 * k + 1 < first ? 0.f : d[k].y; }
-      }
-      if (EDGE && in.may_end(i)) {
+        for (int q = 0; q < VEC / 4; ++q) {
+          const float4 ours = edges.get(edge_at[i], q);
+          f[i][2 * q] = fma2(make_float2(ours.x, ours.y), both(-mean), f[i][2 * q]);
+          f[i][2 * q + 1] = fma2(make_float2(ours.z, ours.w), both(-mean), f[i][2 * q + 1]);
+        }
+      } else {
 #pragma unroll
-        for (int k = 0; k < VEC / 2; ++k) { d[k].x = j + 2 * k < D ? d[k].x : 0.f; d[k].y = j + 2 * k + 1 < D ? d[k].y : 0.f; }
+        for (int k = 0; k < VEC / 2; ++k) f[i][k] = add2(f[i][k], both(-mean));
+        if (EDGE && i == 0) {
+#pragma unroll
+          for (int k = 0; k < VEC / 2; ++k) { f[i][k].x = 2 * k < first ? 0.f : f[i][k].x; f[i][k].y = 2 * k + 1 < first ? 0.f : f[i][k].y; }
+        }
+        if (EDGE && in.may_end(i)) {
+#pragma unroll
+          for (int k = 0; k < VEC / 2; ++k) { f[i][k].x = j + 2 * k < D ? f[i][k].x : 0.f; f[i][k].y = j + 2 * k + 1 < D ? f[i][k].y : 0.f; }
+        }
       }
       if (EDGE || j < D) {
 #pragma unroll
-        for (int k = 0; k < VEC / 2; ++k) { if (k & 1) s2 = fma2(d[k], d[k], s2); else s1 = fma2(d[k], d[k], s1); }
+        for (int k = 0; k < VEC / 2; ++k) { if (k & 1) s2 = fma2(f[i][k], f[i][k], s2); else s1 = fma2(f[i][k], f[i][k], s1); }
       }
     }
     s1 = add2(s1, s2);
@@ -782,7 +821,7 @@ static bool in_vectors(const void* p, int64_t ld, int64_t D, int vec, int64_t by
 // A kernel on the devices it was used on: its dynamic shared memory is allowed once on each.
 struct KernelState {
   std::atomic<uint64_t> allowed{0};
-  std::atomic<int> regs{0};
+  std::atomic<int> regs{0}, smem{0};      // of a thread; of a block, static
 };
 template <class K>
 static int allow_slots(K kernel, KernelState& state) {
@@ -796,6 +835,7 @@ static int allow_slots(K kernel, KernelState& state) {
   if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, kernel);
   if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "layer norm: attributes of a kernel: %s", cudaGetErrorString(e));
   state.regs.store(attr.numRegs, std::memory_order_relaxed);
+  state.smem.store(static_cast<int>(attr.sharedSizeBytes), std::memory_order_relaxed);
   if (dev < 64) state.allowed.fetch_or(bit, std::memory_order_release);
   return HASTE_OK;
 }
@@ -804,7 +844,7 @@ static int allow_slots(K kernel, KernelState& state) {
 // with 6; 32768 x 1024 fp32 backward 62 and 74.
 static int resident_blocks(const KernelState& state, int threads, int smem) {
   const int regs = (state.regs.load(std::memory_order_relaxed) + 7) / 8 * 8, warps = 16384 / (32 * (regs > 0 ? regs : 8)) * 4;
-  const int by_regs = (warps < 64 ? warps : 64) / (threads / 32), by_smem = 228 * 1024 / (smem + 1024 + 256);
+  const int by_regs = (warps < 64 ? warps : 64) / (threads / 32), by_smem = 228 * 1024 / (smem + state.smem.load(std::memory_order_relaxed) + 1024);
   return by_regs < 1 ? 1 : by_regs < by_smem ? by_regs : by_smem < 1 ? 1 : by_smem;
 }
 
@@ -844,7 +884,10 @@ static int ln_fwd_plan(const FwdCall& c, const RowPlan& p) {
   if (p.block) return p.nv == 3 ? ln_fwd_rows<X, VEC, 3, BLOCK, EDGE>(c, p) : ln_fwd_rows<X, VEC, 4, BLOCK, EDGE>(c, p);
   if (p.nv == 1) return ln_fwd_rows<X, VEC, 1, SUB, EDGE>(c, p);
   if (p.nv == 2) return ln_fwd_rows<X, VEC, 2, SUB, EDGE>(c, p);
-  if (p.T < 32) return p.nv == 3 ? ln_fwd_rows<X, VEC, 3, SUB, EDGE>(c, p) : ln_fwd_rows<X, VEC, 4, SUB, EDGE>(c, p);
+  if (p.T < 32) {                       // (whole vectors: 3 only of 8 elements, and never 4)
+    if constexpr (EDGE) return p.nv == 3 ? ln_fwd_rows<X, VEC, 3, SUB, EDGE>(c, p) : ln_fwd_rows<X, VEC, 4, SUB, EDGE>(c, p);
+    else if constexpr (VEC == 8) return ln_fwd_rows<X, VEC, 3, SUB, EDGE>(c, p);
+  }
   if (p.nv == 3) return ln_fwd_rows<X, VEC, 3, FULL, EDGE>(c, p);
   return ln_fwd_rows<X, VEC, 4, FULL, EDGE>(c, p);
 }
@@ -939,7 +982,10 @@ static int ln_bwd_plan(const BwdCall& c, const RowPlan& p, float* partial, Parts
   if (p.block) return p.nv == 3 ? ln_bwd_rows<X, G, VEC, 3, BLOCK, EDGE>(c, p, partial, parts) : ln_bwd_rows<X, G, VEC, 4, BLOCK, EDGE>(c, p, partial, parts);
   if (p.nv == 1) return ln_bwd_rows<X, G, VEC, 1, SUB, EDGE>(c, p, partial, parts);
   if (p.nv == 2) return ln_bwd_rows<X, G, VEC, 2, SUB, EDGE>(c, p, partial, parts);
-  if (p.T < 32) return p.nv == 3 ? ln_bwd_rows<X, G, VEC, 3, SUB, EDGE>(c, p, partial, parts) : ln_bwd_rows<X, G, VEC, 4, SUB, EDGE>(c, p, partial, parts);
+  if (p.T < 32) {                       // (whole vectors: never 4)
+    if constexpr (EDGE) return p.nv == 3 ? ln_bwd_rows<X, G, VEC, 3, SUB, EDGE>(c, p, partial, parts) : ln_bwd_rows<X, G, VEC, 4, SUB, EDGE>(c, p, partial, parts);
+    else return ln_bwd_rows<X, G, VEC, 3, SUB, EDGE>(c, p, partial, parts);
+  }
   if (p.nv == 3) return ln_bwd_rows<X, G, VEC, 3, FULL, EDGE>(c, p, partial, parts);
   return ln_bwd_rows<X, G, VEC, 4, FULL, EDGE>(c, p, partial, parts);
 }
