@@ -3,15 +3,17 @@
 PyTorch is used for device memory and streams only.  Every function validates what the C side cannot
 see (device, dtype, contiguity) and raises RuntimeError otherwise.
 """
-import array
 import contextlib
-import functools
-import operator
+import ctypes
 
 import torch
 
 from . import _lib
 from ._lib import lib, check
+try:
+    from . import _dense
+except ImportError as e:
+    raise ImportError(f"haste_b200._dense does not load ({e}): run `python -m haste_b200.build` (with --force after torch was replaced)") from e
 
 
 def _stream(t):
@@ -391,256 +393,56 @@ def topk_update(z, C, col0, vals, idx):
         check(lib.haste_topk_update(_ptr(z), z.stride(0), B, C, col0, k, _ptr(vals), _ptr(idx), _stream(z)), "topk_update")
 
 
-# ---------------------------------------------------------------- layer norm
-_TYPES = {torch.bfloat16: _lib.BF16, torch.float32: _lib.FP32}
-_current_device = getattr(torch._C, "_cuda_getDevice", None)
+# ---------------------------------------------------------------- layer norm, AdamW, gradient norm
+# (arguments are checked, outputs allocated and the library called by the extension module, csrc/dense_binding.cpp)
+_dense.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+    "haste_last_error_string", "haste_layer_norm_forward", "haste_layer_norm_backward_scratch", "haste_layer_norm_backward", "haste_adamw_step",
+    "haste_grad_norm", "haste_dequantize_moment")))
 
-
-def _type_of(t, name):
-    code = _TYPES.get(t.dtype)
-    if code is None:
-        raise RuntimeError(f"{name} must be torch.bfloat16 or torch.float32, got {t.dtype}")
-    return code
-
-
-def _call(dev, what, fn, *args):
-    """``fn(*args, stream)`` on the current stream of device number ``dev``, with that device current."""
-    if _current_device() == dev:
-        rc = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _raw_stream(dev))
-    if rc:
-        check(rc, what)
-
-
-def _rows_of(t, D):
-    """``t`` [..., D] as rows of unit column stride, and their stride; copied only where no such view exists."""
-    if t.is_contiguous():
-        return t, D
-    t = t.reshape(-1, D)
-    if D > 1 and t.stride(1) != 1:
-        t = t.contiguous()
-    return t, (t.stride(0) if t.shape[0] > 1 else D)
-
-
-def _check_x(x):
-    """(device number, D, type) of x [..., D]."""
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        raise RuntimeError("x must be a CUDA tensor (this library has no CPU path)")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise RuntimeError(f"x must be [..., D] with D >= 1, got {tuple(x.shape)}")
-    return x.get_device(), x.shape[-1], _type_of(x, "x")
-
-
-def _check_norm_parameter(t, name, dev, D):
-    """Element type of weight or bias [D]."""
-    if t.get_device() != dev:
-        raise RuntimeError(f"{name} must be a CUDA tensor on cuda:{dev}, as x is, got {t.device}")
-    if t.dim() != 1 or t.shape[0] != D or not t.is_contiguous():
-        raise RuntimeError(f"{name} must be a contiguous [{D}], got {tuple(t.shape)}")
-    return _type_of(t, name)
+MOMENT_BLOCK = 256           # elements of a moment that share a scale; every tensor's moments start at a multiple of it
 
 
 def layer_norm_forward(x, weight, bias, eps=1e-5, stats=True):
     """Layer norm over the last dimension of ``x`` [..., D] (bf16 or fp32; any strides, copied if its rows are not of unit
     stride): ``(y, mean, rstd)``, y of x's type, the statistics fp32 [...]; y alone with ``stats=False`` (inference).
     ``weight`` and ``bias``: [D], bf16 or fp32 whatever x is, or None."""
-    dev, D, x_type = _check_x(x)
-    w_type, w, b = None, 0, 0
-    if weight is not None:
-        w_type, w = _check_norm_parameter(weight, "weight", dev, D), weight.data_ptr()
-    if bias is not None:
-        b_type, b = _check_norm_parameter(bias, "bias", dev, D), bias.data_ptr()
-        if w_type is None:
-            w_type = b_type
-        elif w_type != b_type:
-            raise RuntimeError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
-    src, ldx = _rows_of(x, D)
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    if not stats:
-        _call(dev, "layer_norm_forward", lib.haste_layer_norm_forward, src.data_ptr(), w, b, y.data_ptr(), 0, 0, x.numel() // D, D, ldx, eps, x_type,
-              w_type or 0)
-        return y
-    rows = x.numel() // D
-    mean = torch.empty(rows, dtype=torch.float32, device=dev)
-    rstd = torch.empty_like(mean)
-    _call(dev, "layer_norm_forward", lib.haste_layer_norm_forward, src.data_ptr(), w, b, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), rows, D, ldx, eps, x_type,
-          w_type or 0)
-    if x.dim() != 2:
-        mean, rstd = mean.view(x.shape[:-1]), rstd.view(x.shape[:-1])
-    return y, mean, rstd
-
-
-@functools.lru_cache(maxsize=4096)
-def _norm_scratch_bytes(dev, rows, D):
-    with torch.cuda.device(dev):
-        return lib.haste_layer_norm_backward_scratch(rows, D)
+    return _dense.layer_norm_forward(x, weight, bias, eps, stats)
 
 
 def layer_norm_backward(dy, x, weight, mean, rstd, want_weight=True, want_bias=True, param_dtype=None):
     """``(dx, dweight, dbias)`` of ``layer_norm_forward``: dx of x's type, the other two of ``param_dtype`` (default: the weight's type,
     x's without a weight), None where not wanted.  ``dy`` [..., D] is bf16 or fp32, whatever x is; a broadcast gradient (row stride 0) is
     read in place.  The sums over rows are fp32 and give the same bits on every call."""
-    dev, D, x_type = _check_x(x)
-    rows = x.numel() // D
-    if not isinstance(dy, torch.Tensor) or dy.get_device() != dev or dy.shape != x.shape:
-        raise RuntimeError(f"dy must be a CUDA tensor of x's shape {tuple(x.shape)} on {x.device}")
-    dy_type = _type_of(dy, "dy")
-    for name, t in (("mean", mean), ("rstd", rstd)):
-        if t.get_device() != dev or t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous():
-            raise RuntimeError(f"{name} must be contiguous and hold {rows} fp32 values on {x.device}")
-    if weight is None:
-        param_dtype = param_dtype or x.dtype
-        w, w_type = 0, _TYPES.get(param_dtype)
-    else:
-        w, w_type = weight.data_ptr(), _check_norm_parameter(weight, "weight", dev, D)
-        param_dtype = param_dtype or weight.dtype
-        if param_dtype != weight.dtype:
-            w_type = None
-    if w_type is None:
-        raise RuntimeError(f"param_dtype must be the weight's type, torch.bfloat16 or torch.float32, got {param_dtype}")
-    src, ldx = _rows_of(x, D)
-    grad, lddy = _rows_of(dy, D)
-    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
-    dw = db = scratch = None
-    n = 0
-    if want_weight:
-        dw = torch.empty(D, dtype=param_dtype, device=dev) if weight is None else torch.empty_like(weight)
-    if want_bias:
-        db = torch.empty(D, dtype=param_dtype, device=dev) if weight is None else torch.empty_like(weight)
-    if want_weight or want_bias:
-        n = _norm_scratch_bytes(dev, rows, D)
-        scratch = torch.empty(n, dtype=torch.uint8, device=dev)
-    _call(dev, "layer_norm_backward", lib.haste_layer_norm_backward, grad.data_ptr(), src.data_ptr(), w, mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), _ptr(dw),
-          _ptr(db), _ptr(scratch), n, rows, D, lddy, ldx, x_type, dy_type, w_type)
-    return dx, dw, db
-
-
-# ---------------------------------------------------------------- AdamW and gradient norm over many tensors
-MOMENT_BLOCK = 256           # elements of a moment that share a scale; every tensor's moments start at a multiple of it
-
-# over a hundred tensors a call spends its time asking each of them: by these, without a Python loop
-_data_ptr, _get_device, _is_contiguous, _numel, _dim = torch.Tensor.data_ptr, torch.Tensor.get_device, torch.Tensor.is_contiguous, torch.Tensor.numel, torch.Tensor.dim
-_dtype = operator.attrgetter("dtype")
-
-
-def _tensor_list(tensors, what):
-    """(device number, array of device pointers) of a list of contiguous CUDA tensors on one device."""
-    devs = set(map(_get_device, tensors))
-    if len(devs) != 1 or min(devs) < 0:
-        raise RuntimeError(f"{what} must be CUDA tensors on one device (this library has no CPU path)")
-    if not all(map(_is_contiguous, tensors)):
-        raise RuntimeError(f"{what} must be contiguous")
-    return devs.pop(), array.array("Q", list(map(_data_ptr, tensors)))
-
-
-def _sizes(tensors):
-    return array.array("q", list(map(_numel, tensors)))
-
-
-def _present(tensors):
-    """The list, without its None if it has any."""
-    return [t for t in tensors if t is not None] if type(None) in set(map(type, tensors)) else tensors
-
-
-def _address(a):
-    return a.buffer_info()[0]
-
-
-def _norm_of(dev, ptrs, types, sizes, grad_scale):
-    buf = torch.empty(1 + _lib.GRAD_NORM_PARTIALS, dtype=torch.float32, device=dev)          # the norm and the kernel's scratch
-    norm = buf[0]
-    at = buf.data_ptr()
-    _call(dev, "grad_norm", lib.haste_grad_norm, _address(ptrs), _address(types), _address(sizes), len(ptrs), grad_scale, at + 4, at)
-    return norm
+    return _dense.layer_norm_backward(dy, x, weight, mean, rstd, want_weight, want_bias, param_dtype)
 
 
 def grad_norm(grads, grad_scale=1.0):
     """2-norm of all tensors of ``grads`` (bf16 or fp32, mixed or not; None is skipped) together, times |grad_scale|: fp32 scalar on the
     device, the same bits on every call."""
-    grads = _present(grads)
-    if not grads:
-        raise RuntimeError("grad_norm needs at least one tensor")
-    dev, ptrs = _tensor_list(grads, "gradients")
-    types = _TYPES.get(grads[0].dtype), set(map(_dtype, grads))
-    if not types[1] <= _TYPES.keys():
-        raise RuntimeError(f"gradients must be torch.bfloat16 or torch.float32, got {types[1]}")
-    types = array.array("i", [types[0]]) * len(grads) if len(types[1]) == 1 else array.array("i", map(_TYPES.__getitem__, map(_dtype, grads)))
-    return _norm_of(dev, ptrs, types, _sizes(grads), grad_scale)
+    return _dense.grad_norm(grads, grad_scale)
 
 
 def adamw_step(params, grads, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, bits, *, step, lr, betas, eps, weight_decay, grad_scale=1.0, norm=None,
                max_norm=None, seed=123, stream_index=0, flags=0):
     """One launch of the AdamW kernel (haste_adamw_step), behind those of the gradients' norm where ``max_norm`` is given and ``norm`` is not;
     returns that norm or None.  ``grads`` may hold None: that tensor is left alone."""
-    if len(params) != len(grads):
-        raise RuntimeError(f"{len(params)} parameters and {len(grads)} gradients")
-    there = _present(grads)
-    if not there:
-        return None                                      # nothing to do
-    gdev, gptrs = _tensor_list(there, "gradients")
-    g_sizes, g_dtype = _sizes(there), set(map(_dtype, there))
-    g_type = _type_of(there[0], "gradients")
-    if max_norm is None:
-        norm = None
-    elif norm is None:
-        if len(g_dtype) == 1:                            # (else refused below) the norm is on its way while the parameters are looked at
-            norm = _norm_of(gdev, gptrs, array.array("i", [g_type]) * len(gptrs), g_sizes, grad_scale)
-    elif norm.get_device() != gdev or norm.dtype != torch.float32 or norm.numel() != 1:
-        raise RuntimeError("norm must be one fp32 value on the parameters' device")
-    dev, ptrs = _tensor_list(params, "parameters")
-    if dev != gdev:
-        raise RuntimeError("parameters and gradients must be on one device")
-    sizes = _sizes(params)
-    all_gptrs, paired, paired_sizes = gptrs, params, sizes
-    if there is not grads:
-        paired = [p for p, g in zip(params, grads) if g is not None]
-        paired_sizes = _sizes(paired)
-        rest = iter(gptrs)
-        all_gptrs = array.array("Q", [0 if g is None else next(rest) for g in grads])
-    dims = list(map(_dim, paired))
-    if (len(set(map(_dtype, params))) != 1 or len(g_dtype) != 1 or dims != list(map(_dim, there)) or paired_sizes != g_sizes
-            or (max(dims) > 1 and any(d > 1 and p.shape != g.shape for d, p, g in zip(dims, paired, there)))):
-        raise RuntimeError("all parameters must have one type, all gradients one type, and every gradient its parameter's shape")
-    p_type = _type_of(params[0], "parameters")
-    moments = exp_avg.numel()
-    dtype = torch.float32 if bits == 32 else torch.uint8
-    for t in (exp_avg, exp_avg_sq):
-        if t.get_device() != dev or t.dtype != dtype or t.numel() != moments or not t.is_contiguous():
-            raise RuntimeError(f"both moments must be contiguous {dtype} tensors of one size on the parameters' device")
-    ms = vs = 0
-    if bits == 8:
-        for t in (exp_avg_scale, exp_avg_sq_scale):
-            if t.get_device() != dev or t.dtype != torch.float32 or t.numel() * MOMENT_BLOCK < moments or not t.is_contiguous():
-                raise RuntimeError(f"scales must be contiguous, fp32, one value per {MOMENT_BLOCK} elements of the moments, on the parameters' device")
-        ms, vs = exp_avg_scale.data_ptr(), exp_avg_sq_scale.data_ptr()
-    _call(dev, "adamw_step", lib.haste_adamw_step, _address(ptrs), _address(all_gptrs), _address(sizes), len(ptrs), exp_avg.data_ptr(), ms, exp_avg_sq.data_ptr(), vs,
-          moments, bits, p_type, g_type, float(lr), betas[0], betas[1], eps, weight_decay, step, grad_scale, max_norm or 0.0, _ptr(norm), seed & 0xFFFFFFFFFFFFFFFF,
-          stream_index, flags)
-    return norm
+    return _dense.adamw_step(params, grads, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, bits, step, lr, betas[0], betas[1], eps, weight_decay, grad_scale,
+                             norm, max_norm, seed, stream_index, flags)
 
 
 def quantize_moment(x, signed):
     """(codes uint8, scales fp32) of fp32 values, a multiple of 256 of them, rounded to the nearest code."""
     _req(x, "x", torch.float32)
-    dev = x.get_device()
-    codes = torch.empty(x.shape, dtype=torch.uint8, device=dev)
-    scales = torch.empty(x.numel() // MOMENT_BLOCK, dtype=torch.float32, device=dev)
-    _call(dev, "quantize_moment", lib.haste_quantize_moment, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.numel(), int(signed))
+    codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(x.numel() // MOMENT_BLOCK, dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        check(lib.haste_quantize_moment(_ptr(x), _ptr(codes), _ptr(scales), x.numel(), int(signed), _stream(x)), "quantize_moment")
     return codes, scales
 
 
 def dequantize_moment(codes, scales, signed, dtype=torch.float32):
-    _req(codes, "codes", torch.uint8); _req(scales, "scales", torch.float32)
-    if scales.numel() * MOMENT_BLOCK != codes.numel() or scales.device != codes.device:
-        raise RuntimeError(f"scales must hold one value per {MOMENT_BLOCK} codes, on their device")
-    if dtype not in _TYPES:
-        raise RuntimeError(f"dtype must be torch.bfloat16 or torch.float32, got {dtype}")
-    dev = codes.get_device()
-    out = torch.empty(codes.shape, dtype=dtype, device=dev)
-    _call(dev, "dequantize_moment", lib.haste_dequantize_moment, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), codes.numel(), int(signed), _TYPES[dtype])
-    return out
+    """The values (bf16 or fp32) that codes of 8 bits and their scales stand for."""
+    return _dense.dequantize_moment(codes, scales, signed, dtype)
 
 
 def check_locations(loc, D):

@@ -167,3 +167,20 @@ def test_optimizer_refuses_what_it_does_not_do():
     for kw in (dict(lr=-1.0), dict(weight_decay=-1.0), dict(betas=(0.9, 1.0)), dict(eps=0.0), dict(state_bits=4), dict(max_grad_norm=-1.0)):
         with pytest.raises(ValueError):
             AdamW([p], **kw)
+
+
+def test_the_extension_refuses_what_is_no_tensor():
+    from haste_b200 import ffi
+    from haste_b200.norm import layer_norm_backward, layer_norm_forward
+    from haste_b200.optim import adamw_step, grad_norm
+    t = torch.zeros(4)
+    for call in (lambda: layer_norm_forward(None, None, None), lambda: layer_norm_forward([1.0], None, None), lambda: layer_norm_backward(t, 3, t, t, t),
+                 lambda: grad_norm([t, "t"]), lambda: grad_norm([None, None]), lambda: grad_norm([]), lambda: adamw_step([t], [], t, t, step=1),
+                 lambda: adamw_step([t], [3], t, t, step=1), lambda: ffi.dequantize_moment(None, None, True)):
+        with pytest.raises(RuntimeError):
+            call()
+    for call in (lambda: grad_norm(t[0].item()), lambda: grad_norm([t], "1"), lambda: layer_norm_forward(t, None, None, "eps"), lambda: ffi._dense.grad_norm([t]),
+                 lambda: adamw_step([t], [t], t, t, step=1, lr="1")):
+        with pytest.raises((TypeError, RuntimeError)):
+            call()
+    assert adamw_step([t, t], [None, None], t, t, step=1) is None                    # nothing to do
