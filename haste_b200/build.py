@@ -63,7 +63,7 @@ def _build_dense(force):
     cmd += [src, "-o", made]
     for path in cpp_extension.library_paths():
         cmd += ["-L" + path]
-    cmd += ["-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    cmd += ["-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
     p = subprocess.run(cmd, capture_output=True, text=True)
     if p.returncode != 0:
         raise RuntimeError(f"compiling dense_binding.cpp failed:\n{p.stdout}\n{p.stderr}")

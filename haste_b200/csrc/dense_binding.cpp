@@ -8,6 +8,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -56,7 +57,10 @@ const at::Tensor& tensor(PyObject* o, const char* name) {
 }
 // On no device that this library runs on: -1
 int gpu_of(const at::Tensor& t) { return t.is_cuda() ? t.get_device() : -1; }
-at::Tensor empty_on(int dev, at::IntArrayRef sizes, at::ScalarType type) { return at::empty(sizes, at::TensorOptions().dtype(type).device(at::kCUDA, static_cast<c10::DeviceIndex>(dev))); }
+// (half a microsecond less than through the dispatcher; every output is written in full)
+at::Tensor empty_on(int dev, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::detail::empty_cuda(sizes, type, c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(dev)), std::nullopt);
+}
 void* address(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // f(stream) with device `dev` current, and without the interpreter's lock (a launch may have to wait for room in the stream)

@@ -422,14 +422,6 @@ def grad_norm(grads, grad_scale=1.0):
     return _dense.grad_norm(grads, grad_scale)
 
 
-def adamw_step(params, grads, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, bits, *, step, lr, betas, eps, weight_decay, grad_scale=1.0, norm=None,
-               max_norm=None, seed=123, stream_index=0, flags=0):
-    """One launch of the AdamW kernel (haste_adamw_step), behind those of the gradients' norm where ``max_norm`` is given and ``norm`` is not;
-    returns that norm or None.  ``grads`` may hold None: that tensor is left alone."""
-    return _dense.adamw_step(params, grads, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, bits, step, lr, betas[0], betas[1], eps, weight_decay, grad_scale,
-                             norm, max_norm, seed, stream_index, flags)
-
-
 def quantize_moment(x, signed):
     """(codes uint8, scales fp32) of fp32 values, a multiple of 256 of them, rounded to the nearest code."""
     _req(x, "x", torch.float32)

@@ -16,7 +16,7 @@ from torch.optim import Optimizer
 
 from . import _lib
 from . import ffi as _ffi
-from .ffi import MOMENT_BLOCK, grad_norm  # noqa: F401
+from .ffi import MOMENT_BLOCK, _dense, grad_norm  # noqa: F401
 
 
 class Quantized(NamedTuple):
@@ -57,9 +57,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step, lr=1e-3, betas=(0.9,
     if quantized != isinstance(exp_avg_sq, Quantized) or (quantized and not (exp_avg.signed and not exp_avg_sq.signed)):
         raise RuntimeError("both moments in 32 bits, or a signed and an unsigned Quantized")
     m, ms, v, vs = (*exp_avg[:2], *exp_avg_sq[:2]) if quantized else (exp_avg, None, exp_avg_sq, None)
-    return _ffi.adamw_step(params, grads, m, ms, v, vs, 8 if quantized else 32, step=step, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
-                           grad_scale=grad_scale, norm=norm, max_norm=max_norm, seed=seed, stream_index=stream_index,
-                           flags=_lib.F_SR if stochastic_rounding else 0)
+    return _dense.adamw_step(params, grads, m, ms, v, vs, 8 if quantized else 32, step, lr, betas[0], betas[1], eps, weight_decay, grad_scale, norm, max_norm, seed,
+                             stream_index, _lib.F_SR if stochastic_rounding else 0)
 
 
 class _Moments:
