@@ -301,3 +301,16 @@ def test_refusals():
             call()
             pytest.fail(f"call {k} was not refused")
     assert _lib.lib.haste_poll_status() == _lib.OK
+
+
+@pytest.mark.parametrize("xt", [BF, F32])
+@pytest.mark.parametrize("D", [2, 12, 16, 72, 96, 101, 192, 257, 333, 384, 500, 513, 767, 1017, 1018, 1023, 1025, 2047, 4093, 8191, 16383])
+def test_groups_of_lanes_and_vectors(D, xt):
+    """Widths between which a row changes its lanes, vectors or block, with more rows than one turn of the groups takes where that is cheap."""
+    from haste_b200.norm import layer_norm_backward, layer_norm_forward
+    rows = 9001 if D <= 192 else 2311 if D <= 1025 else 83
+    x, w, b, dy = _inputs(rows, D, xt, BF)
+    dy = dy.to(xt)
+    got = layer_norm_forward(x, w, b, 1e-5)
+    _check_forward(x, w, b, 1e-5, got)
+    _check_backward(dy, x, w, got[1], got[2], layer_norm_backward(dy, x, w, got[1], got[2]))
