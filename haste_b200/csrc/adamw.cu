@@ -445,9 +445,11 @@ template <int N>
 __global__ void __cluster_dims__(NORM_CLUSTER, 1, 1) __launch_bounds__(NORM_THREADS) grad_norm_small_kernel(const __grid_constant__ TensorTable<N> tab,
                                                                                                            float grad_scale, float* __restrict__ norm) {
   __shared__ float sums[NORM_CLUSTER];
+  cluster_started_arrive();
   auto cluster = cooperative_groups::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank()), blocks = tab.first[tab.count];
   const float s = sum_of_squares<NORM_THREADS>(tab, blocks * rank / NORM_CLUSTER, blocks * (rank + 1) / NORM_CLUSTER);
+  cluster_started_wait();
   if (threadIdx.x == 0) *cluster.map_shared_rank(&sums[rank], 0) = s;
   cluster.sync();
   if (rank == 0 && threadIdx.x == 0) {

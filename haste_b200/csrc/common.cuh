@@ -20,6 +20,12 @@ int validate_shape(const char* who, int64_t B, int64_t D, int64_t F, int64_t L, 
 __host__ __device__ __forceinline__ int64_t imin64(int64_t a, int64_t b) { return a < b ? a : b; }
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// ---------------------------------------------------------------- clusters
+// A block's shared memory may be accessed by the others of its cluster only once it has started, and only a cluster barrier tells: all threads
+// arrive on entry and wait before the first access, so that the wait costs nothing where there is work in between.
+__device__ __forceinline__ void cluster_started_arrive() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void cluster_started_wait() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- Philox4x32-10
 // Same generator as triton.language.random.philox_impl (which the reference reaches through
 // tl.randint at shared_ffi/sr_triton.py:11): round constants 0xD2511F53 / 0xCD9E8D57, key

@@ -139,6 +139,7 @@ __device__ __forceinline__ void finish_columns(const float* __restrict__ partial
   constexpr int SPLIT = LN_FINISH_THREADS / 32;
   __shared__ float buf[SPLIT][33];
   __shared__ float shares[CLUSTER][32];
+  if constexpr (CLUSTER > 1) cluster_started_arrive();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, rank = blockIdx.x % CLUSTER;
   const int64_t c = static_cast<int64_t>(blockIdx.x / CLUSTER) * 32 + tx;      // column of dw, or D more: of db
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -150,6 +151,7 @@ __device__ __forceinline__ void finish_columns(const float* __restrict__ partial
   }
   buf[ty][tx] = s;
   __syncthreads();
+  if constexpr (CLUSTER > 1) cluster_started_wait();
   if (ty == 0) {
 #pragma unroll
     for (int i = 1; i < SPLIT; ++i) s += buf[i][tx];
