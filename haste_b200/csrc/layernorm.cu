@@ -5,7 +5,7 @@
 //   h  = dy w             dx = r (h - mean(h) - z mean(h z))     dw = sum_rows dy z     db = sum_rows dy
 //
 // All sums are fp32; the variance is taken around the mean, not from the sum of squares, which cancels for rows whose mean is large
-// against their spread.  x is added up times a power of two, 1 / D or the next below, so that a row of the largest numbers has a mean.
+// against their spread.  x is added up times a power of two below 1 / D, so that a row of the largest numbers has a mean, which is not beyond them.
 // Inputs and outputs are bf16 or fp32, rounded once (nearest even) when stored.
 //
 // Memory bounds all of it: x in and y out, or dy and x in and dx out.  A row is read once and stays on the chip: 1 to 32 lanes of a
@@ -42,8 +42,13 @@ __device__ __forceinline__ float block_sum(float v, float* buf) {
   return s;
 }
 
-// The largest power of two that is not above 1 / D.
-__device__ __forceinline__ float power_below(int64_t D) { return __int_as_float((127 - (64 - __clzll(D - 1))) << 23); }
+// Half the largest power of two that is not above 1 / D: a sum of so much of D finite numbers is finite, whatever its roundings.
+__device__ __forceinline__ float power_below(int64_t D) { return __int_as_float((126 - (64 - __clzll(D - 1))) << 23); }
+// A mean that was made from that sum: it may have been rounded beyond the largest number, where the mean of finite numbers is not.
+__device__ __forceinline__ float in_range(float mean, float sum) {
+  const float most = __int_as_float(0x7F7FFFFF);
+  return fabsf(sum) <= most ? fminf(fmaxf(mean, -most), most) : mean;
+}
 
 constexpr int LN_THREADS = 256;
 
@@ -58,7 +63,7 @@ __global__ void __launch_bounds__(LN_THREADS) ln_fwd_wide_kernel(const X* __rest
     const X* xr = x + r * ldx;
     float s = 0.f;
     for (int64_t j = threadIdx.x; j < D; j += LN_THREADS) s = fmaf(ld_f(xr + j), part, s);
-    const float mean = block_sum(s, buf) / (static_cast<float>(D) * part);
+    const float sum = block_sum(s, buf), mean = in_range(sum / (static_cast<float>(D) * part), sum);
     s = 0.f;
     for (int64_t j = threadIdx.x; j < D; j += LN_THREADS) { const float d = ld_f(xr + j) - mean; s += d * d; }
     const float rstd = 1.f / sqrtf(block_sum(s, buf) / static_cast<float>(D) + eps);
@@ -569,7 +574,7 @@ __global__ void __launch_bounds__(MODE == BLOCK ? 512 : LN_WARP_THREADS, MODE ==
       for (int k = 0; k < VEC / 2; ++k) { if (k & 1) s2 = fma2(f[i][k], both(part), s2); else s1 = fma2(f[i][k], both(part), s1); }
     }
     s1 = add2(s1, s2);
-    const float mean = grp.sum(s1.x + s1.y, buf) * inv_dp;
+    const float sum = grp.sum(s1.x + s1.y, buf), mean = in_range(sum * inv_dp, sum);
     s1 = s2 = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
