@@ -370,6 +370,7 @@ __global__ void __launch_bounds__(ADAM_THREADS) adamw_kernel(const __grid_consta
 // ---------------------------------------------------------------- 2-norm of the gradients
 // Sum of squares of blocks lo .. hi - 1 of the launch over THREADS threads, in thread 0.  A warp has the loads of 4 blocks on their way at
 // once (56 M bf16 gradients 35 us with one, 27 with 4), and stays with a tensor, which it looks up once (30 us where each block was looked up).
+// Sums of 64 squares go on in 64 bits: an fp32 sum over a tensor of billions would lose what comes after a large value.
 template <int THREADS, int N>
 __device__ __forceinline__ float sum_of_squares(const TensorTable<N>& tab, int lo, int hi) {
   constexpr int WARPS = THREADS / 32;
@@ -378,7 +379,8 @@ __device__ __forceinline__ float sum_of_squares(const TensorTable<N>& tab, int l
   float2 acc[AHEAD];
 #pragma unroll
   for (int k = 0; k < AHEAD; ++k) acc[k] = both(0.f);
-  int t = tensor_of(tab, lo) - 1, next = 0, first = 0, type = HASTE_BF16;
+  double total = 0.0;
+  int t = tensor_of(tab, lo) - 1, next = 0, first = 0, type = HASTE_BF16, turns = 0;
   int64_t size = 0;
   const char* from = nullptr;
   for (int b0 = lo + (threadIdx.x >> 5); b0 < hi; b0 += WARPS * AHEAD) {
@@ -415,10 +417,16 @@ __device__ __forceinline__ float sum_of_squares(const TensorTable<N>& tab, int l
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[k] = fma2(f[i], f[i], acc[k]);
     }
+    if (++turns == 16) {
+      turns = 0;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) { total += static_cast<double>(acc[k].x) + acc[k].y; acc[k] = both(0.f); }
+    }
   }
   float s = 0.f;
 #pragma unroll
   for (int k = 0; k < AHEAD; ++k) s += acc[k].x + acc[k].y;
+  s = static_cast<float>(total + s);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane == 0) sums[threadIdx.x >> 5] = s;
