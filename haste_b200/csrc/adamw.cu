@@ -622,12 +622,12 @@ int launch_adamw(const AdamWCall& c, cudaStream_t st) {
 
 int launch_grad_norm(const void* const* grads, const int32_t* types, const int64_t* sizes, int64_t count, float grad_scale, float* partial, float* norm,
                      cudaStream_t st) {
-  const int64_t tables = count / TABLE_LARGE + 1;           // or one more for every 2^31 blocks, whose grids are as large as they get
+  const int64_t tables = count / TABLE_LARGE + 1;           // or one more for every 2^30 blocks, whose grids are as large as they get
   const int64_t cap = HASTE_GRAD_NORM_PARTIALS / 2 / tables;
   int parts = 0;
   bool done = false;
   const int rc = for_each_table(nullptr, types, grads, sizes, count, [&](const TensorTable<TABLE_LARGE>& tab, int64_t, int64_t blocks) {
-    if (count <= TABLE_MIDDLE && blocks <= NORM_SMALL_BLOCKS) {           // (all of them: one table)
+    if (tab.count == count && count <= TABLE_MIDDLE && blocks <= NORM_SMALL_BLOCKS) {          // all of them, not what is left behind 2^30 blocks
       if (count <= TABLE_SMALL) grad_norm_small_kernel<<<NORM_CLUSTER, NORM_THREADS, 0, st>>>(cut_table<TABLE_SMALL>(tab), grad_scale, norm);
       else grad_norm_small_kernel<<<NORM_CLUSTER, NORM_THREADS, 0, st>>>(cut_table<TABLE_MIDDLE>(tab), grad_scale, norm);
       done = true;
