@@ -152,12 +152,17 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// Root and quotient of the update to a few units in the last place: the update is a small part of the weight, whose own rounding hides
-// them, and neither enters the moments.  (133 M bf16 weights with 32-bit moments: 663 us with correctly rounded ones, 460 so; 56 M with
-// 8-bit moments 386 and 244.)  A second moment below 2^-126 counts as 0 here.
+// Root and quotient of the update to 2^-23 each (133 M bf16 weights with 32-bit moments: 663 us with correctly rounded ones, 460 so; 56 M with 8-bit
+// moments 386 and 244).  They are 2 to 3 ulp of the step, not of the weight, and a weight that starts at zero has them in its first values.
+// The moments in 32 bits do not depend on them; the scale by which values of 8 bits are encoded does, so that one within an ulp of a
+// boundary may take the next code.
+// Second moments in 32 bits may be subnormal: with an eps that is smaller still, a root of 0 would leave eps alone under the first moment.  In
+// 8 bits they count as 0 here (one instruction instead of several), as a block of less than CODE_TINY holds zeros anyway.
+template <int BITS>
 __device__ __forceinline__ float root_of(float v) {
   float r;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  if constexpr (BITS == 32) asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  else asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
 __device__ __forceinline__ float inverse_of(float v) {
@@ -328,7 +333,7 @@ __global__ void __launch_bounds__(ADAM_THREADS) adamw_kernel(const __grid_consta
     for (int i = 0; i < 4; ++i) {
       const float2 gi = mul2(g[i], both(scale));
       const float2 mi = fma2(both(b1), m2[i], mul2(both(a.c1), gi)), vi = fma2(both(b2), v2[i], mul2(mul2(both(a.c2), gi), gi));
-      const float2 den = fma2(make_float2(root_of(vi.x), root_of(vi.y)), both(a.root), both(a.eps));
+      const float2 den = fma2(make_float2(root_of<BITS>(vi.x), root_of<BITS>(vi.y)), both(a.root), both(a.eps));
       const float2 q = mul2(mi, make_float2(inverse_of(den.x), inverse_of(den.y)));
       const float2 wn = fma2(both(-a.rate), q, mul2(w[i], both(a.decay)));
       m[2 * i] = mi.x; m[2 * i + 1] = mi.y; v[2 * i] = vi.x; v[2 * i + 1] = vi.y;

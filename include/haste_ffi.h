@@ -378,7 +378,8 @@ int haste_layer_norm_backward(const void* dy, const void* x, const void* w, cons
  *   g = grad * grad_scale * min(1, max_norm / (*norm + 1e-6))         (without the last factor when norm is NULL)
  *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2
  *   w = w (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
- * in fp32, root and quotient to a few units in the last place; a v below 2^-126 counts as 0 there, and eps is 2^-126 at least.
+ * in fp32, root and quotient to a few units in the last place; eps is 2^-126 at least.  (bits = 8: a v below 2^-126 counts as 0 there, and 256
+ * moments that are all below 2^-120 are kept as zeros, so eps should be large against 2^-60 where gradients are that small.)
  * params, grads, sizes: host arrays of `count` device pointers and element counts, read before the call returns; the
  * parameters all of p_type, the gradients of g_type, both contiguous, aligned as their type.  A tensor whose gradient is NULL is left
  * alone.  bf16 parameters are rounded stochastically with HASTE_F_SR, else to nearest.
