@@ -115,8 +115,8 @@ class AdamW(Optimizer):
     byte and a scale per 256 elements.  ``max_grad_norm``: gradients of all groups are clipped to this norm together; the last step's norm
     is in ``grad_norm`` (a scalar on the device), and a step whose norm is inf or NaN changes nothing but the step count.
 
-    State dicts hold ``exp_avg`` and ``exp_avg_sq`` per parameter, as those of ``torch.optim.AdamW``, which load; so do state dicts of the
-    other ``state_bits``.  Steps are counted per group: a parameter without a gradient is left alone, the count goes on."""
+    State dicts hold ``exp_avg`` and ``exp_avg_sq`` per parameter.  Those of ``torch.optim.AdamW`` load (not the other way round: that class
+    counts its steps per parameter), and so do those of the other ``state_bits``.  Steps are counted per group: a parameter without a gradient is left alone, the count goes on."""
 
     _GROUP_KEYS = dict(state_bits=32, stochastic_rounding=True, seed=123, step_count=0)
 
@@ -136,18 +136,23 @@ class AdamW(Optimizer):
         return dict(super().__getstate__(), max_grad_norm=self.max_grad_norm)
 
     def __setstate__(self, state):
-        """From a pickle, a copy or ``load_state_dict``: the flat moments are made anew from the state's entries at the next step."""
+        """From a pickle, a copy or ``load_state_dict``: the flat moments are made anew from the state's entries at the next step.  Loading, options
+        that the saved groups lack are those of the groups that are replaced, and how moments are held is in any case."""
+        replaced = self.__dict__.get("param_groups", ())
         super().__setstate__(state)
         self._moments = {}
         self.__dict__.setdefault("max_grad_norm", None)
         self.__dict__.setdefault("grad_norm", None)
-        for group in self.param_groups:
-            for k, v in self._GROUP_KEYS.items():
-                group.setdefault(k, v)
+        for i, group in enumerate(self.param_groups):
+            told = dict(replaced[i] if i < len(replaced) else self._GROUP_KEYS, step_count=0)
+            if replaced:
+                group["state_bits"] = told["state_bits"]
+            for k in self._GROUP_KEYS:
+                group.setdefault(k, told[k])
 
     def load_state_dict(self, state_dict):
-        """As ``Optimizer.load_state_dict``, but the moments keep their types (that one casts them to the parameters'), and a state dict of
-        ``torch.optim.AdamW`` brings its step count along."""
+        """As ``Optimizer.load_state_dict``, but the moments keep their types (that one casts them to the parameters'), a state dict of
+        ``torch.optim.AdamW`` brings its step count along, and ``state_bits`` stays what the constructor was told: the moments are converted."""
         if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
             raise RuntimeError("state dicts with amsgrad or maximize are not supported")
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
