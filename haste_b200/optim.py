@@ -108,6 +108,19 @@ class _Moments:
                 new[name].copy_(_ffi.dequantize_moment(flat, s.to(x.device).contiguous(), signed)[:n].view(x.shape))
 
 
+class _Held:
+    """A parameter's saved entries on their way through ``Optimizer.load_state_dict``, which casts the tensors that it finds."""
+
+    def __init__(self, entries):
+        self.entries = entries
+
+
+def _hold(optimizer, state_dict):
+    if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
+        raise RuntimeError("state dicts with amsgrad or maximize are not supported")
+    return dict(state_dict, state={k: _Held(v) for k, v in state_dict["state"].items()})
+
+
 class AdamW(Optimizer):
     """AdamW with decoupled weight decay: one launch for all parameters of a group and type.
 
@@ -144,26 +157,28 @@ class AdamW(Optimizer):
         self.__dict__.setdefault("max_grad_norm", None)
         self.__dict__.setdefault("grad_norm", None)
         for i, group in enumerate(self.param_groups):
-            told = dict(replaced[i] if i < len(replaced) else self._GROUP_KEYS, step_count=0)
+            told = replaced[i] if i < len(replaced) else self._GROUP_KEYS
             if replaced:
                 group["state_bits"] = told["state_bits"]
+            held = {p: self.state[p].entries for p in group["params"] if isinstance(self.state.get(p), _Held)}
+            for p, old in held.items():
+                self.state[p] = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in old.items() if k.startswith("exp_avg")}
+            if "step_count" not in group:
+                group["step_count"] = max((int(old["step"]) for old in held.values() if "step" in old), default=0)
             for k in self._GROUP_KEYS:
                 group.setdefault(k, told[k])
+        for k, v in self.state.items():                                # entries of no parameter, which torch passes on
+            if isinstance(v, _Held):
+                self.state[k] = v.entries
 
     def load_state_dict(self, state_dict):
         """As ``Optimizer.load_state_dict``, but the moments keep their types (that one casts them to the parameters'), a state dict of
         ``torch.optim.AdamW`` brings its step count along, and ``state_bits`` stays what the constructor was told: the moments are converted."""
-        if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
-            raise RuntimeError("state dicts with amsgrad or maximize are not supported")
-        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
-        for saved, group in zip(state_dict["param_groups"], self.param_groups):
-            for key, p in zip(saved["params"], group["params"]):
-                old = state_dict["state"].get(key)
-                if old is None:
-                    continue
-                self.state[p] = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in old.items() if k.startswith("exp_avg")}
-                if "step_count" not in saved and "step" in old:
-                    group["step_count"] = max(group["step_count"], int(old["step"]))
+        last = self.register_load_state_dict_pre_hook(_hold)          # behind those of the user, which may replace the dict
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            last.remove()
 
     def _flat(self, index, group, dtype):
         """The moments of the group's parameters of one type; built at the first step, and again when they or the state were replaced."""
