@@ -9,6 +9,8 @@ The moments of a list of tensors lie in one buffer each, every tensor's at a mul
 each 256 elements share an fp32 scale; codes are rounded stochastically, so that a second moment, which moves by a thousandth a
 step, follows its gradients (include/haste_ffi.h has the format).
 """
+import itertools
+import operator
 from typing import NamedTuple
 
 import torch
@@ -61,13 +63,19 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step, lr=1e-3, betas=(0.9,
                              stream_index, _lib.F_SR if stochastic_rounding else 0)
 
 
+def _same(a, b):
+    """Whether two lists hold the same objects."""
+    return len(a) == len(b) and all(map(operator.is_, a, b))
+
+
 class _Moments:
     """The flat moments of the parameters of one type in a parameter group, and each parameter's part of them."""
 
     def __init__(self, params, bits):
         self.params, self.bits = list(params), bits
         dev = self.params[0].device
-        self.offsets = moment_offsets([p.numel() for p in self.params])
+        self.sizes = [p.numel() for p in self.params]
+        self.offsets = moment_offsets(self.sizes)
         n = self.offsets[-1]
         if bits == 32:
             self.avg, self.sq = torch.zeros(n, device=dev), torch.zeros(n, device=dev)
@@ -141,7 +149,7 @@ class AdamW(Optimizer):
         if not (lr >= 0 and weight_decay >= 0 and eps > 0 and all(0 <= b < 1 for b in betas)):
             raise ValueError("lr and weight_decay must not be negative, eps must be positive, betas in [0, 1)")
         self.max_grad_norm, self.grad_norm = max_grad_norm, None
-        self._moments = {}
+        self._moments, self._seen = {}, None                               # flat moments by group and type; the state's entries beside them
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, stochastic_rounding=stochastic_rounding,
                                       seed=seed, step_count=0))
 
@@ -153,7 +161,7 @@ class AdamW(Optimizer):
         that the saved groups lack are those of the groups that are replaced, and how moments are held is in any case."""
         replaced = self.__dict__.get("param_groups", ())
         super().__setstate__(state)
-        self._moments = {}
+        self._moments, self._seen = {}, None
         self.__dict__.setdefault("max_grad_norm", None)
         self.__dict__.setdefault("grad_norm", None)
         for i, group in enumerate(self.param_groups):
@@ -180,21 +188,29 @@ class AdamW(Optimizer):
         finally:
             last.remove()
 
-    def _flat(self, index, group, dtype):
-        """The moments of the group's parameters of one type; built at the first step, and again when they or the state were replaced."""
-        params = [p for p in group["params"] if p.dtype == dtype]
+    def _flat(self, index, group, dtype, params):
+        """The moments of the group's parameters of one type; built at the first step, and again when they, their sizes or entries of the state
+        were replaced."""
         m = self._moments.get((index, dtype))
-        if m is not None and m.bits == group["state_bits"] and len(m.params) == len(params) and all(a is b for a, b in zip(m.params, params)):
+        if m is not None and m.bits == group["state_bits"] and _same(m.params, params) and m.sizes == [p.numel() for p in params]:
             return m
+        ours = {*map(id, params)}                                          # other buffers of theirs (of another type or group) hold them no longer
+        self._moments = {k: other for k, other in self._moments.items() if ours.isdisjoint(map(id, other.params))}
         m = _Moments(params, group["state_bits"])
         for i, p in enumerate(params):
-            if self.state[p]:
-                m.adopt(i, self.state[p])
-            self.state[p].update(m.views(i))
-            for gone in [k for k in self.state[p] if k not in m.views(i)]:
-                del self.state[p][gone]
-        self._moments[(index, dtype)] = m
+            state, views = self.state[p], m.views(i)
+            if state:
+                m.adopt(i, state)
+            state.update(views)
+            for gone in {"exp_avg_scale", "exp_avg_sq_scale"} & (state.keys() - views.keys()):
+                del state[gone]
+        self._moments[(index, dtype)], self._seen = m, None
         return m
+
+    def _entries(self):
+        """What the state holds: keys, entries, and what is in these."""
+        entries = [s for s in self.state.values() if isinstance(s, dict)]
+        return [*self.state, *entries, *itertools.chain.from_iterable(map(dict.values, entries))]
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -202,27 +218,35 @@ class AdamW(Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        all_grads = [[p.grad for p in group["params"]] for group in self.param_groups]
         norm = None
         if self.max_grad_norm is not None:
-            grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
+            grads = [g if g.is_contiguous() else g.contiguous() for grads in all_grads for g in grads if g is not None]
             if grads:
-                norm = self.grad_norm = grad_norm([g if g.is_contiguous() else g.contiguous() for g in grads])
-        for index, group in enumerate(self.param_groups):
+                norm = self.grad_norm = grad_norm(grads)
+        if self._seen is None or not _same(self._seen, self._entries()):
+            self._moments = {}                                             # something was taken away or replaced
+        for index, (group, grads) in enumerate(zip(self.param_groups, all_grads)):
             group["step_count"] += 1
-            types = {p.dtype for p in group["params"] if p.grad is not None}
+            params = group["params"]
+            dtypes = [p.dtype for p in params]
+            types = {t for t, g in zip(dtypes, grads) if g is not None}
             for k, dtype in enumerate((torch.bfloat16, torch.float32)):
                 if dtype in types:
-                    self._step_type(group, self._flat(index, group, dtype), 2 * index + k, norm)
+                    of = (lambda x: x) if dtypes.count(dtype) == len(dtypes) else lambda x: [a for a, t in zip(x, dtypes) if t == dtype]
+                    self._step_type(group, self._flat(index, group, dtype, of(params)), of(grads), 2 * index + k, norm)
             if types - {torch.bfloat16, torch.float32}:
                 raise RuntimeError(f"parameters must be torch.bfloat16 or torch.float32, got {types - {torch.bfloat16, torch.float32}}")
+        if self._seen is None:
+            self._seen = self._entries()
         return loss
 
-    def _step_type(self, group, m, stream_index, norm):
+    def _step_type(self, group, m, grads, stream_index, norm):
         params = [p if p.is_contiguous() else p.contiguous() for p in m.params]
-        grads = [p.grad for p in m.params]
         g_types = {g.dtype for g in grads if g is not None}
         for g_type in g_types:                                         # one launch, unless some gradients have another type
-            part = [None if g is None or g.dtype != g_type else g if g.is_contiguous() else g.contiguous() for g in grads]
+            part = grads if len(g_types) == 1 else [g if g is not None and g.dtype == g_type else None for g in grads]
+            part = [g if g is None or g.is_contiguous() else g.contiguous() for g in part]
             adamw_step(params, part, m.avg, m.sq, step=group["step_count"], lr=group["lr"], betas=group["betas"], eps=group["eps"],
                        weight_decay=group["weight_decay"], max_norm=self.max_grad_norm if norm is not None else None, norm=norm,
                        stochastic_rounding=group["stochastic_rounding"], seed=group["seed"], stream_index=stream_index)
