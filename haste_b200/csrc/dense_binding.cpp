@@ -61,6 +61,10 @@ int gpu_of(const at::Tensor& t) { return t.is_cuda() ? t.get_device() : -1; }
 at::Tensor empty_on(int dev, at::IntArrayRef sizes, at::ScalarType type) {
   return at::detail::empty_cuda(sizes, type, c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(dev)), std::nullopt);
 }
+// A tensor that was written by address: a graph that holds its old values is to be refused (inference tensors are in none)
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 void* address(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // f(stream) with device `dev` current, and without the interpreter's lock (a launch may have to wait for room in the stream)
@@ -201,17 +205,17 @@ PyObject* layer_norm_backward(PyObject* const* a) {
   return out;
 }
 
-// A list or tuple of tensors, or anything that can be walked over
+// A list or tuple of tensors, or anything that can be walked over, as it is now: other threads may change a list while a launch has let go of the lock
 struct Sequence {
-  PyObject* fast;
-  explicit Sequence(PyObject* o) : fast(PySequence_Fast(o, "a list of tensors is expected")) {
-    if (fast == nullptr) throw python_error();
+  PyObject* items;
+  explicit Sequence(PyObject* o) : items(PySequence_Tuple(o)) {
+    if (items == nullptr) throw python_error();
   }
-  ~Sequence() { Py_DECREF(fast); }
+  ~Sequence() { Py_DECREF(items); }
   Sequence(const Sequence&) = delete;
   Sequence& operator=(const Sequence&) = delete;
-  int64_t size() const { return PySequence_Fast_GET_SIZE(fast); }
-  PyObject* operator[](int64_t i) const { return PySequence_Fast_GET_ITEM(fast, i); }
+  int64_t size() const { return PyTuple_GET_SIZE(items); }
+  PyObject* operator[](int64_t i) const { return PyTuple_GET_ITEM(items, i); }
 };
 
 struct TensorList {
@@ -323,6 +327,12 @@ PyObject* adamw_step(PyObject* const* a) {
     return lib.adamw_step(const_cast<void* const*>(p.p.data()), g.p.data(), p.sizes.data(), params.size(), mp, ms, vp, vs, moments, static_cast<int32_t>(bits), p.types[0], g_type,
                           number[0], number[1], number[2], number[3], number[4], step, static_cast<float>(number[5]), static_cast<float>(max_norm), np, seed, stream_index, flags, st);
   });
+  for (int64_t i = 0; i < params.size(); ++i)
+    if (grads[i] != Py_None) written(THPVariable_Unpack(params[i]));
+  written(m);
+  written(v);
+  if (bits == 8)
+    for (int i : {3, 5}) written(THPVariable_Unpack(a[i]));
   if (!norm.defined()) Py_RETURN_NONE;
   return THPVariable_Wrap(norm);
 }

@@ -54,7 +54,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step, lr=1e-3, betas=(0.9,
     ``exp_avg`` and ``exp_avg_sq`` are the flat moments: fp32 tensors, or ``Quantized``.  ``step`` counts from 1.  Gradients are
     multiplied with ``grad_scale``; with ``max_norm`` they are also clipped to that norm, which is returned (fp32 on the device; taken
     from ``norm`` where that is given, as when one norm is over the tensors of several calls), and a norm that is not finite leaves
-    everything as it was.  Random bits follow from (seed, step, place in the moments, stream_index)."""
+    everything as it was.  Autograd takes what is written for changed in place.  Random bits follow from (seed, step, place in the moments, stream_index)."""
     quantized = isinstance(exp_avg, Quantized)
     if quantized != isinstance(exp_avg_sq, Quantized) or (quantized and not (exp_avg.signed and not exp_avg_sq.signed)):
         raise RuntimeError("both moments in 32 bits, or a signed and an unsigned Quantized")
