@@ -357,6 +357,13 @@ PyObject* dequantize_moment(PyObject* const* a) {
   return THPVariable_Wrap(out);
 }
 
+// (three tensors or None) -> whether one has a tangent of forward-mode differentiation
+PyObject* has_tangent(PyObject* const* a) {
+  for (int i = 0; i < 3; ++i)
+    if (THPVariable_Check(a[i]) && THPVariable_Unpack(a[i])._fw_grad(/*level=*/0).defined()) Py_RETURN_TRUE;
+  Py_RETURN_FALSE;
+}
+
 // Addresses of the library's functions, in the order of Library's members
 PyObject* bind(PyObject* const* a) {
   void* at[7];
@@ -391,7 +398,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 #define ENTRY(f, n) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<f, n>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ENTRY(bind, 7), ENTRY(layer_norm_forward, 5), ENTRY(layer_norm_backward, 8), ENTRY(grad_norm, 2), ENTRY(adamw_step, 19),
-                         ENTRY(dequantize_moment, 4), {nullptr, nullptr, 0, nullptr}};
+                         ENTRY(dequantize_moment, 4), ENTRY(has_tangent, 3), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_dense", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

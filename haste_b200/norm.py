@@ -31,7 +31,9 @@ class _LayerNormFunction(torch.autograd.Function):
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
-    """Layer norm over the last dimension of ``x`` [..., D], differentiable (once) in x, weight and bias."""
+    """Layer norm over the last dimension of ``x`` [..., D], differentiable (once, in reverse mode) in x, weight and bias."""
+    if _ffi._dense.has_tangent(x, weight, bias):
+        raise NotImplementedError("layer_norm has no forward-mode derivative")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNormFunction.apply(x, weight, bias, float(eps))
     return _ffi.layer_norm_forward(x, weight, bias, float(eps), stats=False)
