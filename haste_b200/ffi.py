@@ -5,15 +5,12 @@ see (device, dtype, contiguity) and raises RuntimeError otherwise.
 """
 import contextlib
 import ctypes
+import importlib
 
 import torch
 
 from . import _lib
 from ._lib import lib, check
-try:
-    from . import _dense
-except ImportError as e:
-    raise ImportError(f"haste_b200._dense does not load ({e}): run `python -m haste_b200.build` (with --force after torch was replaced)") from e
 
 
 def _stream(t):
@@ -395,9 +392,25 @@ def topk_update(z, C, col0, vals, idx):
 
 # ---------------------------------------------------------------- layer norm, AdamW, gradient norm
 # (arguments are checked, outputs allocated and the library called by the extension module, csrc/dense_binding.cpp)
-_dense.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
-    "haste_last_error_string", "haste_layer_norm_forward", "haste_layer_norm_backward_scratch", "haste_layer_norm_backward", "haste_adamw_step",
-    "haste_grad_norm", "haste_dequantize_moment")))
+class _Extension:
+    """The extension module, loaded at its first use: it is built against one torch, which the sparse layer's calls need not know of."""
+
+    _BOUND = ("haste_last_error_string", "haste_layer_norm_forward", "haste_layer_norm_backward_scratch", "haste_layer_norm_backward", "haste_adamw_step",
+              "haste_grad_norm", "haste_dequantize_moment")
+
+    def __getattr__(self, name):
+        try:
+            module = importlib.import_module("._dense", __package__)
+        except ImportError as e:
+            raise ImportError(f"haste_b200._dense does not load ({e}): run `python -m haste_b200.build`") from e
+        module.bind(*(ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in self._BOUND))
+        self.__dict__.update((k, v) for k, v in vars(module).items() if not k.startswith("__"))
+        if name not in self.__dict__:
+            raise AttributeError(name)
+        return self.__dict__[name]
+
+
+_dense = _Extension()
 
 MOMENT_BLOCK = 256           # elements of a moment that share a scale; every tensor's moments start at a multiple of it
 
