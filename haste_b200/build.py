@@ -5,7 +5,7 @@ extension ``_dense`` through which torch tensors reach the dense operators.
     python -m haste_b200.build --force
 
 nvcc cross-compiles without a GPU.  The library links the CUDA runtime statically and depends on
-nothing else (no torch, no Python).  The extension is host code alone, built against the installed torch (after another torch: --force).
+nothing else (no torch, no Python).  The extension is host code alone, built against the installed torch, and again when that is another.
 """
 import os
 import subprocess
@@ -52,10 +52,13 @@ def _compile(src, force):
 def _build_dense(force):
     src = os.path.join(CSRC, "dense_binding.cpp")
     newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(HERE, "..", "include", "haste_ffi.h")))
-    if not force and os.path.exists(DENSE) and os.path.getmtime(DENSE) > newest:
-        return
     import torch
     from torch.utils import cpp_extension
+    stamp, against = os.path.join(OBJ, "_dense.torch"), f"{torch.__version__} {torch.__file__}"
+    if not force and os.path.exists(DENSE) and os.path.getmtime(DENSE) > newest and os.path.exists(stamp):
+        with open(stamp) as f:
+            if f.read() == against:
+                return
     made = os.path.join(OBJ, os.path.basename(DENSE))
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     for path in cpp_extension.include_paths() + [sysconfig.get_path("include"), os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")]:
@@ -68,6 +71,8 @@ def _build_dense(force):
     if p.returncode != 0:
         raise RuntimeError(f"compiling dense_binding.cpp failed:\n{p.stdout}\n{p.stderr}")
     os.replace(made, DENSE)
+    with open(stamp, "w") as f:
+        f.write(against)
 
 
 def build(force=False, verbose=False):
