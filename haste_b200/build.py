@@ -80,7 +80,6 @@ def build(force=False, verbose=False):
     with ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
         dense = ex.submit(_build_dense, force)
         results = list(ex.map(lambda s: _compile(s, force), SOURCES))
-        dense.result()
     objs = [o for o, _ in results]
     log = "".join(l for _, l in results)
     if log:
@@ -93,6 +92,7 @@ def build(force=False, verbose=False):
         p = subprocess.run(cmd, capture_output=True, text=True)
         if p.returncode != 0:
             raise RuntimeError(f"link failed:\n{p.stdout}\n{p.stderr}")
+    dense.result()                                      # without the extension there is the library, which needs none of it
     return LIB
 
 

@@ -38,3 +38,11 @@ def test_another_torch_is_noticed(build, monkeypatch):
         assert len(calls) == 2
     b._build_dense(True)
     assert len(calls) == 3
+
+
+def test_the_library_is_there_where_the_extension_fails(build, monkeypatch):
+    b, calls = build
+    monkeypatch.setattr(b, "compiler_fails", lambda cmd: "dense_binding.cpp" in " ".join(cmd), raising=False)
+    with pytest.raises(RuntimeError, match="dense_binding.cpp failed"):
+        b.build()
+    assert os.path.exists(b.LIB) and not os.path.exists(b.DENSE)
