@@ -1,7 +1,8 @@
 """A training step of the output layer together with the dense part in front of it: projection, layer norm, sparse layer.
 
 The reference puts a Linear between the encoder and the sparse layer (src/model.py:157-161, 242-243), trains it with the encoder's
-optimizer and the sparse layer with its own (src/runner.py:129-137, 197).  ``ProjectedFusedStep`` is that without an autograd graph:
+optimizer and the sparse layer with its own (src/runner.py:129-137, 197).  ``ProjectedFusedStep`` is that with a layer norm behind the Linear,
+which it needs, and without an autograd graph:
 
     a = h W^T + b         library GEMM
     x = layer norm of a   ``layer_norm_forward``

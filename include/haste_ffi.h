@@ -399,7 +399,7 @@ int haste_adamw_step(void* const* params, const void* const* grads, const int64_
                      double beta2, double eps, double weight_decay, int64_t step, float grad_scale, float max_norm, const float* norm, uint64_t seed,
                      uint32_t stream_index, uint32_t flags, haste_stream_t stream);
 
-/* 2-norm of all gradients together, times |grad_scale|, into *norm (device): sums of squares in fp32, joined in 64 bits in an order
+/* 2-norm of all gradients together, times |grad_scale|, into *norm (device): sums of squares in fp32, 64 at most and then in 64 bits, in an order
  * that depends on the sizes alone.  types: one of HASTE_BF16 / HASTE_F32 per tensor.  scratch: HASTE_GRAD_NORM_PARTIALS floats of device memory.  No tensors: 0. */
 #define HASTE_GRAD_NORM_PARTIALS 4096
 int haste_grad_norm(const void* const* grads, const int32_t* types, const int64_t* sizes, int64_t count, float grad_scale, float* scratch, float* norm,
