@@ -69,6 +69,16 @@ SIGNATURES = {
     "haste_grad_norm": [P, P, P, I64, F32, P, P, P],
     "haste_quantize_moment": [P, P, P, I64, I32, P],
     "haste_dequantize_moment": [P, P, P, I64, I32, I32, P],
+    "haste_embedding_forward": [P, I32, P, P, I64, I64, I64, I64, F32, I32, P],
+    "haste_embedding_backward_scratch": [I64, I64, I64],
+    "haste_embedding_backward": [P, I32, P, P, P, I64, I64, I64, I64, I64, F32, I64, I32, I32, P],
+    "haste_gated_forward_scratch": [I64, I64, I64, I64, I32],
+    "haste_gated_forward": [P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I32, P],
+    "haste_gated_backward_scratch": [I64, I64, I64, I64, I32],
+    "haste_gated_backward": [P, P, P, P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, I32, P],
+    "haste_muon_scratch": [P, P, I64],
+    "haste_muon_step": [P, P, P, P, I64, P, I64, I32, I32, F64, F64, I32, F64, I32, I32, F64, F64, F64, F64, I64, U64, U32, U32, P, I64, P],
+    "haste_orthogonalize": [P, P, P, P, I64, I32, I32, F64, F64, F64, F64, P, I64, P],
     "haste_ffi_set_max_ctas": [I32],
     "haste_poll_status": [],
     "haste_debug_set_wait_limit": [c_longlong],
@@ -87,13 +97,16 @@ lib.haste_last_error_string.restype = c_char_p
 lib.haste_last_error_string.argtypes = []
 lib.haste_version.restype = c_int
 lib.haste_ffi_topk_fused_scratch.restype = I64          # bytes, not a status
-lib.haste_layer_norm_backward_scratch.restype = I64
+for _name in ("haste_layer_norm_backward_scratch", "haste_embedding_backward_scratch", "haste_gated_forward_scratch", "haste_gated_backward_scratch", "haste_muon_scratch"):
+    getattr(lib, _name).restype = I64
 lib.haste_version.argtypes = []
 
 # status codes and flags (include/haste_ffi.h)
 OK, ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_INDEX_RANGE, ERR_LAUNCH, ERR_TIMEOUT, ERR_TOO_LARGE = range(7)
 LOSS_BCE, LOSS_SQHINGE = 0, 1
 BF16, FP32 = 0, 1
+ACTIVATIONS = dict(silu=0, gelu=1, gelu_tanh=2, relu=3)
+MUON_ADJUST = dict(original=0, match_rms_adamw=1)
 GRAD_NORM_PARTIALS = 4096
 F_SR, F_CONTRACT, F_RNG_PACKED, F_ZERO_DXT, F_LOSS = 1, 2, 4, 8, 16
 

@@ -618,4 +618,192 @@ int haste_dequantize_moment(const uint8_t* codes, const float* scales, void* out
   return launch_dequantize(codes, scales, out, n, is_signed, out_type, static_cast<cudaStream_t>(stream));
 }
 
+// ---------------------------------------------------------------- token embedding
+static int check_embedding(const char* who, int32_t id_bytes, int64_t tokens, int64_t D, int64_t V) {
+  if (id_bytes != 4 && id_bytes != 8) return fail(HASTE_ERR_UNSUPPORTED, "%s: ids of %d bytes", who, id_bytes);
+  if (tokens < 0 || D < 1 || V < 1) return fail(HASTE_ERR_BAD_ARG, "%s: tokens=%lld, D=%lld, V=%lld", who, (long long)tokens, (long long)D, (long long)V);
+  if (tokens > (1ll << 40) || D > (1ll << 24) || V > (1ll << 40)) return fail(HASTE_ERR_TOO_LARGE, "%s: tokens=%lld, D=%lld, V=%lld", who, (long long)tokens, (long long)D, (long long)V);
+  return HASTE_OK;
+}
+
+int haste_embedding_forward(const void* ids, int32_t id_bytes, const void* table, void* y, int64_t tokens, int64_t D, int64_t V, int64_t ld, float scale, int32_t type,
+                            haste_stream_t stream) {
+  const char* who = "haste_embedding_forward";
+  if (int rc = check_embedding(who, id_bytes, tokens, D, V)) return rc;
+  if (int rc = check_type(who, "table", type)) return rc;
+  if (ld < D && V > 1) return fail(HASTE_ERR_BAD_ARG, "%s: ld=%lld < D=%lld", who, (long long)ld, (long long)D);
+  if (tokens > 0) { REQUIRE_PTR(ids, who); REQUIRE_PTR(table, who); REQUIRE_PTR(y, who); }
+  return launch_embedding_forward(ids, id_bytes == 8, table, y, tokens, D, V, ld, scale, type, static_cast<cudaStream_t>(stream));
+}
+
+int64_t haste_embedding_backward_scratch(int64_t tokens, int64_t D, int64_t V) {
+  if (check_embedding("haste_embedding_backward_scratch", 4, tokens, D, V) != HASTE_OK || tokens + V >= (1ll << 31)) return 0;
+  return embedding_backward_scratch(tokens, D, V);
+}
+
+int haste_embedding_backward(const void* ids, int32_t id_bytes, const void* dy, void* dtable, void* scratch, int64_t scratch_bytes, int64_t tokens, int64_t D, int64_t V,
+                             int64_t lddy, float scale, int64_t padding, int32_t dy_type, int32_t out_type, haste_stream_t stream) {
+  const char* who = "haste_embedding_backward";
+  if (int rc = check_embedding(who, id_bytes, tokens, D, V)) return rc;
+  if (int rc = check_type(who, "dy", dy_type)) return rc;
+  if (int rc = check_type(who, "table", out_type)) return rc;
+  if (tokens + V >= (1ll << 31)) return fail(HASTE_ERR_TOO_LARGE, "%s: %lld tokens and %lld rows (fewer than 2^31 together are supported)", who, (long long)tokens, (long long)V);
+  if (lddy < 0) return fail(HASTE_ERR_BAD_ARG, "%s: lddy=%lld", who, (long long)lddy);
+  if (tokens > 0) { REQUIRE_PTR(ids, who); REQUIRE_PTR(dy, who); }
+  REQUIRE_PTR(dtable, who); REQUIRE_PTR(scratch, who); REQUIRE_ALIGNED(scratch, who);
+  const int64_t need = embedding_backward_scratch(tokens, D, V);
+  if (scratch_bytes < need) return fail(HASTE_ERR_BAD_ARG, "%s: %lld bytes of scratch, %lld needed", who, (long long)scratch_bytes, (long long)need);
+  return launch_embedding_backward(ids, id_bytes == 8, dy, dtable, scratch, tokens, D, V, lddy, scale, padding, dy_type, out_type, static_cast<cudaStream_t>(stream));
+}
+
+// ---------------------------------------------------------------- gated feed-forward block
+static int check_gated(const char* who, int64_t T, int64_t D, int64_t F, int64_t O) {
+  if (T < 0 || D < 1 || F < 1 || O < 1) return fail(HASTE_ERR_BAD_ARG, "%s: T=%lld, D=%lld, F=%lld, O=%lld", who, (long long)T, (long long)D, (long long)F, (long long)O);
+  const int64_t most = (1ll << 31) - 1024;         // coordinates of tensor maps are 32 bits
+  if (T > most || D > (1ll << 24) || F > (1ll << 24) || O > (1ll << 24))
+    return fail(HASTE_ERR_TOO_LARGE, "%s: T=%lld, D=%lld, F=%lld, O=%lld", who, (long long)T, (long long)D, (long long)F, (long long)O);
+  return HASTE_OK;
+}
+static int check_act(const char* who, int32_t act) {
+  if (act < HASTE_ACT_SILU || act > HASTE_ACT_RELU) return fail(HASTE_ERR_UNSUPPORTED, "%s: unknown activation %d", who, act);
+  return HASTE_OK;
+}
+static int check_scratch(const char* who, const void* scratch, int64_t bytes, int64_t need) {
+  if (need == 0) return HASTE_OK;
+  REQUIRE_PTR(scratch, who);
+  if (reinterpret_cast<uintptr_t>(scratch) & 255) return fail(HASTE_ERR_BAD_ARG, "%s: scratch must be 256-byte aligned", who);
+  if (bytes < need) return fail(HASTE_ERR_BAD_ARG, "%s: %lld bytes of scratch, %lld needed", who, (long long)bytes, (long long)need);
+  return HASTE_OK;
+}
+
+int64_t haste_gated_forward_scratch(int64_t T, int64_t D, int64_t F, int64_t O, int32_t aligned) {
+  if (check_gated("haste_gated_forward_scratch", T, D, F, O) != HASTE_OK || T == 0) return 0;
+  GatedCall c = {};
+  c.T = T; c.D = D; c.F = F; c.O = O; c.aligned = aligned != 0 && (D | F | O) % 8 == 0;
+  return gated_forward_scratch(c);
+}
+
+int haste_gated_forward(const void* x, const void* wg, const void* wu, const void* wd, void* gate, void* up, void* y, void* scratch, int64_t scratch_bytes, int64_t T, int64_t D,
+                        int64_t F, int64_t O, int64_t ldx, int64_t ldh, int32_t act, haste_stream_t stream) {
+  const char* who = "haste_gated_forward";
+  if (int rc = check_gated(who, T, D, F, O)) return rc;
+  if (int rc = check_act(who, act)) return rc;
+  if (ldx < D && T > 1) return fail(HASTE_ERR_BAD_ARG, "%s: ldx=%lld < D=%lld", who, (long long)ldx, (long long)D);
+  if (T == 0) return HASTE_OK;
+  REQUIRE_PTR(x, who); REQUIRE_PTR(wg, who); REQUIRE_PTR(wu, who); REQUIRE_PTR(wd, who); REQUIRE_PTR(y, who);
+  if ((gate == nullptr) != (up == nullptr)) return fail(HASTE_ERR_BAD_ARG, "%s: gate and up are kept together or not at all", who);
+  if (gate != nullptr) {
+    REQUIRE_ALIGNED(gate, who); REQUIRE_ALIGNED(up, who);
+    if (ldh < F || ldh % 8 != 0) return fail(HASTE_ERR_BAD_ARG, "%s: ldh=%lld must be a multiple of 8 and at least F=%lld", who, (long long)ldh, (long long)F);
+  }
+  GatedCall c = {x, wg, wu, wd, gate, up, y, ldx, ldh, T, D, F, O, act, false};
+  c.aligned = (D | F | O | ldx) % 8 == 0 && aligned16(x) && aligned16(wg) && aligned16(wu) && aligned16(wd) && aligned16(y);
+  if (int rc = check_scratch(who, scratch, scratch_bytes, gated_forward_scratch(c))) return rc;
+  return launch_gated_forward(c, scratch, static_cast<cudaStream_t>(stream));
+}
+
+int64_t haste_gated_backward_scratch(int64_t T, int64_t D, int64_t F, int64_t O, int32_t aligned) {
+  if (check_gated("haste_gated_backward_scratch", T, D, F, O) != HASTE_OK || T == 0) return 0;
+  GatedGradCall c = {};
+  c.T = T; c.D = D; c.F = F; c.O = O; c.aligned = aligned != 0 && (D | F | O) % 8 == 0;
+  void* some_place = reinterpret_cast<void*>(static_cast<uintptr_t>(256));
+  c.dx = some_place;
+  int64_t most = 0;
+  for (int some = 0; some < 8; ++some) {           // which are wanted decides how the products are cut
+    c.dwg = some & 1 ? some_place : nullptr; c.dwu = some & 2 ? some_place : nullptr; c.dwd = some & 4 ? some_place : nullptr;
+    const int64_t n = gated_backward_scratch(c);
+    if (n > most) most = n;
+  }
+  return most;
+}
+
+int haste_gated_backward(const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* gate, const void* up, void* dx, void* dwg, void* dwu, void* dwd,
+                         void* scratch, int64_t scratch_bytes, int64_t T, int64_t D, int64_t F, int64_t O, int64_t lddy, int64_t ldx, int64_t ldgate, int64_t ldup, int32_t act,
+                         haste_stream_t stream) {
+  const char* who = "haste_gated_backward";
+  if (int rc = check_gated(who, T, D, F, O)) return rc;
+  if (int rc = check_act(who, act)) return rc;
+  if (T > 1 && (lddy < O || ldx < D || ldgate < F || ldup < F)) return fail(HASTE_ERR_BAD_ARG, "%s: a row stride is smaller than its row", who);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (T == 0) {
+    cudaError_t e = cudaSuccess;
+    if (dwg != nullptr) e = cudaMemsetAsync(dwg, 0, F * D * 2, st);
+    if (e == cudaSuccess && dwu != nullptr) e = cudaMemsetAsync(dwu, 0, F * D * 2, st);
+    if (e == cudaSuccess && dwd != nullptr) e = cudaMemsetAsync(dwd, 0, O * F * 2, st);
+    return e == cudaSuccess ? HASTE_OK : fail(HASTE_ERR_LAUNCH, "%s: %s", who, cudaGetErrorString(e));
+  }
+  REQUIRE_PTR(dy, who); REQUIRE_PTR(x, who); REQUIRE_PTR(wg, who); REQUIRE_PTR(wu, who); REQUIRE_PTR(wd, who); REQUIRE_PTR(gate, who); REQUIRE_PTR(up, who);
+  GatedGradCall c = {dy, x, wg, wu, wd, gate, up, dx, dwg, dwu, dwd, lddy, ldx, ldgate, ldup, T, D, F, O, act, false};
+  c.aligned = (D | F | O | lddy | ldx | ldgate) % 8 == 0 && ldgate == ldup;
+  for (const void* p : {dy, x, wg, wu, wd, gate, up, static_cast<const void*>(dx), static_cast<const void*>(dwg), static_cast<const void*>(dwu), static_cast<const void*>(dwd)})
+    c.aligned = c.aligned && aligned16(p);
+  if (int rc = check_scratch(who, scratch, scratch_bytes, gated_backward_scratch(c))) return rc;
+  return launch_gated_backward(c, scratch, st);
+}
+
+// ---------------------------------------------------------------- Muon
+static int check_matrices(const char* who, const void* const* grads, const int64_t* rows, const int64_t* cols, int64_t count, int64_t* moments) {
+  if (count < 0) return fail(HASTE_ERR_BAD_ARG, "%s: count=%lld < 0", who, (long long)count);
+  if (count > 0) { REQUIRE_PTR(rows, who); REQUIRE_PTR(cols, who); }
+  *moments = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (rows[i] < 0 || cols[i] < 0) return fail(HASTE_ERR_BAD_ARG, "%s: matrix %lld is %lld x %lld", who, (long long)i, (long long)rows[i], (long long)cols[i]);
+    const int64_t least = rows[i] < cols[i] ? rows[i] : cols[i];
+    if (rows[i] > (1 << 24) || cols[i] > (1 << 24) || least > (1 << 16))
+      return fail(HASTE_ERR_TOO_LARGE, "%s: matrix %lld is %lld x %lld (2^24 by 2^16 at most)", who, (long long)i, (long long)rows[i], (long long)cols[i]);
+    *moments += (rows[i] * cols[i] + 255) / 256 * 256;
+  }
+  return HASTE_OK;
+}
+static int check_polynomial(const char* who, int32_t steps, double a, double b, double c, double eps) {
+  if (steps < 1 || steps > 1000) return fail(HASTE_ERR_BAD_ARG, "%s: %d steps", who, steps);
+  if (!is_finite(a) || !is_finite(b) || !is_finite(c)) return fail(HASTE_ERR_BAD_ARG, "%s: the coefficients must be finite", who);
+  if (!(eps >= 0x1p-100 && is_finite(eps))) return fail(HASTE_ERR_BAD_ARG, "%s: eps must be 2^-100 at least", who);
+  return HASTE_OK;
+}
+
+int64_t haste_muon_scratch(const int64_t* rows, const int64_t* cols, int64_t count) {
+  int64_t moments = 0;
+  if (check_matrices("haste_muon_scratch", nullptr, rows, cols, count, &moments) != HASTE_OK) return 0;
+  return muon_scratch(rows, cols, count);
+}
+
+int haste_muon_step(void* const* params, const void* const* grads, const int64_t* rows, const int64_t* cols, int64_t count, float* momentum, int64_t moments, int32_t p_type,
+                    int32_t g_type, double lr, double mu, int32_t nesterov, double weight_decay, int32_t adjust, int32_t steps, double a, double b, double c, double eps,
+                    int64_t step, uint64_t seed, uint32_t stream_index, uint32_t flags, void* scratch, int64_t scratch_bytes, haste_stream_t stream) {
+  const char* who = "haste_muon_step";
+  int64_t need = 0;
+  if (int rc = check_matrices(who, grads, rows, cols, count, &need)) return rc;
+  if (int rc = check_type(who, "parameter", p_type)) return rc;
+  if (int rc = check_type(who, "gradient", g_type)) return rc;
+  if (int rc = check_polynomial(who, steps, a, b, c, eps)) return rc;
+  if (!(lr >= 0 && is_finite(lr) && weight_decay >= 0 && is_finite(weight_decay) && mu >= 0 && mu < 1)) return fail(HASTE_ERR_BAD_ARG, "%s: lr, weight_decay or momentum out of range", who);
+  if (adjust != HASTE_MUON_ORIGINAL && adjust != HASTE_MUON_MATCH_RMS) return fail(HASTE_ERR_UNSUPPORTED, "%s: unknown adjustment %d", who, adjust);
+  if (step < 1) return fail(HASTE_ERR_BAD_ARG, "%s: step=%lld, steps count from 1", who, (long long)step);
+  if (count == 0 || need == 0) return HASTE_OK;
+  REQUIRE_PTR(params, who); REQUIRE_PTR(grads, who); REQUIRE_PTR(momentum, who); REQUIRE_ALIGNED(momentum, who);
+  if (moments < need) return fail(HASTE_ERR_BAD_ARG, "%s: momentum of %lld elements, %lld needed", who, (long long)moments, (long long)need);
+  for (int64_t i = 0; i < count; ++i)
+    if (rows[i] > 0 && cols[i] > 0 && params[i] == nullptr && grads[i] != nullptr) return fail(HASTE_ERR_BAD_ARG, "%s: parameter %lld is NULL", who, (long long)i);
+  if (int rc = check_scratch(who, scratch, scratch_bytes, muon_scratch(rows, cols, count))) return rc;
+  return launch_muon({who, params, grads, rows, cols, count, momentum, true, p_type, g_type, lr, mu, weight_decay, nesterov, adjust, steps, a, b, c, eps, step, seed, stream_index, flags,
+                      scratch}, static_cast<cudaStream_t>(stream));
+}
+
+int haste_orthogonalize(const void* const* in, void* const* out, const int64_t* rows, const int64_t* cols, int64_t count, int32_t in_type, int32_t steps, double a, double b, double c,
+                        double eps, void* scratch, int64_t scratch_bytes, haste_stream_t stream) {
+  const char* who = "haste_orthogonalize";
+  int64_t elements = 0;
+  if (int rc = check_matrices(who, in, rows, cols, count, &elements)) return rc;
+  if (int rc = check_type(who, "input", in_type)) return rc;
+  if (int rc = check_polynomial(who, steps, a, b, c, eps)) return rc;
+  if (count == 0 || elements == 0) return HASTE_OK;
+  REQUIRE_PTR(in, who); REQUIRE_PTR(out, who);
+  for (int64_t i = 0; i < count; ++i)
+    if (rows[i] > 0 && cols[i] > 0 && (in[i] == nullptr || out[i] == nullptr)) return fail(HASTE_ERR_BAD_ARG, "%s: matrix %lld is NULL", who, (long long)i);
+  if (int rc = check_scratch(who, scratch, scratch_bytes, muon_scratch(rows, cols, count))) return rc;
+  return launch_muon({who, out, in, rows, cols, count, nullptr, false, HASTE_BF16, in_type, 0, 0, 0, 0, HASTE_MUON_ORIGINAL, steps, a, b, c, eps, 1, 0, 0, 0, scratch},
+                     static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

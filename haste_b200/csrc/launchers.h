@@ -190,4 +190,51 @@ int launch_grad_norm(const void* const* grads, const int32_t* types, const int64
 int launch_quantize(const float* x, uint8_t* codes, float* scales, int64_t n, int is_signed, cudaStream_t st);
 int launch_dequantize(const uint8_t* codes, const float* scales, void* out, int64_t n, int is_signed, int type, cudaStream_t st);
 
+// Gated feed-forward block (gated.cu).  aligned: every base is on 16 bytes, every row stride and D, F, O are multiples of 8, ldgate = ldup
+struct GatedCall {
+  const void *x, *wg, *wu, *wd;      // [T, D] of row stride ldx, [F, D], [F, D], [O, F]
+  void *gate, *up, *y;               // [T, F] of row stride ldh, a multiple of 8, or NULL; [T, O]
+  int64_t ldx, ldh, T, D, F, O;
+  int act;
+  bool aligned;
+};
+struct GatedGradCall {
+  const void *dy, *x, *wg, *wu, *wd, *gate, *up;
+  void *dx, *dwg, *dwu, *dwd;        // NULL: not wanted
+  int64_t lddy, ldx, ldgate, ldup, T, D, F, O;
+  int act;
+  bool aligned;
+};
+int64_t gated_forward_scratch(const GatedCall& c);
+int64_t gated_backward_scratch(const GatedGradCall& c);
+int launch_gated_forward(const GatedCall& c, void* scratch, cudaStream_t st);
+int launch_gated_backward(const GatedGradCall& c, void* scratch, cudaStream_t st);
+
+// Muon and Newton-Schulz steps (muon.cu)
+struct MuonCall {
+  const char* who;
+  void* const* params;               // host arrays of `count`; a NULL gradient: the matrix is left alone.  Without `update`: where the results go, in bf16
+  const void* const* grads;
+  const int64_t *rows, *cols;
+  int64_t count;
+  float* momentum;                   // of all matrices, each at a multiple of 256 elements; NULL: the gradients themselves are made orthogonal
+  bool update;
+  int p_type, g_type;
+  double lr, mu, weight_decay;
+  int nesterov, adjust, steps;
+  double a, b, c, eps;
+  int64_t step;
+  uint64_t seed;
+  uint32_t stream, flags;
+  void* scratch;
+};
+int64_t muon_scratch(const int64_t* rows, const int64_t* cols, int64_t count);      // bytes
+int launch_muon(const MuonCall& c, cudaStream_t st);
+
+// Token embedding (embedding.cu); wide: ids are int64, else int32
+int launch_embedding_forward(const void* ids, int wide, const void* table, void* y, int64_t tokens, int64_t D, int64_t V, int64_t ld, float scale, int type, cudaStream_t st);
+int64_t embedding_backward_scratch(int64_t tokens, int64_t D, int64_t V);      // bytes
+int launch_embedding_backward(const void* ids, int wide, const void* dy, void* dtable, void* scratch, int64_t tokens, int64_t D, int64_t V, int64_t lddy, float scale, int64_t padding,
+                              int dy_type, int out_type, cudaStream_t st);
+
 }  // namespace haste

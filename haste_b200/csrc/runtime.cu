@@ -93,6 +93,23 @@ int make_tmap_bf16_2d(CUtensorMap* out, const void* base, uint64_t inner, uint64
   return HASTE_OK;
 }
 
+int make_tmap_16bit_3d(CUtensorMap* out, const void* base, bool f16, uint64_t inner, uint64_t outer, uint64_t batch, uint64_t row_stride_bytes, uint64_t batch_stride_bytes,
+                       uint32_t box_inner, uint32_t box_outer) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return fail(HASTE_ERR_LAUNCH, "cuTensorMapEncodeTiled is not available from this driver");
+  if (((reinterpret_cast<uintptr_t>(base) | row_stride_bytes | batch_stride_bytes) & 15u) != 0)
+    return fail(HASTE_ERR_BAD_ARG, "tensor map: base and strides must be multiples of 16 bytes");
+  const cuuint64_t dims[3] = {inner, outer, batch};
+  const cuuint64_t strides[2] = {row_stride_bytes, batch_stride_bytes};
+  const cuuint32_t box[3] = {box_inner, box_outer, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(out, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, box_inner == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(HASTE_ERR_LAUNCH, "cuTensorMapEncodeTiled failed (CUresult %d)", static_cast<int>(r));
+  return HASTE_OK;
+}
+
 }  // namespace haste
 
 extern "C" {

@@ -24,5 +24,8 @@ int take_stall_tile();
 // box of 64 columns, 64 bytes for 32.
 int make_tmap_bf16_2d(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner,
                       uint32_t box_outer);
+// The same for a batch of matrices of bf16 or fp16.
+int make_tmap_16bit_3d(CUtensorMap* out, const void* base, bool f16, uint64_t inner, uint64_t outer, uint64_t batch, uint64_t row_stride_bytes, uint64_t batch_stride_bytes,
+                       uint32_t box_inner, uint32_t box_outer);
 
 }  // namespace haste

@@ -10,7 +10,7 @@ import importlib
 import torch
 
 from . import _lib
-from ._lib import lib, check
+from ._lib import ACTIVATIONS, lib, check
 
 
 def _stream(t):
@@ -390,13 +390,15 @@ def topk_update(z, C, col0, vals, idx):
         check(lib.haste_topk_update(_ptr(z), z.stride(0), B, C, col0, k, _ptr(vals), _ptr(idx), _stream(z)), "topk_update")
 
 
-# ---------------------------------------------------------------- layer norm, AdamW, gradient norm
+# ---------------------------------------------------------------- dense operators: layer norm, AdamW, gradient norm, embedding, gated feed-forward, Muon
 # (arguments are checked, outputs allocated and the library called by the extension module, csrc/dense_binding.cpp)
 class _Extension:
     """The extension module, loaded at its first use: it is built against one torch, which the sparse layer's calls need not know of."""
 
     _BOUND = ("haste_last_error_string", "haste_layer_norm_forward", "haste_layer_norm_backward_scratch", "haste_layer_norm_backward", "haste_adamw_step",
-              "haste_grad_norm", "haste_dequantize_moment")
+              "haste_grad_norm", "haste_dequantize_moment", "haste_embedding_forward", "haste_embedding_backward_scratch", "haste_embedding_backward",
+              "haste_gated_forward_scratch", "haste_gated_forward", "haste_gated_backward_scratch", "haste_gated_backward", "haste_muon_scratch", "haste_muon_step",
+              "haste_orthogonalize")
 
     def __getattr__(self, name):
         try:
@@ -448,6 +450,40 @@ def quantize_moment(x, signed):
 def dequantize_moment(codes, scales, signed, dtype=torch.float32):
     """The values (bf16 or fp32) that codes of 8 bits and their scales stand for."""
     return _dense.dequantize_moment(codes, scales, signed, dtype)
+
+
+def embedding_forward(ids, table, scale=1.0):
+    """``scale * table[ids]``: [*ids.shape, D], of the table's type (bf16 or fp32, [V, D], any row stride).  ids: int64 or int32, any shape.  An id that
+    is no row of the table makes a row of NaN (a check would have to wait for the device)."""
+    return _dense.embedding_forward(ids, table, scale)
+
+
+def embedding_backward(dy, ids, rows, scale=1.0, padding_idx=None, dtype=None):
+    """The gradient of a table of ``rows`` rows for ``dy`` [*ids.shape, D] (bf16 or fp32), dense, of type ``dtype`` (default: dy's).  Each row's sum is fp32 and runs in the
+    order of its tokens: the same bits on every call.  Rows of no token and row ``padding_idx`` (negative: from the end) get zeros; ids that are no row are left out."""
+    pad = -1
+    if padding_idx is not None:
+        pad = padding_idx + rows if padding_idx < 0 else padding_idx
+        if not 0 <= pad < rows:
+            raise RuntimeError(f"padding_idx {padding_idx} is no row of a table of {rows}")
+    return _dense.embedding_backward(dy, ids, rows, scale, pad, dtype)
+
+
+def _activation(name):
+    if name not in ACTIVATIONS:
+        raise RuntimeError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {name!r}")
+    return ACTIVATIONS[name]
+
+
+def gated_forward(x, w_gate, w_up, w_down, activation="silu", keep=False):
+    """``(act(x w_gate^T) * (x w_up^T)) w_down^T`` for bf16 ``x`` [..., D], ``w_gate`` and ``w_up`` [F, D], ``w_down`` [O, F]: y [..., O]; with ``keep`` ``(y, gate, up)``, the two
+    projections [..., F] (bf16) that the backward pass takes.  ``activation``: "silu", "gelu", "gelu_tanh" or "relu"."""
+    return _dense.gated_forward(x, w_gate, w_up, w_down, _activation(activation), keep)
+
+
+def gated_backward(dy, x, w_gate, w_up, w_down, gate, up, activation="silu", want=(True, True, True, True)):
+    """``(dx, dw_gate, dw_up, dw_down)`` of ``gated_forward``, bf16, None where not wanted.  The same bits on every call."""
+    return _dense.gated_backward(x, w_gate, w_up, w_down, dy, gate, up, _activation(activation), *want)
 
 
 def check_locations(loc, D):

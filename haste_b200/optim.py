@@ -1,8 +1,10 @@
-"""AdamW over many tensors at once, for the dense parameters next to the sparse layer (``SRSgd`` trains the layer itself).
+"""AdamW and Muon over many tensors at once, for the dense parameters next to the sparse layer (``SRSgd`` trains the layer itself).
 
     AdamW(params, ...)          torch optimizer: bf16 (stochastic rounding, no fp32 copies) or fp32 parameters, moments in 32 or 8 bits,
                                 gradients clipped by their global norm without a word from the host
+    Muon(matrices, ...)         torch optimizer: the momentum of every matrix, made orthogonal by Newton-Schulz steps
     adamw_step, grad_norm       the kernels, on lists of tensors and flat moments
+    muon_step, orthogonalize    likewise
     quantize, dequantize        the 8-bit form of moments
 
 The moments of a list of tensors lie in one buffer each, every tensor's at a multiple of 256 elements (``moment_offsets``).  In 8 bits
@@ -61,6 +63,27 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step, lr=1e-3, betas=(0.9,
     m, ms, v, vs = (*exp_avg[:2], *exp_avg_sq[:2]) if quantized else (exp_avg, None, exp_avg_sq, None)
     return _dense.adamw_step(params, grads, m, ms, v, vs, 8 if quantized else 32, step, lr, betas[0], betas[1], eps, weight_decay, grad_scale, norm, max_norm, seed,
                              stream_index, _lib.F_SR if stochastic_rounding else 0)
+
+
+def orthogonalize(matrices, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """The nearest orthogonal matrices, nearly, by ``steps`` Newton-Schulz steps: for each of a list of matrices (all bf16 or all fp32) X = G / max(|G|, eps), then
+    X <- a X + (b A + c A^2) X with A = X X^T, or the same of the transpose where there are more rows than columns.  A list of bf16 matrices; their singular values end
+    between 0.7 and 1.2 with the default coefficients.  A matrix that is not finite becomes NaN, zeros stay zeros."""
+    return _dense.orthogonalize(matrices, steps, *coefficients, eps)
+
+
+def muon_step(params, grads, momentum_buffer, *, step, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.1, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7,
+              adjust="original", stochastic_rounding=True, seed=123, stream_index=0):
+    """One Muon step (decoupled weight decay) over lists of matrices, all bf16 or all fp32, and gradients (None: skipped), in place.
+
+    ``momentum_buffer`` is flat, fp32, every matrix's part at a multiple of 256 elements (``moment_offsets``).  The momentum is an average of gradients; the update is made orthogonal as
+    ``orthogonalize`` does it and multiplied with ``lr`` and sqrt(max(1, rows / columns)), or 0.2 sqrt(max(rows, columns)) with ``adjust="match_rms_adamw"``, by which learning rates of
+    AdamW fit.  ``step`` counts from 1; random bits follow from (seed, step, place in the momentum, stream_index).  A matrix whose gradient or momentum is not finite is left as it was, with
+    its momentum.  Autograd takes what is written for changed in place."""
+    if adjust not in _lib.MUON_ADJUST:
+        raise RuntimeError(f"adjust must be one of {', '.join(_lib.MUON_ADJUST)}, got {adjust!r}")
+    _dense.muon_step(params, grads, momentum_buffer, step, lr, momentum, nesterov, weight_decay, _lib.MUON_ADJUST[adjust], steps, *coefficients, eps, seed, stream_index,
+                     _lib.F_SR if stochastic_rounding else 0)
 
 
 def _same(a, b):
@@ -250,6 +273,114 @@ class AdamW(Optimizer):
             adamw_step(params, part, m.avg, m.sq, step=group["step_count"], lr=group["lr"], betas=group["betas"], eps=group["eps"],
                        weight_decay=group["weight_decay"], max_norm=self.max_grad_norm if norm is not None else None, norm=norm,
                        stochastic_rounding=group["stochastic_rounding"], seed=group["seed"], stream_index=stream_index)
+        for p, q in zip(m.params, params):
+            if p is not q:
+                p.copy_(q)
+
+
+class _Momentum:
+    """The flat momentum of the matrices of one type in a parameter group, and each one's part of it."""
+
+    def __init__(self, params):
+        self.params, self.shapes = list(params), [p.shape for p in params]
+        at = moment_offsets([p.numel() for p in params])
+        self.flat = torch.zeros(at[-1], device=params[0].device)
+        self.views = [self.flat[a:a + p.numel()].view(p.shape) for a, p in zip(at, params)]
+
+
+class Muon(Optimizer):
+    """Muon with decoupled weight decay, for matrices: embeddings, norms and biases are ``AdamW``'s.  All matrices of a group and type go through the same launches.
+
+    bf16 parameters are rounded stochastically (``stochastic_rounding=False``: to nearest), momentum is fp32.  ``steps``, ``coefficients`` and ``eps`` are those of ``orthogonalize``,
+    ``adjust`` is ``muon_step``'s.  A matrix whose gradient is not finite is left as it was.
+
+    State dicts hold ``momentum_buffer`` per parameter; those of ``torch.optim.Muon`` load.  Steps are counted per group, for the random bits."""
+
+    _GROUP_KEYS = dict(momentum=0.95, nesterov=True, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, adjust="original", stochastic_rounding=True, seed=123, step_count=0)
+    _TORCH_KEYS = dict(steps="ns_steps", coefficients="ns_coefficients", adjust="adjust_lr_fn")
+
+    def __init__(self, params, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.1, *, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, adjust="original",
+                 stochastic_rounding=True, seed=123):
+        if not (lr >= 0 and weight_decay >= 0 and eps > 0 and 0 <= momentum < 1 and steps >= 1):
+            raise ValueError("lr and weight_decay must not be negative, eps must be positive, momentum in [0, 1), steps 1 at least")
+        if adjust not in _lib.MUON_ADJUST:
+            raise ValueError(f"adjust must be one of {', '.join(_lib.MUON_ADJUST)}")
+        self._flats = {}                                                   # by group and type
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps, coefficients=tuple(coefficients), eps=eps, adjust=adjust,
+                                      stochastic_rounding=stochastic_rounding, seed=seed, step_count=0))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        if any(p.dim() != 2 for p in self.param_groups[-1]["params"]):
+            del self.param_groups[-1]
+            raise ValueError("Muon takes matrices; other parameters are AdamW's")
+
+    def __setstate__(self, state):
+        """From a pickle, a copy or ``load_state_dict``: the flat momentum is made anew from the state's entries at the next step."""
+        replaced = self.__dict__.get("param_groups", ())
+        super().__setstate__(state)
+        self._flats = {}
+        for i, group in enumerate(self.param_groups):
+            told = replaced[i] if i < len(replaced) else self._GROUP_KEYS
+            for ours, theirs in self._TORCH_KEYS.items():
+                if theirs in group:
+                    value = group.pop(theirs)
+                    group.setdefault(ours, value if value is not None else "original")
+            for k in self._GROUP_KEYS:
+                group.setdefault(k, told[k])
+        for k, v in self.state.items():
+            if isinstance(v, _Held):
+                self.state[k] = {n: t.clone() if isinstance(t, torch.Tensor) else t for n, t in v.entries.items() if n == "momentum_buffer"} if isinstance(k, torch.Tensor) else v.entries
+
+    def load_state_dict(self, state_dict):
+        """As ``Optimizer.load_state_dict``, but the momentum keeps its type (that one casts it to the parameters')."""
+        last = self.register_load_state_dict_pre_hook(_hold)              # behind those of the user, which may replace the dict
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            last.remove()
+
+    def _flat(self, key, params):
+        m = self._flats.get(key)
+        if m is not None and _same(m.params, params) and m.shapes == [p.shape for p in params] and _same(m.views, [self.state[p].get("momentum_buffer") for p in params]):
+            return m
+        m = _Momentum(params)
+        for p, view in zip(params, m.views):
+            old = self.state[p].get("momentum_buffer")
+            if old is not None:
+                if old.shape != view.shape:
+                    raise RuntimeError(f"saved momentum_buffer of shape {tuple(old.shape)} for a parameter of shape {tuple(view.shape)}")
+                view.copy_(old)
+            self.state[p]["momentum_buffer"] = view
+        self._flats[key] = m
+        return m
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for index, group in enumerate(self.param_groups):
+            group["step_count"] += 1
+            types = {p.dtype for p in group["params"] if p.grad is not None}
+            for k, dtype in enumerate((torch.bfloat16, torch.float32)):
+                if dtype in types:
+                    params = [p for p in group["params"] if p.dtype == dtype]
+                    self._step_type(group, self._flat((index, dtype), params), 2 * index + k)
+            if types - {torch.bfloat16, torch.float32}:
+                raise RuntimeError(f"parameters must be torch.bfloat16 or torch.float32, got {types - {torch.bfloat16, torch.float32}}")
+        return loss
+
+    def _step_type(self, group, m, stream_index):
+        params = [p if p.is_contiguous() else p.contiguous() for p in m.params]
+        grads = [p.grad for p in m.params]
+        for g_type in {g.dtype for g in grads if g is not None}:
+            part = [g if g is not None and g.dtype == g_type else None for g in grads]
+            part = [g if g is None or g.is_contiguous() else g.contiguous() for g in part]
+            muon_step(params, part, m.flat, step=group["step_count"], lr=group["lr"], momentum=group["momentum"], nesterov=group["nesterov"], weight_decay=group["weight_decay"],
+                      steps=group["steps"], coefficients=group["coefficients"], eps=group["eps"], adjust=group["adjust"], stochastic_rounding=group["stochastic_rounding"],
+                      seed=group["seed"], stream_index=stream_index)
         for p, q in zip(m.params, params):
             if p is not q:
                 p.copy_(q)

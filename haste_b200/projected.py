@@ -9,7 +9,7 @@ which it needs, and without an autograd graph:
     fused sparse step     ``FusedFFIShard.step``: loss, the gradient of x, the sparse layer's update
     da                    ``layer_norm_backward``, with the gradients of the norm's weight and bias
     dW, db, dh            library GEMMs
-    AdamW                 over W, b and the norm's parameters (and whatever else the optimizer holds), clipped by their joint norm
+    AdamW                 over W, b and the norm's parameters (and whatever else the optimizer holds), clipped by their joint norm; or Muon over W and AdamW over the rest
 """
 import torch
 
@@ -18,14 +18,16 @@ from .norm import layer_norm_backward, layer_norm_forward
 
 class ProjectedFusedStep:
     """``projection``: torch.nn.Linear [H -> P]; ``norm``: ``haste_b200.norm.LayerNorm(P)``; ``shard``: ``FusedFFIShard`` over P features;
-    ``optimizer``: ``haste_b200.optim.AdamW`` that holds the parameters of the first two.  The projection and the features are bf16."""
+    ``optimizer``: ``haste_b200.optim.AdamW`` that holds the parameters of the first two, or a list of optimizers that do (``Muon`` for the matrices beside it).  The
+    projection and the features are bf16."""
 
     def __init__(self, projection, norm, shard, optimizer):
         if projection.out_features != norm.features or norm.features != shard.D:
             raise ValueError(f"the projection has {projection.out_features} outputs, the norm {norm.features} features, the sparse layer {shard.D}")
         if projection.weight.dtype != torch.bfloat16:
             raise ValueError("the projection must be bf16, as the sparse layer's features are")
-        held = {id(p) for group in optimizer.param_groups for p in group["params"]}
+        self.optimizers = list(optimizer) if isinstance(optimizer, (list, tuple)) else [optimizer]
+        held = {id(p) for o in self.optimizers for group in o.param_groups for p in group["params"]}
         if any(id(p) not in held for m in (projection, norm) for p in m.parameters()):
             raise ValueError("the optimizer must hold the projection's and the norm's parameters")
         self.projection, self.norm, self.shard, self.optimizer = projection, norm, shard, optimizer
@@ -57,4 +59,5 @@ class ProjectedFusedStep:
         return da @ lin.weight, loss
 
     def update(self):
-        self.optimizer.step()
+        for o in self.optimizers:
+            o.step()

@@ -45,6 +45,9 @@ enum { HASTE_LOSS_BCE = 0, HASTE_LOSS_SQHINGE = 1 };
 
 /* element types of the dense operators */
 enum { HASTE_BF16 = 0, HASTE_F32 = 1 };
+/* activations of the gated feed-forward block, and what Muon's learning rate is multiplied with */
+enum { HASTE_ACT_SILU = 0, HASTE_ACT_GELU = 1, HASTE_ACT_GELU_TANH = 2, HASTE_ACT_RELU = 3 };
+enum { HASTE_MUON_ORIGINAL = 0, HASTE_MUON_MATCH_RMS = 1 };
 
 /* flags for the update / train-step entry points */
 enum {
@@ -409,6 +412,55 @@ int haste_grad_norm(const void* const* grads, const int32_t* types, const int64_
  * bf16 or fp32.  is_signed: as the first moment, else as the second (no negative values).  x, codes and out 16-byte aligned. */
 int haste_quantize_moment(const float* x, uint8_t* codes, float* scales, int64_t n, int32_t is_signed, haste_stream_t stream);
 int haste_dequantize_moment(const uint8_t* codes, const float* scales, void* out, int64_t n, int32_t is_signed, int32_t out_type, haste_stream_t stream);
+
+/* Token embedding: y[t,:] = scale * table[ids[t],:], y contiguous [tokens, D], of the table's type (bf16 or fp32; [V, D], row stride ld elements).  ids:
+ * int64 (id_bytes = 8) or int32 (4).  An id that is no row of the table (checking that would take a word from the device) makes a row of NaN. */
+int haste_embedding_forward(const void* ids, int32_t id_bytes, const void* table, void* y, int64_t tokens, int64_t D, int64_t V, int64_t ld, float scale, int32_t type,
+                            haste_stream_t stream);
+
+/* Its gradient: dtable [V, D], contiguous, bf16 or fp32, is written in full: dtable[v,:] = scale * sum of dy[t,:] over the tokens with ids[t] = v, in the order of the
+ * tokens and in fp32 (the same bits on every call), zeros for rows of no token.  Tokens with ids[t] = padding (-1: no such id) or an id
+ * that is no row are left out.  dy [tokens, D], row stride lddy (0 = one row for all).  tokens + V < 2^31.  scratch: 16-byte aligned,
+ * haste_embedding_backward_scratch(tokens, D, V) bytes. */
+int64_t haste_embedding_backward_scratch(int64_t tokens, int64_t D, int64_t V);
+int haste_embedding_backward(const void* ids, int32_t id_bytes, const void* dy, void* dtable, void* scratch, int64_t scratch_bytes, int64_t tokens, int64_t D, int64_t V,
+                             int64_t lddy, float scale, int64_t padding, int32_t dy_type, int32_t out_type, haste_stream_t stream);
+
+/* Gated feed-forward block, bf16: y = (act(x Wg^T) * (x Wu^T)) Wd^T with x [T, D] (row stride ldx), Wg, Wu [F, D], Wd [O, F] and y [T, O] contiguous; act: HASTE_ACT_*.
+ * For training gate = x Wg^T and up = x Wu^T [T, F] (row stride ldh, a multiple of 8, 16-byte aligned) are kept, without NULL.  Sums are fp32; the product
+ * act(gate) * up is rounded to bf16 on its way to the second product (not for T <= 8).  Nothing else needs alignment; operands that have it (16-byte bases, row
+ * strides and D, F, O multiples of 8) are read in place, others are copied first.
+ * scratch: 256-byte aligned, haste_gated_forward_scratch(T, D, F, O, aligned) bytes, aligned = 0 unless all operands have that alignment. */
+int64_t haste_gated_forward_scratch(int64_t T, int64_t D, int64_t F, int64_t O, int32_t aligned);
+int haste_gated_forward(const void* x, const void* wg, const void* wu, const void* wd, void* gate, void* up, void* y, void* scratch, int64_t scratch_bytes, int64_t T, int64_t D,
+                        int64_t F, int64_t O, int64_t ldx, int64_t ldh, int32_t act, haste_stream_t stream);
+
+/* Its gradients from the kept projections: dx [T, D], dwg, dwu [F, D] and dwd [O, F], contiguous, any of them NULL where it is not wanted.  dy [T, O] has row stride
+ * lddy, gate and up ldgate and ldup.  With T = 0 the weights' gradients are zeros.  The order of every sum depends on the sizes alone. */
+int64_t haste_gated_backward_scratch(int64_t T, int64_t D, int64_t F, int64_t O, int32_t aligned);
+int haste_gated_backward(const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* gate, const void* up, void* dx, void* dwg, void* dwu, void* dwd,
+                         void* scratch, int64_t scratch_bytes, int64_t T, int64_t D, int64_t F, int64_t O, int64_t lddy, int64_t ldx, int64_t ldgate, int64_t ldup, int32_t act,
+                         haste_stream_t stream);
+
+/* One Muon step over `count` matrices:
+ *   m = mu m + (1 - mu) g,   u = mu m + (1 - mu) g (nesterov) or m,   X = u / max(|u|, eps)  (2-norm of all elements; transposed where rows > cols)
+ *   `steps` times:  A = X X^T,  X = a X + (b A + c A A) X
+ *   w = w (1 - lr weight_decay) - lr r X,   r = sqrt(max(1, rows / cols)) (adjust = HASTE_MUON_ORIGINAL) or 0.2 sqrt(max(rows, cols)) (HASTE_MUON_MATCH_RMS)
+ * params, grads, rows, cols: host arrays, read before the call returns; parameters all of p_type, gradients of g_type, contiguous.  A matrix whose gradient is NULL is
+ * left alone, and so is one whose norm is inf or NaN, with its momentum.  momentum: fp32, 16-byte aligned, `moments` elements of room, matrix after
+ * matrix, every one at a multiple of 256 elements.  Norms are 64 bits, momentum and weights' arithmetic 32, products take fp16 and sum in fp32
+ * (X keeps 22 bits between them).  bf16 parameters are rounded stochastically with HASTE_F_SR, else to nearest: Philox4x32 with 7 rounds, key (lower half of
+ * seed, step), counter (i, i >> 32, stream_index, 2), the lower halves of its words for elements 4i .. 4i+3 of the momentum's buffer.
+ * eps is 2^-100 at least.  scratch: 256-byte aligned, haste_muon_scratch(...) bytes: 6 a element and 4 for every pair of rows of X, 1 GB at most unless one matrix
+ * needs more (matrices are then worked on in rounds). */
+int64_t haste_muon_scratch(const int64_t* rows, const int64_t* cols, int64_t count);
+int haste_muon_step(void* const* params, const void* const* grads, const int64_t* rows, const int64_t* cols, int64_t count, float* momentum, int64_t moments, int32_t p_type,
+                    int32_t g_type, double lr, double mu, int32_t nesterov, double weight_decay, int32_t adjust, int32_t steps, double a, double b, double c, double eps,
+                    int64_t step, uint64_t seed, uint32_t stream_index, uint32_t flags, void* scratch, int64_t scratch_bytes, haste_stream_t stream);
+
+/* The steps alone: out[i] (bf16, contiguous) is X for u = in[i] (all of in_type), NaN where in[i] is not finite.  Scratch as above. */
+int haste_orthogonalize(const void* const* in, void* const* out, const int64_t* rows, const int64_t* cols, int64_t count, int32_t in_type, int32_t steps, double a, double b, double c,
+                        double eps, void* scratch, int64_t scratch_bytes, haste_stream_t stream);
 
 /* Rate probes (measurement only; timed by the benchmark's auxiliary mode; no counterpart in the reference).  Each
  * isolates one access pattern of the fused train step at the step's own sizes:
