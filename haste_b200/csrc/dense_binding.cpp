@@ -425,7 +425,11 @@ PyObject* embedding_backward(PyObject* const* a) {
   const int64_t D = dy.size(-1), tokens = ids.t.numel();
   const auto [grad, stride] = rows_of(dy, D);
   at::Tensor out = empty_on(dev, {V, D}, type), scratch;
-  const int64_t bytes = lib.embedding_backward_scratch(tokens, D, V);
+  int64_t bytes = 0;
+  {
+    const c10::cuda::OptionalCUDAGuard guard(dy.device());
+    bytes = lib.embedding_backward_scratch(tokens, D, V);
+  }
   scratch = empty_on(dev, {bytes}, at::kByte);
   const void *gp = grad.data_ptr(), *ip = ids.t.data_ptr();
   void *op = out.data_ptr(), *sp = scratch.data_ptr();

@@ -11,6 +11,8 @@
 #include "launchers.h"
 #include "sm100.cuh"
 
+#include <cooperative_groups.h>
+
 namespace haste {
 namespace {
 
@@ -54,33 +56,66 @@ struct Vec<float> {
 };
 
 // ---------------------------------------------------------------- forward
-// An id that is no row of the table makes a row of NaN.
-template <class T, bool WHOLE>
-__global__ void __launch_bounds__(256) embedding_kernel(const Ids ids, const T* __restrict__ table, T* __restrict__ y, int64_t tokens, int64_t D, int64_t V, int64_t ld, float scale) {
+// An id that is no row of the table makes a row of NaN.  A thread has AHEAD pieces of 16 bytes of the output, all of whose ids and then rows are on their way at once.
+constexpr int FORWARD_THREADS = 256;
+template <class T, bool WHOLE, int AHEAD>
+__global__ void __launch_bounds__(FORWARD_THREADS) embedding_kernel(const Ids ids, const T* __restrict__ table, T* __restrict__ y, int64_t tokens, int64_t D, int64_t V, int64_t ld,
+                                                                    float scale) {
   constexpr int N = Vec<T>::N;
-  const int64_t n = tokens * D, pieces = (n + N - 1) / N, stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < pieces; i += stride) {
-    float v[N];
-    int64_t t = n <= 0x7FFFFFFF ? static_cast<uint32_t>(i * N) / static_cast<uint32_t>(D) : i * N / D, c = i * N - t * D;
-    if (WHOLE) {                                   // the piece lies in one row, on 16 bytes on both sides
-      const int64_t id = ids[t];
-      if (static_cast<uint64_t>(id) < static_cast<uint64_t>(V)) {
-        Vec<T>::unpack(__ldg(reinterpret_cast<const uint4*>(table + id * ld + c)), v);
+  const int64_t n = tokens * D, pieces = (n + N - 1) / N, first = static_cast<int64_t>(blockIdx.x) * (FORWARD_THREADS * AHEAD) + threadIdx.x;
+  const bool narrow = n <= 0x7FFFFFFF;
+  if (WHOLE) {                                     // a piece lies in one row, on 16 bytes on both sides
+    int64_t id[AHEAD], c[AHEAD];
+    uint4 q[AHEAD];
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] *= scale;
-      } else {
+    for (int k = 0; k < AHEAD; ++k) {
+      const int64_t i = first + k * FORWARD_THREADS;
+      id[k] = -1;
+      if (i < pieces) {
+        const int64_t t = narrow ? static_cast<uint32_t>(i * N) / static_cast<uint32_t>(D) : i * N / D;
+        c[k] = i * N - t * D;
+        id[k] = ids[t];
+      }
+    }
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = __int_as_float(0x7FFFFFFF);
+    for (int k = 0; k < AHEAD; ++k)
+      if (static_cast<uint64_t>(id[k]) < static_cast<uint64_t>(V)) q[k] = __ldg(reinterpret_cast<const uint4*>(table + id[k] * ld + c[k]));
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int64_t i = first + k * FORWARD_THREADS;
+      if (i >= pieces) break;
+      float v[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = __int_as_float(0x7FFFFFFF);
+      if (static_cast<uint64_t>(id[k]) < static_cast<uint64_t>(V)) {
+        Vec<T>::unpack(q[k], v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] *= scale;
       }
       *reinterpret_cast<uint4*>(y + i * N) = Vec<T>::pack(v);
-    } else {
-      int64_t id = ids[t];
+    }
+  } else {
+    // neighbouring elements by neighbouring threads
+    const int64_t from = static_cast<int64_t>(blockIdx.x) * (FORWARD_THREADS * AHEAD * N) + threadIdx.x;
+    int64_t id[AHEAD * N], c[AHEAD * N];
+    T x[AHEAD * N];
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        if (c == D) { c = 0; if (++t < tokens) id = ids[t]; }
-        if (t < tokens) y[i * N + k] = Vec<T>::put(static_cast<uint64_t>(id) < static_cast<uint64_t>(V) ? Vec<T>::get(table[id * ld + c]) * scale : __int_as_float(0x7FFFFFFF));
-        ++c;
+    for (int k = 0; k < AHEAD * N; ++k) {
+      const int64_t i = from + k * FORWARD_THREADS;
+      id[k] = -1;
+      if (i < n) {
+        const int64_t t = narrow ? static_cast<uint32_t>(i) / static_cast<uint32_t>(D) : i / D;
+        c[k] = i - t * D;
+        id[k] = ids[t];
       }
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD * N; ++k)
+      if (static_cast<uint64_t>(id[k]) < static_cast<uint64_t>(V)) x[k] = table[id[k] * ld + c[k]];
+#pragma unroll
+    for (int k = 0; k < AHEAD * N; ++k) {
+      const int64_t i = from + k * FORWARD_THREADS;
+      if (i < n) y[i] = Vec<T>::put(static_cast<uint64_t>(id[k]) < static_cast<uint64_t>(V) ? Vec<T>::get(x[k]) * scale : __int_as_float(0x7FFFFFFF));
     }
   }
 }
@@ -88,18 +123,32 @@ __global__ void __launch_bounds__(256) embedding_kernel(const Ids ids, const T* 
 // ---------------------------------------------------------------- sorting tokens by id
 constexpr int SORT_THREADS = 256, SORT_ITEMS = 16, SORT_TILE = SORT_THREADS * SORT_ITEMS, DIGITS = 256;
 
+// The lanes whose digit (up to DIGITS) is this lane's: nine votes, which take less time than one match
+__device__ __forceinline__ unsigned lanes_alike(int digit) {
+  unsigned same = 0xffffffffu;
+#pragma unroll
+  for (int bit = 0; bit < 9; ++bit) {
+    const bool set = (digit >> bit) & 1;
+    const unsigned votes = __ballot_sync(0xffffffffu, set);
+    same &= set ? votes : ~votes;
+  }
+  return same;
+}
+
 struct SortPass {
-  const int32_t *keys, *tokens;    // NULL in the first pass: from the ids
-  int32_t *keys_out, *tokens_out;
+  const int2* in;                  // key and token; NULL in the first pass: from the ids
+  int2* out;
   int32_t* counts;                 // [DIGITS][blocks]
   int64_t n;
   int shift, blocks;
 };
 // The id, or V where the token has no row or the row is the padding's
-__device__ __forceinline__ int32_t key_of(const SortPass& s, const Ids& ids, int64_t i, int64_t V, int64_t padding) {
-  if (s.keys != nullptr) return s.keys[i];
+__device__ __forceinline__ int2 first_item(const Ids& ids, int64_t i, int64_t V, int64_t padding) {
   const int64_t id = ids[i];
-  return static_cast<uint64_t>(id) < static_cast<uint64_t>(V) && id != padding ? static_cast<int32_t>(id) : static_cast<int32_t>(V);
+  return make_int2(static_cast<uint64_t>(id) < static_cast<uint64_t>(V) && id != padding ? static_cast<int32_t>(id) : static_cast<int32_t>(V), static_cast<int32_t>(i));
+}
+__device__ __forceinline__ int2 item_of(const SortPass& s, const Ids& ids, int64_t i, int64_t V, int64_t padding) {
+  return s.in != nullptr ? s.in[i] : first_item(ids, i, V, padding);
 }
 __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const SortPass s, const Ids ids, int64_t V, int64_t padding) {
   __shared__ int32_t count[DIGITS];
@@ -109,7 +158,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const SortPass
   const int64_t first = static_cast<int64_t>(blockIdx.x) * SORT_TILE;
   for (int k = 0; k < SORT_ITEMS; ++k) {
     const int64_t i = first + k * SORT_THREADS + threadIdx.x;
-    if (i < s.n) atomicAdd(&count[(key_of(s, ids, i, V, padding) >> s.shift) & (DIGITS - 1)], 1);
+    if (i < s.n) atomicAdd(&count[(item_of(s, ids, i, V, padding).x >> s.shift) & (DIGITS - 1)], 1);
   }
   __syncthreads();
   s.counts[static_cast<int64_t>(threadIdx.x) * s.blocks + blockIdx.x] = count[threadIdx.x];
@@ -160,17 +209,18 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(const SortPass
   sm100::grid_dependency_wait();
   __syncthreads();
   const int64_t first = static_cast<int64_t>(blockIdx.x) * SORT_TILE + warp * (32 * SORT_ITEMS) + lane;
-  int32_t key[SORT_ITEMS], rank[SORT_ITEMS];
+  int2 item[SORT_ITEMS];
+  int32_t rank[SORT_ITEMS];
 #pragma unroll
   for (int k = 0; k < SORT_ITEMS; ++k) {
     const int64_t i = first + 32 * k;
-    key[k] = i < s.n ? key_of(s, ids, i, V, padding) : 0;
+    item[k] = i < s.n ? item_of(s, ids, i, V, padding) : make_int2(0, 0);
   }
 #pragma unroll
   for (int k = 0; k < SORT_ITEMS; ++k) {
     const bool live = first + 32 * k < s.n;
-    const int digit = live ? (key[k] >> s.shift) & (DIGITS - 1) : DIGITS;
-    const unsigned same = __match_any_sync(0xffffffffu, digit);
+    const int digit = live ? (item[k].x >> s.shift) & (DIGITS - 1) : DIGITS;
+    const unsigned same = lanes_alike(digit);
     const int before = __popc(same & ((1u << lane) - 1));
     int32_t base = 0;
     if (live) base = count[warp][digit];
@@ -188,35 +238,137 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(const SortPass
   for (int k = 0; k < SORT_ITEMS; ++k) {
     const int64_t i = first + 32 * k;
     if (i < s.n) {
-      const int32_t to = count[warp][(key[k] >> s.shift) & (DIGITS - 1)] + rank[k];
-      s.keys_out[to] = key[k];
-      s.tokens_out[to] = s.tokens != nullptr ? s.tokens[i] : static_cast<int32_t>(i);
+      s.out[count[warp][(item[k].x >> s.shift) & (DIGITS - 1)] + rank[k]] = item[k];
     }
   }
 }
 
+// Up to CLUSTER_MOST tokens: one launch of one cluster, whose blocks keep the tokens in registers and shared memory.  In each pass every block places its tokens as above;
+// how many tokens of each digit the other blocks have comes through their shared memory, and so do the tokens themselves on their way to the block of their new place.
+constexpr int CLUSTER_THREADS = 1024, CLUSTER_BLOCKS = 16, CLUSTER_MOST = CLUSTER_BLOCKS * CLUSTER_THREADS * 8;
+template <int ITEMS>
+constexpr int cluster_smem() { return CLUSTER_THREADS * ITEMS * 8 + 32 * DIGITS * 2 + CLUSTER_BLOCKS * DIGITS * 4 + DIGITS * 4 + 64; }
+
+template <int ITEMS>
+__global__ void __launch_bounds__(CLUSTER_THREADS) sort_cluster_kernel(const Ids ids, int64_t n, int64_t V, int64_t padding, int passes, int2* __restrict__ out) {
+  constexpr int CHUNK = CLUSTER_THREADS * ITEMS;
+  extern __shared__ __align__(16) uint8_t raw[];
+  int2* items = reinterpret_cast<int2*>(raw);                                     // key, token
+  uint16_t* count = reinterpret_cast<uint16_t*>(raw + CHUNK * 8);                 // [32 warps][DIGITS]
+  int32_t* totals = reinterpret_cast<int32_t*>(raw + CHUNK * 8 + 32 * DIGITS * 2);        // [blocks][DIGITS]
+  int32_t* base = totals + CLUSTER_BLOCKS * DIGITS;
+  int32_t* sums = base + DIGITS;                                                  // [8]
+  cluster_started_arrive();
+  auto cluster = cooperative_groups::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank()), blocks = static_cast<int>(cluster.num_blocks()), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int first = warp * (32 * ITEMS) + lane;
+  const int live = static_cast<int>(min(static_cast<int64_t>(CHUNK), max(n - static_cast<int64_t>(rank) * CHUNK, static_cast<int64_t>(0))));
+  int2 item[ITEMS];
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int at = first + 32 * k;
+    item[k] = make_int2(0, 0);
+    if (at < live) {
+      item[k] = first_item(ids, static_cast<int64_t>(rank) * CHUNK + at, V, padding);
+    }
+  }
+  cluster_started_wait();
+  for (int p = 0; p < passes; ++p) {
+    const int shift = 8 * p;
+    for (int i = threadIdx.x; i < 32 * DIGITS / 2; i += CLUSTER_THREADS) reinterpret_cast<uint32_t*>(count)[i] = 0;
+    __syncthreads();
+    uint16_t place[ITEMS];
+    uint16_t* mine = count + warp * DIGITS;
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const bool there = first + 32 * k < live;
+      const int digit = there ? (item[k].x >> shift) & (DIGITS - 1) : DIGITS;
+      const unsigned same = lanes_alike(digit);
+      const int before = __popc(same & ((1u << lane) - 1));
+      int at = 0;
+      if (there) at = mine[digit];
+      __syncwarp();
+      if (there && before == 0) mine[digit] = static_cast<uint16_t>(at + __popc(same));
+      __syncwarp();
+      place[k] = static_cast<uint16_t>(at + before);
+    }
+    __syncthreads();
+    if (threadIdx.x < DIGITS) {
+      int sum = 0;
+#pragma unroll 8
+      for (int w = 0; w < 32; ++w) {
+        const int x = count[w * DIGITS + threadIdx.x];
+        count[w * DIGITS + threadIdx.x] = static_cast<uint16_t>(sum);
+        sum += x;
+      }
+      for (int b = 0; b < blocks; ++b) *cluster.map_shared_rank(&totals[rank * DIGITS + threadIdx.x], b) = sum;
+    }
+    cluster.sync();
+    if (threadIdx.x < DIGITS) {
+      int all = 0, before = 0;
+      for (int b = 0; b < blocks; ++b) {
+        const int x = totals[b * DIGITS + threadIdx.x];
+        if (b < rank) before += x;
+        all += x;
+      }
+      int up = all;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, up, o); if (lane >= o) up += x; }
+      if (lane == 31) sums[warp] = up;
+      base[threadIdx.x] = up - all + before;
+    }
+    __syncthreads();
+    if (threadIdx.x < DIGITS) {
+      int lower = 0;
+      for (int w = 0; w < warp; ++w) lower += sums[w];
+      base[threadIdx.x] += lower;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+      if (first + 32 * k < live) {
+        const int digit = (item[k].x >> shift) & (DIGITS - 1), to = base[digit] + mine[digit] + place[k];
+        if (p + 1 == passes) {
+          out[to] = item[k];
+        } else {
+          *cluster.map_shared_rank(&items[to % CHUNK], to / CHUNK) = item[k];
+        }
+      }
+    if (p + 1 == passes) break;
+    cluster.sync();
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+      if (first + 32 * k < live) item[k] = items[first + 32 * k];
+  }
+}
+
 // ---------------------------------------------------------------- sums
-constexpr int UNITS = 64;          // rows and tokens of a block
+constexpr int UNITS = 128;         // rows and tokens of a block, at most
 constexpr int SUM_THREADS = 128;
 
 // The list of things to do, at place d: v rows are written and i tokens read before it.  A row is written when its last token has been read.
-__device__ __forceinline__ int32_t rows_before(const int32_t* __restrict__ keys, int64_t n, int64_t V, int64_t d) {
+// By a warp: 32 places are looked at together, so that the search takes 4 reads after each other among 65536 tokens and not 16.
+__device__ __forceinline__ int32_t rows_before(const int2* __restrict__ sorted, int64_t n, int64_t V, int64_t d) {
   int64_t lo = d > V ? d - V : 0, hi = d < n ? d : n;              // the number of tokens among the first d
   while (lo < hi) {
-    const int64_t i = (lo + hi) >> 1;                              // is token i among them?  It is before the end of row keys[i], at place i + keys[i].
-    if (keys[i] <= d - 1 - i) lo = i + 1;
-    else hi = i;
+    const int64_t step = (hi - lo + 31) / 32, i = lo + (threadIdx.x & 31) * step;
+    // is token i among them?  It is before the end of its row, at place i + key.
+    const int c = __popc(__ballot_sync(0xffffffffu, i < hi && sorted[i].x <= d - 1 - i));
+    if (c == 0) break;
+    hi = min(hi, lo + c * step);
+    lo += (c - 1) * step + 1;
   }
   return static_cast<int32_t>(d - lo);
 }
 
 struct SumArgs {
-  const int32_t *keys, *tokens;    // sorted
-  int32_t* starts;                 // of each block and the end: the row that is worked on there
+  const int2* sorted;              // key and token
+  int32_t* starts;                 // of each block: the row that is worked on there
+  int32_t* joins;                  // of each block: that row, if others began it and this one ends it, else -1
   float *head, *tail;              // [blocks][D]: parts of a block's first row, begun before it, and of the row after its last one
   int64_t n, V, D, lddy;
   float scale;
-  int blocks;
+  int blocks, units;               // units: of a block
 };
 
 // WHOLE: pieces of 16 bytes on both sides; else a thread has every SUM_THREADS-th element
@@ -227,20 +379,23 @@ __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(const SumArg
   __shared__ int32_t todo[UNITS + AHEAD];          // a token, or ~row at its end
   __shared__ int32_t bounds[2];
   sm100::grid_dependency_wait();
-  const int64_t d0 = static_cast<int64_t>(blockIdx.x) * UNITS, all = a.V + a.n, d1 = d0 + UNITS < all ? d0 + UNITS : all;
-  if (threadIdx.x < 2) {
-    const int32_t v = rows_before(a.keys, a.n, a.V, threadIdx.x ? d1 : d0);
-    bounds[threadIdx.x] = v;
-    if (blockIdx.y == 0 && (threadIdx.x == 0 || d1 == all)) a.starts[blockIdx.x + threadIdx.x] = v;
+  const int64_t d0 = static_cast<int64_t>(blockIdx.x) * a.units, all = a.V + a.n, d1 = d0 + a.units < all ? d0 + a.units : all;
+  if (threadIdx.x < 64) {
+    const int which = threadIdx.x >> 5;
+    const int32_t v = rows_before(a.sorted, a.n, a.V, which ? d1 : d0);
+    if ((threadIdx.x & 31) == 0) {
+      bounds[which] = v;
+      if (blockIdx.y == 0 && which == 0) a.starts[blockIdx.x] = v;
+    }
   }
-  if (threadIdx.x < UNITS + AHEAD) todo[threadIdx.x] = INT32_MIN;
+  for (int i = threadIdx.x; i < UNITS + AHEAD; i += SUM_THREADS) todo[i] = INT32_MIN;
   __syncthreads();
   const int32_t v0 = bounds[0], v1 = bounds[1];
   const int64_t i0 = d0 - v0, i1 = d1 - v1;
   // tokens at their places, which those of their rows precede; the places left are rows' ends
   for (int64_t i = i0 + threadIdx.x; i < i1; i += SUM_THREADS) {
-    const int32_t key = a.keys[i];
-    if (key < a.V) todo[i + key - d0] = a.tokens[i];
+    const int2 it = a.sorted[i];
+    if (it.x < a.V) todo[i + it.x - d0] = it.y;
   }
   __syncthreads();
   const int units = static_cast<int>(d1 - d0);
@@ -255,7 +410,8 @@ __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(const SumArg
     }
   }
   __syncthreads();
-  const bool begun = i0 > 0 && v0 < a.V && a.keys[i0 - 1] == v0;                   // the first row has tokens before this block
+  const bool begun = i0 > 0 && v0 < a.V && a.sorted[i0 - 1].x == v0;                   // the first row has tokens before this block
+  if (blockIdx.y == 0 && threadIdx.x == 0 && a.n > 0) a.joins[blockIdx.x] = begun && v1 > v0 ? v0 : -1;
   const int64_t column = (static_cast<int64_t>(blockIdx.y) * SUM_THREADS + threadIdx.x) * N;
   const int64_t first = WHOLE ? column : static_cast<int64_t>(blockIdx.y) * SUM_THREADS * N + threadIdx.x;
   if (first >= a.D) return;
@@ -312,7 +468,7 @@ __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(const SumArg
       }
     }
   }
-  if (open < a.V && i1 > 0 && a.keys[i1 - 1] == open) {          // some of its tokens are read: here, or before
+  if (open < a.V && i1 > 0 && a.sorted[i1 - 1].x == open) {          // some of its tokens are read: here, or before
     float* h = a.tail + static_cast<int64_t>(blockIdx.x) * a.D;
 #pragma unroll
     for (int e = 0; e < N; ++e)
@@ -321,40 +477,44 @@ __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(const SumArg
 }
 
 // A block whose first row was begun before it, and ends in it: the parts of the blocks before, in order, and its own
-constexpr int JOIN_COLUMNS = 32, JOIN_GROUPS = 8;
+constexpr int JOIN_THREADS = 256;
 template <class T>
-__global__ void __launch_bounds__(JOIN_COLUMNS * JOIN_GROUPS) embedding_join_kernel(const SumArgs a, T* __restrict__ out) {
-  __shared__ float part[JOIN_GROUPS][JOIN_COLUMNS];
+__global__ void __launch_bounds__(JOIN_THREADS) embedding_join_kernel(const SumArgs a, T* __restrict__ out) {
   sm100::grid_dependency_wait();
   const int b = blockIdx.x;
-  const int32_t row = a.starts[b];
-  const int64_t i0 = static_cast<int64_t>(b) * UNITS - row;
-  if (b == 0 || row >= a.V || a.starts[b + 1] <= row || i0 == 0 || a.keys[i0 - 1] != row) return;
+  const int32_t row = a.joins[b], last = a.starts[b > 0 ? b - 1 : 0];
+  if (row < 0) return;
   // the first block whose tail is of this row: the last that started in an earlier row (or with this row's first token)
   int lo = 0, hi = b - 1;
+  if (last < row) lo = hi;                         // nearly always the one before
   while (lo < hi) {
     const int c = (lo + hi + 1) >> 1;
     const int32_t at = a.starts[c];
-    const int64_t i = static_cast<int64_t>(c) * UNITS - at;
-    if (at < row || i == 0 || a.keys[i - 1] != row) lo = c;
+    const int64_t i = static_cast<int64_t>(c) * a.units - at;
+    if (at < row || i == 0 || a.sorted[i - 1].x != row) lo = c;
     else hi = c - 1;
   }
-  const int group = threadIdx.x / JOIN_COLUMNS, x = threadIdx.x % JOIN_COLUMNS;
-  for (int64_t c0 = static_cast<int64_t>(blockIdx.y) * JOIN_COLUMNS; c0 < a.D; c0 += static_cast<int64_t>(gridDim.y) * JOIN_COLUMNS) {
-    const int64_t col = c0 + x;
-    float s = 0.f;
-    if (col < a.D) {
-#pragma unroll 4
-      for (int c = lo + group; c < b; c += JOIN_GROUPS) s += a.tail[static_cast<int64_t>(c) * a.D + col];
+  const float *t = a.tail + static_cast<int64_t>(lo) * a.D, *h = a.head + static_cast<int64_t>(b) * a.D;
+  T* o = out + static_cast<int64_t>(row) * a.D;
+  if (a.D % 4 == 0) {
+    for (int64_t col = (static_cast<int64_t>(blockIdx.y) * JOIN_THREADS + threadIdx.x) * 4; col < a.D; col += static_cast<int64_t>(gridDim.y) * JOIN_THREADS * 4) {
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int c = 0; c < b - lo; ++c) {
+        const float4 x = *reinterpret_cast<const float4*>(t + static_cast<int64_t>(c) * a.D + col);
+        s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+      }
+      const float4 x = *reinterpret_cast<const float4*>(h + col);
+      o[col] = Vec<T>::put((s.x + x.x) * a.scale); o[col + 1] = Vec<T>::put((s.y + x.y) * a.scale);
+      o[col + 2] = Vec<T>::put((s.z + x.z) * a.scale); o[col + 3] = Vec<T>::put((s.w + x.w) * a.scale);
     }
-    part[group][x] = s;
-    __syncthreads();
-    if (group == 0 && col < a.D) {
-      for (int g = 1; g < JOIN_GROUPS; ++g) s += part[g][x];
-      s += a.head[static_cast<int64_t>(b) * a.D + col];
-      out[static_cast<int64_t>(row) * a.D + col] = Vec<T>::put(s * a.scale);
+  } else {
+    for (int64_t col = static_cast<int64_t>(blockIdx.y) * JOIN_THREADS + threadIdx.x; col < a.D; col += static_cast<int64_t>(gridDim.y) * JOIN_THREADS) {
+      float s = 0.f;
+#pragma unroll 8
+      for (int c = 0; c < b - lo; ++c) s += t[static_cast<int64_t>(c) * a.D + col];
+      o[col] = Vec<T>::put((s + h[col]) * a.scale);
     }
-    __syncthreads();
   }
 }
 
@@ -365,7 +525,12 @@ int passes_of(int64_t V) {         // over the digits of keys 0 .. V
   return n;
 }
 int sort_blocks(int64_t tokens) { return static_cast<int>((tokens + SORT_TILE - 1) / SORT_TILE); }
-int64_t sum_blocks(int64_t tokens, int64_t V) { return (tokens + V + UNITS - 1) / UNITS; }
+// Rows and tokens of a block: as many as make one round of all SMs, 7 blocks each
+int units_of(int64_t tokens, int64_t V, int64_t D) {
+  const int64_t pieces = (D + 511) / 512, rounds = static_cast<int64_t>(sm_count()) * 7;
+  const int64_t units = ((tokens + V) * pieces + rounds - 1) / rounds;
+  return static_cast<int>(units < 8 ? 8 : units > UNITS ? UNITS : units);
+}
 
 template <class G, class T>
 int sums(const SumArgs& a, const void* dy, void* out, cudaStream_t st) {
@@ -386,8 +551,9 @@ int sums(const SumArgs& a, const void* dy, void* out, cudaStream_t st) {
   T* o = static_cast<T*>(out);
   cudaError_t e = whole ? cudaLaunchKernelEx(&cfg, embedding_sum_kernel<G, T, true>, a, g, o) : cudaLaunchKernelEx(&cfg, embedding_sum_kernel<G, T, false>, a, g, o);
   if (e == cudaSuccess && a.n > 0) {
-    cfg.gridDim = dim3(grid.x, static_cast<unsigned>(imin64((a.D + JOIN_COLUMNS - 1) / JOIN_COLUMNS, 32)));
-    cfg.blockDim = dim3(JOIN_COLUMNS * JOIN_GROUPS);
+    const int64_t columns = JOIN_THREADS * (a.D % 4 == 0 ? 4 : 1);
+    cfg.gridDim = dim3(grid.x, static_cast<unsigned>(imin64((a.D + columns - 1) / columns, 16)));
+    cfg.blockDim = dim3(JOIN_THREADS);
     cfg.numAttrs = 1;
     e = cudaLaunchKernelEx(&cfg, embedding_join_kernel<T>, a, o);
   }
@@ -397,28 +563,58 @@ int sums(const SumArgs& a, const void* dy, void* out, cudaStream_t st) {
 
 }  // namespace
 
-int launch_embedding_forward(const void* ids, int wide, const void* table, void* y, int64_t tokens, int64_t D, int64_t V, int64_t ld, float scale, int type, cudaStream_t st) {
-  if (tokens == 0) return HASTE_OK;
-  const int n = type == HASTE_BF16 ? 8 : 4;
-  const bool whole = D % n == 0 && ld % n == 0 && aligned16(table) && aligned16(y);
-  const int64_t pieces = (tokens * D + n - 1) / n;
-  const unsigned grid = static_cast<unsigned>(imin64((pieces + 255) / 256, static_cast<int64_t>(sm_count()) * 64));
-  const Ids i = {ids, wide};
-  if (type == HASTE_BF16) {
-    using B = __nv_bfloat16;
-    if (whole) embedding_kernel<B, true><<<grid, 256, 0, st>>>(i, static_cast<const B*>(table), static_cast<B*>(y), tokens, D, V, ld, scale);
-    else embedding_kernel<B, false><<<grid, 256, 0, st>>>(i, static_cast<const B*>(table), static_cast<B*>(y), tokens, D, V, ld, scale);
-  } else if (whole) {
-    embedding_kernel<float, true><<<grid, 256, 0, st>>>(i, static_cast<const float*>(table), static_cast<float*>(y), tokens, D, V, ld, scale);
-  } else {
-    embedding_kernel<float, false><<<grid, 256, 0, st>>>(i, static_cast<const float*>(table), static_cast<float*>(y), tokens, D, V, ld, scale);
-  }
+template <class T>
+static int forward_typed(const Ids& ids, const void* table, void* y, int64_t tokens, int64_t D, int64_t V, int64_t ld, float scale, cudaStream_t st) {
+  constexpr int N = Vec<T>::N;
+  const bool whole = D % N == 0 && ld % N == 0 && aligned16(table) && aligned16(y);
+  const int64_t pieces = (tokens * D + N - 1) / N, most = static_cast<int64_t>(sm_count()) * 8 * FORWARD_THREADS;
+  const T* from = static_cast<const T*>(table);
+  T* to = static_cast<T*>(y);
+  const bool few = pieces <= most;                 // as many threads as run at once have one piece each
+  const int64_t per = FORWARD_THREADS * (few || !whole ? 1 : 4);
+  const unsigned grid = static_cast<unsigned>((pieces + per - 1) / per);
+  if (!whole) embedding_kernel<T, false, 1><<<grid, FORWARD_THREADS, 0, st>>>(ids, from, to, tokens, D, V, ld, scale);
+  else if (few) embedding_kernel<T, true, 1><<<grid, FORWARD_THREADS, 0, st>>>(ids, from, to, tokens, D, V, ld, scale);
+  else embedding_kernel<T, true, 4><<<grid, FORWARD_THREADS, 0, st>>>(ids, from, to, tokens, D, V, ld, scale);
   return check_launch("embedding_kernel");
 }
 
+int launch_embedding_forward(const void* ids, int wide, const void* table, void* y, int64_t tokens, int64_t D, int64_t V, int64_t ld, float scale, int type, cudaStream_t st) {
+  if (tokens == 0) return HASTE_OK;
+  const Ids i = {ids, wide};
+  return type == HASTE_BF16 ? forward_typed<__nv_bfloat16>(i, table, y, tokens, D, V, ld, scale, st) : forward_typed<float>(i, table, y, tokens, D, V, ld, scale, st);
+}
+
 int64_t embedding_backward_scratch(int64_t tokens, int64_t D, int64_t V) {
-  if (tokens == 0) return 256 + up256((sum_blocks(0, V) + 1) * 4);
-  return 4 * up256(tokens * 4) + up256(static_cast<int64_t>(sort_blocks(tokens)) * DIGITS * 4) + up256((sum_blocks(tokens, V) + 1) * 4) + 2 * up256(sum_blocks(tokens, V) * D * 4);
+  const int64_t blocks = (tokens + V + units_of(tokens, V, D) - 1) / units_of(tokens, V, D);
+  const int64_t starts = 2 * up256(blocks * 4);
+  if (tokens == 0) return starts;
+  const int64_t sorting = tokens <= CLUSTER_MOST ? up256(tokens * 8) : 2 * up256(tokens * 8) + up256(static_cast<int64_t>(sort_blocks(tokens)) * DIGITS * 4);
+  return sorting + starts + 2 * up256(blocks * D * 4);
+}
+
+template <int ITEMS>
+static int sort_in_cluster(const Ids& ids, int64_t tokens, int64_t V, int64_t padding, int2* out, cudaStream_t st) {
+  auto kernel = sort_cluster_kernel<ITEMS>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, cluster_smem<ITEMS>());
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  unsigned blocks = 1;
+  while (static_cast<int64_t>(blocks) * CLUSTER_THREADS * ITEMS < tokens) blocks *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(CLUSTER_THREADS);
+  cfg.dynamicSmemBytes = cluster_smem<ITEMS>();
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = blocks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, ids, tokens, V, padding, passes_of(V), out);
+  if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaLaunchKernelEx: %s", cudaGetErrorString(e));
+  return HASTE_OK;
 }
 
 int launch_embedding_backward(const void* ids, int wide, const void* dy, void* dtable, void* scratch, int64_t tokens, int64_t D, int64_t V, int64_t lddy, float scale, int64_t padding,
@@ -426,18 +622,25 @@ int launch_embedding_backward(const void* ids, int wide, const void* dy, void* d
   char* mem = static_cast<char*>(scratch);
   auto take = [&](int64_t bytes) { char* p = mem; mem += up256(bytes); return p; };
   const Ids i = {ids, wide};
-  int32_t *keys[2], *toks[2];
-  for (int k = 0; k < 2; ++k) { keys[k] = reinterpret_cast<int32_t*>(take(tokens * 4)); toks[k] = reinterpret_cast<int32_t*>(take(tokens * 4)); }
-  SortPass s = {};
-  s.n = tokens; s.blocks = sort_blocks(tokens);
-  s.counts = reinterpret_cast<int32_t*>(take(static_cast<int64_t>(s.blocks) * DIGITS * 4));
+  int2* pairs[2] = {};
   int cur = 0;
-  if (tokens > 0) {
+  if (tokens > 0 && tokens <= CLUSTER_MOST) {
+    pairs[0] = reinterpret_cast<int2*>(take(tokens * 8));
+    int rc = 0;
+    if (tokens <= CLUSTER_MOST / 8) rc = sort_in_cluster<1>(i, tokens, V, padding, pairs[0], st);
+    else if (tokens <= CLUSTER_MOST / 2) rc = sort_in_cluster<4>(i, tokens, V, padding, pairs[0], st);
+    else rc = sort_in_cluster<8>(i, tokens, V, padding, pairs[0], st);
+    if (rc) return rc;
+  } else if (tokens > 0) {
+    for (int k = 0; k < 2; ++k) pairs[k] = reinterpret_cast<int2*>(take(tokens * 8));
+    SortPass s = {};
+    s.n = tokens; s.blocks = sort_blocks(tokens);
+    s.counts = reinterpret_cast<int32_t*>(take(static_cast<int64_t>(s.blocks) * DIGITS * 4));
     const int passes = passes_of(V);
     for (int p = 0; p < passes; ++p, cur ^= 1) {
       s.shift = 8 * p;
-      s.keys = p ? keys[cur ^ 1] : nullptr; s.tokens = p ? toks[cur ^ 1] : nullptr;
-      s.keys_out = keys[cur]; s.tokens_out = toks[cur];
+      s.in = p ? pairs[cur ^ 1] : nullptr;
+      s.out = pairs[cur];
       if (p == 0) {
         sort_count_kernel<<<s.blocks, SORT_THREADS, 0, st>>>(s, i, V, padding);
         if (int rc = check_launch("sort_count_kernel")) return rc;
@@ -450,10 +653,12 @@ int launch_embedding_backward(const void* ids, int wide, const void* dy, void* d
     cur ^= 1;
   }
   SumArgs a = {};
-  a.keys = keys[cur]; a.tokens = toks[cur];
+  a.sorted = pairs[cur];
   a.n = tokens; a.V = V; a.D = D; a.lddy = lddy; a.scale = scale;
-  a.blocks = static_cast<int>(sum_blocks(tokens, V));
-  a.starts = reinterpret_cast<int32_t*>(take((a.blocks + 1) * static_cast<int64_t>(4)));
+  a.units = units_of(tokens, V, D);
+  a.blocks = static_cast<int>((tokens + V + a.units - 1) / a.units);
+  a.starts = reinterpret_cast<int32_t*>(take(a.blocks * static_cast<int64_t>(4)));
+  a.joins = reinterpret_cast<int32_t*>(take(a.blocks * static_cast<int64_t>(4)));
   if (tokens > 0) {
     a.head = reinterpret_cast<float*>(take(a.blocks * D * 4));
     a.tail = reinterpret_cast<float*>(take(a.blocks * D * 4));

@@ -97,6 +97,18 @@ def test_many_rows_and_few_tokens():
     assert int(got.any(1).sum()) == 4
 
 
+@pytest.mark.parametrize("tokens", [1024, 1025, 2048, 2049, 16384, 16385, 65536, 65537, 131072, 131073, 200001])
+def test_numbers_of_tokens_at_which_the_sort_changes(tokens):
+    from haste_b200.embedding import embedding_backward
+    gen = torch.Generator().manual_seed(tokens)
+    for rows, kind in ((200, "words"), (70000, "even"), (300, "one")):
+        ids = _ids(tokens, rows, kind, gen).cuda()
+        dy = torch.randn(tokens, 12, generator=gen).cuda()
+        got = embedding_backward(dy, ids, rows)
+        _check_grad(got, dy, ids, rows, 1.0)
+        assert torch.equal(got, embedding_backward(dy, ids, rows))
+
+
 def test_strides_shapes_and_no_tokens():
     from haste_b200.embedding import embedding_backward, embedding_forward
     wide = torch.randn(50, 80, device="cuda")
