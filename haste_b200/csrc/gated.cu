@@ -9,11 +9,14 @@
 // next product or what training keeps, and 2^-8 of each value adds in squares to the result's own rounding.  Up to GEMV_ROWS rows the weights are streamed through CUDA cores instead.
 #include "gemm_sm100.cuh"
 
+#include <type_traits>
+
 namespace haste {
 namespace {
 
+using gemm::Operand;
 using gemm::Problem;
-using gemm::Stager;
+using gemm::steps_of;
 using gemm::Tile;
 using gemm::Work;
 
@@ -54,37 +57,34 @@ __device__ __forceinline__ float activate(float g) {
 template <int ACT>
 struct GatedForward {
   static constexpr bool A_MN = false, B_MN = false, F16 = false, PAIRED_B = true;
-  template <int P>
-  static __device__ __forceinline__ void epilogue(const Work<P>& w, const Problem& p, const Tile& t, int row0, int half, uint32_t tmem, Stager& st, int lane) {
-    const bool keep = w.scale0 != 0.f;
-#pragma unroll 1
-    for (int j = 0; j < 2; ++j) {
-      const int at = half * 64 + j * 32, col = t.n * 128 + at;
-      const bool inside = row0 < p.M && col < p.N;
-      uint32_t g[32], u[32], packed[16];
-      sm100::tmem_ld32(tmem + at, g);
-      sm100::tmem_ld32(tmem + 128 + at, u);
-      sm100::tmem_ld_wait();
-      if (keep) {
+  static constexpr int INPUTS = 0;
+  template <class W, class I, class S>
+  static __device__ __forceinline__ void chunk(const W& w, const Problem& p, const Tile& t, int row0, int col, bool, uint32_t tmem, I&, S& st, int lane) {
+    constexpr int OTHER = I::L::COLUMNS;             // up's accumulator stands behind gate's
+    const bool inside = row0 < p.M && col < p.N;
+    uint32_t g[32], u[32], packed[16];
+    sm100::tmem_ld32(tmem, g);
+    sm100::tmem_ld32(tmem + OTHER, u);
+    sm100::tmem_ld_wait();
+    if (w.scale0 != 0.f) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) packed[i] = gemm::pack_bf16(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
-        uint32_t box = st.get();
-        gemm::box_row(box, lane, packed);
-        st.put(&p.out[0], box, col, row0, t.batch, inside);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) packed[i] = gemm::pack_bf16(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
-        box = st.get();
-        gemm::box_row(box, lane, packed);
-        st.put(&p.out[1], box, col, row0, t.batch, inside);
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        packed[i] = gemm::pack_bf16(activate<ACT>(__uint_as_float(g[2 * i])) * __uint_as_float(u[2 * i]),
-                                    activate<ACT>(__uint_as_float(g[2 * i + 1])) * __uint_as_float(u[2 * i + 1]));
-      const uint32_t box = st.get();
+      for (int i = 0; i < 16; ++i) packed[i] = gemm::pack_bf16(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
+      uint32_t box = st.get();
       gemm::box_row(box, lane, packed);
-      st.put(&p.out[2], box, col, row0, t.batch, inside);
+      st.put(&p.out[0], box, col, row0, t.batch, inside);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) packed[i] = gemm::pack_bf16(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+      box = st.get();
+      gemm::box_row(box, lane, packed);
+      st.put(&p.out[1], box, col, row0, t.batch, inside);
     }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      packed[i] = gemm::pack_bf16(activate<ACT>(__uint_as_float(g[2 * i])) * __uint_as_float(u[2 * i]),
+                                  activate<ACT>(__uint_as_float(g[2 * i + 1])) * __uint_as_float(u[2 * i + 1]));
+    const uint32_t box = st.get();
+    gemm::box_row(box, lane, packed);
+    st.put(&p.out[2], box, col, row0, t.batch, inside);
   }
 };
 
@@ -92,40 +92,36 @@ struct GatedForward {
 template <int ACT>
 struct GatedBackward {
   static constexpr bool A_MN = false, B_MN = true, F16 = false, PAIRED_B = false;
-  template <int P>
-  static __device__ __forceinline__ void epilogue(const Work<P>&, const Problem& p, const Tile& t, int row0, int half, uint32_t tmem, Stager& st, int lane) {
-    const int row = row0 + lane;
-#pragma unroll 1
-    for (int j = 0; j < 4; ++j) {
-      const int at = half * 128 + j * 32, col = t.n * gemm::TILE + at;
-      const bool inside = row0 < p.M && col < p.N;
-      uint32_t g[16], u[16], d[32];
-      gemm::load_row(g, p.in[0] + static_cast<int64_t>(row) * p.ld_in, col, p.ld_in, row < p.M);
-      gemm::load_row(u, p.in[1] + static_cast<int64_t>(row) * p.ld_in, col, p.ld_in, row < p.M);
-      sm100::tmem_ld32(tmem + at, d);
-      sm100::tmem_ld_wait();
-      uint32_t dup[16], h[16];
+  static constexpr int INPUTS = 2;
+  template <class W, class I, class S>
+  static __device__ __forceinline__ void chunk(const W&, const Problem& p, const Tile& t, int row0, int col, bool, uint32_t tmem, I& in, S& st, int lane) {
+    const bool inside = row0 < p.M && col < p.N;
+    uint32_t g[16], u[16], d[32], dup[16], h[16];
+    sm100::tmem_ld32(tmem, d);
+    in.get(0, g);
+    in.get(1, u);
+    in.release();
+    sm100::tmem_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float2 gg = gemm::unpack_bf16(g[i]), uu = gemm::unpack_bf16(u[i]);
-        const float d0 = __uint_as_float(d[2 * i]), d1 = __uint_as_float(d[2 * i + 1]);
-        float a0, s0, a1, s1;
-        activation<ACT>(gg.x, a0, s0);
-        activation<ACT>(gg.y, a1, s1);
-        g[i] = gemm::pack_bf16(d0 * uu.x * s0, d1 * uu.y * s1);
-        dup[i] = gemm::pack_bf16(d0 * a0, d1 * a1);
-        h[i] = gemm::pack_bf16(a0 * uu.x, a1 * uu.y);
-      }
-      uint32_t box = st.get();
-      gemm::box_row(box, lane, g);
-      st.put(&p.out[0], box, col, row0, t.batch, inside);
-      box = st.get();
-      gemm::box_row(box, lane, dup);
-      st.put(&p.out[1], box, col, row0, t.batch, inside);
-      box = st.get();
-      gemm::box_row(box, lane, h);
-      st.put(&p.out[2], box, col, row0, t.batch, inside);
+    for (int i = 0; i < 16; ++i) {
+      const float2 gg = gemm::unpack_bf16(g[i]), uu = gemm::unpack_bf16(u[i]);
+      const float d0 = __uint_as_float(d[2 * i]), d1 = __uint_as_float(d[2 * i + 1]);
+      float a0, s0, a1, s1;
+      activation<ACT>(gg.x, a0, s0);
+      activation<ACT>(gg.y, a1, s1);
+      g[i] = gemm::pack_bf16(d0 * uu.x * s0, d1 * uu.y * s1);
+      dup[i] = gemm::pack_bf16(d0 * a0, d1 * a1);
+      h[i] = gemm::pack_bf16(a0 * uu.x, a1 * uu.y);
     }
+    uint32_t box = st.get();
+    gemm::box_row(box, lane, g);
+    st.put(&p.out[0], box, col, row0, t.batch, inside);
+    box = st.get();
+    gemm::box_row(box, lane, dup);
+    st.put(&p.out[1], box, col, row0, t.batch, inside);
+    box = st.get();
+    gemm::box_row(box, lane, h);
+    st.put(&p.out[2], box, col, row0, t.batch, inside);
   }
 };
 
@@ -133,31 +129,28 @@ struct GatedBackward {
 template <bool A, bool B>
 struct Plain {
   static constexpr bool A_MN = A, B_MN = B, F16 = false, PAIRED_B = false;
-  template <int P>
-  static __device__ __forceinline__ void epilogue(const Work<P>&, const Problem& p, const Tile& t, int row0, int half, uint32_t tmem, Stager& st, int lane) {
-#pragma unroll 1
-    for (int j = 0; j < 4; ++j) {
-      const int at = half * 128 + j * 32, col = t.n * gemm::TILE + at;
-      uint32_t v[32];
-      sm100::tmem_ld32(tmem + at, v);
-      sm100::tmem_ld_wait();
-      if (p.partial != nullptr) {
-        const int64_t ld = (p.N + 3) & ~3;
-        if (row0 + lane < p.M) {
-          float* to = p.partial + (static_cast<int64_t>(t.split) * p.M + row0 + lane) * ld;
+  static constexpr int INPUTS = 0;
+  template <class W, class I, class S>
+  static __device__ __forceinline__ void chunk(const W&, const Problem& p, const Tile& t, int row0, int col, bool, uint32_t tmem, I&, S& st, int lane) {
+    uint32_t v[32];
+    sm100::tmem_ld32(tmem, v);
+    sm100::tmem_ld_wait();
+    if (p.partial != nullptr) {
+      const int64_t ld = (p.N + 3) & ~3;
+      if (row0 + lane < p.M) {
+        float* to = p.partial + (static_cast<int64_t>(t.split) * p.M + row0 + lane) * ld;
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (col + 4 * i < ld)
-              *reinterpret_cast<uint4*>(to + col + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        }
-      } else {
-        uint32_t packed[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) packed[i] = gemm::pack_bf16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-        const uint32_t box = st.get();
-        gemm::box_row(box, lane, packed);
-        st.put(&p.out[0], box, col, row0, t.batch, row0 < p.M && col < p.N);
+        for (int i = 0; i < 8; ++i)
+          if (col + 4 * i < ld)
+            *reinterpret_cast<uint4*>(to + col + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
       }
+    } else {
+      uint32_t packed[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) packed[i] = gemm::pack_bf16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+      const uint32_t box = st.get();
+      gemm::box_row(box, lane, packed);
+      st.put(&p.out[0], box, col, row0, t.batch, row0 < p.M && col < p.N);
     }
   }
 };
@@ -367,21 +360,23 @@ struct Aligner {
   }
 };
 
-// A product M x N over `steps` of k is cut along k where its tiles leave SMs idle.  In units of a step of k of one tile (0.28 us): a tile costs its steps and
-// 6 more, the parts are written and read once at 6 TB/s, the launch that adds them takes 2 us.
-int choose_splits(int64_t tiles, int64_t steps, int64_t elements) {
-  const int64_t pairs = sm_count() / 2;
-  int best = 1;
+// The form of a launch, and into how many parts k is cut where its tiles leave SMs idle: the parts are written and read once at 6 TB/s, the launch that adds
+// them takes 2 us.
+struct Form {
+  bool narrow;
+  int splits;
+};
+Form choose_form(int64_t wide, int64_t narrow, int64_t steps, int64_t elements) {
+  Form best = {false, 1};
   double cost = 0;
-  for (int s = 1; s <= 16 && s <= steps; ++s) {
-    const double c = static_cast<double>((tiles * s + pairs - 1) / pairs) * (static_cast<double>((steps + s - 1) / s) + 6) +
-                     (s > 1 ? 7 + static_cast<double>(elements) * s * 8 / 6e6 / 0.28 : 0);
-    if (s == 1 || c < cost) { best = s; cost = c; }
-  }
+  for (int s = 1; s <= 16 && s <= steps; ++s)
+    for (int n = 0; n < 2; ++n) {
+      const double c = gemm::cost_of((n ? narrow : wide) * s, (steps + s - 1) / s, n != 0) + (s > 1 ? 7 + static_cast<double>(elements) * s * 8 / 6e6 / 0.28 : 0);
+      if ((s == 1 && n == 0) || c < cost) { best = {n != 0, s}; cost = c; }
+    }
   return best;
 }
-int64_t tiles_for(int64_t M, int64_t N) { return ((M + gemm::TILE - 1) / gemm::TILE) * ((N + gemm::TILE - 1) / gemm::TILE); }
-int64_t k_steps(int64_t K) { return (K + gemm::KSTEP - 1) / gemm::KSTEP; }
+Form form_for(int64_t M, int64_t N, int64_t steps) { return choose_form(gemm::tiles_for(M, N, gemm::TILE), gemm::tiles_for(M, N, 64), steps, M * N); }
 
 // out [M, N] contiguous at any alignment: straight from the tiles, or through fp32 parts
 struct Output {
@@ -389,21 +384,23 @@ struct Output {
   float* part;
   int splits;
 };
-Output output_of(Arena& arena, void* p, int64_t M, int64_t N, int64_t tiles, int64_t steps, bool always) {
-  Output o = {p, nullptr, choose_splits(tiles, steps, M * N)};
+Output output_of(Arena& arena, void* p, int64_t M, int64_t N, const Form& f, bool always) {
+  Output o = {p, nullptr, f.splits};
   if (always || o.splits > 1 || N % 8 != 0 || !aligned16(p))
     o.part = static_cast<float*>(arena.take(o.splits * M * ((N + 3) & ~int64_t(3)) * 4));
   return o;
 }
-int set_product(Problem& p, const Output& o, int64_t M, int64_t N, int64_t steps0, int64_t steps) {
+void set_sizes(Problem& p, int64_t M, int64_t N, int64_t steps0, int64_t steps) {
   p = Problem();
   p.M = static_cast<int>(M); p.N = static_cast<int>(N);
-  p.tiles_m = static_cast<int>((M + gemm::TILE - 1) / gemm::TILE); p.tiles_n = static_cast<int>((N + gemm::TILE - 1) / gemm::TILE);
-  p.batch = 1; p.splits = o.splits;
+  p.batch = p.splits = 1;
   p.steps0 = static_cast<int>(steps0); p.steps = static_cast<int>(steps);
+}
+template <class Policy>
+int set_output(Problem& p, const Output& o) {
+  p.splits = o.splits;
   p.partial = o.part;
-  if (o.part == nullptr) return gemm::make_map(&p.out[0], o.p, false, N, M, 1, N, 0, gemm::BOX_STORE);
-  return HASTE_OK;
+  return o.part == nullptr ? gemm::map_result<Policy>(&p.out[0], {o.p, p.N, 0}, p.M, p.N) : HASTE_OK;
 }
 void add_sum(Sums& s, const Output& o, int64_t M, int64_t N) {
   if (o.part == nullptr) return;
@@ -418,18 +415,27 @@ int run_sums(const Sums& s, cudaStream_t st) {
   return launch_behind(sum_parts_kernel, static_cast<unsigned>(imin64(blocks, static_cast<int64_t>(sm_count()) * 16)), 256, st, s);
 }
 
-template <template <int> class Policy>
-int launch_by_activation(int act, Work<1>& w, bool behind, cudaStream_t st) {
+#define HASTE_TRY(...) \
+  if (int rc_ = (__VA_ARGS__)) return rc_
+
+// f(policy of the activation, number of columns of the form) for a launch
+template <template <int> class Policy, class F>
+int by_activation(int act, bool narrow, F&& f) {
+  auto with = [&](auto policy) -> int {
+    using K = decltype(policy);
+    return narrow ? f(policy, std::integral_constant<int, gemm::narrow<K>()>()) : f(policy, std::integral_constant<int, 256>());
+  };
   switch (act) {
-    case SILU: return gemm::launch<Policy<SILU>>(w, behind, st);
-    case GELU: return gemm::launch<Policy<GELU>>(w, behind, st);
-    case GELU_TANH: return gemm::launch<Policy<GELU_TANH>>(w, behind, st);
-    default: return gemm::launch<Policy<RELU>>(w, behind, st);
+    case SILU: return with(Policy<SILU>());
+    case GELU: return with(Policy<GELU>());
+    case GELU_TANH: return with(Policy<GELU_TANH>());
+    default: return with(Policy<RELU>());
   }
 }
-
-#define HASTE_TRY(e) \
-  if (int rc_ = (e)) return rc_
+template <class Policy, class F>
+int by_form(bool narrow, F&& f) {
+  return narrow ? f(Policy(), std::integral_constant<int, gemm::narrow<Policy>()>()) : f(Policy(), std::integral_constant<int, 256>());
+}
 
 template <int ACT>
 int few_rows_act(bool vec, int64_t T, const void* x, int64_t ldx, const void* wg, const void* wu, const void* wd, void* gate, void* up, int64_t ldh, void* y, float* h, int64_t D, int64_t F,
@@ -453,34 +459,43 @@ int forward(Arena& arena, const GatedCall& c, cudaStream_t st) {
       default: return few_rows_act<RELU>(vec, c.T, c.x, c.ldx, c.wg, c.wu, c.wd, c.gate, c.up, c.ldh, c.y, h, c.D, c.F, c.O, st);
     }
   }
-  const int64_t ldF = up8(c.F);
+  const int64_t ldF = up8(c.F), sD = steps_of(c.D), sF = steps_of(c.F);
   Aligner align(arena);
   const Rows x = align(c.x, c.ldx, c.T, c.D, any), wg = align(c.wg, c.D, c.F, c.D, any), wu = align(c.wu, c.D, c.F, c.D, any), wd = align(c.wd, c.F, c.O, c.F, any);
   void* h = arena.take(c.T * ldF * 2);
-  const Output y = output_of(arena, c.y, c.T, c.O, tiles_for(c.T, c.O), k_steps(c.F), any);
+  const Form fy = form_for(c.T, c.O, sF);
+  const Output y = output_of(arena, c.y, c.T, c.O, fy, any);
   if (plan) return HASTE_OK;
   HASTE_TRY(align.run(st));
   Work<1> w = {};
   w.problems = 1;
   w.scale0 = c.gate != nullptr ? 1.f : 0.f;
-  Problem& p = w.p[0];
-  p.M = static_cast<int>(c.T); p.N = static_cast<int>(c.F);
-  p.tiles_m = static_cast<int>((c.T + gemm::TILE - 1) / gemm::TILE); p.tiles_n = static_cast<int>((c.F + 127) / 128);
-  p.batch = p.splits = 1;
-  p.steps0 = p.steps = static_cast<int>(k_steps(c.D));
-  HASTE_TRY(gemm::make_map(&p.a[0], x.p, false, c.D, c.T, 1, x.ld, 0, gemm::BOX_K));
-  HASTE_TRY(gemm::make_map(&p.b[0], wg.p, false, c.D, c.F, 1, wg.ld, 0, gemm::BOX_K));
-  HASTE_TRY(gemm::make_map(&p.b[1], wu.p, false, c.D, c.F, 1, wu.ld, 0, gemm::BOX_K));
-  if (c.gate != nullptr) {
-    HASTE_TRY(gemm::make_map(&p.out[0], c.gate, false, c.F, c.T, 1, c.ldh, 0, gemm::BOX_STORE));
-    HASTE_TRY(gemm::make_map(&p.out[1], c.up, false, c.F, c.T, 1, c.ldh, 0, gemm::BOX_STORE));
-  }
-  HASTE_TRY(gemm::make_map(&p.out[2], h, false, c.F, c.T, 1, ldF, 0, gemm::BOX_STORE));
-  HASTE_TRY(launch_by_activation<GatedForward>(c.act, w, align.c.n > 0, st));
-  HASTE_TRY(set_product(p, y, c.T, c.O, k_steps(c.F), k_steps(c.F)));
-  HASTE_TRY(gemm::make_map(&p.a[0], h, false, c.F, c.T, 1, ldF, 0, gemm::BOX_K));
-  HASTE_TRY(gemm::make_map(&p.b[0], wd.p, false, c.F, c.O, 1, wd.ld, 0, gemm::BOX_K));
-  HASTE_TRY((gemm::launch<Plain<false, false>>(w, true, st)));
+  const bool narrow = gemm::cost_of(gemm::tiles_for(c.T, c.F, 64), sD, true) < gemm::cost_of(gemm::tiles_for(c.T, c.F, 128), sD, false);
+  HASTE_TRY(by_activation<GatedForward>(c.act, narrow, [&](auto policy, auto columns) -> int {
+    using K = decltype(policy);
+    constexpr int TN = decltype(columns)::value;
+    Problem& p = w.p[0];
+    set_sizes(p, c.T, c.F, sD, sD);
+    HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], {x.p, x.ld, 0}, c.T, c.D)));
+    HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wg.p, wg.ld, 0}, c.F, c.D)));
+    HASTE_TRY((gemm::map_b<K, TN>(&p.b[1], {wu.p, wu.ld, 0}, c.F, c.D)));
+    if (c.gate != nullptr) {
+      HASTE_TRY(gemm::map_result<K>(&p.out[0], {c.gate, c.ldh, 0}, c.T, c.F));
+      HASTE_TRY(gemm::map_result<K>(&p.out[1], {c.up, c.ldh, 0}, c.T, c.F));
+    }
+    HASTE_TRY(gemm::map_result<K>(&p.out[2], {h, ldF, 0}, c.T, c.F));
+    return gemm::launch<K, TN>(w, align.c.n > 0, st);
+  }));
+  HASTE_TRY(by_form<Plain<false, false>>(fy.narrow, [&](auto policy, auto columns) -> int {
+    using K = decltype(policy);
+    constexpr int TN = decltype(columns)::value;
+    Problem& p = w.p[0];
+    set_sizes(p, c.T, c.O, sF, sF);
+    HASTE_TRY(set_output<K>(p, y));
+    HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], {h, ldF, 0}, c.T, c.F)));
+    HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wd.p, wd.ld, 0}, c.O, c.F)));
+    return gemm::launch<K, TN>(w, true, st);
+  }));
   Sums s = {};
   add_sum(s, y, c.T, c.O);
   return run_sums(s, st);
@@ -488,68 +503,81 @@ int forward(Arena& arena, const GatedCall& c, cudaStream_t st) {
 
 int backward(Arena& arena, const GatedGradCall& c, cudaStream_t st) {
   const bool plan = arena.base == nullptr, any = plan && !c.aligned;
-  const int64_t ldF = up8(c.F);
+  const int64_t ldF = up8(c.F), sT = steps_of(c.T), sF = steps_of(c.F), sO = steps_of(c.O);
   Aligner align(arena);
   const Rows dy = align(c.dy, c.lddy, c.T, c.O, any), x = align(c.x, c.ldx, c.T, c.D, any), wg = align(c.wg, c.D, c.F, c.D, any), wu = align(c.wu, c.D, c.F, c.D, any),
-             wd = align(c.wd, c.F, c.O, c.F, any);
-  Rows gate = align(c.gate, c.ldgate, c.T, c.F, any), up = align(c.up, c.ldup, c.T, c.F, any);
-  if (!plan && gate.ld != up.ld) {                     // the epilogue reads both with one stride
-    if (gate.p == c.gate) gate = align(c.gate, c.ldgate, c.T, c.F, true);
-    if (up.p == c.up) up = align(c.up, c.ldup, c.T, c.F, true);
-  }
+             wd = align(c.wd, c.F, c.O, c.F, any), gate = align(c.gate, c.ldgate, c.T, c.F, any), up = align(c.up, c.ldup, c.T, c.F, any);
   void *dgate = arena.take(c.T * ldF * 2), *dup = arena.take(c.T * ldF * 2), *h = arena.take(c.T * ldF * 2);
-  const int64_t sT = k_steps(c.T), sF = k_steps(c.F), tw = tiles_for(c.F, c.D), td = tiles_for(c.O, c.F);
-  const int64_t all = (c.dwg ? tw : 0) + (c.dwu ? tw : 0) + (c.dwd ? td : 0);
-  const Output dx = output_of(arena, c.dx, c.T, c.D, tiles_for(c.T, c.D), 2 * sF, any);
-  const Output dwg = output_of(arena, c.dwg, c.F, c.D, all, sT, any), dwu = output_of(arena, c.dwu, c.F, c.D, all, sT, any), dwd = output_of(arena, c.dwd, c.O, c.F, all, sT, any);
+  const Form fx = form_for(c.T, c.D, 2 * sF);
+  int64_t tiles[2], elements = 0;
+  for (int n = 0; n < 2; ++n) {
+    const int64_t t = gemm::tiles_for(c.F, c.D, n ? 64 : 256);
+    tiles[n] = (c.dwg ? t : 0) + (c.dwu ? t : 0) + (c.dwd ? gemm::tiles_for(c.O, c.F, n ? 64 : 256) : 0);
+  }
+  elements = (c.dwg ? c.F * c.D : 0) + (c.dwu ? c.F * c.D : 0) + (c.dwd ? c.O * c.F : 0);
+  const Form fw = choose_form(tiles[0], tiles[1], sT, elements);
+  const Output dx = output_of(arena, c.dx, c.T, c.D, fx, any), dwg = output_of(arena, c.dwg, c.F, c.D, fw, any), dwu = output_of(arena, c.dwu, c.F, c.D, fw, any),
+               dwd = output_of(arena, c.dwd, c.O, c.F, fw, any);
   if (plan) return HASTE_OK;
   HASTE_TRY(align.run(st));
   {
     Work<1> w = {};
     w.problems = 1;
-    Problem& p = w.p[0];
-    HASTE_TRY(set_product(p, {dgate, reinterpret_cast<float*>(dgate), 1}, c.T, c.F, k_steps(c.O), k_steps(c.O)));
-    p.partial = nullptr;
-    p.in[0] = static_cast<const uint16_t*>(gate.p); p.in[1] = static_cast<const uint16_t*>(up.p);
-    p.ld_in = gate.ld;
-    HASTE_TRY(gemm::make_map(&p.a[0], dy.p, false, c.O, c.T, 1, dy.ld, 0, gemm::BOX_K));
-    HASTE_TRY(gemm::make_map(&p.b[0], wd.p, false, c.F, c.O, 1, wd.ld, 0, gemm::BOX_MN));
-    void* outs[3] = {dgate, dup, h};
-    for (int i = 0; i < 3; ++i) HASTE_TRY(gemm::make_map(&p.out[i], outs[i], false, c.F, c.T, 1, ldF, 0, gemm::BOX_STORE));
-    HASTE_TRY(launch_by_activation<GatedBackward>(c.act, w, align.c.n > 0, st));
+    const bool narrow = gemm::cost_of(gemm::tiles_for(c.T, c.F, 64), sO, true) < gemm::cost_of(gemm::tiles_for(c.T, c.F, 256), sO, false);
+    HASTE_TRY(by_activation<GatedBackward>(c.act, narrow, [&](auto policy, auto columns) -> int {
+      using K = decltype(policy);
+      constexpr int TN = decltype(columns)::value;
+      Problem& p = w.p[0];
+      set_sizes(p, c.T, c.F, sO, sO);
+      HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], {dy.p, dy.ld, 0}, c.T, c.O)));
+      HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wd.p, wd.ld, 0}, c.F, c.O)));
+      HASTE_TRY(gemm::map_result<K>(&p.in[0], {gate.p, gate.ld, 0}, c.T, c.F));
+      HASTE_TRY(gemm::map_result<K>(&p.in[1], {up.p, up.ld, 0}, c.T, c.F));
+      void* outs[3] = {dgate, dup, h};
+      for (int i = 0; i < 3; ++i) HASTE_TRY(gemm::map_result<K>(&p.out[i], {outs[i], ldF, 0}, c.T, c.F));
+      return gemm::launch<K, TN>(w, align.c.n > 0, st);
+    }));
   }
-  Sums s = {};
   if (c.dx != nullptr) {
     Work<1> w = {};
     w.problems = 1;
-    Problem& p = w.p[0];
-    HASTE_TRY(set_product(p, dx, c.T, c.D, sF, 2 * sF));
-    HASTE_TRY(gemm::make_map(&p.a[0], dgate, false, c.F, c.T, 1, ldF, 0, gemm::BOX_K));
-    HASTE_TRY(gemm::make_map(&p.a[1], dup, false, c.F, c.T, 1, ldF, 0, gemm::BOX_K));
-    HASTE_TRY(gemm::make_map(&p.b[0], wg.p, false, c.D, c.F, 1, wg.ld, 0, gemm::BOX_MN));
-    HASTE_TRY(gemm::make_map(&p.b[1], wu.p, false, c.D, c.F, 1, wu.ld, 0, gemm::BOX_MN));
-    HASTE_TRY((gemm::launch<Plain<false, true>>(w, true, st)));
-    if (dx.part != nullptr) {
-      Sums one = {};
-      add_sum(one, dx, c.T, c.D);
-      HASTE_TRY(run_sums(one, st));
-    }
+    HASTE_TRY(by_form<Plain<false, true>>(fx.narrow, [&](auto policy, auto columns) -> int {
+      using K = decltype(policy);
+      constexpr int TN = decltype(columns)::value;
+      Problem& p = w.p[0];
+      set_sizes(p, c.T, c.D, sF, 2 * sF);
+      HASTE_TRY(set_output<K>(p, dx));
+      HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], {dgate, ldF, 0}, c.T, c.F)));
+      HASTE_TRY((gemm::map_a<K, TN>(&p.a[1], {dup, ldF, 0}, c.T, c.F)));
+      HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wg.p, wg.ld, 0}, c.D, c.F)));
+      HASTE_TRY((gemm::map_b<K, TN>(&p.b[1], {wu.p, wu.ld, 0}, c.D, c.F)));
+      return gemm::launch<K, TN>(w, true, st);
+    }));
+    Sums s = {};
+    add_sum(s, dx, c.T, c.D);
+    HASTE_TRY(run_sums(s, st));
   }
+  if (tiles[0] == 0) return HASTE_OK;
   Work<3> w = {};
-  auto weight = [&](const Output& o, const void* a, int64_t lda, const Rows& b, int64_t M, int64_t N) -> int {
-    if (o.p == nullptr) return HASTE_OK;
-    Problem& p = w.p[w.problems++];
-    HASTE_TRY(set_product(p, o, M, N, sT, sT));
-    HASTE_TRY(gemm::make_map(&p.a[0], a, false, M, c.T, 1, lda, 0, gemm::BOX_MN));
-    HASTE_TRY(gemm::make_map(&p.b[0], b.p, false, N, c.T, 1, b.ld, 0, gemm::BOX_MN));
-    add_sum(s, o, M, N);
-    return HASTE_OK;
-  };
-  HASTE_TRY(weight(dwg, dgate, ldF, x, c.F, c.D));
-  HASTE_TRY(weight(dwu, dup, ldF, x, c.F, c.D));
-  HASTE_TRY(weight(dwd, dy.p, dy.ld, {h, ldF}, c.O, c.F));
-  if (w.problems == 0) return HASTE_OK;
-  HASTE_TRY((gemm::launch<Plain<true, true>>(w, true, st)));
+  Sums s = {};
+  HASTE_TRY(by_form<Plain<true, true>>(fw.narrow, [&](auto policy, auto columns) -> int {
+    using K = decltype(policy);
+    constexpr int TN = decltype(columns)::value;
+    auto weight = [&](const Output& o, const Operand& a, const Operand& b, int64_t M, int64_t N) -> int {
+      if (o.p == nullptr) return HASTE_OK;
+      Problem& p = w.p[w.problems++];
+      set_sizes(p, M, N, sT, sT);
+      HASTE_TRY(set_output<K>(p, o));
+      HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], a, M, c.T)));
+      HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], b, N, c.T)));
+      add_sum(s, o, M, N);
+      return HASTE_OK;
+    };
+    HASTE_TRY(weight(dwg, {dgate, ldF, 0}, {x.p, x.ld, 0}, c.F, c.D));
+    HASTE_TRY(weight(dwu, {dup, ldF, 0}, {x.p, x.ld, 0}, c.F, c.D));
+    HASTE_TRY(weight(dwd, {dy.p, dy.ld, 0}, {h, ldF, 0}, c.O, c.F));
+    return gemm::launch<K, TN>(w, true, st);
+  }));
   return run_sums(s, st);
 }
 

@@ -2,15 +2,22 @@
 //
 //   acc[m, n] = sum_k a[m, k] b[n, k]        (a second pair of operands may go on where the first ends)
 //
-// A cluster of two CTAs has a tile of 256 x 256: each loads its half of both operands by TMA (128 rows of a, 128 of b, 64 along k), the even one
-// issues tcgen05.mma.cta_group::2, whose operands are both CTAs' shared memory and whose accumulator is 128 x 256 fp32 in each CTA's TMEM (two of
+// A cluster of two CTAs has a tile of 256 x TN: each loads its half of both operands by TMA (128 rows of a, TN / 2 of b, 64 along k), the even one
+// issues tcgen05.mma.cta_group::2, whose operands are both CTAs' shared memory and whose accumulator is 128 x TN fp32 in each CTA's TMEM (two of
 // them, so that one is read while the next is summed).  Either operand lies with k or with its rows (m, n) contiguous.  What happens to an accumulator is
-// the policy's: its warps read TMEM, 32 rows x 32 columns at a time, and hand 16-bit tiles of that size to tensor-map stores.
+// the policy's: its warps read TMEM, 32 rows x 32 columns at a time, beside boxes of that size of up to two 16-bit matrices, which each warp has brought by TMA
+// two ahead, and hand such boxes to tensor-map stores.  (With loads of its rows by every lane, when the accumulator was there, the last product of a Newton-Schulz
+// step over 50 M elements took 154 us.)
+//
+// TN = 256 is what keeps the tensor cores fed from L2; where there are fewer such tiles than pairs of SMs a narrow form (TN = 64, or 128 for a paired b) has more
+// and shorter ones.
 //
 // Roles (12 warps): warp 0 TMA, warp 1 MMA (in the even CTA), warp 2 TMEM, warps 4-11 epilogue (lane quarter x column half).  Every wait is bounded;
 // after one has run out all roles go on without touching global memory, the kernel returns and the status word says so.
 #pragma once
 #include <cuda_fp16.h>
+
+#include <atomic>
 
 #include "common.cuh"
 #include "launchers.h"
@@ -22,19 +29,37 @@ namespace gemm {
 
 using namespace sm100;
 
-constexpr int TILE = 256;              // of the pair, both ways
+constexpr int TILE = 256;              // rows of a pair's tile
 constexpr int KSTEP = 64;              // one 128-byte swizzle row of 16-bit values
-constexpr int HALF_BYTES = 128 * KSTEP * 2;
-constexpr int STAGE_BYTES = 2 * HALF_BYTES;
-constexpr int STAGES = 5;
 constexpr int EPI_WARPS = 8;
-constexpr int BOX_BYTES = 32 * 32 * 2; // what a warp stages for one store
-constexpr int BOXES = 4;               // per warp, in turn
+constexpr int BOX_BYTES = 32 * 32 * 2; // what a warp loads or stores at once
+constexpr int AHEAD = 2;               // boxes of each input that a warp has on their way
 constexpr int THREADS = 12 * 32;
-constexpr int OFF_EPI = STAGES * STAGE_BYTES;
-constexpr int OFF_BAR = OFF_EPI + EPI_WARPS * BOXES * BOX_BYTES;
-constexpr int SMEM_BYTES = OFF_BAR + 256 + 1024;      // the last for aligning the first stage
 constexpr int GROUP_M = 8;             // tiles of m that are walked before the next of n: what runs at once shares its operands in L2
+
+// The narrow form of a policy
+template <class Policy>
+constexpr int narrow() { return Policy::PAIRED_B ? 128 : 64; }
+
+template <class Policy, int TN>
+struct Layout {
+  static constexpr int A_BYTES = 128 * KSTEP * 2;
+  static constexpr int B_BYTES = TN / 2 * KSTEP * 2;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int IN_BOXES = AHEAD * Policy::INPUTS;                                  // per warp
+  static constexpr int OUT_BOXES = Policy::INPUTS > 0 ? 2 : 4;
+  static constexpr int STAGES = TN == 256 ? (Policy::INPUTS == 2 ? 4 : 5) : 5;
+  static constexpr int OFF_EPI = STAGES * STAGE_BYTES;
+  static constexpr int OFF_BAR = OFF_EPI + EPI_WARPS * (IN_BOXES + OUT_BOXES) * BOX_BYTES;
+  static constexpr int BARRIERS = 2 * STAGES + 4 + EPI_WARPS * AHEAD;
+  static constexpr int SMEM_BYTES = OFF_BAR + 8 * BARRIERS + 16 + 1024;      // the last for aligning the first stage
+  static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
+  static constexpr int TMEM_COLUMNS = 2 * TN;
+  static constexpr int COLUMNS = Policy::PAIRED_B ? TN / 2 : TN;             // of the result, per tile
+  static constexpr int CHUNKS = COLUMNS / 64;                                // boxes of columns of a warp
+  // an operand b of 32 rows with these contiguous has a swizzle of 64 bytes
+  static constexpr bool B_SMALL = Policy::B_MN && TN == 64;
+};
 
 // ---------------------------------------------------------------- pairs of CTAs
 __device__ __forceinline__ uint32_t cta_rank() {
@@ -57,6 +82,11 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const void* tmap, in
       "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
       "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, int x, int y, int z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(z),
+               "r"(bar)
+               : "memory");
 }
 __device__ __forceinline__ void tma_store_3d(const void* tmap, uint32_t src, int x, int y, int z) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(tmap), "r"(x), "r"(y), "r"(z), "r"(src)
@@ -89,15 +119,14 @@ __device__ __forceinline__ void cluster_sync_all() {
 // One product, or a batch of products of one shape.
 struct Problem {
   CUtensorMap a[2], b[2];          // first and second part of k; a policy with two operands b (one for each CTA) has them in b
-  CUtensorMap out[3];
-  const uint16_t* in[2];           // 16-bit matrices that the policy reads at the tile's place
+  CUtensorMap out[3], in[2];       // in: 16-bit matrices that the policy reads at the tile's place
   float* partial;                  // fp32 sums of the parts that k was cut into
-  int64_t ld_in, batch_in;         // strides of `in` in elements
-  int M, N;
-  int tiles_m, tiles_n;            // tiles_n < 0: symmetric, only tiles with n <= m
+  int M, N;                        // of the result
+  int tiles_m, tiles_n;            // set by launch()
+  int symmetric;                   // only tiles on and below the diagonal
   int batch, splits;
   int steps0, steps;               // steps of k in the first part, and in both
-  int first;                       // number of this problem's first tile
+  int first, each;                 // number of this problem's first tile, and how many a matrix has; set by launch()
 };
 template <int P>
 struct Work {
@@ -111,27 +140,36 @@ struct Tile {
   int problem, batch, split, m, n;
 };
 
-__host__ __device__ inline int tiles_of(const Problem& p) { return p.tiles_n < 0 ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n; }
+// Columns' tiles that a row of tiles of a symmetric result has: those that begin before the row's end
+__host__ __device__ inline int symmetric_tiles(int m, int tiles_n, int per) { return (m + 1) * per < tiles_n ? (m + 1) * per : tiles_n; }
+
+// per: column tiles to a tile's 256 rows
+__host__ __device__ inline int tiles_of(const Problem& p, int per) {
+  if (!p.symmetric) return p.tiles_m * p.tiles_n;
+  int n = 0;
+  for (int m = 0; m < p.tiles_m; ++m) n += symmetric_tiles(m, p.tiles_n, per);
+  return n;
+}
 
 template <int P>
-__device__ __forceinline__ Tile tile_at(const Work<P>& w, int t) {
+__device__ __forceinline__ Tile tile_at(const Work<P>& w, int t, int per) {
   Tile r;
   r.problem = 0;
   if (P > 1)
     while (r.problem + 1 < w.problems && t >= w.p[r.problem + 1].first) ++r.problem;
   const Problem& p = w.p[r.problem];
   t -= p.first;
-  const int each = tiles_of(p);
-  const int bs = t / each;
-  t -= bs * each;
+  const int bs = t / p.each;
+  t -= bs * p.each;
   r.batch = bs / p.splits;
   r.split = bs - r.batch * p.splits;
-  if (p.tiles_n < 0) {
-    int m = static_cast<int>((sqrtf(8.f * static_cast<float>(t) + 1.f) - 1.f) * 0.5f);
-    while (m * (m + 1) / 2 > t) --m;
-    while ((m + 1) * (m + 2) / 2 <= t) ++m;
+  if (p.symmetric) {
+    // rows of tiles grow by `per` until they are as wide as the matrix
+    int m = static_cast<int>((sqrtf(8.f * static_cast<float>(t / per) + 1.f) - 1.f) * 0.5f);
+    while (m * (m + 1) / 2 * per > t) --m;
+    while ((m + 1) * (m + 2) / 2 * per <= t) ++m;
     r.m = m;
-    r.n = t - m * (m + 1) / 2;
+    r.n = t - m * (m + 1) / 2 * per;
   } else {
     const int band = t / (GROUP_M * p.tiles_n), in_band = t - band * GROUP_M * p.tiles_n;
     const int high = min(GROUP_M, p.tiles_m - band * GROUP_M);
@@ -143,6 +181,7 @@ __device__ __forceinline__ Tile tile_at(const Work<P>& w, int t) {
 
 // ---------------------------------------------------------------- epilogue helpers
 // A warp's boxes of 32 rows x 32 16-bit columns on their way to memory (64-byte swizzle: 16-byte chunk j of row r at j ^ (r / 2 % 4)).
+template <int BOXES>
 struct Stager {
   uint32_t base;
   int lane, next;
@@ -190,42 +229,87 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 __device__ __forceinline__ float2 unpack_bf16(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
 __device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-// 32 16-bit values of one row, packed in pairs; zeros beyond the row's `cols`, a multiple of 8 (rows are padded), and where !there
-__device__ __forceinline__ void load_row(uint32_t (&v)[16], const uint16_t* row, int col, int64_t cols, bool there) {
+// Row `lane` of a box, packed in pairs
+__device__ __forceinline__ void row_of_box(uint32_t box, int lane, uint32_t (&p)[16]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint4 q = make_uint4(0, 0, 0, 0);
-    if (there && col + 8 * j < cols) q = *reinterpret_cast<const uint4*>(row + col + 8 * j);
-    v[4 * j] = q.x; v[4 * j + 1] = q.y; v[4 * j + 2] = q.z; v[4 * j + 3] = q.w;
-  }
+  for (int j = 0; j < 4; ++j)
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(p[4 * j]), "=r"(p[4 * j + 1]), "=r"(p[4 * j + 2]), "=r"(p[4 * j + 3]) : "r"(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) : "memory");
 }
 
+// A warp's boxes of the policy's inputs, AHEAD of what it works on: over all chunks of columns of all its tiles, one after the other.  Beyond the matrix they
+// hold zeros.
+template <class Policy, int P, int TN>
+struct Inputs {
+  using L = Layout<Policy, TN>;
+  const Work<P>& w;
+  uint32_t base, bars;             // boxes and barriers of this warp
+  int lane, quarter, half, rank, stride;
+  int issue_t, issue_j, issued, taken;
+  Tile tile;
+
+  __device__ __forceinline__ void issue() {
+    if (issue_t >= w.tiles) return;
+    if (issue_j == 0) tile = tile_at(w, issue_t, TILE / TN);
+    if (lane == 0) {
+      const Problem& p = w.p[tile.problem];
+      const int slot = issued % AHEAD, x = tile.n * L::COLUMNS + half * (L::COLUMNS / 2) + issue_j * 32, y = tile.m * TILE + rank * 128 + quarter * 32;
+      mbar_arrive_expect_tx(bars + 8 * slot, Policy::INPUTS * BOX_BYTES);
+#pragma unroll
+      for (int i = 0; i < Policy::INPUTS; ++i) tma_load_3d(base + (slot * Policy::INPUTS + i) * BOX_BYTES, &p.in[i], x, y, tile.batch, bars + 8 * slot);
+    }
+    ++issued;
+    if (++issue_j == L::CHUNKS) { issue_j = 0; issue_t += stride; }
+  }
+  __device__ __forceinline__ void start() {
+    if (Policy::INPUTS > 0)
+#pragma unroll 1
+      for (int i = 0; i < AHEAD; ++i) issue();
+  }
+  // The next chunk's boxes are there
+  __device__ __forceinline__ bool wait(volatile int* abort_flag) {
+    if (Policy::INPUTS == 0) return true;
+    return __all_sync(0xffffffffu, mbar_wait(bars + 8 * (taken % AHEAD), (taken / AHEAD) & 1, abort_flag, w.err, 306, w.wait_limit));
+  }
+  __device__ __forceinline__ void get(int i, uint32_t (&p)[16]) const { row_of_box(base + (taken % AHEAD * Policy::INPUTS + i) * BOX_BYTES, lane, p); }
+  // All of them have been read
+  __device__ __forceinline__ void release() {
+    if (Policy::INPUTS == 0) return;
+    ++taken;
+    __syncwarp();
+    issue();
+  }
+};
+
 // ---------------------------------------------------------------- the kernel
-// Policy: A_MN, B_MN (the operand's rows are contiguous, not k), F16 (else bf16), PAIRED_B (each CTA has an operand b of its own: 128 columns of
-// two products side by side), and
-//   static void epilogue(w, p, tile, row0, col0, column half, tmem, stager, lane)   one warp's part of a tile
-template <class Policy, int P>
+// Policy: A_MN, B_MN (the operand's rows are contiguous, not k), F16 (else bf16), PAIRED_B (each CTA has an operand b of its own: TN / 2 columns of
+// two products side by side), INPUTS, and
+//   static void chunk(w, p, tile, row0, col, diagonal, tmem, inputs, stager, lane)   32 rows x 32 columns of the result at (row0, col), accumulator at tmem
+template <class Policy, int P, int TN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm100_kernel(const __grid_constant__ Work<P> w) {
+  using L = Layout<Policy, TN>;
+  constexpr int STAGES = L::STAGES, PER = TILE / TN;
   extern __shared__ uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   const uint32_t base = smem_u32(sm);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cta_rank();
-  auto bar_full = [&](int s) { return base + OFF_BAR + 8 * s; };
-  auto bar_empty = [&](int s) { return base + OFF_BAR + 8 * (STAGES + s); };
-  auto bar_done = [&](int s) { return base + OFF_BAR + 8 * (2 * STAGES + s); };
-  auto bar_free = [&](int s) { return base + OFF_BAR + 8 * (2 * STAGES + 2 + s); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + OFF_BAR + 8 * (2 * STAGES + 4));
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + OFF_BAR + 8 * (2 * STAGES + 4) + 8);
+  auto bar_full = [&](int s) { return base + L::OFF_BAR + 8 * s; };
+  auto bar_empty = [&](int s) { return base + L::OFF_BAR + 8 * (STAGES + s); };
+  auto bar_done = [&](int s) { return base + L::OFF_BAR + 8 * (2 * STAGES + s); };
+  auto bar_free = [&](int s) { return base + L::OFF_BAR + 8 * (2 * STAGES + 2 + s); };
+  const uint32_t bar_in = base + L::OFF_BAR + 8 * (2 * STAGES + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + L::OFF_BAR + 8 * L::BARRIERS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::OFF_BAR + 8 * L::BARRIERS + 8);
   const long long WL = w.wait_limit;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(bar_done(s), 1); mbar_init(bar_free(s), 2 * EPI_WARPS); }
+    for (int s = 0; s < EPI_WARPS * AHEAD; ++s) mbar_init(bar_in + 8 * s, 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == 2) tmem_alloc_pair(smem_u32(tmem_slot), 512);
+  if (warp == 2) tmem_alloc_pair(smem_u32(tmem_slot), L::TMEM_COLUMNS);
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();                // the other CTA's barriers are there, and it has started
@@ -238,30 +322,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
     // ---------------- loads
     int it = 0;
     for (int t = first; t < w.tiles && !*abort_flag; t += stride) {
-      const Tile tl = tile_at(w, t);
+      const Tile tl = tile_at(w, t, PER);
       const Problem& p = w.p[tl.problem];
       const int k0 = static_cast<int>(static_cast<int64_t>(p.steps) * tl.split / p.splits), k1 = static_cast<int>(static_cast<int64_t>(p.steps) * (tl.split + 1) / p.splits);
       const int am = tl.m * TILE + static_cast<int>(rank) * 128;
-      const int bn = Policy::PAIRED_B ? tl.n * 128 : tl.n * TILE + static_cast<int>(rank) * 128;
+      const int bn = Policy::PAIRED_B ? tl.n * (TN / 2) : tl.n * TN + static_cast<int>(rank) * (TN / 2);
       for (int k = k0; k < k1; ++k, ++it) {
         const int s = it % STAGES;
         if (!mbar_wait(bar_empty(s), ((it / STAGES) & 1) ^ 1, abort_flag, w.err, 301, WL)) break;
-        if (rank == 0) mbar_arrive_expect_tx(bar_full(s), 2 * STAGE_BYTES);
+        if (rank == 0) mbar_arrive_expect_tx(bar_full(s), 2 * L::STAGE_BYTES);
         const uint32_t bar = leaders(bar_full(s));
         const int part = k >= p.steps0;
         const int kc = (part ? k - p.steps0 : k) * KSTEP;
-        const uint32_t as = base + s * STAGE_BYTES, bs = as + HALF_BYTES;
+        const uint32_t as = base + s * L::STAGE_BYTES, bs = as + L::A_BYTES;
         const CUtensorMap* ta = &p.a[part];
         const CUtensorMap* tb = &p.b[Policy::PAIRED_B ? static_cast<int>(rank) : part];
         if (Policy::A_MN) {
           tma_load_pair(as, ta, am, kc, tl.batch, bar);
-          tma_load_pair(as + HALF_BYTES / 2, ta, am + 64, kc, tl.batch, bar);
+          tma_load_pair(as + L::A_BYTES / 2, ta, am + 64, kc, tl.batch, bar);
         } else {
           tma_load_pair(as, ta, kc, am, tl.batch, bar);
         }
         if (Policy::B_MN) {
           tma_load_pair(bs, tb, bn, kc, tl.batch, bar);
-          tma_load_pair(bs + HALF_BYTES / 2, tb, bn + 64, kc, tl.batch, bar);
+          if (TN == 256) tma_load_pair(bs + L::B_BYTES / 2, tb, bn + 64, kc, tl.batch, bar);
         } else {
           tma_load_pair(bs, tb, kc, bn, tl.batch, bar);
         }
@@ -273,12 +357,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
     // ---------------- products
     constexpr uint32_t FORMAT = Policy::F16 ? 0u : (1u << 7) | (1u << 10);
     constexpr uint32_t IDESC = (1u << 4) | FORMAT | (static_cast<uint32_t>(Policy::A_MN) << 15) | (static_cast<uint32_t>(Policy::B_MN) << 16) |
-                               (static_cast<uint32_t>(TILE >> 3) << 17) | (static_cast<uint32_t>(TILE >> 4) << 24);
-    const uint64_t da = make_sdesc(base, Policy::A_MN ? HALF_BYTES / 2 : 16, 1024), db = make_sdesc(base + HALF_BYTES, Policy::B_MN ? HALF_BYTES / 2 : 16, 1024);
-    constexpr uint64_t KA = Policy::A_MN ? 2048 >> 4 : 32 >> 4, KB = Policy::B_MN ? 2048 >> 4 : 32 >> 4;
+                               (static_cast<uint32_t>(TN >> 3) << 17) | (static_cast<uint32_t>(TILE >> 4) << 24);
+    const uint64_t da = make_sdesc(base, Policy::A_MN ? L::A_BYTES / 2 : 16, 1024);
+    const uint64_t db = L::B_SMALL ? make_sdesc64(base + L::A_BYTES, 16, 512) : make_sdesc(base + L::A_BYTES, Policy::B_MN ? L::B_BYTES / 2 : 16, 1024);
+    constexpr uint64_t KA = Policy::A_MN ? 2048 >> 4 : 32 >> 4, KB = L::B_SMALL ? 1024 >> 4 : Policy::B_MN ? 2048 >> 4 : 32 >> 4;
     int it = 0, n = 0;
     for (int t = first; t < w.tiles; t += stride, ++n) {
-      const Tile tl = tile_at(w, t);
+      const Tile tl = tile_at(w, t, PER);
       const Problem& p = w.p[tl.problem];
       const int steps = static_cast<int>(static_cast<int64_t>(p.steps) * (tl.split + 1) / p.splits) - static_cast<int>(static_cast<int64_t>(p.steps) * tl.split / p.splits);
       const int buf = n & 1;
@@ -291,9 +376,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t off = static_cast<uint64_t>((s * STAGE_BYTES) >> 4);
+          const uint64_t off = static_cast<uint64_t>((s * L::STAGE_BYTES) >> 4);
 #pragma unroll
-          for (int j = 0; j < KSTEP / 16; ++j) umma_pair(tmem + buf * TILE, da + off + j * KA, db + off + j * KB, IDESC, (k | j) != 0);
+          for (int j = 0; j < KSTEP / 16; ++j) umma_pair(tmem + buf * TN, da + off + j * KA, db + off + j * KB, IDESC, (k | j) != 0);
           commit_pair(bar_empty(s));
         }
         __syncwarp();
@@ -305,16 +390,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
   } else if (warp >= 4) {
     // ---------------- epilogue
     const int quarter = warp & 3, half = (warp - 4) >> 2;
-    Stager st = {base + OFF_EPI + static_cast<uint32_t>(warp - 4) * BOXES * BOX_BYTES, lane, 0};
+    const uint32_t mine = base + L::OFF_EPI + static_cast<uint32_t>(warp - 4) * (L::IN_BOXES + L::OUT_BOXES) * BOX_BYTES;
+    Inputs<Policy, P, TN> in = {w, mine + L::OUT_BOXES * BOX_BYTES, bar_in + 8 * AHEAD * (warp - 4), lane, quarter, half, static_cast<int>(rank), stride, first, 0, 0, 0, {}};
+    Stager<L::OUT_BOXES> st = {mine, lane, 0};
+    in.start();
     int n = 0;
     for (int t = first; t < w.tiles; t += stride, ++n) {
-      const Tile tl = tile_at(w, t);
-      const int buf = n & 1;
-      const bool ok = mbar_wait(bar_done(buf), (n >> 1) & 1, abort_flag, w.err, 305, WL);
-      if (!__all_sync(0xffffffffu, ok)) break;
+      const Tile tl = tile_at(w, t, PER);
+      const Problem& p = w.p[tl.problem];
+      const int buf = n & 1, row0 = tl.m * TILE + static_cast<int>(rank) * 128 + quarter * 32, at = half * (L::COLUMNS / 2);
+      bool ok = mbar_wait(bar_done(buf), (n >> 1) & 1, abort_flag, w.err, 305, WL);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       tc_fence_after();
-      Policy::epilogue(w, w.p[tl.problem], tl, tl.m * TILE + static_cast<int>(rank) * 128 + quarter * 32, half,
-                       tmem + buf * TILE + (static_cast<uint32_t>(quarter * 32) << 16), st, lane);
+#pragma unroll 1
+      for (int j = 0; j < L::CHUNKS && ok; ++j) {
+        ok = in.wait(abort_flag);
+        if (ok) Policy::chunk(w, p, tl, row0, tl.n * L::COLUMNS + at + 32 * j, tl.n / PER == tl.m, tmem + buf * TN + (static_cast<uint32_t>(quarter * 32) << 16) + at + 32 * j, in, st, lane);
+      }
+      if (!ok) break;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_at_leader(bar_free(buf));
@@ -333,34 +427,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
   }
   cluster_sync_all();
   tc_fence_after();
-  if (warp == 2) tmem_dealloc_pair(tmem, 512);
+  if (warp == 2) tmem_dealloc_pair(tmem, L::TMEM_COLUMNS);
 }
 
 // ---------------------------------------------------------------- host side
-// A batch of 16-bit matrices [outer][inner] as a tensor map.  An operand with k contiguous: inner = k, box 64 x 128; with its rows contiguous: inner =
-// rows, box 64 x 64; stores: box 32 x 32.  Base and strides are multiples of 16 bytes.
-enum Box { BOX_K, BOX_MN, BOX_STORE };
-inline int make_map(CUtensorMap* out, const void* base, bool f16, int64_t inner, int64_t outer, int64_t batch, int64_t ld, int64_t batch_stride, Box box) {
-  return make_tmap_16bit_3d(out, base, f16, inner, outer, batch, ld * 2, (batch_stride ? batch_stride : ld * outer) * 2, box == BOX_STORE ? 32 : 64,
-                            box == BOX_STORE ? 32 : box == BOX_K ? 128 : 64);
+// A batch of 16-bit matrices [outer][inner] as a tensor map; base and strides are multiples of 16 bytes.
+inline int make_map(CUtensorMap* out, const void* base, bool f16, int64_t inner, int64_t outer, int64_t batch, int64_t ld, int64_t batch_stride, int box_inner, int box_outer) {
+  return make_tmap_16bit_3d(out, base, f16, inner, outer, batch, ld * 2, (batch_stride ? batch_stride : ld * outer) * 2, static_cast<uint32_t>(box_inner), static_cast<uint32_t>(box_outer));
 }
+// Where a 16-bit matrix (or a batch of them) lies
+struct Operand {
+  const void* p;
+  int64_t ld, batch_stride;        // 0: a matrix's size
+};
+// Operand a of `rows` (the result's M) and b of `rows` (its N), k values each; inputs and outputs of the result's size
+template <class Policy, int TN>
+int map_a(CUtensorMap* out, const Operand& o, int64_t rows, int64_t k, int64_t batch = 1) {
+  return Policy::A_MN ? make_map(out, o.p, Policy::F16, rows, k, batch, o.ld, o.batch_stride, 64, 64) : make_map(out, o.p, Policy::F16, k, rows, batch, o.ld, o.batch_stride, 64, 128);
+}
+template <class Policy, int TN>
+int map_b(CUtensorMap* out, const Operand& o, int64_t rows, int64_t k, int64_t batch = 1) {
+  return Policy::B_MN ? make_map(out, o.p, Policy::F16, rows, k, batch, o.ld, o.batch_stride, TN == 64 ? 32 : 64, 64)
+                      : make_map(out, o.p, Policy::F16, k, rows, batch, o.ld, o.batch_stride, 64, TN / 2);
+}
+template <class Policy>
+int map_result(CUtensorMap* out, const Operand& o, int64_t M, int64_t N, int64_t batch = 1) {
+  return make_map(out, o.p, Policy::F16, N, M, batch, o.ld, o.batch_stride, 32, 32);
+}
+inline int64_t steps_of(int64_t k) { return (k + KSTEP - 1) / KSTEP; }
 
-// CTAs that a launch of pairs may have at once on the current device
+// Pairs of CTAs that may run at once on the current device
 template <class K>
-int pairs_resident(K kernel) {
-  static int cached[64] = {};
+int pairs_resident(K kernel, int smem) {
+  static std::atomic<int> cached[64];
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && cached[dev] > 0) return cached[dev];
+  if (dev >= 0 && dev < 64 && cached[dev].load(std::memory_order_relaxed) > 0) return cached[dev].load(std::memory_order_relaxed);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(sm_count() & ~1));
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = 2;
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   int n = 0;
@@ -368,31 +478,45 @@ int pairs_resident(K kernel) {
     cudaGetLastError();
     return sm_count() / 2;
   }
-  if (dev >= 0 && dev < 64) cached[dev] = n;
+  if (n > sm_count() / 2) n = sm_count() / 2;      // one CTA to an SM, also where two would fit
+  if (dev >= 0 && dev < 64) cached[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 
+// Time of a launch of `tiles` tiles of `steps` steps of k each, in units of a step of the wide form (0.28 us)
+inline double cost_of(int64_t tiles, int64_t steps, bool is_narrow) {
+  const int64_t pairs = sm_count() / 2;
+  return static_cast<double>((tiles + pairs - 1) / pairs) * (is_narrow ? 0.6 * static_cast<double>(steps) + 3.5 : static_cast<double>(steps) + 6.0);
+}
+inline int64_t tiles_for(int64_t M, int64_t N, int64_t columns) { return ((M + TILE - 1) / TILE) * ((N + columns - 1) / columns); }
+
 // Launches what is in w.p[0 .. problems): tiles are counted here.  behind: the kernel before it in the stream is one of the same call.
-template <class Policy, int P>
+template <class Policy, int TN, int P>
 int launch(Work<P>& w, bool behind, cudaStream_t st) {
-  auto kernel = gemm_sm100_kernel<Policy, P>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+  using L = Layout<Policy, TN>;
+  auto kernel = gemm_sm100_kernel<Policy, P, TN>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM_BYTES);
   if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   int64_t tiles = 0;
   for (int i = 0; i < w.problems; ++i) {
-    w.p[i].first = static_cast<int>(tiles);
-    tiles += static_cast<int64_t>(tiles_of(w.p[i])) * w.p[i].batch * w.p[i].splits;
+    Problem& p = w.p[i];
+    p.tiles_m = (p.M + TILE - 1) / TILE;
+    p.tiles_n = (p.N + L::COLUMNS - 1) / L::COLUMNS;
+    if (static_cast<int64_t>(p.tiles_m) * p.tiles_n > 0x3FFFFFFF) return fail(HASTE_ERR_TOO_LARGE, "too many tiles for one launch");
+    p.first = static_cast<int>(tiles);
+    p.each = tiles_of(p, TILE / TN);
+    tiles += static_cast<int64_t>(p.each) * p.batch * p.splits;
     if (tiles > 0x3FFFFFFF) return fail(HASTE_ERR_TOO_LARGE, "too many tiles for one launch");
   }
   if (tiles == 0) return HASTE_OK;
   w.tiles = static_cast<int>(tiles);
   if (int rc = device_status_word(&w.err)) return rc;
   w.wait_limit = wait_limit_cycles();
-  const int pairs = static_cast<int>(imin64(pairs_resident(kernel), tiles));
+  const int pairs = static_cast<int>(imin64(pairs_resident(kernel, L::SMEM_BYTES), tiles));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.dynamicSmemBytes = L::SMEM_BYTES;
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -9,7 +9,7 @@
 //
 // Rounding.  The products take fp16: X times 2^8 (its entries are at most 1, later 1.3 or so; the factor keeps small ones out of the subnormals), A and
 // B = b A + c A A.  The term a X, by which small singular values grow 3.4 times a step, takes X as a sum of two fp16 values, hi + lo 2^-11: 22 bits.  Without lo
-// an update of low rank with noise is off by 1.3e-2 after five steps (2-norm of the difference over that of the result), with it by 3e-4, a Gaussian one by 1.7e-3;
+// an update of low rank with noise is off by 1.3e-2 after five steps (2-norm of the difference over that of the result), with it by 1e-3, a Gaussian one by 1.4e-3;
 // with bf16 in place of fp16 1e-1 and 1e-2.  A and A A are symmetric: tiles on and below the diagonal are computed, the others are their mirror.
 #include "gemm_sm100.cuh"
 
@@ -21,7 +21,6 @@ namespace haste {
 namespace {
 
 using gemm::Problem;
-using gemm::Stager;
 using gemm::Tile;
 using gemm::Work;
 
@@ -29,12 +28,13 @@ constexpr float X_SCALE = 256.f;
 constexpr float LO_SCALE = 2048.f;
 
 // ---------------------------------------------------------------- products
-__device__ __forceinline__ void put_symmetric(const Problem& p, const Tile& t, int row0, int col, const uint32_t (&packed)[16], Stager& st, int lane) {
+template <class S>
+__device__ __forceinline__ void put_symmetric(const Problem& p, const Tile& t, int row0, int col, bool diagonal, const uint32_t (&packed)[16], S& st, int lane) {
   const bool inside = row0 < p.M && col < p.N;
   uint32_t box = st.get();
   gemm::box_row(box, lane, packed);
   st.put(&p.out[0], box, col, row0, t.batch, inside);
-  if (t.m != t.n) {
+  if (!diagonal) {
     box = st.get();
     gemm::box_column(box, lane, packed);
     st.put(&p.out[0], box, row0, col, t.batch, inside);
@@ -44,77 +44,75 @@ __device__ __forceinline__ void put_symmetric(const Problem& p, const Tile& t, i
 // A = scale0 X X^T
 struct Gram {
   static constexpr bool A_MN = false, B_MN = false, F16 = true, PAIRED_B = false;
-  template <int P>
-  static __device__ __forceinline__ void epilogue(const Work<P>& w, const Problem& p, const Tile& t, int row0, int half, uint32_t tmem, Stager& st, int lane) {
-#pragma unroll 1
-    for (int j = 0; j < 4; ++j) {
-      const int at = half * 128 + j * 32;
-      uint32_t v[32], packed[16];
-      sm100::tmem_ld32(tmem + at, v);
-      sm100::tmem_ld_wait();
+  static constexpr int INPUTS = 0;
+  template <class W, class I, class S>
+  static __device__ __forceinline__ void chunk(const W& w, const Problem& p, const Tile& t, int row0, int col, bool diagonal, uint32_t tmem, I&, S& st, int lane) {
+    uint32_t v[32], packed[16];
+    sm100::tmem_ld32(tmem, v);
+    sm100::tmem_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) packed[i] = gemm::pack_f16(__uint_as_float(v[2 * i]) * w.scale0, __uint_as_float(v[2 * i + 1]) * w.scale0);
-      put_symmetric(p, t, row0, t.n * gemm::TILE + at, packed, st, lane);
-    }
+    for (int i = 0; i < 16; ++i) packed[i] = gemm::pack_f16(__uint_as_float(v[2 * i]) * w.scale0, __uint_as_float(v[2 * i + 1]) * w.scale0);
+    put_symmetric(p, t, row0, col, diagonal, packed, st, lane);
   }
 };
 
 // B = scale0 A + scale1 A A^T; in[0] = A
 struct Polynomial {
   static constexpr bool A_MN = false, B_MN = false, F16 = true, PAIRED_B = false;
-  template <int P>
-  static __device__ __forceinline__ void epilogue(const Work<P>& w, const Problem& p, const Tile& t, int row0, int half, uint32_t tmem, Stager& st, int lane) {
-    const uint16_t* row = p.in[0] + t.batch * p.batch_in + static_cast<int64_t>(row0 + lane) * p.ld_in;
-#pragma unroll 1
-    for (int j = 0; j < 4; ++j) {
-      const int at = half * 128 + j * 32, col = t.n * gemm::TILE + at;
-      uint32_t v[32], packed[16];
-      gemm::load_row(packed, row, col, p.ld_in, row0 + lane < p.M);
-      sm100::tmem_ld32(tmem + at, v);
-      sm100::tmem_ld_wait();
+  static constexpr int INPUTS = 1;
+  template <class W, class I, class S>
+  static __device__ __forceinline__ void chunk(const W& w, const Problem& p, const Tile& t, int row0, int col, bool diagonal, uint32_t tmem, I& in, S& st, int lane) {
+    uint32_t v[32], packed[16];
+    sm100::tmem_ld32(tmem, v);
+    in.get(0, packed);
+    in.release();
+    sm100::tmem_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float2 a = gemm::unpack_f16(packed[i]);
-        packed[i] = gemm::pack_f16(fmaf(w.scale1, __uint_as_float(v[2 * i]), w.scale0 * a.x), fmaf(w.scale1, __uint_as_float(v[2 * i + 1]), w.scale0 * a.y));
-      }
-      put_symmetric(p, t, row0, col, packed, st, lane);
+    for (int i = 0; i < 16; ++i) {
+      const float2 a = gemm::unpack_f16(packed[i]);
+      packed[i] = gemm::pack_f16(fmaf(w.scale1, __uint_as_float(v[2 * i]), w.scale0 * a.x), fmaf(w.scale1, __uint_as_float(v[2 * i + 1]), w.scale0 * a.y));
     }
+    put_symmetric(p, t, row0, col, diagonal, packed, st, lane);
   }
 };
 
-// X' = scale0 X + B X; in[0] = X's upper, in[1] its lower part; out[0], out[1] those of X' (in[1] and out[1] are one place: a tile reads what it writes).
-// scale1: the last step, nobody wants the lower part any more
+// X' = scale0 X + B X; in[0] = X's upper part, in[1] its lower one, if it has one (LOWER: 2 and 1); out[0] and out[1] those of X', the lower one with LOWER = 2 alone.  (in[1] and
+// out[1] are one place: a tile reads what it writes.)
+template <int LOWER>
 struct Apply {
   static constexpr bool A_MN = false, B_MN = true, F16 = true, PAIRED_B = false;
-  template <int P>
-  static __device__ __forceinline__ void epilogue(const Work<P>& w, const Problem& p, const Tile& t, int row0, int half, uint32_t tmem, Stager& st, int lane) {
-    const int64_t row = t.batch * p.batch_in + static_cast<int64_t>(row0 + lane) * p.ld_in;
-    const bool there = row0 + lane < p.M;
-#pragma unroll 1
-    for (int j = 0; j < 4; ++j) {
-      const int at = half * 128 + j * 32, col = t.n * gemm::TILE + at;
-      const bool inside = row0 < p.M && col < p.N;
-      uint32_t v[32], hi[16], lo[16];
-      gemm::load_row(hi, p.in[0] + row, col, p.ld_in, there);
-      gemm::load_row(lo, p.in[1] + row, col, p.ld_in, there);
-      sm100::tmem_ld32(tmem + at, v);
-      sm100::tmem_ld_wait();
+  static constexpr int INPUTS = LOWER ? 2 : 1;
+  template <class W, class I, class S>
+  static __device__ __forceinline__ void chunk(const W& w, const Problem& p, const Tile& t, int row0, int col, bool, uint32_t tmem, I& in, S& st, int lane) {
+    const bool inside = row0 < p.M && col < p.N;
+    uint32_t v[32], hi[16], lo[16];
+    sm100::tmem_ld32(tmem, v);
+    in.get(0, hi);
+    if (LOWER) in.get(1, lo);
+    in.release();
+    sm100::tmem_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float2 h = gemm::unpack_f16(hi[i]), l = gemm::unpack_f16(lo[i]);
-        const float x = fmaf(w.scale0, fmaf(l.x, 1.f / LO_SCALE, h.x), __uint_as_float(v[2 * i])), y = fmaf(w.scale0, fmaf(l.y, 1.f / LO_SCALE, h.y), __uint_as_float(v[2 * i + 1]));
-        hi[i] = gemm::pack_f16(x, y);
+    for (int i = 0; i < 16; ++i) {
+      float2 h = gemm::unpack_f16(hi[i]);
+      if (LOWER) {
+        const float2 l = gemm::unpack_f16(lo[i]);
+        h.x = fmaf(l.x, 1.f / LO_SCALE, h.x);
+        h.y = fmaf(l.y, 1.f / LO_SCALE, h.y);
+      }
+      const float x = fmaf(w.scale0, h.x, __uint_as_float(v[2 * i])), y = fmaf(w.scale0, h.y, __uint_as_float(v[2 * i + 1]));
+      hi[i] = gemm::pack_f16(x, y);
+      if (LOWER == 2) {
         const float2 r = gemm::unpack_f16(hi[i]);
         lo[i] = gemm::pack_f16((x - r.x) * LO_SCALE, (y - r.y) * LO_SCALE);
       }
-      uint32_t box = st.get();
-      gemm::box_row(box, lane, hi);
-      st.put(&p.out[0], box, col, row0, t.batch, inside);
-      if (w.scale1 == 0.f) {
-        box = st.get();
-        gemm::box_row(box, lane, lo);
-        st.put(&p.out[1], box, col, row0, t.batch, inside);
-      }
+    }
+    uint32_t box = st.get();
+    gemm::box_row(box, lane, hi);
+    st.put(&p.out[0], box, col, row0, t.batch, inside);
+    if (LOWER == 2) {
+      box = st.get();
+      gemm::box_row(box, lane, lo);
+      st.put(&p.out[1], box, col, row0, t.batch, inside);
     }
   }
 };
@@ -428,53 +426,71 @@ struct Shape {
   uint16_t *hi[2], *lo, *A, *B;
 };
 
+// One product of all shapes.  phase 0: A = X X^T, 1: B = b A + c A A, 2: X
+template <class Policy, int TN, int P>
+int run_product(const std::vector<Shape>& shapes, size_t from, size_t to, int phase, int cur, double scale0, double scale1, cudaStream_t st) {
+  static thread_local Work<P> w;
+  w.problems = static_cast<int>(to - from);
+  w.scale0 = static_cast<float>(scale0); w.scale1 = static_cast<float>(scale1);
+  for (size_t i = from; i < to; ++i) {
+    const Shape& h = shapes[i];
+    Problem& p = w.p[i - from];
+    const gemm::Operand x = {h.hi[cur], up8(h.q), h.p * up8(h.q)}, low = {h.lo, x.ld, x.batch_stride}, next = {h.hi[cur ^ 1], x.ld, x.batch_stride}, A = {h.A, up8(h.p), h.p * up8(h.p)},
+                        B = {h.B, A.ld, A.batch_stride};
+    const int64_t k = phase == 0 ? h.q : h.p, N = phase == 2 ? h.q : h.p;
+    p.partial = nullptr;
+    p.M = static_cast<int>(h.p); p.N = static_cast<int>(N);
+    p.symmetric = phase < 2;
+    p.batch = static_cast<int>(h.batch);
+    p.splits = 1;
+    p.steps0 = p.steps = static_cast<int>(gemm::steps_of(k));
+    int rc = gemm::map_a<Policy, TN>(&p.a[0], phase == 0 ? x : phase == 1 ? A : B, h.p, k, h.batch);
+    rc = rc ? rc : gemm::map_b<Policy, TN>(&p.b[0], phase == 1 ? A : x, N, k, h.batch);
+    rc = rc ? rc : gemm::map_result<Policy>(&p.out[0], phase == 0 ? A : phase == 1 ? B : next, h.p, N, h.batch);
+    if (phase == 1) rc = rc ? rc : gemm::map_result<Policy>(&p.in[0], A, h.p, N, h.batch);
+    if (phase == 2) {
+      rc = rc ? rc : gemm::map_result<Policy>(&p.in[0], x, h.p, N, h.batch);
+      rc = rc ? rc : gemm::map_result<Policy>(&p.in[1], low, h.p, N, h.batch);
+      p.out[1] = p.in[1];
+    }
+    if (rc) return rc;
+  }
+  return gemm::launch<Policy, TN>(w, true, st);
+}
+
+// What X is rounded to after the last but two steps is amplified by two steps at most (12 times), which leaves 2^-12 of its values where the products' own roundings
+// are: its lower part is kept up to there.
+constexpr int STEPS_WITHOUT_LOWER = 2;
+
 template <int P>
 int run_steps(const std::vector<Shape>& shapes, size_t from, size_t to, int steps, double a, double b, double c, cudaStream_t st) {
-  const int n = static_cast<int>(to - from);
-  static thread_local Work<P> w;
+  double wide[2] = {}, narrow[2] = {};               // of the symmetric products and of the last one
+  int64_t tiles[2][2] = {}, work[2] = {};
+  for (size_t i = from; i < to; ++i)
+    for (int k = 0; k < 2; ++k) {
+      const Shape& h = shapes[i];
+      const int64_t N = k ? h.q : h.p;
+      for (int n = 0; n < 2; ++n) tiles[k][n] += h.batch * gemm::tiles_for(h.p, N, n ? 64 : 256);
+      work[k] += h.batch * gemm::tiles_for(h.p, N, 256) * gemm::steps_of(h.p);
+    }
+  for (int k = 0; k < 2; ++k) {
+    const int64_t per = (work[k] + tiles[k][0] - 1) / tiles[k][0];          // steps of a tile, on average
+    wide[k] = gemm::cost_of(k ? tiles[k][0] : (tiles[k][0] + 1) / 2, per, false);
+    narrow[k] = gemm::cost_of(k ? tiles[k][1] : (tiles[k][1] + 1) / 2, per, true);
+  }
+  const bool n0 = narrow[0] < wide[0], n1 = narrow[1] < wide[1];
   for (int s = 0; s < steps; ++s) {
     const int cur = s & 1;
-    for (int phase = 0; phase < 3; ++phase) {
-      w.problems = n;
-      w.scale0 = phase == 0 ? 1.f / (X_SCALE * X_SCALE) : static_cast<float>(phase == 1 ? b : a);
-      w.scale1 = phase == 1 ? static_cast<float>(c) : (s + 1 == steps ? 1.f : 0.f);
-      for (int i = 0; i < n; ++i) {
-        const Shape& h = shapes[from + i];
-        Problem& p = w.p[i];
-        const int64_t ldx = up8(h.q), lda = up8(h.p), bx = h.p * ldx, ba = h.p * lda;
-        p.in[0] = p.in[1] = nullptr;
-        p.partial = nullptr;
-        p.M = static_cast<int>(h.p);
-        p.N = static_cast<int>(phase == 2 ? h.q : h.p);
-        p.tiles_m = (p.M + gemm::TILE - 1) / gemm::TILE;
-        p.tiles_n = phase == 2 ? (p.N + gemm::TILE - 1) / gemm::TILE : -1;
-        p.batch = static_cast<int>(h.batch);
-        p.splits = 1;
-        const int64_t k = phase == 0 ? h.q : h.p;
-        p.steps0 = p.steps = static_cast<int>((k + gemm::KSTEP - 1) / gemm::KSTEP);
-        int rc = 0;
-        if (phase == 0) {
-          rc |= gemm::make_map(&p.a[0], h.hi[cur], true, h.q, h.p, h.batch, ldx, bx, gemm::BOX_K);
-          p.b[0] = p.a[0];
-          rc |= gemm::make_map(&p.out[0], h.A, true, h.p, h.p, h.batch, lda, ba, gemm::BOX_STORE);
-        } else if (phase == 1) {
-          rc |= gemm::make_map(&p.a[0], h.A, true, h.p, h.p, h.batch, lda, ba, gemm::BOX_K);
-          p.b[0] = p.a[0];
-          p.in[0] = h.A;
-          p.ld_in = lda; p.batch_in = ba;
-          rc |= gemm::make_map(&p.out[0], h.B, true, h.p, h.p, h.batch, lda, ba, gemm::BOX_STORE);
-        } else {
-          rc |= gemm::make_map(&p.a[0], h.B, true, h.p, h.p, h.batch, lda, ba, gemm::BOX_K);
-          rc |= gemm::make_map(&p.b[0], h.hi[cur], true, h.q, h.p, h.batch, ldx, bx, gemm::BOX_MN);
-          p.in[0] = h.hi[cur]; p.in[1] = h.lo;
-          p.ld_in = ldx; p.batch_in = bx;
-          rc |= gemm::make_map(&p.out[0], h.hi[cur ^ 1], true, h.q, h.p, h.batch, ldx, bx, gemm::BOX_STORE);
-          rc |= gemm::make_map(&p.out[1], h.lo, true, h.q, h.p, h.batch, ldx, bx, gemm::BOX_STORE);
-        }
-        if (rc) return rc;
-      }
-      if (int rc = phase == 0 ? gemm::launch<Gram>(w, true, st) : phase == 1 ? gemm::launch<Polynomial>(w, true, st) : gemm::launch<Apply>(w, true, st)) return rc;
-    }
+    const double gram = 1.0 / (X_SCALE * X_SCALE);
+    int rc = n0 ? run_product<Gram, 64, P>(shapes, from, to, 0, cur, gram, 0, st) : run_product<Gram, 256, P>(shapes, from, to, 0, cur, gram, 0, st);
+    if (rc) return rc;
+    rc = n0 ? run_product<Polynomial, 64, P>(shapes, from, to, 1, cur, b, c, st) : run_product<Polynomial, 256, P>(shapes, from, to, 1, cur, b, c, st);
+    if (rc) return rc;
+    const int left = steps - STEPS_WITHOUT_LOWER - s;
+    if (left > 1) rc = n1 ? run_product<Apply<2>, 64, P>(shapes, from, to, 2, cur, a, 0, st) : run_product<Apply<2>, 256, P>(shapes, from, to, 2, cur, a, 0, st);
+    else if (left == 1 || s == 0) rc = n1 ? run_product<Apply<1>, 64, P>(shapes, from, to, 2, cur, a, 0, st) : run_product<Apply<1>, 256, P>(shapes, from, to, 2, cur, a, 0, st);
+    else rc = n1 ? run_product<Apply<0>, 64, P>(shapes, from, to, 2, cur, a, 0, st) : run_product<Apply<0>, 256, P>(shapes, from, to, 2, cur, a, 0, st);
+    if (rc) return rc;
   }
   return HASTE_OK;
 }
@@ -499,7 +515,7 @@ int for_each_table(const std::vector<Matrix>& all, F&& f) {
   return HASTE_OK;
 }
 
-constexpr int FEW_SHAPES = 4, MANY_SHAPES = 28;
+constexpr int FEW_SHAPES = 4, MANY_SHAPES = 24;
 
 }  // namespace
 
