@@ -15,7 +15,6 @@ namespace haste {
 namespace {
 
 using gemm::Operand;
-using gemm::Problem;
 using gemm::steps_of;
 using gemm::Tile;
 using gemm::Work;
@@ -57,9 +56,9 @@ __device__ __forceinline__ float activate(float g) {
 template <int ACT>
 struct GatedForward {
   static constexpr bool A_MN = false, B_MN = false, F16 = false, PAIRED_B = true;
-  static constexpr int INPUTS = 0;
+  static constexpr int PARTS = 1, OUTPUTS = 3, INPUTS = 0;
   template <class W, class I, class S>
-  static __device__ __forceinline__ void chunk(const W& w, const Problem& p, const Tile& t, int row0, int col, bool, uint32_t tmem, I&, S& st, int lane) {
+  static __device__ __forceinline__ void chunk(const W& w, const gemm::Problem<GatedForward>& p, const Tile& t, int row0, int col, uint32_t tmem, I&, S& st, int lane) {
     constexpr int OTHER = I::L::COLUMNS;             // up's accumulator stands behind gate's
     const bool inside = row0 < p.M && col < p.N;
     uint32_t g[32], u[32], packed[16];
@@ -71,12 +70,12 @@ struct GatedForward {
       for (int i = 0; i < 16; ++i) packed[i] = gemm::pack_bf16(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
       uint32_t box = st.get();
       gemm::box_row(box, lane, packed);
-      st.put(&p.out[0], box, col, row0, t.batch, inside);
+      st.put(&p.out[0], box, col, row0, 0, inside);
 #pragma unroll
       for (int i = 0; i < 16; ++i) packed[i] = gemm::pack_bf16(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
       box = st.get();
       gemm::box_row(box, lane, packed);
-      st.put(&p.out[1], box, col, row0, t.batch, inside);
+      st.put(&p.out[1], box, col, row0, 0, inside);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i)
@@ -84,7 +83,7 @@ struct GatedForward {
                                   activate<ACT>(__uint_as_float(g[2 * i + 1])) * __uint_as_float(u[2 * i + 1]));
     const uint32_t box = st.get();
     gemm::box_row(box, lane, packed);
-    st.put(&p.out[2], box, col, row0, t.batch, inside);
+    st.put(&p.out[2], box, col, row0, 0, inside);
   }
 };
 
@@ -92,9 +91,9 @@ struct GatedForward {
 template <int ACT>
 struct GatedBackward {
   static constexpr bool A_MN = false, B_MN = true, F16 = false, PAIRED_B = false;
-  static constexpr int INPUTS = 2;
+  static constexpr int PARTS = 1, OUTPUTS = 3, INPUTS = 2;
   template <class W, class I, class S>
-  static __device__ __forceinline__ void chunk(const W&, const Problem& p, const Tile& t, int row0, int col, bool, uint32_t tmem, I& in, S& st, int lane) {
+  static __device__ __forceinline__ void chunk(const W&, const gemm::Problem<GatedBackward>& p, const Tile& t, int row0, int col, uint32_t tmem, I& in, S& st, int lane) {
     const bool inside = row0 < p.M && col < p.N;
     uint32_t g[16], u[16], d[32], dup[16], h[16];
     sm100::tmem_ld32(tmem, d);
@@ -115,23 +114,23 @@ struct GatedBackward {
     }
     uint32_t box = st.get();
     gemm::box_row(box, lane, g);
-    st.put(&p.out[0], box, col, row0, t.batch, inside);
+    st.put(&p.out[0], box, col, row0, 0, inside);
     box = st.get();
     gemm::box_row(box, lane, dup);
-    st.put(&p.out[1], box, col, row0, t.batch, inside);
+    st.put(&p.out[1], box, col, row0, 0, inside);
     box = st.get();
     gemm::box_row(box, lane, h);
-    st.put(&p.out[2], box, col, row0, t.batch, inside);
+    st.put(&p.out[2], box, col, row0, 0, inside);
   }
 };
 
 // out[0] = the product in bf16, or fp32 parts in `partial` [splits][M][N rounded up to 4]
-template <bool A, bool B>
+template <bool A, bool B, int K_PARTS = 1>
 struct Plain {
   static constexpr bool A_MN = A, B_MN = B, F16 = false, PAIRED_B = false;
-  static constexpr int INPUTS = 0;
+  static constexpr int PARTS = K_PARTS, OUTPUTS = 1, INPUTS = 0;
   template <class W, class I, class S>
-  static __device__ __forceinline__ void chunk(const W&, const Problem& p, const Tile& t, int row0, int col, bool, uint32_t tmem, I&, S& st, int lane) {
+  static __device__ __forceinline__ void chunk(const W&, const gemm::Problem<Plain>& p, const Tile& t, int row0, int col, uint32_t tmem, I&, S& st, int lane) {
     uint32_t v[32];
     sm100::tmem_ld32(tmem, v);
     sm100::tmem_ld_wait();
@@ -150,7 +149,7 @@ struct Plain {
       for (int i = 0; i < 16; ++i) packed[i] = gemm::pack_bf16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
       const uint32_t box = st.get();
       gemm::box_row(box, lane, packed);
-      st.put(&p.out[0], box, col, row0, t.batch, row0 < p.M && col < p.N);
+      st.put(&p.out[0], box, col, row0, 0, row0 < p.M && col < p.N);
     }
   }
 };
@@ -390,17 +389,17 @@ Output output_of(Arena& arena, void* p, int64_t M, int64_t N, const Form& f, boo
     o.part = static_cast<float*>(arena.take(o.splits * M * ((N + 3) & ~int64_t(3)) * 4));
   return o;
 }
-void set_sizes(Problem& p, int64_t M, int64_t N, int64_t steps0, int64_t steps) {
-  p = Problem();
+void set_sizes(gemm::Sizes& p, int64_t M, int64_t N, int64_t steps0, int64_t steps) {
+  p = gemm::Sizes();
   p.M = static_cast<int>(M); p.N = static_cast<int>(N);
-  p.batch = p.splits = 1;
+  p.splits = 1;
   p.steps0 = static_cast<int>(steps0); p.steps = static_cast<int>(steps);
 }
 template <class Policy>
-int set_output(Problem& p, const Output& o) {
+int set_output(gemm::Problem<Policy>& p, const Output& o) {
   p.splits = o.splits;
   p.partial = o.part;
-  return o.part == nullptr ? gemm::map_result<Policy>(&p.out[0], {o.p, p.N, 0}, p.M, p.N) : HASTE_OK;
+  return o.part == nullptr ? gemm::map_result<Policy>(&p.out[0], {o.p, p.N}, p.M, p.N) : HASTE_OK;
 }
 void add_sum(Sums& s, const Output& o, int64_t M, int64_t N) {
   if (o.part == nullptr) return;
@@ -467,33 +466,35 @@ int forward(Arena& arena, const GatedCall& c, cudaStream_t st) {
   const Output y = output_of(arena, c.y, c.T, c.O, fy, any);
   if (plan) return HASTE_OK;
   HASTE_TRY(align.run(st));
-  Work<1> w = {};
-  w.problems = 1;
-  w.scale0 = c.gate != nullptr ? 1.f : 0.f;
   const bool narrow = gemm::cost_of(gemm::tiles_for(c.T, c.F, 64), sD, true) < gemm::cost_of(gemm::tiles_for(c.T, c.F, 128), sD, false);
   HASTE_TRY(by_activation<GatedForward>(c.act, narrow, [&](auto policy, auto columns) -> int {
     using K = decltype(policy);
     constexpr int TN = decltype(columns)::value;
-    Problem& p = w.p[0];
+    Work<K, 1> w = {};
+    w.problems = 1;
+    w.scale0 = c.gate != nullptr ? 1.f : 0.f;
+    auto& p = w.p[0];
     set_sizes(p, c.T, c.F, sD, sD);
-    HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], {x.p, x.ld, 0}, c.T, c.D)));
-    HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wg.p, wg.ld, 0}, c.F, c.D)));
-    HASTE_TRY((gemm::map_b<K, TN>(&p.b[1], {wu.p, wu.ld, 0}, c.F, c.D)));
+    HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], {x.p, x.ld}, c.T, c.D)));
+    HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wg.p, wg.ld}, c.F, c.D)));
+    HASTE_TRY((gemm::map_b<K, TN>(&p.b[1], {wu.p, wu.ld}, c.F, c.D)));
     if (c.gate != nullptr) {
-      HASTE_TRY(gemm::map_result<K>(&p.out[0], {c.gate, c.ldh, 0}, c.T, c.F));
-      HASTE_TRY(gemm::map_result<K>(&p.out[1], {c.up, c.ldh, 0}, c.T, c.F));
+      HASTE_TRY(gemm::map_result<K>(&p.out[0], {c.gate, c.ldh}, c.T, c.F));
+      HASTE_TRY(gemm::map_result<K>(&p.out[1], {c.up, c.ldh}, c.T, c.F));
     }
-    HASTE_TRY(gemm::map_result<K>(&p.out[2], {h, ldF, 0}, c.T, c.F));
+    HASTE_TRY(gemm::map_result<K>(&p.out[2], {h, ldF}, c.T, c.F));
     return gemm::launch<K, TN>(w, align.c.n > 0, st);
   }));
   HASTE_TRY(by_form<Plain<false, false>>(fy.narrow, [&](auto policy, auto columns) -> int {
     using K = decltype(policy);
     constexpr int TN = decltype(columns)::value;
-    Problem& p = w.p[0];
+    Work<K, 1> w = {};
+    w.problems = 1;
+    auto& p = w.p[0];
     set_sizes(p, c.T, c.O, sF, sF);
     HASTE_TRY(set_output<K>(p, y));
-    HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], {h, ldF, 0}, c.T, c.F)));
-    HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wd.p, wd.ld, 0}, c.O, c.F)));
+    HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], {h, ldF}, c.T, c.F)));
+    HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wd.p, wd.ld}, c.O, c.F)));
     return gemm::launch<K, TN>(w, true, st);
   }));
   Sums s = {};
@@ -521,36 +522,36 @@ int backward(Arena& arena, const GatedGradCall& c, cudaStream_t st) {
   if (plan) return HASTE_OK;
   HASTE_TRY(align.run(st));
   {
-    Work<1> w = {};
-    w.problems = 1;
     const bool narrow = gemm::cost_of(gemm::tiles_for(c.T, c.F, 64), sO, true) < gemm::cost_of(gemm::tiles_for(c.T, c.F, 256), sO, false);
     HASTE_TRY(by_activation<GatedBackward>(c.act, narrow, [&](auto policy, auto columns) -> int {
       using K = decltype(policy);
       constexpr int TN = decltype(columns)::value;
-      Problem& p = w.p[0];
+      Work<K, 1> w = {};
+      w.problems = 1;
+      auto& p = w.p[0];
       set_sizes(p, c.T, c.F, sO, sO);
-      HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], {dy.p, dy.ld, 0}, c.T, c.O)));
-      HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wd.p, wd.ld, 0}, c.F, c.O)));
-      HASTE_TRY(gemm::map_result<K>(&p.in[0], {gate.p, gate.ld, 0}, c.T, c.F));
-      HASTE_TRY(gemm::map_result<K>(&p.in[1], {up.p, up.ld, 0}, c.T, c.F));
+      HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], {dy.p, dy.ld}, c.T, c.O)));
+      HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wd.p, wd.ld}, c.F, c.O)));
+      HASTE_TRY(gemm::map_result<K>(&p.in[0], {gate.p, gate.ld}, c.T, c.F));
+      HASTE_TRY(gemm::map_result<K>(&p.in[1], {up.p, up.ld}, c.T, c.F));
       void* outs[3] = {dgate, dup, h};
-      for (int i = 0; i < 3; ++i) HASTE_TRY(gemm::map_result<K>(&p.out[i], {outs[i], ldF, 0}, c.T, c.F));
+      for (int i = 0; i < 3; ++i) HASTE_TRY(gemm::map_result<K>(&p.out[i], {outs[i], ldF}, c.T, c.F));
       return gemm::launch<K, TN>(w, align.c.n > 0, st);
     }));
   }
   if (c.dx != nullptr) {
-    Work<1> w = {};
-    w.problems = 1;
-    HASTE_TRY(by_form<Plain<false, true>>(fx.narrow, [&](auto policy, auto columns) -> int {
+    HASTE_TRY(by_form<Plain<false, true, 2>>(fx.narrow, [&](auto policy, auto columns) -> int {
       using K = decltype(policy);
       constexpr int TN = decltype(columns)::value;
-      Problem& p = w.p[0];
+      Work<K, 1> w = {};
+      w.problems = 1;
+      auto& p = w.p[0];
       set_sizes(p, c.T, c.D, sF, 2 * sF);
       HASTE_TRY(set_output<K>(p, dx));
-      HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], {dgate, ldF, 0}, c.T, c.F)));
-      HASTE_TRY((gemm::map_a<K, TN>(&p.a[1], {dup, ldF, 0}, c.T, c.F)));
-      HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wg.p, wg.ld, 0}, c.D, c.F)));
-      HASTE_TRY((gemm::map_b<K, TN>(&p.b[1], {wu.p, wu.ld, 0}, c.D, c.F)));
+      HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], {dgate, ldF}, c.T, c.F)));
+      HASTE_TRY((gemm::map_a<K, TN>(&p.a[1], {dup, ldF}, c.T, c.F)));
+      HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wg.p, wg.ld}, c.D, c.F)));
+      HASTE_TRY((gemm::map_b<K, TN>(&p.b[1], {wu.p, wu.ld}, c.D, c.F)));
       return gemm::launch<K, TN>(w, true, st);
     }));
     Sums s = {};
@@ -558,14 +559,14 @@ int backward(Arena& arena, const GatedGradCall& c, cudaStream_t st) {
     HASTE_TRY(run_sums(s, st));
   }
   if (tiles[0] == 0) return HASTE_OK;
-  Work<3> w = {};
   Sums s = {};
   HASTE_TRY(by_form<Plain<true, true>>(fw.narrow, [&](auto policy, auto columns) -> int {
     using K = decltype(policy);
     constexpr int TN = decltype(columns)::value;
+    Work<K, 3> w = {};
     auto weight = [&](const Output& o, const Operand& a, const Operand& b, int64_t M, int64_t N) -> int {
       if (o.p == nullptr) return HASTE_OK;
-      Problem& p = w.p[w.problems++];
+      auto& p = w.p[w.problems++];
       set_sizes(p, M, N, sT, sT);
       HASTE_TRY(set_output<K>(p, o));
       HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], a, M, c.T)));
@@ -573,9 +574,9 @@ int backward(Arena& arena, const GatedGradCall& c, cudaStream_t st) {
       add_sum(s, o, M, N);
       return HASTE_OK;
     };
-    HASTE_TRY(weight(dwg, {dgate, ldF, 0}, {x.p, x.ld, 0}, c.F, c.D));
-    HASTE_TRY(weight(dwu, {dup, ldF, 0}, {x.p, x.ld, 0}, c.F, c.D));
-    HASTE_TRY(weight(dwd, {dy.p, dy.ld, 0}, {h, ldF, 0}, c.O, c.F));
+    HASTE_TRY(weight(dwg, {dgate, ldF}, {x.p, x.ld}, c.F, c.D));
+    HASTE_TRY(weight(dwu, {dup, ldF}, {x.p, x.ld}, c.F, c.D));
+    HASTE_TRY(weight(dwd, {dy.p, dy.ld}, {h, ldF}, c.O, c.F));
     return gemm::launch<K, TN>(w, true, st);
   }));
   return run_sums(s, st);

@@ -6,7 +6,7 @@
 // issues tcgen05.mma.cta_group::2, whose operands are both CTAs' shared memory and whose accumulator is 128 x TN fp32 in each CTA's TMEM (two of
 // them, so that one is read while the next is summed).  Either operand lies with k or with its rows (m, n) contiguous.  What happens to an accumulator is
 // the policy's: its warps read TMEM, 32 rows x 32 columns at a time, beside boxes of that size of up to two 16-bit matrices, which each warp has brought by TMA
-// two ahead, and hand such boxes to tensor-map stores.  (With loads of its rows by every lane, when the accumulator was there, the last product of a Newton-Schulz
+// ahead, and hand such boxes to tensor-map stores.  (With loads of its rows by every lane, when the accumulator was there, the last product of a Newton-Schulz
 // step over 50 M elements took 154 us.)
 //
 // TN = 256 is what keeps the tensor cores fed from L2; where there are fewer such tiles than pairs of SMs a narrow form (TN = 64, or 128 for a paired b) has more
@@ -33,7 +33,6 @@ constexpr int TILE = 256;              // rows of a pair's tile
 constexpr int KSTEP = 64;              // one 128-byte swizzle row of 16-bit values
 constexpr int EPI_WARPS = 8;
 constexpr int BOX_BYTES = 32 * 32 * 2; // what a warp loads or stores at once
-constexpr int AHEAD = 2;               // boxes of each input that a warp has on their way
 constexpr int THREADS = 12 * 32;
 constexpr int GROUP_M = 8;             // tiles of m that are walked before the next of n: what runs at once shares its operands in L2
 
@@ -46,9 +45,10 @@ struct Layout {
   static constexpr int A_BYTES = 128 * KSTEP * 2;
   static constexpr int B_BYTES = TN / 2 * KSTEP * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int AHEAD = TN == 256 ? 2 : 1;                                          // boxes of each input that a warp has on their way
   static constexpr int IN_BOXES = AHEAD * Policy::INPUTS;                                  // per warp
-  static constexpr int OUT_BOXES = Policy::INPUTS > 0 ? 2 : 4;
-  static constexpr int STAGES = TN == 256 ? (Policy::INPUTS == 2 ? 4 : 5) : 5;
+  static constexpr int OUT_BOXES = TN == 256 && Policy::INPUTS > 0 ? 2 : 4;
+  static constexpr int STAGES = TN == 256 && Policy::INPUTS == 2 ? 4 : 5;
   static constexpr int OFF_EPI = STAGES * STAGE_BYTES;
   static constexpr int OFF_BAR = OFF_EPI + EPI_WARPS * (IN_BOXES + OUT_BOXES) * BOX_BYTES;
   static constexpr int BARRIERS = 2 * STAGES + 4 + EPI_WARPS * AHEAD;
@@ -116,66 +116,47 @@ __device__ __forceinline__ void cluster_sync_all() {
 }
 
 // ---------------------------------------------------------------- what a launch works on
-// One product, or a batch of products of one shape.
-struct Problem {
-  CUtensorMap a[2], b[2];          // first and second part of k; a policy with two operands b (one for each CTA) has them in b
-  CUtensorMap out[3], in[2];       // in: 16-bit matrices that the policy reads at the tile's place
+// One product: its sizes, and its tensor maps, as many as the policy has.
+struct Sizes {
   float* partial;                  // fp32 sums of the parts that k was cut into
   int M, N;                        // of the result
   int tiles_m, tiles_n;            // set by launch()
-  int symmetric;                   // only tiles on and below the diagonal
-  int batch, splits;
+  int splits;
   int steps0, steps;               // steps of k in the first part, and in both
-  int first, each;                 // number of this problem's first tile, and how many a matrix has; set by launch()
+  int first;                       // number of this problem's first tile; set by launch()
 };
-template <int P>
+template <class Policy>
+struct Problem : Sizes {
+  CUtensorMap a[Policy::PARTS], b[Policy::PAIRED_B ? 2 : Policy::PARTS];      // by the part of k; of a paired b by the CTA
+  CUtensorMap out[Policy::OUTPUTS], in[Policy::INPUTS > 0 ? Policy::INPUTS : 1];           // in: 16-bit matrices that the policy reads at the tile's place
+};
+template <class Policy, int P>
 struct Work {
-  Problem p[P];
+  Problem<Policy> p[P];
   int problems, tiles;
-  float scale0, scale1;            // the policy's factors
+  float scale0;                    // the policy's
   int* err;
   long long wait_limit;
 };
 struct Tile {
-  int problem, batch, split, m, n;
+  int problem, split, m, n;
 };
 
-// Columns' tiles that a row of tiles of a symmetric result has: those that begin before the row's end
-__host__ __device__ inline int symmetric_tiles(int m, int tiles_n, int per) { return (m + 1) * per < tiles_n ? (m + 1) * per : tiles_n; }
-
-// per: column tiles to a tile's 256 rows
-__host__ __device__ inline int tiles_of(const Problem& p, int per) {
-  if (!p.symmetric) return p.tiles_m * p.tiles_n;
-  int n = 0;
-  for (int m = 0; m < p.tiles_m; ++m) n += symmetric_tiles(m, p.tiles_n, per);
-  return n;
-}
-
-template <int P>
-__device__ __forceinline__ Tile tile_at(const Work<P>& w, int t, int per) {
+template <class Policy, int P>
+__device__ __forceinline__ Tile tile_at(const Work<Policy, P>& w, int t) {
   Tile r;
   r.problem = 0;
   if (P > 1)
     while (r.problem + 1 < w.problems && t >= w.p[r.problem + 1].first) ++r.problem;
-  const Problem& p = w.p[r.problem];
+  const Sizes& p = w.p[r.problem];
   t -= p.first;
-  const int bs = t / p.each;
-  t -= bs * p.each;
-  r.batch = bs / p.splits;
-  r.split = bs - r.batch * p.splits;
-  if (p.symmetric) {
-    // rows of tiles grow by `per` until they are as wide as the matrix
-    int m = static_cast<int>((sqrtf(8.f * static_cast<float>(t / per) + 1.f) - 1.f) * 0.5f);
-    while (m * (m + 1) / 2 * per > t) --m;
-    while ((m + 1) * (m + 2) / 2 * per <= t) ++m;
-    r.m = m;
-    r.n = t - m * (m + 1) / 2 * per;
-  } else {
-    const int band = t / (GROUP_M * p.tiles_n), in_band = t - band * GROUP_M * p.tiles_n;
-    const int high = min(GROUP_M, p.tiles_m - band * GROUP_M);
-    r.n = in_band / high;
-    r.m = band * GROUP_M + in_band - r.n * high;
-  }
+  const int each = p.tiles_m * p.tiles_n;
+  r.split = t / each;
+  t -= r.split * each;
+  const int band = t / (GROUP_M * p.tiles_n), in_band = t - band * GROUP_M * p.tiles_n;
+  const int high = min(GROUP_M, p.tiles_m - band * GROUP_M);
+  r.n = in_band / high;
+  r.m = band * GROUP_M + in_band - r.n * high;
   return r;
 }
 
@@ -241,7 +222,8 @@ __device__ __forceinline__ void row_of_box(uint32_t box, int lane, uint32_t (&p)
 template <class Policy, int P, int TN>
 struct Inputs {
   using L = Layout<Policy, TN>;
-  const Work<P>& w;
+  static constexpr int AHEAD = L::AHEAD;
+  const Work<Policy, P>& w;
   uint32_t base, bars;             // boxes and barriers of this warp
   int lane, quarter, half, rank, stride;
   int issue_t, issue_j, issued, taken;
@@ -249,13 +231,13 @@ struct Inputs {
 
   __device__ __forceinline__ void issue() {
     if (issue_t >= w.tiles) return;
-    if (issue_j == 0) tile = tile_at(w, issue_t, TILE / TN);
+    if (issue_j == 0) tile = tile_at(w, issue_t);
     if (lane == 0) {
-      const Problem& p = w.p[tile.problem];
+      const Problem<Policy>& p = w.p[tile.problem];
       const int slot = issued % AHEAD, x = tile.n * L::COLUMNS + half * (L::COLUMNS / 2) + issue_j * 32, y = tile.m * TILE + rank * 128 + quarter * 32;
       mbar_arrive_expect_tx(bars + 8 * slot, Policy::INPUTS * BOX_BYTES);
 #pragma unroll
-      for (int i = 0; i < Policy::INPUTS; ++i) tma_load_3d(base + (slot * Policy::INPUTS + i) * BOX_BYTES, &p.in[i], x, y, tile.batch, bars + 8 * slot);
+      for (int i = 0; i < Policy::INPUTS; ++i) tma_load_3d(base + (slot * Policy::INPUTS + i) * BOX_BYTES, &p.in[i], x, y, 0, bars + 8 * slot);
     }
     ++issued;
     if (++issue_j == L::CHUNKS) { issue_j = 0; issue_t += stride; }
@@ -282,12 +264,12 @@ struct Inputs {
 
 // ---------------------------------------------------------------- the kernel
 // Policy: A_MN, B_MN (the operand's rows are contiguous, not k), F16 (else bf16), PAIRED_B (each CTA has an operand b of its own: TN / 2 columns of
-// two products side by side), INPUTS, and
-//   static void chunk(w, p, tile, row0, col, diagonal, tmem, inputs, stager, lane)   32 rows x 32 columns of the result at (row0, col), accumulator at tmem
+// two products side by side), PARTS of k, OUTPUTS, INPUTS, and
+//   static void chunk(w, p, tile, row0, col, tmem, inputs, stager, lane)   32 rows x 32 columns of the result at (row0, col), accumulator at tmem
 template <class Policy, int P, int TN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm100_kernel(const __grid_constant__ Work<P> w) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm100_kernel(const __grid_constant__ Work<Policy, P> w) {
   using L = Layout<Policy, TN>;
-  constexpr int STAGES = L::STAGES, PER = TILE / TN;
+  constexpr int STAGES = L::STAGES, AHEAD = L::AHEAD;
   extern __shared__ uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   const uint32_t base = smem_u32(sm);
@@ -322,8 +304,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
     // ---------------- loads
     int it = 0;
     for (int t = first; t < w.tiles && !*abort_flag; t += stride) {
-      const Tile tl = tile_at(w, t, PER);
-      const Problem& p = w.p[tl.problem];
+      const Tile tl = tile_at(w, t);
+      const Problem<Policy>& p = w.p[tl.problem];
       const int k0 = static_cast<int>(static_cast<int64_t>(p.steps) * tl.split / p.splits), k1 = static_cast<int>(static_cast<int64_t>(p.steps) * (tl.split + 1) / p.splits);
       const int am = tl.m * TILE + static_cast<int>(rank) * 128;
       const int bn = Policy::PAIRED_B ? tl.n * (TN / 2) : tl.n * TN + static_cast<int>(rank) * (TN / 2);
@@ -338,16 +320,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
         const CUtensorMap* ta = &p.a[part];
         const CUtensorMap* tb = &p.b[Policy::PAIRED_B ? static_cast<int>(rank) : part];
         if (Policy::A_MN) {
-          tma_load_pair(as, ta, am, kc, tl.batch, bar);
-          tma_load_pair(as + L::A_BYTES / 2, ta, am + 64, kc, tl.batch, bar);
+          tma_load_pair(as, ta, am, kc, 0, bar);
+          tma_load_pair(as + L::A_BYTES / 2, ta, am + 64, kc, 0, bar);
         } else {
-          tma_load_pair(as, ta, kc, am, tl.batch, bar);
+          tma_load_pair(as, ta, kc, am, 0, bar);
         }
         if (Policy::B_MN) {
-          tma_load_pair(bs, tb, bn, kc, tl.batch, bar);
-          if (TN == 256) tma_load_pair(bs + L::B_BYTES / 2, tb, bn + 64, kc, tl.batch, bar);
+          tma_load_pair(bs, tb, bn, kc, 0, bar);
+          if (TN == 256) tma_load_pair(bs + L::B_BYTES / 2, tb, bn + 64, kc, 0, bar);
         } else {
-          tma_load_pair(bs, tb, kc, bn, tl.batch, bar);
+          tma_load_pair(bs, tb, kc, bn, 0, bar);
         }
       }
     }
@@ -363,8 +345,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
     constexpr uint64_t KA = Policy::A_MN ? 2048 >> 4 : 32 >> 4, KB = L::B_SMALL ? 1024 >> 4 : Policy::B_MN ? 2048 >> 4 : 32 >> 4;
     int it = 0, n = 0;
     for (int t = first; t < w.tiles; t += stride, ++n) {
-      const Tile tl = tile_at(w, t, PER);
-      const Problem& p = w.p[tl.problem];
+      const Tile tl = tile_at(w, t);
+      const Problem<Policy>& p = w.p[tl.problem];
       const int steps = static_cast<int>(static_cast<int64_t>(p.steps) * (tl.split + 1) / p.splits) - static_cast<int>(static_cast<int64_t>(p.steps) * tl.split / p.splits);
       const int buf = n & 1;
       if (!mbar_wait(bar_free(buf), ((n >> 1) & 1) ^ 1, abort_flag, w.err, 303, WL)) break;
@@ -396,8 +378,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
     in.start();
     int n = 0;
     for (int t = first; t < w.tiles; t += stride, ++n) {
-      const Tile tl = tile_at(w, t, PER);
-      const Problem& p = w.p[tl.problem];
+      const Tile tl = tile_at(w, t);
+      const Problem<Policy>& p = w.p[tl.problem];
       const int buf = n & 1, row0 = tl.m * TILE + static_cast<int>(rank) * 128 + quarter * 32, at = half * (L::COLUMNS / 2);
       bool ok = mbar_wait(bar_done(buf), (n >> 1) & 1, abort_flag, w.err, 305, WL);
       ok = __all_sync(0xffffffffu, ok);
@@ -406,7 +388,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
 #pragma unroll 1
       for (int j = 0; j < L::CHUNKS && ok; ++j) {
         ok = in.wait(abort_flag);
-        if (ok) Policy::chunk(w, p, tl, row0, tl.n * L::COLUMNS + at + 32 * j, tl.n / PER == tl.m, tmem + buf * TN + (static_cast<uint32_t>(quarter * 32) << 16) + at + 32 * j, in, st, lane);
+        if (ok) Policy::chunk(w, p, tl, row0, tl.n * L::COLUMNS + at + 32 * j, tmem + buf * TN + (static_cast<uint32_t>(quarter * 32) << 16) + at + 32 * j, in, st, lane);
       }
       if (!ok) break;
       tc_fence_before();
@@ -435,24 +417,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
 inline int make_map(CUtensorMap* out, const void* base, bool f16, int64_t inner, int64_t outer, int64_t batch, int64_t ld, int64_t batch_stride, int box_inner, int box_outer) {
   return make_tmap_16bit_3d(out, base, f16, inner, outer, batch, ld * 2, (batch_stride ? batch_stride : ld * outer) * 2, static_cast<uint32_t>(box_inner), static_cast<uint32_t>(box_outer));
 }
-// Where a 16-bit matrix (or a batch of them) lies
+// Where a 16-bit matrix lies
 struct Operand {
   const void* p;
-  int64_t ld, batch_stride;        // 0: a matrix's size
+  int64_t ld;
 };
 // Operand a of `rows` (the result's M) and b of `rows` (its N), k values each; inputs and outputs of the result's size
 template <class Policy, int TN>
-int map_a(CUtensorMap* out, const Operand& o, int64_t rows, int64_t k, int64_t batch = 1) {
-  return Policy::A_MN ? make_map(out, o.p, Policy::F16, rows, k, batch, o.ld, o.batch_stride, 64, 64) : make_map(out, o.p, Policy::F16, k, rows, batch, o.ld, o.batch_stride, 64, 128);
+int map_a(CUtensorMap* out, const Operand& o, int64_t rows, int64_t k) {
+  return Policy::A_MN ? make_map(out, o.p, Policy::F16, rows, k, 1, o.ld, 0, 64, 64) : make_map(out, o.p, Policy::F16, k, rows, 1, o.ld, 0, 64, 128);
 }
 template <class Policy, int TN>
-int map_b(CUtensorMap* out, const Operand& o, int64_t rows, int64_t k, int64_t batch = 1) {
-  return Policy::B_MN ? make_map(out, o.p, Policy::F16, rows, k, batch, o.ld, o.batch_stride, TN == 64 ? 32 : 64, 64)
-                      : make_map(out, o.p, Policy::F16, k, rows, batch, o.ld, o.batch_stride, 64, TN / 2);
+int map_b(CUtensorMap* out, const Operand& o, int64_t rows, int64_t k) {
+  return Policy::B_MN ? make_map(out, o.p, Policy::F16, rows, k, 1, o.ld, 0, TN == 64 ? 32 : 64, 64)
+                      : make_map(out, o.p, Policy::F16, k, rows, 1, o.ld, 0, 64, TN / 2);
 }
 template <class Policy>
-int map_result(CUtensorMap* out, const Operand& o, int64_t M, int64_t N, int64_t batch = 1) {
-  return make_map(out, o.p, Policy::F16, N, M, batch, o.ld, o.batch_stride, 32, 32);
+int map_result(CUtensorMap* out, const Operand& o, int64_t M, int64_t N) {
+  return make_map(out, o.p, Policy::F16, N, M, 1, o.ld, 0, 32, 32);
 }
 inline int64_t steps_of(int64_t k) { return (k + KSTEP - 1) / KSTEP; }
 
@@ -492,20 +474,19 @@ inline int64_t tiles_for(int64_t M, int64_t N, int64_t columns) { return ((M + T
 
 // Launches what is in w.p[0 .. problems): tiles are counted here.  behind: the kernel before it in the stream is one of the same call.
 template <class Policy, int TN, int P>
-int launch(Work<P>& w, bool behind, cudaStream_t st) {
+int launch(Work<Policy, P>& w, bool behind, cudaStream_t st) {
   using L = Layout<Policy, TN>;
   auto kernel = gemm_sm100_kernel<Policy, P, TN>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM_BYTES);
   if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   int64_t tiles = 0;
   for (int i = 0; i < w.problems; ++i) {
-    Problem& p = w.p[i];
+    Sizes& p = w.p[i];
     p.tiles_m = (p.M + TILE - 1) / TILE;
     p.tiles_n = (p.N + L::COLUMNS - 1) / L::COLUMNS;
     if (static_cast<int64_t>(p.tiles_m) * p.tiles_n > 0x3FFFFFFF) return fail(HASTE_ERR_TOO_LARGE, "too many tiles for one launch");
     p.first = static_cast<int>(tiles);
-    p.each = tiles_of(p, TILE / TN);
-    tiles += static_cast<int64_t>(p.each) * p.batch * p.splits;
+    tiles += static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
     if (tiles > 0x3FFFFFFF) return fail(HASTE_ERR_TOO_LARGE, "too many tiles for one launch");
   }
   if (tiles == 0) return HASTE_OK;

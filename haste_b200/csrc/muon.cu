@@ -1,128 +1,37 @@
 // Muon: the update of a matrix is its momentum, made orthogonal by Newton-Schulz steps.
 //
 //   m = mu m + (1 - mu) g,   u = mu m + (1 - mu) g (Nesterov) or m,   X = u / max(|u|, eps)        (X has the smaller side as rows)
-//   steps times:  A = X X^T,  X <- a X + (b A + c A A) X
+//   steps times:  A = X X^T,  B = a I + b A + c A A,  X <- B X
 //   w = w (1 - lr weight_decay) - lr rate X
 //
-// For a list of matrices at once: one launch for the norms, one that writes the momentum and X, three products a step over all matrices (those of one shape
-// are a batch, shapes are problems of one launch, gemm_sm100.cuh), one that updates the weights.
+// For a list of matrices at once: one launch for the norms, one that writes the momentum and X (rows and columns padded with zeros to multiples of 64, which stay
+// zeros: so matrices of nearly one size are one batch), one for all steps (newton_schulz.cuh), one that updates the weights.
 //
 // Rounding.  The products take fp16: X times 2^8 (its entries are at most 1, later 1.3 or so; the factor keeps small ones out of the subnormals), A and
-// B = b A + c A A.  The term a X, by which small singular values grow 3.4 times a step, takes X as a sum of two fp16 values, hi + lo 2^-11: 22 bits.  Without lo
-// an update of low rank with noise is off by 1.3e-2 after five steps (2-norm of the difference over that of the result), with it by 1e-3, a Gaussian one by 1.4e-3;
-// with bf16 in place of fp16 1e-1 and 1e-2.  A and A A are symmetric: tiles on and below the diagonal are computed, the others are their mirror.
-#include "gemm_sm100.cuh"
-
+// B.  By the term a I small singular values grow 3.4 times a step, and so does what rounding X adds to them; it takes X as a sum of two fp16 values, hi + lo 2^-11:
+// 22 bits.  Without lo an update of low rank with noise is off by 1.3e-2 after five steps (2-norm of the difference over that of the result), with it in the first three by
+// 1.4e-3, and so is a Gaussian one; with bf16 in place of fp16 1e-1 and 1e-2.  A and A A are symmetric: tiles on and below the diagonal are computed, the others are
+// their mirror.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <vector>
+
+#include "newton_schulz.cuh"
 
 namespace haste {
 namespace {
 
-using gemm::Problem;
-using gemm::Tile;
-using gemm::Work;
-
-constexpr float X_SCALE = 256.f;
-constexpr float LO_SCALE = 2048.f;
-
-// ---------------------------------------------------------------- products
-template <class S>
-__device__ __forceinline__ void put_symmetric(const Problem& p, const Tile& t, int row0, int col, bool diagonal, const uint32_t (&packed)[16], S& st, int lane) {
-  const bool inside = row0 < p.M && col < p.N;
-  uint32_t box = st.get();
-  gemm::box_row(box, lane, packed);
-  st.put(&p.out[0], box, col, row0, t.batch, inside);
-  if (!diagonal) {
-    box = st.get();
-    gemm::box_column(box, lane, packed);
-    st.put(&p.out[0], box, row0, col, t.batch, inside);
-  }
-}
-
-// A = scale0 X X^T
-struct Gram {
-  static constexpr bool A_MN = false, B_MN = false, F16 = true, PAIRED_B = false;
-  static constexpr int INPUTS = 0;
-  template <class W, class I, class S>
-  static __device__ __forceinline__ void chunk(const W& w, const Problem& p, const Tile& t, int row0, int col, bool diagonal, uint32_t tmem, I&, S& st, int lane) {
-    uint32_t v[32], packed[16];
-    sm100::tmem_ld32(tmem, v);
-    sm100::tmem_ld_wait();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) packed[i] = gemm::pack_f16(__uint_as_float(v[2 * i]) * w.scale0, __uint_as_float(v[2 * i + 1]) * w.scale0);
-    put_symmetric(p, t, row0, col, diagonal, packed, st, lane);
-  }
-};
-
-// B = scale0 A + scale1 A A^T; in[0] = A
-struct Polynomial {
-  static constexpr bool A_MN = false, B_MN = false, F16 = true, PAIRED_B = false;
-  static constexpr int INPUTS = 1;
-  template <class W, class I, class S>
-  static __device__ __forceinline__ void chunk(const W& w, const Problem& p, const Tile& t, int row0, int col, bool diagonal, uint32_t tmem, I& in, S& st, int lane) {
-    uint32_t v[32], packed[16];
-    sm100::tmem_ld32(tmem, v);
-    in.get(0, packed);
-    in.release();
-    sm100::tmem_ld_wait();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float2 a = gemm::unpack_f16(packed[i]);
-      packed[i] = gemm::pack_f16(fmaf(w.scale1, __uint_as_float(v[2 * i]), w.scale0 * a.x), fmaf(w.scale1, __uint_as_float(v[2 * i + 1]), w.scale0 * a.y));
-    }
-    put_symmetric(p, t, row0, col, diagonal, packed, st, lane);
-  }
-};
-
-// X' = scale0 X + B X; in[0] = X's upper part, in[1] its lower one, if it has one (LOWER: 2 and 1); out[0] and out[1] those of X', the lower one with LOWER = 2 alone.  (in[1] and
-// out[1] are one place: a tile reads what it writes.)
-template <int LOWER>
-struct Apply {
-  static constexpr bool A_MN = false, B_MN = true, F16 = true, PAIRED_B = false;
-  static constexpr int INPUTS = LOWER ? 2 : 1;
-  template <class W, class I, class S>
-  static __device__ __forceinline__ void chunk(const W& w, const Problem& p, const Tile& t, int row0, int col, bool, uint32_t tmem, I& in, S& st, int lane) {
-    const bool inside = row0 < p.M && col < p.N;
-    uint32_t v[32], hi[16], lo[16];
-    sm100::tmem_ld32(tmem, v);
-    in.get(0, hi);
-    if (LOWER) in.get(1, lo);
-    in.release();
-    sm100::tmem_ld_wait();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float2 h = gemm::unpack_f16(hi[i]);
-      if (LOWER) {
-        const float2 l = gemm::unpack_f16(lo[i]);
-        h.x = fmaf(l.x, 1.f / LO_SCALE, h.x);
-        h.y = fmaf(l.y, 1.f / LO_SCALE, h.y);
-      }
-      const float x = fmaf(w.scale0, h.x, __uint_as_float(v[2 * i])), y = fmaf(w.scale0, h.y, __uint_as_float(v[2 * i + 1]));
-      hi[i] = gemm::pack_f16(x, y);
-      if (LOWER == 2) {
-        const float2 r = gemm::unpack_f16(hi[i]);
-        lo[i] = gemm::pack_f16((x - r.x) * LO_SCALE, (y - r.y) * LO_SCALE);
-      }
-    }
-    uint32_t box = st.get();
-    gemm::box_row(box, lane, hi);
-    st.put(&p.out[0], box, col, row0, t.batch, inside);
-    if (LOWER == 2) {
-      box = st.get();
-      gemm::box_row(box, lane, lo);
-      st.put(&p.out[1], box, col, row0, t.batch, inside);
-    }
-  }
-};
+using newton_schulz::LO_SCALE;
+using newton_schulz::X_SCALE;
 
 // ---------------------------------------------------------------- elementwise
 constexpr int NORM_THREADS = 256;
-constexpr int NORM_PARTS = 256;                    // of a matrix, at most
+constexpr int NORM_PARTS = 64;                     // of a matrix, at most
 constexpr int NORM_ELEMENTS = 8192;                // of a block, at least
-constexpr int TABLE = 192;                         // matrices of one launch
+constexpr int FEW = 8, MANY = 192;                 // matrices of one launch
 constexpr int SIDE = 64;                           // of an elementwise tile
+constexpr int ROWS = SIDE / 16;                    // of a thread: 16 of a block's threads have a row, 4 elements each
 
 struct Matrix {
   const void* g;
@@ -130,40 +39,63 @@ struct Matrix {
   float* m;                        // momentum, NULL without
   uint16_t *hi, *lo;               // X's parts, rows of ld elements
   double* parts;                   // sums of squares, by block
+  unsigned long long* done;        // the steps' counter
   int64_t at;                      // place in the momentum, for the random bits
-  int rows, cols, ld;
-  int nparts, first_part, first_tile;
+  int rows, cols, ld, nparts;      // ld: X's columns, padded
   float rate;
 };
+template <int N>
 struct Matrices {
-  Matrix a[TABLE];
-  int n, parts, tiles;
+  int first_part[N + 1], first_tile[N + 1];        // of each matrix, and the ends
+  int n;
+  Matrix a[N];
 };
 struct Coefficients {
   float mu, one_mu, decay, eps;
   int nesterov, sr;
   uint32_t seed, step, stream;
 };
+// The last matrix that begins at `block` or before (a walk over all of them took longer than the work: every step a miss in the constants' cache)
+__device__ __forceinline__ int matrix_of(const int* first, int n, int block) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first[mid] <= block) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
 
-__device__ __forceinline__ void load4(const __nv_bfloat16* p, int n, bool vec, float (&v)[4]) {
-  if (vec) {
-    const uint2 q = *reinterpret_cast<const uint2*>(p);
+// Four neighbouring elements as they lie in memory: looked into only when all loads are on their way
+template <class T>
+struct Raw;
+template <>
+struct Raw<__nv_bfloat16> {
+  uint2 q;
+  __device__ __forceinline__ void zero() { q = make_uint2(0, 0); }
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { q = *reinterpret_cast<const uint2*>(p); }
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, int n) {
+    const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? u[i] : 0;
+    q = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
+  }
+  __device__ __forceinline__ void get(float (&v)[4]) const {
     const float2 a = gemm::unpack_bf16(q.x), b = gemm::unpack_bf16(q.y);
     v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < n ? __bfloat162float(p[i]) : 0.f;
   }
-}
-__device__ __forceinline__ void load4(const float* p, int n, bool vec, float (&v)[4]) {
-  if (vec) {
-    const float4 q = *reinterpret_cast<const float4*>(p);
-    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : 0.f;
-  }
-}
+};
+template <>
+struct Raw<float> {
+  float4 q;
+  __device__ __forceinline__ void zero() { q = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void load(const float* p) { q = *reinterpret_cast<const float4*>(p); }
+  __device__ __forceinline__ void load(const float* p, int n) { q = make_float4(n > 0 ? p[0] : 0.f, n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, n > 3 ? p[3] : 0.f); }
+  __device__ __forceinline__ void get(float (&v)[4]) const { v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w; }
+};
+template <class T>
+__device__ __forceinline__ bool on_four(const T* p) { return (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0; }
 __device__ __forceinline__ void store4(float* p, int n, bool vec, const float (&v)[4]) {
   if (vec) {
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
@@ -184,25 +116,47 @@ __device__ __forceinline__ float direction(const Coefficients& c, float g, float
 }
 
 // Sum of squares of each matrix's direction, in 64 bits (a square of fp32 has a place there whatever its size), in an order that the sizes alone decide
-template <class G>
-__global__ void __launch_bounds__(NORM_THREADS) muon_squares_kernel(const __grid_constant__ Matrices t, const Coefficients c) {
+template <class G, int N>
+__global__ void __launch_bounds__(NORM_THREADS) muon_squares_kernel(const __grid_constant__ Matrices<N> t, const Coefficients c) {
+  constexpr int AT_ONCE = 4;
   __shared__ double warps[NORM_THREADS / 32];
-  int k = 0;
-  while (k + 1 < t.n && static_cast<int>(blockIdx.x) >= t.a[k + 1].first_part) ++k;
+  const int k = matrix_of(t.first_part, t.n, blockIdx.x), part = blockIdx.x - t.first_part[k];
   const Matrix& a = t.a[k];
-  const int part = blockIdx.x - a.first_part;
   const int64_t n = static_cast<int64_t>(a.rows) * a.cols, groups = (n + 3) / 4;
   const G* g = static_cast<const G*>(a.g);
+  const float* m = a.m;
+  const bool vec = on_four(g);
+  const int64_t stride = static_cast<int64_t>(a.nparts) * NORM_THREADS;
   double sum = 0;
-  for (int64_t i = static_cast<int64_t>(part) * NORM_THREADS + threadIdx.x; i < groups; i += static_cast<int64_t>(a.nparts) * NORM_THREADS) {
-    const int have = static_cast<int>(imin64(4, n - 4 * i));
-    float gv[4], mv[4] = {0, 0, 0, 0};
-    load4(g + 4 * i, have, vec4(g + 4 * i, have), gv);
-    if (a.m != nullptr) load4(a.m + 4 * i, have, have == 4, mv);
+  for (int64_t i0 = static_cast<int64_t>(part) * NORM_THREADS + threadIdx.x; i0 < groups; i0 += stride * AT_ONCE) {
+    Raw<G> gr[AT_ONCE];
+    Raw<float> mr[AT_ONCE];
+    if (vec && 4 * (i0 + (AT_ONCE - 1) * stride) + 4 <= n) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const double u = direction(c, gv[x], mv[x], a.m != nullptr);
-      if (x < have) sum += u * u;
+      for (int j = 0; j < AT_ONCE; ++j) gr[j].load(g + 4 * (i0 + j * stride));
+      if (m != nullptr) {
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) mr[j].load(m + 4 * (i0 + j * stride));
+      }
+    } else {                                       // zeros beyond the matrix
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const int64_t i = i0 + j * stride;
+        const int have = static_cast<int>(imin64(4, n - 4 * i));
+        gr[j].load(g + 4 * i, have);
+        if (m != nullptr) mr[j].load(m + 4 * i, have);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      float gv[4], mv[4] = {0.f, 0.f, 0.f, 0.f};
+      gr[j].get(gv);
+      if (m != nullptr) mr[j].get(mv);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const double u = direction(c, gv[x], mv[x], m != nullptr);
+        sum = fma(u, u, sum);
+      }
     }
   }
 #pragma unroll
@@ -215,80 +169,133 @@ __global__ void __launch_bounds__(NORM_THREADS) muon_squares_kernel(const __grid
   }
 }
 
-// 1 / max(norm, eps), NaN or 0 where the norm is NaN or inf; by all threads of a block
-__device__ __forceinline__ float inverse_norm(const Matrix& a, float eps, double* shared) {
-  double s = threadIdx.x < a.nparts ? a.parts[threadIdx.x] : 0.0;
+// 1 / max(norm, eps), NaN or 0 where the norm is NaN or inf; by every warp for itself, so the root is taken in 32 bits: of the sum times an even power of two
+__device__ __forceinline__ float inverse_norm(const Matrix& a, float eps) {
+  const int lane = threadIdx.x & 31;
+  double s = (lane < a.nparts ? a.parts[lane] : 0.0) + (lane + 32 < a.nparts ? a.parts[lane + 32] : 0.0);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = s;
-  __syncthreads();
-  s = 0;
-  for (int i = 0; i < NORM_THREADS / 32; ++i) s += shared[i];
-  const double norm = sqrt(s);
-  return static_cast<float>(1.0 / (norm < eps ? static_cast<double>(eps) : norm));
+  if (!(s < INFINITY)) return static_cast<float>(s) - static_cast<float>(s);       // NaN
+  const int high = __double2hiint(s), k = ((high >> 20) - 1023) >> 1;              // s = m 4^k, 1 <= m < 4
+  const float m = __double2float_rn(s == 0.0 ? 0.0 : __hiloint2double(high - (k << 21), __double2loint(s)));
+  const float root = sqrtf(m);
+  // |u| = root 2^k against eps, and its inverse
+  const float norm = ldexpf(root, k);
+  return norm < eps ? 1.f / eps : ldexpf(1.f / root, -k);
 }
 __device__ __forceinline__ bool usable(float inverse) { return inverse > 0.f && inverse < INFINITY; }
 
-__device__ __forceinline__ const Matrix& tile_of(const Matrices& t, int block, int& row0, int& col0) {
-  int k = 0;
-  while (k + 1 < t.n && block >= t.a[k + 1].first_tile) ++k;
-  const Matrix& a = t.a[k];
-  const int across = (a.cols + SIDE - 1) / SIDE, i = block - a.first_tile;
-  row0 = i / across * SIDE;
-  col0 = (i - i / across * across) * SIDE;
-  return a;
+// A block's share of all tiles of 64 x 64, one after the other: what a matrix needs is looked up once
+template <int N>
+struct Walk {
+  const Matrices<N>& t;
+  int at, end, k, across, row0, col0;
+  __device__ __forceinline__ explicit Walk(const Matrices<N>& m) : t(m) {
+    const int tiles = t.first_tile[t.n];
+    at = static_cast<int>(static_cast<int64_t>(tiles) * blockIdx.x / gridDim.x);
+    end = static_cast<int>(static_cast<int64_t>(tiles) * (blockIdx.x + 1) / gridDim.x);
+    k = matrix_of(t.first_tile, t.n, at);
+    across = (t.a[k].cols + SIDE - 1) / SIDE;
+    const int i = at - t.first_tile[k];
+    row0 = i / across * SIDE;
+    col0 = (i - i / across * across) * SIDE;
+  }
+  __device__ __forceinline__ bool more() const { return at < end; }
+  // whether the next tile is of another matrix
+  __device__ __forceinline__ bool next() {
+    ++at;
+    col0 += SIDE;
+    if (col0 >= across * SIDE) {
+      col0 = 0;
+      row0 += SIDE;
+    }
+    if (at < end && at >= t.first_tile[k + 1]) {
+      ++k;
+      across = (t.a[k].cols + SIDE - 1) / SIDE;
+      row0 = col0 = 0;
+      return true;
+    }
+    return false;
+  }
+};
+__device__ __forceinline__ void store_x(const Matrix& a, int row, int col, const float (&x)[4]) {
+  const uint32_t h0 = gemm::pack_f16(x[0], x[1]), h1 = gemm::pack_f16(x[2], x[3]);
+  const float2 a0 = gemm::unpack_f16(h0), a1 = gemm::unpack_f16(h1);
+  const int64_t to = static_cast<int64_t>(row) * a.ld + col;
+  *reinterpret_cast<uint2*>(a.hi + to) = make_uint2(h0, h1);
+  *reinterpret_cast<uint2*>(a.lo + to) = make_uint2(gemm::pack_f16((x[0] - a0.x) * LO_SCALE, (x[1] - a0.y) * LO_SCALE), gemm::pack_f16((x[2] - a1.x) * LO_SCALE, (x[3] - a1.y) * LO_SCALE));
 }
 
-// Momentum and X.  A matrix whose norm is not finite keeps its momentum.
-template <class G>
-__global__ void __launch_bounds__(256) muon_start_kernel(const __grid_constant__ Matrices t, const Coefficients c) {
-  __shared__ double sums[NORM_THREADS / 32];
+// Momentum and X, zeros in its padding.  A matrix whose norm is not finite keeps its momentum.
+template <class G, int N>
+__global__ void __launch_bounds__(256) muon_start_kernel(const __grid_constant__ Matrices<N> t, const Coefficients c) {
   __shared__ float turned[SIDE][SIDE + 1];
-  int row0, col0;
-  const Matrix& a = tile_of(t, blockIdx.x, row0, col0);
+  Walk<N> walk(t);
+  const int cg = (threadIdx.x & 15) * 4, r0 = threadIdx.x / 16;
   sm100::grid_dependency_wait();
-  const float inv = inverse_norm(a, c.eps, sums), factor = inv * X_SCALE;
-  const bool tall = a.rows > a.cols, momentum = a.m != nullptr, write = momentum && usable(inv);
-  const int cg = (threadIdx.x & 15) * 4, col = col0 + cg, have = min(4, a.cols - col);
+  float inv = walk.more() ? inverse_norm(t.a[walk.k], c.eps) : 0.f;
+  while (walk.more()) {
+    const Matrix& a = t.a[walk.k];
+    const int row0 = walk.row0, col0 = walk.col0;
+    const bool tall = a.rows > a.cols, momentum = a.m != nullptr, write = momentum && usable(inv);
+    const float factor = inv * X_SCALE;
+    const int col = col0 + cg, have = min(4, a.cols - col);
+    const G* g = static_cast<const G*>(a.g);
+    Raw<G> gr[ROWS];
+    Raw<float> mr[ROWS];
+    // a tile within the matrix, whose rows all start on four elements
+    const bool whole = row0 + SIDE <= a.rows && col0 + SIDE <= a.cols && a.cols % 4 == 0 && on_four(g);
+    const int64_t from = static_cast<int64_t>(row0 + r0) * a.cols + col, step = static_cast<int64_t>(16) * a.cols;
+    if (whole) {
 #pragma unroll
-  for (int k = 0; k < SIDE / 16; ++k) {
-    const int r = threadIdx.x / 16 + 16 * k, row = row0 + r;
-    if (row < a.rows && have > 0) {
+      for (int k = 0; k < ROWS; ++k) gr[k].load(g + from + k * step);
+      if (momentum) {
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) mr[k].load(a.m + from + k * step);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) {
+        const int n = row0 + r0 + 16 * k < a.rows ? have : 0;
+        gr[k].load(g + from + k * step, n);
+        if (momentum) mr[k].load(a.m + from + k * step, n);
+      }
+    }
+    if (row0 == 0 && col0 == 0 && threadIdx.x == 0) *a.done = 0;
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      const int r = r0 + 16 * k, row = row0 + r;
       const int64_t i = static_cast<int64_t>(row) * a.cols + col;
-      const G* g = static_cast<const G*>(a.g) + i;
-      float gv[4], mv[4] = {0, 0, 0, 0}, x[4];
-      load4(g, have, vec4(g, have), gv);
-      if (momentum) load4(a.m + i, have, vec4(a.m + i, have), mv);
+      const bool there = row < a.rows;
+      float x[4], gv[4], mv[4] = {0.f, 0.f, 0.f, 0.f};
+      gr[k].get(gv);
+      if (momentum) mr[k].get(mv);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = direction(c, gv[e], mv[e], momentum) * factor;
-      if (write) store4(a.m + i, have, vec4(a.m + i, have), mv);
+      for (int e = 0; e < 4; ++e) {
+        x[e] = direction(c, gv[e], mv[e], momentum) * factor;
+        if (!there || e >= have) x[e] = 0.f;
+      }
+      if (write && there && have > 0) store4(a.m + i, have, vec4(a.m + i, have), mv);
       if (tall) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) turned[cg + e][r] = x[e];
       } else {
-        const uint32_t h0 = gemm::pack_f16(x[0], x[1]), h1 = gemm::pack_f16(x[2], x[3]);
-        const float2 a0 = gemm::unpack_f16(h0), a1 = gemm::unpack_f16(h1);
-        const int64_t to = static_cast<int64_t>(row) * a.ld + col;
-        *reinterpret_cast<uint2*>(a.hi + to) = make_uint2(h0, h1);           // rows are padded to a multiple of 8
-        *reinterpret_cast<uint2*>(a.lo + to) = make_uint2(gemm::pack_f16((x[0] - a0.x) * LO_SCALE, (x[1] - a0.y) * LO_SCALE), gemm::pack_f16((x[2] - a1.x) * LO_SCALE, (x[3] - a1.y) * LO_SCALE));
+        store_x(a, row, col, x);
       }
     }
-  }
-  if (!tall) return;
-  __syncthreads();
+    if (tall) {
+      __syncthreads();
 #pragma unroll
-  for (int k = 0; k < SIDE / 16; ++k) {
-    const int r = threadIdx.x / 16 + 16 * k, row = col0 + r, at = row0 + cg;       // of X
-    if (row < a.cols && at < a.rows) {
-      float x[4];
+      for (int k = 0; k < ROWS; ++k) {
+        const int r = r0 + 16 * k;
+        float x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = at + e < a.rows ? turned[r][cg + e] : 0.f;
-      const uint32_t h0 = gemm::pack_f16(x[0], x[1]), h1 = gemm::pack_f16(x[2], x[3]);
-      const float2 a0 = gemm::unpack_f16(h0), a1 = gemm::unpack_f16(h1);
-      const int64_t to = static_cast<int64_t>(row) * a.ld + at;
-      *reinterpret_cast<uint2*>(a.hi + to) = make_uint2(h0, h1);
-      *reinterpret_cast<uint2*>(a.lo + to) = make_uint2(gemm::pack_f16((x[0] - a0.x) * LO_SCALE, (x[1] - a0.y) * LO_SCALE), gemm::pack_f16((x[2] - a1.x) * LO_SCALE, (x[3] - a1.y) * LO_SCALE));
+        for (int e = 0; e < 4; ++e) x[e] = turned[r][cg + e];
+        store_x(a, col0 + r, row0 + cg, x);
+      }
+      __syncthreads();
     }
+    if (walk.next()) inv = inverse_norm(t.a[walk.k], c.eps);
   }
 }
 
@@ -329,70 +336,81 @@ __device__ __forceinline__ void store_weights(__nv_bfloat16* p, int have, const 
 }
 
 // UPDATE: the weights; else X itself, in bf16
-template <class W, bool UPDATE>
-__global__ void __launch_bounds__(256) muon_finish_kernel(const __grid_constant__ Matrices t, const Coefficients c) {
-  __shared__ double sums[NORM_THREADS / 32];
+template <class W, bool UPDATE, int N>
+__global__ void __launch_bounds__(256) muon_finish_kernel(const __grid_constant__ Matrices<N> t, const Coefficients c) {
   __shared__ float turned[SIDE][SIDE + 1];
-  int row0, col0;
-  const Matrix& a = tile_of(t, blockIdx.x, row0, col0);
+  Walk<N> walk(t);
+  const int cg = (threadIdx.x & 15) * 4, r0 = threadIdx.x / 16;
   sm100::grid_dependency_wait();
-  if (UPDATE && !usable(inverse_norm(a, c.eps, sums))) return;       // the same for all of the block
-  const bool tall = a.rows > a.cols;
-  const int cg = (threadIdx.x & 15) * 4;
-  if (tall) {
+  float inv = UPDATE && walk.more() ? inverse_norm(t.a[walk.k], c.eps) : 1.f;
+  while (walk.more()) {
+    const Matrix& a = t.a[walk.k];
+    const int row0 = walk.row0, col0 = walk.col0, col = col0 + cg, have = min(4, a.cols - col);
+    const bool tall = a.rows > a.cols;
+    W* w = static_cast<W*>(a.w);
+    if (usable(inv)) {                             // the same for all of the block
+      Raw<W> wr[ROWS];
+      uint2 q[ROWS];
+      float x[ROWS][4];
+      const int64_t from = static_cast<int64_t>(row0 + r0) * a.cols + col, step = static_cast<int64_t>(16) * a.cols;
+      const uint16_t* hi = a.hi + static_cast<int64_t>((tall ? col0 : row0) + r0) * a.ld + (tall ? row0 : col0) + cg;
+      if (UPDATE) {
+        if (row0 + SIDE <= a.rows && col0 + SIDE <= a.cols && a.cols % 4 == 0 && on_four(w)) {
 #pragma unroll
-    for (int k = 0; k < SIDE / 16; ++k) {
-      const int r = threadIdx.x / 16 + 16 * k, row = col0 + r, at = row0 + cg;
-      if (row < a.cols && at < a.rows) {
-        const uint2 q = *reinterpret_cast<const uint2*>(a.hi + static_cast<int64_t>(row) * a.ld + at);
-        const float2 x0 = gemm::unpack_f16(q.x), x1 = gemm::unpack_f16(q.y);
-        turned[cg][r] = x0.x; turned[cg + 1][r] = x0.y; turned[cg + 2][r] = x1.x; turned[cg + 3][r] = x1.y;
+          for (int k = 0; k < ROWS; ++k) wr[k].load(w + from + k * step);
+        } else {
+#pragma unroll
+          for (int k = 0; k < ROWS; ++k) wr[k].load(w + from + k * step, row0 + r0 + 16 * k < a.rows ? have : 0);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) q[k] = *reinterpret_cast<const uint2*>(hi + static_cast<int64_t>(16 * k) * a.ld);
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) {
+        const float2 x0 = gemm::unpack_f16(q[k].x), x1 = gemm::unpack_f16(q[k].y);
+        x[k][0] = x0.x; x[k][1] = x0.y; x[k][2] = x1.x; x[k][3] = x1.y;
+      }
+      if (tall) {
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) turned[cg + e][r0 + 16 * k] = x[k][e];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[k][e] = turned[r0 + 16 * k][cg + e];
+        __syncthreads();
+      }
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) {
+        const int row = row0 + r0 + 16 * k;
+        if (row < a.rows && have > 0) {
+          const int64_t i = static_cast<int64_t>(row) * a.cols + col;
+          float v[4];
+          if (UPDATE) wr[k].get(v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = UPDATE ? fmaf(-a.rate * (1.f / X_SCALE), x[k][e], v[e] * c.decay) : x[k][e] * (1.f / X_SCALE);
+          store_weights(w + i, have, v, c, a.at + i);
+        }
       }
     }
-    __syncthreads();
-  }
-  const int col = col0 + cg, have = min(4, a.cols - col);
-  if (have <= 0) return;
-#pragma unroll
-  for (int k = 0; k < SIDE / 16; ++k) {
-    const int r = threadIdx.x / 16 + 16 * k, row = row0 + r;
-    if (row >= a.rows) break;
-    float x[4];
-    if (tall) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = turned[r][cg + e];
-    } else {
-      const uint2 q = *reinterpret_cast<const uint2*>(a.hi + static_cast<int64_t>(row) * a.ld + col);
-      const float2 x0 = gemm::unpack_f16(q.x), x1 = gemm::unpack_f16(q.y);
-      x[0] = x0.x; x[1] = x0.y; x[2] = x1.x; x[3] = x1.y;
-    }
-    const int64_t i = static_cast<int64_t>(row) * a.cols + col;
-    W* to = static_cast<W*>(a.w) + i;
-    float v[4];
-    if (UPDATE) {
-      load4(to, have, vec4(to, have), v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = fmaf(-a.rate * (1.f / X_SCALE), x[e], v[e] * c.decay);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = x[e] * (1.f / X_SCALE);
-    }
-    store_weights(to, have, v, c, a.at + i);
+    if (walk.next() && UPDATE) inv = inverse_norm(t.a[walk.k], c.eps);
   }
 }
 
 // ---------------------------------------------------------------- host side
 constexpr int64_t ROUND_BYTES = int64_t(1) << 30;      // of scratch memory, unless one matrix needs more: a round of so much keeps the GPU busy for a millisecond
 
-int64_t up8(int64_t n) { return (n + 7) & ~int64_t(7); }
+int64_t up64(int64_t n) { return (n + 63) & ~int64_t(63); }
 int64_t up256(int64_t n) { return (n + 255) & ~int64_t(255); }
 struct Sizes {
-  int64_t p, q;                    // rows and columns of X
-  int64_t x() const { return p * up8(q); }
-  int64_t a() const { return p * up8(p); }
-  int64_t bytes() const { return 2 * (3 * up256(x()) + 2 * up256(a())) + 8 * NORM_PARTS; }
+  int64_t p, q;                    // rows and columns of X, padded
+  int64_t x() const { return p * q; }
+  int64_t a() const { return p * p; }
+  int64_t bytes() const { return 2 * (3 * x() + 2 * a()) + 5 * 256 + 8 * NORM_PARTS + 8; }
 };
-Sizes sizes_of(int64_t rows, int64_t cols) { return {std::min(rows, cols), std::max(rows, cols)}; }
+Sizes sizes_of(int64_t rows, int64_t cols) { return {up64(std::min(rows, cols)), up64(std::max(rows, cols))}; }
 
 // The matrices with a gradient, by shape, cut into rounds
 struct Plan {
@@ -414,108 +432,38 @@ Plan plan_of(const void* const* grads, const int64_t* rows, const int64_t* cols,
       used = 0;
     }
     used += need;
-    p.bytes = std::max(p.bytes, used);
+    p.bytes = std::max(p.bytes, used + 512);
   }
   p.rounds.push_back(p.order.size());
   return p;
 }
 
-// A batch of matrices of one shape in the scratch memory
-struct Shape {
-  int64_t p, q, batch;
-  uint16_t *hi[2], *lo, *A, *B;
-};
-
-// One product of all shapes.  phase 0: A = X X^T, 1: B = b A + c A A, 2: X
-template <class Policy, int TN, int P>
-int run_product(const std::vector<Shape>& shapes, size_t from, size_t to, int phase, int cur, double scale0, double scale1, cudaStream_t st) {
-  static thread_local Work<P> w;
-  w.problems = static_cast<int>(to - from);
-  w.scale0 = static_cast<float>(scale0); w.scale1 = static_cast<float>(scale1);
-  for (size_t i = from; i < to; ++i) {
-    const Shape& h = shapes[i];
-    Problem& p = w.p[i - from];
-    const gemm::Operand x = {h.hi[cur], up8(h.q), h.p * up8(h.q)}, low = {h.lo, x.ld, x.batch_stride}, next = {h.hi[cur ^ 1], x.ld, x.batch_stride}, A = {h.A, up8(h.p), h.p * up8(h.p)},
-                        B = {h.B, A.ld, A.batch_stride};
-    const int64_t k = phase == 0 ? h.q : h.p, N = phase == 2 ? h.q : h.p;
-    p.partial = nullptr;
-    p.M = static_cast<int>(h.p); p.N = static_cast<int>(N);
-    p.symmetric = phase < 2;
-    p.batch = static_cast<int>(h.batch);
-    p.splits = 1;
-    p.steps0 = p.steps = static_cast<int>(gemm::steps_of(k));
-    int rc = gemm::map_a<Policy, TN>(&p.a[0], phase == 0 ? x : phase == 1 ? A : B, h.p, k, h.batch);
-    rc = rc ? rc : gemm::map_b<Policy, TN>(&p.b[0], phase == 1 ? A : x, N, k, h.batch);
-    rc = rc ? rc : gemm::map_result<Policy>(&p.out[0], phase == 0 ? A : phase == 1 ? B : next, h.p, N, h.batch);
-    if (phase == 1) rc = rc ? rc : gemm::map_result<Policy>(&p.in[0], A, h.p, N, h.batch);
-    if (phase == 2) {
-      rc = rc ? rc : gemm::map_result<Policy>(&p.in[0], x, h.p, N, h.batch);
-      rc = rc ? rc : gemm::map_result<Policy>(&p.in[1], low, h.p, N, h.batch);
-      p.out[1] = p.in[1];
-    }
-    if (rc) return rc;
+// f(table, blocks of squares, elementwise tiles) for the matrices, as many at a time as a launch's parameters hold
+template <int N, class F>
+int with_table(const std::vector<Matrix>& all, size_t from, F&& f) {
+  static thread_local Matrices<N> t;
+  t.n = static_cast<int>(std::min<size_t>(N, all.size() - from));
+  int64_t parts = 0, tiles = 0;
+  for (int k = 0; k < t.n; ++k) {
+    const Matrix& a = t.a[k] = all[from + k];
+    t.first_part[k] = static_cast<int>(parts);
+    t.first_tile[k] = static_cast<int>(tiles);
+    parts += a.nparts;
+    tiles += static_cast<int64_t>((a.rows + SIDE - 1) / SIDE) * ((a.cols + SIDE - 1) / SIDE);
+    if (tiles > 0x7FFFFFFF) return fail(HASTE_ERR_TOO_LARGE, "matrices of too many elements for one call");
   }
-  return gemm::launch<Policy, TN>(w, true, st);
+  t.first_part[t.n] = static_cast<int>(parts); t.first_tile[t.n] = static_cast<int>(tiles);
+  // the elementwise launches' blocks share the tiles: as many as run at once
+  return f(t, std::integral_constant<int, N>(), static_cast<unsigned>(parts), static_cast<unsigned>(imin64(tiles, static_cast<int64_t>(sm_count()) * 6)));
 }
-
-// What X is rounded to after the last but two steps is amplified by two steps at most (12 times), which leaves 2^-12 of its values where the products' own roundings
-// are: its lower part is kept up to there.
-constexpr int STEPS_WITHOUT_LOWER = 2;
-
-template <int P>
-int run_steps(const std::vector<Shape>& shapes, size_t from, size_t to, int steps, double a, double b, double c, cudaStream_t st) {
-  double wide[2] = {}, narrow[2] = {};               // of the symmetric products and of the last one
-  int64_t tiles[2][2] = {}, work[2] = {};
-  for (size_t i = from; i < to; ++i)
-    for (int k = 0; k < 2; ++k) {
-      const Shape& h = shapes[i];
-      const int64_t N = k ? h.q : h.p;
-      for (int n = 0; n < 2; ++n) tiles[k][n] += h.batch * gemm::tiles_for(h.p, N, n ? 64 : 256);
-      work[k] += h.batch * gemm::tiles_for(h.p, N, 256) * gemm::steps_of(h.p);
-    }
-  for (int k = 0; k < 2; ++k) {
-    const int64_t per = (work[k] + tiles[k][0] - 1) / tiles[k][0];          // steps of a tile, on average
-    wide[k] = gemm::cost_of(k ? tiles[k][0] : (tiles[k][0] + 1) / 2, per, false);
-    narrow[k] = gemm::cost_of(k ? tiles[k][1] : (tiles[k][1] + 1) / 2, per, true);
-  }
-  const bool n0 = narrow[0] < wide[0], n1 = narrow[1] < wide[1];
-  for (int s = 0; s < steps; ++s) {
-    const int cur = s & 1;
-    const double gram = 1.0 / (X_SCALE * X_SCALE);
-    int rc = n0 ? run_product<Gram, 64, P>(shapes, from, to, 0, cur, gram, 0, st) : run_product<Gram, 256, P>(shapes, from, to, 0, cur, gram, 0, st);
-    if (rc) return rc;
-    rc = n0 ? run_product<Polynomial, 64, P>(shapes, from, to, 1, cur, b, c, st) : run_product<Polynomial, 256, P>(shapes, from, to, 1, cur, b, c, st);
-    if (rc) return rc;
-    const int left = steps - STEPS_WITHOUT_LOWER - s;
-    if (left > 1) rc = n1 ? run_product<Apply<2>, 64, P>(shapes, from, to, 2, cur, a, 0, st) : run_product<Apply<2>, 256, P>(shapes, from, to, 2, cur, a, 0, st);
-    else if (left == 1 || s == 0) rc = n1 ? run_product<Apply<1>, 64, P>(shapes, from, to, 2, cur, a, 0, st) : run_product<Apply<1>, 256, P>(shapes, from, to, 2, cur, a, 0, st);
-    else rc = n1 ? run_product<Apply<0>, 64, P>(shapes, from, to, 2, cur, a, 0, st) : run_product<Apply<0>, 256, P>(shapes, from, to, 2, cur, a, 0, st);
-    if (rc) return rc;
-  }
-  return HASTE_OK;
-}
-
 template <class F>
 int for_each_table(const std::vector<Matrix>& all, F&& f) {
-  for (size_t i = 0; i < all.size(); i += TABLE) {
-    static thread_local Matrices t;
-    t.n = static_cast<int>(std::min<size_t>(TABLE, all.size() - i));
-    int64_t parts = 0, tiles = 0;
-    for (int k = 0; k < t.n; ++k) {
-      t.a[k] = all[i + k];
-      t.a[k].first_part = static_cast<int>(parts);
-      t.a[k].first_tile = static_cast<int>(tiles);
-      parts += t.a[k].nparts;
-      tiles += static_cast<int64_t>((t.a[k].rows + SIDE - 1) / SIDE) * ((t.a[k].cols + SIDE - 1) / SIDE);
-      if (tiles > 0x7FFFFFFF) return fail(HASTE_ERR_TOO_LARGE, "matrices of too many elements for one call");
-    }
-    t.parts = static_cast<int>(parts); t.tiles = static_cast<int>(tiles);
-    if (int rc = f(t)) return rc;
+  for (size_t i = 0; i < all.size(); i += MANY) {
+    const int rc = all.size() - i <= FEW ? with_table<FEW>(all, i, f) : with_table<MANY>(all, i, f);
+    if (rc) return rc;
   }
   return HASTE_OK;
 }
-
-constexpr int FEW_SHAPES = 4, MANY_SHAPES = 24;
 
 }  // namespace
 
@@ -539,53 +487,61 @@ int launch_muon(const MuonCall& c, cudaStream_t st) {
   for (size_t r = 0; r + 1 < plan.rounds.size(); ++r) {
     char* mem = static_cast<char*>(c.scratch);
     auto take = [&](int64_t bytes) { char* p = mem; mem += up256(bytes); return p; };
+    const int64_t n = static_cast<int64_t>(plan.rounds[r + 1] - plan.rounds[r]);
+    auto* done = reinterpret_cast<unsigned long long*>(take(8 * n));
+    auto* parts = reinterpret_cast<double*>(take(8 * NORM_PARTS * n));
+    int64_t elements = 0;
+    for (size_t i = plan.rounds[r]; i < plan.rounds[r + 1]; ++i) elements += c.rows[plan.order[i]] * c.cols[plan.order[i]];
+    // blocks of squares: 8 for every SM, shared by size
+    const int64_t each = std::max<int64_t>(NORM_ELEMENTS, elements / (static_cast<int64_t>(sm_count()) * 8));
     std::vector<Matrix> all;
-    std::vector<Shape> shapes;
+    std::vector<newton_schulz::Batch> batches;
     for (size_t i = plan.rounds[r]; i < plan.rounds[r + 1];) {
       const Sizes s = sizes_of(c.rows[plan.order[i]], c.cols[plan.order[i]]);
       size_t end = i;
       while (end < plan.rounds[r + 1] && sizes_of(c.rows[plan.order[end]], c.cols[plan.order[end]]).p == s.p && sizes_of(c.rows[plan.order[end]], c.cols[plan.order[end]]).q == s.q) ++end;
-      Shape h;
-      h.p = s.p; h.q = s.q; h.batch = static_cast<int64_t>(end - i);
-      for (uint16_t** x : {&h.hi[0], &h.hi[1], &h.lo}) *x = reinterpret_cast<uint16_t*>(take(2 * h.batch * s.x()));
-      for (uint16_t** x : {&h.A, &h.B}) *x = reinterpret_cast<uint16_t*>(take(2 * h.batch * s.a()));
+      newton_schulz::Batch h;
+      h.p = s.p; h.q = s.q; h.count = static_cast<int64_t>(end - i);
+      for (uint16_t** x : {&h.hi[0], &h.hi[1], &h.lo}) *x = reinterpret_cast<uint16_t*>(take(2 * h.count * s.x()));
+      for (uint16_t** x : {&h.A, &h.B}) *x = reinterpret_cast<uint16_t*>(take(2 * h.count * s.a()));
       for (size_t j = i; j < end; ++j) {
-        const int64_t o = plan.order[j], x = static_cast<int64_t>(j - i) * s.x();
+        const int64_t o = plan.order[j], x = static_cast<int64_t>(j - i) * s.x(), size = c.rows[o] * c.cols[o];
         Matrix m = {};
         m.g = c.grads[o]; m.w = c.params[o];
         m.m = c.momentum ? c.momentum + at[o] : nullptr;
         m.hi = h.hi[0] + x; m.lo = h.lo + x;
         m.at = at[o];
-        m.rows = static_cast<int>(c.rows[o]); m.cols = static_cast<int>(c.cols[o]); m.ld = static_cast<int>(up8(s.q));
-        m.nparts = static_cast<int>(std::min<int64_t>(NORM_PARTS, (s.p * s.q + NORM_ELEMENTS - 1) / NORM_ELEMENTS));
-        m.parts = reinterpret_cast<double*>(take(8 * NORM_PARTS));
-        m.rate = static_cast<float>(c.lr * (c.adjust == HASTE_MUON_MATCH_RMS ? 0.2 * std::sqrt(static_cast<double>(s.q))
+        m.rows = static_cast<int>(c.rows[o]); m.cols = static_cast<int>(c.cols[o]); m.ld = static_cast<int>(s.q);
+        m.nparts = static_cast<int>(std::min<int64_t>(NORM_PARTS, (size + each - 1) / each));
+        m.parts = parts + NORM_PARTS * all.size();
+        m.done = done + all.size();
+        m.rate = static_cast<float>(c.lr * (c.adjust == HASTE_MUON_MATCH_RMS ? 0.2 * std::sqrt(static_cast<double>(std::max(c.rows[o], c.cols[o])))
                                                                               : std::sqrt(std::max(1.0, static_cast<double>(c.rows[o]) / static_cast<double>(c.cols[o])))));
         all.push_back(m);
       }
-      shapes.push_back(h);
+      batches.push_back(h);
       i = end;
     }
     const bool gb = c.g_type == HASTE_BF16;
-    int rc = for_each_table(all, [&](const Matrices& t) -> int {
-      if (gb) muon_squares_kernel<__nv_bfloat16><<<t.parts, NORM_THREADS, 0, st>>>(t, k);
-      else muon_squares_kernel<float><<<t.parts, NORM_THREADS, 0, st>>>(t, k);
+    int rc = for_each_table(all, [&](const auto& t, auto size, unsigned parts, unsigned tiles) -> int {
+      constexpr int N = decltype(size)::value;
+      if (gb) muon_squares_kernel<__nv_bfloat16, N><<<parts, NORM_THREADS, 0, st>>>(t, k);
+      else muon_squares_kernel<float, N><<<parts, NORM_THREADS, 0, st>>>(t, k);
       if (int e = check_launch("muon_squares_kernel")) return e;
-      return gb ? launch_behind(muon_start_kernel<__nv_bfloat16>, t.tiles, 256, st, t, k) : launch_behind(muon_start_kernel<float>, t.tiles, 256, st, t, k);
+      return gb ? launch_behind(muon_start_kernel<__nv_bfloat16, N>, tiles, 256, st, t, k) : launch_behind(muon_start_kernel<float, N>, tiles, 256, st, t, k);
     });
     if (rc) return rc;
-    for (size_t from = 0; from < shapes.size(); from += MANY_SHAPES) {
-      const size_t to = std::min(shapes.size(), from + MANY_SHAPES);
-      rc = to - from <= FEW_SHAPES ? run_steps<FEW_SHAPES>(shapes, from, to, c.steps, c.a, c.b, c.c, st) : run_steps<MANY_SHAPES>(shapes, from, to, c.steps, c.a, c.b, c.c, st);
-      if (rc) return rc;
+    rc = newton_schulz::run(batches, done, c.steps, c.a, c.b, c.c, st);
+    if (rc) return rc;
+    if (c.steps & 1) {                 // X is in the other buffer
+      size_t k = 0;
+      for (const newton_schulz::Batch& h : batches)
+        for (int64_t j = 0; j < h.count; ++j, ++k) all[k].hi = h.hi[1] + j * h.p * h.q;
     }
-    if (c.steps & 1)                   // X is in the other buffer
-      for (Matrix& m : all)
-        for (const Shape& h : shapes)
-          if (m.hi >= h.hi[0] && m.hi < h.hi[0] + h.batch * h.p * up8(h.q)) { m.hi = h.hi[1] + (m.hi - h.hi[0]); break; }
-    rc = for_each_table(all, [&](const Matrices& t) -> int {
-      if (!c.update) return launch_behind(muon_finish_kernel<__nv_bfloat16, false>, t.tiles, 256, st, t, k);
-      return c.p_type == HASTE_BF16 ? launch_behind(muon_finish_kernel<__nv_bfloat16, true>, t.tiles, 256, st, t, k) : launch_behind(muon_finish_kernel<float, true>, t.tiles, 256, st, t, k);
+    rc = for_each_table(all, [&](const auto& t, auto size, unsigned, unsigned tiles) -> int {
+      constexpr int N = decltype(size)::value;
+      if (!c.update) return launch_behind(muon_finish_kernel<__nv_bfloat16, false, N>, tiles, 256, st, t, k);
+      return c.p_type == HASTE_BF16 ? launch_behind(muon_finish_kernel<__nv_bfloat16, true, N>, tiles, 256, st, t, k) : launch_behind(muon_finish_kernel<float, true, N>, tiles, 256, st, t, k);
     });
     if (rc) return rc;
   }

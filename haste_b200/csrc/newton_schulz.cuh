@@ -1,0 +1,588 @@
+// All Newton-Schulz steps over many matrices in one launch:  steps times  A = X X^T,  B = a I + b A + c A A,  X <- B X   (X [p, q], p and q multiples of 64)
+//
+// The three products of all steps are one list of tiles, which the pairs of CTAs take in turn.  A tile may be worked on when the matrix's product before it is complete:
+// every warp that has stored its part of a tile adds one to the matrix's counter, and who needs the result waits for the count.  The list walks the matrices in groups:
+// a group's A tiles, its B tiles, its X tiles, the next step, ..., then the next group, so that
+//   - what a tile waits for was begun by other pairs about a product earlier, and no pair idles at the end of one (a launch for each product left a quarter of the
+//     SMs without work in the last tiles of 5, and took 3 us and the first loads' latency each time);
+//   - a group is chosen to fit L2, so that only its first and last X pass through memory.
+// Every tile's predecessors stand before it in the list, and a pair works through its part of the list in order, so with all pairs resident (a cooperative launch) the first
+// unfinished tile can always proceed.  Waits are bounded as everywhere.
+//
+// A and B are symmetric: only tiles on and below the diagonal are computed and stored.  Where an operand's block lies above it, the block on the other side is loaded and
+// read by the tensor core with its rows and columns exchanged.
+//
+// Tiles are 256 x TN of a pair, with roles and barriers as in gemm_sm100.cuh; warp 3 looks up what comes next and waits for it, ahead of the others.  An epilogue warp
+// has a box for each of its columns' chunks, into which the chunk's input is loaded and from which its result is stored, and one more for X's upper part beside the lower.
+#pragma once
+#include "gemm_sm100.cuh"
+
+namespace haste {
+namespace newton_schulz {
+
+using namespace sm100;
+using gemm::EPI_WARPS;
+using gemm::KSTEP;
+using gemm::THREADS;
+using gemm::TILE;
+
+constexpr float X_SCALE = 256.f;       // X is kept times this in fp16
+constexpr float LO_SCALE = 2048.f;     // and its lower part times this as well
+// What X is rounded to after the last but two steps is amplified by two steps at most (12 times), which leaves 2^-12 of its values where the products' own roundings
+// are: its lower part is kept up to there.
+constexpr int STEPS_WITHOUT_LOWER = 2;
+__host__ __device__ constexpr bool has_lower(int step, int steps) { return step == 0 || step < steps - STEPS_WITHOUT_LOWER; }       // X before this step
+
+// Tensor maps of a batch of matrices of one shape: X's two buffers as operand a and b with k contiguous and as operand b with its rows contiguous, A and B as operand a (A's also b)
+// either way, and the epilogue's boxes of A, B, X and X's lower part.  In the wide form operands a and b are alike.
+enum Map { X_A, X_N = 2, A_A = 4, B_A, A_T, B_T, A_BOX, B_BOX, X_BOX, LO_BOX = 12, MAPS_WIDE, X_B = 13, A_B = 15, A_TB, MAPS_NARROW };
+
+struct Info {
+  int p, q, tiles_m, tiles_n, tiles_q; // tiles_n: columns' tiles of A and B, tiles_q: of X
+  int symmetric, full;                 // tiles of A or B, and of X, in a matrix
+};
+struct Segment {                       // neighbouring matrices of one shape in a group
+  int shape, batch, count, matrix;     // first batch entry, how many, number of the first matrix
+  int symmetric0, full0;               // tiles of the group before it
+};
+struct Group {
+  int first;                           // tile number
+  int segment, symmetric, full;        // first segment; tiles of a product of all of it
+};
+template <int TN>
+struct Steps {
+  static constexpr int MAPS = TN == TILE ? static_cast<int>(MAPS_WIDE) : static_cast<int>(MAPS_NARROW);
+  static constexpr int SHAPES = TN == TILE ? 16 : 12, SEGMENTS = 64, GROUPS = 32;
+  CUtensorMap map[SHAPES][MAPS];
+  Info info[SHAPES];
+  Segment segment[SEGMENTS + 1];       // the last one: the end
+  Group group[GROUPS + 1];
+  int groups, tiles, steps;
+  float a, b, c;
+  unsigned long long* done;            // by matrix
+  int* err;
+  long long wait_limit;
+};
+
+struct Task {
+  int shape, batch, matrix, m, n, phase, step;
+  unsigned long long need;             // of the matrix's counter
+};
+
+template <int TN>
+__device__ __forceinline__ Task task_at(const Steps<TN>& w, int t, int& g) {
+  constexpr int PER = TILE / TN;
+  while (g + 1 < w.groups && t >= w.group[g + 1].first) ++g;
+  const Group& gr = w.group[g];
+  Task r;
+  t -= gr.first;
+  const int per = 2 * gr.symmetric + gr.full;
+  r.step = t / per;
+  t -= r.step * per;
+  r.phase = t < gr.symmetric ? 0 : t < 2 * gr.symmetric ? 1 : 2;
+  t -= r.phase * gr.symmetric;
+  const int end = w.group[g + 1].segment;
+  int s = gr.segment;
+  while (s + 1 < end && t >= (r.phase < 2 ? w.segment[s + 1].symmetric0 : w.segment[s + 1].full0)) ++s;
+  const Segment& sg = w.segment[s];
+  const Info& info = w.info[sg.shape];
+  t -= r.phase < 2 ? sg.symmetric0 : sg.full0;
+  const int each = r.phase < 2 ? info.symmetric : info.full, i = t / each;
+  t -= i * each;
+  r.shape = sg.shape;
+  r.batch = sg.batch + i;
+  r.matrix = sg.matrix + i;
+  if (r.phase < 2) {
+    // rows of tiles grow by PER until they are as wide as the matrix
+    int m = static_cast<int>((sqrtf(8.f * static_cast<float>(t / PER) + 1.f) - 1.f) * 0.5f);
+    while (m * (m + 1) / 2 * PER > t) --m;
+    while ((m + 1) * (m + 2) / 2 * PER <= t) ++m;
+    r.m = m;
+    r.n = t - m * (m + 1) / 2 * PER;
+  } else {
+    r.n = t / info.tiles_m;
+    r.m = t - r.n * info.tiles_m;
+  }
+  const unsigned long long whole = 2ull * info.symmetric + info.full;
+  r.need = (r.step * whole + static_cast<unsigned long long>(r.phase) * info.symmetric) * (2 * EPI_WARPS);
+  return r;
+}
+
+// ---------------------------------------------------------------- counters
+__device__ __forceinline__ unsigned long long load_acquire(const unsigned long long* p) {
+  unsigned long long v;
+  asm volatile("ld.acquire.gpu.global.b64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
+// Until the count is there: what was stored before it may then be read, by copies too
+__device__ __noinline__ bool wait_count(const unsigned long long* p, unsigned long long need, volatile int* abort_flag, int* err, int code, long long limit) {
+  const long long t0 = clock64();
+  while (load_acquire(p) < need) {
+    if (*abort_flag) return false;
+    if (clock64() - t0 > limit) {
+      *abort_flag = 1;
+      if (err != nullptr) *reinterpret_cast<volatile int*>(err) = code;
+      return false;
+    }
+    __nanosleep(32);
+  }
+  fence_proxy_async_all();
+  return true;
+}
+// What this thread's stores (bulk groups) wrote, once it has waited for them, is there for whoever sees the count
+__device__ __forceinline__ void add_count_only(unsigned long long* p) {
+  fence_proxy_async_all();
+  __threadfence();
+  asm volatile("red.release.gpu.global.add.u64 [%0], %1;" ::"l"(p), "l"(1ull) : "memory");
+}
+__device__ __forceinline__ void add_count(unsigned long long* p) {
+  bulk_wait<0>();
+  add_count_only(p);
+}
+
+// ---------------------------------------------------------------- the kernel
+template <int TN>
+struct Layout {
+  static constexpr int A_BYTES = 128 * KSTEP * 2, B_BYTES = TN / 2 * KSTEP * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = TN == TILE ? 4 : 8, TASKS = 4;
+  static constexpr int BOX_COLUMNS = TN == TILE ? 64 : 32, BOX_BYTES = 32 * BOX_COLUMNS * 2, CHUNKS = TN / 2 / BOX_COLUMNS, BOXES = CHUNKS + 1;
+  static constexpr int OFF_EPI = STAGES * STAGE_BYTES;
+  static constexpr int OFF_TASK = OFF_EPI + EPI_WARPS * BOXES * BOX_BYTES;
+  static constexpr int OFF_BAR = OFF_TASK + TASKS * 64;
+  static constexpr int BARRIERS = 2 * STAGES + 4 + 2 * TASKS + EPI_WARPS * CHUNKS;
+  static constexpr int SMEM_BYTES = OFF_BAR + 8 * BARRIERS + 16 + 1024;
+  static_assert(SMEM_BYTES <= 227 * 1024 && sizeof(Task) <= 64, "shared memory");
+};
+// Where 16-byte piece j of row r of a box lies
+template <int TN>
+__device__ __forceinline__ uint32_t piece(uint32_t box, int r, int j) {
+  return TN == TILE ? box + r * 128 + ((j ^ (r & 7)) << 4) : box + r * 64 + ((j ^ ((r >> 1) & 3)) << 4);
+}
+__device__ __forceinline__ void load_piece(uint32_t at, uint32_t* p) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(p[0]), "=r"(p[1]), "=r"(p[2]), "=r"(p[3]) : "r"(at) : "memory");
+}
+
+template <int TN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) newton_schulz_kernel(const __grid_constant__ Steps<TN> w) {
+  using L = Layout<TN>;
+  constexpr int STAGES = L::STAGES, TASKS = L::TASKS;
+  constexpr bool WIDE = TN == TILE;
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t base = smem_u32(sm);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = gemm::cta_rank();
+  auto bar_full = [&](int s) { return base + L::OFF_BAR + 8 * s; };
+  auto bar_empty = [&](int s) { return base + L::OFF_BAR + 8 * (STAGES + s); };
+  auto bar_done = [&](int s) { return base + L::OFF_BAR + 8 * (2 * STAGES + s); };
+  auto bar_free = [&](int s) { return base + L::OFF_BAR + 8 * (2 * STAGES + 2 + s); };
+  auto bar_task = [&](int s) { return base + L::OFF_BAR + 8 * (2 * STAGES + 4 + s); };
+  auto bar_slot = [&](int s) { return base + L::OFF_BAR + 8 * (2 * STAGES + 4 + TASKS + s); };
+  const uint32_t bar_in = base + L::OFF_BAR + 8 * (2 * STAGES + 4 + 2 * TASKS);
+  auto slot_of = [&](int n) -> volatile Task& { return *reinterpret_cast<volatile Task*>(sm + L::OFF_TASK + (n % TASKS) * 64); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + L::OFF_BAR + 8 * L::BARRIERS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::OFF_BAR + 8 * L::BARRIERS + 8);
+  const long long WL = w.wait_limit;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(bar_done(s), 1); mbar_init(bar_free(s), 2 * EPI_WARPS); }
+    // read by the warps for loads, products (in the even CTA) and the epilogue
+    for (int s = 0; s < TASKS; ++s) { mbar_init(bar_task(s), 1); mbar_init(bar_slot(s), EPI_WARPS + (rank == 0 ? 2 : 1)); }
+    for (int s = 0; s < EPI_WARPS * L::CHUNKS; ++s) mbar_init(bar_in + 8 * s, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 2) gemm::tmem_alloc_pair(smem_u32(tmem_slot), 2 * TN);
+  tc_fence_before();
+  __syncthreads();
+  gemm::cluster_sync_all();          // the other CTA's barriers are there, and it has started
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+  const int mine = w.tiles > first ? (w.tiles - first + stride - 1) / stride : 0;          // tiles of this pair
+  // The n-th of them, when it may be worked on; by one thread, or by a warp with every = true
+  auto take = [&](int n, bool every, Task& k) -> bool {
+    bool ok = mbar_wait(bar_task(n % TASKS), (n / TASKS) & 1, abort_flag, w.err, 329, WL);
+    if (every) ok = __all_sync(0xffffffffu, ok);
+    if (!ok) return false;
+    volatile Task& s = slot_of(n);
+    k.shape = s.shape; k.batch = s.batch; k.matrix = s.matrix; k.m = s.m; k.n = s.n; k.phase = s.phase; k.step = s.step;
+    if (every) __syncwarp();
+    if (!every || lane == 0) mbar_arrive(bar_slot(n % TASKS));
+    return true;
+  };
+  // Whether block kc of k lies above the diagonal for an operand's rows
+  auto above = [](int kc, int row) { return kc / TILE > row / TILE; };
+
+  if (warp == 3 && lane == 0) {
+    // ---------------- what comes next
+    int g = 0;
+    for (int n = 0; n < mine; ++n) {
+      const Task k = task_at(w, first + n * stride, g);
+      if (!mbar_wait(bar_slot(n % TASKS), ((n / TASKS) & 1) ^ 1, abort_flag, w.err, 320, WL)) break;
+      if (!wait_count(w.done + k.matrix, k.need, abort_flag, w.err, 321, WL)) break;
+      volatile Task& s = slot_of(n);
+      s.shape = k.shape; s.batch = k.batch; s.matrix = k.matrix; s.m = k.m; s.n = k.n; s.phase = k.phase; s.step = k.step;
+      mbar_arrive(bar_task(n % TASKS));
+    }
+  } else if (warp == 0 && lane == 0) {
+    // ---------------- loads
+    int it = 0;
+    Task k;
+    for (int n = 0; n < mine && take(n, false, k); ++n) {
+      fence_proxy_async_all();
+      const Info& info = w.info[k.shape];
+      const int cur = k.step & 1, steps = (k.phase == 0 ? info.q : info.p) / KSTEP;
+      const CUtensorMap* maps = w.map[k.shape];
+      const CUtensorMap* ta = maps + (k.phase == 0 ? X_A + cur : k.phase == 1 ? A_A : B_A);
+      const CUtensorMap* tat = maps + (k.phase == 1 ? A_T : B_T);
+      const CUtensorMap* tb = maps + (k.phase == 0 ? (WIDE ? X_A : X_B) + cur : k.phase == 1 ? (WIDE ? A_A : A_B) : X_N + cur);
+      const CUtensorMap* tbt = k.phase == 1 ? maps + (WIDE ? A_T : A_TB) : tb;
+      const int am = k.m * TILE + static_cast<int>(rank) * 128, bn = k.n * TN + static_cast<int>(rank) * (TN / 2);
+      for (int i = 0; i < steps; ++i, ++it) {
+        const int s = it % STAGES, kc = i * KSTEP;
+        if (!mbar_wait(bar_empty(s), ((it / STAGES) & 1) ^ 1, abort_flag, w.err, 322, WL)) break;
+        if (rank == 0) mbar_arrive_expect_tx(bar_full(s), 2 * L::STAGE_BYTES);
+        const uint32_t bar = gemm::leaders(bar_full(s)), as = base + s * L::STAGE_BYTES, bs = as + L::A_BYTES;
+        if (k.phase > 0 && above(kc, am)) {
+          gemm::tma_load_pair(as, tat, am, kc, k.batch, bar);
+          gemm::tma_load_pair(as + L::A_BYTES / 2, tat, am + 64, kc, k.batch, bar);
+        } else {
+          gemm::tma_load_pair(as, ta, kc, am, k.batch, bar);
+        }
+        if (k.phase == 2 || (k.phase == 1 && above(kc, bn))) {
+          gemm::tma_load_pair(bs, tbt, bn, kc, k.batch, bar);
+          if (WIDE) gemm::tma_load_pair(bs + L::B_BYTES / 2, tbt, bn + 64, kc, k.batch, bar);
+        } else {
+          gemm::tma_load_pair(bs, tb, kc, bn, k.batch, bar);
+        }
+      }
+      if (*abort_flag) break;
+    }
+    for (int i = it > STAGES ? it - STAGES : 0; i < it; ++i) mbar_wait(bar_empty(i % STAGES), (i / STAGES) & 1, abort_flag, w.err, 323, WL);
+  } else if (warp == 1 && rank == 0) {
+    // ---------------- products
+    constexpr uint32_t IDESC = (1u << 4) | (static_cast<uint32_t>(TN >> 3) << 17) | (static_cast<uint32_t>(TILE >> 4) << 24);
+    const uint64_t da = make_sdesc(base, 16, 1024), dat = make_sdesc(base, L::A_BYTES / 2, 1024);
+    const uint64_t db = make_sdesc(base + L::A_BYTES, 16, 1024), dbt = WIDE ? make_sdesc(base + L::A_BYTES, L::B_BYTES / 2, 1024) : make_sdesc64(base + L::A_BYTES, 16, 512);
+    constexpr uint32_t KBT = WIDE ? 2048 >> 4 : 1024 >> 4;
+    int it = 0;
+    Task k;
+    for (int n = 0; n < mine && take(n, true, k); ++n) {
+      const Info& info = w.info[k.shape];
+      const int buf = n & 1, steps = (k.phase == 0 ? info.q : info.p) / KSTEP, am = k.m * TILE, bn = k.n * TN;
+      if (!mbar_wait(bar_free(buf), ((n >> 1) & 1) ^ 1, abort_flag, w.err, 324, WL)) break;
+      tc_fence_after();
+      bool ok = true;
+      for (int i = 0; i < steps; ++i, ++it) {
+        const int s = it % STAGES;
+        ok = mbar_wait(bar_full(s), (it / STAGES) & 1, abort_flag, w.err, 325, WL);
+        if (!ok) break;
+        tc_fence_after();
+        const bool at = k.phase > 0 && above(i * KSTEP, am), bt = k.phase == 2 || (k.phase == 1 && above(i * KSTEP, bn));
+        const uint64_t off = static_cast<uint64_t>((s * L::STAGE_BYTES) >> 4), a = (at ? dat : da) + off, b = (bt ? dbt : db) + off;
+        const uint32_t ka = at ? 2048 >> 4 : 32 >> 4, kb = bt ? KBT : 32 >> 4, idesc = IDESC | (static_cast<uint32_t>(at) << 15) | (static_cast<uint32_t>(bt) << 16);
+        if (elect_one()) {
+#pragma unroll
+          for (int j = 0; j < KSTEP / 16; ++j) gemm::umma_pair(tmem + buf * TN, a + j * ka, b + j * kb, idesc, (i | j) != 0);
+          gemm::commit_pair(bar_empty(s));
+        }
+        __syncwarp();
+      }
+      if (!ok) break;
+      if (elect_one()) gemm::commit_pair(bar_done(buf));
+      __syncwarp();
+    }
+  } else if (warp >= 4) {
+    // ---------------- epilogue
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t boxes = base + L::OFF_EPI + static_cast<uint32_t>(warp - 4) * L::BOXES * L::BOX_BYTES, second = boxes + L::CHUNKS * L::BOX_BYTES;
+    const uint32_t bars = bar_in + 8 * L::CHUNKS * (warp - 4);
+    unsigned long long* pending = nullptr;             // counter of the tile before, whose stores may be on their way
+    int inputs = 0;                                    // tiles with input so far
+    auto flush = [&] {
+      if (pending != nullptr && lane == 0) add_count(pending);
+      pending = nullptr;
+    };
+    Task k;
+    for (int n = 0; n < mine; ++n) {
+      // nobody may wait for this warp's last tile while it waits itself
+      if (!mbar_test(bar_task(n % TASKS), (n / TASKS) & 1)) flush();
+      if (!take(n, true, k)) break;
+      const CUtensorMap* maps = w.map[k.shape];
+      const Info& info = w.info[k.shape];
+      const int buf = n & 1, cur = k.step & 1, row0 = k.m * TILE + static_cast<int>(rank) * 128 + quarter * 32, col0 = k.n * TN + half * (TN / 2);
+      const int N = k.phase == 2 ? info.q : info.p;
+      const bool low = k.phase == 2 && has_lower(k.step, w.steps), more = k.phase == 2 && has_lower(k.step + 1, w.steps), input = k.phase == 1 || low;
+      if (lane == 0) bulk_wait_read<0>();              // the boxes are free
+      __syncwarp();
+      if (input && lane == 0) {
+        fence_proxy_async_all();
+#pragma unroll
+        for (int j = 0; j < L::CHUNKS; ++j) {
+          mbar_arrive_expect_tx(bars + 8 * j, L::BOX_BYTES);
+          gemm::tma_load_3d(boxes + j * L::BOX_BYTES, maps + (k.phase == 1 ? A_BOX : LO_BOX), col0 + j * L::BOX_COLUMNS, row0, k.batch, bars + 8 * j);
+        }
+      }
+      if (!mbar_test(bar_done(buf), (n >> 1) & 1)) flush();
+      bool ok = mbar_wait(bar_done(buf), (n >> 1) & 1, abort_flag, w.err, 327, WL);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll 1
+      for (int j = 0; j < L::CHUNKS; ++j) {
+        const int col = col0 + j * L::BOX_COLUMNS;
+        const bool inside = row0 < info.p && col < N;
+        const uint32_t box = boxes + j * L::BOX_BYTES;
+        if (input) {
+          ok = __all_sync(0xffffffffu, mbar_wait(bars + 8 * j, inputs & 1, abort_flag, w.err, 328, WL));
+          if (!ok) break;
+        }
+        if (more && j > 0) {
+          if (lane == 0) bulk_wait_read<1>();          // the chunk before has left the second box
+          __syncwarp();
+        }
+#pragma unroll
+        for (int h = 0; h < L::BOX_COLUMNS / 32; ++h) {
+          uint32_t v[32], e[16], hi[16];
+          tmem_ld32(tmem + buf * TN + (static_cast<uint32_t>(quarter * 32) << 16) + half * (TN / 2) + j * L::BOX_COLUMNS + 32 * h, v);
+          if (input) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) load_piece(piece<TN>(box, lane, 4 * h + q), e + 4 * q);
+          }
+          tmem_ld_wait();
+          if (k.phase == 0) {
+            constexpr float SCALE = 1.f / (X_SCALE * X_SCALE);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) hi[i] = gemm::pack_f16(__uint_as_float(v[2 * i]) * SCALE, __uint_as_float(v[2 * i + 1]) * SCALE);
+          } else if (k.phase == 1) {
+            const int own = row0 + lane - col - 32 * h;    // where the diagonal is in this row
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 a = gemm::unpack_f16(e[i]);
+              float x = fmaf(w.c, __uint_as_float(v[2 * i]), w.b * a.x), y = fmaf(w.c, __uint_as_float(v[2 * i + 1]), w.b * a.y);
+              if (2 * i == own) x += w.a;
+              if (2 * i + 1 == own) y += w.a;
+              hi[i] = gemm::pack_f16(x, y);
+            }
+          } else {
+            const float scale = w.a * (1.f / LO_SCALE);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float x = __uint_as_float(v[2 * i]), y = __uint_as_float(v[2 * i + 1]);
+              if (low) {
+                const float2 l = gemm::unpack_f16(e[i]);
+                x = fmaf(scale, l.x, x);
+                y = fmaf(scale, l.y, y);
+              }
+              hi[i] = gemm::pack_f16(x, y);
+              if (more) {
+                const float2 r = gemm::unpack_f16(hi[i]);
+                e[i] = gemm::pack_f16((x - r.x) * LO_SCALE, (y - r.y) * LO_SCALE);
+              }
+            }
+          }
+          const uint32_t to = more ? second : box;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) gemm::st_shared_v4(piece<TN>(to, lane, 4 * h + q), hi[4 * q], hi[4 * q + 1], hi[4 * q + 2], hi[4 * q + 3]);
+          if (more) {                                  // in the place of what it was made of
+#pragma unroll
+            for (int q = 0; q < 4; ++q) gemm::st_shared_v4(piece<TN>(box, lane, 4 * h + q), e[4 * q], e[4 * q + 1], e[4 * q + 2], e[4 * q + 3]);
+          }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {                               // two groups for every chunk, whatever is in them
+          if (inside) gemm::tma_store_3d(maps + (k.phase == 0 ? A_BOX : k.phase == 1 ? B_BOX : X_BOX + (cur ^ 1)), more ? second : box, col, row0, k.batch);
+          bulk_commit();
+          if (inside && more) gemm::tma_store_3d(maps + LO_BOX, box, col, row0, k.batch);      // the tile's own place, which it has read
+          bulk_commit();
+          if (j == 0 && pending != nullptr) {          // the tile before: all but this chunk's groups
+            bulk_wait<2>();
+            add_count_only(pending);
+          }
+        }
+        if (j == 0) pending = nullptr;
+      }
+      if (!ok) break;
+      if (input) ++inputs;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) gemm::arrive_at_leader(bar_free(buf));
+      pending = w.done + k.matrix;
+    }
+    flush();
+    if (lane == 0) bulk_wait<0>();
+    __syncwarp();
+  }
+
+  // ---------------- teardown, as in gemm_sm100.cuh
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < (1ll << 24)) __nanosleep(1000);
+  }
+  gemm::cluster_sync_all();
+  tc_fence_after();
+  if (warp == 2) gemm::tmem_dealloc_pair(tmem, 2 * TN);
+}
+
+// ---------------------------------------------------------------- host side
+// A batch of matrices of one shape: X [batch][p][q] in two buffers and its lower part, A and B [batch][p][p]
+struct Batch {
+  int64_t p, q, count;
+  uint16_t *hi[2], *lo, *A, *B;
+};
+#ifndef X_GROUP
+#define X_GROUP 250
+#endif
+constexpr int64_t GROUP_BYTES = int64_t(X_GROUP) << 20;
+
+inline int64_t bytes_of(const Batch& b) { return 2 * (3 * b.p * b.q + 2 * b.p * b.p); }
+
+template <int TN>
+int set_shape(Steps<TN>& w, int i, const Batch& b) {
+  using gemm::make_map;
+  Info& f = w.info[i];
+  f.p = static_cast<int>(b.p); f.q = static_cast<int>(b.q);
+  f.tiles_m = (f.p + TILE - 1) / TILE; f.tiles_n = (f.p + TN - 1) / TN; f.tiles_q = (f.q + TN - 1) / TN;
+  f.symmetric = 0;
+  for (int m = 0; m < f.tiles_m; ++m) f.symmetric += std::min((m + 1) * (TILE / TN), f.tiles_n);
+  f.full = f.tiles_m * f.tiles_q;
+  CUtensorMap* m = w.map[i];
+  const int64_t n = b.count;
+  int rc = 0;
+  auto map = [&](int at, const void* base, int64_t inner, int box_inner, int box_outer) {
+    if (rc == 0) rc = make_map(&m[at], base, true, inner, b.p, n, inner, 0, box_inner, box_outer);
+  };
+  for (int k = 0; k < 2; ++k) {
+    map(X_A + k, b.hi[k], b.q, 64, 128);
+    map(X_N + k, b.hi[k], b.q, TN == TILE ? 64 : 32, 64);
+    map(X_BOX + k, b.hi[k], b.q, Layout<TN>::BOX_COLUMNS, 32);
+    if (TN != TILE) map(X_B + k, b.hi[k], b.q, 64, TN / 2);
+  }
+  map(A_A, b.A, b.p, 64, 128);
+  map(B_A, b.B, b.p, 64, 128);
+  map(A_T, b.A, b.p, 64, 64);
+  map(B_T, b.B, b.p, 64, 64);
+  map(A_BOX, b.A, b.p, Layout<TN>::BOX_COLUMNS, 32);
+  map(B_BOX, b.B, b.p, Layout<TN>::BOX_COLUMNS, 32);
+  map(LO_BOX, b.lo, b.q, Layout<TN>::BOX_COLUMNS, 32);
+  if (TN != TILE) {
+    map(A_B, b.A, b.p, 64, TN / 2);
+    map(A_TB, b.A, b.p, 32, 64);
+  }
+  return rc;
+}
+
+// The steps for batches [from, to), as many as a launch's parameters hold; `from` moves on.  done: a counter for every matrix from the first one of batches[from] on, zeros.
+template <int TN>
+int launch(const std::vector<Batch>& batches, size_t& from, int64_t& start, unsigned long long*& done, int steps, double a, double b, double c, cudaStream_t st) {
+  using S = Steps<TN>;
+  static thread_local S w;
+  // groups of about one size
+  int64_t total = 0;
+  for (size_t i = from; i < batches.size(); ++i) total += bytes_of(batches[i]) * (batches[i].count - (i == from ? start : 0));
+  const int64_t want = std::max<int64_t>(1, (total + GROUP_BYTES - 1) / GROUP_BYTES), limit = (total + want - 1) / want;
+  int shapes = 0, segments = 0, groups = 0, matrices = 0;
+  int64_t tiles = 0, used = 0;
+  bool open = false;
+  auto close = [&] {
+    Group& gr = w.group[groups];
+    tiles += static_cast<int64_t>(steps) * (2ll * gr.symmetric + gr.full);
+    ++groups;
+    open = false;
+  };
+  while (from < batches.size() && shapes < S::SHAPES && groups < S::GROUPS && segments < S::SEGMENTS) {
+    const Batch& x = batches[from];
+    if (int rc = set_shape(w, shapes, x)) return rc;
+    const Info& f = w.info[shapes];
+    bool full = false;
+    while (start < x.count) {
+      if (groups >= S::GROUPS || segments >= S::SEGMENTS) { full = true; break; }
+      if (!open) {
+        w.group[groups] = {static_cast<int>(tiles), segments, 0, 0};
+        used = 0;
+        open = true;
+      }
+      Group& gr = w.group[groups];
+      const int64_t room = std::max<int64_t>(1, (limit - used + bytes_of(x) / 2) / bytes_of(x)), k = std::min(x.count - start, room);
+      const int64_t in_group = static_cast<int64_t>(steps) * (2 * (gr.symmetric + k * f.symmetric) + gr.full + k * f.full);
+      if (tiles + in_group > 0x3FFFFFFF) {
+        if (segments == 0) return fail(HASTE_ERR_TOO_LARGE, "matrices of too many tiles for one launch");
+        full = true;
+        break;
+      }
+      w.segment[segments++] = {shapes, static_cast<int>(start), static_cast<int>(k), matrices, gr.symmetric, gr.full};
+      gr.symmetric += static_cast<int>(k * f.symmetric);
+      gr.full += static_cast<int>(k * f.full);
+      used += k * bytes_of(x);
+      matrices += static_cast<int>(k);
+      start += k;
+      if (used + bytes_of(x) / 2 > limit) close();
+    }
+    ++shapes;
+    if (full) break;
+    ++from;
+    start = 0;
+  }
+  if (open) {
+    if (w.group[groups].symmetric > 0) close();
+  }
+  w.group[groups] = {static_cast<int>(tiles), segments, 0, 0};
+  w.groups = groups;
+  w.tiles = static_cast<int>(tiles);
+  w.steps = steps;
+  w.a = static_cast<float>(a); w.b = static_cast<float>(b); w.c = static_cast<float>(c);
+  w.done = done;
+  done += matrices;
+  if (tiles == 0) return HASTE_OK;
+  if (int rc = device_status_word(&w.err)) return rc;
+  w.wait_limit = wait_limit_cycles();
+  auto kernel = newton_schulz_kernel<TN>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<TN>::SMEM_BYTES);
+  if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  const int pairs = static_cast<int>(imin64(gemm::pairs_resident(kernel, Layout<TN>::SMEM_BYTES), tiles));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = Layout<TN>::SMEM_BYTES;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeCooperative;          // its blocks wait for each other
+  attr.val.cooperative = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, w);
+  if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaLaunchKernelEx: %s", cudaGetErrorString(e));
+  return HASTE_OK;
+}
+
+// The wide form, or the narrow one where wide tiles would leave pairs without work: a product's time in either, over the matrices that are worked on together
+inline bool take_narrow(const std::vector<Batch>& batches) {
+  int64_t total = 0, tiles[2] = {}, work = 0;
+  for (const Batch& b : batches) {
+    total += bytes_of(b) * b.count;
+    for (int n = 0; n < 2; ++n) tiles[n] += b.count * gemm::tiles_for(b.p, b.q, n ? 64 : TILE);
+    work += b.count * gemm::tiles_for(b.p, b.q, TILE) * gemm::steps_of(b.p);
+  }
+  const int64_t groups = std::max<int64_t>(1, (total + GROUP_BYTES - 1) / GROUP_BYTES), per = (work + tiles[0] - 1) / tiles[0];
+  return gemm::cost_of(tiles[1] / groups, per, true) < gemm::cost_of(tiles[0] / groups, per, false);
+}
+
+inline int run(const std::vector<Batch>& batches, unsigned long long* done, int steps, double a, double b, double c, cudaStream_t st) {
+  const bool narrow = take_narrow(batches);
+  size_t from = 0;
+  int64_t start = 0;
+  while (from < batches.size()) {
+    if (int rc = narrow ? launch<64>(batches, from, start, done, steps, a, b, c, st) : launch<TILE>(batches, from, start, done, steps, a, b, c, st)) return rc;
+  }
+  return HASTE_OK;
+}
+
+}  // namespace newton_schulz
+}  // namespace haste

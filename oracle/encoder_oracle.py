@@ -120,18 +120,19 @@ def orthogonalize(g, steps=5, coefficients=(A, B, C), eps=1e-7):
 
 
 def orthogonalize_rounded(g, steps=5, coefficients=(A, B, C), eps=1e-7):
-    """The same with the kernels' roundings and no others: products take X (times 256), A and B in fp16, the term a X takes 22 bits of X in the
-    first step and up to the last but two, 11 behind it."""
+    """The same with the kernels' roundings and no others: products take X (times 256), A and B = a I + b A + c A^2 in fp16; X has 11 more bits, which a
+    alone multiplies, in the first step and up to the last but two."""
     a, b, c = coefficients
     f16 = lambda v: v.to(torch.float16).double()
     tall = g.shape[0] > g.shape[1]
     x = g.double()
     x = (x.t() if tall else x) / max(float(x.norm()), eps) * 256
+    eye = torch.eye(x.shape[0], dtype=torch.float64, device=x.device)
     for k in range(steps):
         hi = f16(x)
-        x = hi + f16((x - hi) * 2048) / 2048 if k == 0 or k < steps - 2 else hi
+        low = f16((x - hi) * 2048) / 2048 if k == 0 or k < steps - 2 else torch.zeros_like(x)
         s = f16(hi @ hi.t() / 65536)
-        x = a * x + f16(b * s + c * (s @ s)) @ hi
+        x = f16(a * eye + b * s + c * (s @ s)) @ hi + a * low
     x = f16(x) / 256
     return x.t() if tall else x
 
