@@ -57,33 +57,26 @@ template <int ACT>
 struct GatedForward {
   static constexpr bool A_MN = false, B_MN = false, F16 = false, PAIRED_B = true;
   static constexpr int PARTS = 1, OUTPUTS = 3, INPUTS = 0;
-  template <class W, class I, class S>
-  static __device__ __forceinline__ void chunk(const W& w, const gemm::Problem<GatedForward>& p, const Tile& t, int row0, int col, uint32_t tmem, I&, S& st, int lane) {
-    constexpr int OTHER = I::L::COLUMNS;             // up's accumulator stands behind gate's
-    const bool inside = row0 < p.M && col < p.N;
+  template <int TN, class W, class I>
+  static __device__ __forceinline__ void chunk(const W& w, const gemm::Problem<GatedForward>& p, const Tile&, int row, int col, uint32_t tmem, I&) {
     uint32_t g[32], u[32], packed[16];
     sm100::tmem_ld32(tmem, g);
-    sm100::tmem_ld32(tmem + OTHER, u);
+    sm100::tmem_ld32(tmem + TN / 2, u);              // up's accumulator stands behind gate's
     sm100::tmem_ld_wait();
+    if (row >= p.M) return;
     if (w.scale0 != 0.f) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) packed[i] = gemm::pack_bf16(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
-      uint32_t box = st.get();
-      gemm::box_row(box, lane, packed);
-      st.put(&p.out[0], box, col, row0, 0, inside);
+      gemm::store_row(p.out[0], row, col, packed);
 #pragma unroll
       for (int i = 0; i < 16; ++i) packed[i] = gemm::pack_bf16(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
-      box = st.get();
-      gemm::box_row(box, lane, packed);
-      st.put(&p.out[1], box, col, row0, 0, inside);
+      gemm::store_row(p.out[1], row, col, packed);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       packed[i] = gemm::pack_bf16(activate<ACT>(__uint_as_float(g[2 * i])) * __uint_as_float(u[2 * i]),
                                   activate<ACT>(__uint_as_float(g[2 * i + 1])) * __uint_as_float(u[2 * i + 1]));
-    const uint32_t box = st.get();
-    gemm::box_row(box, lane, packed);
-    st.put(&p.out[2], box, col, row0, 0, inside);
+    gemm::store_row(p.out[2], row, col, packed);
   }
 };
 
@@ -92,35 +85,26 @@ template <int ACT>
 struct GatedBackward {
   static constexpr bool A_MN = false, B_MN = true, F16 = false, PAIRED_B = false;
   static constexpr int PARTS = 1, OUTPUTS = 3, INPUTS = 2;
-  template <class W, class I, class S>
-  static __device__ __forceinline__ void chunk(const W&, const gemm::Problem<GatedBackward>& p, const Tile& t, int row0, int col, uint32_t tmem, I& in, S& st, int lane) {
-    const bool inside = row0 < p.M && col < p.N;
-    uint32_t g[16], u[16], d[32], dup[16], h[16];
+  template <int TN, class W, class I>
+  static __device__ __forceinline__ void chunk(const W&, const gemm::Problem<GatedBackward>& p, const Tile&, int row, int col, uint32_t tmem, I& in) {
+    uint32_t d[32], dup[16], h[16];
     sm100::tmem_ld32(tmem, d);
-    in.get(0, g);
-    in.get(1, u);
-    in.release();
     sm100::tmem_ld_wait();
+    if (row >= p.M) return;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float2 gg = gemm::unpack_bf16(g[i]), uu = gemm::unpack_bf16(u[i]);
+      const float2 gg = gemm::unpack_bf16(in[0][i]), uu = gemm::unpack_bf16(in[1][i]);
       const float d0 = __uint_as_float(d[2 * i]), d1 = __uint_as_float(d[2 * i + 1]);
       float a0, s0, a1, s1;
       activation<ACT>(gg.x, a0, s0);
       activation<ACT>(gg.y, a1, s1);
-      g[i] = gemm::pack_bf16(d0 * uu.x * s0, d1 * uu.y * s1);
+      in[0][i] = gemm::pack_bf16(d0 * uu.x * s0, d1 * uu.y * s1);
       dup[i] = gemm::pack_bf16(d0 * a0, d1 * a1);
       h[i] = gemm::pack_bf16(a0 * uu.x, a1 * uu.y);
     }
-    uint32_t box = st.get();
-    gemm::box_row(box, lane, g);
-    st.put(&p.out[0], box, col, row0, 0, inside);
-    box = st.get();
-    gemm::box_row(box, lane, dup);
-    st.put(&p.out[1], box, col, row0, 0, inside);
-    box = st.get();
-    gemm::box_row(box, lane, h);
-    st.put(&p.out[2], box, col, row0, 0, inside);
+    gemm::store_row(p.out[0], row, col, in[0]);
+    gemm::store_row(p.out[1], row, col, dup);
+    gemm::store_row(p.out[2], row, col, h);
   }
 };
 
@@ -129,27 +113,23 @@ template <bool A, bool B, int K_PARTS = 1>
 struct Plain {
   static constexpr bool A_MN = A, B_MN = B, F16 = false, PAIRED_B = false;
   static constexpr int PARTS = K_PARTS, OUTPUTS = 1, INPUTS = 0;
-  template <class W, class I, class S>
-  static __device__ __forceinline__ void chunk(const W&, const gemm::Problem<Plain>& p, const Tile& t, int row0, int col, uint32_t tmem, I&, S& st, int lane) {
+  template <int TN, class W, class I>
+  static __device__ __forceinline__ void chunk(const W&, const gemm::Problem<Plain>& p, const Tile& t, int row, int col, uint32_t tmem, I&) {
     uint32_t v[32];
     sm100::tmem_ld32(tmem, v);
     sm100::tmem_ld_wait();
+    if (row >= p.M) return;
     if (p.partial != nullptr) {
       const int64_t ld = (p.N + 3) & ~3;
-      if (row0 + lane < p.M) {
-        float* to = p.partial + (static_cast<int64_t>(t.split) * p.M + row0 + lane) * ld;
+      float* to = p.partial + (static_cast<int64_t>(t.split) * p.M + row) * ld;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (col + 4 * i < ld)
-            *reinterpret_cast<uint4*>(to + col + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-      }
+      for (int i = 0; i < 8; ++i)
+        if (col + 4 * i < ld) *reinterpret_cast<uint4*>(to + col + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
     } else {
       uint32_t packed[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) packed[i] = gemm::pack_bf16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-      const uint32_t box = st.get();
-      gemm::box_row(box, lane, packed);
-      st.put(&p.out[0], box, col, row0, 0, row0 < p.M && col < p.N);
+      gemm::store_row(p.out[0], row, col, packed);
     }
   }
 };
@@ -396,10 +376,10 @@ void set_sizes(gemm::Sizes& p, int64_t M, int64_t N, int64_t steps0, int64_t ste
   p.steps0 = static_cast<int>(steps0); p.steps = static_cast<int>(steps);
 }
 template <class Policy>
-int set_output(gemm::Problem<Policy>& p, const Output& o) {
+void set_output(gemm::Problem<Policy>& p, const Output& o) {
   p.splits = o.splits;
   p.partial = o.part;
-  return o.part == nullptr ? gemm::map_result<Policy>(&p.out[0], {o.p, p.N}, p.M, p.N) : HASTE_OK;
+  p.out[0] = gemm::result({o.p, p.N});
 }
 void add_sum(Sums& s, const Output& o, int64_t M, int64_t N) {
   if (o.part == nullptr) return;
@@ -479,10 +459,10 @@ int forward(Arena& arena, const GatedCall& c, cudaStream_t st) {
     HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wg.p, wg.ld}, c.F, c.D)));
     HASTE_TRY((gemm::map_b<K, TN>(&p.b[1], {wu.p, wu.ld}, c.F, c.D)));
     if (c.gate != nullptr) {
-      HASTE_TRY(gemm::map_result<K>(&p.out[0], {c.gate, c.ldh}, c.T, c.F));
-      HASTE_TRY(gemm::map_result<K>(&p.out[1], {c.up, c.ldh}, c.T, c.F));
+      p.out[0] = gemm::result({c.gate, c.ldh});
+      p.out[1] = gemm::result({c.up, c.ldh});
     }
-    HASTE_TRY(gemm::map_result<K>(&p.out[2], {h, ldF}, c.T, c.F));
+    p.out[2] = gemm::result({h, ldF});
     return gemm::launch<K, TN>(w, align.c.n > 0, st);
   }));
   HASTE_TRY(by_form<Plain<false, false>>(fy.narrow, [&](auto policy, auto columns) -> int {
@@ -492,7 +472,7 @@ int forward(Arena& arena, const GatedCall& c, cudaStream_t st) {
     w.problems = 1;
     auto& p = w.p[0];
     set_sizes(p, c.T, c.O, sF, sF);
-    HASTE_TRY(set_output<K>(p, y));
+    set_output<K>(p, y);
     HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], {h, ldF}, c.T, c.F)));
     HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wd.p, wd.ld}, c.O, c.F)));
     return gemm::launch<K, TN>(w, true, st);
@@ -532,10 +512,10 @@ int backward(Arena& arena, const GatedGradCall& c, cudaStream_t st) {
       set_sizes(p, c.T, c.F, sO, sO);
       HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], {dy.p, dy.ld}, c.T, c.O)));
       HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wd.p, wd.ld}, c.F, c.O)));
-      HASTE_TRY(gemm::map_result<K>(&p.in[0], {gate.p, gate.ld}, c.T, c.F));
-      HASTE_TRY(gemm::map_result<K>(&p.in[1], {up.p, up.ld}, c.T, c.F));
+      p.in[0] = gemm::result({gate.p, gate.ld});
+      p.in[1] = gemm::result({up.p, up.ld});
       void* outs[3] = {dgate, dup, h};
-      for (int i = 0; i < 3; ++i) HASTE_TRY(gemm::map_result<K>(&p.out[i], {outs[i], ldF}, c.T, c.F));
+      for (int i = 0; i < 3; ++i) p.out[i] = gemm::result({outs[i], ldF});
       return gemm::launch<K, TN>(w, align.c.n > 0, st);
     }));
   }
@@ -547,7 +527,7 @@ int backward(Arena& arena, const GatedGradCall& c, cudaStream_t st) {
       w.problems = 1;
       auto& p = w.p[0];
       set_sizes(p, c.T, c.D, sF, 2 * sF);
-      HASTE_TRY(set_output<K>(p, dx));
+      set_output<K>(p, dx);
       HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], {dgate, ldF}, c.T, c.F)));
       HASTE_TRY((gemm::map_a<K, TN>(&p.a[1], {dup, ldF}, c.T, c.F)));
       HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wg.p, wg.ld}, c.D, c.F)));
@@ -568,7 +548,7 @@ int backward(Arena& arena, const GatedGradCall& c, cudaStream_t st) {
       if (o.p == nullptr) return HASTE_OK;
       auto& p = w.p[w.problems++];
       set_sizes(p, M, N, sT, sT);
-      HASTE_TRY(set_output<K>(p, o));
+      set_output<K>(p, o);
       HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], a, M, c.T)));
       HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], b, N, c.T)));
       add_sum(s, o, M, N);

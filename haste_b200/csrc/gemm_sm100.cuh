@@ -5,9 +5,9 @@
 // A cluster of two CTAs has a tile of 256 x TN: each loads its half of both operands by TMA (128 rows of a, TN / 2 of b, 64 along k), the even one
 // issues tcgen05.mma.cta_group::2, whose operands are both CTAs' shared memory and whose accumulator is 128 x TN fp32 in each CTA's TMEM (two of
 // them, so that one is read while the next is summed).  Either operand lies with k or with its rows (m, n) contiguous.  What happens to an accumulator is
-// the policy's: its warps read TMEM, 32 rows x 32 columns at a time, beside boxes of that size of up to two 16-bit matrices, which each warp has brought by TMA
-// ahead, and hand such boxes to tensor-map stores.  (With loads of its rows by every lane, when the accumulator was there, the last product of a Newton-Schulz
-// step over 50 M elements took 154 us.)
+// the policy's: its warps read TMEM, 32 rows x 32 columns at a time, a lane's own row of 64 bytes of up to two 16-bit matrices beside it, loaded a chunk ahead, and
+// store a lane's row in whole 32-byte sectors.  The epilogue keeps out of shared memory, whose bandwidth the tensor cores' operands and their copies take in full: with tiles staged
+// for tensor-map stores, and inputs brought by them, a Newton-Schulz step over 50 M elements took 1870 K cycles, 980 K without its stores and inputs.
 //
 // TN = 256 is what keeps the tensor cores fed from L2; where there are fewer such tiles than pairs of SMs a narrow form (TN = 64, or 128 for a paired b) has more
 // and shorter ones.
@@ -32,7 +32,6 @@ using namespace sm100;
 constexpr int TILE = 256;              // rows of a pair's tile
 constexpr int KSTEP = 64;              // one 128-byte swizzle row of 16-bit values
 constexpr int EPI_WARPS = 8;
-constexpr int BOX_BYTES = 32 * 32 * 2; // what a warp loads or stores at once
 constexpr int THREADS = 12 * 32;
 constexpr int GROUP_M = 8;             // tiles of m that are walked before the next of n: what runs at once shares its operands in L2
 
@@ -40,25 +39,16 @@ constexpr int GROUP_M = 8;             // tiles of m that are walked before the 
 template <class Policy>
 constexpr int narrow() { return Policy::PAIRED_B ? 128 : 64; }
 
-template <class Policy, int TN>
+template <int TN>
 struct Layout {
   static constexpr int A_BYTES = 128 * KSTEP * 2;
   static constexpr int B_BYTES = TN / 2 * KSTEP * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int AHEAD = TN == 256 ? 2 : 1;                                          // boxes of each input that a warp has on their way
-  static constexpr int IN_BOXES = AHEAD * Policy::INPUTS;                                  // per warp
-  static constexpr int OUT_BOXES = TN == 256 && Policy::INPUTS > 0 ? 2 : 4;
-  static constexpr int STAGES = TN == 256 && Policy::INPUTS == 2 ? 4 : 5;
-  static constexpr int OFF_EPI = STAGES * STAGE_BYTES;
-  static constexpr int OFF_BAR = OFF_EPI + EPI_WARPS * (IN_BOXES + OUT_BOXES) * BOX_BYTES;
-  static constexpr int BARRIERS = 2 * STAGES + 4 + EPI_WARPS * AHEAD;
+  static constexpr int STAGES = 224 * 1024 / STAGE_BYTES;
+  static constexpr int OFF_BAR = STAGES * STAGE_BYTES;
+  static constexpr int BARRIERS = 2 * STAGES + 4;
   static constexpr int SMEM_BYTES = OFF_BAR + 8 * BARRIERS + 16 + 1024;      // the last for aligning the first stage
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
-  static constexpr int TMEM_COLUMNS = 2 * TN;
-  static constexpr int COLUMNS = Policy::PAIRED_B ? TN / 2 : TN;             // of the result, per tile
-  static constexpr int CHUNKS = COLUMNS / 64;                                // boxes of columns of a warp
-  // an operand b of 32 rows with these contiguous has a swizzle of 64 bytes
-  static constexpr bool B_SMALL = Policy::B_MN && TN == 64;
 };
 
 // ---------------------------------------------------------------- pairs of CTAs
@@ -82,15 +72,6 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const void* tmap, in
       "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
       "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
-}
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, int x, int y, int z, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(z),
-               "r"(bar)
-               : "memory");
-}
-__device__ __forceinline__ void tma_store_3d(const void* tmap, uint32_t src, int x, int y, int z) {
-  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(tmap), "r"(x), "r"(y), "r"(z), "r"(src)
-               : "memory");
 }
 __device__ __forceinline__ void umma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -116,7 +97,7 @@ __device__ __forceinline__ void cluster_sync_all() {
 }
 
 // ---------------------------------------------------------------- what a launch works on
-// One product: its sizes, and its tensor maps, as many as the policy has.
+// One product: its sizes, its operands' tensor maps and what the policy reads and writes.
 struct Sizes {
   float* partial;                  // fp32 sums of the parts that k was cut into
   int M, N;                        // of the result
@@ -125,10 +106,16 @@ struct Sizes {
   int steps0, steps;               // steps of k in the first part, and in both
   int first;                       // number of this problem's first tile; set by launch()
 };
+// A 16-bit matrix of the result's size that the policy reads or writes: rows of ld elements, a multiple of 8, from 16 bytes on; wide: both on 32 bytes
+struct Matrix16 {
+  uint16_t* p;
+  int64_t ld;
+  int wide;
+};
 template <class Policy>
 struct Problem : Sizes {
   CUtensorMap a[Policy::PARTS], b[Policy::PAIRED_B ? 2 : Policy::PARTS];      // by the part of k; of a paired b by the CTA
-  CUtensorMap out[Policy::OUTPUTS], in[Policy::INPUTS > 0 ? Policy::INPUTS : 1];           // in: 16-bit matrices that the policy reads at the tile's place
+  Matrix16 out[Policy::OUTPUTS], in[Policy::INPUTS > 0 ? Policy::INPUTS : 1];
 };
 template <class Policy, int P>
 struct Work {
@@ -161,45 +148,6 @@ __device__ __forceinline__ Tile tile_at(const Work<Policy, P>& w, int t) {
 }
 
 // ---------------------------------------------------------------- epilogue helpers
-// A warp's boxes of 32 rows x 32 16-bit columns on their way to memory (64-byte swizzle: 16-byte chunk j of row r at j ^ (r / 2 % 4)).
-template <int BOXES>
-struct Stager {
-  uint32_t base;
-  int lane, next;
-  // The next free box
-  __device__ __forceinline__ uint32_t get() {
-    if (lane == 0) bulk_wait_read<BOXES - 1>();
-    __syncwarp();
-    const uint32_t at = base + next * BOX_BYTES;
-    next = (next + 1) % BOXES;
-    return at;
-  }
-  __device__ __forceinline__ void put(const void* tmap, uint32_t box, int x, int y, int z, bool inside) {
-    fence_proxy_async();
-    __syncwarp();
-    if (lane == 0) {
-      if (inside) tma_store_3d(tmap, box, x, y, z);
-      bulk_commit();
-    }
-  }
-};
-__device__ __forceinline__ void st_shared_v4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-__device__ __forceinline__ void st_shared_u16(uint32_t at, uint32_t v) {
-  asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(static_cast<uint16_t>(v)) : "memory");
-}
-// Row `lane` of a box: 32 values packed in pairs
-__device__ __forceinline__ void box_row(uint32_t box, int lane, const uint32_t (&p)[16]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) st_shared_v4(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
-}
-// Column `lane` of a box
-__device__ __forceinline__ void box_column(uint32_t box, int lane, const uint32_t (&p)[16]) {
-#pragma unroll
-  for (int c = 0; c < 32; ++c)
-    st_shared_u16(box + c * 64 + (((lane >> 3) ^ ((c >> 1) & 3)) << 4) + (lane & 7) * 2, c & 1 ? p[c >> 1] >> 16 : p[c >> 1] & 0xFFFFu);
-}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -210,66 +158,55 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 __device__ __forceinline__ float2 unpack_bf16(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
 __device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-// Row `lane` of a box, packed in pairs
-__device__ __forceinline__ void row_of_box(uint32_t box, int lane, uint32_t (&p)[16]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(p[4 * j]), "=r"(p[4 * j + 1]), "=r"(p[4 * j + 2]), "=r"(p[4 * j + 3]) : "r"(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) : "memory");
+__device__ __forceinline__ void store_32_bytes(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
-
-// A warp's boxes of the policy's inputs, AHEAD of what it works on: over all chunks of columns of all its tiles, one after the other.  Beyond the matrix they
-// hold zeros.
-template <class Policy, int P, int TN>
-struct Inputs {
-  using L = Layout<Policy, TN>;
-  static constexpr int AHEAD = L::AHEAD;
-  const Work<Policy, P>& w;
-  uint32_t base, bars;             // boxes and barriers of this warp
-  int lane, quarter, half, rank, stride;
-  int issue_t, issue_j, issued, taken;
-  Tile tile;
-
-  __device__ __forceinline__ void issue() {
-    if (issue_t >= w.tiles) return;
-    if (issue_j == 0) tile = tile_at(w, issue_t);
-    if (lane == 0) {
-      const Problem<Policy>& p = w.p[tile.problem];
-      const int slot = issued % AHEAD, x = tile.n * L::COLUMNS + half * (L::COLUMNS / 2) + issue_j * 32, y = tile.m * TILE + rank * 128 + quarter * 32;
-      mbar_arrive_expect_tx(bars + 8 * slot, Policy::INPUTS * BOX_BYTES);
+// 32 columns of a row, packed in pairs: what lies in the (padded) row
+__device__ __forceinline__ void store_row(const Matrix16& m, int row, int col, const uint32_t (&v)[16]) {
+  uint16_t* to = m.p + static_cast<int64_t>(row) * m.ld + col;
+  if (m.wide) {
 #pragma unroll
-      for (int i = 0; i < Policy::INPUTS; ++i) tma_load_3d(base + (slot * Policy::INPUTS + i) * BOX_BYTES, &p.in[i], x, y, 0, bars + 8 * slot);
-    }
-    ++issued;
-    if (++issue_j == L::CHUNKS) { issue_j = 0; issue_t += stride; }
+    for (int j = 0; j < 2; ++j)
+      if (col + 16 * j < m.ld) store_32_bytes(to + 16 * j, v + 8 * j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + 8 * j < m.ld) *reinterpret_cast<uint4*>(to + 8 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
   }
-  __device__ __forceinline__ void start() {
-    if (Policy::INPUTS > 0)
-#pragma unroll 1
-      for (int i = 0; i < AHEAD; ++i) issue();
+}
+// and zeros beyond it
+__device__ __forceinline__ void load_row(const Matrix16& m, int row, int col, bool there, uint32_t (&v)[16]) {
+  const uint16_t* from = m.p + static_cast<int64_t>(row) * m.ld + col;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = 0;
+  if (!there) return;
+  if (m.wide) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (col + 16 * j < m.ld)
+        asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(v[8 * j]), "=r"(v[8 * j + 1]), "=r"(v[8 * j + 2]), "=r"(v[8 * j + 3]), "=r"(v[8 * j + 4]), "=r"(v[8 * j + 5]), "=r"(v[8 * j + 6]), "=r"(v[8 * j + 7])
+                     : "l"(from + 16 * j));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + 8 * j < m.ld) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4*>(from + 8 * j));
+        v[4 * j] = q.x; v[4 * j + 1] = q.y; v[4 * j + 2] = q.z; v[4 * j + 3] = q.w;
+      }
   }
-  // The next chunk's boxes are there
-  __device__ __forceinline__ bool wait(volatile int* abort_flag) {
-    if (Policy::INPUTS == 0) return true;
-    return __all_sync(0xffffffffu, mbar_wait(bars + 8 * (taken % AHEAD), (taken / AHEAD) & 1, abort_flag, w.err, 306, w.wait_limit));
-  }
-  __device__ __forceinline__ void get(int i, uint32_t (&p)[16]) const { row_of_box(base + (taken % AHEAD * Policy::INPUTS + i) * BOX_BYTES, lane, p); }
-  // All of them have been read
-  __device__ __forceinline__ void release() {
-    if (Policy::INPUTS == 0) return;
-    ++taken;
-    __syncwarp();
-    issue();
-  }
-};
+}
 
 // ---------------------------------------------------------------- the kernel
 // Policy: A_MN, B_MN (the operand's rows are contiguous, not k), F16 (else bf16), PAIRED_B (each CTA has an operand b of its own: TN / 2 columns of
 // two products side by side), PARTS of k, OUTPUTS, INPUTS, and
-//   static void chunk(w, p, tile, row0, col, tmem, inputs, stager, lane)   32 rows x 32 columns of the result at (row0, col), accumulator at tmem
+//   static void chunk<TN>(w, p, tile, row, col, tmem, inputs)   32 columns of this lane's row of the result, accumulator at tmem
 template <class Policy, int P, int TN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm100_kernel(const __grid_constant__ Work<Policy, P> w) {
-  using L = Layout<Policy, TN>;
-  constexpr int STAGES = L::STAGES, AHEAD = L::AHEAD;
+  using L = Layout<TN>;
+  constexpr int STAGES = L::STAGES, TMEM_COLUMNS = 2 * TN;
+  constexpr int COLUMNS = Policy::PAIRED_B ? TN / 2 : TN, CHUNKS = COLUMNS / 64;         // columns of the result in a tile, and a warp's chunks of 32 of them
+  constexpr bool B_SMALL = Policy::B_MN && TN == 64;         // an operand b of 32 rows with these contiguous has a swizzle of 64 bytes
   extern __shared__ uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   const uint32_t base = smem_u32(sm);
@@ -279,7 +216,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
   auto bar_empty = [&](int s) { return base + L::OFF_BAR + 8 * (STAGES + s); };
   auto bar_done = [&](int s) { return base + L::OFF_BAR + 8 * (2 * STAGES + s); };
   auto bar_free = [&](int s) { return base + L::OFF_BAR + 8 * (2 * STAGES + 2 + s); };
-  const uint32_t bar_in = base + L::OFF_BAR + 8 * (2 * STAGES + 4);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + L::OFF_BAR + 8 * L::BARRIERS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::OFF_BAR + 8 * L::BARRIERS + 8);
   const long long WL = w.wait_limit;
@@ -287,11 +223,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(bar_done(s), 1); mbar_init(bar_free(s), 2 * EPI_WARPS); }
-    for (int s = 0; s < EPI_WARPS * AHEAD; ++s) mbar_init(bar_in + 8 * s, 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == 2) tmem_alloc_pair(smem_u32(tmem_slot), L::TMEM_COLUMNS);
+  if (warp == 2) tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLUMNS);
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();                // the other CTA's barriers are there, and it has started
@@ -341,8 +276,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
     constexpr uint32_t IDESC = (1u << 4) | FORMAT | (static_cast<uint32_t>(Policy::A_MN) << 15) | (static_cast<uint32_t>(Policy::B_MN) << 16) |
                                (static_cast<uint32_t>(TN >> 3) << 17) | (static_cast<uint32_t>(TILE >> 4) << 24);
     const uint64_t da = make_sdesc(base, Policy::A_MN ? L::A_BYTES / 2 : 16, 1024);
-    const uint64_t db = L::B_SMALL ? make_sdesc64(base + L::A_BYTES, 16, 512) : make_sdesc(base + L::A_BYTES, Policy::B_MN ? L::B_BYTES / 2 : 16, 1024);
-    constexpr uint64_t KA = Policy::A_MN ? 2048 >> 4 : 32 >> 4, KB = L::B_SMALL ? 1024 >> 4 : Policy::B_MN ? 2048 >> 4 : 32 >> 4;
+    const uint64_t db = B_SMALL ? make_sdesc64(base + L::A_BYTES, 16, 512) : make_sdesc(base + L::A_BYTES, Policy::B_MN ? L::B_BYTES / 2 : 16, 1024);
+    constexpr uint64_t KA = Policy::A_MN ? 2048 >> 4 : 32 >> 4, KB = B_SMALL ? 1024 >> 4 : Policy::B_MN ? 2048 >> 4 : 32 >> 4;
     int it = 0, n = 0;
     for (int t = first; t < w.tiles; t += stride, ++n) {
       const Tile tl = tile_at(w, t);
@@ -372,31 +307,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
   } else if (warp >= 4) {
     // ---------------- epilogue
     const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const uint32_t mine = base + L::OFF_EPI + static_cast<uint32_t>(warp - 4) * (L::IN_BOXES + L::OUT_BOXES) * BOX_BYTES;
-    Inputs<Policy, P, TN> in = {w, mine + L::OUT_BOXES * BOX_BYTES, bar_in + 8 * AHEAD * (warp - 4), lane, quarter, half, static_cast<int>(rank), stride, first, 0, 0, 0, {}};
-    Stager<L::OUT_BOXES> st = {mine, lane, 0};
-    in.start();
+    constexpr int INPUTS = Policy::INPUTS > 0 ? Policy::INPUTS : 1;
     int n = 0;
     for (int t = first; t < w.tiles; t += stride, ++n) {
       const Tile tl = tile_at(w, t);
       const Problem<Policy>& p = w.p[tl.problem];
-      const int buf = n & 1, row0 = tl.m * TILE + static_cast<int>(rank) * 128 + quarter * 32, at = half * (L::COLUMNS / 2);
+      const int buf = n & 1, row = tl.m * TILE + static_cast<int>(rank) * 128 + quarter * 32 + lane, at = half * (COLUMNS / 2), col0 = tl.n * COLUMNS + at;
+      uint32_t in[INPUTS][16], ahead[INPUTS][16];
+      if (Policy::INPUTS > 0) {
+#pragma unroll
+        for (int i = 0; i < INPUTS; ++i) load_row(p.in[i], row, col0, row < p.M, ahead[i]);
+      }
       bool ok = mbar_wait(bar_done(buf), (n >> 1) & 1, abort_flag, w.err, 305, WL);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
 #pragma unroll 1
-      for (int j = 0; j < L::CHUNKS && ok; ++j) {
-        ok = in.wait(abort_flag);
-        if (ok) Policy::chunk(w, p, tl, row0, tl.n * L::COLUMNS + at + 32 * j, tmem + buf * TN + (static_cast<uint32_t>(quarter * 32) << 16) + at + 32 * j, in, st, lane);
+      for (int j = 0; j < CHUNKS; ++j) {
+        if (Policy::INPUTS > 0) {
+#pragma unroll
+          for (int i = 0; i < INPUTS; ++i) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) in[i][e] = ahead[i][e];
+            if (j + 1 < CHUNKS) load_row(p.in[i], row, col0 + 32 * (j + 1), row < p.M, ahead[i]);
+          }
+        }
+        __syncwarp();                // TMEM is read by whole warps
+        Policy::template chunk<TN>(w, p, tl, row, col0 + 32 * j, tmem + buf * TN + (static_cast<uint32_t>(quarter * 32) << 16) + at + 32 * j, in);
       }
-      if (!ok) break;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_at_leader(bar_free(buf));
     }
-    if (lane == 0) bulk_wait<0>();
-    __syncwarp();
   }
 
   // ---------------- teardown.  After an abort copies may be on their way into this CTA's shared memory, and products into its TMEM: they have some
@@ -409,7 +351,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
   }
   cluster_sync_all();
   tc_fence_after();
-  if (warp == 2) tmem_dealloc_pair(tmem, L::TMEM_COLUMNS);
+  if (warp == 2) tmem_dealloc_pair(tmem, TMEM_COLUMNS);
 }
 
 // ---------------------------------------------------------------- host side
@@ -432,9 +374,8 @@ int map_b(CUtensorMap* out, const Operand& o, int64_t rows, int64_t k) {
   return Policy::B_MN ? make_map(out, o.p, Policy::F16, rows, k, 1, o.ld, 0, TN == 64 ? 32 : 64, 64)
                       : make_map(out, o.p, Policy::F16, k, rows, 1, o.ld, 0, 64, TN / 2);
 }
-template <class Policy>
-int map_result(CUtensorMap* out, const Operand& o, int64_t M, int64_t N) {
-  return make_map(out, o.p, Policy::F16, N, M, 1, o.ld, 0, 32, 32);
+inline Matrix16 result(const Operand& o) {
+  return {static_cast<uint16_t*>(const_cast<void*>(o.p)), o.ld, o.ld % 16 == 0 && (reinterpret_cast<uintptr_t>(o.p) & 31) == 0};
 }
 inline int64_t steps_of(int64_t k) { return (k + KSTEP - 1) / KSTEP; }
 
@@ -475,7 +416,8 @@ inline int64_t tiles_for(int64_t M, int64_t N, int64_t columns) { return ((M + T
 // Launches what is in w.p[0 .. problems): tiles are counted here.  behind: the kernel before it in the stream is one of the same call.
 template <class Policy, int TN, int P>
 int launch(Work<Policy, P>& w, bool behind, cudaStream_t st) {
-  using L = Layout<Policy, TN>;
+  using L = Layout<TN>;
+  constexpr int COLUMNS = Policy::PAIRED_B ? TN / 2 : TN;
   auto kernel = gemm_sm100_kernel<Policy, P, TN>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM_BYTES);
   if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
@@ -483,7 +425,7 @@ int launch(Work<Policy, P>& w, bool behind, cudaStream_t st) {
   for (int i = 0; i < w.problems; ++i) {
     Sizes& p = w.p[i];
     p.tiles_m = (p.M + TILE - 1) / TILE;
-    p.tiles_n = (p.N + L::COLUMNS - 1) / L::COLUMNS;
+    p.tiles_n = (p.N + COLUMNS - 1) / COLUMNS;
     if (static_cast<int64_t>(p.tiles_m) * p.tiles_n > 0x3FFFFFFF) return fail(HASTE_ERR_TOO_LARGE, "too many tiles for one launch");
     p.first = static_cast<int>(tiles);
     tiles += static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;

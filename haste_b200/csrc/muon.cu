@@ -316,7 +316,11 @@ __device__ __forceinline__ uint32_t word(const uint4& r, int i) { return i == 0 
 __device__ __forceinline__ void store_weights(float* p, int have, const float (&v)[4], const Coefficients&, int64_t) { store4(p, have, vec4(p, have), v); }
 __device__ __forceinline__ void store_weights(__nv_bfloat16* p, int have, const float (&v)[4], const Coefficients& c, int64_t i) {
   uint32_t b[4];
-  if (c.sr) {
+  if (c.sr && (i & 3) == 0) {
+    const uint4 r = random_words(c, i >> 2);
+    b[0] = sr_bf16_bits(v[0], r.x & 0xFFFFu); b[1] = sr_bf16_bits(v[1], r.y & 0xFFFFu);
+    b[2] = sr_bf16_bits(v[2], r.z & 0xFFFFu); b[3] = sr_bf16_bits(v[3], r.w & 0xFFFFu);
+  } else if (c.sr) {
     const uint4 first = random_words(c, i >> 2);
     const int skip = static_cast<int>(i & 3);
     const uint4 second = skip ? random_words(c, (i >> 2) + 1) : first;
@@ -408,7 +412,7 @@ struct Sizes {
   int64_t p, q;                    // rows and columns of X, padded
   int64_t x() const { return p * q; }
   int64_t a() const { return p * p; }
-  int64_t bytes() const { return 2 * (3 * x() + 2 * a()) + 5 * 256 + 8 * NORM_PARTS + 8; }
+  int64_t bytes() const { return 2 * (3 * x() + a()) + 4 * 256 + 8 * NORM_PARTS + 8; }
 };
 Sizes sizes_of(int64_t rows, int64_t cols) { return {up64(std::min(rows, cols)), up64(std::max(rows, cols))}; }
 
@@ -503,7 +507,7 @@ int launch_muon(const MuonCall& c, cudaStream_t st) {
       newton_schulz::Batch h;
       h.p = s.p; h.q = s.q; h.count = static_cast<int64_t>(end - i);
       for (uint16_t** x : {&h.hi[0], &h.hi[1], &h.lo}) *x = reinterpret_cast<uint16_t*>(take(2 * h.count * s.x()));
-      for (uint16_t** x : {&h.A, &h.B}) *x = reinterpret_cast<uint16_t*>(take(2 * h.count * s.a()));
+      h.B = reinterpret_cast<uint16_t*>(take(2 * h.count * s.a()));
       for (size_t j = i; j < end; ++j) {
         const int64_t o = plan.order[j], x = static_cast<int64_t>(j - i) * s.x(), size = c.rows[o] * c.cols[o];
         Matrix m = {};

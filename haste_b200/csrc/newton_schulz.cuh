@@ -1,19 +1,19 @@
 // All Newton-Schulz steps over many matrices in one launch:  steps times  A = X X^T,  B = a I + b A + c A A,  X <- B X   (X [p, q], p and q multiples of 64)
 //
 // The three products of all steps are one list of tiles, which the pairs of CTAs take in turn.  A tile may be worked on when the matrix's product before it is complete:
-// every warp that has stored its part of a tile adds one to the matrix's counter, and who needs the result waits for the count.  The list walks the matrices in groups:
-// a group's A tiles, its B tiles, its X tiles, the next step, ..., then the next group, so that
-//   - what a tile waits for was begun by other pairs about a product earlier, and no pair idles at the end of one (a launch for each product left a quarter of the
-//     SMs without work in the last tiles of 5, and took 3 us and the first loads' latency each time);
-//   - a group is chosen to fit L2, so that only its first and last X pass through memory.
+// every warp that has stored its part of a tile adds one to the matrix's counter, and who needs the result waits for the count.  (A launch for each product left a quarter of
+// the SMs without work in the last tiles of 5, and took 3 us and the first loads' latency each time.)
+//
+// The list walks the matrices in groups that fit L2, so that only a group's first and last X pass through memory.  A group has two halves, a and b, whose products alternate so
+// that others stand between a product and the one that needs it:
+//   A of a, half of X of b (of the step before), B of a, the other half, half of X of a, A of b, the other half, B of b, and the next step
 // Every tile's predecessors stand before it in the list, and a pair works through its part of the list in order, so with all pairs resident (a cooperative launch) the first
 // unfinished tile can always proceed.  Waits are bounded as everywhere.
 //
 // A and B are symmetric: only tiles on and below the diagonal are computed and stored.  Where an operand's block lies above it, the block on the other side is loaded and
 // read by the tensor core with its rows and columns exchanged.
 //
-// Tiles are 256 x TN of a pair, with roles and barriers as in gemm_sm100.cuh; warp 3 looks up what comes next and waits for it, ahead of the others.  An epilogue warp
-// has a box for each of its columns' chunks, into which the chunk's input is loaded and from which its result is stored, and one more for X's upper part beside the lower.
+// Tiles are 256 x TN of a pair, with roles, barriers and an epilogue as in gemm_sm100.cuh; warp 3 looks up what comes next and waits for it, ahead of the others.
 #pragma once
 #include "gemm_sm100.cuh"
 
@@ -34,29 +34,64 @@ constexpr int STEPS_WITHOUT_LOWER = 2;
 __host__ __device__ constexpr bool has_lower(int step, int steps) { return step == 0 || step < steps - STEPS_WITHOUT_LOWER; }       // X before this step
 
 // Tensor maps of a batch of matrices of one shape: X's two buffers as operand a and b with k contiguous and as operand b with its rows contiguous, A and B as operand a (A's also b)
-// either way, and the epilogue's boxes of A, B, X and X's lower part.  In the wide form operands a and b are alike.
-enum Map { X_A, X_N = 2, A_A = 4, B_A, A_T, B_T, A_BOX, B_BOX, X_BOX, LO_BOX = 12, MAPS_WIDE, X_B = 13, A_B = 15, A_TB, MAPS_NARROW };
+// either way, and boxes of 32 x 32 of A, B, X and X's lower part for stores.  In the wide form operands a and b are alike.  A is kept where the next X will be, so there are two of its maps too.
+enum Map { X_A, X_N = 2, X_BOX = 4, A_A = 6, A_T = 8, A_BOX = 10, B_A = 12, B_T, B_BOX, LO_BOX, MAPS_WIDE, X_B = 16, A_B = 18, A_TB = 20, MAPS_NARROW = 22 };
 
 struct Info {
   int p, q, tiles_m, tiles_n, tiles_q; // tiles_n: columns' tiles of A and B, tiles_q: of X
   int symmetric, full;                 // tiles of A or B, and of X, in a matrix
+  uint16_t *x[2], *low, *b;            // X's buffers (A is in the other one), its lower part, B
 };
-struct Segment {                       // neighbouring matrices of one shape in a group
+struct Segment {                       // neighbouring matrices of one shape in half a group
   int shape, batch, count, matrix;     // first batch entry, how many, number of the first matrix
-  int symmetric0, full0;               // tiles of the group before it
+  int symmetric0, full0;               // tiles of the half before it
+};
+struct Half {
+  int segment, end, symmetric, full;   // segments; tiles of a product of all of it
 };
 struct Group {
   int first;                           // tile number
-  int segment, symmetric, full;        // first segment; tiles of a product of all of it
+  Half half[2];
 };
+// A place in a group's list: which product of which half in which step, and the tile's number there
+struct Place {
+  int half, phase, step, tile;
+};
+__host__ __device__ inline Place place_of(const Half& a, const Half& b, int steps, int t) {
+  const int own = 2 * a.symmetric + a.full + 2 * b.symmetric, period = own + b.full;
+  int step = 0, late = 0;              // tiles of b's X in this period
+  if (t >= own) {
+    step = 1 + (t - own) / period;
+    t -= own + (step - 1) * period;
+    late = b.full;
+    if (step == steps) return {1, 2, steps - 1, t};
+  }
+  const int a1 = a.full / 2, b1 = late / 2;
+  if (t < a.symmetric) return {0, 0, step, t};
+  t -= a.symmetric;
+  if (t < b1) return {1, 2, step - 1, t};
+  t -= b1;
+  if (t < a.symmetric) return {0, 1, step, t};
+  t -= a.symmetric;
+  if (t < late - b1) return {1, 2, step - 1, b1 + t};
+  t -= late - b1;
+  if (t < a1) return {0, 2, step, t};
+  t -= a1;
+  if (t < b.symmetric) return {1, 0, step, t};
+  t -= b.symmetric;
+  if (t < a.full - a1) return {0, 2, step, a1 + t};
+  return {1, 1, step, t - (a.full - a1)};
+}
+__host__ __device__ inline int64_t tiles_of(const Half& a, const Half& b, int steps) { return static_cast<int64_t>(steps) * (2ll * a.symmetric + a.full + 2ll * b.symmetric + b.full); }
+
 template <int TN>
 struct Steps {
   static constexpr int MAPS = TN == TILE ? static_cast<int>(MAPS_WIDE) : static_cast<int>(MAPS_NARROW);
-  static constexpr int SHAPES = TN == TILE ? 16 : 12, SEGMENTS = 64, GROUPS = 32;
+  static constexpr int SHAPES = TN == TILE ? 14 : 10, SEGMENTS = 64, GROUPS = 32;
   CUtensorMap map[SHAPES][MAPS];
   Info info[SHAPES];
-  Segment segment[SEGMENTS + 1];       // the last one: the end
-  Group group[GROUPS + 1];
+  Segment segment[SEGMENTS];
+  Group group[GROUPS];
   int groups, tiles, steps;
   float a, b, c;
   unsigned long long* done;            // by matrix
@@ -74,16 +109,14 @@ __device__ __forceinline__ Task task_at(const Steps<TN>& w, int t, int& g) {
   constexpr int PER = TILE / TN;
   while (g + 1 < w.groups && t >= w.group[g + 1].first) ++g;
   const Group& gr = w.group[g];
+  const Place at = place_of(gr.half[0], gr.half[1], w.steps, t - gr.first);
+  const Half& h = gr.half[at.half];
   Task r;
-  t -= gr.first;
-  const int per = 2 * gr.symmetric + gr.full;
-  r.step = t / per;
-  t -= r.step * per;
-  r.phase = t < gr.symmetric ? 0 : t < 2 * gr.symmetric ? 1 : 2;
-  t -= r.phase * gr.symmetric;
-  const int end = w.group[g + 1].segment;
-  int s = gr.segment;
-  while (s + 1 < end && t >= (r.phase < 2 ? w.segment[s + 1].symmetric0 : w.segment[s + 1].full0)) ++s;
+  t = at.tile;
+  r.phase = at.phase;
+  r.step = at.step;
+  int s = h.segment;
+  while (s + 1 < h.end && t >= (r.phase < 2 ? w.segment[s + 1].symmetric0 : w.segment[s + 1].full0)) ++s;
   const Segment& sg = w.segment[s];
   const Info& info = w.info[sg.shape];
   t -= r.phase < 2 ? sg.symmetric0 : sg.full0;
@@ -106,6 +139,29 @@ __device__ __forceinline__ Task task_at(const Steps<TN>& w, int t, int& g) {
   const unsigned long long whole = 2ull * info.symmetric + info.full;
   r.need = (r.step * whole + static_cast<unsigned long long>(r.phase) * info.symmetric) * (2 * EPI_WARPS);
   return r;
+}
+
+// 32 columns of a row of what other SMs may have written
+__device__ __forceinline__ void load_row(const uint16_t* p, uint32_t* v) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    uint32_t* r = v + 8 * j;
+    asm volatile("ld.relaxed.gpu.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "l"(p + 16 * j) : "memory");
+  }
+}
+__device__ __forceinline__ void tma_store_3d(const void* tmap, uint32_t src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(tmap), "r"(x), "r"(y), "r"(z), "r"(src)
+               : "memory");
+}
+// A warp's box of 32 rows x 32 columns (64-byte swizzle: 16-byte piece j of row r at j ^ (r / 2 % 4)), and on its way to memory
+constexpr int BOX_BYTES = 32 * 32 * 2;
+__device__ __forceinline__ void fill_box(uint32_t box, int lane, const uint32_t (&p)[16]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t at = box + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(p[4 * j]), "r"(p[4 * j + 1]), "r"(p[4 * j + 2]), "r"(p[4 * j + 3]) : "memory");
+  }
 }
 
 // ---------------------------------------------------------------- counters
@@ -131,37 +187,24 @@ __device__ __noinline__ bool wait_count(const unsigned long long* p, unsigned lo
   return true;
 }
 // What this thread's stores (bulk groups) wrote, once it has waited for them, is there for whoever sees the count
-__device__ __forceinline__ void add_count_only(unsigned long long* p) {
+__device__ __forceinline__ void add_count(unsigned long long* p) {
   fence_proxy_async_all();
   __threadfence();
   asm volatile("red.release.gpu.global.add.u64 [%0], %1;" ::"l"(p), "l"(1ull) : "memory");
-}
-__device__ __forceinline__ void add_count(unsigned long long* p) {
-  bulk_wait<0>();
-  add_count_only(p);
 }
 
 // ---------------------------------------------------------------- the kernel
 template <int TN>
 struct Layout {
   static constexpr int A_BYTES = 128 * KSTEP * 2, B_BYTES = TN / 2 * KSTEP * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = TN == TILE ? 4 : 8, TASKS = 4;
-  static constexpr int BOX_COLUMNS = TN == TILE ? 64 : 32, BOX_BYTES = 32 * BOX_COLUMNS * 2, CHUNKS = TN / 2 / BOX_COLUMNS, BOXES = CHUNKS + 1;
+  static constexpr int TASKS = 4, CHUNKS = TN / 64, BOXES = 2, EPI_BYTES = EPI_WARPS * BOXES * BOX_BYTES, STAGES = (224 * 1024 - EPI_BYTES) / STAGE_BYTES;
   static constexpr int OFF_EPI = STAGES * STAGE_BYTES;
-  static constexpr int OFF_TASK = OFF_EPI + EPI_WARPS * BOXES * BOX_BYTES;
+  static constexpr int OFF_TASK = OFF_EPI + EPI_BYTES;
   static constexpr int OFF_BAR = OFF_TASK + TASKS * 64;
-  static constexpr int BARRIERS = 2 * STAGES + 4 + 2 * TASKS + EPI_WARPS * CHUNKS;
+  static constexpr int BARRIERS = 2 * STAGES + 4 + 2 * TASKS;
   static constexpr int SMEM_BYTES = OFF_BAR + 8 * BARRIERS + 16 + 1024;
   static_assert(SMEM_BYTES <= 227 * 1024 && sizeof(Task) <= 64, "shared memory");
 };
-// Where 16-byte piece j of row r of a box lies
-template <int TN>
-__device__ __forceinline__ uint32_t piece(uint32_t box, int r, int j) {
-  return TN == TILE ? box + r * 128 + ((j ^ (r & 7)) << 4) : box + r * 64 + ((j ^ ((r >> 1) & 3)) << 4);
-}
-__device__ __forceinline__ void load_piece(uint32_t at, uint32_t* p) {
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(p[0]), "=r"(p[1]), "=r"(p[2]), "=r"(p[3]) : "r"(at) : "memory");
-}
 
 template <int TN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) newton_schulz_kernel(const __grid_constant__ Steps<TN> w) {
@@ -179,18 +222,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) newton_s
   auto bar_free = [&](int s) { return base + L::OFF_BAR + 8 * (2 * STAGES + 2 + s); };
   auto bar_task = [&](int s) { return base + L::OFF_BAR + 8 * (2 * STAGES + 4 + s); };
   auto bar_slot = [&](int s) { return base + L::OFF_BAR + 8 * (2 * STAGES + 4 + TASKS + s); };
-  const uint32_t bar_in = base + L::OFF_BAR + 8 * (2 * STAGES + 4 + 2 * TASKS);
   auto slot_of = [&](int n) -> volatile Task& { return *reinterpret_cast<volatile Task*>(sm + L::OFF_TASK + (n % TASKS) * 64); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + L::OFF_BAR + 8 * L::BARRIERS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::OFF_BAR + 8 * L::BARRIERS + 8);
   const long long WL = w.wait_limit;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
+    for (int s = 0; s < STAGES; ++s) { mbar_init(bar_full(s), 2); mbar_init(bar_empty(s), 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(bar_done(s), 1); mbar_init(bar_free(s), 2 * EPI_WARPS); }
     // read by the warps for loads, products (in the even CTA) and the epilogue
-    for (int s = 0; s < TASKS; ++s) { mbar_init(bar_task(s), 1); mbar_init(bar_slot(s), EPI_WARPS + (rank == 0 ? 2 : 1)); }
-    for (int s = 0; s < EPI_WARPS * L::CHUNKS; ++s) mbar_init(bar_in + 8 * s, 1);
+    for (int s = 0; s < TASKS; ++s) { mbar_init(bar_task(s), 1); mbar_init(bar_slot(s), EPI_WARPS + (rank == 0 ? 3 : 2)); }
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -228,36 +269,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) newton_s
       s.shape = k.shape; s.batch = k.batch; s.matrix = k.matrix; s.m = k.m; s.n = k.n; s.phase = k.phase; s.step = k.step;
       mbar_arrive(bar_task(n % TASKS));
     }
-  } else if (warp == 0 && lane == 0) {
-    // ---------------- loads
+  } else if ((warp == 0 || warp == 2) && lane == 0) {
+    // ---------------- loads: of operand a by warp 0, of b by warp 2 (one thread's instructions for both took longer than the narrow form's products)
     int it = 0;
     Task k;
     for (int n = 0; n < mine && take(n, false, k); ++n) {
       fence_proxy_async_all();
       const Info& info = w.info[k.shape];
-      const int cur = k.step & 1, steps = (k.phase == 0 ? info.q : info.p) / KSTEP;
+      const int cur = k.step & 1, next = cur ^ 1, steps = (k.phase == 0 ? info.q : info.p) / KSTEP;
       const CUtensorMap* maps = w.map[k.shape];
-      const CUtensorMap* ta = maps + (k.phase == 0 ? X_A + cur : k.phase == 1 ? A_A : B_A);
-      const CUtensorMap* tat = maps + (k.phase == 1 ? A_T : B_T);
-      const CUtensorMap* tb = maps + (k.phase == 0 ? (WIDE ? X_A : X_B) + cur : k.phase == 1 ? (WIDE ? A_A : A_B) : X_N + cur);
-      const CUtensorMap* tbt = k.phase == 1 ? maps + (WIDE ? A_T : A_TB) : tb;
-      const int am = k.m * TILE + static_cast<int>(rank) * 128, bn = k.n * TN + static_cast<int>(rank) * (TN / 2);
+      const CUtensorMap *straight, *turned;
+      int row, skip;                                   // of the operand; turned from block `skip` of k on
+      if (warp == 0) {
+        straight = maps + (k.phase == 0 ? X_A + cur : k.phase == 1 ? A_A + next : B_A);
+        turned = maps + (k.phase == 1 ? A_T + next : B_T);
+        row = k.m * TILE + static_cast<int>(rank) * 128;
+        skip = k.phase == 0 ? steps : (row / TILE + 1) * (TILE / KSTEP);
+      } else {
+        straight = maps + (k.phase == 0 ? (WIDE ? X_A : X_B) + cur : (WIDE ? A_A : A_B) + next);
+        turned = maps + (k.phase == 1 ? (WIDE ? A_T : A_TB) + next : X_N + cur);
+        row = k.n * TN + static_cast<int>(rank) * (TN / 2);
+        skip = k.phase == 0 ? steps : k.phase == 1 ? (row / TILE + 1) * (TILE / KSTEP) : 0;
+      }
+      const bool two = warp == 0 || WIDE;              // blocks of 64 rows of a turned operand
       for (int i = 0; i < steps; ++i, ++it) {
         const int s = it % STAGES, kc = i * KSTEP;
         if (!mbar_wait(bar_empty(s), ((it / STAGES) & 1) ^ 1, abort_flag, w.err, 322, WL)) break;
-        if (rank == 0) mbar_arrive_expect_tx(bar_full(s), 2 * L::STAGE_BYTES);
-        const uint32_t bar = gemm::leaders(bar_full(s)), as = base + s * L::STAGE_BYTES, bs = as + L::A_BYTES;
-        if (k.phase > 0 && above(kc, am)) {
-          gemm::tma_load_pair(as, tat, am, kc, k.batch, bar);
-          gemm::tma_load_pair(as + L::A_BYTES / 2, tat, am + 64, kc, k.batch, bar);
+        if (rank == 0) mbar_arrive_expect_tx(bar_full(s), 2 * (warp == 0 ? L::A_BYTES : L::B_BYTES));
+        const uint32_t bar = gemm::leaders(bar_full(s)), to = base + s * L::STAGE_BYTES + (warp == 0 ? 0 : L::A_BYTES);
+        if (i < skip) {
+          gemm::tma_load_pair(to, straight, kc, row, k.batch, bar);
         } else {
-          gemm::tma_load_pair(as, ta, kc, am, k.batch, bar);
-        }
-        if (k.phase == 2 || (k.phase == 1 && above(kc, bn))) {
-          gemm::tma_load_pair(bs, tbt, bn, kc, k.batch, bar);
-          if (WIDE) gemm::tma_load_pair(bs + L::B_BYTES / 2, tbt, bn + 64, kc, k.batch, bar);
-        } else {
-          gemm::tma_load_pair(bs, tb, kc, bn, k.batch, bar);
+          gemm::tma_load_pair(to, turned, row, kc, k.batch, bar);
+          if (two) gemm::tma_load_pair(to + 64 * KSTEP * 2, turned, row + 64, kc, k.batch, bar);
         }
       }
       if (*abort_flag) break;
@@ -299,122 +343,110 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) newton_s
   } else if (warp >= 4) {
     // ---------------- epilogue
     const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const uint32_t boxes = base + L::OFF_EPI + static_cast<uint32_t>(warp - 4) * L::BOXES * L::BOX_BYTES, second = boxes + L::CHUNKS * L::BOX_BYTES;
-    const uint32_t bars = bar_in + 8 * L::CHUNKS * (warp - 4);
+    const uint32_t boxes = base + L::OFF_EPI + static_cast<uint32_t>(warp - 4) * L::BOXES * BOX_BYTES;
     unsigned long long* pending = nullptr;             // counter of the tile before, whose stores may be on their way
-    int inputs = 0;                                    // tiles with input so far
-    auto flush = [&] {
-      if (pending != nullptr && lane == 0) add_count(pending);
+    int stores = 0;
+    auto tell = [&] {
+      if (pending != nullptr && lane == 0) {
+        bulk_wait<0>();
+        add_count(pending);
+      }
       pending = nullptr;
+    };
+    // 32 x 32 of the result on their way, from the box of the store before the last; one group each
+    auto put = [&](const CUtensorMap* map, const uint32_t (&v)[16], int col, int row0, int batch, bool inside) {
+      if (lane == 0) bulk_wait_read<L::BOXES - 1>();
+      __syncwarp();
+      const uint32_t box = boxes + (stores++ % L::BOXES) * BOX_BYTES;
+      fill_box(box, lane, v);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        if (inside) tma_store_3d(map, box, col, row0, batch);
+        bulk_commit();
+      }
     };
     Task k;
     for (int n = 0; n < mine; ++n) {
       // nobody may wait for this warp's last tile while it waits itself
-      if (!mbar_test(bar_task(n % TASKS), (n / TASKS) & 1)) flush();
+      if (!mbar_test(bar_task(n % TASKS), (n / TASKS) & 1)) tell();
       if (!take(n, true, k)) break;
-      const CUtensorMap* maps = w.map[k.shape];
       const Info& info = w.info[k.shape];
+      const CUtensorMap* maps = w.map[k.shape];
       const int buf = n & 1, cur = k.step & 1, row0 = k.m * TILE + static_cast<int>(rank) * 128 + quarter * 32, col0 = k.n * TN + half * (TN / 2);
       const int N = k.phase == 2 ? info.q : info.p;
-      const bool low = k.phase == 2 && has_lower(k.step, w.steps), more = k.phase == 2 && has_lower(k.step + 1, w.steps), input = k.phase == 1 || low;
-      if (lane == 0) bulk_wait_read<0>();              // the boxes are free
-      __syncwarp();
-      if (input && lane == 0) {
-        fence_proxy_async_all();
+      const bool low = k.phase == 2 && has_lower(k.step, w.steps), more = k.phase == 2 && has_lower(k.step + 1, w.steps), there = row0 < info.p;
+      const CUtensorMap* to = maps + (k.phase == 0 ? A_BOX + (cur ^ 1) : k.phase == 1 ? B_BOX : X_BOX + (cur ^ 1));
+      // the tile's input, all of it, while it is summed
+      uint32_t in[L::CHUNKS][16];
+      if (k.phase == 1 || low) {
+        const uint16_t* from = (k.phase == 1 ? info.x[cur ^ 1] : info.low) + static_cast<int64_t>(k.batch) * info.p * info.q + static_cast<int64_t>(row0 + lane) * N + col0;
 #pragma unroll
-        for (int j = 0; j < L::CHUNKS; ++j) {
-          mbar_arrive_expect_tx(bars + 8 * j, L::BOX_BYTES);
-          gemm::tma_load_3d(boxes + j * L::BOX_BYTES, maps + (k.phase == 1 ? A_BOX : LO_BOX), col0 + j * L::BOX_COLUMNS, row0, k.batch, bars + 8 * j);
-        }
+        for (int j = 0; j < L::CHUNKS; ++j)
+          if (there && col0 + 32 * j < N) load_row(from + 32 * j, in[j]);
       }
-      if (!mbar_test(bar_done(buf), (n >> 1) & 1)) flush();
+      if (!mbar_test(bar_done(buf), (n >> 1) & 1)) tell();
       bool ok = mbar_wait(bar_done(buf), (n >> 1) & 1, abort_flag, w.err, 327, WL);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-#pragma unroll 1
+#pragma unroll
       for (int j = 0; j < L::CHUNKS; ++j) {
-        const int col = col0 + j * L::BOX_COLUMNS;
-        const bool inside = row0 < info.p && col < N;
-        const uint32_t box = boxes + j * L::BOX_BYTES;
-        if (input) {
-          ok = __all_sync(0xffffffffu, mbar_wait(bars + 8 * j, inputs & 1, abort_flag, w.err, 328, WL));
-          if (!ok) break;
-        }
-        if (more && j > 0) {
-          if (lane == 0) bulk_wait_read<1>();          // the chunk before has left the second box
-          __syncwarp();
-        }
+        const int col = col0 + 32 * j;
+        uint32_t v[32], hi[16];
+        uint32_t(&e)[16] = in[j];
+        __syncwarp();                                  // TMEM is read by whole warps
+        tmem_ld32(tmem + buf * TN + (static_cast<uint32_t>(quarter * 32) << 16) + half * (TN / 2) + 32 * j, v);
+        tmem_ld_wait();
+        if (k.phase == 0) {
+          constexpr float SCALE = 1.f / (X_SCALE * X_SCALE);
 #pragma unroll
-        for (int h = 0; h < L::BOX_COLUMNS / 32; ++h) {
-          uint32_t v[32], e[16], hi[16];
-          tmem_ld32(tmem + buf * TN + (static_cast<uint32_t>(quarter * 32) << 16) + half * (TN / 2) + j * L::BOX_COLUMNS + 32 * h, v);
-          if (input) {
+          for (int i = 0; i < 16; ++i) hi[i] = gemm::pack_f16(__uint_as_float(v[2 * i]) * SCALE, __uint_as_float(v[2 * i + 1]) * SCALE);
+        } else if (k.phase == 1) {
+          const int own = row0 + lane - col;           // where the diagonal is in this row
 #pragma unroll
-            for (int q = 0; q < 4; ++q) load_piece(piece<TN>(box, lane, 4 * h + q), e + 4 * q);
+          for (int i = 0; i < 16; ++i) {
+            const float2 a = gemm::unpack_f16(e[i]);
+            float x = fmaf(w.c, __uint_as_float(v[2 * i]), w.b * a.x), y = fmaf(w.c, __uint_as_float(v[2 * i + 1]), w.b * a.y);
+            if (2 * i == own) x += w.a;
+            if (2 * i + 1 == own) y += w.a;
+            hi[i] = gemm::pack_f16(x, y);
           }
-          tmem_ld_wait();
-          if (k.phase == 0) {
-            constexpr float SCALE = 1.f / (X_SCALE * X_SCALE);
+        } else {
+          const float scale = w.a * (1.f / LO_SCALE);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) hi[i] = gemm::pack_f16(__uint_as_float(v[2 * i]) * SCALE, __uint_as_float(v[2 * i + 1]) * SCALE);
-          } else if (k.phase == 1) {
-            const int own = row0 + lane - col - 32 * h;    // where the diagonal is in this row
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float2 a = gemm::unpack_f16(e[i]);
-              float x = fmaf(w.c, __uint_as_float(v[2 * i]), w.b * a.x), y = fmaf(w.c, __uint_as_float(v[2 * i + 1]), w.b * a.y);
-              if (2 * i == own) x += w.a;
-              if (2 * i + 1 == own) y += w.a;
-              hi[i] = gemm::pack_f16(x, y);
+          for (int i = 0; i < 16; ++i) {
+            float x = __uint_as_float(v[2 * i]), y = __uint_as_float(v[2 * i + 1]);
+            if (low) {
+              const float2 l = gemm::unpack_f16(e[i]);
+              x = fmaf(scale, l.x, x);
+              y = fmaf(scale, l.y, y);
             }
-          } else {
-            const float scale = w.a * (1.f / LO_SCALE);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float x = __uint_as_float(v[2 * i]), y = __uint_as_float(v[2 * i + 1]);
-              if (low) {
-                const float2 l = gemm::unpack_f16(e[i]);
-                x = fmaf(scale, l.x, x);
-                y = fmaf(scale, l.y, y);
-              }
-              hi[i] = gemm::pack_f16(x, y);
-              if (more) {
-                const float2 r = gemm::unpack_f16(hi[i]);
-                e[i] = gemm::pack_f16((x - r.x) * LO_SCALE, (y - r.y) * LO_SCALE);
-              }
+            hi[i] = gemm::pack_f16(x, y);
+            if (more) {
+              const float2 r = gemm::unpack_f16(hi[i]);
+              e[i] = gemm::pack_f16((x - r.x) * LO_SCALE, (y - r.y) * LO_SCALE);
             }
           }
-          const uint32_t to = more ? second : box;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) gemm::st_shared_v4(piece<TN>(to, lane, 4 * h + q), hi[4 * q], hi[4 * q + 1], hi[4 * q + 2], hi[4 * q + 3]);
-          if (more) {                                  // in the place of what it was made of
-#pragma unroll
-            for (int q = 0; q < 4; ++q) gemm::st_shared_v4(piece<TN>(box, lane, 4 * h + q), e[4 * q], e[4 * q + 1], e[4 * q + 2], e[4 * q + 3]);
-          }
         }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) {                               // two groups for every chunk, whatever is in them
-          if (inside) gemm::tma_store_3d(maps + (k.phase == 0 ? A_BOX : k.phase == 1 ? B_BOX : X_BOX + (cur ^ 1)), more ? second : box, col, row0, k.batch);
-          bulk_commit();
-          if (inside && more) gemm::tma_store_3d(maps + LO_BOX, box, col, row0, k.batch);      // the tile's own place, which it has read
-          bulk_commit();
-          if (j == 0 && pending != nullptr) {          // the tile before: all but this chunk's groups
-            bulk_wait<2>();
-            add_count_only(pending);
+        const bool inside = there && col < N;
+        put(to, hi, col, row0, k.batch, inside);
+        if (more) put(maps + LO_BOX, e, col, row0, k.batch, inside);       // in the place of what it was made of
+        if (j == 0 && pending != nullptr) {
+          if (lane == 0) {                             // the tile before: all groups but this chunk's
+            if (more) bulk_wait<2>();
+            else bulk_wait<1>();
+            add_count(pending);
           }
+          pending = nullptr;
         }
-        if (j == 0) pending = nullptr;
       }
-      if (!ok) break;
-      if (input) ++inputs;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) gemm::arrive_at_leader(bar_free(buf));
       pending = w.done + k.matrix;
     }
-    flush();
+    tell();
     if (lane == 0) bulk_wait<0>();
     __syncwarp();
   }
@@ -432,17 +464,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) newton_s
 }
 
 // ---------------------------------------------------------------- host side
-// A batch of matrices of one shape: X [batch][p][q] in two buffers and its lower part, A and B [batch][p][p]
+// A batch of matrices of one shape: X [batch][p][q] in two buffers and its lower part, B [batch][p][p]
 struct Batch {
   int64_t p, q, count;
-  uint16_t *hi[2], *lo, *A, *B;
+  uint16_t *hi[2], *lo, *B;
 };
 #ifndef X_GROUP
-#define X_GROUP 250
+#define X_GROUP 160
 #endif
 constexpr int64_t GROUP_BYTES = int64_t(X_GROUP) << 20;
 
-inline int64_t bytes_of(const Batch& b) { return 2 * (3 * b.p * b.q + 2 * b.p * b.p); }
+inline int64_t bytes_of(const Batch& b) { return 2 * (2 * b.p * b.q + b.p * b.p); }      // of a matrix, that L2 is to hold: X's lower part just passes
 
 template <int TN>
 int set_shape(Steps<TN>& w, int i, const Batch& b) {
@@ -453,87 +485,85 @@ int set_shape(Steps<TN>& w, int i, const Batch& b) {
   f.symmetric = 0;
   for (int m = 0; m < f.tiles_m; ++m) f.symmetric += std::min((m + 1) * (TILE / TN), f.tiles_n);
   f.full = f.tiles_m * f.tiles_q;
+  f.x[0] = b.hi[0]; f.x[1] = b.hi[1]; f.low = b.lo; f.b = b.B;
   CUtensorMap* m = w.map[i];
-  const int64_t n = b.count;
   int rc = 0;
-  auto map = [&](int at, const void* base, int64_t inner, int box_inner, int box_outer) {
-    if (rc == 0) rc = make_map(&m[at], base, true, inner, b.p, n, inner, 0, box_inner, box_outer);
+  auto map = [&](int at, const void* base, int64_t inner, int64_t each, int box_inner, int box_outer) {
+    if (rc == 0) rc = make_map(&m[at], base, true, inner, b.p, b.count, inner, each, box_inner, box_outer);
   };
   for (int k = 0; k < 2; ++k) {
-    map(X_A + k, b.hi[k], b.q, 64, 128);
-    map(X_N + k, b.hi[k], b.q, TN == TILE ? 64 : 32, 64);
-    map(X_BOX + k, b.hi[k], b.q, Layout<TN>::BOX_COLUMNS, 32);
-    if (TN != TILE) map(X_B + k, b.hi[k], b.q, 64, TN / 2);
+    map(X_A + k, b.hi[k], b.q, b.p * b.q, 64, 128);
+    map(X_N + k, b.hi[k], b.q, b.p * b.q, TN == TILE ? 64 : 32, 64);
+    map(X_BOX + k, b.hi[k], b.q, b.p * b.q, 32, 32);
+    map(A_BOX + k, b.hi[k], b.p, b.p * b.q, 32, 32);
+    map(A_A + k, b.hi[k], b.p, b.p * b.q, 64, 128);
+    map(A_T + k, b.hi[k], b.p, b.p * b.q, 64, 64);
+    if (TN != TILE) {
+      map(X_B + k, b.hi[k], b.q, b.p * b.q, 64, TN / 2);
+      map(A_B + k, b.hi[k], b.p, b.p * b.q, 64, TN / 2);
+      map(A_TB + k, b.hi[k], b.p, b.p * b.q, 32, 64);
+    }
   }
-  map(A_A, b.A, b.p, 64, 128);
-  map(B_A, b.B, b.p, 64, 128);
-  map(A_T, b.A, b.p, 64, 64);
-  map(B_T, b.B, b.p, 64, 64);
-  map(A_BOX, b.A, b.p, Layout<TN>::BOX_COLUMNS, 32);
-  map(B_BOX, b.B, b.p, Layout<TN>::BOX_COLUMNS, 32);
-  map(LO_BOX, b.lo, b.q, Layout<TN>::BOX_COLUMNS, 32);
-  if (TN != TILE) {
-    map(A_B, b.A, b.p, 64, TN / 2);
-    map(A_TB, b.A, b.p, 32, 64);
-  }
+  map(B_A, b.B, b.p, b.p * b.p, 64, 128);
+  map(B_T, b.B, b.p, b.p * b.p, 64, 64);
+  map(B_BOX, b.B, b.p, b.p * b.p, 32, 32);
+  map(LO_BOX, b.lo, b.q, b.p * b.q, 32, 32);
   return rc;
 }
 
-// The steps for batches [from, to), as many as a launch's parameters hold; `from` moves on.  done: a counter for every matrix from the first one of batches[from] on, zeros.
+// The steps for batches from `from` on (and in that one from matrix `start` on), as many as a launch's parameters hold; both move on.  done: a counter for every matrix, zeros.
 template <int TN>
 int launch(const std::vector<Batch>& batches, size_t& from, int64_t& start, unsigned long long*& done, int steps, double a, double b, double c, cudaStream_t st) {
   using S = Steps<TN>;
   static thread_local S w;
-  // groups of about one size
+  // halves of about one size
   int64_t total = 0;
   for (size_t i = from; i < batches.size(); ++i) total += bytes_of(batches[i]) * (batches[i].count - (i == from ? start : 0));
-  const int64_t want = std::max<int64_t>(1, (total + GROUP_BYTES - 1) / GROUP_BYTES), limit = (total + want - 1) / want;
-  int shapes = 0, segments = 0, groups = 0, matrices = 0;
+  const int64_t want = 2 * std::max<int64_t>(1, (total + GROUP_BYTES - 1) / GROUP_BYTES), limit = (total + want - 1) / want;
+  int shapes = 0, segments = 0, halves = 0, matrices = 0;
   int64_t tiles = 0, used = 0;
-  bool open = false;
-  auto close = [&] {
-    Group& gr = w.group[groups];
-    tiles += static_cast<int64_t>(steps) * (2ll * gr.symmetric + gr.full);
-    ++groups;
-    open = false;
-  };
-  while (from < batches.size() && shapes < S::SHAPES && groups < S::GROUPS && segments < S::SEGMENTS) {
+  auto half = [&](int i) -> Half& { return w.group[i / 2].half[i % 2]; };
+  bool full = false;
+  half(0) = {0, 0, 0, 0};
+  while (!full && from < batches.size() && shapes < S::SHAPES) {
     const Batch& x = batches[from];
     if (int rc = set_shape(w, shapes, x)) return rc;
     const Info& f = w.info[shapes];
-    bool full = false;
     while (start < x.count) {
-      if (groups >= S::GROUPS || segments >= S::SEGMENTS) { full = true; break; }
-      if (!open) {
-        w.group[groups] = {static_cast<int>(tiles), segments, 0, 0};
+      if (half(halves).end > half(halves).segment && used + bytes_of(x) / 2 > limit) {           // the half has what it should: the next one
+        if (halves + 1 == 2 * S::GROUPS) { full = true; break; }
+        half(++halves) = {segments, segments, 0, 0};
         used = 0;
-        open = true;
       }
-      Group& gr = w.group[groups];
+      if (segments == S::SEGMENTS) { full = true; break; }
+      Half& h = half(halves);
       const int64_t room = std::max<int64_t>(1, (limit - used + bytes_of(x) / 2) / bytes_of(x)), k = std::min(x.count - start, room);
-      const int64_t in_group = static_cast<int64_t>(steps) * (2 * (gr.symmetric + k * f.symmetric) + gr.full + k * f.full);
-      if (tiles + in_group > 0x3FFFFFFF) {
+      tiles += static_cast<int64_t>(steps) * k * (2 * f.symmetric + f.full);
+      if (tiles > 0x3FFFFFFF) {
         if (segments == 0) return fail(HASTE_ERR_TOO_LARGE, "matrices of too many tiles for one launch");
         full = true;
         break;
       }
-      w.segment[segments++] = {shapes, static_cast<int>(start), static_cast<int>(k), matrices, gr.symmetric, gr.full};
-      gr.symmetric += static_cast<int>(k * f.symmetric);
-      gr.full += static_cast<int>(k * f.full);
+      w.segment[segments++] = {shapes, static_cast<int>(start), static_cast<int>(k), matrices, h.symmetric, h.full};
+      h.end = segments;
+      h.symmetric += static_cast<int>(k * f.symmetric);
+      h.full += static_cast<int>(k * f.full);
       used += k * bytes_of(x);
       matrices += static_cast<int>(k);
       start += k;
-      if (used + bytes_of(x) / 2 > limit) close();
     }
     ++shapes;
     if (full) break;
     ++from;
     start = 0;
   }
-  if (open) {
-    if (w.group[groups].symmetric > 0) close();
+  if (halves % 2 == 0) half(halves + 1) = {segments, segments, 0, 0};
+  const int groups = halves / 2 + 1;
+  tiles = 0;
+  for (int i = 0; i < groups; ++i) {
+    w.group[i].first = static_cast<int>(tiles);
+    tiles += tiles_of(w.group[i].half[0], w.group[i].half[1], steps);
   }
-  w.group[groups] = {static_cast<int>(tiles), segments, 0, 0};
   w.groups = groups;
   w.tiles = static_cast<int>(tiles);
   w.steps = steps;
