@@ -4,9 +4,8 @@
 // every warp that has stored its part of a tile adds one to the matrix's counter, and who needs the result waits for the count.  (A launch for each product left a quarter of
 // the SMs without work in the last tiles of 5, and took 3 us and the first loads' latency each time.)
 //
-// The list walks the matrices in groups that fit L2, so that only a group's first and last X pass through memory.  A group has two halves, a and b, whose products alternate so
-// that others stand between a product and the one that needs it:
-//   A of a, half of X of b (of the step before), B of a, the other half, half of X of a, A of b, the other half, B of b, and the next step
+// The list walks the matrices in groups: a group's A tiles, its B tiles, its X tiles, the next step, ..., then the next group.  Groups are large enough that what a tile waits for
+// was begun a product earlier by others (see GROUP_BYTES).
 // Every tile's predecessors stand before it in the list, and a pair works through its part of the list in order, so with all pairs resident (a cooperative launch) the first
 // unfinished tile can always proceed.  Waits are bounded as everywhere.
 //
@@ -42,48 +41,15 @@ struct Info {
   int symmetric, full;                 // tiles of A or B, and of X, in a matrix
   uint16_t *x[2], *low, *b;            // X's buffers (A is in the other one), its lower part, B
 };
-struct Segment {                       // neighbouring matrices of one shape in half a group
+struct Segment {                       // neighbouring matrices of one shape in a group
   int shape, batch, count, matrix;     // first batch entry, how many, number of the first matrix
-  int symmetric0, full0;               // tiles of the half before it
-};
-struct Half {
-  int segment, end, symmetric, full;   // segments; tiles of a product of all of it
+  int symmetric0, full0;               // tiles of the group before it
 };
 struct Group {
   int first;                           // tile number
-  Half half[2];
+  int segment, end;                    // its segments
+  int symmetric, full;                 // tiles of a product of all of it
 };
-// A place in a group's list: which product of which half in which step, and the tile's number there
-struct Place {
-  int half, phase, step, tile;
-};
-__host__ __device__ inline Place place_of(const Half& a, const Half& b, int steps, int t) {
-  const int own = 2 * a.symmetric + a.full + 2 * b.symmetric, period = own + b.full;
-  int step = 0, late = 0;              // tiles of b's X in this period
-  if (t >= own) {
-    step = 1 + (t - own) / period;
-    t -= own + (step - 1) * period;
-    late = b.full;
-    if (step == steps) return {1, 2, steps - 1, t};
-  }
-  const int a1 = a.full / 2, b1 = late / 2;
-  if (t < a.symmetric) return {0, 0, step, t};
-  t -= a.symmetric;
-  if (t < b1) return {1, 2, step - 1, t};
-  t -= b1;
-  if (t < a.symmetric) return {0, 1, step, t};
-  t -= a.symmetric;
-  if (t < late - b1) return {1, 2, step - 1, b1 + t};
-  t -= late - b1;
-  if (t < a1) return {0, 2, step, t};
-  t -= a1;
-  if (t < b.symmetric) return {1, 0, step, t};
-  t -= b.symmetric;
-  if (t < a.full - a1) return {0, 2, step, a1 + t};
-  return {1, 1, step, t - (a.full - a1)};
-}
-__host__ __device__ inline int64_t tiles_of(const Half& a, const Half& b, int steps) { return static_cast<int64_t>(steps) * (2ll * a.symmetric + a.full + 2ll * b.symmetric + b.full); }
-
 template <int TN>
 struct Steps {
   static constexpr int MAPS = TN == TILE ? static_cast<int>(MAPS_WIDE) : static_cast<int>(MAPS_NARROW);
@@ -109,14 +75,15 @@ __device__ __forceinline__ Task task_at(const Steps<TN>& w, int t, int& g) {
   constexpr int PER = TILE / TN;
   while (g + 1 < w.groups && t >= w.group[g + 1].first) ++g;
   const Group& gr = w.group[g];
-  const Place at = place_of(gr.half[0], gr.half[1], w.steps, t - gr.first);
-  const Half& h = gr.half[at.half];
   Task r;
-  t = at.tile;
-  r.phase = at.phase;
-  r.step = at.step;
-  int s = h.segment;
-  while (s + 1 < h.end && t >= (r.phase < 2 ? w.segment[s + 1].symmetric0 : w.segment[s + 1].full0)) ++s;
+  t -= gr.first;
+  const int per = 2 * gr.symmetric + gr.full;
+  r.step = t / per;
+  t -= r.step * per;
+  r.phase = t < gr.symmetric ? 0 : t < 2 * gr.symmetric ? 1 : 2;
+  t -= r.phase * gr.symmetric;
+  int s = gr.segment;
+  while (s + 1 < gr.end && t >= (r.phase < 2 ? w.segment[s + 1].symmetric0 : w.segment[s + 1].full0)) ++s;
   const Segment& sg = w.segment[s];
   const Info& info = w.info[sg.shape];
   t -= r.phase < 2 ? sg.symmetric0 : sg.full0;
@@ -469,12 +436,12 @@ struct Batch {
   int64_t p, q, count;
   uint16_t *hi[2], *lo, *B;
 };
-#ifndef X_GROUP
-#define X_GROUP 160
-#endif
-constexpr int64_t GROUP_BYTES = int64_t(X_GROUP) << 20;
+// What a group's matrices have in their two buffers of X and in B.  Fewer fit L2 (126 MB), but too few tiles for a product let pairs wait for each other: Muon step over 101 M elements, groups of
+// 80, 160, 250, 400 MB: 3057, 3033, 2927, 2952 us; steps over 50 M 1279, 1198, 1214, 1185.  Two halves of a group whose products alternate, so that others stand between a product and the one
+// that needs it, gave nothing there and cost 130 us of 450 with 7 matrices.
+constexpr int64_t GROUP_BYTES = int64_t(250) << 20;
 
-inline int64_t bytes_of(const Batch& b) { return 2 * (2 * b.p * b.q + b.p * b.p); }      // of a matrix, that L2 is to hold: X's lower part just passes
+inline int64_t bytes_of(const Batch& b) { return 2 * (2 * b.p * b.q + b.p * b.p); }      // of a matrix
 
 template <int TN>
 int set_shape(Steps<TN>& w, int i, const Batch& b) {
@@ -516,38 +483,37 @@ template <int TN>
 int launch(const std::vector<Batch>& batches, size_t& from, int64_t& start, unsigned long long*& done, int steps, double a, double b, double c, cudaStream_t st) {
   using S = Steps<TN>;
   static thread_local S w;
-  // halves of about one size
+  // groups of about one size
   int64_t total = 0;
   for (size_t i = from; i < batches.size(); ++i) total += bytes_of(batches[i]) * (batches[i].count - (i == from ? start : 0));
-  const int64_t want = 2 * std::max<int64_t>(1, (total + GROUP_BYTES - 1) / GROUP_BYTES), limit = (total + want - 1) / want;
-  int shapes = 0, segments = 0, halves = 0, matrices = 0;
+  const int64_t want = std::max<int64_t>(1, (total + GROUP_BYTES - 1) / GROUP_BYTES), limit = (total + want - 1) / want;
+  int shapes = 0, segments = 0, groups = 0, matrices = 0;
   int64_t tiles = 0, used = 0;
-  auto half = [&](int i) -> Half& { return w.group[i / 2].half[i % 2]; };
   bool full = false;
-  half(0) = {0, 0, 0, 0};
   while (!full && from < batches.size() && shapes < S::SHAPES) {
     const Batch& x = batches[from];
     if (int rc = set_shape(w, shapes, x)) return rc;
     const Info& f = w.info[shapes];
     while (start < x.count) {
-      if (half(halves).end > half(halves).segment && used + bytes_of(x) / 2 > limit) {           // the half has what it should: the next one
-        if (halves + 1 == 2 * S::GROUPS) { full = true; break; }
-        half(++halves) = {segments, segments, 0, 0};
+      if (groups == 0 || used + bytes_of(x) / 2 > limit) {                     // the group has what it should: the next one
+        if (groups == S::GROUPS || segments == S::SEGMENTS) { full = true; break; }
+        w.group[groups++] = {static_cast<int>(tiles), segments, segments, 0, 0};
         used = 0;
       }
       if (segments == S::SEGMENTS) { full = true; break; }
-      Half& h = half(halves);
+      Group& gr = w.group[groups - 1];
       const int64_t room = std::max<int64_t>(1, (limit - used + bytes_of(x) / 2) / bytes_of(x)), k = std::min(x.count - start, room);
-      tiles += static_cast<int64_t>(steps) * k * (2 * f.symmetric + f.full);
-      if (tiles > 0x3FFFFFFF) {
+      const int64_t more = static_cast<int64_t>(steps) * k * (2 * f.symmetric + f.full);
+      if (tiles + more > 0x3FFFFFFF) {
         if (segments == 0) return fail(HASTE_ERR_TOO_LARGE, "matrices of too many tiles for one launch");
         full = true;
         break;
       }
-      w.segment[segments++] = {shapes, static_cast<int>(start), static_cast<int>(k), matrices, h.symmetric, h.full};
-      h.end = segments;
-      h.symmetric += static_cast<int>(k * f.symmetric);
-      h.full += static_cast<int>(k * f.full);
+      tiles += more;
+      w.segment[segments++] = {shapes, static_cast<int>(start), static_cast<int>(k), matrices, gr.symmetric, gr.full};
+      gr.end = segments;
+      gr.symmetric += static_cast<int>(k * f.symmetric);
+      gr.full += static_cast<int>(k * f.full);
       used += k * bytes_of(x);
       matrices += static_cast<int>(k);
       start += k;
@@ -557,13 +523,7 @@ int launch(const std::vector<Batch>& batches, size_t& from, int64_t& start, unsi
     ++from;
     start = 0;
   }
-  if (halves % 2 == 0) half(halves + 1) = {segments, segments, 0, 0};
-  const int groups = halves / 2 + 1;
-  tiles = 0;
-  for (int i = 0; i < groups; ++i) {
-    w.group[i].first = static_cast<int>(tiles);
-    tiles += tiles_of(w.group[i].half[0], w.group[i].half[1], steps);
-  }
+  if (groups > 0 && w.group[groups - 1].end == w.group[groups - 1].segment) --groups;          // an empty last one
   w.groups = groups;
   w.tiles = static_cast<int>(tiles);
   w.steps = steps;

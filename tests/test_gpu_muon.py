@@ -65,6 +65,28 @@ def test_many_of_one_shape_and_many_shapes():
         _check(a, b, what=f"{tuple(b.shape)}")
 
 
+def test_more_shapes_and_matrices_than_a_launch_holds():
+    """Shapes that differ by their multiples of 64 in each direction, more of them than one launch's parameters, in the wide form and in the narrow one; matrices that fill two
+    groups, and a round of the workspace."""
+    from haste_b200.optim import orthogonalize
+    gen = torch.Generator().manual_seed(51)
+    shapes = [(64 * i + 1, 64 * j + 3) for i in range(7) for j in range(i, 7)]
+    g = [_gradient(s, "gauss", gen).cuda() for s in shapes]
+    for a, b in zip(orthogonalize(g), g):
+        _check(a, b, what=f"{tuple(b.shape)}")
+    g = [_gradient(s, "gauss", gen).cuda() for s in shapes] * 6
+    got = orthogonalize(g)
+    for i in (0, 27, 28, 100, 167):
+        _check(got[i], g[i], what=f"{tuple(g[i].shape)}")
+        assert torch.equal(got[i], got[i % 28])
+    one = [_gradient((1024, 1024), "gauss", gen).cuda() for _ in range(3)]
+    for count in (48, 150):
+        got = orthogonalize([one[i % 3] for i in range(count)])
+        for i in range(3):
+            _check(got[i], one[i])
+        assert all(torch.equal(x, got[i % 3]) for i, x in enumerate(got))
+
+
 def test_scales_zeros_and_what_is_not_finite():
     from haste_b200.optim import orthogonalize
     gen = torch.Generator().manual_seed(6)
