@@ -211,6 +211,7 @@ __global__ void __launch_bounds__(GEMV_THREADS) gated_few_kernel(const __nv_bflo
                                                                  int64_t ldh, float* __restrict__ h, int T, int64_t D, int64_t F) {
   const int lane = threadIdx.x & 31;
   const int64_t f = static_cast<int64_t>(blockIdx.x) * (GEMV_THREADS / 32) + (threadIdx.x >> 5);
+  sm100::grid_launch_dependents();                 // the next launch fetches its weights meanwhile
   if (f >= F) return;
   float g[ROWS], u[ROWS];
 #pragma unroll
@@ -243,30 +244,48 @@ __global__ void __launch_bounds__(GEMV_THREADS) gated_few_kernel(const __nv_bflo
   }
 }
 
-// y[t, o] = sum_f h[t, f] Wd[o, f]: WARPS warps for each o
+// y[t, o] = sum_f h[t, f] Wd[o, f]: `warps` warps for each o.  A lane's first EARLY pieces of the weights are on their way before h is there.
 template <int ROWS, bool VEC>
 __global__ void __launch_bounds__(GEMV_THREADS) down_few_kernel(const float* __restrict__ h, const __nv_bfloat16* __restrict__ wd, __nv_bfloat16* __restrict__ y, int T, int64_t F,
                                                                 int64_t O, int warps) {
+  constexpr int EARLY = 2;
   __shared__ float part[GEMV_THREADS / 32][ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t o = static_cast<int64_t>(blockIdx.x) * (GEMV_THREADS / 32 / warps) + warp / warps;
+  const int64_t o = static_cast<int64_t>(blockIdx.x) * (GEMV_THREADS / 32 / warps) + warp / warps, step = warps * 256;
   const int mine = warp % warps;
-  float s[ROWS];
+  const int64_t first = (mine * 32 + lane) * 8;
+  const __nv_bfloat16* row = wd + o * F;
+  float s[ROWS], early[EARLY][8];
 #pragma unroll
   for (int t = 0; t < ROWS; ++t) s[t] = 0.f;
-  sm100::grid_dependency_wait();
-  if (o < O) {
-#pragma unroll 2
-    for (int64_t i = (mine * 32 + lane) * 8; i < F; i += warps * 256) {
-      float a[8];
-      load8<VEC>(wd + o * F, i, F, a);
 #pragma unroll
-      for (int t = 0; t < ROWS; ++t)
-        if (t < T) {
+  for (int k = 0; k < EARLY; ++k)
+    if (o < O && first + k * step < F) load8<VEC>(row, first + k * step, F, early[k]);
+  sm100::grid_dependency_wait();
+  auto add = [&](const float (&a)[8], int64_t i) {
+#pragma unroll
+    for (int t = 0; t < ROWS; ++t)
+      if (t < T) {
+        if (VEC) {
+          const float4 p = *reinterpret_cast<const float4*>(h + t * F + i), q = *reinterpret_cast<const float4*>(h + t * F + i + 4);
+          s[t] = fmaf(a[0], p.x, fmaf(a[1], p.y, fmaf(a[2], p.z, fmaf(a[3], p.w, s[t]))));
+          s[t] = fmaf(a[4], q.x, fmaf(a[5], q.y, fmaf(a[6], q.z, fmaf(a[7], q.w, s[t]))));
+        } else {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            if (VEC || i + k < F) s[t] = fmaf(a[k], h[t * F + i + k], s[t]);
+            if (i + k < F) s[t] = fmaf(a[k], h[t * F + i + k], s[t]);
         }
+      }
+  };
+  if (o < O) {
+#pragma unroll
+    for (int k = 0; k < EARLY; ++k)
+      if (first + k * step < F) add(early[k], first + k * step);
+#pragma unroll 2
+    for (int64_t i = first + EARLY * step; i < F; i += step) {
+      float a[8];
+      load8<VEC>(row, i, F, a);
+      add(a, i);
     }
   }
 #pragma unroll
@@ -363,10 +382,9 @@ struct Output {
   float* part;
   int splits;
 };
-Output output_of(Arena& arena, void* p, int64_t M, int64_t N, const Form& f, bool always) {
+Output output_of(Arena& arena, void* p, int64_t M, int64_t N, const Form& f) {
   Output o = {p, nullptr, f.splits};
-  if (always || o.splits > 1 || N % 8 != 0 || !aligned16(p))
-    o.part = static_cast<float*>(arena.take(o.splits * M * ((N + 3) & ~int64_t(3)) * 4));
+  if (o.splits > 1) o.part = static_cast<float*>(arena.take(o.splits * M * ((N + 3) & ~int64_t(3)) * 4));
   return o;
 }
 void set_sizes(gemm::Sizes& p, int64_t M, int64_t N, int64_t steps0, int64_t steps) {
@@ -443,7 +461,7 @@ int forward(Arena& arena, const GatedCall& c, cudaStream_t st) {
   const Rows x = align(c.x, c.ldx, c.T, c.D, any), wg = align(c.wg, c.D, c.F, c.D, any), wu = align(c.wu, c.D, c.F, c.D, any), wd = align(c.wd, c.F, c.O, c.F, any);
   void* h = arena.take(c.T * ldF * 2);
   const Form fy = form_for(c.T, c.O, sF);
-  const Output y = output_of(arena, c.y, c.T, c.O, fy, any);
+  const Output y = output_of(arena, c.y, c.T, c.O, fy);
   if (plan) return HASTE_OK;
   HASTE_TRY(align.run(st));
   const bool narrow = gemm::cost_of(gemm::tiles_for(c.T, c.F, 64), sD, true) < gemm::cost_of(gemm::tiles_for(c.T, c.F, 128), sD, false);
@@ -497,8 +515,8 @@ int backward(Arena& arena, const GatedGradCall& c, cudaStream_t st) {
   }
   elements = (c.dwg ? c.F * c.D : 0) + (c.dwu ? c.F * c.D : 0) + (c.dwd ? c.O * c.F : 0);
   const Form fw = choose_form(tiles[0], tiles[1], sT, elements);
-  const Output dx = output_of(arena, c.dx, c.T, c.D, fx, any), dwg = output_of(arena, c.dwg, c.F, c.D, fw, any), dwu = output_of(arena, c.dwu, c.F, c.D, fw, any),
-               dwd = output_of(arena, c.dwd, c.O, c.F, fw, any);
+  const Output dx = output_of(arena, c.dx, c.T, c.D, fx), dwg = output_of(arena, c.dwg, c.F, c.D, fw), dwu = output_of(arena, c.dwu, c.F, c.D, fw),
+               dwd = output_of(arena, c.dwd, c.O, c.F, fw);
   if (plan) return HASTE_OK;
   HASTE_TRY(align.run(st));
   {
