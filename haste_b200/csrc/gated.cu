@@ -382,9 +382,9 @@ struct Output {
   float* part;
   int splits;
 };
-Output output_of(Arena& arena, void* p, int64_t M, int64_t N, const Form& f) {
+Output output_of(Arena& arena, void* p, int64_t M, int64_t N, const Form& f, bool always) {
   Output o = {p, nullptr, f.splits};
-  if (o.splits > 1) o.part = static_cast<float*>(arena.take(o.splits * M * ((N + 3) & ~int64_t(3)) * 4));
+  if (always || o.splits > 1 || N % 8 != 0 || !aligned16(p)) o.part = static_cast<float*>(arena.take(o.splits * M * ((N + 3) & ~int64_t(3)) * 4));
   return o;
 }
 void set_sizes(gemm::Sizes& p, int64_t M, int64_t N, int64_t steps0, int64_t steps) {
@@ -461,7 +461,7 @@ int forward(Arena& arena, const GatedCall& c, cudaStream_t st) {
   const Rows x = align(c.x, c.ldx, c.T, c.D, any), wg = align(c.wg, c.D, c.F, c.D, any), wu = align(c.wu, c.D, c.F, c.D, any), wd = align(c.wd, c.F, c.O, c.F, any);
   void* h = arena.take(c.T * ldF * 2);
   const Form fy = form_for(c.T, c.O, sF);
-  const Output y = output_of(arena, c.y, c.T, c.O, fy);
+  const Output y = output_of(arena, c.y, c.T, c.O, fy, any);
   if (plan) return HASTE_OK;
   HASTE_TRY(align.run(st));
   const bool narrow = gemm::cost_of(gemm::tiles_for(c.T, c.F, 64), sD, true) < gemm::cost_of(gemm::tiles_for(c.T, c.F, 128), sD, false);
@@ -515,8 +515,8 @@ int backward(Arena& arena, const GatedGradCall& c, cudaStream_t st) {
   }
   elements = (c.dwg ? c.F * c.D : 0) + (c.dwu ? c.F * c.D : 0) + (c.dwd ? c.O * c.F : 0);
   const Form fw = choose_form(tiles[0], tiles[1], sT, elements);
-  const Output dx = output_of(arena, c.dx, c.T, c.D, fx), dwg = output_of(arena, c.dwg, c.F, c.D, fw), dwu = output_of(arena, c.dwu, c.F, c.D, fw),
-               dwd = output_of(arena, c.dwd, c.O, c.F, fw);
+  const Output dx = output_of(arena, c.dx, c.T, c.D, fx, any), dwg = output_of(arena, c.dwg, c.F, c.D, fw, any), dwu = output_of(arena, c.dwu, c.F, c.D, fw, any),
+               dwd = output_of(arena, c.dwd, c.O, c.F, fw, any);
   if (plan) return HASTE_OK;
   HASTE_TRY(align.run(st));
   {

@@ -106,7 +106,8 @@ struct Sizes {
   int steps0, steps;               // steps of k in the first part, and in both
   int first;                       // number of this problem's first tile; set by launch()
 };
-// A 16-bit matrix of the result's size that the policy reads or writes: rows of ld elements.  on: the bytes that base and rows are multiples of, 32, 16 or 2 (results alone)
+// A 16-bit matrix of the result's size that the policy reads or writes: rows of ld elements.  on: the bytes that base and rows are multiples of, 32 or 16 (with a
+// third form for any, every lane storing its row's values one by one, the weights' gradients of 333 x 509 x 1021 took 43 us, through fp32 parts 14 and 6)
 struct Matrix16 {
   uint16_t* p;
   int64_t ld;
@@ -168,14 +169,10 @@ __device__ __forceinline__ void store_row(const Matrix16& m, int row, int col, c
 #pragma unroll
     for (int j = 0; j < 2; ++j)
       if (col + 16 * j < m.ld) store_32_bytes(to + 16 * j, v + 8 * j);
-  } else if (m.on == 16) {
+  } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (col + 8 * j < m.ld) *reinterpret_cast<uint4*>(to + 8 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (col + j < m.ld) to[j] = static_cast<uint16_t>(j & 1 ? v[j >> 1] >> 16 : v[j >> 1]);
   }
 }
 // and zeros beyond it
@@ -379,8 +376,7 @@ int map_b(CUtensorMap* out, const Operand& o, int64_t rows, int64_t k) {
                       : make_map(out, o.p, Policy::F16, k, rows, 1, o.ld, 0, 64, TN / 2);
 }
 inline Matrix16 result(const Operand& o) {
-  const auto at = reinterpret_cast<uintptr_t>(o.p);
-  return {static_cast<uint16_t*>(const_cast<void*>(o.p)), o.ld, o.ld % 16 == 0 && at % 32 == 0 ? 32 : o.ld % 8 == 0 && at % 16 == 0 ? 16 : 2};
+  return {static_cast<uint16_t*>(const_cast<void*>(o.p)), o.ld, o.ld % 16 == 0 && reinterpret_cast<uintptr_t>(o.p) % 32 == 0 ? 32 : 16};
 }
 inline int64_t steps_of(int64_t k) { return (k + KSTEP - 1) / KSTEP; }
 
