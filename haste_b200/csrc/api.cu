@@ -706,15 +706,8 @@ int64_t haste_gated_backward_scratch(int64_t T, int64_t D, int64_t F, int64_t O,
   if (check_gated("haste_gated_backward_scratch", T, D, F, O) != HASTE_OK || T == 0) return 0;
   GatedGradCall c = {};
   c.T = T; c.D = D; c.F = F; c.O = O; c.aligned = aligned != 0 && (D | F | O) % 8 == 0;
-  void* some_place = reinterpret_cast<void*>(static_cast<uintptr_t>(256));
-  c.dx = some_place;
-  int64_t most = 0;
-  for (int some = 0; some < 8; ++some) {           // which are wanted decides how the products are cut
-    c.dwg = some & 1 ? some_place : nullptr; c.dwu = some & 2 ? some_place : nullptr; c.dwd = some & 4 ? some_place : nullptr;
-    const int64_t n = gated_backward_scratch(c);
-    if (n > most) most = n;
-  }
-  return most;
+  c.dx = c.dwg = c.dwu = c.dwd = reinterpret_cast<void*>(static_cast<uintptr_t>(256));         // all of them, aligned
+  return gated_backward_scratch(c);
 }
 
 int haste_gated_backward(const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* gate, const void* up, void* dx, void* dwg, void* dwu, void* dwd,

@@ -13,6 +13,8 @@
 
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 namespace haste {
 namespace {
 
@@ -596,9 +598,17 @@ int64_t embedding_backward_scratch(int64_t tokens, int64_t D, int64_t V) {
 template <int ITEMS>
 static int sort_in_cluster(const Ids& ids, int64_t tokens, int64_t V, int64_t padding, int2* out, cudaStream_t st) {
   auto kernel = sort_cluster_kernel<ITEMS>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, cluster_smem<ITEMS>());
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  static std::atomic<bool> allowed[64];            // by device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const bool keep = dev >= 0 && dev < 64;
+  cudaError_t e = cudaSuccess;
+  if (!keep || !allowed[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, cluster_smem<ITEMS>());
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    if (keep) allowed[dev].store(true, std::memory_order_release);
+  }
   unsigned blocks = 1;
   while (static_cast<int64_t>(blocks) * CLUSTER_THREADS * ITEMS < tokens) blocks *= 2;
   cudaLaunchConfig_t cfg = {};

@@ -365,11 +365,12 @@ struct Form {
   int splits;
 };
 Form choose_form(int64_t wide, int64_t narrow, int64_t steps, int64_t elements) {
+  const int64_t pairs = sm_count() / 2;
   Form best = {false, 1};
   double cost = 0;
   for (int s = 1; s <= 16 && s <= steps; ++s)
     for (int n = 0; n < 2; ++n) {
-      const double c = gemm::cost_of((n ? narrow : wide) * s, (steps + s - 1) / s, n != 0) + (s > 1 ? 7 + static_cast<double>(elements) * s * 8 / 6e6 / 0.28 : 0);
+      const double c = gemm::cost_of((n ? narrow : wide) * s, (steps + s - 1) / s, n != 0, pairs) + (s > 1 ? 7 + static_cast<double>(elements) * s * 8 / 6e6 / 0.28 : 0);
       if ((s == 1 && n == 0) || c < cost) { best = {n != 0, s}; cost = c; }
     }
   return best;
@@ -464,7 +465,8 @@ int forward(Arena& arena, const GatedCall& c, cudaStream_t st) {
   const Output y = output_of(arena, c.y, c.T, c.O, fy, any);
   if (plan) return HASTE_OK;
   HASTE_TRY(align.run(st));
-  const bool narrow = gemm::cost_of(gemm::tiles_for(c.T, c.F, 64), sD, true) < gemm::cost_of(gemm::tiles_for(c.T, c.F, 128), sD, false);
+  const int64_t pairs = sm_count() / 2;
+  const bool narrow = gemm::cost_of(gemm::tiles_for(c.T, c.F, 64), sD, true, pairs) < gemm::cost_of(gemm::tiles_for(c.T, c.F, 128), sD, false, pairs);
   HASTE_TRY(by_activation<GatedForward>(c.act, narrow, [&](auto policy, auto columns) -> int {
     using K = decltype(policy);
     constexpr int TN = decltype(columns)::value;
@@ -508,19 +510,16 @@ int backward(Arena& arena, const GatedGradCall& c, cudaStream_t st) {
              wd = align(c.wd, c.F, c.O, c.F, any), gate = align(c.gate, c.ldgate, c.T, c.F, any), up = align(c.up, c.ldup, c.T, c.F, any);
   void *dgate = arena.take(c.T * ldF * 2), *dup = arena.take(c.T * ldF * 2), *h = arena.take(c.T * ldF * 2);
   const Form fx = form_for(c.T, c.D, 2 * sF);
-  int64_t tiles[2], elements = 0;
-  for (int n = 0; n < 2; ++n) {
-    const int64_t t = gemm::tiles_for(c.F, c.D, n ? 64 : 256);
-    tiles[n] = (c.dwg ? t : 0) + (c.dwu ? t : 0) + (c.dwd ? gemm::tiles_for(c.O, c.F, n ? 64 : 256) : 0);
-  }
-  elements = (c.dwg ? c.F * c.D : 0) + (c.dwu ? c.F * c.D : 0) + (c.dwd ? c.O * c.F : 0);
-  const Form fw = choose_form(tiles[0], tiles[1], sT, elements);
+  int64_t tiles[2];                                // of all three, whichever are wanted: a gradient's bits do not depend on that
+  for (int n = 0; n < 2; ++n) tiles[n] = 2 * gemm::tiles_for(c.F, c.D, n ? 64 : 256) + gemm::tiles_for(c.O, c.F, n ? 64 : 256);
+  const Form fw = choose_form(tiles[0], tiles[1], sT, 2 * c.F * c.D + c.O * c.F);
   const Output dx = output_of(arena, c.dx, c.T, c.D, fx, any), dwg = output_of(arena, c.dwg, c.F, c.D, fw, any), dwu = output_of(arena, c.dwu, c.F, c.D, fw, any),
                dwd = output_of(arena, c.dwd, c.O, c.F, fw, any);
   if (plan) return HASTE_OK;
   HASTE_TRY(align.run(st));
   {
-    const bool narrow = gemm::cost_of(gemm::tiles_for(c.T, c.F, 64), sO, true) < gemm::cost_of(gemm::tiles_for(c.T, c.F, 256), sO, false);
+    const int64_t pairs = sm_count() / 2;
+    const bool narrow = gemm::cost_of(gemm::tiles_for(c.T, c.F, 64), sO, true, pairs) < gemm::cost_of(gemm::tiles_for(c.T, c.F, 256), sO, false, pairs);
     HASTE_TRY(by_activation<GatedBackward>(c.act, narrow, [&](auto policy, auto columns) -> int {
       using K = decltype(policy);
       constexpr int TN = decltype(columns)::value;
@@ -556,7 +555,7 @@ int backward(Arena& arena, const GatedGradCall& c, cudaStream_t st) {
     add_sum(s, dx, c.T, c.D);
     HASTE_TRY(run_sums(s, st));
   }
-  if (tiles[0] == 0) return HASTE_OK;
+  if (c.dwg == nullptr && c.dwu == nullptr && c.dwd == nullptr) return HASTE_OK;
   Sums s = {};
   HASTE_TRY(by_form<Plain<true, true>>(fw.narrow, [&](auto policy, auto columns) -> int {
     using K = decltype(policy);

@@ -380,13 +380,16 @@ inline Matrix16 result(const Operand& o) {
 }
 inline int64_t steps_of(int64_t k) { return (k + KSTEP - 1) / KSTEP; }
 
-// Pairs of CTAs that may run at once on the current device
-template <class K>
-int pairs_resident(K kernel, int smem) {
+// Pairs of CTAs that may run at once on the current device.  The first call on a device allows the kernel its shared memory there, which its launches need.
+template <auto KERNEL>                 // (the address: kernels of one type have their own)
+int pairs_resident(int smem, int* pairs) {
   static std::atomic<int> cached[64];
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && cached[dev].load(std::memory_order_relaxed) > 0) return cached[dev].load(std::memory_order_relaxed);
+  const bool keep = dev >= 0 && dev < 64;
+  if (keep && (*pairs = cached[dev].load(std::memory_order_acquire)) > 0) return HASTE_OK;
+  const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(sm_count() & ~1));
   cfg.blockDim = dim3(THREADS);
@@ -398,18 +401,18 @@ int pairs_resident(K kernel, int smem) {
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+  if (cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess || n < 1) {
     cudaGetLastError();
-    return sm_count() / 2;
+    *pairs = sm_count() / 2;
+    return HASTE_OK;
   }
-  if (n > sm_count() / 2) n = sm_count() / 2;      // one CTA to an SM, also where two would fit
-  if (dev >= 0 && dev < 64) cached[dev].store(n, std::memory_order_relaxed);
-  return n;
+  *pairs = n < sm_count() / 2 ? n : sm_count() / 2;
+  if (keep) cached[dev].store(*pairs, std::memory_order_release);
+  return HASTE_OK;
 }
 
 // Time of a launch of `tiles` tiles of `steps` steps of k each, in units of a step of the wide form (0.28 us)
-inline double cost_of(int64_t tiles, int64_t steps, bool is_narrow) {
-  const int64_t pairs = sm_count() / 2;
+inline double cost_of(int64_t tiles, int64_t steps, bool is_narrow, int64_t pairs) {
   return static_cast<double>((tiles + pairs - 1) / pairs) * (is_narrow ? 0.6 * static_cast<double>(steps) + 3.5 : static_cast<double>(steps) + 6.0);
 }
 inline int64_t tiles_for(int64_t M, int64_t N, int64_t columns) { return ((M + TILE - 1) / TILE) * ((N + columns - 1) / columns); }
@@ -419,9 +422,7 @@ template <class Policy, int TN, int P>
 int launch(Work<Policy, P>& w, bool behind, cudaStream_t st) {
   using L = Layout<TN>;
   constexpr int COLUMNS = Policy::PAIRED_B ? TN / 2 : TN;
-  auto kernel = gemm_sm100_kernel<Policy, P, TN>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM_BYTES);
-  if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  constexpr auto kernel = &gemm_sm100_kernel<Policy, P, TN>;
   int64_t tiles = 0;
   for (int i = 0; i < w.problems; ++i) {
     Sizes& p = w.p[i];
@@ -436,7 +437,9 @@ int launch(Work<Policy, P>& w, bool behind, cudaStream_t st) {
   w.tiles = static_cast<int>(tiles);
   if (int rc = device_status_word(&w.err)) return rc;
   w.wait_limit = wait_limit_cycles();
-  const int pairs = static_cast<int>(imin64(pairs_resident(kernel, L::SMEM_BYTES), tiles));
+  int pairs = 0;
+  if (int rc = pairs_resident<kernel>(L::SMEM_BYTES, &pairs)) return rc;
+  pairs = static_cast<int>(imin64(pairs, tiles));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
   cfg.blockDim = dim3(THREADS);
@@ -447,7 +450,7 @@ int launch(Work<Policy, P>& w, bool behind, cudaStream_t st) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = behind ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, kernel, w);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, w);
   if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaLaunchKernelEx: %s", cudaGetErrorString(e));
   return HASTE_OK;
 }

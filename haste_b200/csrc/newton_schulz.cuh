@@ -533,10 +533,10 @@ int launch(const std::vector<Batch>& batches, size_t& from, int64_t& start, unsi
   if (tiles == 0) return HASTE_OK;
   if (int rc = device_status_word(&w.err)) return rc;
   w.wait_limit = wait_limit_cycles();
-  auto kernel = newton_schulz_kernel<TN>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<TN>::SMEM_BYTES);
-  if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  const int pairs = static_cast<int>(imin64(gemm::pairs_resident(kernel, Layout<TN>::SMEM_BYTES), tiles));
+  constexpr auto kernel = &newton_schulz_kernel<TN>;
+  int pairs = 0;
+  if (int rc = gemm::pairs_resident<kernel>(Layout<TN>::SMEM_BYTES, &pairs)) return rc;
+  pairs = static_cast<int>(imin64(pairs, tiles));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
   cfg.blockDim = dim3(THREADS);
@@ -547,7 +547,7 @@ int launch(const std::vector<Batch>& batches, size_t& from, int64_t& start, unsi
   attr.val.cooperative = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, w);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, w);
   if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaLaunchKernelEx: %s", cudaGetErrorString(e));
   return HASTE_OK;
 }
@@ -560,8 +560,8 @@ inline bool take_narrow(const std::vector<Batch>& batches) {
     for (int n = 0; n < 2; ++n) tiles[n] += b.count * gemm::tiles_for(b.p, b.q, n ? 64 : TILE);
     work += b.count * gemm::tiles_for(b.p, b.q, TILE) * gemm::steps_of(b.p);
   }
-  const int64_t groups = std::max<int64_t>(1, (total + GROUP_BYTES - 1) / GROUP_BYTES), per = (work + tiles[0] - 1) / tiles[0];
-  return gemm::cost_of(tiles[1] / groups, per, true) < gemm::cost_of(tiles[0] / groups, per, false);
+  const int64_t groups = std::max<int64_t>(1, (total + GROUP_BYTES - 1) / GROUP_BYTES), per = (work + tiles[0] - 1) / tiles[0], pairs = sm_count() / 2;
+  return gemm::cost_of(tiles[1] / groups, per, true, pairs) < gemm::cost_of(tiles[0] / groups, per, false, pairs);
 }
 
 inline int run(const std::vector<Batch>& batches, unsigned long long* done, int steps, double a, double b, double c, cudaStream_t st) {
