@@ -6,6 +6,7 @@
 #include "runtime.h"
 
 #include <atomic>
+#include <exception>
 
 namespace haste {
 
@@ -622,7 +623,7 @@ int haste_dequantize_moment(const uint8_t* codes, const float* scales, void* out
 static int check_embedding(const char* who, int32_t id_bytes, int64_t tokens, int64_t D, int64_t V) {
   if (id_bytes != 4 && id_bytes != 8) return fail(HASTE_ERR_UNSUPPORTED, "%s: ids of %d bytes", who, id_bytes);
   if (tokens < 0 || D < 1 || V < 1) return fail(HASTE_ERR_BAD_ARG, "%s: tokens=%lld, D=%lld, V=%lld", who, (long long)tokens, (long long)D, (long long)V);
-  if (tokens > (1ll << 40) || D > (1ll << 24) || V > (1ll << 40)) return fail(HASTE_ERR_TOO_LARGE, "%s: tokens=%lld, D=%lld, V=%lld", who, (long long)tokens, (long long)D, (long long)V);
+  if (tokens > (1ll << 40) || D > (1ll << 24) || V > (1ll << 40) || tokens > (1ll << 40) / D) return fail(HASTE_ERR_TOO_LARGE, "%s: tokens=%lld, D=%lld, V=%lld", who, (long long)tokens, (long long)D, (long long)V);
   return HASTE_OK;
 }
 
@@ -755,10 +756,20 @@ static int check_polynomial(const char* who, int32_t steps, double a, double b, 
   return HASTE_OK;
 }
 
+// f(), whose lists of matrices may not fit the host's memory
+static const auto with_lists = [](const char* who, auto&& f) -> int {
+  try {
+    return f();
+  } catch (const std::exception& e) {
+    return fail(HASTE_ERR_TOO_LARGE, "%s: %s", who, e.what());
+  }
+};
+
 int64_t haste_muon_scratch(const int64_t* rows, const int64_t* cols, int64_t count) {
-  int64_t moments = 0;
+  int64_t moments = 0, bytes = 0;
   if (check_matrices("haste_muon_scratch", nullptr, rows, cols, count, &moments) != HASTE_OK) return 0;
-  return muon_scratch(rows, cols, count);
+  with_lists("haste_muon_scratch", [&] { bytes = muon_scratch(rows, cols, count); return HASTE_OK; });
+  return bytes;
 }
 
 int haste_muon_step(void* const* params, const void* const* grads, const int64_t* rows, const int64_t* cols, int64_t count, float* momentum, int64_t moments, int32_t p_type,
@@ -778,9 +789,11 @@ int haste_muon_step(void* const* params, const void* const* grads, const int64_t
   if (moments < need) return fail(HASTE_ERR_BAD_ARG, "%s: momentum of %lld elements, %lld needed", who, (long long)moments, (long long)need);
   for (int64_t i = 0; i < count; ++i)
     if (rows[i] > 0 && cols[i] > 0 && params[i] == nullptr && grads[i] != nullptr) return fail(HASTE_ERR_BAD_ARG, "%s: parameter %lld is NULL", who, (long long)i);
-  if (int rc = check_scratch(who, scratch, scratch_bytes, muon_scratch(rows, cols, count))) return rc;
-  return launch_muon({who, params, grads, rows, cols, count, momentum, true, p_type, g_type, lr, mu, weight_decay, nesterov, adjust, steps, a, b, c, eps, step, seed, stream_index, flags,
-                      scratch}, static_cast<cudaStream_t>(stream));
+  return with_lists(who, [&]() -> int {
+    if (int rc = check_scratch(who, scratch, scratch_bytes, muon_scratch(rows, cols, count))) return rc;
+    return launch_muon({who, params, grads, rows, cols, count, momentum, true, p_type, g_type, lr, mu, weight_decay, nesterov, adjust, steps, a, b, c, eps, step, seed, stream_index, flags,
+                        scratch}, static_cast<cudaStream_t>(stream));
+  });
 }
 
 int haste_orthogonalize(const void* const* in, void* const* out, const int64_t* rows, const int64_t* cols, int64_t count, int32_t in_type, int32_t steps, double a, double b, double c,
@@ -794,9 +807,11 @@ int haste_orthogonalize(const void* const* in, void* const* out, const int64_t* 
   REQUIRE_PTR(in, who); REQUIRE_PTR(out, who);
   for (int64_t i = 0; i < count; ++i)
     if (rows[i] > 0 && cols[i] > 0 && (in[i] == nullptr || out[i] == nullptr)) return fail(HASTE_ERR_BAD_ARG, "%s: matrix %lld is NULL", who, (long long)i);
-  if (int rc = check_scratch(who, scratch, scratch_bytes, muon_scratch(rows, cols, count))) return rc;
-  return launch_muon({who, out, in, rows, cols, count, nullptr, false, HASTE_BF16, in_type, 0, 0, 0, 0, HASTE_MUON_ORIGINAL, steps, a, b, c, eps, 1, 0, 0, 0, scratch},
-                     static_cast<cudaStream_t>(stream));
+  return with_lists(who, [&]() -> int {
+    if (int rc = check_scratch(who, scratch, scratch_bytes, muon_scratch(rows, cols, count))) return rc;
+    return launch_muon({who, out, in, rows, cols, count, nullptr, false, HASTE_BF16, in_type, 0, 0, 0, 0, HASTE_MUON_ORIGINAL, steps, a, b, c, eps, 1, 0, 0, 0, scratch},
+                       static_cast<cudaStream_t>(stream));
+  });
 }
 
 }  // extern "C"

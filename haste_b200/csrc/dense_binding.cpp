@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
 #include <stdexcept>
 #include <string>
 #include <tuple>
@@ -619,6 +620,11 @@ PyObject* muon_step(PyObject* const* a) {
     }
     if (!fine) refuse("all parameters must have one type, all gradients one type, and every gradient its parameter's shape");
   }
+  std::vector<const void*> once;
+  for (int64_t i = 0; i < params.size(); ++i)
+    if (p.p[i] != nullptr && p.sizes[i] > 0 && grads[i] != Py_None) once.push_back(p.p[i]);
+  std::sort(once.begin(), once.end());
+  if (std::adjacent_find(once.begin(), once.end()) != once.end()) refuse("a parameter stands in the list twice");
   const at::Tensor& m = tensor(a[2], "momentum_buffer");
   if (gpu_of(m) != p.dev || m.scalar_type() != at::kFloat || !m.is_contiguous()) refuse("momentum_buffer must be a contiguous fp32 tensor on the parameters' device");
   int64_t bytes = 0;

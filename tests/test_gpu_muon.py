@@ -195,7 +195,7 @@ def test_refusals():
                  lambda: orthogonalize([a, None]), lambda: orthogonalize([a], 0), lambda: orthogonalize([a], eps=0.0), lambda: orthogonalize([a], 5, (float("nan"), 0.0, 0.0)),
                  lambda: muon_step([a], [b, b], m, step=1), lambda: muon_step([a], [b[:2]], m, step=1), lambda: muon_step([a], [b], m[:100], step=1), lambda: muon_step([a], [b], m.cpu(), step=1),
                  lambda: muon_step([a], [b], m, step=0), lambda: muon_step([a], [b], m, step=1, lr=-1.0), lambda: muon_step([a], [b], m, step=1, momentum=1.0),
-                 lambda: muon_step([a], [b], m, step=1, adjust="rms"), lambda: muon_step([a.view(-1)], [b.view(-1)], m, step=1), lambda: muon_step([a], [b], m.to(BF), step=1)):
+                 lambda: muon_step([a], [b], m, step=1, adjust="rms"), lambda: muon_step([a, a], [b, b], torch.zeros(512, device="cuda"), step=1), lambda: muon_step([a.view(-1)], [b.view(-1)], m, step=1), lambda: muon_step([a], [b], m.to(BF), step=1)):
         with pytest.raises(RuntimeError):
             call()
     muon_step([a], [None], m, step=1)
