@@ -54,6 +54,7 @@ struct Coefficients {
   float mu, one_mu, decay, eps;
   int nesterov, sr;
   uint32_t seed, step, stream;
+  unsigned long long* drawn;       // the steps' numbers
 };
 // The last matrix that begins at `block` or before (a walk over all of them took longer than the work: every step a miss in the constants' cache)
 __device__ __forceinline__ int matrix_of(const int* first, int n, int block) {
@@ -233,6 +234,7 @@ __global__ void __launch_bounds__(256) muon_start_kernel(const __grid_constant__
   Walk<N> walk(t);
   const int cg = (threadIdx.x & 15) * 4, r0 = threadIdx.x / 16;
   sm100::grid_dependency_wait();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *c.drawn = 0;
   float inv = walk.more() ? inverse_norm(t.a[walk.k], c.eps) : 0.f;
   while (walk.more()) {
     const Matrix& a = t.a[walk.k];
@@ -492,7 +494,8 @@ int launch_muon(const MuonCall& c, cudaStream_t st) {
     char* mem = static_cast<char*>(c.scratch);
     auto take = [&](int64_t bytes) { char* p = mem; mem += up256(bytes); return p; };
     const int64_t n = static_cast<int64_t>(plan.rounds[r + 1] - plan.rounds[r]);
-    auto* done = reinterpret_cast<unsigned long long*>(take(8 * n));
+    auto* done = reinterpret_cast<unsigned long long*>(take(8 * (n + 1)));
+    k.drawn = done + n;
     auto* parts = reinterpret_cast<double*>(take(8 * NORM_PARTS * n));
     int64_t elements = 0;
     for (size_t i = plan.rounds[r]; i < plan.rounds[r + 1]; ++i) elements += c.rows[plan.order[i]] * c.cols[plan.order[i]];
@@ -535,7 +538,7 @@ int launch_muon(const MuonCall& c, cudaStream_t st) {
       return gb ? launch_behind(muon_start_kernel<__nv_bfloat16, N>, tiles, 256, st, t, k) : launch_behind(muon_start_kernel<float, N>, tiles, 256, st, t, k);
     });
     if (rc) return rc;
-    rc = newton_schulz::run(batches, done, c.steps, c.a, c.b, c.c, st);
+    rc = newton_schulz::run(batches, done, k.drawn, c.steps, c.a, c.b, c.c, st);
     if (rc) return rc;
     if (c.steps & 1) {                 // X is in the other buffer
       size_t k = 0;

@@ -6,8 +6,9 @@
 //
 // The list walks the matrices in groups: a group's A tiles, its B tiles, its X tiles, the next step, ..., then the next group.  Groups are large enough that what a tile waits for
 // was begun a product earlier by others (see GROUP_BYTES).
-// Every tile's predecessors stand before it in the list, and a pair works through its part of the list in order, so with all pairs resident (a cooperative launch) the first
-// unfinished tile can always proceed.  Waits are bounded as everywhere.
+// Every tile's predecessors stand before it in the list, a pair draws the next tile's number from a counter when it runs, and it works on its tiles in that order: the first unfinished
+// tile is with a pair that runs and has nothing before it, so it can always proceed, however many pairs the launch has got (it is a cooperative one besides).  Waits
+// are bounded as everywhere.
 //
 // A and B are symmetric: only tiles on and below the diagonal are computed and stored.  Where an operand's block lies above it, the block on the other side is loaded and
 // read by the tensor core with its rows and columns exchanged.
@@ -61,6 +62,8 @@ struct Steps {
   int groups, tiles, steps;
   float a, b, c;
   unsigned long long* done;            // by matrix
+  unsigned long long* drawn;           // numbers of tiles, from `base` on
+  unsigned long long base;
   int* err;
   long long wait_limit;
 };
@@ -160,6 +163,20 @@ __device__ __forceinline__ void add_count(unsigned long long* p) {
   asm volatile("red.release.gpu.global.add.u64 [%0], %1;" ::"l"(p), "l"(1ull) : "memory");
 }
 
+// The next tile's number
+template <int TN>
+__device__ __forceinline__ int draw(const Steps<TN>& w) {
+  const unsigned long long n = atomicAdd(w.drawn, 1ull) - w.base;
+  return n < static_cast<unsigned long long>(w.tiles) ? static_cast<int>(n) : w.tiles;
+}
+// A number into the odd CTA's shared memory, where its arrival counts at a barrier
+__device__ __forceinline__ void send(uint32_t to, int value, uint32_t bar) {
+  uint32_t there, bar_there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 1;" : "=r"(there) : "r"(to));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 1;" : "=r"(bar_there) : "r"(bar));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];" ::"r"(there), "r"(value), "r"(bar_there) : "memory");
+}
+
 // ---------------------------------------------------------------- the kernel
 template <int TN>
 struct Layout {
@@ -167,8 +184,9 @@ struct Layout {
   static constexpr int TASKS = 4, CHUNKS = TN / 64, BOXES = 2, EPI_BYTES = EPI_WARPS * BOXES * BOX_BYTES, STAGES = (224 * 1024 - EPI_BYTES) / STAGE_BYTES;
   static constexpr int OFF_EPI = STAGES * STAGE_BYTES;
   static constexpr int OFF_TASK = OFF_EPI + EPI_BYTES;
-  static constexpr int OFF_BAR = OFF_TASK + TASKS * 64;
-  static constexpr int BARRIERS = 2 * STAGES + 4 + 2 * TASKS;
+  static constexpr int OFF_MAIL = OFF_TASK + TASKS * 64;
+  static constexpr int OFF_BAR = OFF_MAIL + TASKS * 8;
+  static constexpr int BARRIERS = 2 * STAGES + 4 + 4 * TASKS;
   static constexpr int SMEM_BYTES = OFF_BAR + 8 * BARRIERS + 16 + 1024;
   static_assert(SMEM_BYTES <= 227 * 1024 && sizeof(Task) <= 64, "shared memory");
 };
@@ -189,6 +207,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) newton_s
   auto bar_free = [&](int s) { return base + L::OFF_BAR + 8 * (2 * STAGES + 2 + s); };
   auto bar_task = [&](int s) { return base + L::OFF_BAR + 8 * (2 * STAGES + 4 + s); };
   auto bar_slot = [&](int s) { return base + L::OFF_BAR + 8 * (2 * STAGES + 4 + TASKS + s); };
+  auto bar_mail = [&](int s) { return base + L::OFF_BAR + 8 * (2 * STAGES + 4 + 2 * TASKS + s); };         // in the odd CTA: a number has come
+  auto bar_read = [&](int s) { return base + L::OFF_BAR + 8 * (2 * STAGES + 4 + 3 * TASKS + s); };         // in the even one: it has been read there
   auto slot_of = [&](int n) -> volatile Task& { return *reinterpret_cast<volatile Task*>(sm + L::OFF_TASK + (n % TASKS) * 64); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + L::OFF_BAR + 8 * L::BARRIERS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::OFF_BAR + 8 * L::BARRIERS + 8);
@@ -198,7 +218,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) newton_s
     for (int s = 0; s < STAGES; ++s) { mbar_init(bar_full(s), 2); mbar_init(bar_empty(s), 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(bar_done(s), 1); mbar_init(bar_free(s), 2 * EPI_WARPS); }
     // read by the warps for loads, products (in the even CTA) and the epilogue
-    for (int s = 0; s < TASKS; ++s) { mbar_init(bar_task(s), 1); mbar_init(bar_slot(s), EPI_WARPS + (rank == 0 ? 3 : 2)); }
+    for (int s = 0; s < TASKS; ++s) { mbar_init(bar_task(s), 1); mbar_init(bar_slot(s), EPI_WARPS + (rank == 0 ? 3 : 2)); mbar_init(bar_mail(s), 1); mbar_init(bar_read(s), 1); }
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -209,15 +229,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) newton_s
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
-  const int mine = w.tiles > first ? (w.tiles - first + stride - 1) / stride : 0;          // tiles of this pair
-  // The n-th of them, when it may be worked on; by one thread, or by a warp with every = true
+  // The n-th tile of this pair, when it may be worked on, by one thread, or by a warp with every = true; false after the last one
   auto take = [&](int n, bool every, Task& k) -> bool {
     bool ok = mbar_wait(bar_task(n % TASKS), (n / TASKS) & 1, abort_flag, w.err, 329, WL);
     if (every) ok = __all_sync(0xffffffffu, ok);
     if (!ok) return false;
     volatile Task& s = slot_of(n);
-    k.shape = s.shape; k.batch = s.batch; k.matrix = s.matrix; k.m = s.m; k.n = s.n; k.phase = s.phase; k.step = s.step;
+    k.shape = s.shape;
+    if (k.shape < 0) return false;
+    k.batch = s.batch; k.matrix = s.matrix; k.m = s.m; k.n = s.n; k.phase = s.phase; k.step = s.step;
     if (every) __syncwarp();
     if (!every || lane == 0) mbar_arrive(bar_slot(n % TASKS));
     return true;
@@ -227,20 +247,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) newton_s
 
   if (warp == 3 && lane == 0) {
     // ---------------- what comes next
-    int g = 0;
-    for (int n = 0; n < mine; ++n) {
-      const Task k = task_at(w, first + n * stride, g);
-      if (!mbar_wait(bar_slot(n % TASKS), ((n / TASKS) & 1) ^ 1, abort_flag, w.err, 320, WL)) break;
-      if (!wait_count(w.done + k.matrix, k.need, abort_flag, w.err, 321, WL)) break;
+    int g = 0, next = rank == 0 ? draw(w) : 0;
+    for (int n = 0;; ++n) {
+      const int slot = n % TASKS, parity = (n / TASKS) & 1;
+      int t = next;
+      if (rank == 0) {                                 // draws for both, one ahead
+        if (t < w.tiles) next = draw(w);
+        if (!mbar_wait(bar_read(slot), parity ^ 1, abort_flag, w.err, 330, WL)) break;
+        send(base + L::OFF_MAIL + 8 * slot, t, bar_mail(slot));
+      } else {
+        mbar_arrive_expect_tx(bar_mail(slot), 4);
+        if (!mbar_wait(bar_mail(slot), parity, abort_flag, w.err, 331, WL)) break;
+        t = *reinterpret_cast<volatile int*>(sm + L::OFF_MAIL + 8 * slot);
+        gemm::arrive_at_leader(bar_read(slot));
+      }
+      if (!mbar_wait(bar_slot(slot), parity ^ 1, abort_flag, w.err, 320, WL)) break;
       volatile Task& s = slot_of(n);
+      if (t >= w.tiles) {
+        s.shape = -1;
+        mbar_arrive(bar_task(slot));
+        break;
+      }
+      const Task k = task_at(w, t, g);
+      if (!wait_count(w.done + k.matrix, k.need, abort_flag, w.err, 321, WL)) break;
       s.shape = k.shape; s.batch = k.batch; s.matrix = k.matrix; s.m = k.m; s.n = k.n; s.phase = k.phase; s.step = k.step;
-      mbar_arrive(bar_task(n % TASKS));
+      mbar_arrive(bar_task(slot));
     }
   } else if ((warp == 0 || warp == 2) && lane == 0) {
     // ---------------- loads: of operand a by warp 0, of b by warp 2 (one thread's instructions for both took longer than the narrow form's products)
     int it = 0;
     Task k;
-    for (int n = 0; n < mine && take(n, false, k); ++n) {
+    for (int n = 0; take(n, false, k); ++n) {
       fence_proxy_async_all();
       const Info& info = w.info[k.shape];
       const int cur = k.step & 1, next = cur ^ 1, steps = (k.phase == 0 ? info.q : info.p) / KSTEP;
@@ -282,7 +319,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) newton_s
     constexpr uint32_t KBT = WIDE ? 2048 >> 4 : 1024 >> 4;
     int it = 0;
     Task k;
-    for (int n = 0; n < mine && take(n, true, k); ++n) {
+    for (int n = 0; take(n, true, k); ++n) {
       const Info& info = w.info[k.shape];
       const int buf = n & 1, steps = (k.phase == 0 ? info.q : info.p) / KSTEP, am = k.m * TILE, bn = k.n * TN;
       if (!mbar_wait(bar_free(buf), ((n >> 1) & 1) ^ 1, abort_flag, w.err, 324, WL)) break;
@@ -334,7 +371,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) newton_s
       }
     };
     Task k;
-    for (int n = 0; n < mine; ++n) {
+    for (int n = 0;; ++n) {
       // nobody may wait for this warp's last tile while it waits itself
       if (!mbar_test(bar_task(n % TASKS), (n / TASKS) & 1)) tell();
       if (!take(n, true, k)) break;
@@ -478,9 +515,10 @@ int set_shape(Steps<TN>& w, int i, const Batch& b) {
   return rc;
 }
 
-// The steps for batches from `from` on (and in that one from matrix `start` on), as many as a launch's parameters hold; both move on.  done: a counter for every matrix, zeros.
+// The steps for batches from `from` on (and in that one from matrix `start` on), as many as a launch's parameters hold; both move on, and done and base with them.
 template <int TN>
-int launch(const std::vector<Batch>& batches, size_t& from, int64_t& start, unsigned long long*& done, int steps, double a, double b, double c, cudaStream_t st) {
+int launch(const std::vector<Batch>& batches, size_t& from, int64_t& start, unsigned long long*& done, unsigned long long* drawn, unsigned long long& base, int steps, double a, double b, double c,
+           cudaStream_t st) {
   using S = Steps<TN>;
   static thread_local S w;
   // groups of about one size
@@ -529,6 +567,8 @@ int launch(const std::vector<Batch>& batches, size_t& from, int64_t& start, unsi
   w.steps = steps;
   w.a = static_cast<float>(a); w.b = static_cast<float>(b); w.c = static_cast<float>(c);
   w.done = done;
+  w.drawn = drawn;
+  w.base = base;
   done += matrices;
   if (tiles == 0) return HASTE_OK;
   if (int rc = device_status_word(&w.err)) return rc;
@@ -537,6 +577,7 @@ int launch(const std::vector<Batch>& batches, size_t& from, int64_t& start, unsi
   int pairs = 0;
   if (int rc = gemm::pairs_resident<kernel>(Layout<TN>::SMEM_BYTES, &pairs)) return rc;
   pairs = static_cast<int>(imin64(pairs, tiles));
+  base += static_cast<unsigned long long>(tiles) + pairs;          // every pair draws one number behind the last tile's
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
   cfg.blockDim = dim3(THREADS);
@@ -564,12 +605,14 @@ inline bool take_narrow(const std::vector<Batch>& batches) {
   return gemm::cost_of(tiles[1] / groups, per, true, pairs) < gemm::cost_of(tiles[0] / groups, per, false, pairs);
 }
 
-inline int run(const std::vector<Batch>& batches, unsigned long long* done, int steps, double a, double b, double c, cudaStream_t st) {
+// done: a counter for every matrix; drawn: one more.  All zeros.
+inline int run(const std::vector<Batch>& batches, unsigned long long* done, unsigned long long* drawn, int steps, double a, double b, double c, cudaStream_t st) {
   const bool narrow = take_narrow(batches);
   size_t from = 0;
   int64_t start = 0;
+  unsigned long long base = 0;
   while (from < batches.size()) {
-    if (int rc = narrow ? launch<64>(batches, from, start, done, steps, a, b, c, st) : launch<TILE>(batches, from, start, done, steps, a, b, c, st)) return rc;
+    if (int rc = narrow ? launch<64>(batches, from, start, done, drawn, base, steps, a, b, c, st) : launch<TILE>(batches, from, start, done, drawn, base, steps, a, b, c, st)) return rc;
   }
   return HASTE_OK;
 }
