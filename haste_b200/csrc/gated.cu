@@ -156,12 +156,12 @@ __global__ void align_rows_kernel(const __grid_constant__ Copies c) {
   }
 }
 
-// Sums of the parts of up to three products, in order, rounded to bf16
+// Sums of the parts of up to four products, in order, rounded to bf16
 struct Sums {
-  const float* part[3];
-  __nv_bfloat16* out[3];
-  int64_t rows[3], cols[3], ld_out[3], first[4];
-  int splits[3], n;
+  const float* part[4];
+  __nv_bfloat16* out[4];
+  int64_t rows[4], cols[4], ld_out[4], first[5];
+  int splits[4], n;
 };
 __global__ void sum_parts_kernel(const __grid_constant__ Sums s) {
   sm100::grid_dependency_wait();
@@ -536,6 +536,7 @@ int backward(Arena& arena, const GatedGradCall& c, cudaStream_t st) {
       return gemm::launch<K, TN>(w, align.c.n > 0, st);
     }));
   }
+  Sums s = {};
   if (c.dx != nullptr) {
     HASTE_TRY(by_form<Plain<false, true, 2>>(fx.narrow, [&](auto policy, auto columns) -> int {
       using K = decltype(policy);
@@ -551,12 +552,9 @@ int backward(Arena& arena, const GatedGradCall& c, cudaStream_t st) {
       HASTE_TRY((gemm::map_b<K, TN>(&p.b[1], {wu.p, wu.ld}, c.D, c.F)));
       return gemm::launch<K, TN>(w, true, st);
     }));
-    Sums s = {};
     add_sum(s, dx, c.T, c.D);
-    HASTE_TRY(run_sums(s, st));
   }
-  if (c.dwg == nullptr && c.dwu == nullptr && c.dwd == nullptr) return HASTE_OK;
-  Sums s = {};
+  if (c.dwg == nullptr && c.dwu == nullptr && c.dwd == nullptr) return run_sums(s, st);
   HASTE_TRY(by_form<Plain<true, true>>(fw.narrow, [&](auto policy, auto columns) -> int {
     using K = decltype(policy);
     constexpr int TN = decltype(columns)::value;
