@@ -4,7 +4,9 @@ layer, behind the reference's Python surface.
     haste_b200.shared_ffi   drop-in mirror of the reference's ``shared_ffi`` package
     haste_b200.fused        fused train step and label sharding across GPUs
     haste_b200.norm         layer norm for the features ahead of the layer
-    haste_b200.optim        AdamW over many tensors (moments in 32 or 8 bits), gradient norm
+    haste_b200.embedding    token embedding for an encoder in front of the layer
+    haste_b200.feedforward  gated feed-forward block
+    haste_b200.optim        AdamW over many tensors (moments in 32 or 8 bits), gradient norm; Muon for matrices
     haste_b200.projected    projection, layer norm and sparse layer in one training step
     haste_b200.ffi          tensor-level wrappers over the C ABI (include/haste_ffi.h)
 
