@@ -727,6 +727,7 @@ int haste_gated_backward(const void* dy, const void* x, const void* wg, const vo
     return e == cudaSuccess ? HASTE_OK : fail(HASTE_ERR_LAUNCH, "%s: %s", who, cudaGetErrorString(e));
   }
   REQUIRE_PTR(dy, who); REQUIRE_PTR(x, who); REQUIRE_PTR(wg, who); REQUIRE_PTR(wu, who); REQUIRE_PTR(wd, who); REQUIRE_PTR(gate, who); REQUIRE_PTR(up, who);
+  if (T == 1) { lddy = O; ldx = D; ldgate = ldup = F; }          // no second row to reach
   GatedGradCall c = {dy, x, wg, wu, wd, gate, up, dx, dwg, dwu, dwd, lddy, ldx, ldgate, ldup, T, D, F, O, act, false};
   c.aligned = (D | F | O | lddy | ldx | ldgate) % 8 == 0 && ldgate == ldup;
   for (const void* p : {dy, x, wg, wu, wd, gate, up, static_cast<const void*>(dx), static_cast<const void*>(dwg), static_cast<const void*>(dwu), static_cast<const void*>(dwd)})

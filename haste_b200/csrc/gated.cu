@@ -7,6 +7,10 @@
 // Backward: one for dh whose epilogue makes dgate, dup and h from the kept projections, one for dx (k runs over dgate and then over dup), one for the three weight
 // gradients.  Operands are bf16, sums fp32.  gate, up, h, dgate and dup are rounded to bf16 where they leave the chip: they are operands of the
 // next product or what training keeps, and 2^-8 of each value adds in squares to the result's own rounding.  Up to GEMV_ROWS rows the weights are streamed through CUDA cores instead.
+//
+// Measured (bf16): forward with gate and up kept, T = 65536, D = O = 1024, F = 2048: 410 us for the first launch (1341 TFLOP/s), 176 for the second (1562); backward,
+// T = 16384, D = F = O = 4096: 402 us for dh (1368), 716 for dx (1535), 1173 for the weights' (1406).  The power limit bounds all of them, and the first launch of either direction
+// the three matrices that its epilogue writes besides.
 #include "gemm_sm100.cuh"
 
 #include <type_traits>
@@ -55,7 +59,7 @@ __device__ __forceinline__ float activate(float g) {
 // out[0] = gate, out[1] = up (kept for training where scale0 is set), out[2] = h
 template <int ACT>
 struct GatedForward {
-  static constexpr bool A_MN = false, B_MN = false, F16 = false, PAIRED_B = true;
+  static constexpr bool A_MN = false, B_MN = false, PAIRED_B = true;
   static constexpr int PARTS = 1, OUTPUTS = 3, INPUTS = 0;
   template <int TN, class W, class I>
   static __device__ __forceinline__ void chunk(const W& w, const gemm::Problem<GatedForward>& p, const Tile&, int row, int col, uint32_t tmem, I&) {
@@ -83,7 +87,7 @@ struct GatedForward {
 // The accumulator is dh; in[0] = gate, in[1] = up; out[0] = dgate, out[1] = dup, out[2] = h
 template <int ACT>
 struct GatedBackward {
-  static constexpr bool A_MN = false, B_MN = true, F16 = false, PAIRED_B = false;
+  static constexpr bool A_MN = false, B_MN = true, PAIRED_B = false;
   static constexpr int PARTS = 1, OUTPUTS = 3, INPUTS = 2;
   template <int TN, class W, class I>
   static __device__ __forceinline__ void chunk(const W&, const gemm::Problem<GatedBackward>& p, const Tile&, int row, int col, uint32_t tmem, I& in) {
@@ -111,7 +115,7 @@ struct GatedBackward {
 // out[0] = the product in bf16, or fp32 parts in `partial` [splits][M][N rounded up to 4]
 template <bool A, bool B, int K_PARTS = 1>
 struct Plain {
-  static constexpr bool A_MN = A, B_MN = B, F16 = false, PAIRED_B = false;
+  static constexpr bool A_MN = A, B_MN = B, PAIRED_B = false;
   static constexpr int PARTS = K_PARTS, OUTPUTS = 1, INPUTS = 0;
   template <int TN, class W, class I>
   static __device__ __forceinline__ void chunk(const W&, const gemm::Problem<Plain>& p, const Tile& t, int row, int col, uint32_t tmem, I&) {
@@ -135,7 +139,8 @@ struct Plain {
 };
 
 // ---------------------------------------------------------------- helpers around the products
-// Rows whose stride or base is not a multiple of 16 bytes are copied to where they are: tensor maps need it.
+// Rows whose stride or base is not a multiple of 16 bytes are copied to where they are: tensor maps need it.  Memory alone: x, dy and the three weights of 333 rows, 509 x 1021, in 5 us,
+// most of it the launch's.
 constexpr int MAX_JOBS = 8;
 struct Copies {
   const uint16_t* src[MAX_JOBS];
@@ -156,7 +161,8 @@ __global__ void align_rows_kernel(const __grid_constant__ Copies c) {
   }
 }
 
-// Sums of the parts of up to four products, in order, rounded to bf16
+// Sums of the parts of up to four products, in order, rounded to bf16.  Memory alone; one launch for all of a call (333 rows, 509 x 1021: 6 us for 6 MB, which L2 has; a
+// second launch for dx cost 2 us more).
 struct Sums {
   const float* part[4];
   __nv_bfloat16* out[4];
@@ -204,7 +210,9 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// h[t, f] for T <= ROWS rows, one warp for each f
+// h[t, f] for T <= ROWS rows, one warp for each f.  Bound by the weights' bytes: one row, D = 768, F = 2048 (6 MB): 5.0 us, and 4.7 for the second launch, which overlaps
+// it: 7.3 in all, 8.2 before its weights were fetched early.  From L2, as the weights are from call to call; with more rows the sums in CUDA cores bind (8 rows: 19 us;
+// 9 rows take the tensor cores).
 template <int ACT, int ROWS, bool VEC>
 __global__ void __launch_bounds__(GEMV_THREADS) gated_few_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, const __nv_bfloat16* __restrict__ wg,
                                                                  const __nv_bfloat16* __restrict__ wu, __nv_bfloat16* __restrict__ gate, __nv_bfloat16* __restrict__ up,
@@ -398,7 +406,7 @@ template <class Policy>
 void set_output(gemm::Problem<Policy>& p, const Output& o) {
   p.splits = o.splits;
   p.partial = o.part;
-  p.out[0] = gemm::result({o.p, p.N});
+  p.out[0] = gemm::result({o.p, p.N}, p.N);
 }
 void add_sum(Sums& s, const Output& o, int64_t M, int64_t N) {
   if (o.part == nullptr) return;
@@ -479,10 +487,10 @@ int forward(Arena& arena, const GatedCall& c, cudaStream_t st) {
     HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wg.p, wg.ld}, c.F, c.D)));
     HASTE_TRY((gemm::map_b<K, TN>(&p.b[1], {wu.p, wu.ld}, c.F, c.D)));
     if (c.gate != nullptr) {
-      p.out[0] = gemm::result({c.gate, c.ldh});
-      p.out[1] = gemm::result({c.up, c.ldh});
+      p.out[0] = gemm::result({c.gate, c.ldh}, c.F);
+      p.out[1] = gemm::result({c.up, c.ldh}, c.F);
     }
-    p.out[2] = gemm::result({h, ldF});
+    p.out[2] = gemm::result({h, ldF}, c.F);
     return gemm::launch<K, TN>(w, align.c.n > 0, st);
   }));
   HASTE_TRY(by_form<Plain<false, false>>(fy.narrow, [&](auto policy, auto columns) -> int {
@@ -529,10 +537,10 @@ int backward(Arena& arena, const GatedGradCall& c, cudaStream_t st) {
       set_sizes(p, c.T, c.F, sO, sO);
       HASTE_TRY((gemm::map_a<K, TN>(&p.a[0], {dy.p, dy.ld}, c.T, c.O)));
       HASTE_TRY((gemm::map_b<K, TN>(&p.b[0], {wd.p, wd.ld}, c.F, c.O)));
-      p.in[0] = gemm::result({gate.p, gate.ld});
-      p.in[1] = gemm::result({up.p, up.ld});
+      p.in[0] = gemm::result({gate.p, gate.ld}, c.F);
+      p.in[1] = gemm::result({up.p, up.ld}, c.F);
       void* outs[3] = {dgate, dup, h};
-      for (int i = 0; i < 3; ++i) p.out[i] = gemm::result({outs[i], ldF});
+      for (int i = 0; i < 3; ++i) p.out[i] = gemm::result({outs[i], ldF}, c.F);
       return gemm::launch<K, TN>(w, align.c.n > 0, st);
     }));
   }

@@ -6,11 +6,15 @@
 // issues tcgen05.mma.cta_group::2, whose operands are both CTAs' shared memory and whose accumulator is 128 x TN fp32 in each CTA's TMEM (two of
 // them, so that one is read while the next is summed).  Either operand lies with k or with its rows (m, n) contiguous.  What happens to an accumulator is
 // the policy's: its warps read TMEM, 32 rows x 32 columns at a time, a lane's own row of 64 bytes of up to two 16-bit matrices beside it, loaded a chunk ahead, and
-// store a lane's row in whole 32-byte sectors.  The epilogue keeps out of shared memory, whose bandwidth the tensor cores' operands and their copies take in full: with tiles staged
-// for tensor-map stores, and inputs brought by them, a Newton-Schulz step over 50 M elements took 1870 K cycles, 980 K without its stores and inputs.
+// store a lane's row in whole 32-byte sectors, so that all shared memory is left to the operands' stages.  Staged in shared memory and stored through tensor maps
+// instead, with a stage less, a product whose epilogue reads two matrices and writes three took 450 us (16384 x 4096 x 4096; here 398), one that writes one 181 to 186 us
+// (65536 x 1024 x 2048; 173), one that writes three beside a longer sum 394 to 413 us (2 x 65536 x 2048 x 1024; 406).
+//
+// Bound: the tensor cores, and over more than some 100 us the power limit under them.  Alone, the products of the gated block run at 1340 to 1560 TFLOP/s, 82 to 95 % of
+// a library product's burst rate here (1640); in a stream of them both settle near 1370.
 //
 // TN = 256 is what keeps the tensor cores fed from L2; where there are fewer such tiles than pairs of SMs a narrow form (TN = 64, or 128 for a paired b) has more
-// and shorter ones.
+// and shorter ones: cost_of() weighs both.  The gradients of a gated block of 333 rows, 509 x 1021: 57 us with the wide form alone, 43 with both.
 //
 // Roles (12 warps): warp 0 TMA, warp 1 MMA (in the even CTA), warp 2 TMEM, warps 4-11 epilogue (lane quarter x column half).  Every wait is bounded;
 // after one has run out all roles go on without touching global memory, the kernel returns and the status word says so.
@@ -106,12 +110,12 @@ struct Sizes {
   int steps0, steps;               // steps of k in the first part, and in both
   int first;                       // number of this problem's first tile; set by launch()
 };
-// A 16-bit matrix of the result's size that the policy reads or writes: rows of ld elements.  on: the bytes that base and rows are multiples of, 32 or 16 (with a
-// third form for any, every lane storing its row's values one by one, the weights' gradients of 333 x 509 x 1021 took 43 us, through fp32 parts 14 and 6)
+// A 16-bit matrix of the result's size that the policy reads or writes: rows of ld elements, of which the first `cols` (the result's columns, rounded up to a multiple of 8)
+// are read or written and what is behind them is others'.  on: the bytes that base, rows and cols are multiples of, 32 or 16 (with a third form for any, every lane storing its row's values one by one, the weights' gradients of 333 x 509 x 1021 took 43 us, through fp32 parts 14 and 6)
 struct Matrix16 {
   uint16_t* p;
   int64_t ld;
-  int on;
+  int cols, on;
 };
 template <class Policy>
 struct Problem : Sizes {
@@ -162,17 +166,17 @@ __device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2
 __device__ __forceinline__ void store_32_bytes(void* p, const uint32_t* v) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
-// 32 columns of a row, packed in pairs: what lies in the (padded) row
+// 32 columns of a row, packed in pairs: those that the matrix has
 __device__ __forceinline__ void store_row(const Matrix16& m, int row, int col, const uint32_t (&v)[16]) {
   uint16_t* to = m.p + static_cast<int64_t>(row) * m.ld + col;
   if (m.on == 32) {
 #pragma unroll
     for (int j = 0; j < 2; ++j)
-      if (col + 16 * j < m.ld) store_32_bytes(to + 16 * j, v + 8 * j);
+      if (col + 16 * j < m.cols) store_32_bytes(to + 16 * j, v + 8 * j);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (col + 8 * j < m.ld) *reinterpret_cast<uint4*>(to + 8 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      if (col + 8 * j < m.cols) *reinterpret_cast<uint4*>(to + 8 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
   }
 }
 // and zeros beyond it
@@ -184,14 +188,14 @@ __device__ __forceinline__ void load_row(const Matrix16& m, int row, int col, bo
   if (m.on == 32) {
 #pragma unroll
     for (int j = 0; j < 2; ++j)
-      if (col + 16 * j < m.ld)
+      if (col + 16 * j < m.cols)
         asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                      : "=r"(v[8 * j]), "=r"(v[8 * j + 1]), "=r"(v[8 * j + 2]), "=r"(v[8 * j + 3]), "=r"(v[8 * j + 4]), "=r"(v[8 * j + 5]), "=r"(v[8 * j + 6]), "=r"(v[8 * j + 7])
                      : "l"(from + 16 * j));
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (col + 8 * j < m.ld) {
+      if (col + 8 * j < m.cols) {
         const uint4 q = __ldg(reinterpret_cast<const uint4*>(from + 8 * j));
         v[4 * j] = q.x; v[4 * j + 1] = q.y; v[4 * j + 2] = q.z; v[4 * j + 3] = q.w;
       }
@@ -199,7 +203,7 @@ __device__ __forceinline__ void load_row(const Matrix16& m, int row, int col, bo
 }
 
 // ---------------------------------------------------------------- the kernel
-// Policy: A_MN, B_MN (the operand's rows are contiguous, not k), F16 (else bf16), PAIRED_B (each CTA has an operand b of its own: TN / 2 columns of
+// Policy: A_MN, B_MN (the operand's rows are contiguous, not k), PAIRED_B (each CTA has an operand b of its own: TN / 2 columns of
 // two products side by side), PARTS of k, OUTPUTS, INPUTS, and
 //   static void chunk<TN>(w, p, tile, row, col, tmem, inputs)   32 columns of this lane's row of the result, accumulator at tmem
 template <class Policy, int P, int TN>
@@ -273,7 +277,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) gemm_sm1
     for (int i = it > STAGES ? it - STAGES : 0; i < it; ++i) mbar_wait(bar_empty(i % STAGES), (i / STAGES) & 1, abort_flag, w.err, 302, WL);
   } else if (warp == 1 && rank == 0) {
     // ---------------- products
-    constexpr uint32_t FORMAT = Policy::F16 ? 0u : (1u << 7) | (1u << 10);
+    constexpr uint32_t FORMAT = (1u << 7) | (1u << 10);          // both operands bf16
     constexpr uint32_t IDESC = (1u << 4) | FORMAT | (static_cast<uint32_t>(Policy::A_MN) << 15) | (static_cast<uint32_t>(Policy::B_MN) << 16) |
                                (static_cast<uint32_t>(TN >> 3) << 17) | (static_cast<uint32_t>(TILE >> 4) << 24);
     const uint64_t da = make_sdesc(base, Policy::A_MN ? L::A_BYTES / 2 : 16, 1024);
@@ -368,15 +372,16 @@ struct Operand {
 // Operand a of `rows` (the result's M) and b of `rows` (its N), k values each; inputs and outputs of the result's size
 template <class Policy, int TN>
 int map_a(CUtensorMap* out, const Operand& o, int64_t rows, int64_t k) {
-  return Policy::A_MN ? make_map(out, o.p, Policy::F16, rows, k, 1, o.ld, 0, 64, 64) : make_map(out, o.p, Policy::F16, k, rows, 1, o.ld, 0, 64, 128);
+  return Policy::A_MN ? make_map(out, o.p, false, rows, k, 1, o.ld, 0, 64, 64) : make_map(out, o.p, false, k, rows, 1, o.ld, 0, 64, 128);
 }
 template <class Policy, int TN>
 int map_b(CUtensorMap* out, const Operand& o, int64_t rows, int64_t k) {
-  return Policy::B_MN ? make_map(out, o.p, Policy::F16, rows, k, 1, o.ld, 0, TN == 64 ? 32 : 64, 64)
-                      : make_map(out, o.p, Policy::F16, k, rows, 1, o.ld, 0, 64, TN / 2);
+  return Policy::B_MN ? make_map(out, o.p, false, rows, k, 1, o.ld, 0, TN == 64 ? 32 : 64, 64)
+                      : make_map(out, o.p, false, k, rows, 1, o.ld, 0, 64, TN / 2);
 }
-inline Matrix16 result(const Operand& o) {
-  return {static_cast<uint16_t*>(const_cast<void*>(o.p)), o.ld, o.ld % 16 == 0 && reinterpret_cast<uintptr_t>(o.p) % 32 == 0 ? 32 : 16};
+inline Matrix16 result(const Operand& o, int64_t columns) {
+  const int cols = static_cast<int>((columns + 7) & ~int64_t(7));
+  return {static_cast<uint16_t*>(const_cast<void*>(o.p)), o.ld, cols, o.ld % 16 == 0 && cols % 16 == 0 && reinterpret_cast<uintptr_t>(o.p) % 32 == 0 ? 32 : 16};
 }
 inline int64_t steps_of(int64_t k) { return (k + KSTEP - 1) / KSTEP; }
 

@@ -427,7 +427,8 @@ int haste_embedding_backward(const void* ids, int32_t id_bytes, const void* dy, 
                              int64_t lddy, float scale, int64_t padding, int32_t dy_type, int32_t out_type, haste_stream_t stream);
 
 /* Gated feed-forward block, bf16: y = (act(x Wg^T) * (x Wu^T)) Wd^T with x [T, D] (row stride ldx), Wg, Wu [F, D], Wd [O, F] and y [T, O] contiguous; act: HASTE_ACT_*.
- * For training gate = x Wg^T and up = x Wu^T [T, F] (row stride ldh, a multiple of 8, 16-byte aligned) are kept, without NULL.  Sums are fp32; the product
+ * For training gate = x Wg^T and up = x Wu^T [T, F] (row stride ldh, a multiple of 8, 16-byte aligned) are kept, without NULL; of their rows F elements, rounded up to a
+ * multiple of 8, may be written and nothing behind them.  Sums are fp32; the product
  * act(gate) * up is rounded to bf16 on its way to the second product (not for T <= 8).  Nothing else needs alignment; operands that have it (16-byte bases, row
  * strides and D, F, O multiples of 8) are read in place, others are copied first.
  * scratch: 256-byte aligned, haste_gated_forward_scratch(T, D, F, O, aligned) bytes, aligned = 0 unless all operands have that alignment. */

@@ -215,3 +215,26 @@ def test_in_graphs_beside_eager_calls():
     torch.cuda.synchronize()
     for out in (*outs, eager):
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("F", [72, 77, 136, 160])
+@pytest.mark.parametrize("T", [5, 40, 300])
+def test_kept_projections_side_by_side(T, F):
+    """gate and up as halves of one matrix, through the C entry: a row ends at F, rounded up to a multiple of 8, and what is behind it stays."""
+    from haste_b200 import _lib
+    from haste_b200.feedforward import gated_backward, gated_forward
+    x, wg, wu, wd, dy = _inputs(T, 64, F, 48)
+    up8 = -(-F // 8) * 8
+    kept = torch.full((T + 2, 2 * up8 + 8), 7.0, dtype=BF, device="cuda")
+    gate, up, y = kept[1:-1, :up8], kept[1:-1, up8:2 * up8], torch.empty(T, 48, dtype=BF, device="cuda")
+    need = _lib.lib.haste_gated_forward_scratch(T, 64, F, 48, 0)
+    scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    assert _lib.lib.haste_gated_forward(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), gate.data_ptr(), up.data_ptr(), y.data_ptr(), scratch.data_ptr(), need, T, 64, F, 48, 64,
+                                        kept.stride(0), _lib.ACTIVATIONS["silu"], stream) == _lib.OK
+    want = gated_forward(x, wg, wu, wd, keep=True)
+    assert torch.equal(y, want[0]) and torch.equal(gate[:, :F], want[1]) and torch.equal(up[:, :F], want[2])
+    assert (kept[0] == 7).all() and (kept[-1] == 7).all() and (kept[:, 2 * up8:] == 7).all()
+    kept[:, 2 * up8:] = float("nan")                                       # and what is behind a row that is read does not count
+    grads, from_halves = gated_backward(dy, x, wg, wu, wd, *want[1:]), gated_backward(dy, x, wg, wu, wd, gate[:, :F], up[:, :F])
+    assert all(torch.equal(a, b) for a, b in zip(grads, from_halves))
