@@ -6,7 +6,7 @@
 // Forward: one launch for both projections, the activation and the product (a pair of CTAs sums 128 columns of gate and of up side by side), one for y.
 // Backward: one for dh whose epilogue makes dgate, dup and h from the kept projections, one for dx (k runs over dgate and then over dup), one for the three weight
 // gradients.  Operands are bf16, sums fp32.  gate, up, h, dgate and dup are rounded to bf16 where they leave the chip: they are operands of the
-// next product or what training keeps, and 2^-8 of each value adds in squares to the result's own rounding.  Up to GEMV_ROWS rows the weights are streamed through CUDA cores instead.
+// next product or what training keeps, and 2^-8 of each value adds in squares to the result's own rounding.  Up to FEW_ROWS rows the weights are streamed through registers instead.
 //
 // Measured (bf16): forward with gate and up kept, T = 65536, D = O = 1024, F = 2048: 410 us for the first launch (1341 TFLOP/s), 176 for the second (1562); backward,
 // T = 16384, D = F = O = 4096: 402 us for dh (1368), 716 for dx (1535), 1173 for the weights' (1406).  The power limit bounds all of them, and the first launch of either direction
@@ -188,9 +188,10 @@ __global__ void sum_parts_kernel(const __grid_constant__ Sums s) {
   }
 }
 
-// ---------------------------------------------------------------- few rows
-constexpr int GEMV_ROWS = 8;
-constexpr int GEMV_THREADS = 256;
+// ---------------------------------------------------------------- one row
+// One row's sums in CUDA cores, which have neither sums of warps to collect nor operands to shape: 3.3, 5.5, 8.6, 11.4 and 24.4 us a call at the sizes of the table below, in the
+// form for few rows 4.3, 7.0, 11.0, 11.9 and 25.4.  (A call of 768 x 2048 was 8.2 us before the second launch fetched its weights early.)
+constexpr int ONE_THREADS = 256;
 
 template <bool VEC>
 __device__ __forceinline__ void load8(const __nv_bfloat16* p, int64_t i, int64_t n, float (&v)[8]) {
@@ -210,80 +211,58 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// h[t, f] for T <= ROWS rows, one warp for each f.  Bound by the weights' bytes: one row, D = 768, F = 2048 (6 MB): 5.0 us, and 4.7 for the second launch, which overlaps
-// it: 7.3 in all, 8.2 before its weights were fetched early.  From L2, as the weights are from call to call; with more rows the sums in CUDA cores bind (8 rows: 19 us;
-// 9 rows take the tensor cores).
-template <int ACT, int ROWS, bool VEC>
-__global__ void __launch_bounds__(GEMV_THREADS) gated_few_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, const __nv_bfloat16* __restrict__ wg,
-                                                                 const __nv_bfloat16* __restrict__ wu, __nv_bfloat16* __restrict__ gate, __nv_bfloat16* __restrict__ up,
-                                                                 int64_t ldh, float* __restrict__ h, int T, int64_t D, int64_t F) {
+// h[f], one warp for each f
+template <int ACT, bool VEC>
+__global__ void __launch_bounds__(ONE_THREADS) gated_one_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ wg, const __nv_bfloat16* __restrict__ wu,
+                                                                __nv_bfloat16* __restrict__ gate, __nv_bfloat16* __restrict__ up, float* __restrict__ h, int64_t D, int64_t F) {
   const int lane = threadIdx.x & 31;
-  const int64_t f = static_cast<int64_t>(blockIdx.x) * (GEMV_THREADS / 32) + (threadIdx.x >> 5);
+  const int64_t f = static_cast<int64_t>(blockIdx.x) * (ONE_THREADS / 32) + (threadIdx.x >> 5);
   sm100::grid_launch_dependents();                 // the next launch fetches its weights meanwhile
   if (f >= F) return;
-  float g[ROWS], u[ROWS];
-#pragma unroll
-  for (int t = 0; t < ROWS; ++t) g[t] = u[t] = 0.f;
+  float g = 0.f, u = 0.f;
 #pragma unroll 2
   for (int64_t i = lane * 8; i < D; i += 256) {
     float a[8], b[8], v[8];
     load8<VEC>(wg + f * D, i, D, a);
     load8<VEC>(wu + f * D, i, D, b);
+    load8<VEC>(x, i, D, v);
 #pragma unroll
-    for (int t = 0; t < ROWS; ++t) {
-      if (t < T) {
-        load8<VEC>(x + t * ldx, i, D, v);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) { g[t] = fmaf(a[k], v[k], g[t]); u[t] = fmaf(b[k], v[k], u[t]); }
-      }
-    }
+    for (int k = 0; k < 8; ++k) { g = fmaf(a[k], v[k], g); u = fmaf(b[k], v[k], u); }
   }
-#pragma unroll
-  for (int t = 0; t < ROWS; ++t) {
-    if (t >= T) break;
-    const float gs = warp_sum(g[t]), us = warp_sum(u[t]);
-    if (lane == 0) {
-      h[t * F + f] = activate<ACT>(gs) * us;
-      if (gate != nullptr) {
-        gate[t * ldh + f] = __float2bfloat16_rn(gs);
-        up[t * ldh + f] = __float2bfloat16_rn(us);
-      }
+  g = warp_sum(g);
+  u = warp_sum(u);
+  if (lane == 0) {
+    h[f] = activate<ACT>(g) * u;
+    if (gate != nullptr) {
+      gate[f] = __float2bfloat16_rn(g);
+      up[f] = __float2bfloat16_rn(u);
     }
   }
 }
 
-// y[t, o] = sum_f h[t, f] Wd[o, f]: `warps` warps for each o.  A lane's first EARLY pieces of the weights are on their way before h is there.
-template <int ROWS, bool VEC>
-__global__ void __launch_bounds__(GEMV_THREADS) down_few_kernel(const float* __restrict__ h, const __nv_bfloat16* __restrict__ wd, __nv_bfloat16* __restrict__ y, int T, int64_t F,
-                                                                int64_t O, int warps) {
+// y[o] = sum_f h[f] Wd[o, f]: `warps` warps for each o.  A lane's first EARLY pieces of the weights are on their way before h is there.
+template <bool VEC>
+__global__ void __launch_bounds__(ONE_THREADS) down_one_kernel(const float* h, const __nv_bfloat16* __restrict__ wd, __nv_bfloat16* __restrict__ y, int64_t F, int64_t O, int warps) {
   constexpr int EARLY = 2;
-  __shared__ float part[GEMV_THREADS / 32][ROWS];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t o = static_cast<int64_t>(blockIdx.x) * (GEMV_THREADS / 32 / warps) + warp / warps, step = warps * 256;
-  const int mine = warp % warps;
-  const int64_t first = (mine * 32 + lane) * 8;
+  __shared__ float part[ONE_THREADS / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = warp % warps;
+  const int64_t o = static_cast<int64_t>(blockIdx.x) * (ONE_THREADS / 32 / warps) + warp / warps, step = warps * 256, first = (mine * 32 + lane) * 8;
   const __nv_bfloat16* row = wd + o * F;
-  float s[ROWS], early[EARLY][8];
-#pragma unroll
-  for (int t = 0; t < ROWS; ++t) s[t] = 0.f;
+  float s = 0.f, early[EARLY][8];
 #pragma unroll
   for (int k = 0; k < EARLY; ++k)
     if (o < O && first + k * step < F) load8<VEC>(row, first + k * step, F, early[k]);
   sm100::grid_dependency_wait();
   auto add = [&](const float (&a)[8], int64_t i) {
+    if (VEC) {
+      const float4 p = *reinterpret_cast<const float4*>(h + i), q = *reinterpret_cast<const float4*>(h + i + 4);
+      s = fmaf(a[0], p.x, fmaf(a[1], p.y, fmaf(a[2], p.z, fmaf(a[3], p.w, s))));
+      s = fmaf(a[4], q.x, fmaf(a[5], q.y, fmaf(a[6], q.z, fmaf(a[7], q.w, s))));
+    } else {
 #pragma unroll
-    for (int t = 0; t < ROWS; ++t)
-      if (t < T) {
-        if (VEC) {
-          const float4 p = *reinterpret_cast<const float4*>(h + t * F + i), q = *reinterpret_cast<const float4*>(h + t * F + i + 4);
-          s[t] = fmaf(a[0], p.x, fmaf(a[1], p.y, fmaf(a[2], p.z, fmaf(a[3], p.w, s[t]))));
-          s[t] = fmaf(a[4], q.x, fmaf(a[5], q.y, fmaf(a[6], q.z, fmaf(a[7], q.w, s[t]))));
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (i + k < F) s[t] = fmaf(a[k], h[t * F + i + k], s[t]);
-        }
-      }
+      for (int k = 0; k < 8; ++k)
+        if (i + k < F) s = fmaf(a[k], h[i + k], s);
+    }
   };
   if (o < O) {
 #pragma unroll
@@ -296,31 +275,212 @@ __global__ void __launch_bounds__(GEMV_THREADS) down_few_kernel(const float* __r
       add(a, i);
     }
   }
-#pragma unroll
-  for (int t = 0; t < ROWS; ++t) {
-    s[t] = warp_sum(s[t]);
-    if (lane == 0) part[warp][t] = s[t];
-  }
+  s = warp_sum(s);
+  if (lane == 0) part[warp] = s;
   __syncthreads();
-  if (mine == 0 && o < O && lane < T && lane < ROWS) {
+  if (mine == 0 && o < O && lane == 0) {
     float v = 0.f;
-    for (int k = 0; k < warps; ++k) v += part[warp + k][lane];
-    y[lane * O + o] = __float2bfloat16_rn(v);
+    for (int k = 0; k < warps; ++k) v += part[warp + k];
+    y[o] = __float2bfloat16_rn(v);
+  }
+}
+template <int ACT, bool VEC>
+int one_row(const GatedCall& c, float* h, cudaStream_t st) {
+  using B = __nv_bfloat16;
+  constexpr int WARPS = ONE_THREADS / 32;
+  gated_one_kernel<ACT, VEC><<<static_cast<unsigned>((c.F + WARPS - 1) / WARPS), ONE_THREADS, 0, st>>>(
+      static_cast<const B*>(c.x), static_cast<const B*>(c.wg), static_cast<const B*>(c.wu), static_cast<B*>(c.gate), static_cast<B*>(c.up), h, c.D, c.F);
+  if (int rc = check_launch("gated_one_kernel")) return rc;
+  int warps = 1;
+  while (warps < WARPS && c.O * warps < static_cast<int64_t>(sm_count()) * 16 && c.F > warps * 256) warps *= 2;
+  return launch_behind(down_one_kernel<VEC>, static_cast<unsigned>((c.O * warps + WARPS - 1) / WARPS), ONE_THREADS, st, static_cast<const float*>(h), static_cast<const B*>(c.wd),
+                       static_cast<B*>(c.y), c.F, c.O, warps);
+}
+
+// ---------------------------------------------------------------- few rows
+// Up to FEW_ROWS rows the weights' bytes are what it takes: every weight is read once, straight into the registers of a product of 16 of a matrix's rows with 8 of x (a warp's
+// tensor-core instruction, which keeps up with memory; the sums in CUDA cores do not).  A block has 16 rows, its warps share k, and their sums meet in shared memory.
+// us a call, weights from L2 (the first) or memory (the last):     D x F = O x F 512 x 1024   768 x 2048   1024 x 4096   2048 x 2560   4096 x 4096
+//   8 rows, here                                                          4.6          7.6          11.6          12.5          25.8
+//   8 rows, in CUDA cores                                                 9.0         15.8          24.2          34.5         104.8
+//   32 rows, here                                                         5.7          9.8          14.4          16.1          33.3
+//   32 rows, in tiles (as from 33 on)                                    14.5         18.4          22.2          23.5          35.7
+// The weights take 0.5, 1.4, 3.8, 4.8 and 15.4 us at the rate of memory: what is left is two launches, each with the latency of its first loads.
+constexpr int FEW_ROWS = 32;
+constexpr int EXACT_ROWS = 8;      // h stays in 32 bits up to these, and is bf16 beyond, as in the tiled form
+constexpr int FEW_LINE = 64;       // k of a warp at a time: 128 bytes of each of its rows
+
+template <int NT>
+constexpr int few_warps() { return NT == 4 ? 8 : 16; }       // of a block, at most: what their sums' place in shared memory allows
+
+// Elements i .. i + 7 of a row of n, zeros where there are none
+template <bool VEC>
+__device__ __forceinline__ uint4 piece(const __nv_bfloat16* row, int i, int n, bool there) {
+  if (VEC) return there && i < n ? *reinterpret_cast<const uint4*>(row + i) : make_uint4(0, 0, 0, 0);
+  const uint16_t* s = reinterpret_cast<const uint16_t*>(row) + i;
+  uint32_t v[8];
+#pragma unroll
+  for (int x = 0; x < 8; ++x) v[x] = there && i + x < n ? s[x] : 0;
+  return make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+}
+__device__ __forceinline__ void mma_16x8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 32 of k: a lane has 8 neighbours of each operand, which the instruction takes for its own order of them, the same for both
+__device__ __forceinline__ void add_products(float (&d)[4], const uint4& low, const uint4& high, const uint4& b) {
+  mma_16x8(d, low.x, high.x, low.y, high.y, b.x, b.y);
+  mma_16x8(d, low.z, high.z, low.w, high.w, b.z, b.w);
+}
+// A warp's sums [16 rows of the matrix][8 NT of x] to where the block adds them
+template <int NT>
+__device__ __forceinline__ void put_sums(float (*to)[20], const float (&d)[NT][4], int lane) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to[8 * t + 2 * (lane & 3) + (e & 1)][(lane >> 2) + 8 * (e >> 1)] = d[t][e];
+}
+
+// h[t, f], 16 of f a block
+template <int ACT, int NT, bool VEC>
+__global__ void __launch_bounds__(few_warps<NT>() * 32, 1) gated_few_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, const __nv_bfloat16* __restrict__ wg,
+                                                                         const __nv_bfloat16* __restrict__ wu, __nv_bfloat16* __restrict__ gate, __nv_bfloat16* __restrict__ up,
+                                                                         int64_t ldh, __nv_bfloat16* __restrict__ h, int T, int D, int F) {
+  __shared__ float part[few_warps<NT>()][2][8 * NT][20];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int f0 = blockIdx.x * 16, low = f0 + (lane >> 2), high = low + 8;
+  const __nv_bfloat16 *g_low = wg + static_cast<int64_t>(low) * D, *g_high = g_low + static_cast<int64_t>(8) * D, *u_low = wu + (g_low - wg), *u_high = wu + (g_high - wg);
+  sm100::grid_launch_dependents();                 // the next launch fetches its weights meanwhile
+  float g[NT][4] = {}, u[NT][4] = {};
+#pragma unroll 1                                   // (unrolled twice it is slower at every size: 512 x 1024 6.0 us a call instead of 4.5)
+  for (int k0 = warp * FEW_LINE; k0 < D; k0 += warps * FEW_LINE) {
+    uint4 gl[2], gh[2], ul[2], uh[2], xs[2][NT];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int k = k0 + c * 32 + (lane & 3) * 8;
+      gl[c] = piece<VEC>(g_low, k, D, low < F); gh[c] = piece<VEC>(g_high, k, D, high < F);
+      ul[c] = piece<VEC>(u_low, k, D, low < F); uh[c] = piece<VEC>(u_high, k, D, high < F);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) xs[c][t] = piece<VEC>(x + (8 * t + (lane >> 2)) * ldx, k, D, 8 * t + (lane >> 2) < T);
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        add_products(g[t], gl[c], gh[c], xs[c][t]);
+        add_products(u[t], ul[c], uh[c], xs[c][t]);
+      }
+  }
+  put_sums<NT>(part[warp][0], g, lane);
+  put_sums<NT>(part[warp][1], u, lane);
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * T; i += blockDim.x) {
+    const int t = i >> 4, row = i & 15;
+    if (f0 + row >= F) continue;
+    float gs = 0.f, us = 0.f;
+    for (int w = 0; w < warps; ++w) { gs += part[w][0][t][row]; us += part[w][1][t][row]; }
+    const float v = activate<ACT>(gs) * us;
+    __nv_bfloat16* to = h + static_cast<int64_t>(t) * F + f0 + row;
+    if (NT * 8 <= EXACT_ROWS) {
+      // the sum of three bf16, without a rounding: 8 bits of it each
+      float rest = v;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        const uint32_t top = __float_as_uint(rest) & 0xFFFF0000u;
+        to[static_cast<int64_t>(k) * T * F] = __ushort_as_bfloat16(static_cast<uint16_t>(top >> 16));
+        rest = (top & 0x7F800000u) == 0x7F800000u ? 0.f : rest - __uint_as_float(top);             // (inf and NaN are in the first alone)
+      }
+    } else {
+      *to = __float2bfloat16_rn(v);
+    }
+    if (gate != nullptr) {
+      gate[t * ldh + f0 + row] = __float2bfloat16_rn(gs);
+      up[t * ldh + f0 + row] = __float2bfloat16_rn(us);
+    }
   }
 }
 
-template <int ACT, int ROWS, bool VEC>
-int few_rows(const void* x, int64_t ldx, const void* wg, const void* wu, const void* wd, void* gate, void* up, int64_t ldh, void* y, float* h, int64_t T, int64_t D, int64_t F,
-             int64_t O, cudaStream_t st) {
+// y[t, o] = sum_f h[t, f] Wd[o, f], 16 of o a block.  The first pieces of the weights are on their way before h is there.
+template <int NT, bool VEC>
+__global__ void __launch_bounds__(few_warps<NT>() * 32, 1) down_few_kernel(const __nv_bfloat16* h, const __nv_bfloat16* __restrict__ wd, __nv_bfloat16* __restrict__ y, int T, int F, int O) {
+  constexpr int C = NT == 1 ? 2 : 4, PARTS = NT * 8 <= EXACT_ROWS ? 3 : 1;         // C: pieces of each row that are on their way at once
+  __shared__ float part[few_warps<NT>()][8 * NT][20];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int o0 = blockIdx.x * 16, low = o0 + (lane >> 2), high = low + 8;
+  const __nv_bfloat16 *w_low = wd + static_cast<int64_t>(low) * F, *w_high = w_low + static_cast<int64_t>(8) * F, *h_mine = h + static_cast<int64_t>(lane >> 2) * F;
+  auto at = [&](int k0, int c) { return k0 + (c >> 1) * warps * FEW_LINE + (c & 1) * 32 + (lane & 3) * 8; };
+  float s[PARTS][NT][4] = {};
+  uint4 wl[C], wh[C];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      wl[c] = piece<VEC>(w_low, at(k0, c), F, low < O);
+      wh[c] = piece<VEC>(w_high, at(k0, c), F, high < O);
+    }
+  };
+  int k0 = warp * FEW_LINE;
+  fetch(k0);
+  sm100::grid_dependency_wait();
+#pragma unroll 1
+  while (k0 < F) {
+    uint4 hs[C][NT][PARTS];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) hs[c][t][k] = piece<VEC>(h_mine + (static_cast<int64_t>(k) * T + 8 * t) * F, at(k0, c), F, 8 * t + (lane >> 2) < T);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) add_products(s[k][t], wl[c], wh[c], hs[c][t][k]);
+    k0 += warps * FEW_LINE * (C / 2);
+    if (k0 < F) fetch(k0);
+  }
+#pragma unroll
+  for (int k = 1; k < PARTS; ++k)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[0][t][e] += s[k][t][e];
+  put_sums<NT>(part[warp], s[0], lane);
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * T; i += blockDim.x) {
+    const int t = i >> 4, row = i & 15;
+    if (o0 + row >= O) continue;
+    float v = 0.f;
+    for (int w = 0; w < warps; ++w) v += part[w][t][row];
+    y[static_cast<int64_t>(t) * O + o0 + row] = __float2bfloat16_rn(v);
+  }
+}
+
+// Warps of a block: as many as there are lines of k; 8 at most where there are more blocks than SMs (D = 1024, F = 4096: 11.0 us a call, 12.4 with 16), 16 elsewhere
+template <int NT>
+int warps_for(int64_t k, int64_t blocks) {
+  const int64_t most = blocks <= sm_count() ? few_warps<NT>() : 8, lines = (k + FEW_LINE - 1) / FEW_LINE;
+  return static_cast<int>(imin64(most, lines));
+}
+template <int ACT, int NT, bool VEC>
+int few_rows(const GatedCall& c, __nv_bfloat16* h, cudaStream_t st) {
   using B = __nv_bfloat16;
-  constexpr int WARPS = GEMV_THREADS / 32;
-  gated_few_kernel<ACT, ROWS, VEC><<<static_cast<unsigned>((F + WARPS - 1) / WARPS), GEMV_THREADS, 0, st>>>(
-      static_cast<const B*>(x), ldx, static_cast<const B*>(wg), static_cast<const B*>(wu), static_cast<B*>(gate), static_cast<B*>(up), ldh, h, static_cast<int>(T), D, F);
+  const int D = static_cast<int>(c.D), F = static_cast<int>(c.F), O = static_cast<int>(c.O), T = static_cast<int>(c.T);
+  const int64_t up = (c.F + 15) / 16, down = (c.O + 15) / 16;
+  gated_few_kernel<ACT, NT, VEC><<<static_cast<unsigned>(up), 32 * warps_for<NT>(c.D, up), 0, st>>>(
+      static_cast<const B*>(c.x), c.ldx, static_cast<const B*>(c.wg), static_cast<const B*>(c.wu), static_cast<B*>(c.gate), static_cast<B*>(c.up), c.ldh, h, T, D, F);
   if (int rc = check_launch("gated_few_kernel")) return rc;
-  int warps = 1;
-  while (warps < WARPS && O * warps < static_cast<int64_t>(sm_count()) * 16 && F > warps * 256) warps *= 2;
-  return launch_behind(down_few_kernel<ROWS, VEC>, static_cast<unsigned>((O * warps + WARPS - 1) / WARPS), GEMV_THREADS, st, static_cast<const float*>(h), static_cast<const B*>(wd),
-                       static_cast<B*>(y), static_cast<int>(T), F, O, warps);
+  return launch_behind(down_few_kernel<NT, VEC>, static_cast<unsigned>(down), 32 * warps_for<NT>(c.F, down), st, static_cast<const B*>(h), static_cast<const B*>(c.wd),
+                       static_cast<B*>(c.y), T, F, O);
+}
+template <int ACT>
+int few_rows_act(const GatedCall& c, void* scratch, bool vec, cudaStream_t st) {
+  if (c.T == 1) return vec ? one_row<ACT, true>(c, static_cast<float*>(scratch), st) : one_row<ACT, false>(c, static_cast<float*>(scratch), st);
+  __nv_bfloat16* h = static_cast<__nv_bfloat16*>(scratch);
+  if (c.T <= 8) return vec ? few_rows<ACT, 1, true>(c, h, st) : few_rows<ACT, 1, false>(c, h, st);
+  if (c.T <= 16) return vec ? few_rows<ACT, 2, true>(c, h, st) : few_rows<ACT, 2, false>(c, h, st);
+  return vec ? few_rows<ACT, 4, true>(c, h, st) : few_rows<ACT, 4, false>(c, h, st);
 }
 
 // ---------------------------------------------------------------- host side
@@ -443,26 +603,18 @@ int by_form(bool narrow, F&& f) {
   return narrow ? f(Policy(), std::integral_constant<int, gemm::narrow<Policy>()>()) : f(Policy(), std::integral_constant<int, 256>());
 }
 
-template <int ACT>
-int few_rows_act(bool vec, int64_t T, const void* x, int64_t ldx, const void* wg, const void* wu, const void* wd, void* gate, void* up, int64_t ldh, void* y, float* h, int64_t D, int64_t F,
-                 int64_t O, cudaStream_t st) {
-#define HASTE_FEW(R) (vec ? few_rows<ACT, R, true>(x, ldx, wg, wu, wd, gate, up, ldh, y, h, T, D, F, O, st) : few_rows<ACT, R, false>(x, ldx, wg, wu, wd, gate, up, ldh, y, h, T, D, F, O, st))
-  return T == 1 ? HASTE_FEW(1) : T <= 4 ? HASTE_FEW(4) : HASTE_FEW(8);
-#undef HASTE_FEW
-}
-
 // arena.base == NULL: only what it takes, with aligned operands or with any
 int forward(Arena& arena, const GatedCall& c, cudaStream_t st) {
   const bool plan = arena.base == nullptr, any = plan && !c.aligned;
-  if (c.T <= GEMV_ROWS) {
-    float* h = static_cast<float*>(arena.take(c.T * c.F * 4));
+  if (c.T <= FEW_ROWS) {
+    void* h = arena.take(c.T * c.F * (c.T == 1 ? 4 : c.T <= EXACT_ROWS ? 6 : 2));
     if (plan) return HASTE_OK;
     const bool vec = c.D % 8 == 0 && c.F % 8 == 0 && c.ldx % 8 == 0 && aligned16(c.x) && aligned16(c.wg) && aligned16(c.wu) && aligned16(c.wd);
     switch (c.act) {
-      case SILU: return few_rows_act<SILU>(vec, c.T, c.x, c.ldx, c.wg, c.wu, c.wd, c.gate, c.up, c.ldh, c.y, h, c.D, c.F, c.O, st);
-      case GELU: return few_rows_act<GELU>(vec, c.T, c.x, c.ldx, c.wg, c.wu, c.wd, c.gate, c.up, c.ldh, c.y, h, c.D, c.F, c.O, st);
-      case GELU_TANH: return few_rows_act<GELU_TANH>(vec, c.T, c.x, c.ldx, c.wg, c.wu, c.wd, c.gate, c.up, c.ldh, c.y, h, c.D, c.F, c.O, st);
-      default: return few_rows_act<RELU>(vec, c.T, c.x, c.ldx, c.wg, c.wu, c.wd, c.gate, c.up, c.ldh, c.y, h, c.D, c.F, c.O, st);
+      case SILU: return few_rows_act<SILU>(c, h, vec, st);
+      case GELU: return few_rows_act<GELU>(c, h, vec, st);
+      case GELU_TANH: return few_rows_act<GELU_TANH>(c, h, vec, st);
+      default: return few_rows_act<RELU>(c, h, vec, st);
     }
   }
   const int64_t ldF = up8(c.F), sD = steps_of(c.D), sF = steps_of(c.F);

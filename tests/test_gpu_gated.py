@@ -238,3 +238,19 @@ def test_kept_projections_side_by_side(T, F):
     kept[:, 2 * up8:] = float("nan")                                       # and what is behind a row that is read does not count
     grads, from_halves = gated_backward(dy, x, wg, wu, wd, *want[1:]), gated_backward(dy, x, wg, wu, wd, gate[:, :F], up[:, :F])
     assert all(torch.equal(a, b) for a, b in zip(grads, from_halves))
+
+
+@pytest.mark.parametrize("sizes", [(72, 136, 40), (77, 131, 33), (1, 1, 1), (64, 2104, 24), (1160, 40, 2400), (513, 65, 17)])
+@pytest.mark.parametrize("T", [2, 3, 7, 8, 9, 15, 16, 17, 31, 32, 33])
+def test_few_rows(T, sizes):
+    """Around the steps of the forms for few rows: values, kept projections, rows that do not depend on their neighbours, whatever these hold."""
+    from haste_b200.feedforward import gated_forward
+    x, wg, wu, wd, _ = _inputs(T, *sizes)
+    got = gated_forward(x, wg, wu, wd, "gelu_tanh", keep=True)
+    _check(("y", "gate", "up"), got, *eo.gated(x, wg, wu, wd, "gelu_tanh"))
+    spoilt = x.clone()
+    spoilt[T // 2] = float("nan")
+    spoilt[0, -1] = float("inf")
+    y = gated_forward(spoilt, wg, wu, wd, "gelu_tanh")
+    others = [t for t in range(T) if t not in (0, T // 2)]
+    assert y[T // 2].isnan().all() and not y[0].isfinite().all() and torch.equal(y[others], got[0][others])
