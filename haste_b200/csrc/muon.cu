@@ -306,8 +306,9 @@ __device__ __forceinline__ uint4 random_words(const Coefficients& c, int64_t i) 
   uint32_t c0 = static_cast<uint32_t>(i), c1 = static_cast<uint32_t>(static_cast<uint64_t>(i) >> 32), c2 = c.stream, c3 = 2, k0 = c.seed, k1 = c.step;
 #pragma unroll
   for (int r = 0; r < 7; ++r) {
-    const uint32_t hi0 = __umulhi(0xD2511F53u, c0), lo0 = 0xD2511F53u * c0, hi1 = __umulhi(0xCD9E8D57u, c2), lo1 = 0xCD9E8D57u * c2;
-    c0 = hi1 ^ c1 ^ k0; c2 = hi0 ^ c3 ^ k1; c1 = lo1; c3 = lo0;
+    const uint64_t p0 = static_cast<uint64_t>(0xD2511F53u) * c0, p1 = static_cast<uint64_t>(0xCD9E8D57u) * c2;
+    c0 = static_cast<uint32_t>(p1 >> 32) ^ c1 ^ k0; c2 = static_cast<uint32_t>(p0 >> 32) ^ c3 ^ k1;
+    c1 = static_cast<uint32_t>(p1); c3 = static_cast<uint32_t>(p0);
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
@@ -341,6 +342,20 @@ __device__ __forceinline__ void store_weights(__nv_bfloat16* p, int have, const 
   }
 }
 
+// Four elements whose place in memory and in the momentum is a multiple of four
+__device__ __forceinline__ void store_whole(float* p, const float (&v)[4], const Coefficients&, int64_t) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store_whole(__nv_bfloat16* p, const float (&v)[4], const Coefficients& c, int64_t i) {
+  if (c.sr) {
+    const uint4 r = random_words(c, i >> 2);
+    uint32_t b[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(v[e]) + (b[e] & 0xFFFFu);          // the upper halves are what sr_bf16_bits() gives
+    *reinterpret_cast<uint2*>(p) = make_uint2(__byte_perm(b[0], b[1], 0x7632), __byte_perm(b[2], b[3], 0x7632));
+  } else {
+    *reinterpret_cast<uint2*>(p) = make_uint2(gemm::pack_bf16(v[0], v[1]), gemm::pack_bf16(v[2], v[3]));
+  }
+}
+
 // UPDATE: the weights; else X itself, in bf16
 template <class W, bool UPDATE, int N>
 __global__ void __launch_bounds__(256) muon_finish_kernel(const __grid_constant__ Matrices<N> t, const Coefficients c) {
@@ -360,8 +375,9 @@ __global__ void __launch_bounds__(256) muon_finish_kernel(const __grid_constant_
       float x[ROWS][4];
       const int64_t from = static_cast<int64_t>(row0 + r0) * a.cols + col, step = static_cast<int64_t>(16) * a.cols;
       const uint16_t* hi = a.hi + static_cast<int64_t>((tall ? col0 : row0) + r0) * a.ld + (tall ? row0 : col0) + cg;
+      const bool whole = row0 + SIDE <= a.rows && col0 + SIDE <= a.cols && a.cols % 4 == 0 && on_four(w);
       if (UPDATE) {
-        if (row0 + SIDE <= a.rows && col0 + SIDE <= a.cols && a.cols % 4 == 0 && on_four(w)) {
+        if (whole) {
 #pragma unroll
           for (int k = 0; k < ROWS; ++k) wr[k].load(w + from + k * step);
         } else {
@@ -397,7 +413,8 @@ __global__ void __launch_bounds__(256) muon_finish_kernel(const __grid_constant_
           if (UPDATE) wr[k].get(v);
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] = UPDATE ? fmaf(-a.rate * (1.f / X_SCALE), x[k][e], v[e] * c.decay) : x[k][e] * (1.f / X_SCALE);
-          store_weights(w + i, have, v, c, a.at + i);
+          if (whole) store_whole(w + i, v, c, a.at + i);
+          else store_weights(w + i, have, v, c, a.at + i);
         }
       }
     }
