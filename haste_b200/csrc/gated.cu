@@ -8,8 +8,8 @@
 // gradients.  Operands are bf16, sums fp32.  gate, up, h, dgate and dup are rounded to bf16 where they leave the chip: they are operands of the
 // next product or what training keeps, and 2^-8 of each value adds in squares to the result's own rounding.  Up to FEW_ROWS rows the weights are streamed through registers instead.
 //
-// Measured (bf16): forward with gate and up kept, T = 65536, D = O = 1024, F = 2048: 410 us for the first launch (1341 TFLOP/s), 176 for the second (1562); backward,
-// T = 16384, D = F = O = 4096: 402 us for dh (1368), 716 for dx (1535), 1173 for the weights' (1406).  The power limit bounds all of them, and the first launch of either direction
+// Measured (bf16): forward with gate and up kept, T = 65536, D = O = 1024, F = 2048: 404 us for the first launch (1361 TFLOP/s), 171 for the second (1608); backward,
+// T = 16384, D = F = O = 4096: 397 us for dh (1385), 701 for dx (1568), 1149 for the weights' (1435).  The power limit bounds all of them, and the first launch of either direction
 // the three matrices that its epilogue writes besides.
 #include "gemm_sm100.cuh"
 

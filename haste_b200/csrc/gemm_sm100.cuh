@@ -10,7 +10,7 @@
 // instead, with a stage less, a product whose epilogue reads two matrices and writes three took 450 us (16384 x 4096 x 4096; here 398), one that writes one 181 to 186 us
 // (65536 x 1024 x 2048; 173), one that writes three beside a longer sum 394 to 413 us (2 x 65536 x 2048 x 1024; 406).
 //
-// Bound: the tensor cores, and over more than some 100 us the power limit under them.  Alone, the products of the gated block run at 1340 to 1560 TFLOP/s, 82 to 95 % of
+// Bound: the tensor cores, and over more than some 100 us the power limit under them.  Alone, the products of the gated block run at 1360 to 1610 TFLOP/s, 83 to 98 % of
 // a library product's burst rate here (1640); in a stream of them both settle near 1370.
 //
 // TN = 256 is what keeps the tensor cores fed from L2; where there are fewer such tiles than pairs of SMs a narrow form (TN = 64, or 128 for a paired b) has more
