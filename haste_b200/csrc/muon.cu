@@ -440,16 +440,17 @@ struct Sizes {
 };
 Sizes sizes_of(int64_t rows, int64_t cols) { return {up64(std::min(rows, cols)), up64(std::max(rows, cols))}; }
 
-// The matrices with a gradient, by shape, cut into rounds
+// The matrices by shape, cut into rounds.  Rounds are those of the whole list, whichever of it have a gradient: fewer of them in a round need less, but other rounds could need more than the
+// scratch memory that was asked for.
 struct Plan {
   std::vector<int64_t> order;
   std::vector<size_t> rounds;      // where in `order` each begins, and the end
   int64_t bytes = 0;
 };
-Plan plan_of(const void* const* grads, const int64_t* rows, const int64_t* cols, int64_t count) {
+Plan plan_of(const int64_t* rows, const int64_t* cols, int64_t count) {
   Plan p;
   for (int64_t i = 0; i < count; ++i)
-    if ((grads == nullptr || grads[i] != nullptr) && rows[i] > 0 && cols[i] > 0) p.order.push_back(i);
+    if (rows[i] > 0 && cols[i] > 0) p.order.push_back(i);
   auto key = [&](int64_t i) { const Sizes s = sizes_of(rows[i], cols[i]); return std::make_pair(s.p, s.q); };
   std::stable_sort(p.order.begin(), p.order.end(), [&](int64_t i, int64_t j) { return key(i) > key(j); });
   int64_t used = 0;
@@ -495,11 +496,11 @@ int for_each_table(const std::vector<Matrix>& all, F&& f) {
 
 }  // namespace
 
-int64_t muon_scratch(const int64_t* rows, const int64_t* cols, int64_t count) { return plan_of(nullptr, rows, cols, count).bytes; }
+int64_t muon_scratch(const int64_t* rows, const int64_t* cols, int64_t count) { return plan_of(rows, cols, count).bytes; }
 
 int launch_muon(const MuonCall& c, cudaStream_t st) {
   if (int rc = report_pending_status(c.who)) return rc;
-  const Plan plan = plan_of(c.grads, c.rows, c.cols, c.count);
+  const Plan plan = plan_of(c.rows, c.cols, c.count);
   std::vector<int64_t> at(c.count);
   int64_t total = 0;
   for (int64_t i = 0; i < c.count; ++i) {
@@ -515,26 +516,30 @@ int launch_muon(const MuonCall& c, cudaStream_t st) {
   for (size_t r = 0; r + 1 < plan.rounds.size(); ++r) {
     char* mem = static_cast<char*>(c.scratch);
     auto take = [&](int64_t bytes) { char* p = mem; mem += up256(bytes); return p; };
-    const int64_t n = static_cast<int64_t>(plan.rounds[r + 1] - plan.rounds[r]);
+    std::vector<int64_t> some;         // those with a gradient
+    for (size_t i = plan.rounds[r]; i < plan.rounds[r + 1]; ++i)
+      if (c.grads[plan.order[i]] != nullptr) some.push_back(plan.order[i]);
+    if (some.empty()) continue;
+    const int64_t n = static_cast<int64_t>(some.size());
     auto* done = reinterpret_cast<unsigned long long*>(take(8 * (n + 1)));
     k.drawn = done + n;
     auto* parts = reinterpret_cast<double*>(take(8 * NORM_PARTS * n));
     int64_t elements = 0;
-    for (size_t i = plan.rounds[r]; i < plan.rounds[r + 1]; ++i) elements += c.rows[plan.order[i]] * c.cols[plan.order[i]];
+    for (int64_t o : some) elements += c.rows[o] * c.cols[o];
     // blocks of squares: 8 for every SM, shared by size
     const int64_t each = std::max<int64_t>(NORM_ELEMENTS, elements / (static_cast<int64_t>(sm_count()) * 8));
     std::vector<Matrix> all;
     std::vector<newton_schulz::Batch> batches;
-    for (size_t i = plan.rounds[r]; i < plan.rounds[r + 1];) {
-      const Sizes s = sizes_of(c.rows[plan.order[i]], c.cols[plan.order[i]]);
+    for (size_t i = 0; i < some.size();) {
+      const Sizes s = sizes_of(c.rows[some[i]], c.cols[some[i]]);
       size_t end = i;
-      while (end < plan.rounds[r + 1] && sizes_of(c.rows[plan.order[end]], c.cols[plan.order[end]]).p == s.p && sizes_of(c.rows[plan.order[end]], c.cols[plan.order[end]]).q == s.q) ++end;
+      while (end < some.size() && sizes_of(c.rows[some[end]], c.cols[some[end]]).p == s.p && sizes_of(c.rows[some[end]], c.cols[some[end]]).q == s.q) ++end;
       newton_schulz::Batch h;
       h.p = s.p; h.q = s.q; h.count = static_cast<int64_t>(end - i);
       for (uint16_t** x : {&h.hi[0], &h.hi[1], &h.lo}) *x = reinterpret_cast<uint16_t*>(take(2 * h.count * s.x()));
       h.B = reinterpret_cast<uint16_t*>(take(2 * h.count * s.a()));
       for (size_t j = i; j < end; ++j) {
-        const int64_t o = plan.order[j], x = static_cast<int64_t>(j - i) * s.x(), size = c.rows[o] * c.cols[o];
+        const int64_t o = some[j], x = static_cast<int64_t>(j - i) * s.x(), size = c.rows[o] * c.cols[o];
         Matrix m = {};
         m.g = c.grads[o]; m.w = c.params[o];
         m.m = c.momentum ? c.momentum + at[o] : nullptr;

@@ -1,5 +1,6 @@
 """Newton-Schulz steps and the Muon update against the 64-bit oracle: shapes, types, what a step leaves alone, random bits, the optimizer's state."""
 import copy
+import ctypes
 
 import numpy as np
 import pytest
@@ -296,3 +297,23 @@ def test_in_a_graph():
     version = w[0]._version
     muon_step(w, g, m, step=1)
     assert w[0]._version > version and m._version > 0
+
+
+def test_rounds_of_a_list_with_gaps():
+    """Matrices of more scratch memory than one round takes: without one of them the others stay in the rounds that the whole list's memory was asked for."""
+    from haste_b200 import _lib
+    from haste_b200.optim import moment_offsets, muon_step
+    shapes = [(64, 1677696), (64, 1258304), (64, 1090496)]
+    sizes = lambda which: ((ctypes.c_int64 * len(which))(*(shapes[i][0] for i in which)), (ctypes.c_int64 * len(which))(*(shapes[i][1] for i in which)), len(which))
+    assert _lib.lib.haste_muon_scratch(*sizes([0, 2])) > _lib.lib.haste_muon_scratch(*sizes([0, 1, 2])) > _lib.lib.haste_muon_scratch(*sizes([0]))
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    params = [torch.randn(s, generator=gen, device="cuda").to(BF) for s in shapes]
+    grads = [torch.randn(s, generator=gen, device="cuda").to(BF) for s in shapes]
+    alone = []
+    for i in (0, 2):
+        p = params[i].clone()
+        muon_step([p], [grads[i]], torch.zeros(p.numel(), device="cuda"), step=1, lr=0.1, stochastic_rounding=False)
+        alone.append(p)
+    before = params[1].clone()
+    muon_step(params, [grads[0], None, grads[2]], torch.zeros(moment_offsets([p.numel() for p in params])[-1], device="cuda"), step=1, lr=0.1, stochastic_rounding=False)
+    assert torch.equal(params[0], alone[0]) and torch.equal(params[1], before) and torch.equal(params[2], alone[1])
