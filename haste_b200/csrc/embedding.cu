@@ -496,12 +496,17 @@ __global__ void __launch_bounds__(JOIN_THREADS) embedding_join_kernel(const SumA
   // the first block whose tail is of this row: the last that started in an earlier row (or with this row's first token)
   int lo = 0, hi = b - 1;
   if (last < row) lo = hi;                         // nearly always the one before
-  while (lo < hi) {
-    const int c = (lo + hi + 1) >> 1;
-    const int32_t at = a.starts[c];
-    const int64_t i = static_cast<int64_t>(c) * a.units - at;
-    if (at < row || i == 0 || a.sorted[i - 1].x != row) lo = c;
-    else hi = c - 1;
+  while (lo < hi) {                                // by a warp, 32 at a time
+    const int step = (hi - lo + 31) / 32, c = lo + ((threadIdx.x & 31) + 1) * step;
+    bool before = false;
+    if (c <= hi) {
+      const int32_t at = a.starts[c];
+      const int64_t i = static_cast<int64_t>(c) * a.units - at;
+      before = at < row || i == 0 || a.sorted[i - 1].x != row;
+    }
+    const int n = __popc(__ballot_sync(0xffffffffu, before));
+    hi = min(hi, lo + (n + 1) * step - 1);
+    lo += n * step;
   }
   const float *t = a.tail + static_cast<int64_t>(lo) * a.D, *h = a.head + static_cast<int64_t>(b) * a.D;
   T* o = out + static_cast<int64_t>(row) * a.D;
