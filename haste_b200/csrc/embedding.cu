@@ -378,7 +378,7 @@ struct SumArgs {
 };
 
 // Bound: memory, and the wait for each block's first gradients: 65536 tokens of 1024 bf16 into 32000 rows 33 us (200 MB: 31 at a plain copy's rate).  With equal shares no word, however frequent, holds a
-// block up (a block for each row took 151 us a call, of now 61).  64 units a block instead of 128: 71 us a call.
+// block up (a block for each row took 151 us a call, of now 60).  64 units a block instead of 128: 71 us a call.
 // WHOLE: pieces of 16 bytes on both sides; else a thread has every SUM_THREADS-th element
 template <class G, class T, bool WHOLE>
 __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(const SumArgs a, const G* __restrict__ dy, T* __restrict__ out) {
@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(SUM_THREADS) embedding_sum_kernel(const SumArg
 }
 
 // A block whose first row was begun before it, and ends in it: the parts of the blocks before, in order, and its own.  11 us after 65536 tokens, 8 after 4099: the chain of the most frequent word's parts,
-// eight of which are on their way at once.
+// eight of which are on their way at once (sixteen: a call 1.5 us longer).
 constexpr int JOIN_THREADS = 256;
 template <class T>
 __global__ void __launch_bounds__(JOIN_THREADS) embedding_join_kernel(const SumArgs a, T* __restrict__ out) {

@@ -304,11 +304,16 @@ int one_row(const GatedCall& c, float* h, cudaStream_t st) {
 //   8 rows, here                                                          4.6          7.6          11.6          12.5          25.8
 //   8 rows, in CUDA cores                                                 9.0         15.8          24.2          34.5         104.8
 //   32 rows, here                                                         5.7          9.8          14.4          16.1          33.3
-//   32 rows, in tiles (as from 33 on)                                    14.5         18.4          22.2          23.5          35.7
+//   32 rows, in tiles                                                     14.5         18.4          22.2          23.5          35.7
 // The weights take 0.5, 1.4, 3.8, 4.8 and 15.4 us at the rate of memory: what is left is two launches, each with the latency of its first loads.
-constexpr int FEW_ROWS = 32;
+// With more weights than memory's latency hides, tiles catch up where 17 rows or more make a block read x as often as weights: 17 to 32 rows of 8192 x 8192 104 to 108 us here, 83 to 84 in
+// tiles, of 2048 x 16384 56 to 60 and 52 to 57 (but of 16384 x 2048 72 to 77 and 79 to 82); 8 and 16 rows of 8192 x 8192 90 and 78, 82 and 83 in tiles, of 16384 x 2048 48 and 45, 80.
+constexpr int FEW_ROWS = 32, FEW_ROWS_ALWAYS = 16;
+constexpr int64_t FEW_WEIGHTS = int64_t(1) << 26;      // elements of the three matrices
 constexpr int EXACT_ROWS = 8;      // h stays in 32 bits up to these, and is bf16 beyond, as in the tiled form
 constexpr int FEW_LINE = 64;       // k of a warp at a time: 128 bytes of each of its rows
+
+bool takes_few(const GatedCall& c) { return c.T <= FEW_ROWS_ALWAYS || (c.T <= FEW_ROWS && (2 * c.D + c.O) * c.F <= FEW_WEIGHTS); }
 
 template <int NT>
 constexpr int few_warps() { return NT == 4 ? 8 : 16; }       // of a block, at most: what their sums' place in shared memory allows
@@ -606,7 +611,7 @@ int by_form(bool narrow, F&& f) {
 // arena.base == NULL: only what it takes, with aligned operands or with any
 int forward(Arena& arena, const GatedCall& c, cudaStream_t st) {
   const bool plan = arena.base == nullptr, any = plan && !c.aligned;
-  if (c.T <= FEW_ROWS) {
+  if (takes_few(c)) {
     void* h = arena.take(c.T * c.F * (c.T == 1 ? 4 : c.T <= EXACT_ROWS ? 6 : 2));
     if (plan) return HASTE_OK;
     const bool vec = c.D % 8 == 0 && c.F % 8 == 0 && c.ldx % 8 == 0 && aligned16(c.x) && aligned16(c.wg) && aligned16(c.wu) && aligned16(c.wd);

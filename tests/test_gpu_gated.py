@@ -254,3 +254,11 @@ def test_few_rows(T, sizes):
     y = gated_forward(spoilt, wg, wu, wd, "gelu_tanh")
     others = [t for t in range(T) if t not in (0, T // 2)]
     assert y[T // 2].isnan().all() and not y[0].isfinite().all() and torch.equal(y[others], got[0][others])
+
+
+@pytest.mark.parametrize("T", [16, 17, 32])
+def test_few_rows_of_many_weights(T):
+    """Where the tiled form takes over earlier."""
+    from haste_b200.feedforward import gated_forward
+    x, wg, wu, wd, _ = _inputs(T, 2304, 11264, 1536)
+    _check(("y", "gate", "up"), gated_forward(x, wg, wu, wd, "silu", keep=True), *eo.gated(x, wg, wu, wd, "silu"))
