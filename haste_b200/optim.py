@@ -361,15 +361,16 @@ class Muon(Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for index, group in enumerate(self.param_groups):
+        types = [{p.dtype for p in group["params"] if p.grad is not None} for group in self.param_groups]
+        unknown = set().union(*types) - {torch.bfloat16, torch.float32}
+        if unknown:
+            raise RuntimeError(f"parameters must be torch.bfloat16 or torch.float32, got {', '.join(map(str, unknown))}")
+        for index, (group, types) in enumerate(zip(self.param_groups, types)):
             group["step_count"] += 1
-            types = {p.dtype for p in group["params"] if p.grad is not None}
             for k, dtype in enumerate((torch.bfloat16, torch.float32)):
                 if dtype in types:
                     params = [p for p in group["params"] if p.dtype == dtype]
                     self._step_type(group, self._flat((index, dtype), params), 2 * index + k)
-            if types - {torch.bfloat16, torch.float32}:
-                raise RuntimeError(f"parameters must be torch.bfloat16 or torch.float32, got {types - {torch.bfloat16, torch.float32}}")
         return loss
 
     def _step_type(self, group, m, stream_index):

@@ -447,7 +447,7 @@ int haste_gated_backward(const void* dy, const void* x, const void* wg, const vo
  *   m = mu m + (1 - mu) g,   u = mu m + (1 - mu) g (nesterov) or m,   X = u / max(|u|, eps)  (2-norm of all elements; transposed where rows > cols)
  *   `steps` times:  A = X X^T,  X = a X + (b A + c A A) X
  *   w = w (1 - lr weight_decay) - lr r X,   r = sqrt(max(1, rows / cols)) (adjust = HASTE_MUON_ORIGINAL) or 0.2 sqrt(max(rows, cols)) (HASTE_MUON_MATCH_RMS)
- * params, grads, rows, cols: host arrays, read before the call returns; parameters all of p_type, gradients of g_type, contiguous.  A matrix whose gradient is NULL is
+ * params, grads, rows, cols: host arrays, read before the call returns; parameters all of p_type, gradients of g_type, contiguous, no parameter twice.  A matrix whose gradient is NULL is
  * left alone, and so is one whose norm is inf or NaN, with its momentum.  momentum: fp32, 16-byte aligned, `moments` elements of room, matrix after
  * matrix, every one at a multiple of 256 elements.  Norms are 64 bits, momentum and weights' arithmetic 32, products take fp16 and sum in fp32
  * (X keeps 22 bits between them).  bf16 parameters are rounded stochastically with HASTE_F_SR, else to nearest: Philox4x32 with 7 rounds, key (lower half of

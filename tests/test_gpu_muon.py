@@ -317,3 +317,16 @@ def test_rounds_of_a_list_with_gaps():
     before = params[1].clone()
     muon_step(params, [grads[0], None, grads[2]], torch.zeros(moment_offsets([p.numel() for p in params])[-1], device="cuda"), step=1, lr=0.1, stochastic_rounding=False)
     assert torch.equal(params[0], alone[0]) and torch.equal(params[1], before) and torch.equal(params[2], alone[1])
+
+
+def test_a_type_that_is_refused_changes_nothing():
+    from haste_b200.optim import Muon
+    fine, other = (torch.nn.Parameter(torch.ones(8, 8, device="cuda", dtype=t)) for t in (BF, torch.float16))
+    opt = Muon([dict(params=[fine]), dict(params=[other])], lr=0.1)
+    fine.grad, other.grad = torch.randn_like(fine), torch.randn_like(other)
+    with pytest.raises(RuntimeError, match="float16"):
+        opt.step()
+    assert (fine == 1).all() and opt.param_groups[0]["step_count"] == 0
+    other.grad = None
+    opt.step()
+    assert not (fine == 1).all()
