@@ -112,7 +112,9 @@ struct GatedBackward {
   }
 };
 
-// out[0] = the product in bf16, or fp32 parts in `partial` [splits][M][N rounded up to 4]
+// Rows of fp32 parts: whole sectors, stored at once (in halves the weights' gradients of 333 rows, 509 x 1021, took 14.4 us, now 12)
+__host__ __device__ constexpr int64_t parts_ld(int64_t N) { return (N + 7) & ~int64_t(7); }
+// out[0] = the product in bf16, or fp32 parts in `partial` [splits][M][parts_ld(N)]
 template <bool A, bool B, int K_PARTS = 1>
 struct Plain {
   static constexpr bool A_MN = A, B_MN = B, PAIRED_B = false;
@@ -124,11 +126,11 @@ struct Plain {
     sm100::tmem_ld_wait();
     if (row >= p.M) return;
     if (p.partial != nullptr) {
-      const int64_t ld = (p.N + 3) & ~3;
+      const int64_t ld = parts_ld(p.N);
       float* to = p.partial + (static_cast<int64_t>(t.split) * p.M + row) * ld;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (col + 4 * i < ld) *reinterpret_cast<uint4*>(to + col + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      for (int i = 0; i < 4; ++i)
+        if (col + 8 * i < ld) gemm::store_32_bytes(to + col + 8 * i, v + 8 * i);
     } else {
       uint32_t packed[16];
 #pragma unroll
@@ -174,7 +176,7 @@ __global__ void sum_parts_kernel(const __grid_constant__ Sums s) {
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < s.first[s.n]; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     int k = 0;
     while (i >= s.first[k + 1]) ++k;
-    const int64_t ld = (s.cols[k] + 3) & ~int64_t(3), j = (i - s.first[k]) * 4, row = j / ld, col = j - row * ld, each = s.rows[k] * ld;
+    const int64_t ld = parts_ld(s.cols[k]), j = (i - s.first[k]) * 4, row = j / ld, col = j - row * ld, each = s.rows[k] * ld;
     float4 v = *reinterpret_cast<const float4*>(s.part[k] + j);
     for (int p = 1; p < s.splits[k]; ++p) {
       const float4 q = *reinterpret_cast<const float4*>(s.part[k] + p * each + j);
@@ -558,7 +560,7 @@ struct Output {
 };
 Output output_of(Arena& arena, void* p, int64_t M, int64_t N, const Form& f, bool always) {
   Output o = {p, nullptr, f.splits};
-  if (always || o.splits > 1 || N % 8 != 0 || !aligned16(p)) o.part = static_cast<float*>(arena.take(o.splits * M * ((N + 3) & ~int64_t(3)) * 4));
+  if (always || o.splits > 1 || N % 8 != 0 || !aligned16(p)) o.part = static_cast<float*>(arena.take(o.splits * M * parts_ld(N) * 4));
   return o;
 }
 void set_sizes(gemm::Sizes& p, int64_t M, int64_t N, int64_t steps0, int64_t steps) {
@@ -578,7 +580,7 @@ void add_sum(Sums& s, const Output& o, int64_t M, int64_t N) {
   const int k = s.n++;
   s.part[k] = o.part; s.out[k] = static_cast<__nv_bfloat16*>(o.p);
   s.rows[k] = M; s.cols[k] = N; s.ld_out[k] = N; s.splits[k] = o.splits;
-  s.first[k + 1] = s.first[k] + M * (((N + 3) & ~int64_t(3)) / 4);
+  s.first[k + 1] = s.first[k] + M * (parts_ld(N) / 4);
 }
 int run_sums(const Sums& s, cudaStream_t st) {
   if (s.n == 0) return HASTE_OK;

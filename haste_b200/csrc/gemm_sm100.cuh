@@ -111,7 +111,7 @@ struct Sizes {
   int first;                       // number of this problem's first tile; set by launch()
 };
 // A 16-bit matrix of the result's size that the policy reads or writes: rows of ld elements, of which the first `cols` (the result's columns, rounded up to a multiple of 8)
-// are read or written and what is behind them is others'.  on: the bytes that base, rows and cols are multiples of, 32 or 16 (with a third form for any, every lane storing its row's values one by one, the weights' gradients of 333 x 509 x 1021 took 43 us, through fp32 parts 14 and 6)
+// are read or written and what is behind them is others'.  on: the bytes that base, rows and cols are multiples of, 32 or 16 (with a third form for any, every lane storing its row's values one by one, the weights' gradients of 333 x 509 x 1021 took 43 us, through fp32 parts 12 and 6)
 struct Matrix16 {
   uint16_t* p;
   int64_t ld;
