@@ -320,18 +320,32 @@ __device__ __forceinline__ uint4 random_words(const Coefficients& c, int64_t i) 
 __device__ __forceinline__ uint32_t word(const uint4& r, int i) { return i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w; }
 
 __device__ __forceinline__ void store_weights(float* p, int have, const float (&v)[4], const Coefficients&, int64_t) { store4(p, have, vec4(p, have), v); }
+// No random bits for a NaN: it is 0x7FFFFFFF here, and adding any would run over into the sign and leave -0.  A sum that is no NaN has none among its terms: nearly always one test is all
+// that it takes.
+__device__ __forceinline__ void spare_nans(uint32_t (&random)[4], const float (&v)[4]) {
+  const float any = (v[0] + v[1]) + (v[2] + v[3]);
+  if (any != any) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (v[e] != v[e]) random[e] = 0;
+  }
+}
+
 __device__ __forceinline__ void store_weights(__nv_bfloat16* p, int have, const float (&v)[4], const Coefficients& c, int64_t i) {
   uint32_t b[4];
-  if (c.sr && (i & 3) == 0) {
-    const uint4 r = random_words(c, i >> 2);
-    b[0] = sr_bf16_bits(v[0], r.x & 0xFFFFu); b[1] = sr_bf16_bits(v[1], r.y & 0xFFFFu);
-    b[2] = sr_bf16_bits(v[2], r.z & 0xFFFFu); b[3] = sr_bf16_bits(v[3], r.w & 0xFFFFu);
-  } else if (c.sr) {
+  if (c.sr) {
     const uint4 first = random_words(c, i >> 2);
-    const int skip = static_cast<int>(i & 3);
-    const uint4 second = skip ? random_words(c, (i >> 2) + 1) : first;
+    if ((i & 3) == 0) {
+      b[0] = first.x; b[1] = first.y; b[2] = first.z; b[3] = first.w;
+    } else {
+      const int skip = static_cast<int>(i & 3);
+      const uint4 second = random_words(c, (i >> 2) + 1);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) b[e] = sr_bf16_bits(v[e], word(e + skip < 4 ? first : second, (e + skip) & 3) & 0xFFFFu);
+      for (int e = 0; e < 4; ++e) b[e] = word(e + skip < 4 ? first : second, (e + skip) & 3);
+    }
+    spare_nans(b, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = sr_bf16_bits(v[e], b[e] & 0xFFFFu);
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e) b[e] = rn_bf16_bits(v[e]);
@@ -351,6 +365,7 @@ __device__ __forceinline__ void store_whole(__nv_bfloat16* p, const float (&v)[4
   if (c.sr) {
     const uint4 r = random_words(c, i >> 2);
     uint32_t b[4] = {r.x, r.y, r.z, r.w};
+    spare_nans(b, v);
 #pragma unroll
     for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(v[e]) + (b[e] & 0xFFFFu);          // the upper halves are what sr_bf16_bits() gives
     *reinterpret_cast<uint2*>(p) = make_uint2(__byte_perm(b[0], b[1], 0x7632), __byte_perm(b[2], b[3], 0x7632));
