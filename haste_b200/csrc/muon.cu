@@ -39,7 +39,7 @@ struct Matrix {
   float* m;                        // momentum, NULL without
   uint16_t *hi, *lo;               // X's parts, rows of ld elements
   double* parts;                   // sums of squares, by block
-  unsigned long long* done;        // the steps' counter
+  unsigned long long *done, need;  // the steps' counter, and what it shows when they are complete
   int64_t at;                      // place in the momentum, for the random bits
   int rows, cols, ld, nparts;      // ld: X's columns, padded
   float rate;
@@ -186,6 +186,8 @@ __device__ __forceinline__ float inverse_norm(const Matrix& a, float eps) {
   return norm < eps ? 1.f / eps : ldexpf(1.f / root, -k);
 }
 __device__ __forceinline__ bool usable(float inverse) { return inverse > 0.f && inverse < INFINITY; }
+// Whether the steps' launch has done all of them: a wait may have run out in it, and then X's buffer holds something else
+__device__ __forceinline__ bool complete(const Matrix& a) { return __ldcg(a.done) == a.need; }
 
 // A block's share of all tiles of 64 x 64, one after the other: what a matrix needs is looked up once
 template <int N>
@@ -376,7 +378,7 @@ __device__ __forceinline__ void store_whole(__nv_bfloat16* p, const float (&v)[4
 
 // Bound: instruction issue (random words and rounding), then memory: 101 M bf16 weights rounded stochastically 159 us, 58 % of a plain copy's rate for 6 bytes an element; 170 with whole tiles stored as
 // the ragged ones are and random words from separate halves of products.  50 M elements of X alone, 4 bytes each: 44 us, 70 %.
-// UPDATE: the weights; else X itself, in bf16
+// UPDATE: the weights, left alone where the norm is not finite or the steps are not complete; else X itself, in bf16, NaN where they are not
 template <class W, bool UPDATE, int N>
 __global__ void __launch_bounds__(256) muon_finish_kernel(const __grid_constant__ Matrices<N> t, const Coefficients c) {
   __shared__ float turned[SIDE][SIDE + 1];
@@ -384,12 +386,14 @@ __global__ void __launch_bounds__(256) muon_finish_kernel(const __grid_constant_
   const int cg = (threadIdx.x & 15) * 4, r0 = threadIdx.x / 16;
   sm100::grid_dependency_wait();
   float inv = UPDATE && walk.more() ? inverse_norm(t.a[walk.k], c.eps) : 1.f;
+  bool done = walk.more() && complete(t.a[walk.k]);
   while (walk.more()) {
     const Matrix& a = t.a[walk.k];
     const int row0 = walk.row0, col0 = walk.col0, col = col0 + cg, have = min(4, a.cols - col);
     const bool tall = a.rows > a.cols;
     W* w = static_cast<W*>(a.w);
-    if (usable(inv)) {                             // the same for all of the block
+    if (!UPDATE || (done && usable(inv))) {     // the same for all of the block
+      const float unit = done ? 1.f / X_SCALE : __int_as_float(0x7FFFFFFF);
       Raw<W> wr[ROWS];
       uint2 q[ROWS];
       float x[ROWS][4];
@@ -432,13 +436,16 @@ __global__ void __launch_bounds__(256) muon_finish_kernel(const __grid_constant_
           float v[4];
           if (UPDATE) wr[k].get(v);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = UPDATE ? fmaf(-a.rate * (1.f / X_SCALE), x[k][e], v[e] * c.decay) : x[k][e] * (1.f / X_SCALE);
+          for (int e = 0; e < 4; ++e) v[e] = UPDATE ? fmaf(-a.rate * (1.f / X_SCALE), x[k][e], v[e] * c.decay) : x[k][e] * unit;
           if (whole) store_whole(w + i, v, c, a.at + i);
           else store_weights(w + i, have, v, c, a.at + i);
         }
       }
     }
-    if (walk.next() && UPDATE) inv = inverse_norm(t.a[walk.k], c.eps);
+    if (walk.next()) {
+      if (UPDATE) inv = inverse_norm(t.a[walk.k], c.eps);
+      done = complete(t.a[walk.k]);
+    }
   }
 }
 
@@ -571,7 +578,7 @@ int launch_muon(const MuonCall& c, cudaStream_t st) {
       batches.push_back(h);
       i = end;
     }
-    const bool gb = c.g_type == HASTE_BF16;
+    const bool gb = c.g_type == HASTE_BF16, narrow = newton_schulz::take_narrow(batches);
     int rc = for_each_table(all, [&](const auto& t, auto size, unsigned parts, unsigned tiles) -> int {
       constexpr int N = decltype(size)::value;
       if (gb) muon_squares_kernel<__nv_bfloat16, N><<<parts, NORM_THREADS, 0, st>>>(t, k);
@@ -580,12 +587,15 @@ int launch_muon(const MuonCall& c, cudaStream_t st) {
       return gb ? launch_behind(muon_start_kernel<__nv_bfloat16, N>, tiles, 256, st, t, k) : launch_behind(muon_start_kernel<float, N>, tiles, 256, st, t, k);
     });
     if (rc) return rc;
-    rc = newton_schulz::run(batches, done, k.drawn, c.steps, c.a, c.b, c.c, st);
+    rc = newton_schulz::run(batches, narrow, done, k.drawn, c.steps, c.a, c.b, c.c, st);
     if (rc) return rc;
-    if (c.steps & 1) {                 // X is in the other buffer
-      size_t k = 0;
-      for (const newton_schulz::Batch& h : batches)
-        for (int64_t j = 0; j < h.count; ++j, ++k) all[k].hi = h.hi[1] + j * h.p * h.q;
+    size_t at_matrix = 0;
+    for (const newton_schulz::Batch& h : batches) {
+      const unsigned long long need = newton_schulz::count_of(h, narrow, c.steps);
+      for (int64_t j = 0; j < h.count; ++j, ++at_matrix) {
+        all[at_matrix].need = need;
+        if (c.steps & 1) all[at_matrix].hi = h.hi[1] + j * h.p * h.q;          // X is in the other buffer
+      }
     }
     rc = for_each_table(all, [&](const auto& t, auto size, unsigned, unsigned tiles) -> int {
       constexpr int N = decltype(size)::value;

@@ -485,15 +485,32 @@ constexpr int64_t GROUP_BYTES = int64_t(250) << 20;
 
 inline int64_t bytes_of(const Batch& b) { return 2 * (2 * b.p * b.q + b.p * b.p); }      // of a matrix
 
+// Tiles of a product of one matrix: of A or B, on and below the diagonal, and of X
+struct Tiles {
+  int symmetric, full;
+};
+inline Tiles tiles_of(const Batch& b, int columns) {
+  const int m = static_cast<int>((b.p + TILE - 1) / TILE), n = static_cast<int>((b.p + columns - 1) / columns);
+  Tiles t = {0, static_cast<int>(m * ((b.q + columns - 1) / columns))};
+  for (int i = 0; i < m; ++i) t.symmetric += std::min((i + 1) * (TILE / columns), n);
+  return t;
+}
+inline int columns_of(bool narrow) { return narrow ? 64 : TILE; }
+// What a matrix's counter shows when all of its steps are complete; less where a wait has run out
+inline unsigned long long count_of(const Batch& b, bool narrow, int steps) {
+  const Tiles t = tiles_of(b, columns_of(narrow));
+  return static_cast<unsigned long long>(steps) * (2ull * t.symmetric + t.full) * (2 * EPI_WARPS);
+}
+
 template <int TN>
 int set_shape(Steps<TN>& w, int i, const Batch& b) {
   using gemm::make_map;
   Info& f = w.info[i];
   f.p = static_cast<int>(b.p); f.q = static_cast<int>(b.q);
   f.tiles_m = (f.p + TILE - 1) / TILE; f.tiles_n = (f.p + TN - 1) / TN; f.tiles_q = (f.q + TN - 1) / TN;
-  f.symmetric = 0;
-  for (int m = 0; m < f.tiles_m; ++m) f.symmetric += std::min((m + 1) * (TILE / TN), f.tiles_n);
-  f.full = f.tiles_m * f.tiles_q;
+  const Tiles t = tiles_of(b, TN);
+  f.symmetric = t.symmetric;
+  f.full = t.full;
   f.x[0] = b.hi[0]; f.x[1] = b.hi[1]; f.low = b.lo; f.b = b.B;
   CUtensorMap* m = w.map[i];
   int rc = 0;
@@ -610,9 +627,8 @@ inline bool take_narrow(const std::vector<Batch>& batches) {
   return gemm::cost_of(tiles[1] / groups, per, true, pairs) < gemm::cost_of(tiles[0] / groups, per, false, pairs);
 }
 
-// done: a counter for every matrix; drawn: one more.  All zeros.
-inline int run(const std::vector<Batch>& batches, unsigned long long* done, unsigned long long* drawn, int steps, double a, double b, double c, cudaStream_t st) {
-  const bool narrow = take_narrow(batches);
+// narrow: what take_narrow() says; done: a counter for every matrix; drawn: one more.  All zeros.
+inline int run(const std::vector<Batch>& batches, bool narrow, unsigned long long* done, unsigned long long* drawn, int steps, double a, double b, double c, cudaStream_t st) {
   size_t from = 0;
   int64_t start = 0;
   unsigned long long base = 0;

@@ -448,7 +448,8 @@ int haste_gated_backward(const void* dy, const void* x, const void* wg, const vo
  *   `steps` times:  A = X X^T,  X = a X + (b A + c A A) X
  *   w = w (1 - lr weight_decay) - lr r X,   r = sqrt(max(1, rows / cols)) (adjust = HASTE_MUON_ORIGINAL) or 0.2 sqrt(max(rows, cols)) (HASTE_MUON_MATCH_RMS)
  * params, grads, rows, cols: host arrays, read before the call returns; parameters all of p_type, gradients of g_type, contiguous, no parameter twice.  A matrix whose gradient is NULL is
- * left alone, and so is one whose norm is inf or NaN, with its momentum.  momentum: fp32, 16-byte aligned, `moments` elements of room, matrix after
+ * left alone, and so is one whose norm is inf or NaN, with its momentum.  Where a wait of the steps runs out (haste_poll_status) a matrix whose steps are not complete keeps its
+ * weights; its momentum is that after this step.  momentum: fp32, 16-byte aligned, `moments` elements of room, matrix after
  * matrix, every one at a multiple of 256 elements.  Norms are 64 bits, momentum and weights' arithmetic 32, products take fp16 and sum in fp32
  * (X keeps 22 bits between them).  bf16 parameters are rounded stochastically with HASTE_F_SR, else to nearest: Philox4x32 with 7 rounds, key (lower half of
  * seed, step), counter (i, i >> 32, stream_index, 2), the lower halves of its words for elements 4i .. 4i+3 of the momentum's buffer.
@@ -459,7 +460,7 @@ int haste_muon_step(void* const* params, const void* const* grads, const int64_t
                     int32_t g_type, double lr, double mu, int32_t nesterov, double weight_decay, int32_t adjust, int32_t steps, double a, double b, double c, double eps,
                     int64_t step, uint64_t seed, uint32_t stream_index, uint32_t flags, void* scratch, int64_t scratch_bytes, haste_stream_t stream);
 
-/* The steps alone: out[i] (bf16, contiguous) is X for u = in[i] (all of in_type), NaN where in[i] is not finite.  Scratch as above. */
+/* The steps alone: out[i] (bf16, contiguous) is X for u = in[i] (all of in_type), NaN where in[i] is not finite or a wait ran out before its steps were complete.  Scratch as above. */
 int haste_orthogonalize(const void* const* in, void* const* out, const int64_t* rows, const int64_t* cols, int64_t count, int32_t in_type, int32_t steps, double a, double b, double c,
                         double eps, void* scratch, int64_t scratch_bytes, haste_stream_t stream);
 
