@@ -447,12 +447,16 @@ __global__ void __launch_bounds__(few_warps<NT>() * 32, 1) down_few_kernel(const
     k0 += warps * FEW_LINE * (C / 2);
     if (k0 < F) fetch(k0);
   }
+  // Where the first parts' sum is not finite, infinite weights or h have made it so, and it is the result: the other parts of h, which may be zeros, would make NaN of an infinity.
 #pragma unroll
-  for (int k = 1; k < PARTS; ++k)
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int e = 0; e < 4; ++e) {
+      float sum = s[0][t][e];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[0][t][e] += s[k][t][e];
+      for (int k = 1; k < PARTS; ++k) sum += s[k][t][e];
+      if (fabsf(s[0][t][e]) < INFINITY) s[0][t][e] = sum;
+    }
   put_sums<NT>(part[warp], s[0], lane);
   __syncthreads();
   for (int i = threadIdx.x; i < 16 * T; i += blockDim.x) {

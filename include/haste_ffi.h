@@ -429,7 +429,7 @@ int haste_embedding_backward(const void* ids, int32_t id_bytes, const void* dy, 
 /* Gated feed-forward block, bf16: y = (act(x Wg^T) * (x Wu^T)) Wd^T with x [T, D] (row stride ldx), Wg, Wu [F, D], Wd [O, F] and y [T, O] contiguous; act: HASTE_ACT_*.
  * For training gate = x Wg^T and up = x Wu^T [T, F] (row stride ldh, a multiple of 8, 16-byte aligned) are kept, without NULL; of their rows F elements, rounded up to a
  * multiple of 8, may be written and nothing behind them.  Sums are fp32; the product
- * act(gate) * up is rounded to bf16 on its way to the second product (not for T <= 8, where an infinite weight may give NaN in place of an infinity).  Nothing else needs alignment; operands that have it (16-byte bases, row
+ * act(gate) * up is rounded to bf16 on its way to the second product (not for T <= 8).  Nothing else needs alignment; operands that have it (16-byte bases, row
  * strides and D, F, O multiples of 8) are read in place, others are copied first.
  * scratch: 256-byte aligned, haste_gated_forward_scratch(T, D, F, O, aligned) bytes, aligned = 0 unless all operands have that alignment. */
 int64_t haste_gated_forward_scratch(int64_t T, int64_t D, int64_t F, int64_t O, int32_t aligned);
