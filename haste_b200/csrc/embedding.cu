@@ -9,6 +9,7 @@
 // adds such parts, again in a fixed order.  Sums are fp32.
 #include "common.cuh"
 #include "launchers.h"
+#include "runtime.h"
 #include "sm100.cuh"
 
 #include <cooperative_groups.h>
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(const SortPass
   }
 }
 
-// Up to CLUSTER_MOST tokens (what the registers and shared memory of 16 blocks hold): one launch of one cluster, whose blocks keep the tokens in registers and shared memory.  In each pass every block places its tokens as above;
+// Up to CLUSTER_MOST tokens (what the registers and shared memory of 16 blocks hold), where the device can place it: one launch of one cluster, whose blocks keep the tokens in registers and shared memory.  In each pass every block places its tokens as above;
 // how many tokens of each digit the other blocks have comes through their shared memory, and so do the tokens themselves on their way to the block of their new place.
 // Bound: a pass's chain of latencies, some 8 us: 65536 tokens in two passes 18 us, 4099 in 8.  Whole backward calls of 128 columns, this way and through the launches above: 1000 tokens 16.0 and 28.1
 // us, 16384: 21.0 and 39.1, 65536: 32.9 and 45.8, 131072: 58.8 and 64.6.  Clusters of 8 blocks (which any device must have) took 32 us for the sort of 65536.
@@ -603,39 +604,50 @@ int64_t embedding_backward_scratch(int64_t tokens, int64_t D, int64_t V) {
   const int64_t blocks = (tokens + V + units_of(tokens, V, D) - 1) / units_of(tokens, V, D);
   const int64_t starts = 2 * up256(blocks * 4);
   if (tokens == 0) return starts;
-  const int64_t sorting = tokens <= CLUSTER_MOST ? up256(tokens * 8) : 2 * up256(tokens * 8) + up256(static_cast<int64_t>(sort_blocks(tokens)) * DIGITS * 4);
+  const int64_t sorting = 2 * up256(tokens * 8) + up256(static_cast<int64_t>(sort_blocks(tokens)) * DIGITS * 4);      // what sorting in several launches takes
   return sorting + starts + 2 * up256(blocks * D * 4);
 }
 
+// Whether the current device can place a cluster of so many blocks, which it is asked once.  It need not: more than 8 are beyond what every device has, and a part of one has fewer SMs side by side.
 template <int ITEMS>
-static int sort_in_cluster(const Ids& ids, int64_t tokens, int64_t V, int64_t padding, int2* out, cudaStream_t st) {
+static bool cluster_fits(cudaLaunchConfig_t& cfg, unsigned blocks) {
+  static std::atomic<int> known[64][CLUSTER_BLOCKS + 1];             // by device: 1 it can, -1 it cannot, 0 not asked yet
+  if (blocks > static_cast<unsigned>(cluster_limit())) return false;
   auto kernel = sort_cluster_kernel<ITEMS>;
-  static std::atomic<bool> allowed[64];            // by device
   int dev = 0;
   cudaGetDevice(&dev);
   const bool keep = dev >= 0 && dev < 64;
-  cudaError_t e = cudaSuccess;
-  if (!keep || !allowed[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, cluster_smem<ITEMS>());
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-    if (keep) allowed[dev].store(true, std::memory_order_release);
-  }
+  if (keep)
+    if (const int can = known[dev][blocks].load(std::memory_order_acquire)) return can > 0;
+  int clusters = 0;
+  const bool can = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, cluster_smem<ITEMS>()) == cudaSuccess &&
+                   cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                   cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0;
+  if (!can) cudaGetLastError();
+  if (keep) known[dev][blocks].store(can ? 1 : -1, std::memory_order_release);
+  return can;
+}
+
+// *sorted stays false where the cluster cannot be placed
+template <int ITEMS>
+static int sort_in_cluster(const Ids& ids, int64_t tokens, int64_t V, int64_t padding, int2* out, bool* sorted, cudaStream_t st) {
   unsigned blocks = 1;
   while (static_cast<int64_t>(blocks) * CLUSTER_THREADS * ITEMS < tokens) blocks *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks);
   cfg.blockDim = dim3(CLUSTER_THREADS);
   cfg.dynamicSmemBytes = cluster_smem<ITEMS>();
-  cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = blocks;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, ids, tokens, V, padding, passes_of(V), out);
+  if (!cluster_fits<ITEMS>(cfg, blocks)) return HASTE_OK;
+  cfg.stream = st;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, sort_cluster_kernel<ITEMS>, ids, tokens, V, padding, passes_of(V), out);
   if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaLaunchKernelEx: %s", cudaGetErrorString(e));
+  *sorted = true;
   return HASTE_OK;
 }
 
@@ -646,15 +658,17 @@ int launch_embedding_backward(const void* ids, int wide, const void* dy, void* d
   const Ids i = {ids, wide};
   int2* pairs[2] = {};
   int cur = 0;
+  bool sorted = false;
+  if (tokens > 0) pairs[0] = reinterpret_cast<int2*>(take(tokens * 8));
   if (tokens > 0 && tokens <= CLUSTER_MOST) {
-    pairs[0] = reinterpret_cast<int2*>(take(tokens * 8));
     int rc = 0;
-    if (tokens <= CLUSTER_MOST / 8) rc = sort_in_cluster<1>(i, tokens, V, padding, pairs[0], st);
-    else if (tokens <= CLUSTER_MOST / 2) rc = sort_in_cluster<4>(i, tokens, V, padding, pairs[0], st);
-    else rc = sort_in_cluster<8>(i, tokens, V, padding, pairs[0], st);
+    if (tokens <= CLUSTER_MOST / 8) rc = sort_in_cluster<1>(i, tokens, V, padding, pairs[0], &sorted, st);
+    else if (tokens <= CLUSTER_MOST / 2) rc = sort_in_cluster<4>(i, tokens, V, padding, pairs[0], &sorted, st);
+    else rc = sort_in_cluster<8>(i, tokens, V, padding, pairs[0], &sorted, st);
     if (rc) return rc;
-  } else if (tokens > 0) {
-    for (int k = 0; k < 2; ++k) pairs[k] = reinterpret_cast<int2*>(take(tokens * 8));
+  }
+  if (tokens > 0 && !sorted) {
+    pairs[1] = reinterpret_cast<int2*>(take(tokens * 8));
     SortPass s = {};
     s.n = tokens; s.blocks = sort_blocks(tokens);
     s.counts = reinterpret_cast<int32_t*>(take(static_cast<int64_t>(s.blocks) * DIGITS * 4));

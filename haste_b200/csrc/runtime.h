@@ -17,6 +17,8 @@ long long wait_limit_cycles();
 // stream finishes (only inside dependent_launch_scope(1), and unless switched off for measurement).
 int dependent_launch_enabled();
 void dependent_launch_scope(int on);
+// Test hook: blocks of the largest cluster that counts as one which the device can place.
+int cluster_limit();
 // Test hook: tile index at which the next debug step withholds one barrier arrival (-1 = none); reading clears it.
 int take_stall_tile();
 

@@ -213,6 +213,9 @@ int haste_debug_stall_next_step(int32_t tile);
  * reads anything); haste_debug_set_dependent_launch(0) launches it the ordinary way (measurement of the
  * difference).  haste_ffi_train_step on its own is always launched the ordinary way. */
 int haste_debug_set_dependent_launch(int32_t on);
+/* Test hook: larger clusters than this (default 16) count as ones that the device cannot place, and what would use them goes the other way (the embedding's gradient sorts in several
+ * launches). */
+int haste_debug_set_cluster_limit(int32_t blocks);
 
 /* Elementwise stochastic rounding fp32 -> bf16 with the reference stream over the flat index.
  * Replaces sr_triton.stochastic_rounding (shared_ffi/sr_triton.py:27-59). */
