@@ -23,7 +23,11 @@ int device_status_word(int** dev_ptr) {
   std::lock_guard<std::mutex> lock(g_mu);
   if (g_status_host == nullptr) {
     int* h = nullptr;
+    // The first launch may be one that a stream captures, during which allocations are refused unless the thread says that it means them: this one is no part of what is captured.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    const cudaError_t swapped = cudaThreadExchangeStreamCaptureMode(&mode);
     cudaError_t e = cudaHostAlloc(reinterpret_cast<void**>(&h), sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+    if (swapped == cudaSuccess) cudaThreadExchangeStreamCaptureMode(&mode);
     if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaHostAlloc(status word): %s", cudaGetErrorString(e));
     *h = 0;
     g_status_host = h;
