@@ -7,8 +7,8 @@
 // The list walks the matrices in groups: a group's A tiles, its B tiles, its X tiles, the next step, ..., then the next group.  Groups are large enough that what a tile waits for
 // was begun a product earlier by others (see GROUP_BYTES).
 // Every tile's predecessors stand before it in the list, a pair draws the next tile's number from a counter when it runs, and it works on its tiles in that order: the first unfinished
-// tile is with a pair that runs and has nothing before it, so it can always proceed, however many pairs the launch has got (it is a cooperative one besides).  Waits
-// are bounded as everywhere.
+// tile is with a pair that runs and has nothing before it, so it can always proceed, however many pairs of the launch run at once: it is an ordinary launch, not a cooperative one, which
+// a device may refuse.  Waits are bounded as everywhere.
 //
 // A and B are symmetric: only tiles on and below the diagonal are computed and stored.  Where an operand's block lies above it, the block on the other side is loaded and
 // read by the tensor core with its rows and columns exchanged.
@@ -598,6 +598,7 @@ int launch(const std::vector<Batch>& batches, size_t& from, int64_t& start, unsi
   constexpr auto kernel = &newton_schulz_kernel<TN>;
   int pairs = 0;
   if (int rc = gemm::pairs_resident<kernel>(Layout<TN>::SMEM_BYTES, &pairs)) return rc;
+  if (const int n = product_pairs()) pairs = n;
   pairs = static_cast<int>(imin64(pairs, tiles));
   base += static_cast<unsigned long long>(tiles) + pairs;          // every pair draws one number behind the last tile's
   cudaLaunchConfig_t cfg = {};
@@ -605,11 +606,6 @@ int launch(const std::vector<Batch>& batches, size_t& from, int64_t& start, unsi
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = Layout<TN>::SMEM_BYTES;
   cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeCooperative;          // its blocks wait for each other
-  attr.val.cooperative = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, w);
   if (e != cudaSuccess) return fail(HASTE_ERR_LAUNCH, "cudaLaunchKernelEx: %s", cudaGetErrorString(e));
   return HASTE_OK;

@@ -16,7 +16,7 @@ static std::mutex g_mu;
 static int* g_status_host = nullptr;
 static long long g_wait_limit = 4000000000ll;   // clock cycles (~2 s)
 static int g_stall_tile = -1;                   // test hook: consumed by the next debug step
-static std::atomic<int> g_cluster_limit{16};    // test hook
+static std::atomic<int> g_cluster_limit{16}, g_product_pairs{0};         // test hooks
 static int g_dependent_launch = 1;              // the fused step is launched with programmatic stream serialization
 
 int device_status_word(int** dev_ptr) {
@@ -60,6 +60,7 @@ static thread_local int t_dependent_scope = 0;
 void dependent_launch_scope(int on) { t_dependent_scope = on; }
 int dependent_launch_enabled() { return g_dependent_launch && t_dependent_scope; }
 int cluster_limit() { return g_cluster_limit.load(std::memory_order_relaxed); }
+int product_pairs() { return g_product_pairs.load(std::memory_order_relaxed); }
 int take_stall_tile() {
   std::lock_guard<std::mutex> lock(g_mu);
   const int t = g_stall_tile;
@@ -139,6 +140,12 @@ int haste_debug_set_dependent_launch(int on) {
 int haste_debug_set_cluster_limit(int blocks) {
   if (blocks < 0) return haste::fail(HASTE_ERR_BAD_ARG, "haste_debug_set_cluster_limit: %d blocks", blocks);
   haste::g_cluster_limit.store(blocks, std::memory_order_relaxed);
+  return HASTE_OK;
+}
+
+int haste_debug_set_product_pairs(int pairs) {
+  if (pairs < 0) return haste::fail(HASTE_ERR_BAD_ARG, "haste_debug_set_product_pairs: %d pairs", pairs);
+  haste::g_product_pairs.store(pairs, std::memory_order_relaxed);
   return HASTE_OK;
 }
 

@@ -19,6 +19,8 @@ int dependent_launch_enabled();
 void dependent_launch_scope(int on);
 // Test hook: blocks of the largest cluster that counts as one which the device can place.
 int cluster_limit();
+// Test hook: pairs of blocks that Newton-Schulz steps are launched with, 0: as many as run at once.
+int product_pairs();
 // Test hook: tile index at which the next debug step withholds one barrier arrival (-1 = none); reading clears it.
 int take_stall_tile();
 

@@ -216,6 +216,8 @@ int haste_debug_set_dependent_launch(int32_t on);
 /* Test hook: larger clusters than this (default 16) count as ones that the device cannot place, and what would use them goes the other way (the embedding's gradient sorts in several
  * launches). */
 int haste_debug_set_cluster_limit(int32_t blocks);
+/* Test hook: Newton-Schulz steps are launched with so many pairs of blocks, fewer or more than the device runs at once (0, the default: as many as it does).  They come to the same end. */
+int haste_debug_set_product_pairs(int32_t pairs);
 
 /* Elementwise stochastic rounding fp32 -> bf16 with the reference stream over the flat index.
  * Replaces sr_triton.stochastic_rounding (shared_ffi/sr_triton.py:27-59). */
