@@ -591,6 +591,14 @@ at::Tensor muon_workspace(int dev, const std::vector<int64_t>& rows, const std::
   return empty_on(dev, {bytes}, at::kByte);
 }
 
+// The number of Newton-Schulz steps: what does not fit the library's 32 bits is no other number of steps
+int32_t steps_of(PyObject* o) {
+  const long steps = PyLong_AsLong(o);
+  if (PyErr_Occurred()) throw python_error();
+  if (steps != static_cast<int32_t>(steps)) refuse("steps=" + std::to_string(steps) + " is out of range");
+  return static_cast<int32_t>(steps);
+}
+
 // (params, grads, momentum, step, lr, mu, nesterov, weight_decay, adjust, steps, a, b, c, eps, seed, stream_index, flags)
 PyObject* muon_step(PyObject* const* a) {
   const Sequence params(a[0]), grads(a[1]);
@@ -598,12 +606,13 @@ PyObject* muon_step(PyObject* const* a) {
   const int64_t step = PyLong_AsLongLong(a[3]);
   const double lr = PyFloat_AsDouble(a[4]), mu = PyFloat_AsDouble(a[5]), weight_decay = PyFloat_AsDouble(a[7]);
   const int nesterov = PyObject_IsTrue(a[6]);
-  const long adjust = PyLong_AsLong(a[8]), steps = PyLong_AsLong(a[9]);
+  const long adjust = PyLong_AsLong(a[8]);
   double number[4];                     // a, b, c, eps
   for (int i = 0; i < 4; ++i) number[i] = PyFloat_AsDouble(a[10 + i]);
   const uint64_t seed = PyLong_AsUnsignedLongLongMask(a[14]);
   const uint32_t stream_index = static_cast<uint32_t>(PyLong_AsUnsignedLongMask(a[15])), flags = static_cast<uint32_t>(PyLong_AsUnsignedLongMask(a[16]));
   if (PyErr_Occurred()) throw python_error();
+  const int32_t steps = steps_of(a[9]);
   const TensorList g(grads, "gradients");
   if (g.present == 0) Py_RETURN_NONE;       // nothing to do
   const TensorList p(params, "parameters");
@@ -634,7 +643,7 @@ PyObject* muon_step(PyObject* const* a) {
   const int64_t moments = m.numel();
   run(p.dev, "muon_step", [&](haste_stream_t st) {
     return lib.muon_step(const_cast<void* const*>(p.p.data()), g.p.data(), rows.data(), cols.data(), params.size(), mp, moments, p.types[0], g_type, lr, mu, nesterov, weight_decay,
-                         static_cast<int32_t>(adjust), static_cast<int32_t>(steps), number[0], number[1], number[2], number[3], step, seed, stream_index, flags, sp, bytes, st);
+                         static_cast<int32_t>(adjust), steps, number[0], number[1], number[2], number[3], step, seed, stream_index, flags, sp, bytes, st);
   });
   for (int64_t i = 0; i < params.size(); ++i)
     if (grads[i] != Py_None) written(THPVariable_Unpack(params[i]));
@@ -645,7 +654,7 @@ PyObject* muon_step(PyObject* const* a) {
 // (matrices, steps, a, b, c, eps) -> list of bf16 matrices
 PyObject* orthogonalize(PyObject* const* a) {
   const Sequence list(a[0]);
-  const long steps = PyLong_AsLong(a[1]);
+  const int32_t steps = steps_of(a[1]);
   double number[4];
   for (int i = 0; i < 4; ++i) number[i] = PyFloat_AsDouble(a[2 + i]);
   if (PyErr_Occurred()) throw python_error();
@@ -666,7 +675,7 @@ PyObject* orthogonalize(PyObject* const* a) {
     const at::Tensor scratch = muon_workspace(in.dev, rows, cols, bytes);
     void* sp = scratch.data_ptr();
     run(in.dev, "orthogonalize", [&](haste_stream_t st) {
-      return lib.orthogonalize(in.p.data(), to.data(), rows.data(), cols.data(), list.size(), in.types[0], static_cast<int32_t>(steps), number[0], number[1], number[2], number[3], sp, bytes, st);
+      return lib.orthogonalize(in.p.data(), to.data(), rows.data(), cols.data(), list.size(), in.types[0], steps, number[0], number[1], number[2], number[3], sp, bytes, st);
     });
   }
   PyObject* result = PyList_New(list.size());
