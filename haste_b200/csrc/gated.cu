@@ -9,8 +9,8 @@
 // next product or what training keeps, and 2^-8 of each value adds in squares to the result's own rounding.  Up to FEW_ROWS rows the weights are streamed through registers instead.
 //
 // Measured (bf16): forward with gate and up kept, T = 65536, D = O = 1024, F = 2048: 404 us for the first launch (1361 TFLOP/s), 171 for the second (1608); backward,
-// T = 16384, D = F = O = 4096: 397 us for dh (1385), 701 for dx (1568), 1149 for the weights' (1435).  The power limit bounds all of them, and the first launch of either direction
-// the three matrices that its epilogue writes besides.
+// T = 16384, D = F = O = 4096: 397 us for dh (1385), 701 for dx (1568), 1149 for the weights' (1435).  That is each launch alone; call after call the power limit bounds all of them (gemm_sm100.cuh), and
+// the first launch of either direction the three matrices that its epilogue writes besides.
 #include "gemm_sm100.cuh"
 
 #include <type_traits>
@@ -84,7 +84,8 @@ struct GatedForward {
   }
 };
 
-// The accumulator is dh; in[0] = gate, in[1] = up; out[0] = dgate, out[1] = dup, out[2] = h
+// The accumulator is dh; in[0] = gate, in[1] = up; out[0] = dgate, out[1] = dup, out[2] = h.  (The loop holds a row's piece of six matrices.  With erf in the narrow form and tanh in the wide one that is
+// more than 168 registers, and 76 and 32 bytes a thread go through local memory.  12 warps leave no more registers.)
 template <int ACT>
 struct GatedBackward {
   static constexpr bool A_MN = false, B_MN = true, PAIRED_B = false;
@@ -309,7 +310,8 @@ int one_row(const GatedCall& c, float* h, cudaStream_t st) {
 //   32 rows, in tiles                                                     14.5         18.4          22.2          23.5          35.7
 // The weights take 0.5, 1.4, 3.8, 4.8 and 15.4 us at the rate of memory: what is left is two launches, each with the latency of its first loads.
 // With more weights than memory's latency hides, tiles catch up where 17 rows or more make a block read x as often as weights: 17 to 32 rows of 8192 x 8192 104 to 108 us here, 83 to 84 in
-// tiles, of 2048 x 16384 56 to 60 and 52 to 57 (but of 16384 x 2048 72 to 77 and 79 to 82); 8 and 16 rows of 8192 x 8192 90 and 78, 82 and 83 in tiles, of 16384 x 2048 48 and 45, 80.
+// tiles, of 2048 x 16384 56 to 60 and 52 to 57; of 16384 x 2048 72 to 77 and 79 to 82, where this rule by the number of weights alone takes the slower form.  8 and 16 rows of 8192 x 8192 90 and 78,
+// 82 and 83 in tiles, of 16384 x 2048 48 and 45, 80.
 constexpr int FEW_ROWS = 32, FEW_ROWS_ALWAYS = 16;
 constexpr int64_t FEW_WEIGHTS = int64_t(1) << 26;      // elements of the three matrices
 constexpr int EXACT_ROWS = 8;      // h stays in 32 bits up to these, and is bf16 beyond, as in the tiled form

@@ -11,7 +11,8 @@
 // (65536 x 1024 x 2048; 173), one that writes three beside a longer sum 394 to 413 us (2 x 65536 x 2048 x 1024; 406).
 //
 // Bound: the tensor cores, and over more than some 100 us the power limit under them.  Alone, the products of the gated block run at 1360 to 1610 TFLOP/s, 83 to 98 % of
-// a library product's burst rate here (1640); in a stream of them both settle near 1370.
+// a library product's burst rate here (1640), with the tensor pipe 75 to 81 % busy and L2 at 55 and 37 % of its rate.  Call after call, at the power limit (993 W), clocks fall to 1250 MHz: the block's
+// forward pass settles at 1150 TFLOP/s, its backward pass at 1237; a library's two products of the forward pass alone, with nothing applied or kept, at 1238 (1425 MHz), of 8192^3 at 1408 (1335 MHz).
 //
 // TN = 256 is what keeps the tensor cores fed from L2; where there are fewer such tiles than pairs of SMs a narrow form (TN = 64, or 128 for a paired b) has more
 // and shorter ones: cost_of() weighs both.  The gradients of a gated block of 333 rows, 509 x 1021: 57 us with the wide form alone, 43 with both.
@@ -416,7 +417,19 @@ int pairs_resident(int smem, int* pairs) {
   return HASTE_OK;
 }
 
-// Time of a launch of `tiles` tiles of `steps` steps of k each, in units of a step of the wide form (0.28 us)
+// Time of a launch of `tiles` tiles of `steps` steps of k each, in units of a step of the wide form (0.28 us).  Both forms, us a call (all launches of a call in the form, or as the rule has them):
+//                                        rule   wide  narrow                                     rule   wide  narrow
+//   forward       40 x  512 x 1024       14.9   17.8    14.9      steps, one   64 x 64            72.2  101.7    72.1
+//                333 x 1024 x 2048       21.4   25.2    21.3                  512 x 768          117.7  149.2   117.1
+//               1024 x  768 x 2048       23.3   26.2    24.4                 1024 x 1024         178.2  186.7   172.6
+//               1024 x 4096 x 4096       78.8   79.2   127.0                 2048 x 2048         354.9  338.9   445.2
+//               4096 x 1024 x 2048       48.8   47.7    71.9      steps,  4 of 768 x 768         175.9  175.0   174.5
+//              16384 x 1024 x 2048      158.5  159.0   246.3               20 of 256 x 512       144.7  144.9   139.9
+//   gradients     40 x  512 x 1024       23.1   28.3    23.0               40 of 256 x 512       173.4  174.2   186.9
+//                333 x 1024 x 2048       36.1   42.9    42.0               40 of 512 x 512       249.2  250.7   434.8
+//               1024 x  768 x 2048       47.0   45.2    56.3              100 of  64 x 128       105.7  136.6   105.6
+//              16384 x 1024 x 2048      369.9  404.7   825.6
+// It is 5 % off where both are close: it does not know of the parts that an epilogue of fp32 stores, nor that narrow tiles of Newton-Schulz wait for fewer others.
 inline double cost_of(int64_t tiles, int64_t steps, bool is_narrow, int64_t pairs) {
   return static_cast<double>((tiles + pairs - 1) / pairs) * (is_narrow ? 0.6 * static_cast<double>(steps) + 3.5 : static_cast<double>(steps) + 6.0);
 }

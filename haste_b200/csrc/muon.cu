@@ -8,10 +8,10 @@
 // zeros: so matrices of nearly one size are one batch), one for all steps (newton_schulz.cuh), one that updates the weights.
 //
 // Rounding.  The products take fp16: X times 2^8 (its entries are at most 1, later 1.3 or so; the factor keeps small ones out of the subnormals), A and
-// B.  By the term a I small singular values grow 3.4 times a step, and so does what rounding X adds to them; it takes X as a sum of two fp16 values, hi + lo 2^-11:
-// 22 bits.  Without lo an update of low rank with noise is off by 1.3e-2 after five steps (2-norm of the difference over that of the result), with it in the first three by
-// 1.4e-3, and so is a Gaussian one; with bf16 in place of fp16 1e-1 and 1e-2.  A and A A are symmetric: tiles on and below the diagonal are computed, the others are
-// their mirror.
+// B = a I + b A + c A A.  By the term a I small singular values grow 3.4 times a step, and so does what rounding X adds to them: up to the last but two steps a X takes X as a sum of two fp16 values,
+// hi + lo 2^-11, 22 bits, while hi goes through B; in the last two steps X has hi's 11 bits.  Without lo an update of low rank with noise is off by 1.3e-2 after five steps (2-norm of the difference
+// over that of the result), with it in the first three by 2.2e-3 at most and a Gaussian one by 1.2e-3 to 1.7e-3 (of 300 x 40: 2.9e-3); with lo in all steps and a outside B 5e-4, with bf16 in place of
+// fp16 1e-1 and 1e-2.  The result's own rounding to bf16 is 1.7e-3.  A and A A are symmetric: tiles on and below the diagonal are computed, the others are their mirror.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -376,8 +376,8 @@ __device__ __forceinline__ void store_whole(__nv_bfloat16* p, const float (&v)[4
   }
 }
 
-// Bound: instruction issue (random words and rounding), then memory: 101 M bf16 weights rounded stochastically 159 us, 58 % of a plain copy's rate for 6 bytes an element; 170 with whole tiles stored as
-// the ragged ones are and random words from separate halves of products.  50 M elements of X alone, 4 bytes each: 44 us, 70 %.
+// Bound: instruction issue (random words and rounding), then memory: 101 M bf16 weights rounded stochastically 164 us, 56 % of a plain copy's rate for 6 bytes an element; 11 more with whole tiles stored as
+// the ragged ones are and random words from separate halves of products.  50 M elements of X alone, 4 bytes each: 47 us, 65 %.
 // UPDATE: the weights, left alone where the norm is not finite or the steps are not complete; else X itself, in bf16, NaN where they are not
 template <class W, bool UPDATE, int N>
 __global__ void __launch_bounds__(256) muon_finish_kernel(const __grid_constant__ Matrices<N> t, const Coefficients c) {

@@ -13,9 +13,9 @@
 // A and B are symmetric: only tiles on and below the diagonal are computed and stored.  Where an operand's block lies above it, the block on the other side is loaded and
 // read by the tensor core with its rows and columns exchanged.
 //
-// Bound, many matrices: 50 M elements in matrices of 768 x 768 and 768 x 2048, 5 steps: 870 us, 820 TFLOP/s, 60 % of what a library's product sustains; 101 M of 1024 x 1024 and 1024 x 2048: 1990 us, 990.
+// Bound, many matrices: 50 M elements in matrices of 768 x 768 and 768 x 2048, 5 steps: 860 us, 830 TFLOP/s, 61 % of what a library's product sustains; 101 M of 1024 x 1024 and 1024 x 2048: 1909 us, 1030.
 // Products alone, without inputs and stores, take two thirds of that with these stages: the rest is stores into lines that L2 keeps for both dies, and waits for what they
-// count.  Bound, one matrix: latency; 512 x 768 110 us, 15 products of 7.3: 1.1 from the count to the first operands, 1.7 until the last of them has come at an SM's share of L2's rate,
+// count.  Nothing is at its rate meanwhile: tensor pipe 57 % busy, L2 at 53 % (11.4 GB), DRAM at 41 % (2.6 GB).  Bound, one matrix: latency; 512 x 768 110 us, 15 products of 7.3: 1.1 from the count to the first operands, 1.7 until the last of them has come at an SM's share of L2's rate,
 // 1 for the epilogue, 1 until its stores have arrived, 1 until the count has and is seen.
 //
 // Tiles are 256 x TN of a pair, with roles, barriers and an epilogue as in gemm_sm100.cuh; warp 3 looks up what comes next and waits for it, ahead of the others.

@@ -456,7 +456,7 @@ int haste_gated_backward(const void* dy, const void* x, const void* wg, const vo
  * left alone, and so is one whose norm is inf or NaN, with its momentum.  Where a wait of the steps runs out (haste_poll_status) a matrix whose steps are not complete keeps its
  * weights; its momentum is that after this step.  momentum: fp32, 16-byte aligned, `moments` elements of room, matrix after
  * matrix, every one at a multiple of 256 elements.  Norms are 64 bits, momentum and weights' arithmetic 32, products take fp16 and sum in fp32
- * (X keeps 22 bits between them).  bf16 parameters are rounded stochastically with HASTE_F_SR, else to nearest: Philox4x32 with 7 rounds, key (lower half of
+ * (X keeps 22 bits between them up to the last two steps, 11 in these; a is rounded to fp16 with the rest of a I + b A + c A A).  bf16 parameters are rounded stochastically with HASTE_F_SR, else to nearest: Philox4x32 with 7 rounds, key (lower half of
  * seed, step), counter (i, i >> 32, stream_index, 2), the lower halves of its words for elements 4i .. 4i+3 of the momentum's buffer.
  * eps is 2^-100 at least.  scratch: 256-byte aligned, haste_muon_scratch(...) bytes: 6 an element and 2 for every pair of rows of X (with sides rounded up to
  * multiples of 64), 1 GB at most unless one matrix needs more (matrices are then worked on in rounds). */
