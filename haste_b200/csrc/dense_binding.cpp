@@ -100,6 +100,13 @@ std::pair<at::Tensor, int64_t> rows_of(const at::Tensor& t, int64_t D) {
   return {r, r.size(0) > 1 ? r.stride(0) : D};
 }
 
+// rows_of, but with rows that do not overlap
+std::pair<at::Tensor, int64_t> own_rows_of(const at::Tensor& t, int64_t D) {
+  auto r = rows_of(t, D);
+  if (r.second < D) return {r.first.contiguous(), D};
+  return r;
+}
+
 struct Rows {
   int dev, type;
   int64_t D;
@@ -394,7 +401,7 @@ PyObject* embedding_forward(PyObject* const* a) {
   const double scale = PyFloat_AsDouble(a[2]);
   if (PyErr_Occurred()) throw python_error();
   const int64_t V = table.size(0), D = table.size(1), tokens = ids.t.numel();
-  const auto [src, stride] = rows_of(table, D);
+  const auto [src, stride] = own_rows_of(table, D);
   std::vector<int64_t> sizes(ids.t.sizes().begin(), ids.t.sizes().end());
   sizes.push_back(D);
   at::Tensor y = empty_on(dev, sizes, table.scalar_type());
@@ -470,12 +477,6 @@ GatedSizes check_gated(PyObject* const* a) {
   if (wg.size(1) != s.D || !wu.sizes().equals(wg.sizes()) || wd.size(1) != s.F)
     refuse("w_gate and w_up must be [F, " + std::to_string(s.D) + "], w_down [O, F], got " + text(wg.sizes()) + ", " + text(wu.sizes()) + " and " + text(wd.sizes()));
   return s;
-}
-// rows_of, but with rows that do not overlap
-std::pair<at::Tensor, int64_t> own_rows_of(const at::Tensor& t, int64_t D) {
-  auto r = rows_of(t, D);
-  if (r.second < D) return {r.first.contiguous(), D};
-  return r;
 }
 bool on16(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
 // rows x F, a row's stride a multiple of 8
