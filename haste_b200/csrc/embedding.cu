@@ -620,11 +620,12 @@ static bool cluster_fits(cudaLaunchConfig_t& cfg, unsigned blocks) {
   if (keep)
     if (const int can = known[dev][blocks].load(std::memory_order_acquire)) return can > 0;
   int clusters = 0;
-  const bool can = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, cluster_smem<ITEMS>()) == cudaSuccess &&
-                   cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
-                   cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0;
-  if (!can) cudaGetLastError();
-  if (keep) known[dev][blocks].store(can ? 1 : -1, std::memory_order_release);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, cluster_smem<ITEMS>());
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg);
+  const bool can = e == cudaSuccess && clusters > 0;
+  if (e != cudaSuccess) cudaGetLastError();                          // no answer: it is asked again
+  else if (keep) known[dev][blocks].store(can ? 1 : -1, std::memory_order_release);
   return can;
 }
 
