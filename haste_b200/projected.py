@@ -26,11 +26,16 @@ class ProjectedFusedStep:
             raise ValueError(f"the projection has {projection.out_features} outputs, the norm {norm.features} features, the sparse layer {shard.D}")
         if projection.weight.dtype != torch.bfloat16:
             raise ValueError("the projection must be bf16, as the sparse layer's features are")
-        self.optimizers = list(optimizer) if isinstance(optimizer, (list, tuple)) else [optimizer]
+        self.optimizer = optimizer
         held = {id(p) for o in self.optimizers for group in o.param_groups for p in group["params"]}
         if any(id(p) not in held for m in (projection, norm) for p in m.parameters()):
             raise ValueError("the optimizer must hold the projection's and the norm's parameters")
-        self.projection, self.norm, self.shard, self.optimizer = projection, norm, shard, optimizer
+        self.projection, self.norm, self.shard = projection, norm, shard
+
+    @property
+    def optimizers(self):
+        """``optimizer`` as a list: what ``update`` steps."""
+        return list(self.optimizer) if isinstance(self.optimizer, (list, tuple)) else [self.optimizer]
 
     @torch.no_grad()
     def step(self, h, targets, want_loss=True):
