@@ -420,14 +420,18 @@ int pairs_resident(int smem, int* pairs) {
 // Time of a launch of `tiles` tiles of `steps` steps of k each, in units of a step of the wide form (0.28 us).  Both forms, us a call (all launches of a call in the form, or as the rule has them):
 //                                        rule   wide  narrow                                     rule   wide  narrow
 //   forward       40 x  512 x 1024       14.9   17.8    14.9      steps, one   64 x 64            72.2  101.7    72.1
-//                333 x 1024 x 2048       21.4   25.2    21.3                  512 x 768          117.7  149.2   117.1
-//               1024 x  768 x 2048       23.3   26.2    24.4                 1024 x 1024         178.2  186.7   172.6
-//               1024 x 4096 x 4096       78.8   79.2   127.0                 2048 x 2048         354.9  338.9   445.2
-//               4096 x 1024 x 2048       48.8   47.7    71.9      steps,  4 of 768 x 768         175.9  175.0   174.5
-//              16384 x 1024 x 2048      158.5  159.0   246.3               20 of 256 x 512       144.7  144.9   139.9
-//   gradients     40 x  512 x 1024       23.1   28.3    23.0               40 of 256 x 512       173.4  174.2   186.9
-//                333 x 1024 x 2048       36.1   42.9    42.0               40 of 512 x 512       249.2  250.7   434.8
-//               1024 x  768 x 2048       47.0   45.2    56.3              100 of  64 x 128       105.7  136.6   105.6
+//                 64 x  768 x 2048       16.4   20.0    16.4                  512 x 768          117.7  149.2   117.1
+//                333 x 1024 x 2048       21.4   25.2    21.3                 1024 x 1024         178.2  186.7   172.6
+//               1024 x  768 x 2048       23.3   26.2    24.4                 2048 x 2048         354.9  338.9   445.2
+//               1024 x 4096 x 4096       78.8   79.2   127.0      steps,  4 of 768 x 768         175.9  175.0   174.5
+//               2048 x 1024 x 2048       36.9   36.8    43.8               20 of 256 x 512       144.7  144.9   139.9
+//               4096 x 1024 x 2048       48.8   47.7    71.9               40 of 256 x 512       173.4  174.2   186.9
+//              16384 x 1024 x 2048      158.5  159.0   246.3               40 of 512 x 512       249.2  250.7   434.8
+//   gradients     40 x  512 x 1024       23.1   28.3    23.0              100 of  64 x 128       105.7  136.6   105.6
+//                 64 x  768 x 2048       24.7   31.5    27.7
+//                333 x 1024 x 2048       36.1   42.9    42.0
+//               1024 x  768 x 2048       47.0   45.2    56.3
+//               4096 x 1024 x 2048      106.2  106.5   212.8
 //              16384 x 1024 x 2048      369.9  404.7   825.6
 // It is 5 % off where both are close: it does not know of the parts that an epilogue of fp32 stores, nor that narrow tiles of Newton-Schulz wait for fewer others.
 inline double cost_of(int64_t tiles, int64_t steps, bool is_narrow, int64_t pairs) {
