@@ -5,7 +5,8 @@
 //   w = w (1 - lr weight_decay) - lr rate X
 //
 // For a list of matrices at once: one launch for the norms, one that writes the momentum and X (rows and columns padded with zeros to multiples of 64, which stay
-// zeros: so matrices of nearly one size are one batch), one for all steps (newton_schulz.cuh), one that updates the weights.
+// zeros: so matrices of nearly one size are one batch), one for all steps (newton_schulz.cuh), one that updates the weights.  Matrices with a side of 32 or less take three others, in 64 bits ("few rows"
+// below).
 //
 // Rounding.  The products take fp16: X times 2^8 (its entries are at most 1, later 1.3 or so; the factor keeps small ones out of the subnormals), A and
 // B = a I + b A + c A A.  By the term a I small singular values grow 3.4 times a step, and so does what rounding X adds to them: up to the last but two steps a X takes X as a sum of two fp16 values,
@@ -449,6 +450,284 @@ __global__ void __launch_bounds__(256) muon_finish_kernel(const __grid_constant_
   }
 }
 
+// ---------------------------------------------------------------- few rows
+// X of at most FEW_ROWS rows.  A few roundings of A and B to fp16 do not average out: steps with the products above are off by up to 1.2e-2 for 2 x 3 and 6.9e-3 for 2 x 300 (worst of 400), 4.3e-3 for
+// 8 x 30, 3.1e-3 for 24 x 300, 2.4e-3 for 32 x 300; from 33 rows on by 2.3e-3, where rounding the result alone gives 1.7e-3.  All X_k are polynomials of G = u u^T times u, and G is p x p:
+//   X_k = F_k u,   A_k = F_k G F_k,   M = a I + b A_k + c A_k A_k,   F_{k+1} = M F_k,   A_{k+1} = M (M A_k)        (symmetric matrices that commute)
+// All of that is in 64 bits: F grows 3.4 times a step where singular values are small, and what G is rounded to with its square, so that 32 bits would leave 1e-3.  One launch for G, in parts along the
+// longer side, one that adds them and takes the steps, one for F u and what is done with it.  Nothing is rounded to fewer than 32 bits but the result.
+//
+// Bound: the 64-bit products (16 a clock and SM) of the one block that takes a matrix's steps, 5 us for 16 rows and 20 for 32, and three launches' latency; long ones by those of G and F u.  A call, in
+// brackets with the products above: 8 x 8 15 us (66), 32 x 32 31 (66), 32 x 768 41 (85), 16 x 4096 25 (158), 30 x 40000 80 (1020), 32 x 1000000 859 (23410), 40 of 20 x 300 50 (109), 200 of 32 x 512
+// 213 (301).  Beside larger matrices the three launches come first: 512 x 768 and 20 of 16 x 1000 147 (182), 512 x 768 and 8 of 32 x 32 150 (129).
+constexpr int FEW_ROWS = 32, FEW_THREADS = 256;
+constexpr int FEW_SLOTS = 2048;                    // elements that a block has at a time: 8 a thread
+constexpr int GRAM_LOOPS = 4, GRAM_PARTS = 128;    // times so many for a part of G at least, and its parts at most
+static_assert(FEW_SLOTS == 8 * FEW_THREADS, "");
+
+__host__ __device__ __forceinline__ int log_rows(int p) { return p <= 4 ? 2 : p <= 8 ? 3 : p <= 16 ? 4 : 5; }        // of X's rows in a block, a power of two
+// G's tiles of 4 x 4 on and below the diagonal, all of one part after the other's
+__host__ __device__ __forceinline__ int gram_tiles(int p) { const int n = (p + 3) >> 2; return n * (n + 1) / 2; }
+__host__ __device__ __forceinline__ int gram_size(int p) { return 16 * gram_tiles(p); }
+
+// A thread's 8 elements of the direction from place j0 along the longer side on, zeros beyond it: all loads are on their way before one is looked at (looked at one by one they took 4 us of 5)
+template <class G>
+struct Eight {
+  G g[8];
+  float m[8];
+  int64_t at[8];                   // in the matrix, -1 where there is none
+  int to[8];                       // row * rows' stride + place, or the other way round
+  // by_row: whether a row's places are neighbours in shared memory
+  __device__ __forceinline__ void load(const Matrix& a, bool by_row, int p, int lp, int ld, int64_t j0, int n) {
+    const bool tall = a.rows > a.cols;
+    const int lj = 11 - lp, rows = 1 << lp, places = 1 << lj;
+    const int64_t longer = max(a.rows, a.cols);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int e = threadIdx.x + FEW_THREADS * x, i = tall ? e & (rows - 1) : e >> lj, j = tall ? e >> lp : e & (places - 1);
+      to[x] = by_row ? i * ld + j : j * ld + i;
+      at[x] = i >= p || j >= n ? -1 : tall ? (j0 + j) * p + i : i * longer + j0 + j;
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+      if (at[x] >= 0) g[x] = static_cast<const G*>(a.g)[at[x]];
+    if (a.m != nullptr) {
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        if (at[x] >= 0) m[x] = a.m[at[x]];
+    }
+  }
+  // The direction, and the momentum after this step in m
+  __device__ __forceinline__ float direction_of(int x, const Coefficients& c, bool momentum) { return at[x] < 0 ? 0.f : direction(c, static_cast<float>(g[x]), m[x], momentum); }
+};
+
+template <class G, int N>
+__global__ void __launch_bounds__(FEW_THREADS) muon_gram_kernel(const __grid_constant__ Matrices<N> t, const Coefficients c) {
+  __shared__ __align__(16) double mem[16 * FEW_THREADS];            // u, [places][rows + 2]; at last the threads' sums
+  const int k = matrix_of(t.first_part, t.n, blockIdx.x), part = blockIdx.x - t.first_part[k];
+  const Matrix& a = t.a[k];
+  const int p = min(a.rows, a.cols), lp = log_rows(p), places = FEW_SLOTS >> lp, ld = (1 << lp) + 2;
+  const int64_t longer = max(a.rows, a.cols), begin = longer * part / a.nparts, end = longer * (part + 1) / a.nparts;
+  const int tiles = gram_tiles(p), slices = FEW_THREADS / tiles, slice = threadIdx.x / tiles, tile = threadIdx.x - slice * tiles;
+  int ti = 0;
+  while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
+  const int tj = tile - ti * (ti + 1) / 2;
+  double acc[4][4] = {};
+  for (int64_t j0 = begin; j0 < end; j0 += places) {
+    const int n = static_cast<int>(imin64(places, end - j0));
+    Eight<G> u;
+    u.load(a, false, p, lp, ld, j0, n);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) mem[u.to[x]] = u.direction_of(x, c, a.m != nullptr);
+    __syncthreads();
+    if (slice < slices)
+      for (int j = slice; j < n; j += slices) {
+        const double2 *x = reinterpret_cast<const double2*>(mem + j * ld + 4 * ti), *y = reinterpret_cast<const double2*>(mem + j * ld + 4 * tj);
+        const double2 x0 = x[0], x1 = x[1], y0 = y[0], y1 = y[1];
+        const double xs[4] = {x0.x, x0.y, x1.x, x1.y}, ys[4] = {y0.x, y0.y, y1.x, y1.y};
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) acc[r][q] = fma(xs[r], ys[q], acc[r][q]);
+      }
+    __syncthreads();
+  }
+  if (slice < slices) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mem[(slice * tiles + tile) * 16 + e] = acc[e >> 2][e & 3];
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < 16 * tiles; e += FEW_THREADS) {
+    double sum = 0;
+    for (int s = 0; s < slices; ++s) sum += mem[s * tiles * 16 + e];
+    a.parts[static_cast<int64_t>(part) * 16 * tiles + e] = sum;
+  }
+}
+
+// Rows of the matrices in shared memory.  What stands on the left of a product is symmetric, so that two neighbours of its column are two of its row: 16 bytes at a time (8 at a time, and a product for each of the two of M below,
+// the second launch took 30 us for 32 rows).
+constexpr int FEW_LD = FEW_ROWS + 2;
+struct Square {
+  double2 at[FEW_ROWS][FEW_LD / 2];
+  __device__ __forceinline__ double& operator()(int i, int j) { return reinterpret_cast<double*>(at[i])[j]; }
+};
+// 2 x 2 of x y, at (i, j), for matrices of p rows
+__device__ __forceinline__ void times(const Square& x, const Square& y, int p, int i, int j, double (&out)[2][2]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e >> 1][e & 1] = 0;
+#pragma unroll 4
+  for (int k = 0; k < p; ++k) {
+    const double2 l = x.at[k][i >> 1], r = y.at[k][j >> 1];
+    out[0][0] = fma(l.x, r.x, out[0][0]); out[0][1] = fma(l.x, r.y, out[0][1]);
+    out[1][0] = fma(l.y, r.x, out[1][0]); out[1][1] = fma(l.y, r.y, out[1][1]);
+  }
+}
+__device__ __forceinline__ void times(const Square& x, const Square& y, const Square& z, int p, int i, int j, double (&out)[2][2], double (&other)[2][2]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e >> 1][e & 1] = other[e >> 1][e & 1] = 0;
+#pragma unroll 4
+  for (int k = 0; k < p; ++k) {
+    const double2 l = x.at[k][i >> 1], r = y.at[k][j >> 1], q = z.at[k][j >> 1];
+    out[0][0] = fma(l.x, r.x, out[0][0]); out[0][1] = fma(l.x, r.y, out[0][1]);
+    out[1][0] = fma(l.y, r.x, out[1][0]); out[1][1] = fma(l.y, r.y, out[1][1]);
+    other[0][0] = fma(l.x, q.x, other[0][0]); other[0][1] = fma(l.x, q.y, other[0][1]);
+    other[1][0] = fma(l.y, q.x, other[1][0]); other[1][1] = fma(l.y, q.y, other[1][1]);
+  }
+}
+__device__ __forceinline__ void put(Square& to, int i, int j, const double (&v)[2][2]) {
+  to.at[i][j >> 1] = make_double2(v[0][0], v[0][1]);
+  to.at[i + 1][j >> 1] = make_double2(v[1][0], v[1][1]);
+}
+// Where a matrix's F / |u| [p][p] lies, behind G's parts, and behind it whether the norm is finite (1 or 0)
+__device__ __forceinline__ double* factor_of(const Matrix& a, int p) { return a.parts + static_cast<int64_t>(a.nparts) * gram_size(p); }
+
+// A block for each matrix
+template <int N>
+__global__ void __launch_bounds__(FEW_THREADS) muon_few_steps_kernel(const __grid_constant__ Matrices<N> t, const Coefficients c, int steps, double ca, double cb, double cc) {
+  __shared__ Square A, M, F, T;
+  const Matrix& a = t.a[blockIdx.x];
+  const int p = min(a.rows, a.cols), size = gram_size(p), i = 2 * (threadIdx.x >> 4), j = 2 * (threadIdx.x & 15);
+  sm100::grid_dependency_wait();
+  for (int e = threadIdx.x; e < FEW_ROWS * FEW_ROWS; e += FEW_THREADS) {
+    const int r = e / FEW_ROWS, q = e % FEW_ROWS, hi = max(r, q), lo = min(r, q);
+    double sum = 0;
+    if (hi < p) {
+      const double* from = a.parts + 16 * ((hi >> 2) * ((hi >> 2) + 1) / 2 + (lo >> 2)) + 4 * (hi & 3) + (lo & 3);
+#pragma unroll 8
+      for (int k = 0; k < a.nparts; ++k) sum += from[static_cast<int64_t>(k) * size];
+    }
+    A(r, q) = sum;
+  }
+  __syncthreads();
+  double squares = 0;
+  for (int k = 0; k < p; ++k) squares += A(k, k);
+  const bool finite = squares < INFINITY;          // (not NaN either)
+  const double norm = sqrt(squares), inv = 1.0 / (norm < c.eps ? static_cast<double>(c.eps) : norm);
+  __syncthreads();
+  for (int e = threadIdx.x; e < FEW_ROWS * FEW_ROWS; e += FEW_THREADS) A(e / FEW_ROWS, e % FEW_ROWS) *= inv * inv;
+  __syncthreads();
+  const bool mine = i < p && j < p;
+  for (int s = 0; s < steps; ++s) {
+    const bool more = s + 1 < steps;
+    double v[2][2], w[2][2];
+    if (mine) {
+      times(A, A, p, i, j, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = i + (e >> 1), q = j + (e & 1);
+        v[e >> 1][e & 1] = fma(cc, v[e >> 1][e & 1], fma(cb, A(r, q), r == q ? ca : 0.0));
+      }
+      put(M, i, j, v);
+      if (s == 0) put(F, i, j, v);
+    }
+    __syncthreads();
+    if (mine) {
+      if (s == 0) {
+        if (more) times(M, A, p, i, j, w);
+      } else if (more) {
+        times(M, F, A, p, i, j, v, w);
+      } else {
+        times(M, F, p, i, j, v);
+      }
+    }
+    __syncthreads();
+    if (mine) {
+      if (s > 0) put(F, i, j, v);
+      if (more) put(T, i, j, w);
+    }
+    __syncthreads();
+    if (mine && more && i >= j) {
+      // A is kept symmetric to the last bit, and M with it: what it were not would grow by 4 times a step and more (2e-9 of the result after 9 steps, 1e-2 after 15)
+      times(M, T, p, i, j, v);
+      if (i == j) v[0][1] = v[1][0];
+      put(A, i, j, v);
+      if (i > j) {
+        const double turned[2][2] = {{v[0][0], v[1][0]}, {v[0][1], v[1][1]}};
+        put(A, j, i, turned);
+      }
+    }
+    __syncthreads();
+  }
+  double* to = factor_of(a, p);
+  for (int e = threadIdx.x; e < p * p; e += FEW_THREADS) to[e] = F(e / p, e % p) * inv;
+  if (threadIdx.x == 0) to[p * p] = finite ? 1.0 : 0.0;
+}
+
+// UPDATE: momentum and weights, left alone where the norm is not finite; else X itself, NaN there
+template <class G, class W, bool UPDATE, int N>
+__global__ void __launch_bounds__(FEW_THREADS) muon_few_finish_kernel(const __grid_constant__ Matrices<N> t, const Coefficients c) {
+  __shared__ double F[FEW_ROWS][FEW_ROWS], u[FEW_SLOTS + FEW_ROWS];           // u, and X: [rows][places + 1]
+  __shared__ float x[FEW_SLOTS + FEW_ROWS];
+  sm100::grid_dependency_wait();
+  const int all = t.first_tile[t.n];
+  int at = static_cast<int>(static_cast<int64_t>(all) * blockIdx.x / gridDim.x);
+  const int end = static_cast<int>(static_cast<int64_t>(all) * (blockIdx.x + 1) / gridDim.x);
+  int k = matrix_of(t.first_tile, t.n, at);
+  bool fresh = true, finite = false;
+  for (; at < end; ++at) {
+    if (at >= t.first_tile[k + 1]) { ++k; fresh = true; }
+    const Matrix& a = t.a[k];
+    const bool tall = a.rows > a.cols;
+    const int p = min(a.rows, a.cols), lp = log_rows(p), rows = 1 << lp, places = FEW_SLOTS >> lp, ld = places + 1;
+    const int64_t longer = max(a.rows, a.cols), j0 = static_cast<int64_t>(at - t.first_tile[k]) * places;
+    const int n = static_cast<int>(imin64(places, longer - j0));
+    if (fresh) {
+      const double* from = factor_of(a, p);
+      for (int e = threadIdx.x; e < FEW_ROWS * FEW_ROWS; e += FEW_THREADS) {
+        const int r = e / FEW_ROWS, q = e % FEW_ROWS;
+        F[r][q] = r < p && q < p ? from[r * p + q] : 0.0;
+      }
+      finite = from[p * p] == 1.0;
+      fresh = false;
+    }
+    if (!UPDATE || finite) {                       // the same for all of the block
+      Eight<G> v;
+      v.load(a, true, p, lp, ld, j0, n);
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        u[v.to[s]] = v.direction_of(s, c, a.m != nullptr);
+        if (UPDATE && v.at[s] >= 0) a.m[v.at[s]] = v.m[s];
+      }
+      __syncthreads();
+      // 8 rows of X a thread (4, where there are no more)
+      const int groups = rows >> 3 ? rows >> 3 : 1, i0 = 8 * (threadIdx.x % groups);
+      for (int j = threadIdx.x / groups; j < n; j += FEW_THREADS / groups) {
+        double sum[8] = {};
+        for (int r = 0; r < p; ++r) {
+          const double y = u[r * ld + j];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum[e] = fma(F[r][i0 + e], y, sum[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (i0 + e < p) x[(i0 + e) * ld + j] = finite ? static_cast<float>(sum[e]) : __int_as_float(0x7FFFFFFF);
+      }
+      __syncthreads();
+      // four neighbours in memory at a time
+      W* w = static_cast<W*>(a.w);
+      const int across = tall ? (p + 3) >> 2 : (n + 3) >> 2, lines = tall ? n : p;
+      for (int e = threadIdx.x; e < across * lines; e += FEW_THREADS) {
+        const int line = e / across, first = 4 * (e - line * across), have = min(4, (tall ? p : n) - first);
+        const int64_t i = tall ? (j0 + line) * p + first : line * longer + j0 + first;
+        float y[4], z[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) y[q] = q < have ? (tall ? x[(first + q) * ld + line] : x[line * ld + first + q]) : 0.f;
+        if (UPDATE) {
+          Raw<W> old;
+          old.load(w + i, have);
+          old.get(z);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) y[q] = fmaf(-a.rate, y[q], z[q] * c.decay);
+        }
+        store_weights(w + i, have, y, c, a.at + i);
+      }
+      __syncthreads();
+    } else {
+      __syncthreads();                             // F is read by all before it is another one's
+    }
+  }
+}
+
 // ---------------------------------------------------------------- host side
 constexpr int64_t ROUND_BYTES = int64_t(1) << 30;      // of scratch memory, unless one matrix needs more: a round of so much keeps the GPU busy for a millisecond
 
@@ -461,6 +740,16 @@ struct Sizes {
   int64_t bytes() const { return 2 * (3 * x() + a()) + 4 * 256 + 8 * NORM_PARTS + 8; }
 };
 Sizes sizes_of(int64_t rows, int64_t cols) { return {up64(std::min(rows, cols)), up64(std::max(rows, cols))}; }
+bool few_rows(int64_t rows, int64_t cols) { return std::min(rows, cols) <= FEW_ROWS; }
+int gram_parts(int64_t rows, int64_t cols) {
+  const int64_t each = static_cast<int64_t>(GRAM_LOOPS) * (FEW_SLOTS >> log_rows(static_cast<int>(std::min(rows, cols))));
+  return static_cast<int>(std::min<int64_t>(GRAM_PARTS, (std::max(rows, cols) + each - 1) / each));
+}
+int64_t few_bytes(int64_t rows, int64_t cols) {              // of G's parts and F
+  const int p = static_cast<int>(std::min(rows, cols));
+  return up256(8 * (static_cast<int64_t>(gram_parts(rows, cols)) * gram_size(p) + p * p + 1));
+}
+int64_t bytes_of(int64_t rows, int64_t cols) { return few_rows(rows, cols) ? few_bytes(rows, cols) : sizes_of(rows, cols).bytes(); }
 
 // The matrices by shape, cut into rounds.  Rounds are those of the whole list, whichever of it have a gradient: fewer of them in a round need less, but other rounds could need more than the
 // scratch memory that was asked for.
@@ -477,7 +766,7 @@ Plan plan_of(const int64_t* rows, const int64_t* cols, int64_t count) {
   std::stable_sort(p.order.begin(), p.order.end(), [&](int64_t i, int64_t j) { return key(i) > key(j); });
   int64_t used = 0;
   for (size_t k = 0; k < p.order.size(); ++k) {
-    const int64_t need = sizes_of(rows[p.order[k]], cols[p.order[k]]).bytes();
+    const int64_t need = bytes_of(rows[p.order[k]], cols[p.order[k]]);
     if (k == 0 || used + need > ROUND_BYTES) {
       p.rounds.push_back(k);
       used = 0;
@@ -490,7 +779,7 @@ Plan plan_of(const int64_t* rows, const int64_t* cols, int64_t count) {
 }
 
 // f(table, blocks of squares, elementwise tiles) for the matrices, as many at a time as a launch's parameters hold
-template <int N, class F>
+template <bool FEW_OF_X, int N, class F>
 int with_table(const std::vector<Matrix>& all, size_t from, F&& f) {
   static thread_local Matrices<N> t;
   t.n = static_cast<int>(std::min<size_t>(N, all.size() - from));
@@ -500,20 +789,38 @@ int with_table(const std::vector<Matrix>& all, size_t from, F&& f) {
     t.first_part[k] = static_cast<int>(parts);
     t.first_tile[k] = static_cast<int>(tiles);
     parts += a.nparts;
-    tiles += static_cast<int64_t>((a.rows + SIDE - 1) / SIDE) * ((a.cols + SIDE - 1) / SIDE);
+    if (FEW_OF_X) tiles += (std::max(a.rows, a.cols) + (FEW_SLOTS >> log_rows(std::min(a.rows, a.cols))) - 1) / (FEW_SLOTS >> log_rows(std::min(a.rows, a.cols)));
+    else tiles += static_cast<int64_t>((a.rows + SIDE - 1) / SIDE) * ((a.cols + SIDE - 1) / SIDE);
     if (tiles > 0x7FFFFFFF) return fail(HASTE_ERR_TOO_LARGE, "matrices of too many elements for one call");
   }
   t.first_part[t.n] = static_cast<int>(parts); t.first_tile[t.n] = static_cast<int>(tiles);
   // the elementwise launches' blocks share the tiles: as many as run at once
   return f(t, std::integral_constant<int, N>(), static_cast<unsigned>(parts), static_cast<unsigned>(imin64(tiles, static_cast<int64_t>(sm_count()) * 6)));
 }
-template <class F>
+template <bool FEW_OF_X, class F>
 int for_each_table(const std::vector<Matrix>& all, F&& f) {
   for (size_t i = 0; i < all.size(); i += MANY) {
-    const int rc = all.size() - i <= FEW ? with_table<FEW>(all, i, f) : with_table<MANY>(all, i, f);
+    const int rc = all.size() - i <= FEW ? with_table<FEW_OF_X, FEW>(all, i, f) : with_table<FEW_OF_X, MANY>(all, i, f);
     if (rc) return rc;
   }
   return HASTE_OK;
+}
+
+// Everything for matrices of few rows
+int launch_few_rows(const std::vector<Matrix>& all, const MuonCall& c, const Coefficients& k, cudaStream_t st) {
+  const bool gb = c.g_type == HASTE_BF16;
+  return for_each_table<true>(all, [&](const auto& t, auto size, unsigned parts, unsigned tiles) -> int {
+    constexpr int N = decltype(size)::value;
+    using B = __nv_bfloat16;
+    if (gb) muon_gram_kernel<B, N><<<parts, FEW_THREADS, 0, st>>>(t, k);
+    else muon_gram_kernel<float, N><<<parts, FEW_THREADS, 0, st>>>(t, k);
+    if (int e = check_launch("muon_gram_kernel")) return e;
+    if (int e = launch_behind(muon_few_steps_kernel<N>, static_cast<unsigned>(t.n), FEW_THREADS, st, t, k, c.steps, c.a, c.b, c.c)) return e;
+    auto finish = [&](auto kernel) { return launch_behind(kernel, tiles, FEW_THREADS, st, t, k); };
+    if (!c.update) return gb ? finish(muon_few_finish_kernel<B, B, false, N>) : finish(muon_few_finish_kernel<float, B, false, N>);
+    if (c.p_type == HASTE_BF16) return gb ? finish(muon_few_finish_kernel<B, B, true, N>) : finish(muon_few_finish_kernel<float, B, true, N>);
+    return gb ? finish(muon_few_finish_kernel<B, float, true, N>) : finish(muon_few_finish_kernel<float, float, true, N>);
+  });
 }
 
 }  // namespace
@@ -538,9 +845,32 @@ int launch_muon(const MuonCall& c, cudaStream_t st) {
   for (size_t r = 0; r + 1 < plan.rounds.size(); ++r) {
     char* mem = static_cast<char*>(c.scratch);
     auto take = [&](int64_t bytes) { char* p = mem; mem += up256(bytes); return p; };
-    std::vector<int64_t> some;         // those with a gradient
-    for (size_t i = plan.rounds[r]; i < plan.rounds[r + 1]; ++i)
-      if (c.grads[plan.order[i]] != nullptr) some.push_back(plan.order[i]);
+    std::vector<int64_t> some, few;    // those with a gradient
+    for (size_t i = plan.rounds[r]; i < plan.rounds[r + 1]; ++i) {
+      const int64_t o = plan.order[i];
+      if (c.grads[o] != nullptr) (few_rows(c.rows[o], c.cols[o]) ? few : some).push_back(o);
+    }
+    const bool gb = c.g_type == HASTE_BF16;
+    auto matrix = [&](int64_t o) {
+      Matrix m = {};
+      m.g = c.grads[o]; m.w = c.params[o];
+      m.m = c.momentum ? c.momentum + at[o] : nullptr;
+      m.at = at[o];
+      m.rows = static_cast<int>(c.rows[o]); m.cols = static_cast<int>(c.cols[o]);
+      m.rate = static_cast<float>(c.lr * (c.adjust == HASTE_MUON_MATCH_RMS ? 0.2 * std::sqrt(static_cast<double>(std::max(c.rows[o], c.cols[o])))
+                                                                            : std::sqrt(std::max(1.0, static_cast<double>(c.rows[o]) / static_cast<double>(c.cols[o])))));
+      return m;
+    };
+    if (!few.empty()) {
+      std::vector<Matrix> all;
+      for (int64_t o : few) {
+        Matrix m = matrix(o);
+        m.nparts = gram_parts(c.rows[o], c.cols[o]);
+        m.parts = reinterpret_cast<double*>(take(few_bytes(c.rows[o], c.cols[o])));
+        all.push_back(m);
+      }
+      if (int rc = launch_few_rows(all, c, k, st)) return rc;
+    }
     if (some.empty()) continue;
     const int64_t n = static_cast<int64_t>(some.size());
     auto* done = reinterpret_cast<unsigned long long*>(take(8 * (n + 1)));
@@ -562,24 +892,19 @@ int launch_muon(const MuonCall& c, cudaStream_t st) {
       h.B = reinterpret_cast<uint16_t*>(take(2 * h.count * s.a()));
       for (size_t j = i; j < end; ++j) {
         const int64_t o = some[j], x = static_cast<int64_t>(j - i) * s.x(), size = c.rows[o] * c.cols[o];
-        Matrix m = {};
-        m.g = c.grads[o]; m.w = c.params[o];
-        m.m = c.momentum ? c.momentum + at[o] : nullptr;
+        Matrix m = matrix(o);
         m.hi = h.hi[0] + x; m.lo = h.lo + x;
-        m.at = at[o];
-        m.rows = static_cast<int>(c.rows[o]); m.cols = static_cast<int>(c.cols[o]); m.ld = static_cast<int>(s.q);
+        m.ld = static_cast<int>(s.q);
         m.nparts = static_cast<int>(std::min<int64_t>(NORM_PARTS, (size + each - 1) / each));
         m.parts = parts + NORM_PARTS * all.size();
         m.done = done + all.size();
-        m.rate = static_cast<float>(c.lr * (c.adjust == HASTE_MUON_MATCH_RMS ? 0.2 * std::sqrt(static_cast<double>(std::max(c.rows[o], c.cols[o])))
-                                                                              : std::sqrt(std::max(1.0, static_cast<double>(c.rows[o]) / static_cast<double>(c.cols[o])))));
         all.push_back(m);
       }
       batches.push_back(h);
       i = end;
     }
-    const bool gb = c.g_type == HASTE_BF16, narrow = newton_schulz::take_narrow(batches);
-    int rc = for_each_table(all, [&](const auto& t, auto size, unsigned parts, unsigned tiles) -> int {
+    const bool narrow = newton_schulz::take_narrow(batches);
+    int rc = for_each_table<false>(all, [&](const auto& t, auto size, unsigned parts, unsigned tiles) -> int {
       constexpr int N = decltype(size)::value;
       if (gb) muon_squares_kernel<__nv_bfloat16, N><<<parts, NORM_THREADS, 0, st>>>(t, k);
       else muon_squares_kernel<float, N><<<parts, NORM_THREADS, 0, st>>>(t, k);
@@ -597,7 +922,7 @@ int launch_muon(const MuonCall& c, cudaStream_t st) {
         if (c.steps & 1) all[at_matrix].hi = h.hi[1] + j * h.p * h.q;          // X is in the other buffer
       }
     }
-    rc = for_each_table(all, [&](const auto& t, auto size, unsigned, unsigned tiles) -> int {
+    rc = for_each_table<false>(all, [&](const auto& t, auto size, unsigned, unsigned tiles) -> int {
       constexpr int N = decltype(size)::value;
       if (!c.update) return launch_behind(muon_finish_kernel<__nv_bfloat16, false, N>, tiles, 256, st, t, k);
       return c.p_type == HASTE_BF16 ? launch_behind(muon_finish_kernel<__nv_bfloat16, true, N>, tiles, 256, st, t, k) : launch_behind(muon_finish_kernel<float, true, N>, tiles, 256, st, t, k);

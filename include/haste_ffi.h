@@ -456,10 +456,11 @@ int haste_gated_backward(const void* dy, const void* x, const void* wg, const vo
  * left alone, and so is one whose norm is inf or NaN, with its momentum.  Where a wait of the steps runs out (haste_poll_status) a matrix whose steps are not complete keeps its
  * weights; its momentum is that after this step.  momentum: fp32, 16-byte aligned, `moments` elements of room, matrix after
  * matrix, every one at a multiple of 256 elements.  Norms are 64 bits, momentum and weights' arithmetic 32, products take fp16 and sum in fp32
- * (X keeps 22 bits between them up to the last two steps, 11 in these; a is rounded to fp16 with the rest of a I + b A + c A A).  bf16 parameters are rounded stochastically with HASTE_F_SR, else to nearest: Philox4x32 with 7 rounds, key (lower half of
+ * (X keeps 22 bits between them up to the last two steps, 11 in these; a is rounded to fp16 with the rest of a I + b A + c A A; matrices with a side of
+ * 32 or less are computed in 64 bits throughout).  bf16 parameters are rounded stochastically with HASTE_F_SR, else to nearest: Philox4x32 with 7 rounds, key (lower half of
  * seed, step), counter (i, i >> 32, stream_index, 2), the lower halves of its words for elements 4i .. 4i+3 of the momentum's buffer.
  * eps is 2^-100 at least.  scratch: 256-byte aligned, haste_muon_scratch(...) bytes: 6 an element and 2 for every pair of rows of X (with sides rounded up to
- * multiples of 64), 1 GB at most unless one matrix needs more (matrices are then worked on in rounds). */
+ * multiples of 64; less for matrices with a side of 32 or less), 1 GB at most unless one matrix needs more (matrices are then worked on in rounds). */
 int64_t haste_muon_scratch(const int64_t* rows, const int64_t* cols, int64_t count);
 int haste_muon_step(void* const* params, const void* const* grads, const int64_t* rows, const int64_t* cols, int64_t count, float* momentum, int64_t moments, int32_t p_type,
                     int32_t g_type, double lr, double mu, int32_t nesterov, double weight_decay, int32_t adjust, int32_t steps, double a, double b, double c, double eps,
